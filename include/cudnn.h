@@ -252,6 +252,70 @@ cudnnStatus_t cudnnBatchNormalizationForwardTraining(
     double exponentialAverageFactor, void* resultRunningMean, void* resultRunningVariance,
     double epsilon, void* resultSaveMean, void* resultSaveInvVariance);
 
+/* Losses over a linear head's vocabulary, forward and with gradients (extensions).
+ *
+ * x holds T tokens of H features: a tensor descriptor with c = H, cStride 1 and its
+ * (n, h, w) positions a uniform stride apart.  w is the head: a 1x1 filter, k = V words
+ * of c = H features.  Both BFLOAT16 or both HALF; z = x w^T / temperature and everything
+ * computed from it is fp32 until a 16-bit output.  The T x V logits are never stored.
+ *
+ *   cross entropy   loss[t] = lse(z[t]) - z[t][labels[t]]
+ *   distillation    q = softmax(teacherLogits[t] / temperature) over the row's topK
+ *                   (1..256) entries, loss[t] = sum_k q_k (log q_k - (z[t][index_k] - lse))
+ *
+ * A negative label leaves its token out; a negative teacher index, or a teacher logit of
+ * -inf, leaves its entry out, and a token without entries is left out.  A token that is
+ * left out has loss 0, logSumExp 0 and no gradient, whatever its x and dloss hold.
+ * Equal indices of a token add up.  A label or index of V or more makes its token's loss,
+ * and the gradients it enters, NaN.  labels and teacherIndex [T][topK] are int64 (as
+ * training programs hold them); teacherLogits [T][topK], loss and logSumExp are float.
+ *
+ * Backward computes the gradients of sum_t dloss[t] * loss[t] in one pass over the
+ * tokens; it computes the losses too and writes them when loss / logSumExp are not null,
+ * so a training step whose dloss is known needs no Forward.  dx (like x; it may be x
+ * itself) or dw (like w) may be null with its descriptor: it is not computed.  Results
+ * do not depend on the stream's other work: no atomics.
+ *
+ * The workspace: null uses the handle's own (grown to what GetWorkspaceSize reports: at
+ * most 2 GiB for 16-bit numerators of a piece of the tokens, plus V*H floats when T
+ * needs several pieces).  A workspace given (aligned to 256 bytes) bounds the memory
+ * instead: smaller ones mean smaller pieces, down to 128 tokens; BAD_PARAM below that.
+ */
+cudnnStatus_t cudnnGetLinearCrossEntropyWorkspaceSize(cudnnHandle_t handle,
+                                                      cudnnTensorDescriptor_t xDesc,
+                                                      cudnnFilterDescriptor_t wDesc, int gradients,
+                                                      size_t* sizeInBytes);
+cudnnStatus_t cudnnLinearCrossEntropyForward(cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc,
+                                             const void* x, cudnnFilterDescriptor_t wDesc,
+                                             const void* w, const int64_t* labels, void* workSpace,
+                                             size_t workSpaceSizeInBytes, float* loss,
+                                             float* logSumExp);
+cudnnStatus_t cudnnLinearCrossEntropyBackward(cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc,
+                                              const void* x, cudnnFilterDescriptor_t wDesc,
+                                              const void* w, const int64_t* labels,
+                                              const float* dloss, void* workSpace,
+                                              size_t workSpaceSizeInBytes, float* loss,
+                                              float* logSumExp, cudnnTensorDescriptor_t dxDesc,
+                                              void* dx, cudnnFilterDescriptor_t dwDesc, void* dw);
+cudnnStatus_t cudnnGetLinearDistillationWorkspaceSize(cudnnHandle_t handle,
+                                                      cudnnTensorDescriptor_t xDesc,
+                                                      cudnnFilterDescriptor_t wDesc, int topK,
+                                                      int gradients, size_t* sizeInBytes);
+cudnnStatus_t cudnnLinearDistillationForward(cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc,
+                                             const void* x, cudnnFilterDescriptor_t wDesc,
+                                             const void* w, int topK, const int64_t* teacherIndex,
+                                             const float* teacherLogits, double temperature,
+                                             void* workSpace, size_t workSpaceSizeInBytes,
+                                             float* loss, float* logSumExp);
+cudnnStatus_t cudnnLinearDistillationBackward(cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc,
+                                              const void* x, cudnnFilterDescriptor_t wDesc,
+                                              const void* w, int topK, const int64_t* teacherIndex,
+                                              const float* teacherLogits, double temperature,
+                                              const float* dloss, void* workSpace,
+                                              size_t workSpaceSizeInBytes, float* loss,
+                                              float* logSumExp, cudnnTensorDescriptor_t dxDesc,
+                                              void* dx, cudnnFilterDescriptor_t dwDesc, void* dw);
+
 #ifdef __cplusplus
 }
 #endif

@@ -85,6 +85,7 @@ def curand() -> C.CDLL:
 
 # ------------------------------------------------------------------- cuDNN --
 CUDNN_STATUS_SUCCESS = 0
+CUDNN_STATUS_ALLOC_FAILED = 2
 CUDNN_STATUS_BAD_PARAM = 3
 CUDNN_STATUS_EXECUTION_FAILED = 8
 CUDNN_STATUS_NOT_SUPPORTED = 9
@@ -153,6 +154,15 @@ CUDNN_PROTOS = {
                                                  vp, C.c_double], i32),
     "cudnnBatchNormalizationForwardTraining": ([vp, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp,
                                                 C.c_double, vp, vp, C.c_double, vp, vp], i32),
+    "cudnnGetLinearCrossEntropyWorkspaceSize": ([vp, vp, vp, i32, P(sz)], i32),
+    "cudnnLinearCrossEntropyForward": ([vp, vp, vp, vp, vp, vp, vp, sz, vp, vp], i32),
+    "cudnnLinearCrossEntropyBackward": ([vp, vp, vp, vp, vp, vp, vp, vp, sz, vp, vp, vp, vp, vp,
+                                         vp], i32),
+    "cudnnGetLinearDistillationWorkspaceSize": ([vp, vp, vp, i32, i32, P(sz)], i32),
+    "cudnnLinearDistillationForward": ([vp, vp, vp, vp, vp, i32, vp, vp, C.c_double, vp, sz, vp,
+                                        vp], i32),
+    "cudnnLinearDistillationBackward": ([vp, vp, vp, vp, vp, i32, vp, vp, C.c_double, vp, vp, sz,
+                                         vp, vp, vp, vp, vp, vp], i32),
 }
 
 

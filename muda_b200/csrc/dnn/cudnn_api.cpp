@@ -16,16 +16,20 @@
 #include <cuda_runtime_api.h>
 
 #include <algorithm>
+#include <climits>
+#include <cmath>
 #include <cstdint>
 #include <initializer_list>
 #include <memory>
 #include <mutex>
+#include <new>
 #include <utility>
 
 #include "common/device.hpp"
 #include "common/lru.hpp"
 #include "common/registry.hpp"
 #include "dnn/dnn.hpp"
+#include "dnn/vocab_loss.hpp"
 
 namespace {
 
@@ -1088,6 +1092,278 @@ cudnnStatus_t cudnnBatchNormalizationForwardTraining(
   const std::size_t need = mb200::dnn::bn_training_workspace(xs.v);
   if (need == 0) return status_of(run(nullptr));
   return with_workspace(*h, need, st, run);
+}
+
+}  // extern "C"
+
+// --------------------------------------------------------------- vocabulary losses --
+namespace {
+
+using mb200::dnn::VocabLossArgs;
+
+// The (n, h, w) positions of a descriptor as rows of c contiguous elements, `ld` apart.
+bool rows_of(const View4& v, std::int64_t* rows, std::int64_t* ld) {
+  if (v.c > 1 && v.cs != 1) return false;
+  *rows = static_cast<std::int64_t>(v.n) * v.h * v.w;
+  *ld = v.w > 1 ? v.ws : v.h > 1 ? v.hs : v.n > 1 ? v.ns : v.c;
+  if (v.w > 1 && v.h > 1 && v.hs != v.w * *ld) return false;
+  if ((v.w > 1 || v.h > 1) && v.n > 1 && v.ns != v.h * (v.w * *ld)) return false;
+  return *ld >= v.c;
+}
+
+struct FilterSnap {
+  bool configured;
+  cudnnDataType_t dtype;
+  int k, c, h, w;
+};
+
+FilterSnap snap(FilterDesc& d) {
+  std::lock_guard<std::mutex> g(d.mu);
+  return {d.configured, d.dtype, d.k, d.c, d.h, d.w};
+}
+
+// Sizes and types of the head.
+cudnnStatus_t vocab_head(TensorDesc& xd, FilterDesc& wd, VocabLossArgs* a) {
+  const TensorSnap xs = snap(xd);
+  const FilterSnap f = snap(wd);
+  if (!xs.configured || !f.configured) return CUDNN_STATUS_BAD_PARAM;
+  if (f.h != 1 || f.w != 1 || f.c != xs.v.c || f.dtype != xs.dtype) return CUDNN_STATUS_BAD_PARAM;
+  if (xs.dtype == CUDNN_DATA_FLOAT) return CUDNN_STATUS_NOT_SUPPORTED;
+  std::int64_t rows;
+  if (!rows_of(xs.v, &rows, &a->ldx)) return CUDNN_STATUS_NOT_SUPPORTED;
+  if (rows > (1 << 30) || f.k > (1 << 30)) return CUDNN_STATUS_NOT_SUPPORTED;
+  a->bf16 = xs.dtype == CUDNN_DATA_BFLOAT16;
+  a->tokens = static_cast<int>(rows);
+  a->features = f.c;
+  a->vocab = f.k;
+  return CUDNN_STATUS_SUCCESS;
+}
+
+cudnnStatus_t vocab_workspace(cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc,
+                              cudnnFilterDescriptor_t wDesc, int topK, int gradients,
+                              std::size_t* size) {
+  if (size == nullptr) return CUDNN_STATUS_BAD_PARAM;
+  auto h = handles().get(handle);
+  auto xd = tensors().get(xDesc);
+  auto wd = filters().get(wDesc);
+  if (!h || !xd || !wd) return CUDNN_STATUS_BAD_PARAM;
+  VocabLossArgs a{};
+  const cudnnStatus_t s = vocab_head(*xd, *wd, &a);
+  if (s != CUDNN_STATUS_SUCCESS) return s;
+  a.top_k = topK;
+  a.gradients = gradients != 0;
+  // any aligned address stands for the operands: only alignment enters the plan
+  void* aligned = reinterpret_cast<void*>(std::uintptr_t{256});
+  a.x = a.w = aligned;
+  if (a.gradients) a.dx = a.dw = aligned;
+  *size = mb200::dnn::vocab_loss_workspace(a);
+  return CUDNN_STATUS_SUCCESS;
+}
+
+struct Span {
+  const void* p;
+  std::size_t bytes;
+};
+
+bool overlap(const Span& a, const Span& b) {
+  if (a.bytes == 0 || b.bytes == 0) return false;
+  const auto x = reinterpret_cast<std::uintptr_t>(a.p), y = reinterpret_cast<std::uintptr_t>(b.p);
+  return x < y + b.bytes && y < x + a.bytes;
+}
+
+// Rows of dx against rows of x: the same rows, apart, or side by side in wider rows.
+bool rows_compatible(const VocabLossArgs& a, const Span& x, const Span& dx) {
+  if (!overlap(x, dx)) return true;
+  if (a.tokens > 1 && a.ldx != a.lddx) return false;
+  if (a.x == a.dx) return true;
+  if (a.tokens == 1) return false;
+  const std::int64_t row = a.ldx * 2, used = static_cast<std::int64_t>(a.features) * 2;
+  const auto d = static_cast<std::int64_t>(reinterpret_cast<std::uintptr_t>(a.dx) -
+                                           reinterpret_cast<std::uintptr_t>(a.x));
+  const std::int64_t m = ((d % row) + row) % row;
+  return m >= used && row - m >= used;
+}
+
+std::size_t row_span(std::int64_t rows, std::int64_t ld, int c) {
+  return static_cast<std::size_t>((rows - 1) * ld + c) * 2;
+}
+
+// Checks the pointers of `a` (sizes are set) and runs it.
+cudnnStatus_t vocab_run(DnnContext& h, const VocabLossArgs& a, void* workSpace,
+                        std::size_t workSpaceSize) {
+  const std::size_t T = a.tokens, V = a.vocab, H = a.features, K = a.top_k;
+  const Span x{a.x, row_span(a.tokens, a.ldx, a.features)}, w{a.w, V * H * 2};
+  const Span labels{a.labels, K == 0 ? T * 8 : 0}, index{a.teacher_index, T * K * 8};
+  const Span teacher{a.teacher_logits, T * K * 4};
+  const Span dloss{a.dloss, a.gradients ? T * 4 : 0};
+  const Span loss{a.loss, a.loss != nullptr ? T * 4 : 0}, lse{a.lse, a.lse != nullptr ? T * 4 : 0};
+  const Span dx{a.dx, a.dx != nullptr ? row_span(a.tokens, a.lddx, a.features) : 0};
+  const Span dw{a.dw, a.dw != nullptr ? V * H * 2 : 0};
+  const Span ws{workSpace, workSpace != nullptr ? workSpaceSize : 0};
+  for (const auto& [s, align] : {std::pair<Span, std::size_t>{x, 2}, {w, 2}, {labels, 8},
+                                 {index, 8}, {teacher, 4}, {dloss, 4}, {loss, 4}, {lse, 4},
+                                 {dx, 2}, {dw, 2}, {ws, 256}}) {
+    if (s.bytes == 0) continue;
+    if (!mb200::aligned_to(s.p, align) || !mb200::device_span_ok(s.p, s.bytes))
+      return CUDNN_STATUS_BAD_PARAM;
+  }
+  const Span in[] = {x, w, labels, index, teacher, dloss};
+  const Span out[] = {loss, lse, dw, ws, dx};
+  for (int i = 0; i < 5; ++i) {
+    for (int j = 0; j < i; ++j)
+      if (overlap(out[i], out[j])) return CUDNN_STATUS_BAD_PARAM;
+    for (int j = 0; j < 6; ++j)
+      if (!(i == 4 && j == 0) && overlap(out[i], in[j])) return CUDNN_STATUS_BAD_PARAM;
+  }
+  if (!rows_compatible(a, x, dx)) return CUDNN_STATUS_BAD_PARAM;
+  const cudaStream_t st = stream_of(h);
+  if (workSpace != nullptr) {
+    if (workSpaceSize < mb200::dnn::vocab_loss_min_workspace(a)) return CUDNN_STATUS_BAD_PARAM;
+    return status_of(mb200::dnn::launch_vocab_loss(a, workSpace, workSpaceSize, st));
+  }
+  const std::size_t need = mb200::dnn::vocab_loss_workspace(a);
+  return with_workspace(h, need, st, [&](void* p) {
+    return mb200::dnn::launch_vocab_loss(a, p, need, st);
+  });
+}
+
+// Argument checks shared by the four calls; `fill` sets the targets.
+template <class Fill>
+cudnnStatus_t vocab_call(cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc, const void* x,
+                         cudnnFilterDescriptor_t wDesc, const void* w, bool gradients,
+                         const float* dloss, void* workSpace, std::size_t workSpaceSize,
+                         float* loss, float* lse, cudnnTensorDescriptor_t dxDesc, void* dx,
+                         cudnnFilterDescriptor_t dwDesc, void* dw, Fill&& fill) {
+  try {
+    if (x == nullptr || w == nullptr) return CUDNN_STATUS_BAD_PARAM;
+    if (!gradients && loss == nullptr && lse == nullptr) return CUDNN_STATUS_BAD_PARAM;
+    if (gradients && (dloss == nullptr || (dx == nullptr && dw == nullptr)))
+      return CUDNN_STATUS_BAD_PARAM;
+    auto h = handles().get(handle);
+    auto xd = tensors().get(xDesc);
+    auto wd = filters().get(wDesc);
+    if (!h || !xd || !wd) return CUDNN_STATUS_BAD_PARAM;
+    VocabLossArgs a{};
+    cudnnStatus_t s = vocab_head(*xd, *wd, &a);
+    if (s != CUDNN_STATUS_SUCCESS) return s;
+    a.x = x;
+    a.w = w;
+    a.inv_tau = 1.0f;
+    a.loss = loss;
+    a.lse = lse;
+    a.gradients = gradients;
+    a.dloss = dloss;
+    if (!fill(a)) return CUDNN_STATUS_BAD_PARAM;
+    if (dx != nullptr) {
+      auto dxd = tensors().get(dxDesc);
+      if (!dxd) return CUDNN_STATUS_BAD_PARAM;
+      const TensorSnap xs = snap(*xd), ds = snap(*dxd);
+      if (!ds.configured || ds.dtype != xs.dtype || ds.v.n != xs.v.n || ds.v.c != xs.v.c ||
+          ds.v.h != xs.v.h || ds.v.w != xs.v.w)
+        return CUDNN_STATUS_BAD_PARAM;
+      std::int64_t rows;
+      if (!rows_of(ds.v, &rows, &a.lddx)) return CUDNN_STATUS_NOT_SUPPORTED;
+      a.dx = dx;
+    }
+    if (dw != nullptr) {
+      auto dwd = filters().get(dwDesc);
+      if (!dwd) return CUDNN_STATUS_BAD_PARAM;
+      const FilterSnap f = snap(*wd), g = snap(*dwd);
+      if (!g.configured || g.dtype != f.dtype || g.k != f.k || g.c != f.c || g.h != 1 || g.w != 1)
+        return CUDNN_STATUS_BAD_PARAM;
+      a.dw = dw;
+    }
+    return vocab_run(*h, a, workSpace, workSpaceSize);
+  } catch (const std::bad_alloc&) {
+    return CUDNN_STATUS_ALLOC_FAILED;
+  } catch (...) {
+    return CUDNN_STATUS_INTERNAL_ERROR;
+  }
+}
+
+bool fill_labels(VocabLossArgs& a, const std::int64_t* labels) {
+  a.labels = labels;
+  return labels != nullptr;
+}
+
+bool fill_teacher(VocabLossArgs& a, int topK, const std::int64_t* index, const float* logits,
+                  double temperature) {
+  if (topK < 1 || topK > mb200::dnn::kVocabMaxTopK || index == nullptr || logits == nullptr)
+    return false;
+  // 2^-64..2^64: the fp32 reciprocal and its products with log2(e) stay normal
+  if (!(temperature >= 0x1p-64 && temperature <= 0x1p64)) return false;
+  a.top_k = topK;
+  a.teacher_index = index;
+  a.teacher_logits = logits;
+  a.inv_tau = static_cast<float>(1.0 / temperature);
+  return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+cudnnStatus_t cudnnGetLinearCrossEntropyWorkspaceSize(cudnnHandle_t handle,
+                                                      cudnnTensorDescriptor_t xDesc,
+                                                      cudnnFilterDescriptor_t wDesc, int gradients,
+                                                      size_t* sizeInBytes) {
+  return vocab_workspace(handle, xDesc, wDesc, 0, gradients, sizeInBytes);
+}
+
+cudnnStatus_t cudnnLinearCrossEntropyForward(cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc,
+                                             const void* x, cudnnFilterDescriptor_t wDesc,
+                                             const void* w, const int64_t* labels, void* workSpace,
+                                             size_t workSpaceSizeInBytes, float* loss,
+                                             float* logSumExp) {
+  return vocab_call(handle, xDesc, x, wDesc, w, false, nullptr, workSpace, workSpaceSizeInBytes,
+                    loss, logSumExp, nullptr, nullptr, nullptr, nullptr,
+                    [&](VocabLossArgs& a) { return fill_labels(a, labels); });
+}
+
+cudnnStatus_t cudnnLinearCrossEntropyBackward(cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc,
+                                              const void* x, cudnnFilterDescriptor_t wDesc,
+                                              const void* w, const int64_t* labels,
+                                              const float* dloss, void* workSpace,
+                                              size_t workSpaceSizeInBytes, float* loss,
+                                              float* logSumExp, cudnnTensorDescriptor_t dxDesc,
+                                              void* dx, cudnnFilterDescriptor_t dwDesc, void* dw) {
+  return vocab_call(handle, xDesc, x, wDesc, w, true, dloss, workSpace, workSpaceSizeInBytes, loss,
+                    logSumExp, dxDesc, dx, dwDesc, dw,
+                    [&](VocabLossArgs& a) { return fill_labels(a, labels); });
+}
+
+cudnnStatus_t cudnnGetLinearDistillationWorkspaceSize(cudnnHandle_t handle,
+                                                      cudnnTensorDescriptor_t xDesc,
+                                                      cudnnFilterDescriptor_t wDesc, int topK,
+                                                      int gradients, size_t* sizeInBytes) {
+  if (topK < 1 || topK > mb200::dnn::kVocabMaxTopK) return CUDNN_STATUS_BAD_PARAM;
+  return vocab_workspace(handle, xDesc, wDesc, topK, gradients, sizeInBytes);
+}
+
+cudnnStatus_t cudnnLinearDistillationForward(cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc,
+                                             const void* x, cudnnFilterDescriptor_t wDesc,
+                                             const void* w, int topK, const int64_t* teacherIndex,
+                                             const float* teacherLogits, double temperature,
+                                             void* workSpace, size_t workSpaceSizeInBytes,
+                                             float* loss, float* logSumExp) {
+  return vocab_call(handle, xDesc, x, wDesc, w, false, nullptr, workSpace, workSpaceSizeInBytes,
+                    loss, logSumExp, nullptr, nullptr, nullptr, nullptr, [&](VocabLossArgs& a) {
+                      return fill_teacher(a, topK, teacherIndex, teacherLogits, temperature);
+                    });
+}
+
+cudnnStatus_t cudnnLinearDistillationBackward(cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc,
+                                              const void* x, cudnnFilterDescriptor_t wDesc,
+                                              const void* w, int topK, const int64_t* teacherIndex,
+                                              const float* teacherLogits, double temperature,
+                                              const float* dloss, void* workSpace,
+                                              size_t workSpaceSizeInBytes, float* loss,
+                                              float* logSumExp, cudnnTensorDescriptor_t dxDesc,
+                                              void* dx, cudnnFilterDescriptor_t dwDesc, void* dw) {
+  return vocab_call(handle, xDesc, x, wDesc, w, true, dloss, workSpace, workSpaceSizeInBytes, loss,
+                    logSumExp, dxDesc, dx, dwDesc, dw, [&](VocabLossArgs& a) {
+                      return fill_teacher(a, topK, teacherIndex, teacherLogits, temperature);
+                    });
 }
 
 }  // extern "C"

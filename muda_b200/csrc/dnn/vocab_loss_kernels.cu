@@ -1,0 +1,1111 @@
+// vocab_loss_kernels.cu — losses over a linear head's vocabulary, and their gradients
+// (sm_100a, tcgen05).  The mathematics is stated in vocab_loss.hpp.
+//
+// The T x V logits z = x w^T / tau never exist in memory as such.  A call runs over
+// pieces of tokens; in each piece
+//   1. vocab_logits_kernel walks 128-token x BN-word tiles of z.  The fp32 tile stays in
+//      tensor memory; the epilogue reduces it to one (reference, sum) pair per token and
+//      tile, lse's running maximum and sum, and picks the target words' logits.  With
+//      gradients it also writes the tile's numerators 2^(z2 - reference) in 16 bits;
+//   2. vocab_finish_kernel joins a token's pairs into its log-sum-exp and loss, and turns
+//      the numerators in place into dz = dloss / tau * (p - q);
+//   3. dx = dz w and dw = dz^T x run on the framework's persistent tensor-core loop.
+// All exponents are in powers of two: z2 = z * log2(e), with log2(e) / tau folded into one
+// multiply, so that 2^(z2 - reference) is one fma and one ex2.
+//
+// Precision: products of the 16-bit inputs accumulate in fp32; maxima, sums, target
+// logits and losses are fp32.  The numerators are rounded to 16 bits in step 1 and again
+// in step 2 (dz is a 16-bit operand of the tensor cores either way; keeping fp32
+// numerators would double the piece's traffic).  The target words, whose p - q cancels,
+// are recomputed in step 2 from their fp32 logits and rounded once.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <array>
+#include <climits>
+#include <cstdint>
+#include <mutex>
+#include <type_traits>
+
+#include "blas/tc_gemm_core.cuh"
+#include "common/device.hpp"
+#include "dnn/vocab_loss.hpp"
+
+namespace mb200::dnn {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kGroupM = 16;  // tile rows visited together, so CTAs in flight share panels in L2
+
+__device__ unsigned int g_vocab_timeouts;
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ std::uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const std::uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const std::uint32_t*>(&h);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float2 unpack2(std::uint32_t v) {
+  if constexpr (std::is_same_v<T, __half>)
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+  else
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+
+template <typename T>
+__device__ __forceinline__ T from_float(float v) {
+  if constexpr (std::is_same_v<T, __half>)
+    return __float2half_rn(v);
+  else
+    return __float2bfloat16_rn(v);
+}
+
+// Target words of the rows of a piece.  Cross entropy: top_k == 0, one label per row.
+// Distillation: per row `count` entries sorted by index (vocab_targets_kernel).
+struct Targets {
+  const std::int64_t* labels;
+  int top_k;
+  const int* index;       // [row][top_k], ascending, INT_MAX behind the valid entries
+  const float* q;         // [row][top_k]
+  const int* count;       // valid entries; 0: row left out, -1: an index of vocab or more
+  const float* neg_entropy;  // sum q log q
+  float* z2;              // [row][max(top_k, 1)]: the target words' z2
+};
+
+// 0: left out, -1: out-of-range target, else the number of target words.
+__device__ __forceinline__ int target_count(const Targets& t, int row, int vocab) {
+  if (t.top_k > 0) return t.count[row];
+  const std::int64_t l = t.labels[row];
+  return l < 0 ? 0 : l >= vocab ? -1 : 1;
+}
+
+// ------------------------------------------------------------------ logits kernel --
+struct LogitsProblem {
+  CUtensorMap mx;  // x: dims (features, rows), box {64, 128, 1}
+  CUtensorMap mw;  // w: dims (features, vocab), box {64, BN, 1}
+  long long tiles_total;
+  int num_kb, rows, vocab, tiles_m, tiles_n;
+  float scale;        // log2(e) / tau
+  float2* stats;      // [row][tiles_n] (reference, sum of 2^(z2 - reference))
+  void* num;          // [row][ldn] numerators (gradients only)
+  std::int64_t ldn;
+  Targets targets;
+
+  __device__ void coords(long long t, int* m, int* n) const {
+    const int in_group = kGroupM * tiles_n;
+    const int r = static_cast<int>(t);
+    const int first = (r / in_group) * kGroupM;
+    const int gsz = min(tiles_m - first, kGroupM);
+    *m = first + (r % in_group) % gsz;
+    *n = (r % in_group) / gsz;
+  }
+};
+
+__device__ __forceinline__ float pick32(const float (&v)[32], int j) {
+  float r = v[0];
+#pragma unroll
+  for (int i = 1; i < 32; ++i) r = (i == j) ? v[i] : r;
+  return r;
+}
+
+// The loop of tc_gemm_core.cuh (TMA producer, MMA issuer, four epilogue warps, two
+// accumulators) with an epilogue that sees a token's whole tile row: it reads the row
+// from tensor memory twice, for the maximum and for the numerators.
+template <typename T, int FMT, int BN, int STAGES, bool STORE>
+__global__ void __launch_bounds__(tc::kThreads, 1)
+    vocab_logits_kernel(const __grid_constant__ LogitsProblem p, unsigned int* timeouts) {
+  using namespace tc;
+  using S = CoreShape<BN, STAGES, 1>;
+  extern __shared__ std::uint8_t smem_raw[];
+  std::uint8_t* base = reinterpret_cast<std::uint8_t*>(
+      (reinterpret_cast<std::uintptr_t>(smem_raw) + 1023) & ~std::uintptr_t{1023});
+  std::uint8_t* sa = base;
+  std::uint8_t* sb = base + STAGES * S::A_STAGE;
+  std::uint64_t* full = reinterpret_cast<std::uint64_t*>(sb + STAGES * S::B_STAGE);
+  std::uint64_t* empty = full + STAGES;
+  std::uint64_t* acc_full = empty + STAGES;
+  std::uint64_t* acc_empty = acc_full + kAcc;
+  std::uint64_t* mma_done = acc_empty + kAcc;
+  std::uint32_t* tmem_slot = reinterpret_cast<std::uint32_t*>(mma_done + 1);
+  volatile int* aborted = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < kAcc; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 4);
+    }
+    mbar_init(mma_done, 1);
+    *aborted = 0;
+    mbar_fence_init();
+    prefetch_tensormap(&p.mx);
+    prefetch_tensormap(&p.mw);
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, S::TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const std::uint32_t tmem_base = *tmem_slot;
+  const int num_kb = p.num_kb;
+  auto fail = [&]() {
+    *aborted = 1;
+    atomicAdd(timeouts, 1u);
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      std::uint32_t phase = 0;
+      std::uint32_t issued_phase[STAGES];
+      bool issued[STAGES];
+      for (int s = 0; s < STAGES; ++s) issued[s] = false;
+      for (long long t = blockIdx.x; t < p.tiles_total && !*aborted; t += gridDim.x) {
+        int m, n;
+        p.coords(t, &m, &n);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1u)) {
+            fail();
+            break;
+          }
+          mbar_arrive_expect_tx(&full[stage], S::A_STAGE + S::B_STAGE);
+          tma_load_3d(sa + stage * S::A_STAGE, &p.mx, kb * kBK, m * kBM, 0, &full[stage]);
+          tma_load_3d(sb + stage * S::B_STAGE, &p.mw, kb * kBK, n * BN, 0, &full[stage]);
+          issued[stage] = true;
+          issued_phase[stage] = phase;
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      for (int s = 0; s < STAGES; ++s)
+        if (issued[s] && !mbar_wait(&full[s], issued_phase[s])) fail();
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr std::uint32_t idesc = f16_idesc(FMT, kBM, BN);
+      int stage = 0;
+      std::uint32_t phase = 0;
+      int acc = 0;
+      std::uint32_t acc_phase = 0;
+      for (long long t = blockIdx.x; t < p.tiles_total && !*aborted; t += gridDim.x) {
+        if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1u)) {
+          fail();
+          break;
+        }
+        tc_fence_after();
+        const std::uint32_t d_tmem = tmem_base + static_cast<std::uint32_t>(acc * BN);
+        bool ok = true;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&full[stage], phase)) {
+            fail();
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const std::uint32_t a0 = smem_addr(sa + stage * S::A_STAGE);
+          const std::uint32_t b0 = smem_addr(sb + stage * S::B_STAGE);
+#pragma unroll
+          for (int k = 0; k < kRowBytes / kStepBytes; ++k)
+            mma_f16(d_tmem, operand_desc<false>(a0, k), operand_desc<false>(b0, k), idesc,
+                    (kb | k) != 0 ? 1u : 0u);
+          mma_commit(&empty[stage]);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        mma_commit(&acc_full[acc]);
+        if (++acc == kAcc) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+      mma_commit(mma_done);
+      if (!mbar_wait(mma_done, 0)) fail();
+    }
+  } else {
+    const int quarter = warp & 3;
+    int acc = 0;
+    std::uint32_t acc_phase = 0;
+    for (long long t = blockIdx.x; t < p.tiles_total && !*aborted; t += gridDim.x) {
+      int mt, nt;
+      p.coords(t, &mt, &nt);
+      const int row = mt * kBM + quarter * 32 + lane;
+      const bool live = row < p.rows;
+      const int n0 = nt * BN;
+      const int cols = min(BN, p.vocab - n0);  // words of this tile
+
+      // this row's first target word at or after n0 (none: INT_MAX)
+      const int tk = max(p.targets.top_k, 1);
+      int next = INT_MAX, at = 0;
+      if (live) {
+        if (p.targets.top_k == 0) {
+          const std::int64_t l = p.targets.labels[row];
+          if (l >= n0 && l < n0 + cols) next = static_cast<int>(l);
+        } else {
+          const int* idx = p.targets.index + static_cast<std::int64_t>(row) * tk;
+          int hi = tk;
+          while (at < hi) {
+            const int mid = (at + hi) >> 1;
+            if (idx[mid] < n0) at = mid + 1; else hi = mid;
+          }
+          if (at < tk) next = idx[at];
+        }
+      }
+
+      if (!mbar_wait(&acc_full[acc], acc_phase)) {
+        fail();
+        break;
+      }
+      tc_fence_after();
+      const std::uint32_t t_row = tmem_base + (static_cast<std::uint32_t>(quarter * 32) << 16) +
+                                  static_cast<std::uint32_t>(acc * BN);
+      float mx = -INFINITY;
+#pragma unroll 1
+      for (int c0 = 0; c0 < cols; c0 += 32) {
+        float v[32];
+        __syncwarp();  // the load is a whole warp's
+        tmem_load_32cols(t_row + static_cast<std::uint32_t>(c0), v);
+        if (c0 + 32 <= cols) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) mx = fmaxf(mx, v[j]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c0 + j < cols) mx = fmaxf(mx, v[j]);
+        }
+      }
+      // a row of -inf (or NaN) has no finite maximum: 0 keeps -inf's numerators at 0
+      const float ref = mx == -INFINITY ? 0.0f : __fmul_rn(mx, p.scale);
+      float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+      for (int c0 = 0; c0 < cols; c0 += 32) {
+        float v[32];
+        __syncwarp();  // the load is a whole warp's
+        tmem_load_32cols(t_row + static_cast<std::uint32_t>(c0), v);
+        while (next < n0 + c0 + 32) {  // rare: a target word among these 32
+          const float z2 = __fmul_rn(pick32(v, next - n0 - c0), p.scale);
+          p.targets.z2[static_cast<std::int64_t>(row) * tk + at] = z2;
+          ++at;
+          next = at < p.targets.top_k
+                     ? p.targets.index[static_cast<std::int64_t>(row) * tk + at] : INT_MAX;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = exp2_approx(fmaf(v[j], p.scale, -ref));
+        if (c0 + 32 > cols) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c0 + j >= cols) v[j] = 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; ++j) s[j & 3] += v[j];
+        if constexpr (STORE) {
+          if (live) {
+            T* out = static_cast<T*>(p.num) + static_cast<std::int64_t>(row) * p.ldn + n0 + c0;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              if (n0 + c0 + 8 * g < p.ldn)
+                *reinterpret_cast<uint4*>(out + 8 * g) =
+                    make_uint4(pack2<T>(v[8 * g], v[8 * g + 1]), pack2<T>(v[8 * g + 2], v[8 * g + 3]),
+                               pack2<T>(v[8 * g + 4], v[8 * g + 5]),
+                               pack2<T>(v[8 * g + 6], v[8 * g + 7]));
+            }
+          }
+        }
+      }
+      if (live)
+        p.stats[static_cast<std::int64_t>(row) * p.tiles_n + nt] =
+            make_float2(ref, (s[0] + s[1]) + (s[2] + s[3]));
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[acc]);
+      if (++acc == kAcc) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, S::TMEM_COLS);
+  }
+}
+
+// ----------------------------------------------------------------- small kernels --
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+__device__ __forceinline__ int warp_sum(int v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// One warp per token: the teacher's distribution over the valid entries, and the entries
+// sorted by word (rank counting: top_k^2 / 32 comparisons per lane).
+constexpr int kTargetWarps = 4;
+
+__global__ void __launch_bounds__(32 * kTargetWarps)
+    vocab_targets_kernel(const std::int64_t* __restrict__ teacher_index,
+                         const float* __restrict__ teacher_logits, int rows, int top_k, int vocab,
+                         float inv_tau, int* __restrict__ index, float* __restrict__ q,
+                         int* __restrict__ count, float* __restrict__ neg_entropy) {
+  __shared__ int key_all[kTargetWarps][kVocabMaxTopK];
+  const int lane = threadIdx.x & 31;
+  int* key = key_all[threadIdx.x >> 5];
+  const int row = blockIdx.x * kTargetWarps + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const std::int64_t r0 = static_cast<std::int64_t>(row) * top_k;
+  float mx = -INFINITY;
+  int valid = 0, bad = 0;
+  for (int k = lane; k < top_k; k += 32) {
+    const std::int64_t i = teacher_index[r0 + k];
+    const float t = teacher_logits[r0 + k];
+    const bool ok = i >= 0 && i < vocab && t != -INFINITY;
+    bad |= i >= vocab;
+    key[k] = ok ? static_cast<int>(i) : INT_MAX;
+    if (ok) {
+      mx = fmaxf(mx, t * inv_tau);
+      ++valid;
+    }
+  }
+  __syncwarp();
+  mx = warp_max(mx);
+  valid = warp_sum(valid);
+  bad = __any_sync(0xffffffffu, bad);
+  float total = 0.0f;
+  for (int k = lane; k < top_k; k += 32)
+    if (key[k] != INT_MAX) total += expf(teacher_logits[r0 + k] * inv_tau - mx);
+  total = warp_sum(total);
+  const float log_total = logf(total);
+  float ent = 0.0f;
+  for (int k = lane; k < top_k; k += 32) {
+    const int mine = key[k];
+    int rank = 0;
+    for (int j = 0; j < top_k; ++j) rank += key[j] < mine || (key[j] == mine && j < k);
+    float qk = 0.0f;
+    if (mine != INT_MAX) {
+      const float d = teacher_logits[r0 + k] * inv_tau - mx;
+      qk = expf(d) / total;
+      if (qk != 0.0f) ent += qk * (d - log_total);
+    }
+    index[r0 + rank] = mine;
+    q[r0 + rank] = qk;
+  }
+  ent = warp_sum(ent);
+  if (lane == 0) {
+    count[row] = bad ? -1 : valid;
+    neg_entropy[row] = ent;
+  }
+}
+
+// fp16 only: a power of two that brings the piece's largest |dloss / tau| (over the rows
+// that are not left out) to [2^13, 2^14), so dz, at most that in magnitude, fills fp16's
+// range; scale[1] undoes it after the products.
+__global__ void __launch_bounds__(1024)
+    vocab_grad_scale_kernel(const float* __restrict__ dloss, int rows, int vocab, Targets targets,
+                            float inv_tau, float* __restrict__ scale) {
+  __shared__ float red[32];
+  float mx = 0.0f;
+  for (int i = threadIdx.x; i < rows; i += 1024) {
+    const float g = fabsf(dloss[i] * inv_tau);
+    if (target_count(targets, i, vocab) > 0 && g < INFINITY) mx = fmaxf(mx, g);
+  }
+  mx = warp_max(mx);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mx;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    mx = warp_max(red[threadIdx.x]);
+    if (threadIdx.x == 0) {
+      int e = 0;
+      if (mx > 0.0f) frexpf(mx, &e);  // mx in [2^(e-1), 2^e)
+      e = max(-100, min(100, e));
+      scale[0] = ldexpf(1.0f, 14 - e);
+      scale[1] = ldexpf(1.0f, e - 14);
+    }
+  }
+}
+
+constexpr int kFinishThreads = 256;
+
+__device__ __forceinline__ float block_reduce(float v, bool is_max, float* red) {
+  v = is_max ? warp_max(v) : warp_sum(v);
+  __syncthreads();  // red[] may still be read by the previous reduction
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float r = red[0];
+#pragma unroll
+  for (int i = 1; i < kFinishThreads / 32; ++i) r = is_max ? fmaxf(r, red[i]) : r + red[i];
+  return r;
+}
+
+struct FinishArgs {
+  const float2* stats;  // [row][tiles_n]
+  int tiles_n, bn, rows, vocab;
+  Targets targets;
+  float* loss;  // may be null
+  float* lse;   // may be null
+  const float* dloss;
+  float inv_tau;
+  const float* scale;  // fp16: the gradient scale, else null
+  void* num;
+  std::int64_t ldn;
+};
+
+// One row per blockIdx.x; blockIdx.y splits its words (each split joins the row's pairs
+// again, a few KB from L2).
+template <typename T, bool GRAD>
+__global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const FinishArgs a) {
+  __shared__ float red[kFinishThreads / 32];
+  const int row = blockIdx.x;
+  const int n = target_count(a.targets, row, a.vocab);
+  const std::int64_t chunks = a.ldn / 8;
+  const std::int64_t per = (chunks + gridDim.y - 1) / gridDim.y;
+  const std::int64_t c_begin = per * blockIdx.y, c_end = min(chunks, c_begin + per);
+  uint4* num = reinterpret_cast<uint4*>(static_cast<T*>(a.num) + row * a.ldn);
+  if (n == 0) {  // left out
+    if (blockIdx.y == 0 && threadIdx.x == 0) {
+      if (a.loss != nullptr) a.loss[row] = 0.0f;
+      if (a.lse != nullptr) a.lse[row] = 0.0f;
+    }
+    if constexpr (GRAD) {
+      for (std::int64_t c = c_begin + threadIdx.x; c < c_end; c += kFinishThreads)
+        num[c] = make_uint4(0, 0, 0, 0);
+    }
+    return;
+  }
+  const float2* st = a.stats + static_cast<std::int64_t>(row) * a.tiles_n;
+  float mx = -INFINITY;
+  for (int i = threadIdx.x; i < a.tiles_n; i += kFinishThreads)
+    if (st[i].y != 0.0f) mx = fmaxf(mx, st[i].x);
+  mx = block_reduce(mx, true, red);
+  float sum = 0.0f;
+  for (int i = threadIdx.x; i < a.tiles_n; i += kFinishThreads)
+    if (st[i].y != 0.0f) sum += st[i].y * exp2f(st[i].x - mx);
+  sum = block_reduce(sum, false, red);
+  const float lse2 = mx + log2f(sum);
+
+  const int tk = max(a.targets.top_k, 1);
+  const std::int64_t r0 = static_cast<std::int64_t>(row) * tk;
+  if (blockIdx.y == 0) {
+    float loss;
+    if (n < 0) {
+      loss = NAN;
+    } else if (a.targets.top_k == 0) {
+      loss = (lse2 - a.targets.z2[r0]) * kLn2;
+    } else {
+      float cross = 0.0f;
+      for (int k = threadIdx.x; k < n; k += kFinishThreads)
+        if (a.targets.q[r0 + k] != 0.0f)
+          cross += a.targets.q[r0 + k] * ((lse2 - a.targets.z2[r0 + k]) * kLn2);
+      loss = a.targets.neg_entropy[row] + block_reduce(cross, false, red);
+    }
+    if (threadIdx.x == 0) {
+      if (a.loss != nullptr) a.loss[row] = loss;
+      if (a.lse != nullptr) a.lse[row] = lse2 * kLn2;
+    }
+  }
+  if constexpr (GRAD) {
+    float g = n < 0 ? NAN : a.dloss[row] * a.inv_tau;
+    if (a.scale != nullptr) g *= a.scale[0];
+    for (std::int64_t c = c_begin + threadIdx.x; c < c_end; c += kFinishThreads) {
+      const float f = g * exp2f(st[c * 8 / a.bn].x - lse2);
+      uint4 u = num[c];
+      std::uint32_t* w = reinterpret_cast<std::uint32_t*>(&u);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 v = unpack2<T>(w[j]);
+        w[j] = pack2<T>(f * v.x, f * v.y);
+      }
+      num[c] = u;
+    }
+    __syncthreads();
+    T* d = static_cast<T*>(a.num) + row * a.ldn;
+    if (a.targets.top_k == 0) {
+      const std::int64_t l = a.targets.labels[row];
+      if (threadIdx.x == 0 && n > 0 && l >= c_begin * 8 && l < c_end * 8)
+        d[l] = from_float<T>(g * expm1f((a.targets.z2[r0] - lse2) * kLn2));
+    } else {
+      for (int k = threadIdx.x; k < n; k += kFinishThreads) {
+        const int w = a.targets.index[r0 + k];
+        if (w < c_begin * 8 || w >= c_end * 8) continue;
+        if (k > 0 && a.targets.index[r0 + k - 1] == w) continue;  // the run's first entry adds all
+        float q = a.targets.q[r0 + k];
+        for (int j = k + 1; j < n && a.targets.index[r0 + j] == w; ++j) q += a.targets.q[r0 + j];
+        d[w] = from_float<T>(g * (exp2f(a.targets.z2[r0 + k] - lse2) - q));
+      }
+    }
+  }
+}
+
+// xt[h][row] = x[row][h], rows that are left out as zeros (their x may hold anything, and
+// 0 * NaN would reach dw).  K-major x for dw's product: reading x MN-major instead would
+// make both operands MN-major, the slowest form of the tensor-core loop.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    vocab_transpose_kernel(const T* __restrict__ x, std::int64_t ldx, int rows, int features,
+                           Targets targets, int vocab, T* __restrict__ xt, std::int64_t ldt) {
+  __shared__ T tile[64][66];
+  const int r0 = blockIdx.x * 64, h0 = blockIdx.y * 64;
+  const int lx = threadIdx.x & 63, ly = threadIdx.x >> 6;
+  for (int i = ly; i < 64; i += 4) {
+    const int r = r0 + i, h = h0 + lx;
+    T v = from_float<T>(0.0f);
+    if (r < rows && h < features && target_count(targets, r, vocab) != 0) v = x[r * ldx + h];
+    tile[i][lx] = v;
+  }
+  __syncthreads();
+  for (int i = ly; i < 64; i += 4) {
+    const int h = h0 + i, r = r0 + lx;
+    if (h < features && r < rows) xt[h * ldt + r] = tile[lx][i];
+  }
+}
+
+// dst[r][c] = src[r][c] into rows of ldd elements: operands that TMA cannot read in place.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    vocab_pack_kernel(const T* __restrict__ src, std::int64_t lds, std::int64_t rows, int cols,
+                      T* __restrict__ dst, std::int64_t ldd) {
+  for (std::int64_t r = blockIdx.x; r < rows; r += gridDim.x)
+    for (int c = threadIdx.x; c < cols; c += 256) dst[r * ldd + c] = src[r * lds + c];
+}
+
+// ------------------------------------------------------------------ gradient GEMMs --
+// dx^T = w^T dz^T: A = w^T is MN-major in w, B = dz is K-major, the fastest operand forms
+// of the loop; a thread's 32 columns are 32 tokens of one feature, so a warp's stores of
+// one token are 32 consecutive features.  The words (K) split across `ksplit` CTAs.
+template <typename T, int BN>
+struct DxProblem {
+  static constexpr bool kAMn = true, kBMn = false;
+  CUtensorMap ma;  // w: dims (features, vocab), box {64, 64, 1}
+  CUtensorMap mb;  // dz: dims (vocab, rows), box {64, BN, 1}
+  long long tiles_total;
+  int num_kb;  // k-blocks per split
+  int rows, features, tiles_m, tiles_n;
+  T* dx;
+  std::int64_t lddx;
+  float* partial;  // ksplit > 1: [split][row][feature]
+  const float* scale;
+
+  __device__ void prefetch() const {
+    tc::prefetch_tensormap(&ma);
+    tc::prefetch_tensormap(&mb);
+  }
+  __device__ void coords(long long t, int (&c)[3]) const {
+    const int per = tiles_m * tiles_n;
+    const int r = static_cast<int>(t % per);
+    c[0] = static_cast<int>(t / per);
+    const int in_group = kGroupM * tiles_n;
+    const int first = (r / in_group) * kGroupM;
+    const int gsz = min(tiles_m - first, kGroupM);
+    c[1] = first + (r % in_group) % gsz;
+    c[2] = (r % in_group) / gsz;
+  }
+  __device__ void load(const int (&c)[3], int kb, void* sa, void* sb, std::uint64_t* bar) const {
+    const int k = (c[0] * num_kb + kb) * tc::kBK;  // past the vocabulary: zeros
+#pragma unroll
+    for (int j = 0; j < tc::kBM / 64; ++j)
+      tc::tma_load_3d(static_cast<std::uint8_t*>(sa) + j * tc::kMnBoxBytes, &ma,
+                      c[1] * tc::kBM + 64 * j, k, 0, bar);
+    tc::tma_load_3d(sb, &mb, k, c[2] * BN, 0, bar);
+  }
+  __device__ void scalars(float& a, float& b) const {
+    a = scale != nullptr ? scale[1] : 1.0f;
+    b = 0.0f;
+  }
+  __device__ void store(const int (&c)[3], int row, int col0, const float (&v)[32], float a,
+                        float) const {
+    const int h = c[1] * tc::kBM + row;
+    if (h >= features) return;
+    const int t0 = c[2] * BN + col0;
+    if (partial != nullptr) {
+      float* o = partial + (static_cast<std::int64_t>(c[0]) * rows + t0) * features + h;
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (t0 + j < rows) o[static_cast<std::int64_t>(j) * features] = v[j];
+      return;
+    }
+    T* o = dx + static_cast<std::int64_t>(t0) * lddx + h;
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (t0 + j < rows) o[j * lddx] = from_float<T>(a * v[j]);
+  }
+};
+
+// dx = scale * (sum of the splits, in split order).
+template <typename T>
+__global__ void __launch_bounds__(256)
+    vocab_dx_reduce_kernel(const float* __restrict__ partial, int ksplit, int rows, int features,
+                           T* __restrict__ dx, std::int64_t lddx, const float* scale) {
+  const float a = scale != nullptr ? scale[1] : 1.0f;
+  const std::int64_t plane = static_cast<std::int64_t>(rows) * features;
+  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+    for (int h = blockIdx.x * 256 + threadIdx.x; h < features; h += gridDim.x * 256) {
+      const float* p = partial + static_cast<std::int64_t>(r) * features + h;
+      float s = p[0];
+      for (int i = 1; i < ksplit; ++i) s += p[i * plane];
+      dx[r * lddx + h] = from_float<T>(a * s);
+    }
+  }
+}
+
+// dw = dz^T x: A = dz^T is MN-major in dz, B = x^T (transposed copy) K-major.  A call of
+// several pieces adds its pieces in fp32 and rounds once, in the last.
+template <typename T>
+struct DwProblem {
+  static constexpr bool kAMn = true, kBMn = false;
+  static constexpr int BN = 256;
+  CUtensorMap ma;  // dz: dims (vocab, rows), box {64, 64, 1}
+  CUtensorMap mb;  // x^T: dims (rows, features), box {64, 256, 1}
+  long long tiles_total;
+  int num_kb;
+  int vocab, features, tiles_m, tiles_n;
+  T* dw;
+  float* sum;  // pieces: [word][feature] running sum, else null
+  bool first, last;
+  bool vec;    // dw's 8-element runs are 16-byte aligned
+  const float* scale;
+
+  __device__ void prefetch() const {
+    tc::prefetch_tensormap(&ma);
+    tc::prefetch_tensormap(&mb);
+  }
+  __device__ void coords(long long t, int (&c)[3]) const {
+    const int r = static_cast<int>(t);
+    const int in_group = kGroupM * tiles_n;
+    const int group0 = (r / in_group) * kGroupM;
+    const int gsz = min(tiles_m - group0, kGroupM);
+    c[0] = 0;
+    c[1] = group0 + (r % in_group) % gsz;
+    c[2] = (r % in_group) / gsz;
+  }
+  __device__ void load(const int (&c)[3], int kb, void* sa, void* sb, std::uint64_t* bar) const {
+#pragma unroll
+    for (int j = 0; j < tc::kBM / 64; ++j)
+      tc::tma_load_3d(static_cast<std::uint8_t*>(sa) + j * tc::kMnBoxBytes, &ma,
+                      c[1] * tc::kBM + 64 * j, kb * tc::kBK, 0, bar);
+    tc::tma_load_3d(sb, &mb, kb * tc::kBK, c[2] * BN, 0, bar);
+  }
+  __device__ void scalars(float& a, float& b) const {
+    a = scale != nullptr ? scale[1] : 1.0f;
+    b = 0.0f;
+  }
+  __device__ void store(const int (&c)[3], int row, int col0, const float (&v)[32], float a,
+                        float) const {
+    const int w = c[1] * tc::kBM + row;
+    if (w >= vocab) return;
+    const int h0 = c[2] * BN + col0;
+    const std::int64_t o = static_cast<std::int64_t>(w) * features + h0;
+    float r[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) r[j] = a * v[j];
+    if (sum != nullptr) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        if (h0 + j >= features) continue;
+        if (!first) r[j] += sum[o + j];
+        if (!last) sum[o + j] = r[j];
+      }
+      if (!last) return;
+    }
+    if (vec && h0 + 32 <= features) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<uint4*>(dw + o + 8 * g) =
+            make_uint4(pack2<T>(r[8 * g], r[8 * g + 1]), pack2<T>(r[8 * g + 2], r[8 * g + 3]),
+                       pack2<T>(r[8 * g + 4], r[8 * g + 5]), pack2<T>(r[8 * g + 6], r[8 * g + 7]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (h0 + j < features) dw[o + j] = from_float<T>(r[j]);
+    }
+  }
+};
+
+// ------------------------------------------------------------------------- planning --
+constexpr std::size_t kNumeratorCap = std::size_t{2} << 30;  // bytes of a piece's numerators
+constexpr int kScoreRows = 16384;                             // tokens of a piece without them
+
+std::int64_t round_up(std::int64_t v, std::int64_t m) { return (v + m - 1) / m * m; }
+
+int sms() {
+  const int n = sm_count(current_device());
+  return n > 0 ? n : 148;
+}
+
+// Words per tile of the logits kernel.
+int logits_bn(int rows) { return rows <= 128 ? 128 : 256; }
+
+// Tokens per tile of dx's product: a narrower tile does not multiply empty columns.
+int dx_bn(int rows) { return rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
+
+// Splits of the words in dx's product: the count that ends soonest, a wave of CTAs
+// taking 512 MMA clocks per k-block and each split's partial sums a write and a read.
+int dx_splits(int rows, int features, int vocab) {
+  const int bn = dx_bn(rows);
+  const std::int64_t tiles = ((features + tc::kBM - 1) / tc::kBM) * static_cast<std::int64_t>((rows + bn - 1) / bn);
+  const int kb = (vocab + tc::kBK - 1) / tc::kBK;
+  const int n = sms();
+  double best = 0.0;
+  int pick = 1;
+  for (int ks = 1; ks <= 16 && ks * 8 <= std::max(kb, 8); ++ks) {
+    const double waves = static_cast<double>((tiles * ks + n - 1) / n);
+    const double loop = waves * ((kb + ks - 1) / ks) * 512.0 * bn / 256 / 1.8e9;
+    const double join = ks == 1 ? 0.0 : 3e-6 + 8.0 * ks * rows * features / 4e12;
+    if (ks == 1 || loop + join < best) {
+      best = loop + join;
+      pick = ks;
+    }
+  }
+  return pick;
+}
+
+bool tma_rows_ok(const void* p, std::int64_t ld) { return aligned_to(p, 16) && ld % 8 == 0; }
+
+struct Plan {
+  int rows;    // tokens per piece (the last may have fewer)
+  int pieces;
+  int ksplit;
+  std::int64_t ldn;   // numerators' row
+  std::int64_t ldt;   // x^T's row
+  std::int64_t ldp;   // row of packed copies of x and w
+  bool pack_x, pack_w;
+  // byte offsets into the workspace
+  std::size_t stats, z2, index, q, count, entropy, scale, xp, wp, num, xt, partial, sum, bytes;
+};
+
+Plan plan_rows(const VocabLossArgs& a, int rows) {
+  Plan p{};
+  p.rows = rows;
+  p.pieces = (a.tokens + rows - 1) / rows;
+  p.ldn = round_up(a.vocab, 8);
+  p.ldt = round_up(rows, 8);
+  p.ldp = round_up(a.features, 8);
+  p.pack_x = a.tokens > 1 ? !tma_rows_ok(a.x, a.ldx) : !aligned_to(a.x, 16);
+  p.pack_w = !tma_rows_ok(a.w, a.features);
+  const bool dx = a.gradients && a.dx != nullptr, dw = a.gradients && a.dw != nullptr;
+  p.ksplit = dx ? dx_splits(rows, a.features, a.vocab) : 1;
+  std::size_t at = 0;
+  auto take = [&](std::size_t n) {
+    const std::size_t o = at;
+    at += (n + 255) / 256 * 256;
+    return o;
+  };
+  const std::size_t R = rows, H = a.features, V = a.vocab, K = a.top_k;
+  const std::size_t tiles_n = (V + logits_bn(rows) - 1) / logits_bn(rows);
+  p.stats = take(R * tiles_n * sizeof(float2));
+  p.z2 = take(R * std::max<std::size_t>(K, 1) * 4);
+  p.index = take(R * K * 4);
+  p.q = take(R * K * 4);
+  p.count = take(K > 0 ? R * 4 : 0);
+  p.entropy = take(K > 0 ? R * 4 : 0);
+  p.scale = take(8);
+  p.xp = take(p.pack_x ? R * p.ldp * 2 : 0);
+  p.wp = take(p.pack_w ? V * p.ldp * 2 : 0);
+  p.num = take(a.gradients ? R * p.ldn * 2 : 0);
+  p.xt = take(dw ? H * p.ldt * 2 : 0);
+  p.partial = take(p.ksplit > 1 ? p.ksplit * R * H * 4 : 0);
+  p.sum = take(dw && p.pieces > 1 ? V * H * 4 : 0);
+  p.bytes = at;
+  return p;
+}
+
+// Pieces of equal size, each at most what the caps allow.
+Plan plan_within(const VocabLossArgs& a, std::size_t limit, bool* ok) {
+  std::int64_t most = kScoreRows;
+  if (a.gradients)
+    most = std::max<std::int64_t>(128, static_cast<std::int64_t>(kNumeratorCap / (round_up(a.vocab, 8) * 2)) / 128 * 128);
+  int pieces = static_cast<int>((a.tokens + most - 1) / most);
+  Plan p{};
+  for (;;) {
+    std::int64_t rows = (a.tokens + pieces - 1) / pieces;
+    if (pieces > 1) rows = round_up(rows, 128);
+    p = plan_rows(a, static_cast<int>(std::min<std::int64_t>(rows, a.tokens)));
+    if (p.bytes <= limit) {
+      *ok = true;
+      return p;
+    }
+    if (rows <= 128) break;
+    // the next count that makes a piece smaller
+    pieces = static_cast<int>((a.tokens + rows - 128 - 1) / std::max<std::int64_t>(rows - 128, 1));
+  }
+  *ok = false;
+  return p;
+}
+
+// Map of 16-bit elements: `inner` contiguous, `outer` rows of ld elements.
+bool make_map(CUtensorMap* map, int fmt, const void* base, std::int64_t inner, std::int64_t outer,
+              std::int64_t ld, int box_inner, int box_outer) {
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer), 1u};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld * 2),
+                                 static_cast<cuuint64_t>(round_up(ld * 2, 16))};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_outer),
+                             1u};
+  return tc::encode_tiled(map, fmt, base, 3, dims, strides, box);
+}
+
+unsigned int* timeout_counter() {
+  static std::mutex mu;
+  static std::array<unsigned int*, 64> addr{};
+  const int dev = current_device();
+  if (dev < 0 || dev >= 64) return nullptr;
+  std::lock_guard<std::mutex> g(mu);
+  if (addr[dev] == nullptr) {
+    void* p = nullptr;
+    if (cudaGetSymbolAddress(&p, g_vocab_timeouts) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return nullptr;
+    }
+    addr[dev] = static_cast<unsigned int*>(p);
+  }
+  return addr[dev];
+}
+
+template <typename T, int FMT, int BN, int STAGES, bool STORE>
+cudaError_t run_logits(const LogitsProblem& p, unsigned int* timeouts, cudaStream_t st) {
+  using S = tc::CoreShape<BN, STAGES, 1>;
+  auto kern = vocab_logits_kernel<T, FMT, BN, STAGES, STORE>;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+  if (e != cudaSuccess) return e;
+  const unsigned grid = static_cast<unsigned>(std::min<long long>(p.tiles_total, sms()));
+  kern<<<grid, tc::kThreads, S::SMEM, st>>>(p, timeouts);
+  return cudaGetLastError();
+}
+
+#define MB200_TRY(expr)                       \
+  do {                                        \
+    const cudaError_t e_ = (expr);            \
+    if (e_ != cudaSuccess) return e_;         \
+  } while (0)
+
+template <typename T, int FMT, int BN>
+cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const void* w, std::int64_t ldw,
+                   const void* num, int rows, T* dx, char* ws, const float* scale,
+                   unsigned int* to, cudaStream_t st) {
+  DxProblem<T, BN> g{};
+  if (!make_map(&g.ma, FMT, w, a.features, a.vocab, ldw, 64, 64) ||
+      !make_map(&g.mb, FMT, num, a.vocab, rows, p.ldn, 64, BN))
+    return cudaErrorInvalidValue;
+  const int kb = (a.vocab + tc::kBK - 1) / tc::kBK;
+  g.num_kb = (kb + p.ksplit - 1) / p.ksplit;
+  const int ks = (kb + g.num_kb - 1) / g.num_kb;  // no split without words
+  g.rows = rows;
+  g.features = a.features;
+  g.tiles_m = (a.features + tc::kBM - 1) / tc::kBM;
+  g.tiles_n = (rows + BN - 1) / BN;
+  g.tiles_total = static_cast<long long>(g.tiles_m) * g.tiles_n * ks;
+  g.dx = dx;
+  g.lddx = a.lddx;
+  g.partial = ks > 1 ? reinterpret_cast<float*>(ws + p.partial) : nullptr;
+  g.scale = scale;
+  constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+  MB200_TRY((tc::launch_tc_gemm<DxProblem<T, BN>, BN, kStages, FMT>(g, sms(), to, st)));
+  if (ks > 1) {
+    const dim3 grid(static_cast<unsigned>((a.features + 255) / 256),
+                    static_cast<unsigned>(std::min(rows, 65535)));
+    vocab_dx_reduce_kernel<T><<<grid, 256, 0, st>>>(g.partial, ks, rows, a.features, dx, a.lddx,
+                                                    scale);
+    MB200_TRY(cudaGetLastError());
+  }
+  return cudaSuccess;
+}
+
+template <typename T, int FMT>
+cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st) {
+  unsigned int* to = timeout_counter();
+  if (to == nullptr) return cudaErrorInvalidDevice;
+  const T* w = static_cast<const T*>(a.w);
+  std::int64_t ldw = a.features;
+  if (p.pack_w) {
+    T* wp = reinterpret_cast<T*>(ws + p.wp);
+    vocab_pack_kernel<T><<<sms() * 8, 256, 0, st>>>(w, ldw, a.vocab, a.features, wp, p.ldp);
+    MB200_TRY(cudaGetLastError());
+    w = wp;
+    ldw = p.ldp;
+  }
+  T* num = reinterpret_cast<T*>(ws + p.num);
+  const int bn = logits_bn(p.rows);
+  for (int piece = 0; piece < p.pieces; ++piece) {
+    const std::int64_t t0 = static_cast<std::int64_t>(piece) * p.rows;
+    const int rows = static_cast<int>(std::min<std::int64_t>(p.rows, a.tokens - t0));
+    const T* x = static_cast<const T*>(a.x) + t0 * a.ldx;
+    std::int64_t ldx = a.tokens > 1 ? a.ldx : p.ldp;  // one row: its stride is never used
+    if (p.pack_x) {
+      T* xp = reinterpret_cast<T*>(ws + p.xp);
+      vocab_pack_kernel<T><<<std::min(rows, sms() * 8), 256, 0, st>>>(x, ldx, rows, a.features, xp,
+                                                                      p.ldp);
+      MB200_TRY(cudaGetLastError());
+      x = xp;
+      ldx = p.ldp;
+    }
+    Targets tg{};
+    tg.top_k = a.top_k;
+    tg.z2 = reinterpret_cast<float*>(ws + p.z2);
+    if (a.top_k == 0) {
+      tg.labels = a.labels + t0;
+    } else {
+      int* index = reinterpret_cast<int*>(ws + p.index);
+      float* q = reinterpret_cast<float*>(ws + p.q);
+      int* count = reinterpret_cast<int*>(ws + p.count);
+      float* ent = reinterpret_cast<float*>(ws + p.entropy);
+      vocab_targets_kernel<<<(rows + kTargetWarps - 1) / kTargetWarps, 32 * kTargetWarps, 0, st>>>(
+          a.teacher_index + t0 * a.top_k, a.teacher_logits + t0 * a.top_k, rows, a.top_k, a.vocab,
+          a.inv_tau, index, q, count, ent);
+      MB200_TRY(cudaGetLastError());
+      tg.index = index;
+      tg.q = q;
+      tg.count = count;
+      tg.neg_entropy = ent;
+    }
+
+    float* scale = nullptr;
+    if (a.gradients && !a.bf16) {
+      scale = reinterpret_cast<float*>(ws + p.scale);
+      vocab_grad_scale_kernel<<<1, 1024, 0, st>>>(a.dloss + t0, rows, a.vocab, tg, a.inv_tau,
+                                                  scale);
+      MB200_TRY(cudaGetLastError());
+    }
+
+    LogitsProblem lp{};
+    if (!make_map(&lp.mx, FMT, x, a.features, rows, ldx, tc::kBK, tc::kBM) ||
+        !make_map(&lp.mw, FMT, w, a.features, a.vocab, ldw, tc::kBK, bn))
+      return cudaErrorInvalidValue;
+    lp.num_kb = (a.features + tc::kBK - 1) / tc::kBK;
+    lp.rows = rows;
+    lp.vocab = a.vocab;
+    lp.tiles_m = (rows + tc::kBM - 1) / tc::kBM;
+    lp.tiles_n = (a.vocab + bn - 1) / bn;
+    lp.tiles_total = static_cast<long long>(lp.tiles_m) * lp.tiles_n;
+    lp.scale = kLog2e * a.inv_tau;
+    lp.stats = reinterpret_cast<float2*>(ws + p.stats);
+    lp.num = num;
+    lp.ldn = p.ldn;
+    lp.targets = tg;
+    if (bn == 128)
+      MB200_TRY((a.gradients ? run_logits<T, FMT, 128, 6, true>(lp, to, st)
+                             : run_logits<T, FMT, 128, 6, false>(lp, to, st)));
+    else
+      MB200_TRY((a.gradients ? run_logits<T, FMT, 256, 4, true>(lp, to, st)
+                             : run_logits<T, FMT, 256, 4, false>(lp, to, st)));
+
+    FinishArgs f{};
+    f.stats = lp.stats;
+    f.tiles_n = lp.tiles_n;
+    f.bn = bn;
+    f.rows = rows;
+    f.vocab = a.vocab;
+    f.targets = tg;
+    f.loss = a.loss != nullptr ? a.loss + t0 : nullptr;
+    f.lse = a.lse != nullptr ? a.lse + t0 : nullptr;
+    f.inv_tau = a.inv_tau;
+    f.scale = scale;
+    f.num = num;
+    f.ldn = p.ldn;
+    if (!a.gradients) {
+      vocab_finish_kernel<T, false><<<rows, kFinishThreads, 0, st>>>(f);
+      MB200_TRY(cudaGetLastError());
+      continue;
+    }
+    f.dloss = a.dloss + t0;
+    // enough CTAs to fill the GPU when there are few rows, each at least 8192 words
+    const int parts = std::max(1, std::min<int>(4 * sms() / rows, static_cast<int>((p.ldn + 8191) / 8192)));
+    vocab_finish_kernel<T, true><<<dim3(rows, parts), kFinishThreads, 0, st>>>(f);
+    MB200_TRY(cudaGetLastError());
+
+    T* xt = reinterpret_cast<T*>(ws + p.xt);
+    if (a.dw != nullptr) {  // before dx, which may be x itself
+      vocab_transpose_kernel<T><<<dim3((rows + 63) / 64, (a.features + 63) / 64), 256, 0, st>>>(
+          x, ldx, rows, a.features, tg, a.vocab, xt, p.ldt);
+      MB200_TRY(cudaGetLastError());
+    }
+    if (a.dx != nullptr) {
+      T* dx = static_cast<T*>(a.dx) + t0 * a.lddx;
+      const int bx = dx_bn(rows);
+      if (bx == 64)
+        MB200_TRY((run_dx<T, FMT, 64>(a, p, w, ldw, num, rows, dx, ws, scale, to, st)));
+      else if (bx == 128)
+        MB200_TRY((run_dx<T, FMT, 128>(a, p, w, ldw, num, rows, dx, ws, scale, to, st)));
+      else
+        MB200_TRY((run_dx<T, FMT, 256>(a, p, w, ldw, num, rows, dx, ws, scale, to, st)));
+    }
+    if (a.dw != nullptr) {
+      DwProblem<T> g{};
+      if (!make_map(&g.ma, FMT, num, a.vocab, rows, p.ldn, 64, 64) ||
+          !make_map(&g.mb, FMT, xt, rows, a.features, p.ldt, tc::kBK, 256))
+        return cudaErrorInvalidValue;
+      g.num_kb = (rows + tc::kBK - 1) / tc::kBK;
+      g.vocab = a.vocab;
+      g.features = a.features;
+      g.tiles_m = (a.vocab + tc::kBM - 1) / tc::kBM;
+      g.tiles_n = (a.features + 255) / 256;
+      g.tiles_total = static_cast<long long>(g.tiles_m) * g.tiles_n;
+      g.dw = static_cast<T*>(a.dw);
+      g.sum = p.pieces > 1 ? reinterpret_cast<float*>(ws + p.sum) : nullptr;
+      g.first = piece == 0;
+      g.last = piece == p.pieces - 1;
+      g.vec = aligned_to(a.dw, 16) && a.features % 8 == 0;
+      g.scale = scale;
+      MB200_TRY((tc::launch_tc_gemm<DwProblem<T>, 256, 4, FMT>(g, sms(), to, st)));
+    }
+  }
+  return cudaSuccess;
+}
+
+}  // namespace
+
+std::size_t vocab_loss_workspace(const VocabLossArgs& a) noexcept {
+  bool ok = false;
+  return plan_within(a, SIZE_MAX, &ok).bytes;
+}
+
+std::size_t vocab_loss_min_workspace(const VocabLossArgs& a) noexcept {
+  const std::size_t least = plan_rows(a, std::min(a.tokens, 128)).bytes;
+  return std::min(least, vocab_loss_workspace(a));
+}
+
+cudaError_t launch_vocab_loss(const VocabLossArgs& a, void* ws, std::size_t ws_bytes,
+                              cudaStream_t stream) noexcept {
+  bool ok = false;
+  const Plan p = plan_within(a, ws_bytes, &ok);
+  if (!ok) return cudaErrorInvalidValue;
+  return a.bf16 ? run<__nv_bfloat16, 1>(a, p, static_cast<char*>(ws), stream)
+                : run<__half, 0>(a, p, static_cast<char*>(ws), stream);
+}
+
+}  // namespace mb200::dnn
