@@ -306,4 +306,117 @@ __host__ __device__ constexpr std::uint32_t f16_idesc(int ab_format, int m, int 
          (static_cast<std::uint32_t>(n >> 3) << 17) | (static_cast<std::uint32_t>(m >> 4) << 24);
 }
 
+// ------------------------------------------------- two-CTA pairs (cta_group::2) --
+// A cluster of two CTAs works on one 256-row MMA: each CTA holds its 128 rows of A, its
+// half of B's rows and its 128 rows of the accumulator; the even CTA issues the MMAs.
+
+__device__ __forceinline__ std::uint32_t cluster_rank() {
+  std::uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+// Barrier of all threads of the cluster (also orders shared-memory accesses).
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile(
+      "barrier.cluster.arrive.release.aligned;\n\t"
+      "barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// shared::cluster address of `p`'s counterpart in CTA `rank` of the cluster.
+__device__ __forceinline__ std::uint32_t cluster_addr(const void* p, std::uint32_t rank) {
+  std::uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+  return a;
+}
+
+__device__ __forceinline__ void mbar_arrive_cluster(std::uint32_t cluster_address) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                   cluster_address)
+               : "memory");
+}
+
+// mbar_wait that also acquires what the arriving threads of the other CTA released.
+__device__ __forceinline__ bool mbar_try_wait_cluster(std::uint64_t* bar, std::uint32_t parity) {
+  std::uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_addr(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+__device__ __forceinline__ bool mbar_wait_cluster(std::uint64_t* bar, std::uint32_t parity) {
+  if (mbar_try_wait_cluster(bar, parity)) return true;
+  const std::uint64_t t0 = global_ns();
+  for (std::uint32_t i = 1;; ++i) {
+    if (mbar_try_wait_cluster(bar, parity)) return true;
+    if ((i & 63u) == 0u && global_ns() - t0 > kWaitLimitNs) return false;
+  }
+}
+
+// 3-D tiled load into this CTA's shared memory that completes on a barrier of either CTA
+// of the pair (a shared::cluster address).
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, std::int32_t x,
+                                                 std::int32_t y, std::int32_t z,
+                                                 std::uint32_t bar_cluster) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      ".cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<std::uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar_cluster)
+      : "memory");
+}
+
+// 3-D tiled store of one box from shared memory (no negative coordinates); joins the
+// thread's bulk group, see bulk_wait_read_all().
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src,
+                                             std::int32_t x, std::int32_t y, std::int32_t z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::
+                   "l"(reinterpret_cast<std::uint64_t>(map)),
+               "r"(smem_addr(src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+
+__device__ __forceinline__ void bulk_commit() {
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
+// Tensor memory of the pair: executed by one whole warp of each CTA.
+__device__ __forceinline__ void tmem_alloc_pair(std::uint32_t* dst_smem, std::uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                   smem_addr(dst_smem)),
+               "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_dealloc_pair(std::uint32_t taddr, std::uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols)
+               : "memory");
+}
+
+// mma_f16 over the pair: M = 256, descriptors valid in both CTAs' shared memory.
+__device__ __forceinline__ void mma_f16_pair(std::uint32_t d_tmem, std::uint64_t adesc,
+                                             std::uint64_t bdesc, std::uint32_t idesc,
+                                             std::uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Arrives once on `bar` in both CTAs when all previously issued pair MMAs complete.
+__device__ __forceinline__ void mma_commit_pair(std::uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+      "[%0], %1;" ::"r"(smem_addr(bar)),
+      "h"(static_cast<std::uint16_t>(3))
+      : "memory");
+}
+
 }  // namespace mb200::tc

@@ -31,6 +31,7 @@
 #include <type_traits>
 
 #include "blas/tc_gemm_core.cuh"
+#include "blas/tc_pair_core.cuh"
 #include "common/device.hpp"
 #include "dnn/vocab_loss.hpp"
 
@@ -95,49 +96,184 @@ __device__ __forceinline__ int target_count(const Targets& t, int row, int vocab
   return l < 0 ? 0 : l >= vocab ? -1 : 1;
 }
 
-// ------------------------------------------------------------------ logits kernel --
+// ------------------------------------------------------------------ logits kernels --
+// Words per (reference, sum) pair: one epilogue thread's share of a tile row.
+constexpr int kUnit = 128;
+
+// k-blocks per accumulator.  Tensor-core accumulation truncates: one chain of 256 MMAs
+// (H = 4096) left lse 3.4e-6 off in the 2-norm, chunks of 32 MMAs added in fp32 registers
+// 4e-7, an fp32 product's level.
+constexpr int kLogitsChunk = 8;
+
 struct LogitsProblem {
-  CUtensorMap mx;  // x: dims (features, rows), box {64, 128, 1}
-  CUtensorMap mw;  // w: dims (features, vocab), box {64, BN, 1}
+  CUtensorMap mx;    // x: dims (features, rows), box {64, 128, 1}
+  CUtensorMap mw;    // w: dims (features, vocab), box {64, 128, 1}
+  CUtensorMap mnum;  // numerators: dims (ldn, rows), box {64, 32, 1} (gradients only)
   long long tiles_total;
-  int num_kb, rows, vocab, tiles_m, tiles_n;
+  int num_kb, rows, vocab, units, tiles_m, tiles_n, group_m;
   float scale;        // log2(e) / tau
-  float2* stats;      // [row][tiles_n] (reference, sum of 2^(z2 - reference))
-  void* num;          // [row][ldn] numerators (gradients only)
+  float2* stats;      // [row][units] (reference, sum of 2^(z2 - reference))
   std::int64_t ldn;
   Targets targets;
 
-  __device__ void coords(long long t, int* m, int* n) const {
-    const int in_group = kGroupM * tiles_n;
+  const CUtensorMap* __device__ map_a() const { return &mx; }
+  const CUtensorMap* __device__ map_b() const { return &mw; }
+  __device__ void coords(long long t, int (&c)[3]) const {
+    const int in_group = group_m * tiles_n;
     const int r = static_cast<int>(t);
-    const int first = (r / in_group) * kGroupM;
-    const int gsz = min(tiles_m - first, kGroupM);
-    *m = first + (r % in_group) % gsz;
-    *n = (r % in_group) / gsz;
+    const int first = (r / in_group) * group_m;
+    const int gsz = min(tiles_m - first, group_m);
+    c[0] = 0;
+    c[1] = first + (r % in_group) % gsz;
+    c[2] = (r % in_group) / gsz;
+  }
+  __device__ int k_begin(const int (&)[3]) const { return 0; }
+};
+
+// A thread's 128 logits of one token, and the token's next target word.
+struct LogitsTile {
+  float v[kUnit];
+  int next;  // INT_MAX: none at or after the unit's first word
+  int at;    // its place among the row's targets
+};
+
+// The row's first target word at or after n0.
+__device__ __forceinline__ void first_target(const LogitsProblem& p, LogitsTile& t, int row,
+                                             int n0) {
+  t.next = INT_MAX;
+  t.at = 0;
+  if (row >= p.rows) return;
+  if (p.targets.top_k == 0) {
+    const std::int64_t l = p.targets.labels[row];
+    if (l >= n0 && l < p.vocab) t.next = static_cast<int>(l);
+    return;
+  }
+  const int tk = p.targets.top_k;
+  const int* idx = p.targets.index + static_cast<std::int64_t>(row) * tk;
+  int lo = 0, hi = tk;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (idx[mid] < n0) lo = mid + 1; else hi = mid;
+  }
+  t.at = lo;
+  if (lo < tk) t.next = idx[lo];
+}
+
+// Adds a finished accumulator's 128 columns (taddr: this thread's lane, first column).
+__device__ __forceinline__ void add_chunk(LogitsTile& t, std::uint32_t taddr) {
+#pragma unroll
+  for (int g = 0; g < kUnit / 16; ++g) {
+    float v[16];
+    tc::tmem_load_16cols(taddr + static_cast<std::uint32_t>(g * 16), v);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) t.v[g * 16 + j] = __fadd_rn(t.v[g * 16 + j], v[j]);
+  }
+}
+
+// Reduces the unit's logits to its pair and picks target words; with STORE leaves the
+// numerators in `stage` as two 128-byte-swizzled boxes of 32 rows x 64 words and sends
+// them to memory (the whole warp calls this).
+template <typename T, bool STORE>
+__device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& t, int row, int n0,
+                                            std::uint8_t* stage) {
+  const int lane = threadIdx.x & 31;
+  const int cols = p.vocab - n0;  // words from here on
+  if (cols <= 0) return;
+  if (cols < kUnit) {
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j)
+      if (j >= cols) t.v[j] = -INFINITY;
+  }
+  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int j = 0; j < kUnit; ++j) m[j & 3] = fmaxf(m[j & 3], t.v[j]);
+  const float mx = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+  // a row of -inf (or NaN) has no finite maximum: 0 keeps -inf's numerators at 0
+  const float ref = mx == -INFINITY ? 0.0f : __fmul_rn(mx, p.scale);
+  while (t.next < n0 + kUnit) {  // rare: a target word among these
+    const int j = t.next - n0;
+    float z = t.v[0];
+#pragma unroll
+    for (int i = 1; i < kUnit; ++i) z = (i == j) ? t.v[i] : z;
+    const int tk = max(p.targets.top_k, 1);
+    const std::int64_t r0 = static_cast<std::int64_t>(row) * tk;
+    p.targets.z2[r0 + t.at] = __fmul_rn(z, p.scale);
+    ++t.at;
+    t.next = t.at < p.targets.top_k ? p.targets.index[r0 + t.at] : INT_MAX;
+  }
+  if constexpr (STORE) {
+    // the previous unit's boxes have left the stage
+    if (lane == 0) tc::bulk_wait_read_all();
+  }
+  __syncwarp();
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int g = 0; g < kUnit / 8; ++g) {
+    float e[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      e[j] = exp2_approx(fmaf(t.v[g * 8 + j], p.scale, -ref));
+      s[j & 3] += e[j];
+    }
+    if constexpr (STORE) {
+      std::uint8_t* box = stage + (g >> 3) * 4096 + lane * 128 + (((g & 7) ^ (lane & 7)) << 4);
+      *reinterpret_cast<uint4*>(box) = make_uint4(pack2<T>(e[0], e[1]), pack2<T>(e[2], e[3]),
+                                                  pack2<T>(e[4], e[5]), pack2<T>(e[6], e[7]));
+    }
+  }
+  if (row < p.rows)
+    p.stats[static_cast<std::int64_t>(row) * p.units + n0 / kUnit] =
+        make_float2(ref, (s[0] + s[1]) + (s[2] + s[3]));
+  if constexpr (STORE) {
+    tc::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0 && row < p.rows) {  // lane 0 has the warp's first row
+      tc::tma_store_3d(&p.mnum, stage, n0, row, 0);
+      if (n0 + 64 < p.ldn) tc::tma_store_3d(&p.mnum, stage + 4096, n0 + 64, row, 0);
+      tc::bulk_commit();
+    }
+  }
+}
+
+// Pair loop: 256 tokens x 256 words.
+template <typename T, bool STORE>
+struct PairLogits : LogitsProblem {
+  static constexpr bool kAMn = false;
+  static constexpr int kChunk = kLogitsChunk;
+  static constexpr int kStageBytes = STORE ? 8192 : 0;
+  using Tile = LogitsTile;
+
+  __device__ __forceinline__ void begin(Tile& t, const int (&c)[3], int row, int half) const {
+    first_target(*this, t, c[1] * 2 * tc::kBM + row, c[2] * tc::kPairN + half * kUnit);
+#pragma unroll
+    for (int j = 0; j < kUnit; ++j) t.v[j] = 0.0f;
+  }
+  __device__ __forceinline__ void chunk(Tile& t, const int (&)[3], int, int, std::uint32_t taddr,
+                                        std::uint8_t*) const {
+    add_chunk(t, taddr);
+  }
+  __device__ __forceinline__ void end(Tile& t, const int (&c)[3], int row, int half,
+                                      std::uint8_t* stage) const {
+    finish_unit<T, STORE>(*this, t, c[1] * 2 * tc::kBM + row, c[2] * tc::kPairN + half * kUnit,
+                          stage);
   }
 };
 
-__device__ __forceinline__ float pick32(const float (&v)[32], int j) {
-  float r = v[0];
-#pragma unroll
-  for (int i = 1; i < 32; ++i) r = (i == j) ? v[i] : r;
-  return r;
-}
-
-// The loop of tc_gemm_core.cuh (TMA producer, MMA issuer, four epilogue warps, two
-// accumulators) with an epilogue that sees a token's whole tile row: it reads the row
-// from tensor memory twice, for the maximum and for the numerators.
-template <typename T, int FMT, int BN, int STAGES, bool STORE>
+// Few tokens (one tile row of 128): tiles of 128 words on single CTAs, the loop of
+// tc_gemm_core.cuh with chunked accumulators.  Reading w is what bounds it.
+template <typename T, int FMT, int STAGES, bool STORE>
 __global__ void __launch_bounds__(tc::kThreads, 1)
     vocab_logits_kernel(const __grid_constant__ LogitsProblem p, unsigned int* timeouts) {
   using namespace tc;
-  using S = CoreShape<BN, STAGES, 1>;
+  using S = CoreShape<kUnit, STAGES, 1>;
+  constexpr int CK = kLogitsChunk;
   extern __shared__ std::uint8_t smem_raw[];
   std::uint8_t* base = reinterpret_cast<std::uint8_t*>(
       (reinterpret_cast<std::uintptr_t>(smem_raw) + 1023) & ~std::uintptr_t{1023});
   std::uint8_t* sa = base;
-  std::uint8_t* sb = base + STAGES * S::A_STAGE;
-  std::uint64_t* full = reinterpret_cast<std::uint64_t*>(sb + STAGES * S::B_STAGE);
+  std::uint8_t* sb = sa + STAGES * S::A_STAGE;
+  std::uint8_t* se = sb + STAGES * S::B_STAGE;  // 8 KB per epilogue warp when STORE
+  std::uint64_t* full = reinterpret_cast<std::uint64_t*>(se + (STORE ? 4 * 8192 : 0));
   std::uint64_t* empty = full + STAGES;
   std::uint64_t* acc_full = empty + STAGES;
   std::uint64_t* acc_empty = acc_full + kAcc;
@@ -181,16 +317,16 @@ __global__ void __launch_bounds__(tc::kThreads, 1)
       bool issued[STAGES];
       for (int s = 0; s < STAGES; ++s) issued[s] = false;
       for (long long t = blockIdx.x; t < p.tiles_total && !*aborted; t += gridDim.x) {
-        int m, n;
-        p.coords(t, &m, &n);
+        int c[3];
+        p.coords(t, c);
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1u)) {
             fail();
             break;
           }
           mbar_arrive_expect_tx(&full[stage], S::A_STAGE + S::B_STAGE);
-          tma_load_3d(sa + stage * S::A_STAGE, &p.mx, kb * kBK, m * kBM, 0, &full[stage]);
-          tma_load_3d(sb + stage * S::B_STAGE, &p.mw, kb * kBK, n * BN, 0, &full[stage]);
+          tma_load_3d(sa + stage * S::A_STAGE, &p.mx, kb * kBK, c[1] * kBM, 0, &full[stage]);
+          tma_load_3d(sb + stage * S::B_STAGE, &p.mw, kb * kBK, c[2] * kUnit, 0, &full[stage]);
           issued[stage] = true;
           issued_phase[stage] = phase;
           if (++stage == STAGES) {
@@ -204,43 +340,49 @@ __global__ void __launch_bounds__(tc::kThreads, 1)
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      constexpr std::uint32_t idesc = f16_idesc(FMT, kBM, BN);
+      constexpr std::uint32_t idesc = f16_idesc(FMT, kBM, kUnit);
       int stage = 0;
       std::uint32_t phase = 0;
       int acc = 0;
       std::uint32_t acc_phase = 0;
-      for (long long t = blockIdx.x; t < p.tiles_total && !*aborted; t += gridDim.x) {
-        if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1u)) {
-          fail();
-          break;
-        }
-        tc_fence_after();
-        const std::uint32_t d_tmem = tmem_base + static_cast<std::uint32_t>(acc * BN);
-        bool ok = true;
+      bool ok = true;
+      for (long long t = blockIdx.x; ok && t < p.tiles_total && !*aborted; t += gridDim.x) {
         for (int kb = 0; kb < num_kb; ++kb) {
+          const bool first = kb % CK == 0;
+          const bool last = kb % CK == CK - 1 || kb == num_kb - 1;
+          if (first) {
+            if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1u)) {
+              fail();
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+          }
           if (!mbar_wait(&full[stage], phase)) {
             fail();
             ok = false;
             break;
           }
           tc_fence_after();
+          const std::uint32_t d_tmem = tmem_base + static_cast<std::uint32_t>(acc * kUnit);
           const std::uint32_t a0 = smem_addr(sa + stage * S::A_STAGE);
           const std::uint32_t b0 = smem_addr(sb + stage * S::B_STAGE);
 #pragma unroll
           for (int k = 0; k < kRowBytes / kStepBytes; ++k)
             mma_f16(d_tmem, operand_desc<false>(a0, k), operand_desc<false>(b0, k), idesc,
-                    (kb | k) != 0 ? 1u : 0u);
+                    (first && k == 0) ? 0u : 1u);
           mma_commit(&empty[stage]);
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1u;
           }
-        }
-        if (!ok) break;
-        mma_commit(&acc_full[acc]);
-        if (++acc == kAcc) {
-          acc = 0;
-          acc_phase ^= 1u;
+          if (last) {
+            mma_commit(&acc_full[acc]);
+            if (++acc == kAcc) {
+              acc = 0;
+              acc_phase ^= 1u;
+            }
+          }
         }
       }
       mma_commit(mma_done);
@@ -248,105 +390,41 @@ __global__ void __launch_bounds__(tc::kThreads, 1)
     }
   } else {
     const int quarter = warp & 3;
+    std::uint8_t* stage = se + (warp - 2) * 8192;
+    const int chunks = (num_kb + CK - 1) / CK;
     int acc = 0;
     std::uint32_t acc_phase = 0;
-    for (long long t = blockIdx.x; t < p.tiles_total && !*aborted; t += gridDim.x) {
-      int mt, nt;
-      p.coords(t, &mt, &nt);
-      const int row = mt * kBM + quarter * 32 + lane;
-      const bool live = row < p.rows;
-      const int n0 = nt * BN;
-      const int cols = min(BN, p.vocab - n0);  // words of this tile
-
-      // this row's first target word at or after n0 (none: INT_MAX)
-      const int tk = max(p.targets.top_k, 1);
-      int next = INT_MAX, at = 0;
-      if (live) {
-        if (p.targets.top_k == 0) {
-          const std::int64_t l = p.targets.labels[row];
-          if (l >= n0 && l < n0 + cols) next = static_cast<int>(l);
-        } else {
-          const int* idx = p.targets.index + static_cast<std::int64_t>(row) * tk;
-          int hi = tk;
-          while (at < hi) {
-            const int mid = (at + hi) >> 1;
-            if (idx[mid] < n0) at = mid + 1; else hi = mid;
-          }
-          if (at < tk) next = idx[at];
+    bool ok = true;
+    for (long long t = blockIdx.x; ok && t < p.tiles_total && !*aborted; t += gridDim.x) {
+      int c[3];
+      p.coords(t, c);
+      const int row = c[1] * kBM + quarter * 32 + lane;
+      LogitsTile tile;
+      first_target(p, tile, row, c[2] * kUnit);
+#pragma unroll
+      for (int j = 0; j < kUnit; ++j) tile.v[j] = 0.0f;
+      for (int ch = 0; ch < chunks; ++ch) {
+        if (!mbar_wait(&acc_full[acc], acc_phase)) {
+          fail();
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        __syncwarp();
+        add_chunk(tile, tmem_base + (static_cast<std::uint32_t>(quarter * 32) << 16) +
+                            static_cast<std::uint32_t>(acc * kUnit));
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[acc]);
+        if (++acc == kAcc) {
+          acc = 0;
+          acc_phase ^= 1u;
         }
       }
-
-      if (!mbar_wait(&acc_full[acc], acc_phase)) {
-        fail();
-        break;
-      }
-      tc_fence_after();
-      const std::uint32_t t_row = tmem_base + (static_cast<std::uint32_t>(quarter * 32) << 16) +
-                                  static_cast<std::uint32_t>(acc * BN);
-      float mx = -INFINITY;
-#pragma unroll 1
-      for (int c0 = 0; c0 < cols; c0 += 32) {
-        float v[32];
-        __syncwarp();  // the load is a whole warp's
-        tmem_load_32cols(t_row + static_cast<std::uint32_t>(c0), v);
-        if (c0 + 32 <= cols) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) mx = fmaxf(mx, v[j]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c0 + j < cols) mx = fmaxf(mx, v[j]);
-        }
-      }
-      // a row of -inf (or NaN) has no finite maximum: 0 keeps -inf's numerators at 0
-      const float ref = mx == -INFINITY ? 0.0f : __fmul_rn(mx, p.scale);
-      float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
-      for (int c0 = 0; c0 < cols; c0 += 32) {
-        float v[32];
-        __syncwarp();  // the load is a whole warp's
-        tmem_load_32cols(t_row + static_cast<std::uint32_t>(c0), v);
-        while (next < n0 + c0 + 32) {  // rare: a target word among these 32
-          const float z2 = __fmul_rn(pick32(v, next - n0 - c0), p.scale);
-          p.targets.z2[static_cast<std::int64_t>(row) * tk + at] = z2;
-          ++at;
-          next = at < p.targets.top_k
-                     ? p.targets.index[static_cast<std::int64_t>(row) * tk + at] : INT_MAX;
-        }
-#pragma unroll
-        for (int j = 0; j < 32; ++j) v[j] = exp2_approx(fmaf(v[j], p.scale, -ref));
-        if (c0 + 32 > cols) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c0 + j >= cols) v[j] = 0.0f;
-        }
-#pragma unroll
-        for (int j = 0; j < 32; ++j) s[j & 3] += v[j];
-        if constexpr (STORE) {
-          if (live) {
-            T* out = static_cast<T*>(p.num) + static_cast<std::int64_t>(row) * p.ldn + n0 + c0;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              if (n0 + c0 + 8 * g < p.ldn)
-                *reinterpret_cast<uint4*>(out + 8 * g) =
-                    make_uint4(pack2<T>(v[8 * g], v[8 * g + 1]), pack2<T>(v[8 * g + 2], v[8 * g + 3]),
-                               pack2<T>(v[8 * g + 4], v[8 * g + 5]),
-                               pack2<T>(v[8 * g + 6], v[8 * g + 7]));
-            }
-          }
-        }
-      }
-      if (live)
-        p.stats[static_cast<std::int64_t>(row) * p.tiles_n + nt] =
-            make_float2(ref, (s[0] + s[1]) + (s[2] + s[3]));
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[acc]);
-      if (++acc == kAcc) {
-        acc = 0;
-        acc_phase ^= 1u;
-      }
+      if (!ok) break;
+      finish_unit<T, STORE>(p, tile, row, c[2] * kUnit, stage);
     }
+    bulk_wait_all();
   }
 
   tc_fence_before();
@@ -475,8 +553,8 @@ __device__ __forceinline__ float block_reduce(float v, bool is_max, float* red) 
 }
 
 struct FinishArgs {
-  const float2* stats;  // [row][tiles_n]
-  int tiles_n, bn, rows, vocab;
+  const float2* stats;  // [row][units]
+  int units, vocab;
   Targets targets;
   float* loss;  // may be null
   float* lse;   // may be null
@@ -509,16 +587,17 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     }
     return;
   }
-  const float2* st = a.stats + static_cast<std::int64_t>(row) * a.tiles_n;
+  const float2* st = a.stats + static_cast<std::int64_t>(row) * a.units;
   float mx = -INFINITY;
-  for (int i = threadIdx.x; i < a.tiles_n; i += kFinishThreads)
+  for (int i = threadIdx.x; i < a.units; i += kFinishThreads)
     if (st[i].y != 0.0f) mx = fmaxf(mx, st[i].x);
   mx = block_reduce(mx, true, red);
   float sum = 0.0f;
-  for (int i = threadIdx.x; i < a.tiles_n; i += kFinishThreads)
+  for (int i = threadIdx.x; i < a.units; i += kFinishThreads)
     if (st[i].y != 0.0f) sum += st[i].y * exp2f(st[i].x - mx);
   sum = block_reduce(sum, false, red);
-  const float lse2 = mx + log2f(sum);
+  const float log_sum = log2f(sum);
+  const float lse2 = mx + log_sum;
 
   const int tk = max(a.targets.top_k, 1);
   const std::int64_t r0 = static_cast<std::int64_t>(row) * tk;
@@ -527,12 +606,13 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     if (n < 0) {
       loss = NAN;
     } else if (a.targets.top_k == 0) {
-      loss = (lse2 - a.targets.z2[r0]) * kLn2;
+      // the references subtract first: a confident word's loss is far below lse's last bit
+      loss = ((mx - a.targets.z2[r0]) + log_sum) * kLn2;
     } else {
       float cross = 0.0f;
       for (int k = threadIdx.x; k < n; k += kFinishThreads)
         if (a.targets.q[r0 + k] != 0.0f)
-          cross += a.targets.q[r0 + k] * ((lse2 - a.targets.z2[r0 + k]) * kLn2);
+          cross += a.targets.q[r0 + k] * (((mx - a.targets.z2[r0 + k]) + log_sum) * kLn2);
       loss = a.targets.neg_entropy[row] + block_reduce(cross, false, red);
     }
     if (threadIdx.x == 0) {
@@ -544,7 +624,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     float g = n < 0 ? NAN : a.dloss[row] * a.inv_tau;
     if (a.scale != nullptr) g *= a.scale[0];
     for (std::int64_t c = c_begin + threadIdx.x; c < c_end; c += kFinishThreads) {
-      const float f = g * exp2f(st[c * 8 / a.bn].x - lse2);
+      const float f = g * exp2f((st[c / (kUnit / 8)].x - mx) - log_sum);
       uint4 u = num[c];
       std::uint32_t* w = reinterpret_cast<std::uint32_t*>(&u);
 #pragma unroll
@@ -559,7 +639,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     if (a.targets.top_k == 0) {
       const std::int64_t l = a.targets.labels[row];
       if (threadIdx.x == 0 && n > 0 && l >= c_begin * 8 && l < c_end * 8)
-        d[l] = from_float<T>(g * expm1f((a.targets.z2[r0] - lse2) * kLn2));
+        d[l] = from_float<T>(g * expm1f(((a.targets.z2[r0] - mx) - log_sum) * kLn2));
     } else {
       for (int k = threadIdx.x; k < n; k += kFinishThreads) {
         const int w = a.targets.index[r0 + k];
@@ -567,7 +647,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
         if (k > 0 && a.targets.index[r0 + k - 1] == w) continue;  // the run's first entry adds all
         float q = a.targets.q[r0 + k];
         for (int j = k + 1; j < n && a.targets.index[r0 + j] == w; ++j) q += a.targets.q[r0 + j];
-        d[w] = from_float<T>(g * (exp2f(a.targets.z2[r0 + k] - lse2) - q));
+        d[w] = from_float<T>(g * (exp2f((a.targets.z2[r0 + k] - mx) - log_sum) - q));
       }
     }
   }
@@ -667,6 +747,65 @@ struct DxProblem {
   }
 };
 
+// The same product on CTA pairs (256 features x 256 tokens), for pieces of more than 128
+// tokens: the wider tile reads each operand half as often.
+template <typename T>
+struct PairDx {
+  static constexpr bool kAMn = true;
+  static constexpr int kChunk = 0;
+  static constexpr int kStageBytes = 0;
+  struct Tile {};
+  CUtensorMap ma;  // w: dims (features, vocab), box {64, 64, 1}
+  CUtensorMap mb;  // dz: dims (vocab, rows), box {64, 128, 1}
+  long long tiles_total;
+  int num_kb;  // k-blocks per split
+  int rows, features, tiles_m, tiles_n;
+  T* dx;
+  std::int64_t lddx;
+  float* partial;  // ksplit > 1: [split][row][feature]
+  const float* scale;
+
+  const CUtensorMap* __device__ map_a() const { return &ma; }
+  const CUtensorMap* __device__ map_b() const { return &mb; }
+  __device__ void coords(long long t, int (&c)[3]) const {
+    const int per = tiles_m * tiles_n;
+    const int r = static_cast<int>(t % per);
+    c[0] = static_cast<int>(t / per);
+    const int in_group = kGroupM * tiles_n;
+    const int first = (r / in_group) * kGroupM;
+    const int gsz = min(tiles_m - first, kGroupM);
+    c[1] = first + (r % in_group) % gsz;
+    c[2] = (r % in_group) / gsz;
+  }
+  __device__ int k_begin(const int (&c)[3]) const { return c[0] * num_kb; }
+  __device__ void begin(Tile&, const int (&)[3], int, int) const {}
+  __device__ void end(Tile&, const int (&)[3], int, int, std::uint8_t*) const {}
+  __device__ __forceinline__ void chunk(Tile&, const int (&c)[3], int row, int half,
+                                        std::uint32_t taddr, std::uint8_t*) const {
+    const int h = c[1] * 2 * tc::kBM + row;
+    const float a = scale != nullptr ? scale[1] : 1.0f;
+#pragma unroll 1
+    for (int g = 0; g < 4; ++g) {
+      float v[32];
+      __syncwarp();
+      tc::tmem_load_32cols(taddr + static_cast<std::uint32_t>(g * 32), v);
+      const int t0 = c[2] * tc::kPairN + half * 128 + g * 32;
+      if (h >= features) continue;
+      if (partial != nullptr) {
+        float* o = partial + (static_cast<std::int64_t>(c[0]) * rows + t0) * features + h;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (t0 + j < rows) o[static_cast<std::int64_t>(j) * features] = v[j];
+      } else {
+        T* o = dx + static_cast<std::int64_t>(t0) * lddx + h;
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (t0 + j < rows) o[j * lddx] = from_float<T>(a * v[j]);
+      }
+    }
+  }
+};
+
 // dx = scale * (sum of the splits, in split order).
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -684,27 +823,30 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// dw = dz^T x: A = dz^T is MN-major in dz, B = x^T (transposed copy) K-major.  A call of
-// several pieces adds its pieces in fp32 and rounds once, in the last.
+// dw = dz^T x on CTA pairs: A = dz^T is MN-major in dz, B = x^T (transposed copy) K-major.
+// Each epilogue warp stages its 32 words x 128 features as two 128-byte-swizzled boxes and
+// sends them by TMA; rows that TMA cannot address go out of the stage in coalesced 2-byte
+// stores.  A call of several pieces adds its pieces in fp32 and rounds once, in the last.
 template <typename T>
-struct DwProblem {
-  static constexpr bool kAMn = true, kBMn = false;
-  static constexpr int BN = 256;
-  CUtensorMap ma;  // dz: dims (vocab, rows), box {64, 64, 1}
-  CUtensorMap mb;  // x^T: dims (rows, features), box {64, 256, 1}
+struct PairDw {
+  static constexpr bool kAMn = true;
+  static constexpr int kChunk = 0;
+  static constexpr int kStageBytes = 8192;
+  struct Tile {};
+  CUtensorMap ma;   // dz: dims (vocab, rows), box {64, 64, 1}
+  CUtensorMap mb;   // x^T: dims (rows, features), box {64, 128, 1}
+  CUtensorMap mdw;  // dw: dims (features, vocab), box {64, 32, 1}, when `tma`
   long long tiles_total;
   int num_kb;
   int vocab, features, tiles_m, tiles_n;
   T* dw;
   float* sum;  // pieces: [word][feature] running sum, else null
   bool first, last;
-  bool vec;    // dw's 8-element runs are 16-byte aligned
+  bool tma;    // dw's rows are 16-byte aligned
   const float* scale;
 
-  __device__ void prefetch() const {
-    tc::prefetch_tensormap(&ma);
-    tc::prefetch_tensormap(&mb);
-  }
+  const CUtensorMap* __device__ map_a() const { return &ma; }
+  const CUtensorMap* __device__ map_b() const { return &mb; }
   __device__ void coords(long long t, int (&c)[3]) const {
     const int r = static_cast<int>(t);
     const int in_group = kGroupM * tiles_n;
@@ -714,45 +856,64 @@ struct DwProblem {
     c[1] = group0 + (r % in_group) % gsz;
     c[2] = (r % in_group) / gsz;
   }
-  __device__ void load(const int (&c)[3], int kb, void* sa, void* sb, std::uint64_t* bar) const {
+  __device__ int k_begin(const int (&)[3]) const { return 0; }
+  __device__ void begin(Tile&, const int (&)[3], int, int) const {}
+  __device__ void end(Tile&, const int (&)[3], int, int, std::uint8_t*) const {}
+  __device__ __forceinline__ void chunk(Tile&, const int (&c)[3], int row, int half,
+                                        std::uint32_t taddr, std::uint8_t* stage) const {
+    const int lane = threadIdx.x & 31;
+    const int w = c[1] * 2 * tc::kBM + row;
+    const int h0 = c[2] * tc::kPairN + half * 128;
+    const float a = scale != nullptr ? scale[1] : 1.0f;
+    if (lane == 0) tc::bulk_wait_read_all();  // the previous tile's boxes have left the stage
+#pragma unroll 1
+    for (int g = 0; g < 4; ++g) {
+      float v[32];
+      __syncwarp();
+      tc::tmem_load_32cols(taddr + static_cast<std::uint32_t>(g * 32), v);
 #pragma unroll
-    for (int j = 0; j < tc::kBM / 64; ++j)
-      tc::tma_load_3d(static_cast<std::uint8_t*>(sa) + j * tc::kMnBoxBytes, &ma,
-                      c[1] * tc::kBM + 64 * j, kb * tc::kBK, 0, bar);
-    tc::tma_load_3d(sb, &mb, kb * tc::kBK, c[2] * BN, 0, bar);
-  }
-  __device__ void scalars(float& a, float& b) const {
-    a = scale != nullptr ? scale[1] : 1.0f;
-    b = 0.0f;
-  }
-  __device__ void store(const int (&c)[3], int row, int col0, const float (&v)[32], float a,
-                        float) const {
-    const int w = c[1] * tc::kBM + row;
-    if (w >= vocab) return;
-    const int h0 = c[2] * BN + col0;
-    const std::int64_t o = static_cast<std::int64_t>(w) * features + h0;
-    float r[32];
+      for (int j = 0; j < 32; ++j) v[j] *= a;
+      if (sum != nullptr && w < vocab) {
+        float* o = sum + static_cast<std::int64_t>(w) * features + h0 + g * 32;
 #pragma unroll
-    for (int j = 0; j < 32; ++j) r[j] = a * v[j];
-    if (sum != nullptr) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        if (h0 + j >= features) continue;
-        if (!first) r[j] += sum[o + j];
-        if (!last) sum[o + j] = r[j];
+        for (int j = 0; j < 32; ++j) {
+          if (h0 + g * 32 + j >= features) continue;
+          if (!first) v[j] += o[j];
+          if (!last) o[j] = v[j];
+        }
       }
-      if (!last) return;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int chunk16 = (g & 1) * 4 + k;
+        std::uint8_t* box = stage + (g >> 1) * 4096 + lane * 128 + ((chunk16 ^ (lane & 7)) << 4);
+        *reinterpret_cast<uint4*>(box) =
+            make_uint4(pack2<T>(v[8 * k], v[8 * k + 1]), pack2<T>(v[8 * k + 2], v[8 * k + 3]),
+                       pack2<T>(v[8 * k + 4], v[8 * k + 5]), pack2<T>(v[8 * k + 6], v[8 * k + 7]));
+      }
     }
-    if (vec && h0 + 32 <= features) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<uint4*>(dw + o + 8 * g) =
-            make_uint4(pack2<T>(r[8 * g], r[8 * g + 1]), pack2<T>(r[8 * g + 2], r[8 * g + 3]),
-                       pack2<T>(r[8 * g + 4], r[8 * g + 5]), pack2<T>(r[8 * g + 6], r[8 * g + 7]));
+    if (!last || h0 >= features) return;
+    if (tma) {
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0 && w < vocab) {  // lane 0 has the warp's first word
+        tc::tma_store_3d(&mdw, stage, h0, w, 0);
+        if (h0 + 64 < features) tc::tma_store_3d(&mdw, stage + 4096, h0 + 64, w, 0);
+        tc::bulk_commit();
+      }
     } else {
+      __syncwarp();
+      const int rows = min(32, vocab - (w - lane));
+      for (int r = 0; r < rows; ++r) {
+        T* o = dw + static_cast<std::int64_t>(w - lane + r) * features + h0;
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (h0 + j < features) dw[o + j] = from_float<T>(r[j]);
+        for (int i = 0; i < 4; ++i) {
+          const int col = i * 32 + lane;
+          const T* e = reinterpret_cast<const T*>(
+              stage + (col >> 6) * 4096 + r * 128 + ((((col & 63) >> 3) ^ (r & 7)) << 4));
+          if (h0 + col < features) o[col] = e[col & 7];
+        }
+      }
+      __syncwarp();
     }
   }
 };
@@ -768,19 +929,17 @@ int sms() {
   return n > 0 ? n : 148;
 }
 
-// Words per tile of the logits kernel.
-int logits_bn(int rows) { return rows <= 128 ? 128 : 256; }
-
 // Tokens per tile of dx's product: a narrower tile does not multiply empty columns.
 int dx_bn(int rows) { return rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
 
-// Splits of the words in dx's product: the count that ends soonest, a wave of CTAs
-// taking 512 MMA clocks per k-block and each split's partial sums a write and a read.
+// Splits of the words in dx's product: the count that ends soonest, a wave of CTAs (or
+// pairs) taking 512 MMA clocks per k-block and each split's partial sums a write and a read.
 int dx_splits(int rows, int features, int vocab) {
   const int bn = dx_bn(rows);
-  const std::int64_t tiles = ((features + tc::kBM - 1) / tc::kBM) * static_cast<std::int64_t>((rows + bn - 1) / bn);
+  const int bm = bn == 256 ? 256 : 128;
+  const std::int64_t tiles = static_cast<std::int64_t>((features + bm - 1) / bm) * ((rows + bn - 1) / bn);
   const int kb = (vocab + tc::kBK - 1) / tc::kBK;
-  const int n = sms();
+  const int n = bn == 256 ? sms() / 2 : sms();
   double best = 0.0;
   int pick = 1;
   for (int ks = 1; ks <= 16 && ks * 8 <= std::max(kb, 8); ++ks) {
@@ -827,8 +986,7 @@ Plan plan_rows(const VocabLossArgs& a, int rows) {
     return o;
   };
   const std::size_t R = rows, H = a.features, V = a.vocab, K = a.top_k;
-  const std::size_t tiles_n = (V + logits_bn(rows) - 1) / logits_bn(rows);
-  p.stats = take(R * tiles_n * sizeof(float2));
+  p.stats = take(R * ((V + kUnit - 1) / kUnit) * sizeof(float2));
   p.z2 = take(R * std::max<std::size_t>(K, 1) * 4);
   p.index = take(R * K * 4);
   p.q = take(R * K * 4);
@@ -896,15 +1054,21 @@ unsigned int* timeout_counter() {
   return addr[dev];
 }
 
-template <typename T, int FMT, int BN, int STAGES, bool STORE>
+template <typename T, int FMT, bool STORE>
 cudaError_t run_logits(const LogitsProblem& p, unsigned int* timeouts, cudaStream_t st) {
-  using S = tc::CoreShape<BN, STAGES, 1>;
-  auto kern = vocab_logits_kernel<T, FMT, BN, STAGES, STORE>;
+  if (p.rows > tc::kBM) {
+    PairLogits<T, STORE> q;
+    static_cast<LogitsProblem&>(q) = p;
+    return tc::launch_tc_pair<PairLogits<T, STORE>, FMT>(q, sms(), timeouts, st);
+  }
+  constexpr int kStages = STORE ? 5 : 6;
+  constexpr int kSmem = tc::CoreShape<kUnit, kStages, 1>::SMEM + (STORE ? 4 * 8192 : 0);
+  auto kern = vocab_logits_kernel<T, FMT, kStages, STORE>;
   const cudaError_t e =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
   const unsigned grid = static_cast<unsigned>(std::min<long long>(p.tiles_total, sms()));
-  kern<<<grid, tc::kThreads, S::SMEM, st>>>(p, timeouts);
+  kern<<<grid, tc::kThreads, kSmem, st>>>(p, timeouts);
   return cudaGetLastError();
 }
 
@@ -918,24 +1082,30 @@ template <typename T, int FMT, int BN>
 cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const void* w, std::int64_t ldw,
                    const void* num, int rows, T* dx, char* ws, const float* scale,
                    unsigned int* to, cudaStream_t st) {
-  DxProblem<T, BN> g{};
+  constexpr bool kPair = BN == 256;
+  std::conditional_t<kPair, PairDx<T>, DxProblem<T, BN>> g{};
   if (!make_map(&g.ma, FMT, w, a.features, a.vocab, ldw, 64, 64) ||
-      !make_map(&g.mb, FMT, num, a.vocab, rows, p.ldn, 64, BN))
+      !make_map(&g.mb, FMT, num, a.vocab, rows, p.ldn, 64, kPair ? BN / 2 : BN))
     return cudaErrorInvalidValue;
   const int kb = (a.vocab + tc::kBK - 1) / tc::kBK;
   g.num_kb = (kb + p.ksplit - 1) / p.ksplit;
   const int ks = (kb + g.num_kb - 1) / g.num_kb;  // no split without words
   g.rows = rows;
   g.features = a.features;
-  g.tiles_m = (a.features + tc::kBM - 1) / tc::kBM;
+  constexpr int kRows = kPair ? 2 * tc::kBM : tc::kBM;
+  g.tiles_m = (a.features + kRows - 1) / kRows;
   g.tiles_n = (rows + BN - 1) / BN;
   g.tiles_total = static_cast<long long>(g.tiles_m) * g.tiles_n * ks;
   g.dx = dx;
   g.lddx = a.lddx;
   g.partial = ks > 1 ? reinterpret_cast<float*>(ws + p.partial) : nullptr;
   g.scale = scale;
-  constexpr int kStages = BN == 256 ? 4 : BN == 128 ? 6 : 8;
-  MB200_TRY((tc::launch_tc_gemm<DxProblem<T, BN>, BN, kStages, FMT>(g, sms(), to, st)));
+  if constexpr (kPair) {
+    MB200_TRY((tc::launch_tc_pair<PairDx<T>, FMT>(g, sms(), to, st)));
+  } else {
+    constexpr int kStages = BN == 128 ? 6 : 8;
+    MB200_TRY((tc::launch_tc_gemm<DxProblem<T, BN>, BN, kStages, FMT>(g, sms(), to, st)));
+  }
   if (ks > 1) {
     const dim3 grid(static_cast<unsigned>((a.features + 255) / 256),
                     static_cast<unsigned>(std::min(rows, 65535)));
@@ -960,7 +1130,6 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     ldw = p.ldp;
   }
   T* num = reinterpret_cast<T*>(ws + p.num);
-  const int bn = logits_bn(p.rows);
   for (int piece = 0; piece < p.pieces; ++piece) {
     const std::int64_t t0 = static_cast<std::int64_t>(piece) * p.rows;
     const int rows = static_cast<int>(std::min<std::int64_t>(p.rows, a.tokens - t0));
@@ -1004,31 +1173,28 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
 
     LogitsProblem lp{};
     if (!make_map(&lp.mx, FMT, x, a.features, rows, ldx, tc::kBK, tc::kBM) ||
-        !make_map(&lp.mw, FMT, w, a.features, a.vocab, ldw, tc::kBK, bn))
+        !make_map(&lp.mw, FMT, w, a.features, a.vocab, ldw, tc::kBK, kUnit) ||
+        (a.gradients && !make_map(&lp.mnum, FMT, num, p.ldn, rows, p.ldn, 64, 32)))
       return cudaErrorInvalidValue;
+    const bool pair = rows > tc::kBM;
     lp.num_kb = (a.features + tc::kBK - 1) / tc::kBK;
     lp.rows = rows;
     lp.vocab = a.vocab;
-    lp.tiles_m = (rows + tc::kBM - 1) / tc::kBM;
-    lp.tiles_n = (a.vocab + bn - 1) / bn;
+    lp.units = (a.vocab + kUnit - 1) / kUnit;
+    lp.tiles_m = pair ? (rows + 2 * tc::kBM - 1) / (2 * tc::kBM) : 1;
+    lp.tiles_n = pair ? (a.vocab + tc::kPairN - 1) / tc::kPairN : lp.units;
     lp.tiles_total = static_cast<long long>(lp.tiles_m) * lp.tiles_n;
+    lp.group_m = kGroupM / 2;
     lp.scale = kLog2e * a.inv_tau;
     lp.stats = reinterpret_cast<float2*>(ws + p.stats);
-    lp.num = num;
     lp.ldn = p.ldn;
     lp.targets = tg;
-    if (bn == 128)
-      MB200_TRY((a.gradients ? run_logits<T, FMT, 128, 6, true>(lp, to, st)
-                             : run_logits<T, FMT, 128, 6, false>(lp, to, st)));
-    else
-      MB200_TRY((a.gradients ? run_logits<T, FMT, 256, 4, true>(lp, to, st)
-                             : run_logits<T, FMT, 256, 4, false>(lp, to, st)));
+    MB200_TRY((a.gradients ? run_logits<T, FMT, true>(lp, to, st)
+                           : run_logits<T, FMT, false>(lp, to, st)));
 
     FinishArgs f{};
     f.stats = lp.stats;
-    f.tiles_n = lp.tiles_n;
-    f.bn = bn;
-    f.rows = rows;
+    f.units = lp.units;
     f.vocab = a.vocab;
     f.targets = tg;
     f.loss = a.loss != nullptr ? a.loss + t0 : nullptr;
@@ -1065,23 +1231,24 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
         MB200_TRY((run_dx<T, FMT, 256>(a, p, w, ldw, num, rows, dx, ws, scale, to, st)));
     }
     if (a.dw != nullptr) {
-      DwProblem<T> g{};
+      PairDw<T> g{};
+      g.tma = tma_rows_ok(a.dw, a.features);
       if (!make_map(&g.ma, FMT, num, a.vocab, rows, p.ldn, 64, 64) ||
-          !make_map(&g.mb, FMT, xt, rows, a.features, p.ldt, tc::kBK, 256))
+          !make_map(&g.mb, FMT, xt, rows, a.features, p.ldt, tc::kBK, 128) ||
+          (g.tma && !make_map(&g.mdw, FMT, a.dw, a.features, a.vocab, a.features, 64, 32)))
         return cudaErrorInvalidValue;
       g.num_kb = (rows + tc::kBK - 1) / tc::kBK;
       g.vocab = a.vocab;
       g.features = a.features;
-      g.tiles_m = (a.vocab + tc::kBM - 1) / tc::kBM;
-      g.tiles_n = (a.features + 255) / 256;
+      g.tiles_m = (a.vocab + 2 * tc::kBM - 1) / (2 * tc::kBM);
+      g.tiles_n = (a.features + tc::kPairN - 1) / tc::kPairN;
       g.tiles_total = static_cast<long long>(g.tiles_m) * g.tiles_n;
       g.dw = static_cast<T*>(a.dw);
       g.sum = p.pieces > 1 ? reinterpret_cast<float*>(ws + p.sum) : nullptr;
       g.first = piece == 0;
       g.last = piece == p.pieces - 1;
-      g.vec = aligned_to(a.dw, 16) && a.features % 8 == 0;
       g.scale = scale;
-      MB200_TRY((tc::launch_tc_gemm<DwProblem<T>, 256, 4, FMT>(g, sms(), to, st)));
+      MB200_TRY((tc::launch_tc_pair<PairDw<T>, FMT>(g, sms(), to, st)));
     }
   }
   return cudaSuccess;
