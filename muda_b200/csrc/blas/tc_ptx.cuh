@@ -306,6 +306,28 @@ __host__ __device__ constexpr std::uint32_t f16_idesc(int ab_format, int m, int 
          (static_cast<std::uint32_t>(n >> 3) << 17) | (static_cast<std::uint32_t>(m >> 4) << 24);
 }
 
+// mbar_wait by a whole converged warp; the result is the same in every lane, so the code
+// behind it stays warp-uniform (operands of tcgen05 and TMA in uniform registers).
+__device__ __forceinline__ bool mbar_wait_warp(std::uint64_t* bar, std::uint32_t parity) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  const std::uint64_t t0 = global_ns();
+  for (std::uint32_t i = 1;; ++i) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if ((i & 63u) == 0u && __any_sync(0xffffffffu, global_ns() - t0 > kWaitLimitNs)) return false;
+  }
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  std::uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
 // ------------------------------------------------- two-CTA pairs (cta_group::2) --
 // A cluster of two CTAs works on one 256-row MMA: each CTA holds its 128 rows of A, its
 // half of B's rows and its 128 rows of the accumulator; the even CTA issues the MMAs.
@@ -349,12 +371,12 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(std::uint64_t* bar, std::u
   return ok != 0;
 }
 
-__device__ __forceinline__ bool mbar_wait_cluster(std::uint64_t* bar, std::uint32_t parity) {
-  if (mbar_try_wait_cluster(bar, parity)) return true;
+__device__ __forceinline__ bool mbar_wait_cluster_warp(std::uint64_t* bar, std::uint32_t parity) {
+  if (__all_sync(0xffffffffu, mbar_try_wait_cluster(bar, parity))) return true;
   const std::uint64_t t0 = global_ns();
   for (std::uint32_t i = 1;; ++i) {
-    if (mbar_try_wait_cluster(bar, parity)) return true;
-    if ((i & 63u) == 0u && global_ns() - t0 > kWaitLimitNs) return false;
+    if (__all_sync(0xffffffffu, mbar_try_wait_cluster(bar, parity))) return true;
+    if ((i & 63u) == 0u && __any_sync(0xffffffffu, global_ns() - t0 > kWaitLimitNs)) return false;
   }
 }
 
@@ -417,6 +439,39 @@ __device__ __forceinline__ void mma_commit_pair(std::uint64_t* bar) {
       "[%0], %1;" ::"r"(smem_addr(bar)),
       "h"(static_cast<std::uint16_t>(3))
       : "memory");
+}
+
+// The load, MMA and commit of a group of one or two CTAs.
+template <int kCtas>
+__device__ __forceinline__ void tma_load_3d_group(void* dst, const CUtensorMap* map,
+                                                  std::int32_t x, std::int32_t y, std::int32_t z,
+                                                  std::uint32_t bar) {
+  if constexpr (kCtas == 2)
+    tma_load_3d_pair(dst, map, x, y, z, bar);
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_addr(dst)),
+        "l"(reinterpret_cast<std::uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+
+template <int kCtas>
+__device__ __forceinline__ void mma_f16_group(std::uint32_t d_tmem, std::uint64_t adesc,
+                                              std::uint64_t bdesc, std::uint32_t idesc,
+                                              std::uint32_t accumulate) {
+  if constexpr (kCtas == 2)
+    mma_f16_pair(d_tmem, adesc, bdesc, idesc, accumulate);
+  else
+    mma_f16(d_tmem, adesc, bdesc, idesc, accumulate);
+}
+
+template <int kCtas>
+__device__ __forceinline__ void mma_commit_group(std::uint64_t* bar) {
+  if constexpr (kCtas == 2)
+    mma_commit_pair(bar);
+  else
+    mma_commit(bar);
 }
 
 }  // namespace mb200::tc

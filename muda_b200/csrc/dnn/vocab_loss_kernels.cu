@@ -30,8 +30,7 @@
 #include <mutex>
 #include <type_traits>
 
-#include "blas/tc_gemm_core.cuh"
-#include "blas/tc_pair_core.cuh"
+#include "blas/tc_epi_core.cuh"
 #include "common/device.hpp"
 #include "dnn/vocab_loss.hpp"
 
@@ -97,7 +96,8 @@ __device__ __forceinline__ int target_count(const Targets& t, int row, int vocab
 }
 
 // ------------------------------------------------------------------ logits kernels --
-// Words per (reference, sum) pair: one epilogue thread's share of a tile row.
+// Most words of an epilogue thread's share of a tile row, its "unit" of one
+// (reference, sum) pair.
 constexpr int kUnit = 128;
 
 // k-blocks per accumulator.  Tensor-core accumulation truncates: one chain of 256 MMAs
@@ -105,12 +105,22 @@ constexpr int kUnit = 128;
 // 4e-7, an fp32 product's level.
 constexpr int kLogitsChunk = 8;
 
+// A thread's logits of one token, and the token's next target word.
+struct LogitsTile {
+  float v[kUnit];
+  int next;  // INT_MAX: none at or after the unit's first word
+  int at;    // its place among the row's targets
+};
+
+// z = x w^T.  Pairs (more than 128 tokens): 256 tokens x 256 words.  Single CTAs: all
+// tokens x tile_n words; reading w bounds these.
 struct LogitsProblem {
   CUtensorMap mx;    // x: dims (features, rows), box {64, 128, 1}
-  CUtensorMap mw;    // w: dims (features, vocab), box {64, 128, 1}
+  CUtensorMap mw;    // w: dims (features, vocab), box {64, 128 or tile_n, 1}
   CUtensorMap mnum;  // numerators: dims (ldn, rows), box {64, 32, 1} (gradients only)
   long long tiles_total;
-  int num_kb, rows, vocab, units, tiles_m, tiles_n, group_m;
+  int num_kb, tile_n, rows, vocab, tiles_m, tiles_n;
+  int unit, units;    // words per unit (tile_n / 2), units per row
   float scale;        // log2(e) / tau
   float2* stats;      // [row][units] (reference, sum of 2^(z2 - reference))
   std::int64_t ldn;
@@ -118,23 +128,17 @@ struct LogitsProblem {
 
   const CUtensorMap* __device__ map_a() const { return &mx; }
   const CUtensorMap* __device__ map_b() const { return &mw; }
+  // Tiles of 8 tile rows (2048 tokens) before the next ones, so CTAs in flight share w.
   __device__ void coords(long long t, int (&c)[3]) const {
-    const int in_group = group_m * tiles_n;
+    const int in_group = kGroupM / 2 * tiles_n;
     const int r = static_cast<int>(t);
-    const int first = (r / in_group) * group_m;
-    const int gsz = min(tiles_m - first, group_m);
+    const int first = (r / in_group) * (kGroupM / 2);
+    const int gsz = min(tiles_m - first, kGroupM / 2);
     c[0] = 0;
     c[1] = first + (r % in_group) % gsz;
     c[2] = (r % in_group) / gsz;
   }
   __device__ int k_begin(const int (&)[3]) const { return 0; }
-};
-
-// A thread's 128 logits of one token, and the token's next target word.
-struct LogitsTile {
-  float v[kUnit];
-  int next;  // INT_MAX: none at or after the unit's first word
-  int at;    // its place among the row's targets
 };
 
 // The row's first target word at or after n0.
@@ -159,14 +163,16 @@ __device__ __forceinline__ void first_target(const LogitsProblem& p, LogitsTile&
   if (lo < tk) t.next = idx[lo];
 }
 
-// Adds a finished accumulator's 128 columns (taddr: this thread's lane, first column).
-__device__ __forceinline__ void add_chunk(LogitsTile& t, std::uint32_t taddr) {
+// Adds a finished accumulator's columns of the unit (taddr: this thread's lane).
+__device__ __forceinline__ void add_chunk(LogitsTile& t, int unit, std::uint32_t taddr) {
 #pragma unroll
   for (int g = 0; g < kUnit / 16; ++g) {
-    float v[16];
-    tc::tmem_load_16cols(taddr + static_cast<std::uint32_t>(g * 16), v);
+    if (g * 16 < unit) {
+      float v[16];
+      tc::tmem_load_16cols(taddr + static_cast<std::uint32_t>(g * 16), v);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) t.v[g * 16 + j] = __fadd_rn(t.v[g * 16 + j], v[j]);
+      for (int j = 0; j < 16; ++j) t.v[g * 16 + j] = __fadd_rn(t.v[g * 16 + j], v[j]);
+    }
   }
 }
 
@@ -177,7 +183,7 @@ template <typename T, bool STORE>
 __device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& t, int row, int n0,
                                             std::uint8_t* stage) {
   const int lane = threadIdx.x & 31;
-  const int cols = p.vocab - n0;  // words from here on
+  const int cols = min(p.unit, p.vocab - n0);
   if (cols <= 0) return;
   if (cols < kUnit) {
 #pragma unroll
@@ -190,7 +196,7 @@ __device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& 
   const float mx = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
   // a row of -inf (or NaN) has no finite maximum: 0 keeps -inf's numerators at 0
   const float ref = mx == -INFINITY ? 0.0f : __fmul_rn(mx, p.scale);
-  while (t.next < n0 + kUnit) {  // rare: a target word among these
+  while (t.next < n0 + cols) {  // rare: a target word among these
     const int j = t.next - n0;
     float z = t.v[0];
 #pragma unroll
@@ -222,7 +228,7 @@ __device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& 
     }
   }
   if (row < p.rows)
-    p.stats[static_cast<std::int64_t>(row) * p.units + n0 / kUnit] =
+    p.stats[static_cast<std::int64_t>(row) * p.units + n0 / p.unit] =
         make_float2(ref, (s[0] + s[1]) + (s[2] + s[3]));
   if constexpr (STORE) {
     tc::fence_proxy_async_smem();
@@ -235,205 +241,35 @@ __device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& 
   }
 }
 
-// Pair loop: 256 tokens x 256 words.
-template <typename T, bool STORE>
-struct PairLogits : LogitsProblem {
+// STORE needs units of 128 words: the stage's boxes are 64 wide.
+template <typename T, bool PAIR, bool STORE>
+struct Logits : LogitsProblem {
+  static constexpr bool kPair = PAIR;
   static constexpr bool kAMn = false;
   static constexpr int kChunk = kLogitsChunk;
   static constexpr int kStageBytes = STORE ? 8192 : 0;
   using Tile = LogitsTile;
 
+  __device__ __forceinline__ int token(const int (&c)[3], int row) const {
+    return c[1] * (PAIR ? 2 : 1) * tc::kBM + row;
+  }
+  __device__ __forceinline__ int word(const int (&c)[3], int half) const {
+    return c[2] * tile_n + half * unit;
+  }
   __device__ __forceinline__ void begin(Tile& t, const int (&c)[3], int row, int half) const {
-    first_target(*this, t, c[1] * 2 * tc::kBM + row, c[2] * tc::kPairN + half * kUnit);
+    first_target(*this, t, token(c, row), word(c, half));
 #pragma unroll
     for (int j = 0; j < kUnit; ++j) t.v[j] = 0.0f;
   }
   __device__ __forceinline__ void chunk(Tile& t, const int (&)[3], int, int, std::uint32_t taddr,
                                         std::uint8_t*) const {
-    add_chunk(t, taddr);
+    add_chunk(t, PAIR ? kUnit : unit, taddr);
   }
   __device__ __forceinline__ void end(Tile& t, const int (&c)[3], int row, int half,
                                       std::uint8_t* stage) const {
-    finish_unit<T, STORE>(*this, t, c[1] * 2 * tc::kBM + row, c[2] * tc::kPairN + half * kUnit,
-                          stage);
+    finish_unit<T, STORE>(*this, t, token(c, row), word(c, half), stage);
   }
 };
-
-// Few tokens (one tile row of 128): tiles of 128 words on single CTAs, the loop of
-// tc_gemm_core.cuh with chunked accumulators.  Reading w is what bounds it.
-template <typename T, int FMT, int STAGES, bool STORE>
-__global__ void __launch_bounds__(tc::kThreads, 1)
-    vocab_logits_kernel(const __grid_constant__ LogitsProblem p, unsigned int* timeouts) {
-  using namespace tc;
-  using S = CoreShape<kUnit, STAGES, 1>;
-  constexpr int CK = kLogitsChunk;
-  extern __shared__ std::uint8_t smem_raw[];
-  std::uint8_t* base = reinterpret_cast<std::uint8_t*>(
-      (reinterpret_cast<std::uintptr_t>(smem_raw) + 1023) & ~std::uintptr_t{1023});
-  std::uint8_t* sa = base;
-  std::uint8_t* sb = sa + STAGES * S::A_STAGE;
-  std::uint8_t* se = sb + STAGES * S::B_STAGE;  // 8 KB per epilogue warp when STORE
-  std::uint64_t* full = reinterpret_cast<std::uint64_t*>(se + (STORE ? 4 * 8192 : 0));
-  std::uint64_t* empty = full + STAGES;
-  std::uint64_t* acc_full = empty + STAGES;
-  std::uint64_t* acc_empty = acc_full + kAcc;
-  std::uint64_t* mma_done = acc_empty + kAcc;
-  std::uint32_t* tmem_slot = reinterpret_cast<std::uint32_t*>(mma_done + 1);
-  volatile int* aborted = reinterpret_cast<volatile int*>(tmem_slot + 1);
-
-  const int warp = threadIdx.x >> 5;
-  const int lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    for (int a = 0; a < kAcc; ++a) {
-      mbar_init(&acc_full[a], 1);
-      mbar_init(&acc_empty[a], 4);
-    }
-    mbar_init(mma_done, 1);
-    *aborted = 0;
-    mbar_fence_init();
-    prefetch_tensormap(&p.mx);
-    prefetch_tensormap(&p.mw);
-  }
-  if (warp == 1) tmem_alloc(tmem_slot, S::TMEM_COLS);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const std::uint32_t tmem_base = *tmem_slot;
-  const int num_kb = p.num_kb;
-  auto fail = [&]() {
-    *aborted = 1;
-    atomicAdd(timeouts, 1u);
-  };
-
-  if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      std::uint32_t phase = 0;
-      std::uint32_t issued_phase[STAGES];
-      bool issued[STAGES];
-      for (int s = 0; s < STAGES; ++s) issued[s] = false;
-      for (long long t = blockIdx.x; t < p.tiles_total && !*aborted; t += gridDim.x) {
-        int c[3];
-        p.coords(t, c);
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(&empty[stage], phase ^ 1u)) {
-            fail();
-            break;
-          }
-          mbar_arrive_expect_tx(&full[stage], S::A_STAGE + S::B_STAGE);
-          tma_load_3d(sa + stage * S::A_STAGE, &p.mx, kb * kBK, c[1] * kBM, 0, &full[stage]);
-          tma_load_3d(sb + stage * S::B_STAGE, &p.mw, kb * kBK, c[2] * kUnit, 0, &full[stage]);
-          issued[stage] = true;
-          issued_phase[stage] = phase;
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
-        }
-      }
-      for (int s = 0; s < STAGES; ++s)
-        if (issued[s] && !mbar_wait(&full[s], issued_phase[s])) fail();
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr std::uint32_t idesc = f16_idesc(FMT, kBM, kUnit);
-      int stage = 0;
-      std::uint32_t phase = 0;
-      int acc = 0;
-      std::uint32_t acc_phase = 0;
-      bool ok = true;
-      for (long long t = blockIdx.x; ok && t < p.tiles_total && !*aborted; t += gridDim.x) {
-        for (int kb = 0; kb < num_kb; ++kb) {
-          const bool first = kb % CK == 0;
-          const bool last = kb % CK == CK - 1 || kb == num_kb - 1;
-          if (first) {
-            if (!mbar_wait(&acc_empty[acc], acc_phase ^ 1u)) {
-              fail();
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-          }
-          if (!mbar_wait(&full[stage], phase)) {
-            fail();
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const std::uint32_t d_tmem = tmem_base + static_cast<std::uint32_t>(acc * kUnit);
-          const std::uint32_t a0 = smem_addr(sa + stage * S::A_STAGE);
-          const std::uint32_t b0 = smem_addr(sb + stage * S::B_STAGE);
-#pragma unroll
-          for (int k = 0; k < kRowBytes / kStepBytes; ++k)
-            mma_f16(d_tmem, operand_desc<false>(a0, k), operand_desc<false>(b0, k), idesc,
-                    (first && k == 0) ? 0u : 1u);
-          mma_commit(&empty[stage]);
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1u;
-          }
-          if (last) {
-            mma_commit(&acc_full[acc]);
-            if (++acc == kAcc) {
-              acc = 0;
-              acc_phase ^= 1u;
-            }
-          }
-        }
-      }
-      mma_commit(mma_done);
-      if (!mbar_wait(mma_done, 0)) fail();
-    }
-  } else {
-    const int quarter = warp & 3;
-    std::uint8_t* stage = se + (warp - 2) * 8192;
-    const int chunks = (num_kb + CK - 1) / CK;
-    int acc = 0;
-    std::uint32_t acc_phase = 0;
-    bool ok = true;
-    for (long long t = blockIdx.x; ok && t < p.tiles_total && !*aborted; t += gridDim.x) {
-      int c[3];
-      p.coords(t, c);
-      const int row = c[1] * kBM + quarter * 32 + lane;
-      LogitsTile tile;
-      first_target(p, tile, row, c[2] * kUnit);
-#pragma unroll
-      for (int j = 0; j < kUnit; ++j) tile.v[j] = 0.0f;
-      for (int ch = 0; ch < chunks; ++ch) {
-        if (!mbar_wait(&acc_full[acc], acc_phase)) {
-          fail();
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        __syncwarp();
-        add_chunk(tile, tmem_base + (static_cast<std::uint32_t>(quarter * 32) << 16) +
-                            static_cast<std::uint32_t>(acc * kUnit));
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[acc]);
-        if (++acc == kAcc) {
-          acc = 0;
-          acc_phase ^= 1u;
-        }
-      }
-      if (!ok) break;
-      finish_unit<T, STORE>(p, tile, row, c[2] * kUnit, stage);
-    }
-    bulk_wait_all();
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem_base, S::TMEM_COLS);
-  }
-}
 
 // ----------------------------------------------------------------- small kernels --
 __device__ __forceinline__ float warp_max(float v) {
@@ -554,7 +390,7 @@ __device__ __forceinline__ float block_reduce(float v, bool is_max, float* red) 
 
 struct FinishArgs {
   const float2* stats;  // [row][units]
-  int units, vocab;
+  int units, unit, vocab;
   Targets targets;
   float* loss;  // may be null
   float* lse;   // may be null
@@ -624,7 +460,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     float g = n < 0 ? NAN : a.dloss[row] * a.inv_tau;
     if (a.scale != nullptr) g *= a.scale[0];
     for (std::int64_t c = c_begin + threadIdx.x; c < c_end; c += kFinishThreads) {
-      const float f = g * exp2f((st[c / (kUnit / 8)].x - mx) - log_sum);
+      const float f = g * exp2f((st[c / (a.unit / 8)].x - mx) - log_sum);
       uint4 u = num[c];
       std::uint32_t* w = reinterpret_cast<std::uint32_t*>(&u);
 #pragma unroll
@@ -686,80 +522,22 @@ __global__ void __launch_bounds__(256)
 }
 
 // ------------------------------------------------------------------ gradient GEMMs --
-// dx^T = w^T dz^T: A = w^T is MN-major in w, B = dz is K-major, the fastest operand forms
-// of the loop; a thread's 32 columns are 32 tokens of one feature, so a warp's stores of
-// one token are 32 consecutive features.  The words (K) split across `ksplit` CTAs.
-template <typename T, int BN>
-struct DxProblem {
-  static constexpr bool kAMn = true, kBMn = false;
-  CUtensorMap ma;  // w: dims (features, vocab), box {64, 64, 1}
-  CUtensorMap mb;  // dz: dims (vocab, rows), box {64, BN, 1}
-  long long tiles_total;
-  int num_kb;  // k-blocks per split
-  int rows, features, tiles_m, tiles_n;
-  T* dx;
-  std::int64_t lddx;
-  float* partial;  // ksplit > 1: [split][row][feature]
-  const float* scale;
-
-  __device__ void prefetch() const {
-    tc::prefetch_tensormap(&ma);
-    tc::prefetch_tensormap(&mb);
-  }
-  __device__ void coords(long long t, int (&c)[3]) const {
-    const int per = tiles_m * tiles_n;
-    const int r = static_cast<int>(t % per);
-    c[0] = static_cast<int>(t / per);
-    const int in_group = kGroupM * tiles_n;
-    const int first = (r / in_group) * kGroupM;
-    const int gsz = min(tiles_m - first, kGroupM);
-    c[1] = first + (r % in_group) % gsz;
-    c[2] = (r % in_group) / gsz;
-  }
-  __device__ void load(const int (&c)[3], int kb, void* sa, void* sb, std::uint64_t* bar) const {
-    const int k = (c[0] * num_kb + kb) * tc::kBK;  // past the vocabulary: zeros
-#pragma unroll
-    for (int j = 0; j < tc::kBM / 64; ++j)
-      tc::tma_load_3d(static_cast<std::uint8_t*>(sa) + j * tc::kMnBoxBytes, &ma,
-                      c[1] * tc::kBM + 64 * j, k, 0, bar);
-    tc::tma_load_3d(sb, &mb, k, c[2] * BN, 0, bar);
-  }
-  __device__ void scalars(float& a, float& b) const {
-    a = scale != nullptr ? scale[1] : 1.0f;
-    b = 0.0f;
-  }
-  __device__ void store(const int (&c)[3], int row, int col0, const float (&v)[32], float a,
-                        float) const {
-    const int h = c[1] * tc::kBM + row;
-    if (h >= features) return;
-    const int t0 = c[2] * BN + col0;
-    if (partial != nullptr) {
-      float* o = partial + (static_cast<std::int64_t>(c[0]) * rows + t0) * features + h;
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (t0 + j < rows) o[static_cast<std::int64_t>(j) * features] = v[j];
-      return;
-    }
-    T* o = dx + static_cast<std::int64_t>(t0) * lddx + h;
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (t0 + j < rows) o[j * lddx] = from_float<T>(a * v[j]);
-  }
-};
-
-// The same product on CTA pairs (256 features x 256 tokens), for pieces of more than 128
-// tokens: the wider tile reads each operand half as often.
-template <typename T>
-struct PairDx {
+// dx^T = w^T dz^T: A = w^T is MN-major in w, B = dz is K-major, the faster operand forms;
+// a thread's columns are tokens of one feature, so a warp's stores of one token are 32
+// consecutive features.  The words (K) split across `ksplit` groups of CTAs.  Pairs (more
+// than 128 tokens): 256 features x 256 tokens; else 128 features x all tokens.
+template <typename T, bool PAIR>
+struct Dx {
+  static constexpr bool kPair = PAIR;
   static constexpr bool kAMn = true;
   static constexpr int kChunk = 0;
   static constexpr int kStageBytes = 0;
   struct Tile {};
   CUtensorMap ma;  // w: dims (features, vocab), box {64, 64, 1}
-  CUtensorMap mb;  // dz: dims (vocab, rows), box {64, 128, 1}
+  CUtensorMap mb;  // dz: dims (vocab, rows), box {64, 128 or tile_n, 1}
   long long tiles_total;
   int num_kb;  // k-blocks per split
-  int rows, features, tiles_m, tiles_n;
+  int tile_n, rows, features, tiles_m, tiles_n;
   T* dx;
   std::int64_t lddx;
   float* partial;  // ksplit > 1: [split][row][feature]
@@ -782,43 +560,58 @@ struct PairDx {
   __device__ void end(Tile&, const int (&)[3], int, int, std::uint8_t*) const {}
   __device__ __forceinline__ void chunk(Tile&, const int (&c)[3], int row, int half,
                                         std::uint32_t taddr, std::uint8_t*) const {
-    const int h = c[1] * 2 * tc::kBM + row;
+    const int h = c[1] * (PAIR ? 2 : 1) * tc::kBM + row;
+    const int cols = (PAIR ? tc::kEpiN : tile_n) / 2;
     const float a = scale != nullptr ? scale[1] : 1.0f;
 #pragma unroll 1
-    for (int g = 0; g < 4; ++g) {
-      float v[32];
+    for (int c0 = 0; c0 < cols; c0 += 16) {
+      float v[16];
       __syncwarp();
-      tc::tmem_load_32cols(taddr + static_cast<std::uint32_t>(g * 32), v);
-      const int t0 = c[2] * tc::kPairN + half * 128 + g * 32;
+      tc::tmem_load_16cols(taddr + static_cast<std::uint32_t>(c0), v);
+      const int t0 = c[2] * (PAIR ? tc::kEpiN : tile_n) + half * cols + c0;
       if (h >= features) continue;
       if (partial != nullptr) {
         float* o = partial + (static_cast<std::int64_t>(c[0]) * rows + t0) * features + h;
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
+        for (int j = 0; j < 16; ++j)
           if (t0 + j < rows) o[static_cast<std::int64_t>(j) * features] = v[j];
       } else {
         T* o = dx + static_cast<std::int64_t>(t0) * lddx + h;
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
+        for (int j = 0; j < 16; ++j)
           if (t0 + j < rows) o[j * lddx] = from_float<T>(a * v[j]);
       }
     }
   }
 };
 
-// dx = scale * (sum of the splits, in split order).
-template <typename T>
+// dx = scale * (sum of the splits, in split order); VEC features per thread, 1 where rows
+// are not whole 16-byte runs.
+template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
     vocab_dx_reduce_kernel(const float* __restrict__ partial, int ksplit, int rows, int features,
                            T* __restrict__ dx, std::int64_t lddx, const float* scale) {
   const float a = scale != nullptr ? scale[1] : 1.0f;
   const std::int64_t plane = static_cast<std::int64_t>(rows) * features;
-  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
-    for (int h = blockIdx.x * 256 + threadIdx.x; h < features; h += gridDim.x * 256) {
-      const float* p = partial + static_cast<std::int64_t>(r) * features + h;
-      float s = p[0];
-      for (int i = 1; i < ksplit; ++i) s += p[i * plane];
-      dx[r * lddx + h] = from_float<T>(a * s);
+  const std::int64_t per = features / VEC;
+  const std::int64_t total = rows * per;
+  for (std::int64_t i = static_cast<std::int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
+       i += static_cast<std::int64_t>(gridDim.x) * 256) {
+    const std::int64_t r = i / per, h = (i - r * per) * VEC;
+    const float* p = partial + r * features + h;
+    T* o = dx + r * lddx + h;
+    if constexpr (VEC == 4) {
+      float4 s = __ldcs(reinterpret_cast<const float4*>(p));
+      for (int k = 1; k < ksplit; ++k) {
+        const float4 v = __ldcs(reinterpret_cast<const float4*>(p + k * plane));
+        s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+      }
+      *reinterpret_cast<uint2*>(o) =
+          make_uint2(pack2<T>(a * s.x, a * s.y), pack2<T>(a * s.z, a * s.w));
+    } else {
+      float s = __ldcs(p);
+      for (int k = 1; k < ksplit; ++k) s += __ldcs(p + k * plane);
+      *o = from_float<T>(a * s);
     }
   }
 }
@@ -828,7 +621,8 @@ __global__ void __launch_bounds__(256)
 // sends them by TMA; rows that TMA cannot address go out of the stage in coalesced 2-byte
 // stores.  A call of several pieces adds its pieces in fp32 and rounds once, in the last.
 template <typename T>
-struct PairDw {
+struct Dw {
+  static constexpr bool kPair = true;
   static constexpr bool kAMn = true;
   static constexpr int kChunk = 0;
   static constexpr int kStageBytes = 8192;
@@ -838,6 +632,7 @@ struct PairDw {
   CUtensorMap mdw;  // dw: dims (features, vocab), box {64, 32, 1}, when `tma`
   long long tiles_total;
   int num_kb;
+  int tile_n;  // 256
   int vocab, features, tiles_m, tiles_n;
   T* dw;
   float* sum;  // pieces: [word][feature] running sum, else null
@@ -863,7 +658,7 @@ struct PairDw {
                                         std::uint32_t taddr, std::uint8_t* stage) const {
     const int lane = threadIdx.x & 31;
     const int w = c[1] * 2 * tc::kBM + row;
-    const int h0 = c[2] * tc::kPairN + half * 128;
+    const int h0 = c[2] * tc::kEpiN + half * 128;
     const float a = scale != nullptr ? scale[1] : 1.0f;
     if (lane == 0) tc::bulk_wait_read_all();  // the previous tile's boxes have left the stage
 #pragma unroll 1
@@ -929,23 +724,45 @@ int sms() {
   return n > 0 ? n : 148;
 }
 
-// Tokens per tile of dx's product: a narrower tile does not multiply empty columns.
-int dx_bn(int rows) { return rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
+// Words per tile of the logits.  Pairs, and the boxes of stored numerators, take 256; a
+// score of at most 128 tokens is bound by reading w, so it takes the multiple of 32 whose
+// whole waves of tiles cover the vocabulary with the least to spare (the widest such: a
+// wider tile reads x less often).
+int logits_tile_n(int rows, int vocab, bool store) {
+  if (rows > tc::kBM || store) return tc::kEpiN;
+  int best = tc::kEpiN;
+  std::int64_t least = INT64_MAX;
+  for (int n = tc::kEpiN; n >= 32; n -= 32) {
+    const std::int64_t tiles = (vocab + n - 1) / n;
+    const std::int64_t cost = (tiles + sms() - 1) / sms() * n;
+    if (cost < least) {
+      least = cost;
+      best = n;
+    }
+  }
+  return best;
+}
 
-// Splits of the words in dx's product: the count that ends soonest, a wave of CTAs (or
-// pairs) taking 512 MMA clocks per k-block and each split's partial sums a write and a read.
+// Tokens per tile of dx's product on single CTAs: no wider than the tokens.
+int dx_tile_n(int rows) { return static_cast<int>(round_up(std::min(rows, tc::kEpiN), 32)); }
+
+// Splits of the words in dx's product: the count that ends soonest.  A k-block takes 512
+// clocks of MMAs on a pair; a single CTA's streams w at its share of memory bandwidth
+// (measured 5.5 TB/s).  Each split's partial sums are written and read once.
 int dx_splits(int rows, int features, int vocab) {
-  const int bn = dx_bn(rows);
-  const int bm = bn == 256 ? 256 : 128;
-  const std::int64_t tiles = static_cast<std::int64_t>((features + bm - 1) / bm) * ((rows + bn - 1) / bn);
+  const bool pair = rows > tc::kBM;
+  const std::int64_t tiles =
+      pair ? static_cast<std::int64_t>((features + 255) / 256) * ((rows + 255) / 256)
+           : (features + tc::kBM - 1) / tc::kBM;
   const int kb = (vocab + tc::kBK - 1) / tc::kBK;
-  const int n = bn == 256 ? sms() / 2 : sms();
+  const int n = pair ? sms() / 2 : sms();
+  const double block = pair ? 512 / 1.6e9 : tc::kBM * tc::kRowBytes * n / 5.5e12;
   double best = 0.0;
   int pick = 1;
-  for (int ks = 1; ks <= 16 && ks * 8 <= std::max(kb, 8); ++ks) {
+  for (int ks = 1; ks <= 32 && ks * 8 <= std::max(kb, 8); ++ks) {
     const double waves = static_cast<double>((tiles * ks + n - 1) / n);
-    const double loop = waves * ((kb + ks - 1) / ks) * 512.0 * bn / 256 / 1.8e9;
-    const double join = ks == 1 ? 0.0 : 3e-6 + 8.0 * ks * rows * features / 4e12;
+    const double loop = waves * ((kb + ks - 1) / ks) * block;
+    const double join = ks == 1 ? 0.0 : 4e-6 + 8.0 * ks * rows * features / 4.5e12;
     if (ks == 1 || loop + join < best) {
       best = loop + join;
       pick = ks;
@@ -986,7 +803,8 @@ Plan plan_rows(const VocabLossArgs& a, int rows) {
     return o;
   };
   const std::size_t R = rows, H = a.features, V = a.vocab, K = a.top_k;
-  p.stats = take(R * ((V + kUnit - 1) / kUnit) * sizeof(float2));
+  const std::size_t unit = logits_tile_n(rows, a.vocab, a.gradients) / 2;
+  p.stats = take(R * ((V + unit - 1) / unit) * sizeof(float2));
   p.z2 = take(R * std::max<std::size_t>(K, 1) * 4);
   p.index = take(R * K * 4);
   p.q = take(R * K * 4);
@@ -1054,22 +872,11 @@ unsigned int* timeout_counter() {
   return addr[dev];
 }
 
-template <typename T, int FMT, bool STORE>
+template <typename T, int FMT, bool PAIR, bool STORE>
 cudaError_t run_logits(const LogitsProblem& p, unsigned int* timeouts, cudaStream_t st) {
-  if (p.rows > tc::kBM) {
-    PairLogits<T, STORE> q;
-    static_cast<LogitsProblem&>(q) = p;
-    return tc::launch_tc_pair<PairLogits<T, STORE>, FMT>(q, sms(), timeouts, st);
-  }
-  constexpr int kStages = STORE ? 5 : 6;
-  constexpr int kSmem = tc::CoreShape<kUnit, kStages, 1>::SMEM + (STORE ? 4 * 8192 : 0);
-  auto kern = vocab_logits_kernel<T, FMT, kStages, STORE>;
-  const cudaError_t e =
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-  if (e != cudaSuccess) return e;
-  const unsigned grid = static_cast<unsigned>(std::min<long long>(p.tiles_total, sms()));
-  kern<<<grid, tc::kThreads, kSmem, st>>>(p, timeouts);
-  return cudaGetLastError();
+  Logits<T, PAIR, STORE> q;
+  static_cast<LogitsProblem&>(q) = p;
+  return tc::launch_tc_epi<Logits<T, PAIR, STORE>, FMT>(q, sms(), timeouts, st);
 }
 
 #define MB200_TRY(expr)                       \
@@ -1078,39 +885,40 @@ cudaError_t run_logits(const LogitsProblem& p, unsigned int* timeouts, cudaStrea
     if (e_ != cudaSuccess) return e_;         \
   } while (0)
 
-template <typename T, int FMT, int BN>
+template <typename T, int FMT, bool PAIR>
 cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const void* w, std::int64_t ldw,
                    const void* num, int rows, T* dx, char* ws, const float* scale,
                    unsigned int* to, cudaStream_t st) {
-  constexpr bool kPair = BN == 256;
-  std::conditional_t<kPair, PairDx<T>, DxProblem<T, BN>> g{};
+  Dx<T, PAIR> g{};
+  g.tile_n = PAIR ? tc::kEpiN : dx_tile_n(rows);
   if (!make_map(&g.ma, FMT, w, a.features, a.vocab, ldw, 64, 64) ||
-      !make_map(&g.mb, FMT, num, a.vocab, rows, p.ldn, 64, kPair ? BN / 2 : BN))
+      !make_map(&g.mb, FMT, num, a.vocab, rows, p.ldn, 64, PAIR ? 128 : g.tile_n))
     return cudaErrorInvalidValue;
   const int kb = (a.vocab + tc::kBK - 1) / tc::kBK;
   g.num_kb = (kb + p.ksplit - 1) / p.ksplit;
   const int ks = (kb + g.num_kb - 1) / g.num_kb;  // no split without words
+  constexpr int kRows = PAIR ? 2 * tc::kBM : tc::kBM;
   g.rows = rows;
   g.features = a.features;
-  constexpr int kRows = kPair ? 2 * tc::kBM : tc::kBM;
   g.tiles_m = (a.features + kRows - 1) / kRows;
-  g.tiles_n = (rows + BN - 1) / BN;
+  g.tiles_n = (rows + g.tile_n - 1) / g.tile_n;
   g.tiles_total = static_cast<long long>(g.tiles_m) * g.tiles_n * ks;
   g.dx = dx;
   g.lddx = a.lddx;
   g.partial = ks > 1 ? reinterpret_cast<float*>(ws + p.partial) : nullptr;
   g.scale = scale;
-  if constexpr (kPair) {
-    MB200_TRY((tc::launch_tc_pair<PairDx<T>, FMT>(g, sms(), to, st)));
-  } else {
-    constexpr int kStages = BN == 128 ? 6 : 8;
-    MB200_TRY((tc::launch_tc_gemm<DxProblem<T, BN>, BN, kStages, FMT>(g, sms(), to, st)));
-  }
+  MB200_TRY((tc::launch_tc_epi<Dx<T, PAIR>, FMT>(g, sms(), to, st)));
   if (ks > 1) {
-    const dim3 grid(static_cast<unsigned>((a.features + 255) / 256),
-                    static_cast<unsigned>(std::min(rows, 65535)));
-    vocab_dx_reduce_kernel<T><<<grid, 256, 0, st>>>(g.partial, ks, rows, a.features, dx, a.lddx,
-                                                    scale);
+    const bool vec = a.features % 4 == 0 && a.lddx % 4 == 0 && aligned_to(dx, 8);
+    const std::int64_t work = static_cast<std::int64_t>(rows) * a.features / (vec ? 4 : 1);
+    const unsigned grid =
+        static_cast<unsigned>(std::min<std::int64_t>((work + 255) / 256, sms() * 32));
+    if (vec)
+      vocab_dx_reduce_kernel<T, 4><<<grid, 256, 0, st>>>(g.partial, ks, rows, a.features, dx,
+                                                         a.lddx, scale);
+    else
+      vocab_dx_reduce_kernel<T, 1><<<grid, 256, 0, st>>>(g.partial, ks, rows, a.features, dx,
+                                                         a.lddx, scale);
     MB200_TRY(cudaGetLastError());
   }
   return cudaSuccess;
@@ -1171,30 +979,36 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
       MB200_TRY(cudaGetLastError());
     }
 
+    const bool pair = rows > tc::kBM;
     LogitsProblem lp{};
+    lp.tile_n = logits_tile_n(p.rows, a.vocab, a.gradients);
     if (!make_map(&lp.mx, FMT, x, a.features, rows, ldx, tc::kBK, tc::kBM) ||
-        !make_map(&lp.mw, FMT, w, a.features, a.vocab, ldw, tc::kBK, kUnit) ||
+        !make_map(&lp.mw, FMT, w, a.features, a.vocab, ldw, tc::kBK, pair ? 128 : lp.tile_n) ||
         (a.gradients && !make_map(&lp.mnum, FMT, num, p.ldn, rows, p.ldn, 64, 32)))
       return cudaErrorInvalidValue;
-    const bool pair = rows > tc::kBM;
     lp.num_kb = (a.features + tc::kBK - 1) / tc::kBK;
     lp.rows = rows;
     lp.vocab = a.vocab;
-    lp.units = (a.vocab + kUnit - 1) / kUnit;
+    lp.unit = lp.tile_n / 2;
+    lp.units = (a.vocab + lp.unit - 1) / lp.unit;
     lp.tiles_m = pair ? (rows + 2 * tc::kBM - 1) / (2 * tc::kBM) : 1;
-    lp.tiles_n = pair ? (a.vocab + tc::kPairN - 1) / tc::kPairN : lp.units;
+    lp.tiles_n = (a.vocab + lp.tile_n - 1) / lp.tile_n;
     lp.tiles_total = static_cast<long long>(lp.tiles_m) * lp.tiles_n;
-    lp.group_m = kGroupM / 2;
     lp.scale = kLog2e * a.inv_tau;
     lp.stats = reinterpret_cast<float2*>(ws + p.stats);
     lp.ldn = p.ldn;
     lp.targets = tg;
-    MB200_TRY((a.gradients ? run_logits<T, FMT, true>(lp, to, st)
-                           : run_logits<T, FMT, false>(lp, to, st)));
+    if (pair)
+      MB200_TRY((a.gradients ? run_logits<T, FMT, true, true>(lp, to, st)
+                             : run_logits<T, FMT, true, false>(lp, to, st)));
+    else
+      MB200_TRY((a.gradients ? run_logits<T, FMT, false, true>(lp, to, st)
+                             : run_logits<T, FMT, false, false>(lp, to, st)));
 
     FinishArgs f{};
     f.stats = lp.stats;
     f.units = lp.units;
+    f.unit = lp.unit;
     f.vocab = a.vocab;
     f.targets = tg;
     f.loss = a.loss != nullptr ? a.loss + t0 : nullptr;
@@ -1222,33 +1036,31 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     }
     if (a.dx != nullptr) {
       T* dx = static_cast<T*>(a.dx) + t0 * a.lddx;
-      const int bx = dx_bn(rows);
-      if (bx == 64)
-        MB200_TRY((run_dx<T, FMT, 64>(a, p, w, ldw, num, rows, dx, ws, scale, to, st)));
-      else if (bx == 128)
-        MB200_TRY((run_dx<T, FMT, 128>(a, p, w, ldw, num, rows, dx, ws, scale, to, st)));
+      if (pair)
+        MB200_TRY((run_dx<T, FMT, true>(a, p, w, ldw, num, rows, dx, ws, scale, to, st)));
       else
-        MB200_TRY((run_dx<T, FMT, 256>(a, p, w, ldw, num, rows, dx, ws, scale, to, st)));
+        MB200_TRY((run_dx<T, FMT, false>(a, p, w, ldw, num, rows, dx, ws, scale, to, st)));
     }
     if (a.dw != nullptr) {
-      PairDw<T> g{};
+      Dw<T> g{};
       g.tma = tma_rows_ok(a.dw, a.features);
       if (!make_map(&g.ma, FMT, num, a.vocab, rows, p.ldn, 64, 64) ||
           !make_map(&g.mb, FMT, xt, rows, a.features, p.ldt, tc::kBK, 128) ||
           (g.tma && !make_map(&g.mdw, FMT, a.dw, a.features, a.vocab, a.features, 64, 32)))
         return cudaErrorInvalidValue;
       g.num_kb = (rows + tc::kBK - 1) / tc::kBK;
+      g.tile_n = tc::kEpiN;
       g.vocab = a.vocab;
       g.features = a.features;
       g.tiles_m = (a.vocab + 2 * tc::kBM - 1) / (2 * tc::kBM);
-      g.tiles_n = (a.features + tc::kPairN - 1) / tc::kPairN;
+      g.tiles_n = (a.features + tc::kEpiN - 1) / tc::kEpiN;
       g.tiles_total = static_cast<long long>(g.tiles_m) * g.tiles_n;
       g.dw = static_cast<T*>(a.dw);
       g.sum = p.pieces > 1 ? reinterpret_cast<float*>(ws + p.sum) : nullptr;
       g.first = piece == 0;
       g.last = piece == p.pieces - 1;
       g.scale = scale;
-      MB200_TRY((tc::launch_tc_pair<PairDw<T>, FMT>(g, sms(), to, st)));
+      MB200_TRY((tc::launch_tc_epi<Dw<T>, FMT>(g, sms(), to, st)));
     }
   }
   return cudaSuccess;
