@@ -1,12 +1,14 @@
 // tc_epi_core.cuh — persistent tcgen05 loop for products whose epilogue needs more than
 // tc_gemm_core.cuh's store() hook: 16-bit operands, k-blocks of 64 elements.
 //
-// Two forms.  kPair: a cluster of two CTAs walks tiles of 256 x 256; each CTA accumulates
+// Three forms.  kPair: a cluster of two CTAs walks tiles of 256 x 256; each CTA accumulates
 // its 128 rows x 256 columns in its own tensor memory and loads its 128 rows of A and its
 // 128 of B's 256 rows, so a k-block costs a CTA 32 KB of loads where a single CTA's
-// 128 x 256 tile costs 48 KB for the same MMA time.  Otherwise single CTAs walk tiles of
-// 128 x tile_n (a multiple of 32 up to 256, chosen at run time): for few rows of one
-// operand, where streaming the other is what takes the time.
+// 128 x 256 tile costs 48 KB for the same MMA time.  kTall as well: tiles of 512 x 256,
+// two stacked 256 x 256 halves that fill tensor memory, 24 KB per CTA and MMA time; the
+// halves drain in turn before the next tile's MMAs, so it is for long K.  Otherwise single
+// CTAs walk tiles of 128 x tile_n (a multiple of 32 up to 256, chosen at run time): for few
+// rows of one operand, where streaming the other is what takes the time.
 //   warp 0      issues the CTA's TMA loads (a pair's complete on the even CTA's barriers);
 //   warp 1      issues the MMAs (a pair's: the even CTA) and commits stages and
 //               accumulators back; allocates tensor memory;
@@ -21,7 +23,7 @@
 // MMAs' 512; warp-uniform it takes 538.
 //
 // The problem type P (a __grid_constant__ parameter) supplies
-//   static constexpr bool kPair;
+//   static constexpr bool kPair, kTall;   // kTall implies kPair and kChunk 0
 //   static constexpr bool kAMn;       // A MN-major (64 x 64 boxes), else K-major; B is K-major
 //   static constexpr int kChunk;      // k-blocks per accumulator, 0: the whole tile
 //   static constexpr int kStageBytes; // shared memory of an epilogue warp, a multiple of 1024
@@ -35,7 +37,8 @@
 //   void chunk(Tile&, c, int row, int half, uint32_t taddr, uint8_t* stage) const;
 //                                                   // reads a finished accumulator
 //   void end(Tile&, c, int row, int half, uint8_t* stage) const;
-// `row` is the row in the tile, `half` the column half, taddr the half's first column.
+// `row` is the row in the tile, `half` the column half, taddr the half's first column.  A
+// tall tile calls chunk() twice, for its upper and then its lower 256 rows.
 // Waits are bounded as in tc_gemm_core.cuh: a wait that runs out marks its CTA aborted,
 // counts the event, and every role leaves its loop; all threads (of both CTAs) then meet at
 // a final barrier, so no CTA leaves while the other may still reach its memory.
@@ -52,7 +55,9 @@ constexpr int kEpiN = 256;  // columns of an accumulator
 template <class P>
 struct EpiShape {
   static constexpr int kCtas = P::kPair ? 2 : 1;
-  static constexpr int A_STAGE = kBM * kRowBytes;            // this CTA's rows of A
+  static constexpr int kHalves = P::kTall ? 2 : 1;
+  static constexpr int A_HALF = kBM * kRowBytes;
+  static constexpr int A_STAGE = kHalves * A_HALF;           // this CTA's rows of A
   static constexpr int B_STAGE = kEpiN / kCtas * kRowBytes;  // and of B
   static constexpr int STAGE = A_STAGE + B_STAGE;
   static constexpr int EPI = kEpiWarps * P::kStageBytes;
@@ -62,6 +67,7 @@ struct EpiShape {
   static constexpr int STAGES = FIT < 6 ? FIT : 6;
   static constexpr int SMEM = STAGES * STAGE + EPI + BAR_BYTES + 1024;
   static_assert(STAGES >= 3, "the ring needs three stages");
+  static_assert(!P::kTall || (P::kPair && P::kChunk == 0), "a tall tile is one chunk of a pair");
 };
 
 template <class P, int FMT>
@@ -138,7 +144,7 @@ __device__ __forceinline__ void epi_body(const P& p, unsigned int* timeouts) {
       int c[3];
       p.coords(t, c);
       int k = p.k_begin(c) * kBK;
-      const int am = c[1] * S::kCtas * kBM + static_cast<int>(rank) * kBM;
+      const int am = c[1] * S::kHalves * S::kCtas * kBM + static_cast<int>(rank) * kBM;
       const int bn = c[2] * tile_n + static_cast<int>(rank) * (kEpiN / 2);
       for (int kb = 0; kb < num_kb; ++kb, k += kBK) {
         if (!mbar_wait_warp(&empty[stage], phase ^ 1u)) {
@@ -149,13 +155,17 @@ __device__ __forceinline__ void epi_body(const P& p, unsigned int* timeouts) {
         if (elect_one()) {
           if (rank == 0) mbar_arrive_expect_tx(&full[stage], tx);
           const std::uint32_t bar = full0 + static_cast<std::uint32_t>(stage) * 8;
-          std::uint8_t* a = sa + stage * S::A_STAGE;
-          if constexpr (P::kAMn) {
 #pragma unroll
-            for (int j = 0; j < kBM / 64; ++j)
-              tma_load_3d_group<S::kCtas>(a + j * kMnBoxBytes, p.map_a(), am + 64 * j, k, 0, bar);
-          } else {
-            tma_load_3d_group<S::kCtas>(a, p.map_a(), k, am, 0, bar);
+          for (int u = 0; u < S::kHalves; ++u) {
+            std::uint8_t* a = sa + stage * S::A_STAGE + u * S::A_HALF;
+            const int m = am + u * 2 * kBM;
+            if constexpr (P::kAMn) {
+#pragma unroll
+              for (int j = 0; j < kBM / 64; ++j)
+                tma_load_3d_group<S::kCtas>(a + j * kMnBoxBytes, p.map_a(), m + 64 * j, k, 0, bar);
+            } else {
+              tma_load_3d_group<S::kCtas>(a, p.map_a(), k, m, 0, bar);
+            }
           }
           tma_load_3d_group<S::kCtas>(sb + stage * S::B_STAGE, p.map_b(), k, bn, 0, bar);
         }
@@ -191,37 +201,40 @@ __device__ __forceinline__ void epi_body(const P& p, unsigned int* timeouts) {
         for (int kb = 0; kb < num_kb; ++kb) {
           const bool first = CK == 0 ? kb == 0 : kb % (CK == 0 ? 1 : CK) == 0;
           const bool last = kb == num_kb - 1 || (CK != 0 && kb % (CK == 0 ? 1 : CK) == CK - 1);
-          if (first) {
-            if (!mbar_wait_cluster_warp(&acc_empty[acc], acc_phase ^ 1u)) {
-              if (lane == 0) fail();
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-          }
           if (!mbar_wait_warp(&full[stage], phase)) {
             if (lane == 0) fail();
             ok = false;
             break;
           }
-          tc_fence_after();
-          if (elect_one()) {
-            const std::uint32_t d_tmem = tmem_base + static_cast<std::uint32_t>(acc * kEpiN);
-            const std::uint64_t a0 = a_desc + static_cast<std::uint32_t>(stage * (S::A_STAGE >> 4));
-            const std::uint64_t b0 = b_desc + static_cast<std::uint32_t>(stage * (S::B_STAGE >> 4));
+          const std::uint64_t b0 = b_desc + static_cast<std::uint32_t>(stage * (S::B_STAGE >> 4));
 #pragma unroll
-            for (int k = 0; k < kRowBytes / kStepBytes; ++k)
-              mma_f16_group<S::kCtas>(d_tmem, a0 + k * a_step, b0 + k * (kStepBytes >> 4), idesc,
-                                      (first && k == 0) ? 0u : 1u);
-            mma_commit_group<S::kCtas>(&empty[stage]);
-            if (last) mma_commit_group<S::kCtas>(&acc_full[acc]);
+          for (int u = 0; u < S::kHalves; ++u) {
+            const int into = P::kTall ? u : acc;  // accumulator
+            if (first && !mbar_wait_cluster_warp(&acc_empty[into], acc_phase ^ 1u)) {
+              if (lane == 0) fail();
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            if (elect_one()) {
+              const std::uint32_t d_tmem = tmem_base + static_cast<std::uint32_t>(into * kEpiN);
+              const std::uint64_t a0 =
+                  a_desc + static_cast<std::uint32_t>((stage * S::A_STAGE + u * S::A_HALF) >> 4);
+#pragma unroll
+              for (int k = 0; k < kRowBytes / kStepBytes; ++k)
+                mma_f16_group<S::kCtas>(d_tmem, a0 + k * a_step, b0 + k * (kStepBytes >> 4), idesc,
+                                        (first && k == 0) ? 0u : 1u);
+              if (u == S::kHalves - 1) mma_commit_group<S::kCtas>(&empty[stage]);
+              if (last) mma_commit_group<S::kCtas>(&acc_full[into]);
+            }
+            __syncwarp();
           }
-          __syncwarp();
+          if (!ok) break;
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1u;
           }
-          if (last && ++acc == kAcc) {
+          if (last && (P::kTall || ++acc == kAcc)) {
             acc = 0;
             acc_phase ^= 1u;
           }
@@ -241,7 +254,8 @@ __device__ __forceinline__ void epi_body(const P& p, unsigned int* timeouts) {
     const std::uint32_t t_lane = tmem_base + (static_cast<std::uint32_t>(quarter * 32) << 16) +
                                  static_cast<std::uint32_t>(half * (tile_n / 2));
     const std::uint32_t release0 = kPair ? cluster_addr(acc_empty, 0) : smem_addr(acc_empty);
-    const int chunks = CK == 0 ? 1 : (num_kb + (CK == 0 ? 1 : CK) - 1) / (CK == 0 ? 1 : CK);
+    const int chunks =
+        CK == 0 ? S::kHalves : (num_kb + (CK == 0 ? 1 : CK) - 1) / (CK == 0 ? 1 : CK);
     int acc = 0;
     std::uint32_t acc_phase = 0;
     bool ok = true;
@@ -251,14 +265,15 @@ __device__ __forceinline__ void epi_body(const P& p, unsigned int* timeouts) {
       typename P::Tile tile;
       p.begin(tile, c, row, half);
       for (int ch = 0; ch < chunks; ++ch) {
-        if (!mbar_wait(&acc_full[acc], acc_phase)) {
+        if (!mbar_wait_idle(&acc_full[acc], acc_phase)) {
           fail();
           ok = false;
           break;
         }
         tc_fence_after();
         __syncwarp();
-        p.chunk(tile, c, row, half, t_lane + static_cast<std::uint32_t>(acc * kEpiN), stage);
+        p.chunk(tile, c, row + (P::kTall ? ch * 2 * kBM : 0), half,
+                t_lane + static_cast<std::uint32_t>(acc * kEpiN), stage);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(release0 + acc * 8);
