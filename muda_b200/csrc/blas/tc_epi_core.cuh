@@ -34,7 +34,7 @@
 //   int k_begin(const int (&c)[3]) const;           // first k-block of the tile
 //   struct Tile;                                    // per-thread epilogue state
 //   void begin(Tile&, c, int row, int half) const;  // before the accumulator is waited for
-//   void chunk(Tile&, c, int row, int half, uint32_t taddr, uint8_t* stage) const;
+//   void chunk(Tile&, c, int row, int half, uint32_t taddr, bool first, uint8_t* stage) const;
 //                                                   // reads a finished accumulator
 //   void end(Tile&, c, int row, int half, uint8_t* stage) const;
 // `row` is the row in the tile, `half` the column half, taddr the half's first column.  A
@@ -210,7 +210,7 @@ __device__ __forceinline__ void epi_body(const P& p, unsigned int* timeouts) {
 #pragma unroll
           for (int u = 0; u < S::kHalves; ++u) {
             const int into = P::kTall ? u : acc;  // accumulator
-            if (first && !mbar_wait_cluster_warp(&acc_empty[into], acc_phase ^ 1u)) {
+            if (first && !mbar_wait_warp(&acc_empty[into], acc_phase ^ 1u)) {
               if (lane == 0) fail();
               ok = false;
               break;
@@ -273,7 +273,7 @@ __device__ __forceinline__ void epi_body(const P& p, unsigned int* timeouts) {
         tc_fence_after();
         __syncwarp();
         p.chunk(tile, c, row + (P::kTall ? ch * 2 * kBM : 0), half,
-                t_lane + static_cast<std::uint32_t>(acc * kEpiN), stage);
+                t_lane + static_cast<std::uint32_t>(acc * kEpiN), ch == 0, stage);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(release0 + acc * 8);

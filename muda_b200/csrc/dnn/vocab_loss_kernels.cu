@@ -94,6 +94,8 @@ struct Targets {
   const float* q;         // [row][top_k]
   const int* count;       // valid entries; 0: row left out, -1: an index of vocab or more
   const float* neg_entropy;  // sum q log q
+  const unsigned* hit;       // [row][hit_words]: bit u set when a target is in unit u
+  int hit_words;
   float* z2;              // [row][max(top_k, 1)]: the target words' z2
 };
 
@@ -114,11 +116,12 @@ constexpr int kUnit = 128;
 // 4e-7, an fp32 product's level.
 constexpr int kLogitsChunk = 8;
 
-// A thread's logits of one token, and the token's next target word.
+// A thread's logits of one token, and what says whether a target word is among them: the
+// token's label, or its word of the map of units with targets.  Loaded before the
+// accumulator is waited for, looked at after.
 struct LogitsTile {
   float v[kUnit];
-  int next;  // INT_MAX: none at or after the unit's first word
-  int at;    // its place among the row's targets
+  std::int64_t hint;
 };
 
 // z = x w^T.  Pairs (more than 128 tokens): 256 tokens x 256 words.  Single CTAs: all
@@ -145,30 +148,48 @@ struct LogitsProblem {
   __device__ int k_begin(const int (&)[3]) const { return 0; }
 };
 
-// The row's first target word at or after n0.
-__device__ __forceinline__ void first_target(const LogitsProblem& p, LogitsTile& t, int row,
-                                             int n0) {
-  t.next = INT_MAX;
-  t.at = 0;
-  if (row >= p.rows) return;
-  if (p.targets.top_k == 0) {
-    const std::int64_t l = p.targets.labels[row];
-    if (l >= n0 && l < p.vocab) t.next = static_cast<int>(l);
-    return;
-  }
+__device__ __forceinline__ std::int64_t target_hint(const LogitsProblem& p, int row, int n0) {
+  if (row >= p.rows || n0 >= p.vocab) return p.targets.top_k == 0 ? -1 : 0;
+  if (p.targets.top_k == 0) return p.targets.labels[row];
+  const int u = n0 / p.unit;
+  return p.targets.hit[static_cast<std::int64_t>(row) * p.targets.hit_words + (u >> 5)];
+}
+
+// Stores the z2 of the row's target words among the `cols` from n0 on.
+__device__ __forceinline__ void pick_targets(const LogitsProblem& p, const LogitsTile& t, int row,
+                                             int n0, int cols) {
+  int at = 0, next = INT_MAX;
   const int tk = p.targets.top_k;
-  const int* idx = p.targets.index + static_cast<std::int64_t>(row) * tk;
-  int lo = 0, hi = tk;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (idx[mid] < n0) lo = mid + 1; else hi = mid;
+  const int* idx = nullptr;
+  if (tk == 0) {
+    if (t.hint >= n0 && t.hint < n0 + cols) next = static_cast<int>(t.hint);
+  } else if ((t.hint >> (n0 / p.unit & 31) & 1) != 0) {
+    idx = p.targets.index + static_cast<std::int64_t>(row) * tk;
+    int hi = tk;
+    while (at < hi) {  // the first entry at or after n0
+      const int mid = (at + hi) >> 1;
+      if (idx[mid] < n0) at = mid + 1; else hi = mid;
+    }
+    if (at < tk) next = idx[at];
   }
-  t.at = lo;
-  if (lo < tk) t.next = idx[lo];
+  while (next < n0 + cols) {
+    const int j = next - n0;
+    float z = t.v[0];
+#pragma unroll
+    for (int i = 1; i < kUnit; ++i) z = (i == j) ? t.v[i] : z;
+    p.targets.z2[static_cast<std::int64_t>(row) * max(tk, 1) + at] = __fmul_rn(z, p.scale);
+    ++at;
+    next = at < tk ? idx[at] : INT_MAX;
+  }
 }
 
 // Adds a finished accumulator's columns of the unit (taddr: this thread's lane).
-__device__ __forceinline__ void add_chunk(LogitsTile& t, int unit, std::uint32_t taddr) {
+__device__ __forceinline__ void add_chunk(LogitsTile& t, int unit, std::uint32_t taddr,
+                                          bool first) {
+  if (first && unit == kUnit) {
+    tc::tmem_load_128cols(taddr, t.v);
+    return;
+  }
 #pragma unroll
   for (int g = 0; g < kUnit / 16; ++g) {
     if (g * 16 < unit) {
@@ -200,17 +221,7 @@ __device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& 
   const float mx = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
   // a row of -inf (or NaN) has no finite maximum: 0 keeps -inf's numerators at 0
   const float ref = mx == -INFINITY ? 0.0f : __fmul_rn(mx, p.scale);
-  while (t.next < n0 + cols) {  // rare: a target word among these
-    const int j = t.next - n0;
-    float z = t.v[0];
-#pragma unroll
-    for (int i = 1; i < kUnit; ++i) z = (i == j) ? t.v[i] : z;
-    const int tk = max(p.targets.top_k, 1);
-    const std::int64_t r0 = static_cast<std::int64_t>(row) * tk;
-    p.targets.z2[r0 + t.at] = __fmul_rn(z, p.scale);
-    ++t.at;
-    t.next = t.at < p.targets.top_k ? p.targets.index[r0 + t.at] : INT_MAX;
-  }
+  pick_targets(p, t, row, n0, cols);
   if constexpr (STORE) {
     // the previous unit's boxes have left the stage
     if (lane == 0) tc::bulk_wait_read_all();
@@ -261,13 +272,15 @@ struct Logits : LogitsProblem {
     return c[2] * tile_n + half * unit;
   }
   __device__ __forceinline__ void begin(Tile& t, const int (&c)[3], int row, int half) const {
-    first_target(*this, t, token(c, row), word(c, half));
+    t.hint = target_hint(*this, token(c, row), word(c, half));
+    if (!PAIR && unit < kUnit) {
 #pragma unroll
-    for (int j = 0; j < kUnit; ++j) t.v[j] = 0.0f;
+      for (int j = 0; j < kUnit; ++j) t.v[j] = 0.0f;
+    }
   }
   __device__ __forceinline__ void chunk(Tile& t, const int (&)[3], int, int, std::uint32_t taddr,
-                                        std::uint8_t*) const {
-    add_chunk(t, PAIR ? kUnit : unit, taddr);
+                                        bool first, std::uint8_t*) const {
+    add_chunk(t, PAIR ? kUnit : unit, taddr, first);
   }
   __device__ __forceinline__ void end(Tile& t, const int (&c)[3], int row, int half,
                                       std::uint8_t* stage) const {
@@ -295,20 +308,25 @@ __device__ __forceinline__ int warp_sum(int v) {
 }
 
 // One warp per token: the teacher's distribution over the valid entries, and the entries
-// sorted by word (rank counting: top_k^2 / 32 comparisons per lane).
+// sorted by word (rank counting: top_k^2 / 32 comparisons per lane), and the map of the
+// units of the logits that hold one.
 constexpr int kTargetWarps = 4;
 
 __global__ void __launch_bounds__(32 * kTargetWarps)
     vocab_targets_kernel(const std::int64_t* __restrict__ teacher_index,
                          const float* __restrict__ teacher_logits, int rows, int top_k, int vocab,
                          float inv_tau, int* __restrict__ index, float* __restrict__ q,
-                         int* __restrict__ count, float* __restrict__ neg_entropy) {
+                         int* __restrict__ count, float* __restrict__ neg_entropy,
+                         unsigned* __restrict__ hit, int hit_words, int unit) {
   __shared__ int key_all[kTargetWarps][kVocabMaxTopK];
   const int lane = threadIdx.x & 31;
   int* key = key_all[threadIdx.x >> 5];
   const int row = blockIdx.x * kTargetWarps + (threadIdx.x >> 5);
   if (row >= rows) return;
   const std::int64_t r0 = static_cast<std::int64_t>(row) * top_k;
+  unsigned* map = hit + static_cast<std::int64_t>(row) * hit_words;
+  for (int k = lane; k < hit_words; k += 32) map[k] = 0u;
+  __syncwarp();
   float mx = -INFINITY;
   int valid = 0, bad = 0;
   for (int k = lane; k < top_k; k += 32) {
@@ -320,6 +338,8 @@ __global__ void __launch_bounds__(32 * kTargetWarps)
     if (ok) {
       mx = fmaxf(mx, t * inv_tau);
       ++valid;
+      const int u = static_cast<int>(i) / unit;
+      atomicOr(map + (u >> 5), 1u << (u & 31));
     }
   }
   __syncwarp();
@@ -463,17 +483,27 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
   if constexpr (GRAD) {
     float g = n < 0 ? NAN : a.dloss[row] * a.inv_tau;
     if (a.scale != nullptr) g *= a.scale[0];
-    for (std::int64_t c = c_begin + threadIdx.x; c < c_end; c += kFinishThreads) {
-      const float f = g * exp2f((st[c / (a.unit / 8)].x - mx) - log_sum);
-      uint4 u = num[c];
+    const int per_unit = a.unit / 8;
+    const auto scaled = [&](uint4 u, std::int64_t c) {
+      const float f = g * exp2f((st[c / per_unit].x - mx) - log_sum);
       std::uint32_t* w = reinterpret_cast<std::uint32_t*>(&u);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 v = unpack2<T>(w[j]);
         w[j] = pack2<T>(f * v.x, f * v.y);
       }
-      num[c] = u;
+      return u;
+    };
+    std::int64_t c = c_begin + threadIdx.x;
+    for (; c + 3 * kFinishThreads < c_end; c += 4 * kFinishThreads) {
+      uint4 u[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] = num[c + j * kFinishThreads];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        num[c + j * kFinishThreads] = scaled(u[j], c + j * kFinishThreads);
     }
+    for (; c < c_end; c += kFinishThreads) num[c] = scaled(num[c], c);
     __syncthreads();
     T* d = static_cast<T*>(a.num) + row * a.ldn;
     if (a.targets.top_k == 0) {
@@ -516,13 +546,36 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// dst[r][c] = src[r][c] into rows of ldd elements: operands that TMA cannot read in place.
+// dst[r][c] = src[r][c] into rows of ldd elements (a multiple of 64): operands whose rows
+// TMA cannot read in place, or that start off a line.  A thread moves 8 elements: five
+// aligned words around them, shifted by half a word where the row is odd.
 template <typename T>
 __global__ void __launch_bounds__(256)
     vocab_pack_kernel(const T* __restrict__ src, std::int64_t lds, std::int64_t rows, int cols,
                       T* __restrict__ dst, std::int64_t ldd) {
-  for (std::int64_t r = blockIdx.x; r < rows; r += gridDim.x)
-    for (int c = threadIdx.x; c < cols; c += 256) dst[r * ldd + c] = src[r * lds + c];
+  const int per = (cols + 7) / 8;
+  const std::int64_t total = rows * per;
+  for (std::int64_t i = static_cast<std::int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
+       i += static_cast<std::int64_t>(gridDim.x) * 256) {
+    const std::int64_t r = i / per;
+    const int c = static_cast<int>(i - r * per) * 8;
+    const T* s = src + r * lds + c;
+    T* d = dst + r * ldd + c;
+    if (c + 8 > cols || i == 0) {  // the ends of the rows, and nothing before the first element
+      for (int j = 0; j < 8 && c + j < cols; ++j) d[j] = s[j];
+      continue;
+    }
+    const auto at = reinterpret_cast<std::uintptr_t>(s);
+    const std::uint32_t* w = reinterpret_cast<const std::uint32_t*>(at & ~std::uintptr_t{3});
+    const unsigned shift = (at & 2) * 8;
+    std::uint32_t v[5];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = w[j];
+    v[4] = shift != 0 ? w[4] : 0u;
+    *reinterpret_cast<uint4*>(d) =
+        make_uint4(__funnelshift_r(v[0], v[1], shift), __funnelshift_r(v[1], v[2], shift),
+                   __funnelshift_r(v[2], v[3], shift), __funnelshift_r(v[3], v[4], shift));
+  }
 }
 
 // ------------------------------------------------------------------ gradient GEMMs --
@@ -564,7 +617,7 @@ struct Dx {
   __device__ void begin(Tile&, const int (&)[3], int, int) const {}
   __device__ void end(Tile&, const int (&)[3], int, int, std::uint8_t*) const {}
   __device__ __forceinline__ void chunk(Tile&, const int (&c)[3], int row, int half,
-                                        std::uint32_t taddr, std::uint8_t*) const {
+                                        std::uint32_t taddr, bool, std::uint8_t*) const {
     const int h = c[1] * kRows + row;
     const int cols = (PAIR ? tc::kEpiN : tile_n) / 2;
     const float a = scale != nullptr ? scale[1] : 1.0f;
@@ -657,7 +710,7 @@ struct Dw {
   __device__ void begin(Tile&, const int (&)[3], int, int) const {}
   __device__ void end(Tile&, const int (&)[3], int, int, std::uint8_t*) const {}
   __device__ __forceinline__ void chunk(Tile&, const int (&c)[3], int row, int half,
-                                        std::uint32_t taddr, std::uint8_t* stage) const {
+                                        std::uint32_t taddr, bool, std::uint8_t* stage) const {
     const int lane = threadIdx.x & 31;
     const int w = c[1] * kRows + row;
     const int hw = c[2] * tc::kEpiN + half * 128;
@@ -720,6 +773,10 @@ struct Dw {
 // ------------------------------------------------------------------------- planning --
 constexpr std::size_t kNumeratorCap = std::size_t{2} << 30;  // bytes of a piece's numerators
 constexpr int kScoreRows = 16384;                             // tokens of a piece without them
+
+// Elements of a 128-byte line: rows that start on one cost the loads of a 64-wide box one
+// line each, others two.
+constexpr int kLine = 64;
 
 std::int64_t round_up(std::int64_t v, std::int64_t m) { return (v + m - 1) / m * m; }
 
@@ -797,18 +854,22 @@ struct Plan {
   std::int64_t ldp;   // row of packed copies of x and w
   bool pack_x, pack_w;
   // byte offsets into the workspace
-  std::size_t stats, z2, index, q, count, entropy, scale, xp, wp, num, xt, partial, sum, bytes;
+  std::size_t stats, z2, index, q, count, entropy, hit, scale, xp, wp, num, xt, partial, sum, bytes;
 };
 
 Plan plan_rows(const VocabLossArgs& a, int rows) {
   Plan p{};
   p.rows = rows;
   p.pieces = (a.tokens + rows - 1) / rows;
-  p.ldn = round_up(a.vocab, 8);
-  p.ldt = round_up(rows, 8);
-  p.ldp = round_up(a.features, 8);
+  p.ldn = round_up(a.vocab, kLine);
+  p.ldt = round_up(rows, kLine);
+  p.ldp = round_up(a.features, kLine);
   p.pack_x = a.tokens > 1 ? !tma_rows_ok(a.x, a.ldx) : !aligned_to(a.x, 16);
   p.pack_w = !tma_rows_ok(a.w, a.features);
+  // x is read once per 256 words: a copy with rows on lines pays at once (1537 x 1000 x
+  // 50021: 532 -> 520 us).  A copy of w does not (520 -> 508..548 us, and 178 -> 219 at 300
+  // tokens).
+  if (rows > tc::kBM && a.ldx % kLine != 0) p.pack_x = true;
   const bool dx = a.gradients && a.dx != nullptr, dw = a.gradients && a.dw != nullptr;
   p.ksplit = dx ? dx_splits(rows, a.features, a.vocab) : 1;
   std::size_t at = 0;
@@ -825,6 +886,7 @@ Plan plan_rows(const VocabLossArgs& a, int rows) {
   p.q = take(R * K * 4);
   p.count = take(K > 0 ? R * 4 : 0);
   p.entropy = take(K > 0 ? R * 4 : 0);
+  p.hit = take(K > 0 ? R * (((V + unit - 1) / unit + 31) / 32) * 4 : 0);
   p.scale = take(8);
   p.xp = take(p.pack_x ? R * p.ldp * 2 : 0);
   p.wp = take(p.pack_w ? V * p.ldp * 2 : 0);
@@ -840,7 +902,7 @@ Plan plan_rows(const VocabLossArgs& a, int rows) {
 Plan plan_within(const VocabLossArgs& a, std::size_t limit, bool* ok) {
   std::int64_t most = kScoreRows;
   if (a.gradients)
-    most = std::max<std::int64_t>(128, static_cast<std::int64_t>(kNumeratorCap / (round_up(a.vocab, 8) * 2)) / 128 * 128);
+    most = std::max<std::int64_t>(128, static_cast<std::int64_t>(kNumeratorCap / (round_up(a.vocab, kLine) * 2)) / 128 * 128);
   int pieces = static_cast<int>((a.tokens + most - 1) / most);
   Plan p{};
   for (;;) {
@@ -991,7 +1053,7 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     std::int64_t ldx = a.tokens > 1 ? a.ldx : p.ldp;  // one row: its stride is never used
     if (p.pack_x) {
       T* xp = reinterpret_cast<T*>(ws + p.xp);
-      vocab_pack_kernel<T><<<std::min(rows, sms() * 8), 256, 0, st>>>(x, ldx, rows, a.features, xp,
+      vocab_pack_kernel<T><<<sms() * 8, 256, 0, st>>>(x, ldx, rows, a.features, xp,
                                                                       p.ldp);
       MB200_TRY(cudaGetLastError());
       x = xp;
@@ -1007,14 +1069,19 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
       float* q = reinterpret_cast<float*>(ws + p.q);
       int* count = reinterpret_cast<int*>(ws + p.count);
       float* ent = reinterpret_cast<float*>(ws + p.entropy);
+      unsigned* hit = reinterpret_cast<unsigned*>(ws + p.hit);
+      const int unit = logits_tile_n(p.rows, a.vocab, a.gradients) / 2;
+      const int hit_words = ((a.vocab + unit - 1) / unit + 31) / 32;
       vocab_targets_kernel<<<(rows + kTargetWarps - 1) / kTargetWarps, 32 * kTargetWarps, 0, st>>>(
           a.teacher_index + t0 * a.top_k, a.teacher_logits + t0 * a.top_k, rows, a.top_k, a.vocab,
-          a.inv_tau, index, q, count, ent);
+          a.inv_tau, index, q, count, ent, hit, hit_words, unit);
       MB200_TRY(cudaGetLastError());
       tg.index = index;
       tg.q = q;
       tg.count = count;
       tg.neg_entropy = ent;
+      tg.hit = hit;
+      tg.hit_words = hit_words;
     }
 
     float* scale = nullptr;
