@@ -122,6 +122,7 @@ __device__ __forceinline__ void epi_body(const P& p, unsigned int* timeouts) {
     __syncthreads();
   tc_fence_after();
   const std::uint32_t tmem_base = *tmem_slot;
+  grid_wait_previous();
   const int num_kb = p.num_kb;
   const int tile_n = kPair ? kEpiN : p.tile_n;
   const long long step = gridDim.x / S::kCtas;
@@ -315,6 +316,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kEpiThreads, 1)
   epi_body<P, FMT>(p, timeouts);
 }
 
+// Launches `kern` so that its prologue may overlap the end of the stream's previous kernel
+// (the kernel calls grid_wait_previous() before it touches memory).  tc_epi kernels do not
+// let the next one start early: its waiting CTAs cost them 2-4 %.
+template <typename... K, typename... A>
+cudaError_t launch_overlapped(void (*kern)(K...), dim3 grid, int threads, std::size_t smem,
+                              cudaStream_t stream, A... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<K>(args)...);
+}
+
 template <class P, int FMT>
 cudaError_t launch_tc_epi(const P& p, int sms, unsigned int* timeouts, cudaStream_t stream) {
   using S = EpiShape<P>;
@@ -335,8 +355,8 @@ cudaError_t launch_tc_epi(const P& p, int sms, unsigned int* timeouts, cudaStrea
   }
   const long long groups = std::min<long long>(p.tiles_total, sms / S::kCtas);
   if (groups <= 0) return cudaSuccess;
-  kern<<<static_cast<unsigned>(S::kCtas * groups), kEpiThreads, S::SMEM, stream>>>(p, timeouts);
-  return cudaGetLastError();
+  return launch_overlapped(kern, dim3(static_cast<unsigned>(S::kCtas * groups)), kEpiThreads,
+                           S::SMEM, stream, p, timeouts);
 }
 
 }  // namespace mb200::tc

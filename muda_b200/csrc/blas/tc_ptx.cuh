@@ -365,6 +365,16 @@ __device__ __forceinline__ bool mbar_wait_idle(std::uint64_t* bar, std::uint32_t
   return true;
 }
 
+// Programmatic dependent launch: lets the stream's next kernel start its prologue, and
+// waits until the kernels before this one have finished and their writes are visible.
+// Every kernel launched with the attribute waits before it touches memory.
+__device__ __forceinline__ void grid_launch_next() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void grid_wait_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // One lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   std::uint32_t p;

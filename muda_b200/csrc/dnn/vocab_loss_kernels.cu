@@ -288,6 +288,204 @@ struct Logits : LogitsProblem {
   }
 };
 
+// ------------------------------------------------------------- scores of few tokens --
+// Up to 8 tokens, losses only: reading w is all there is to do, so w goes from memory
+// straight into mma.sync operands.  A warp takes 16 words at a time: lane (g, t) = (lane / 4,
+// lane % 4) loads 16 bytes of words g and g + 8 and of token g at feature 32 step + 8 t, the
+// four lanes of a word a whole 64 bytes.  The MMA's K order is free as long as both operands
+// agree, so the lane's 8 features serve two k16 MMAs as they lie.  Loads run four steps (4 KB
+// per warp) ahead, across words.  No tensor memory, barriers or shared-memory ring to set up:
+// one token against 32000 x 1024 takes 18 us with its finish, 25 us on the tiles above, and 8
+// against 131072 x 4096 178 us (6.0 TB/s) and 209.
+//
+// A lane keeps its own running (maximum, sum) of the words it sees; the CTA joins them once
+// at the end into one pair per token.  As above, fp32 sums of chunks bound the MMA's drift.
+constexpr int kStreamTokens = 8;
+constexpr int kStreamWords = 16;    // words per warp and round
+constexpr int kStreamThreads = 512;
+// Steps of 32 features in flight per warp: 8 x 2048 x 32000 took 25.9 us with 4 and 27.5 with
+// 8, 8 x 4096 x 131072 179.8 and 177.
+constexpr int kStreamSteps = 4;
+constexpr int kStreamChunk = 4;     // groups of steps per accumulator: 32 MMAs
+
+struct StreamArgs {
+  const void* x;
+  std::int64_t ldx;
+  const void* w;
+  std::int64_t ldw;
+  int rows, features, vocab;
+  float scale;
+  float2* stats;  // [row][gridDim.x]
+  Targets targets;
+};
+
+// 16 bytes that are read once, zeros without `ok`.  The predicate is inside the asm: a branch
+// around the load would make its result wait for the load at once.
+__device__ __forceinline__ uint4 load_once(const void* p, bool ok) {
+  uint4 v;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+      "@q ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+      : "l"(p), "r"(static_cast<int>(ok)));
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], std::uint32_t a0, std::uint32_t a1,
+                                            std::uint32_t a2, std::uint32_t a3, std::uint32_t b0,
+                                            std::uint32_t b1) {
+  if constexpr (std::is_same_v<T, __half>)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// (m, s) joined with (m2, s2): s counts 2^(z2 - m); s == 0 is an empty pair.
+__device__ __forceinline__ void join_pair(float& m, float& s, float m2, float s2) {
+  if (s2 == 0.0f) return;
+  if (s == 0.0f) {
+    m = m2;
+    s = s2;
+    return;
+  }
+  const float top = fmaxf(m, m2);
+  s = s * exp2_approx(m - top) + s2 * exp2_approx(m2 - top);
+  m = top;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kStreamThreads, 1) vocab_stream_kernel(const StreamArgs a) {
+  __shared__ float2 joined[kStreamThreads / 32][kStreamTokens];
+  tc::grid_launch_next();
+  tc::grid_wait_previous();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const T* x = static_cast<const T*>(a.x) + g * a.ldx + 8 * t;
+  const T* w = static_cast<const T*>(a.w);
+  const int rounds_all = (a.vocab + kStreamWords - 1) / kStreamWords;
+  const int groups = (a.features + 32 * kStreamSteps - 1) / (32 * kStreamSteps);
+  // round r of the grid's warps, CTAs fastest so that every SM gets its share
+  const int first = warp * gridDim.x + blockIdx.x;
+  const int stride = gridDim.x * (kStreamThreads / 32);
+
+  int label[2];  // cross entropy: the target words of the lane's tokens 2t and 2t + 1
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    label[j] = -1;
+    if (a.targets.top_k == 0 && 2 * t + j < a.rows) {
+      const std::int64_t l = a.targets.labels[2 * t + j];
+      if (l >= 0 && l < a.vocab) label[j] = static_cast<int>(l);
+    }
+  }
+  float m[2] = {0.0f, 0.0f}, s[2] = {0.0f, 0.0f};
+
+  uint4 in[kStreamSteps][2];  // words g and g + 8 of the steps in flight
+  const auto fetch = [&](int round, int group, int i) {
+    const int w0 = round * kStreamWords + g;
+    const int k = (group * kStreamSteps + i) * 32 + 8 * t;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      in[i][h] = load_once(w + static_cast<std::int64_t>(w0 + 8 * h) * a.ldw + k,
+                           round < rounds_all && w0 + 8 * h < a.vocab && k < a.features);
+  };
+  if (first < rounds_all) {
+#pragma unroll
+    for (int i = 0; i < kStreamSteps; ++i) fetch(first, 0, i);
+  }
+  for (int round = first; round < rounds_all; round += stride) {
+    unsigned hint = 0;  // distillation: the round's word of the lane's token's map
+    if (a.targets.top_k > 0 && lane < a.rows)
+      hint = a.targets.hit[static_cast<std::int64_t>(lane) * a.targets.hit_words + (round >> 5)];
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int group = 0; group < groups; ++group) {
+      const bool more = group + 1 < groups;
+      const int next_round = more ? round : round + stride, next_group = more ? group + 1 : 0;
+#pragma unroll
+      for (int i = 0; i < kStreamSteps; ++i) {
+        const int k = (group * kStreamSteps + i) * 32;
+        uint4 b = make_uint4(0, 0, 0, 0);
+        if (g < a.rows && k + 8 * t < a.features) b = __ldg(reinterpret_cast<const uint4*>(x + k));
+        mma_16x8x16<T>(acc, in[i][0].x, in[i][1].x, in[i][0].y, in[i][1].y, b.x, b.y);
+        mma_16x8x16<T>(acc, in[i][0].z, in[i][1].z, in[i][0].w, in[i][1].w, b.z, b.w);
+        fetch(next_round, next_group, i);
+      }
+      if (group % kStreamChunk == kStreamChunk - 1 || !more) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          z[j] = __fadd_rn(z[j], acc[j]);
+          acc[j] = 0.0f;
+        }
+      }
+    }
+    // z[0..1]: word g, tokens 2t and 2t + 1; z[2..3]: word g + 8
+    const int w0 = round * kStreamWords + g;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      z[j] = w0 + (j >> 1) * 8 < a.vocab ? __fmul_rn(z[j], a.scale) : -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (label[j] == w0) a.targets.z2[2 * t + j] = z[j];
+      if (label[j] == w0 + 8) a.targets.z2[2 * t + j] = z[j + 2];
+      const float top = fmaxf(z[j], z[j + 2]);
+      // -inf adds nothing; NaN has to (fmaxf passes over it)
+      const float ref = top == -INFINITY ? 0.0f : top;
+      join_pair(m[j], s[j], ref, exp2_approx(z[j] - ref) + exp2_approx(z[j + 2] - ref));
+    }
+    if (a.targets.top_k > 0) {
+      unsigned rows = __ballot_sync(0xffffffffu, (hint >> (round & 31) & 1u) != 0u);
+      while (rows != 0) {  // tokens with a target among these words
+        const int row = __ffs(rows) - 1;
+        rows &= rows - 1;
+        const std::int64_t r0 = static_cast<std::int64_t>(row) * a.targets.top_k;
+        const int* idx = a.targets.index + r0;
+        int lo = 0, hi = a.targets.top_k;
+        while (lo < hi) {
+          const int mid = (lo + hi) >> 1;
+          if (idx[mid] < round * kStreamWords) lo = mid + 1; else hi = mid;
+        }
+        for (; lo < a.targets.top_k && idx[lo] < (round + 1) * kStreamWords; ++lo) {
+          const int at = idx[lo] - round * kStreamWords;
+          if ((at & 7) != g || row >> 1 != t) continue;
+          const float even = at < 8 ? z[0] : z[2], odd = at < 8 ? z[1] : z[3];
+          a.targets.z2[r0 + lo] = (row & 1) != 0 ? odd : even;
+        }
+      }
+      __syncwarp();
+    }
+  }
+
+  // join the eight lanes of a token, then the warps
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      const float m2 = __shfl_xor_sync(0xffffffffu, m[j], o);
+      const float s2 = __shfl_xor_sync(0xffffffffu, s[j], o);
+      join_pair(m[j], s[j], m2, s2);
+    }
+    if (g == 0) joined[warp][2 * t + j] = make_float2(m[j], s[j]);
+  }
+  __syncthreads();
+  const int row = threadIdx.x;
+  if (row < a.rows) {
+    float2 p = joined[0][row];
+    for (int i = 1; i < kStreamThreads / 32; ++i)
+      join_pair(p.x, p.y, joined[i][row].x, joined[i][row].y);
+    a.stats[static_cast<std::int64_t>(row) * gridDim.x + blockIdx.x] = p;
+  }
+}
+
 // ----------------------------------------------------------------- small kernels --
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
@@ -318,6 +516,8 @@ __global__ void __launch_bounds__(32 * kTargetWarps)
                          float inv_tau, int* __restrict__ index, float* __restrict__ q,
                          int* __restrict__ count, float* __restrict__ neg_entropy,
                          unsigned* __restrict__ hit, int hit_words, int unit) {
+  tc::grid_launch_next();
+  tc::grid_wait_previous();
   __shared__ int key_all[kTargetWarps][kVocabMaxTopK];
   const int lane = threadIdx.x & 31;
   int* key = key_all[threadIdx.x >> 5];
@@ -378,6 +578,8 @@ __global__ void __launch_bounds__(32 * kTargetWarps)
 __global__ void __launch_bounds__(1024)
     vocab_grad_scale_kernel(const float* __restrict__ dloss, int rows, int vocab, Targets targets,
                             float inv_tau, float* __restrict__ scale) {
+  tc::grid_launch_next();
+  tc::grid_wait_previous();
   __shared__ float red[32];
   float mx = 0.0f;
   for (int i = threadIdx.x; i < rows; i += 1024) {
@@ -429,6 +631,8 @@ struct FinishArgs {
 // again, a few KB from L2).
 template <typename T, bool GRAD>
 __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const FinishArgs a) {
+  tc::grid_launch_next();
+  tc::grid_wait_previous();
   __shared__ float red[kFinishThreads / 32];
   const int row = blockIdx.x;
   const int n = target_count(a.targets, row, a.vocab);
@@ -530,6 +734,8 @@ template <typename T>
 __global__ void __launch_bounds__(256)
     vocab_transpose_kernel(const T* __restrict__ x, std::int64_t ldx, int rows, int features,
                            Targets targets, int vocab, T* __restrict__ xt, std::int64_t ldt) {
+  tc::grid_launch_next();
+  tc::grid_wait_previous();
   __shared__ T tile[64][66];
   const int r0 = blockIdx.x * 64, h0 = blockIdx.y * 64;
   const int lx = threadIdx.x & 63, ly = threadIdx.x >> 6;
@@ -553,6 +759,8 @@ template <typename T>
 __global__ void __launch_bounds__(256)
     vocab_pack_kernel(const T* __restrict__ src, std::int64_t lds, std::int64_t rows, int cols,
                       T* __restrict__ dst, std::int64_t ldd) {
+  tc::grid_launch_next();
+  tc::grid_wait_previous();
   const int per = (cols + 7) / 8;
   const std::int64_t total = rows * per;
   for (std::int64_t i = static_cast<std::int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
@@ -649,6 +857,8 @@ template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
     vocab_dx_reduce_kernel(const float* __restrict__ partial, int ksplit, int rows, int features,
                            T* __restrict__ dx, std::int64_t lddx, const float* scale) {
+  tc::grid_launch_next();
+  tc::grid_wait_previous();
   const float a = scale != nullptr ? scale[1] : 1.0f;
   const std::int64_t plane = static_cast<std::int64_t>(rows) * features;
   const std::int64_t per = features / VEC;
@@ -660,6 +870,7 @@ __global__ void __launch_bounds__(256)
     T* o = dx + r * lddx + h;
     if constexpr (VEC == 4) {
       float4 s = __ldcs(reinterpret_cast<const float4*>(p));
+#pragma unroll 4
       for (int k = 1; k < ksplit; ++k) {
         const float4 v = __ldcs(reinterpret_cast<const float4*>(p + k * plane));
         s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
@@ -668,6 +879,7 @@ __global__ void __launch_bounds__(256)
           make_uint2(pack2<T>(a * s.x, a * s.y), pack2<T>(a * s.z, a * s.w));
     } else {
       float s = __ldcs(p);
+#pragma unroll 4
       for (int k = 1; k < ksplit; ++k) s += __ldcs(p + k * plane);
       *o = from_float<T>(a * s);
     }
@@ -846,6 +1058,9 @@ int band_of(int tiles, std::int64_t tile_bytes, std::int64_t keep) {
 bool tma_rows_ok(const void* p, std::int64_t ld) { return aligned_to(p, 16) && ld % 8 == 0; }
 
 struct Plan {
+  bool stream;  // scores of few tokens (vocab_stream_kernel)
+  int unit, units;  // words per pair of the logits (stream: per bit of the hit map), pairs
+  int hit_words;    // words of a token's hit map
   int rows;    // tokens per piece (the last may have fewer)
   int pieces;
   int ksplit;
@@ -879,14 +1094,17 @@ Plan plan_rows(const VocabLossArgs& a, int rows) {
     return o;
   };
   const std::size_t R = rows, H = a.features, V = a.vocab, K = a.top_k;
-  const std::size_t unit = logits_tile_n(rows, a.vocab, a.gradients) / 2;
-  p.stats = take(R * ((V + unit - 1) / unit) * sizeof(float2));
+  p.stream = !a.gradients && a.tokens <= kStreamTokens && !p.pack_x && !p.pack_w;
+  p.unit = p.stream ? kStreamWords : logits_tile_n(rows, a.vocab, a.gradients) / 2;
+  p.units = p.stream ? sms() : (a.vocab + p.unit - 1) / p.unit;
+  p.hit_words = ((a.vocab + p.unit - 1) / p.unit + 31) / 32;
+  p.stats = take(R * p.units * sizeof(float2));
   p.z2 = take(R * std::max<std::size_t>(K, 1) * 4);
   p.index = take(R * K * 4);
   p.q = take(R * K * 4);
   p.count = take(K > 0 ? R * 4 : 0);
   p.entropy = take(K > 0 ? R * 4 : 0);
-  p.hit = take(K > 0 ? R * (((V + unit - 1) / unit + 31) / 32) * 4 : 0);
+  p.hit = take(K > 0 ? R * p.hit_words * 4 : 0);
   p.scale = take(8);
   p.xp = take(p.pack_x ? R * p.ldp * 2 : 0);
   p.wp = take(p.pack_w ? V * p.ldp * 2 : 0);
@@ -991,12 +1209,9 @@ cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const void* w, std::in
     const unsigned grid =
         static_cast<unsigned>(std::min<std::int64_t>((work + 255) / 256, sms() * 32));
     if (vec)
-      vocab_dx_reduce_kernel<T, 4><<<grid, 256, 0, st>>>(g.partial, ks, rows, a.features, dx,
-                                                         a.lddx, scale);
+      MB200_TRY(tc::launch_overlapped(vocab_dx_reduce_kernel<T, 4>, dim3(grid), 256, 0, st, g.partial, ks, rows, a.features, dx, a.lddx, scale));
     else
-      vocab_dx_reduce_kernel<T, 1><<<grid, 256, 0, st>>>(g.partial, ks, rows, a.features, dx,
-                                                         a.lddx, scale);
-    MB200_TRY(cudaGetLastError());
+      MB200_TRY(tc::launch_overlapped(vocab_dx_reduce_kernel<T, 1>, dim3(grid), 256, 0, st, g.partial, ks, rows, a.features, dx, a.lddx, scale));
   }
   return cudaSuccess;
 }
@@ -1040,8 +1255,7 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
   std::int64_t ldw = a.features;
   if (p.pack_w) {
     T* wp = reinterpret_cast<T*>(ws + p.wp);
-    vocab_pack_kernel<T><<<sms() * 8, 256, 0, st>>>(w, ldw, a.vocab, a.features, wp, p.ldp);
-    MB200_TRY(cudaGetLastError());
+    MB200_TRY(tc::launch_overlapped(vocab_pack_kernel<T>, dim3(static_cast<unsigned>(sms() * 8)), 256, 0, st, w, ldw, a.vocab, a.features, wp, p.ldp));
     w = wp;
     ldw = p.ldp;
   }
@@ -1053,9 +1267,7 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     std::int64_t ldx = a.tokens > 1 ? a.ldx : p.ldp;  // one row: its stride is never used
     if (p.pack_x) {
       T* xp = reinterpret_cast<T*>(ws + p.xp);
-      vocab_pack_kernel<T><<<sms() * 8, 256, 0, st>>>(x, ldx, rows, a.features, xp,
-                                                                      p.ldp);
-      MB200_TRY(cudaGetLastError());
+      MB200_TRY(tc::launch_overlapped(vocab_pack_kernel<T>, dim3(static_cast<unsigned>(sms() * 8)), 256, 0, st, x, ldx, rows, a.features, xp, p.ldp));
       x = xp;
       ldx = p.ldp;
     }
@@ -1070,31 +1282,46 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
       int* count = reinterpret_cast<int*>(ws + p.count);
       float* ent = reinterpret_cast<float*>(ws + p.entropy);
       unsigned* hit = reinterpret_cast<unsigned*>(ws + p.hit);
-      const int unit = logits_tile_n(p.rows, a.vocab, a.gradients) / 2;
-      const int hit_words = ((a.vocab + unit - 1) / unit + 31) / 32;
-      vocab_targets_kernel<<<(rows + kTargetWarps - 1) / kTargetWarps, 32 * kTargetWarps, 0, st>>>(
-          a.teacher_index + t0 * a.top_k, a.teacher_logits + t0 * a.top_k, rows, a.top_k, a.vocab,
-          a.inv_tau, index, q, count, ent, hit, hit_words, unit);
-      MB200_TRY(cudaGetLastError());
+      MB200_TRY(tc::launch_overlapped(vocab_targets_kernel, dim3(static_cast<unsigned>((rows + kTargetWarps - 1) / kTargetWarps)), 32 * kTargetWarps, 0, st,  a.teacher_index + t0 * a.top_k, a.teacher_logits + t0 * a.top_k, rows, a.top_k, a.vocab, a.inv_tau, index, q, count, ent, hit, p.hit_words, p.unit));
       tg.index = index;
       tg.q = q;
       tg.count = count;
       tg.neg_entropy = ent;
       tg.hit = hit;
-      tg.hit_words = hit_words;
+      tg.hit_words = p.hit_words;
     }
 
     float* scale = nullptr;
     if (a.gradients && !a.bf16) {
       scale = reinterpret_cast<float*>(ws + p.scale);
-      vocab_grad_scale_kernel<<<1, 1024, 0, st>>>(a.dloss + t0, rows, a.vocab, tg, a.inv_tau,
-                                                  scale);
-      MB200_TRY(cudaGetLastError());
+      MB200_TRY(tc::launch_overlapped(vocab_grad_scale_kernel, dim3(static_cast<unsigned>(1)), 1024, 0, st, a.dloss + t0, rows, a.vocab, tg, a.inv_tau, scale));
+    }
+
+    FinishArgs f{};
+    f.stats = reinterpret_cast<float2*>(ws + p.stats);
+    f.units = p.units;
+    f.unit = p.unit;
+    f.vocab = a.vocab;
+    f.targets = tg;
+    f.loss = a.loss != nullptr ? a.loss + t0 : nullptr;
+    f.lse = a.lse != nullptr ? a.lse + t0 : nullptr;
+    f.inv_tau = a.inv_tau;
+    f.scale = scale;
+    f.num = num;
+    f.ldn = p.ldn;
+    if (p.stream) {
+      const StreamArgs sa{x, ldx, w, ldw, rows, a.features, a.vocab, kLog2e * a.inv_tau,
+                          reinterpret_cast<float2*>(ws + p.stats), tg};
+      const dim3 grid(static_cast<unsigned>(p.units));
+      MB200_TRY(tc::launch_overlapped(vocab_stream_kernel<T>, grid, kStreamThreads, 0, st, sa));
+      MB200_TRY(tc::launch_overlapped(vocab_finish_kernel<T, false>,
+                                      dim3(static_cast<unsigned>(rows)), kFinishThreads, 0, st, f));
+      continue;
     }
 
     const bool pair = rows > tc::kBM;
     LogitsProblem lp{};
-    lp.tile_n = logits_tile_n(p.rows, a.vocab, a.gradients);
+    lp.tile_n = 2 * p.unit;
     if (!make_map(&lp.mx, FMT, x, a.features, rows, ldx, tc::kBK, tc::kBM) ||
         !make_map(&lp.mw, FMT, w, a.features, a.vocab, ldw, tc::kBK, pair ? 128 : lp.tile_n) ||
         (a.gradients && !make_map(&lp.mnum, FMT, num, p.ldn, rows, p.ldn, 64, 32)))
@@ -1102,8 +1329,8 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     lp.num_kb = (a.features + tc::kBK - 1) / tc::kBK;
     lp.rows = rows;
     lp.vocab = a.vocab;
-    lp.unit = lp.tile_n / 2;
-    lp.units = (a.vocab + lp.unit - 1) / lp.unit;
+    lp.unit = p.unit;
+    lp.units = p.units;
     lp.tiles_m = pair ? (rows + 2 * tc::kBM - 1) / (2 * tc::kBM) : 1;
     lp.tiles_n = (a.vocab + lp.tile_n - 1) / lp.tile_n;
     lp.tiles_total = static_cast<long long>(lp.tiles_m) * lp.tiles_n;
@@ -1121,34 +1348,19 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
       MB200_TRY((a.gradients ? run_logits<T, FMT, false, true>(lp, to, st)
                              : run_logits<T, FMT, false, false>(lp, to, st)));
 
-    FinishArgs f{};
-    f.stats = lp.stats;
-    f.units = lp.units;
-    f.unit = lp.unit;
-    f.vocab = a.vocab;
-    f.targets = tg;
-    f.loss = a.loss != nullptr ? a.loss + t0 : nullptr;
-    f.lse = a.lse != nullptr ? a.lse + t0 : nullptr;
-    f.inv_tau = a.inv_tau;
-    f.scale = scale;
-    f.num = num;
-    f.ldn = p.ldn;
     if (!a.gradients) {
-      vocab_finish_kernel<T, false><<<rows, kFinishThreads, 0, st>>>(f);
-      MB200_TRY(cudaGetLastError());
+      MB200_TRY(tc::launch_overlapped(vocab_finish_kernel<T, false>, dim3(static_cast<unsigned>(rows)), kFinishThreads, 0, st, f));
       continue;
     }
     f.dloss = a.dloss + t0;
-    // enough CTAs to fill the GPU when there are few rows, each at least 8192 words
-    const int parts = std::max(1, std::min<int>(4 * sms() / rows, static_cast<int>((p.ldn + 8191) / 8192)));
-    vocab_finish_kernel<T, true><<<dim3(rows, parts), kFinishThreads, 0, st>>>(f);
-    MB200_TRY(cudaGetLastError());
+    // enough CTAs to fill the GPU when there are few rows, each one round of 2048 words at least
+    const int parts =
+        std::max(1, std::min<int>(4 * sms() / rows, static_cast<int>((p.ldn + 2047) / 2048)));
+    MB200_TRY(tc::launch_overlapped(vocab_finish_kernel<T, true>, dim3(static_cast<unsigned>(rows), static_cast<unsigned>(parts)), kFinishThreads, 0, st, f));
 
     T* xt = reinterpret_cast<T*>(ws + p.xt);
     if (a.dw != nullptr) {  // before dx, which may be x itself
-      vocab_transpose_kernel<T><<<dim3((rows + 63) / 64, (a.features + 63) / 64), 256, 0, st>>>(
-          x, ldx, rows, a.features, tg, a.vocab, xt, p.ldt);
-      MB200_TRY(cudaGetLastError());
+      MB200_TRY(tc::launch_overlapped(vocab_transpose_kernel<T>, dim3(static_cast<unsigned>((rows + 63) / 64), static_cast<unsigned>((a.features + 63) / 64)), 256, 0, st,  x, ldx, rows, a.features, tg, a.vocab, xt, p.ldt));
     }
     if (a.dx != nullptr) {
       T* dx = static_cast<T*>(a.dx) + t0 * a.lddx;
