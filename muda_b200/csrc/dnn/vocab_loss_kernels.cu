@@ -94,10 +94,30 @@ struct Targets {
   const float* q;         // [row][top_k]
   const int* count;       // valid entries; 0: row left out, -1: an index of vocab or more
   const float* neg_entropy;  // sum q log q
-  const unsigned* hit;       // [row][hit_words]: bit u set when a target is in unit u
-  int hit_words;
+  const std::uint32_t* hit;  // [row][hit_units]: the first target word in each unit of words
+  int hit_units;
   float* z2;              // [row][max(top_k, 1)]: the target words' z2
 };
+
+// Entry of the hit map: the word's place in its unit, its rank among the row's targets, and
+// whether the row's next target is in the same unit; 0: none in this unit.
+constexpr std::uint32_t kHitValid = 1u << 31, kHitMore = 1u << 30;
+
+__device__ __forceinline__ std::uint32_t hit_entry(int word, int rank, int next_word, int unit) {
+  const int u = word / unit;
+  const bool more = next_word != INT_MAX && next_word / unit == u;
+  return kHitValid | (more ? kHitMore : 0u) | static_cast<std::uint32_t>(rank) << 8 |
+         static_cast<std::uint32_t>(word - u * unit);
+}
+
+// The entry after the one at place `at` of the row's list (its hit said there is one more).
+__device__ __forceinline__ std::uint32_t next_hit(const Targets& t, std::int64_t at, int row,
+                                                  int unit) {
+  const std::int64_t end = (row + 1ll) * t.top_k;
+  const int word = t.index[at + 1];
+  const int after = at + 2 < end ? t.index[at + 2] : INT_MAX;
+  return hit_entry(word, static_cast<int>(at + 1 - (end - t.top_k)), after, unit);
+}
 
 // 0: left out, -1: out-of-range target, else the number of target words.
 __device__ __forceinline__ int target_count(const Targets& t, int row, int vocab) {
@@ -117,7 +137,7 @@ constexpr int kUnit = 128;
 constexpr int kLogitsChunk = 8;
 
 // A thread's logits of one token, and what says whether a target word is among them: the
-// token's label, or its word of the map of units with targets.  Loaded before the
+// token's label, or its entry of the hit map.  Loaded before the
 // accumulator is waited for, looked at after.
 struct LogitsTile {
   float v[kUnit];
@@ -151,35 +171,39 @@ struct LogitsProblem {
 __device__ __forceinline__ std::int64_t target_hint(const LogitsProblem& p, int row, int n0) {
   if (row >= p.rows || n0 >= p.vocab) return p.targets.top_k == 0 ? -1 : 0;
   if (p.targets.top_k == 0) return p.targets.labels[row];
-  const int u = n0 / p.unit;
-  return p.targets.hit[static_cast<std::int64_t>(row) * p.targets.hit_words + (u >> 5)];
+  return p.targets.hit[static_cast<std::int64_t>(row) * p.targets.hit_units + n0 / p.unit];
+}
+
+// v[j] for a j that differs by lane: halves are selected seven times over.
+__device__ __forceinline__ float pick128(const float (&v)[kUnit], int j) {
+  float r[kUnit / 2];
+#pragma unroll
+  for (int i = 0; i < kUnit / 2; ++i) r[i] = (j & (kUnit / 2)) != 0 ? v[i + kUnit / 2] : v[i];
+#pragma unroll
+  for (int h = kUnit / 4; h > 0; h >>= 1) {
+#pragma unroll
+    for (int i = 0; i < kUnit / 4; ++i)
+      if (i < h) r[i] = (j & h) != 0 ? r[i + h] : r[i];
+  }
+  return r[0];
 }
 
 // Stores the z2 of the row's target words among the `cols` from n0 on.
 __device__ __forceinline__ void pick_targets(const LogitsProblem& p, const LogitsTile& t, int row,
                                              int n0, int cols) {
-  int at = 0, next = INT_MAX;
   const int tk = p.targets.top_k;
-  const int* idx = nullptr;
   if (tk == 0) {
-    if (t.hint >= n0 && t.hint < n0 + cols) next = static_cast<int>(t.hint);
-  } else if ((t.hint >> (n0 / p.unit & 31) & 1) != 0) {
-    idx = p.targets.index + static_cast<std::int64_t>(row) * tk;
-    int hi = tk;
-    while (at < hi) {  // the first entry at or after n0
-      const int mid = (at + hi) >> 1;
-      if (idx[mid] < n0) at = mid + 1; else hi = mid;
-    }
-    if (at < tk) next = idx[at];
+    if (t.hint >= n0 && t.hint < n0 + cols)
+      p.targets.z2[row] = __fmul_rn(pick128(t.v, static_cast<int>(t.hint) - n0), p.scale);
+    return;
   }
-  while (next < n0 + cols) {
-    const int j = next - n0;
-    float z = t.v[0];
-#pragma unroll
-    for (int i = 1; i < kUnit; ++i) z = (i == j) ? t.v[i] : z;
-    p.targets.z2[static_cast<std::int64_t>(row) * max(tk, 1) + at] = __fmul_rn(z, p.scale);
-    ++at;
-    next = at < tk ? idx[at] : INT_MAX;
+  auto hint = static_cast<std::uint32_t>(t.hint);
+  while ((hint & kHitValid) != 0) {
+    const std::int64_t at = static_cast<std::int64_t>(row) * tk + (hint >> 8 & 0xFF);
+    p.targets.z2[at] =
+        __fmul_rn(pick128(t.v, static_cast<int>(hint & (kUnit - 1))), p.scale);
+    if ((hint & kHitMore) == 0) break;
+    hint = next_hit(p.targets, at, row, p.unit);
   }
 }
 
@@ -404,9 +428,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1) vocab_stream_kernel(const S
     for (int i = 0; i < kStreamSteps; ++i) fetch(first, 0, i);
   }
   for (int round = first; round < rounds_all; round += stride) {
-    unsigned hint = 0;  // distillation: the round's word of the lane's token's map
+    std::uint32_t hint = 0;  // distillation: the round's entry of token `lane`'s map
     if (a.targets.top_k > 0 && lane < a.rows)
-      hint = a.targets.hit[static_cast<std::int64_t>(lane) * a.targets.hit_words + (round >> 5)];
+      hint = a.targets.hit[static_cast<std::int64_t>(lane) * a.targets.hit_units + round];
     float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int group = 0; group < groups; ++group) {
       const bool more = group + 1 < groups;
@@ -443,22 +467,20 @@ __global__ void __launch_bounds__(kStreamThreads, 1) vocab_stream_kernel(const S
       join_pair(m[j], s[j], ref, exp2_approx(z[j] - ref) + exp2_approx(z[j + 2] - ref));
     }
     if (a.targets.top_k > 0) {
-      unsigned rows = __ballot_sync(0xffffffffu, (hint >> (round & 31) & 1u) != 0u);
+      unsigned rows = __ballot_sync(0xffffffffu, hint != 0u);
       while (rows != 0) {  // tokens with a target among these words
         const int row = __ffs(rows) - 1;
         rows &= rows - 1;
-        const std::int64_t r0 = static_cast<std::int64_t>(row) * a.targets.top_k;
-        const int* idx = a.targets.index + r0;
-        int lo = 0, hi = a.targets.top_k;
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          if (idx[mid] < round * kStreamWords) lo = mid + 1; else hi = mid;
-        }
-        for (; lo < a.targets.top_k && idx[lo] < (round + 1) * kStreamWords; ++lo) {
-          const int at = idx[lo] - round * kStreamWords;
-          if ((at & 7) != g || row >> 1 != t) continue;
-          const float even = at < 8 ? z[0] : z[2], odd = at < 8 ? z[1] : z[3];
-          a.targets.z2[r0 + lo] = (row & 1) != 0 ? odd : even;
+        std::uint32_t hit = __shfl_sync(0xffffffffu, hint, row);
+        for (;;) {
+          const std::int64_t at = static_cast<std::int64_t>(row) * a.targets.top_k + (hit >> 8 & 0xFF);
+          const int word = static_cast<int>(hit & (kStreamWords - 1));
+          if ((word & 7) == g && row >> 1 == t) {
+            const float even = word < 8 ? z[0] : z[2], odd = word < 8 ? z[1] : z[3];
+            a.targets.z2[at] = (row & 1) != 0 ? odd : even;
+          }
+          if ((hit & kHitMore) == 0) break;
+          hit = next_hit(a.targets, at, row, kStreamWords);
         }
       }
       __syncwarp();
@@ -506,16 +528,16 @@ __device__ __forceinline__ int warp_sum(int v) {
 }
 
 // One warp per token: the teacher's distribution over the valid entries, and the entries
-// sorted by word (rank counting: top_k^2 / 32 comparisons per lane), and the map of the
-// units of the logits that hold one.
+// sorted by word (rank counting: top_k^2 / 32 comparisons per lane), and the hit map of the
+// units that the logits come in.
 constexpr int kTargetWarps = 4;
 
 __global__ void __launch_bounds__(32 * kTargetWarps)
     vocab_targets_kernel(const std::int64_t* __restrict__ teacher_index,
                          const float* __restrict__ teacher_logits, int rows, int top_k, int vocab,
-                         float inv_tau, int* __restrict__ index, float* __restrict__ q,
+                         float inv_tau, int* index, float* __restrict__ q,
                          int* __restrict__ count, float* __restrict__ neg_entropy,
-                         unsigned* __restrict__ hit, int hit_words, int unit) {
+                         std::uint32_t* __restrict__ hit, int hit_units, int unit) {
   tc::grid_launch_next();
   tc::grid_wait_previous();
   __shared__ int key_all[kTargetWarps][kVocabMaxTopK];
@@ -524,9 +546,8 @@ __global__ void __launch_bounds__(32 * kTargetWarps)
   const int row = blockIdx.x * kTargetWarps + (threadIdx.x >> 5);
   if (row >= rows) return;
   const std::int64_t r0 = static_cast<std::int64_t>(row) * top_k;
-  unsigned* map = hit + static_cast<std::int64_t>(row) * hit_words;
-  for (int k = lane; k < hit_words; k += 32) map[k] = 0u;
-  __syncwarp();
+  std::uint32_t* map = hit + static_cast<std::int64_t>(row) * hit_units;
+  for (int k = lane; k < hit_units; k += 32) map[k] = 0u;
   float mx = -INFINITY;
   int valid = 0, bad = 0;
   for (int k = lane; k < top_k; k += 32) {
@@ -538,8 +559,6 @@ __global__ void __launch_bounds__(32 * kTargetWarps)
     if (ok) {
       mx = fmaxf(mx, t * inv_tau);
       ++valid;
-      const int u = static_cast<int>(i) / unit;
-      atomicOr(map + (u >> 5), 1u << (u & 31));
     }
   }
   __syncwarp();
@@ -564,6 +583,13 @@ __global__ void __launch_bounds__(32 * kTargetWarps)
     }
     index[r0 + rank] = mine;
     q[r0 + rank] = qk;
+  }
+  __syncwarp();  // the row's sorted list and its cleared map
+  for (int k = lane; k < valid; k += 32) {
+    const int word = index[r0 + k];
+    if (k == 0 || index[r0 + k - 1] / unit != word / unit)
+      map[word / unit] =
+          hit_entry(word, k, k + 1 < valid ? index[r0 + k + 1] : INT_MAX, unit);
   }
   ent = warp_sum(ent);
   if (lane == 0) {
@@ -730,25 +756,53 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
 // xt[h][row] = x[row][h], rows that are left out as zeros (their x may hold anything, and
 // 0 * NaN would reach dw).  K-major x for dw's product: reading x MN-major instead would
 // make both operands MN-major, the slowest form of the tensor-core loop.
-template <typename T>
+// 64 x 64 tiles, 16 bytes per thread and access (VEC: x's rows allow it; x^T's always do).
+// The tile's pitch of 33 words keeps its column reads to two words of a bank.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
     vocab_transpose_kernel(const T* __restrict__ x, std::int64_t ldx, int rows, int features,
                            Targets targets, int vocab, T* __restrict__ xt, std::int64_t ldt) {
   tc::grid_launch_next();
   tc::grid_wait_previous();
-  __shared__ T tile[64][66];
+  __shared__ std::uint32_t tile[64][33];
+  __shared__ bool in[64];
   const int r0 = blockIdx.x * 64, h0 = blockIdx.y * 64;
-  const int lx = threadIdx.x & 63, ly = threadIdx.x >> 6;
-  for (int i = ly; i < 64; i += 4) {
-    const int r = r0 + i, h = h0 + lx;
-    T v = from_float<T>(0.0f);
-    if (r < rows && h < features && target_count(targets, r, vocab) != 0) v = x[r * ldx + h];
-    tile[i][lx] = v;
+  if (threadIdx.x < 64)
+    in[threadIdx.x] = r0 + threadIdx.x < rows && target_count(targets, r0 + threadIdx.x, vocab) != 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = (threadIdx.x >> 3) + 32 * i, h = (threadIdx.x & 7) * 8;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (in[r] && h0 + h < features) {
+      const T* src = x + static_cast<std::int64_t>(r0 + r) * ldx + h0 + h;
+      if (VEC && h0 + h + 8 <= features) {
+        v = *reinterpret_cast<const uint4*>(src);
+      } else {
+        alignas(16) T e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = h0 + h + j < features ? src[j] : from_float<T>(0.0f);
+        v = *reinterpret_cast<const uint4*>(e);
+      }
+    }
+    std::uint32_t* d = &tile[r][h / 2];
+    d[0] = v.x;
+    d[1] = v.y;
+    d[2] = v.z;
+    d[3] = v.w;
   }
   __syncthreads();
-  for (int i = ly; i < 64; i += 4) {
-    const int h = h0 + i, r = r0 + lx;
-    if (h < features && r < rows) xt[h * ldt + r] = tile[lx][i];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int h = (threadIdx.x >> 3) + 32 * i, r = (threadIdx.x & 7) * 8;
+    if (h0 + h >= features || r0 + r >= rows) continue;  // x^T's rows are padded to whole lines
+    std::uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      o[j] = __byte_perm(tile[r + 2 * j][h / 2], tile[r + 2 * j + 1][h / 2],
+                         (h & 1) != 0 ? 0x7632 : 0x5410);
+    *reinterpret_cast<uint4*>(xt + static_cast<std::int64_t>(h0 + h) * ldt + r0 + r) =
+        make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -1059,8 +1113,8 @@ bool tma_rows_ok(const void* p, std::int64_t ld) { return aligned_to(p, 16) && l
 
 struct Plan {
   bool stream;  // scores of few tokens (vocab_stream_kernel)
-  int unit, units;  // words per pair of the logits (stream: per bit of the hit map), pairs
-  int hit_words;    // words of a token's hit map
+  int unit, units;  // words per pair of the logits (stream: per round), pairs per token
+  int hit_units;    // entries of a token's hit map
   int rows;    // tokens per piece (the last may have fewer)
   int pieces;
   int ksplit;
@@ -1097,14 +1151,14 @@ Plan plan_rows(const VocabLossArgs& a, int rows) {
   p.stream = !a.gradients && a.tokens <= kStreamTokens && !p.pack_x && !p.pack_w;
   p.unit = p.stream ? kStreamWords : logits_tile_n(rows, a.vocab, a.gradients) / 2;
   p.units = p.stream ? sms() : (a.vocab + p.unit - 1) / p.unit;
-  p.hit_words = ((a.vocab + p.unit - 1) / p.unit + 31) / 32;
+  p.hit_units = (a.vocab + p.unit - 1) / p.unit;
   p.stats = take(R * p.units * sizeof(float2));
   p.z2 = take(R * std::max<std::size_t>(K, 1) * 4);
   p.index = take(R * K * 4);
   p.q = take(R * K * 4);
   p.count = take(K > 0 ? R * 4 : 0);
   p.entropy = take(K > 0 ? R * 4 : 0);
-  p.hit = take(K > 0 ? R * p.hit_words * 4 : 0);
+  p.hit = take(K > 0 ? R * p.hit_units * 4 : 0);
   p.scale = take(8);
   p.xp = take(p.pack_x ? R * p.ldp * 2 : 0);
   p.wp = take(p.pack_w ? V * p.ldp * 2 : 0);
@@ -1281,14 +1335,14 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
       float* q = reinterpret_cast<float*>(ws + p.q);
       int* count = reinterpret_cast<int*>(ws + p.count);
       float* ent = reinterpret_cast<float*>(ws + p.entropy);
-      unsigned* hit = reinterpret_cast<unsigned*>(ws + p.hit);
-      MB200_TRY(tc::launch_overlapped(vocab_targets_kernel, dim3(static_cast<unsigned>((rows + kTargetWarps - 1) / kTargetWarps)), 32 * kTargetWarps, 0, st,  a.teacher_index + t0 * a.top_k, a.teacher_logits + t0 * a.top_k, rows, a.top_k, a.vocab, a.inv_tau, index, q, count, ent, hit, p.hit_words, p.unit));
+      auto* hit = reinterpret_cast<std::uint32_t*>(ws + p.hit);
+      MB200_TRY(tc::launch_overlapped(vocab_targets_kernel, dim3(static_cast<unsigned>((rows + kTargetWarps - 1) / kTargetWarps)), 32 * kTargetWarps, 0, st,  a.teacher_index + t0 * a.top_k, a.teacher_logits + t0 * a.top_k, rows, a.top_k, a.vocab, a.inv_tau, index, q, count, ent, hit, p.hit_units, p.unit));
       tg.index = index;
       tg.q = q;
       tg.count = count;
       tg.neg_entropy = ent;
       tg.hit = hit;
-      tg.hit_words = p.hit_words;
+      tg.hit_units = p.hit_units;
     }
 
     float* scale = nullptr;
@@ -1360,7 +1414,12 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
 
     T* xt = reinterpret_cast<T*>(ws + p.xt);
     if (a.dw != nullptr) {  // before dx, which may be x itself
-      MB200_TRY(tc::launch_overlapped(vocab_transpose_kernel<T>, dim3(static_cast<unsigned>((rows + 63) / 64), static_cast<unsigned>((a.features + 63) / 64)), 256, 0, st,  x, ldx, rows, a.features, tg, a.vocab, xt, p.ldt));
+      const dim3 grid(static_cast<unsigned>((rows + 63) / 64),
+                      static_cast<unsigned>((a.features + 63) / 64));
+      const bool vec = tma_rows_ok(x, ldx);
+      MB200_TRY(tc::launch_overlapped(
+          vec ? vocab_transpose_kernel<T, true> : vocab_transpose_kernel<T, false>, grid, 256, 0,
+          st, x, ldx, rows, a.features, tg, a.vocab, xt, p.ldt));
     }
     if (a.dx != nullptr) {
       T* dx = static_cast<T*>(a.dx) + t0 * a.lddx;
