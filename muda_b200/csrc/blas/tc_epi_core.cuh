@@ -1,14 +1,14 @@
 // tc_epi_core.cuh — persistent tcgen05 loop for products whose epilogue needs more than
 // tc_gemm_core.cuh's store() hook: 16-bit operands, k-blocks of 64 elements.
 //
-// Three forms.  kPair: a cluster of two CTAs walks tiles of 256 x 256; each CTA accumulates
-// its 128 rows x 256 columns in its own tensor memory and loads its 128 rows of A and its
-// 128 of B's 256 rows, so a k-block costs a CTA 32 KB of loads where a single CTA's
-// 128 x 256 tile costs 48 KB for the same MMA time.  kTall as well: tiles of 512 x 256,
-// two stacked 256 x 256 halves that fill tensor memory, 24 KB per CTA and MMA time; the
-// halves drain in turn before the next tile's MMAs, so it is for long K.  Otherwise single
-// CTAs walk tiles of 128 x tile_n (a multiple of 32 up to 256, chosen at run time): for few
-// rows of one operand, where streaming the other is what takes the time.
+// Three forms, tile_n a multiple of 32 up to 256 that is chosen at run time.  kPair: a
+// cluster of two CTAs walks tiles of 256 x tile_n; each CTA accumulates its 128 rows in its
+// own tensor memory and loads its 128 rows of A and half of B's rows, so a k-block of a
+// 256-wide tile costs a CTA 32 KB of loads where a single CTA's 128 x 256 tile costs 48 KB
+// for the same MMA time.  kTall as well: tiles of 512 x tile_n, two stacked 256-row halves
+// that fill tensor memory, 24 KB per CTA and MMA time; the halves drain in turn before the
+// next tile's MMAs, so it is for long K.  Otherwise single CTAs walk tiles of 128 x tile_n:
+// for few rows of one operand, where streaming the other is what takes the time.
 //   warp 0      issues the CTA's TMA loads (a pair's complete on the even CTA's barriers);
 //   warp 1      issues the MMAs (a pair's: the even CTA) and commits stages and
 //               accumulators back; allocates tensor memory;
@@ -27,9 +27,9 @@
 //   static constexpr bool kAMn;       // A MN-major (64 x 64 boxes), else K-major; B is K-major
 //   static constexpr int kChunk;      // k-blocks per accumulator, 0: the whole tile
 //   static constexpr int kStageBytes; // shared memory of an epilogue warp, a multiple of 1024
-//   long long tiles_total;  int num_kb;  int tile_n;   // tile_n: 256 when kPair
+//   long long tiles_total;  int num_kb;  int tile_n;
 //   const CUtensorMap* map_a() / map_b();           // K-major boxes: 64 x 128 rows of A,
-//                                                   // 64 x 128 (pair) or tile_n rows of B
+//                                                   // 64 x tile_n (pair: tile_n / 2) of B
 //   void coords(long long t, int (&c)[3]) const;    // c[1], c[2]: tile row and column
 //   int k_begin(const int (&c)[3]) const;           // first k-block of the tile
 //   struct Tile;                                    // per-thread epilogue state
@@ -124,7 +124,7 @@ __device__ __forceinline__ void epi_body(const P& p, unsigned int* timeouts) {
   const std::uint32_t tmem_base = *tmem_slot;
   grid_wait_previous();
   const int num_kb = p.num_kb;
-  const int tile_n = kPair ? kEpiN : p.tile_n;
+  const int tile_n = p.tile_n;
   const long long step = gridDim.x / S::kCtas;
   const long long first_tile = blockIdx.x / S::kCtas;
   auto fail = [&]() {
@@ -136,7 +136,7 @@ __device__ __forceinline__ void epi_body(const P& p, unsigned int* timeouts) {
     // ---------------- TMA producer of this CTA's rows
     const std::uint32_t full0 = kPair ? cluster_addr(full, 0) : smem_addr(full);
     const std::uint32_t tx =
-        kPair ? 2 * S::STAGE : S::A_STAGE + static_cast<std::uint32_t>(tile_n * kRowBytes);
+        S::kCtas * S::A_STAGE + static_cast<std::uint32_t>(tile_n * kRowBytes);
     int stage = 0;
     std::uint32_t phase = 0;
     std::uint32_t issued = 0, issued_phase = 0;  // bit per stage
@@ -146,7 +146,7 @@ __device__ __forceinline__ void epi_body(const P& p, unsigned int* timeouts) {
       p.coords(t, c);
       int k = p.k_begin(c) * kBK;
       const int am = c[1] * S::kHalves * S::kCtas * kBM + static_cast<int>(rank) * kBM;
-      const int bn = c[2] * tile_n + static_cast<int>(rank) * (kEpiN / 2);
+      const int bn = c[2] * tile_n + static_cast<int>(rank) * (tile_n / 2);
       for (int kb = 0; kb < num_kb; ++kb, k += kBK) {
         if (!mbar_wait_warp(&empty[stage], phase ^ 1u)) {
           if (lane == 0) fail();

@@ -858,7 +858,7 @@ struct Dx {
   static constexpr int kBand = 8;
   struct Tile {};
   CUtensorMap ma;  // w: dims (features, vocab), box {64, 64, 1}
-  CUtensorMap mb;  // dz: dims (vocab, rows), box {64, 128 or tile_n, 1}
+  CUtensorMap mb;  // dz: dims (vocab, rows), box {64, tile_n or half of it, 1}
   long long tiles_total;
   int num_kb;  // k-blocks per split
   int tile_n, rows, features, tiles_m, tiles_n;
@@ -881,14 +881,14 @@ struct Dx {
   __device__ __forceinline__ void chunk(Tile&, const int (&c)[3], int row, int half,
                                         std::uint32_t taddr, bool, std::uint8_t*) const {
     const int h = c[1] * kRows + row;
-    const int cols = (PAIR ? tc::kEpiN : tile_n) / 2;
+    const int cols = tile_n / 2;
     const float a = scale != nullptr ? scale[1] : 1.0f;
 #pragma unroll 1
     for (int c0 = 0; c0 < cols; c0 += 16) {
       float v[16];
       __syncwarp();
       tc::tmem_load_16cols(taddr + static_cast<std::uint32_t>(c0), v);
-      const int t0 = c[2] * (PAIR ? tc::kEpiN : tile_n) + half * cols + c0;
+      const int t0 = c[2] * tile_n + half * cols + c0;
       if (h >= features) continue;
       if (partial != nullptr) {
         float* o = partial + (static_cast<std::int64_t>(c[0]) * rows + t0) * features + h;
@@ -943,7 +943,8 @@ __global__ void __launch_bounds__(256)
 // dw = dz^T x on CTA pairs: A = dz^T is MN-major in dz, B = x^T (transposed copy) K-major.
 // Each epilogue warp stages its words' features as 128-byte-swizzled boxes of 32 x 64 and
 // sends them by TMA; rows that TMA cannot address go out of the stage in coalesced 2-byte
-// stores.  A call of several pieces adds its pieces in fp32 and rounds once, in the last.
+// stores (aligned 4-byte pairs, with a shuffle where a row starts at an odd element, were
+// slower: 73 against 64 us at 777 x 1111 x 32003).  A call of several pieces adds its pieces in fp32 and rounds once, in the last.
 template <typename T, bool TALL>
 struct Dw {
   static constexpr bool kPair = true, kTall = TALL;
@@ -953,11 +954,11 @@ struct Dw {
   static constexpr int kRows = (TALL ? 4 : 2) * tc::kBM;  // words per tile
   struct Tile {};
   CUtensorMap ma;   // dz: dims (vocab, rows), box {64, 64, 1}
-  CUtensorMap mb;   // x^T: dims (rows, features), box {64, 128, 1}
+  CUtensorMap mb;   // x^T: dims (rows, features), box {64, tile_n / 2, 1}
   CUtensorMap mdw;  // dw: dims (features, vocab), box {64, 32, 1}, when `tma`
   long long tiles_total;
   int num_kb;
-  int tile_n;  // 256
+  int tile_n;  // 256 with `tma`: its boxes are 64 wide
   int vocab, features, tiles_m, tiles_n;
   int band;    // tile columns (features) that stay in L2 while dz streams past
   T* dw;
@@ -979,15 +980,18 @@ struct Dw {
                                         std::uint32_t taddr, bool, std::uint8_t* stage) const {
     const int lane = threadIdx.x & 31;
     const int w = c[1] * kRows + row;
-    const int hw = c[2] * tc::kEpiN + half * 128;
+    const int hw = c[2] * tile_n + half * (tile_n / 2);
     const float a = scale != nullptr ? scale[1] : 1.0f;
     // 64 features at a time through the stage's one box
 #pragma unroll 1
     for (int b = 0; b < 2; ++b) {
       const int h0 = hw + b * 64;
+      const int cols = min(min(64, tile_n / 2 - b * 64), features - h0);  // of this box
+      if (cols <= 0) break;
       if (lane == 0) tc::bulk_wait_read_all();  // the previous box has left the stage
 #pragma unroll 1
       for (int g = 0; g < 2; ++g) {
+        if (g * 32 >= cols) break;
         float v[32];
         __syncwarp();
         tc::tmem_load_32cols(taddr + static_cast<std::uint32_t>(b * 64 + g * 32), v);
@@ -997,7 +1001,7 @@ struct Dw {
           float* o = sum + static_cast<std::int64_t>(w) * features + h0 + g * 32;
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            if (h0 + g * 32 + j >= features) continue;
+            if (g * 32 + j >= cols) continue;
             if (!first) v[j] += o[j];
             if (!last) o[j] = v[j];
           }
@@ -1010,7 +1014,7 @@ struct Dw {
                          pack2<T>(v[8 * k + 4], v[8 * k + 5]), pack2<T>(v[8 * k + 6], v[8 * k + 7]));
         }
       }
-      if (!last || h0 >= features) continue;
+      if (!last) continue;
       if (tma) {
         tc::fence_proxy_async_smem();
         __syncwarp();
@@ -1027,7 +1031,7 @@ struct Dw {
           for (int i = 0; i < 2; ++i) {
             const int col = i * 32 + lane;
             const T* e = reinterpret_cast<const T*>(stage + r * 128 + (((col >> 3) ^ (r & 7)) << 4));
-            if (h0 + col < features) o[col] = e[col & 7];
+            if (col < cols) o[col] = e[col & 7];
           }
         }
         __syncwarp();
@@ -1070,14 +1074,17 @@ int logits_tile_n(int rows, int vocab, bool store) {
   return best;
 }
 
-// Tokens per tile of dx's product on single CTAs: no wider than the tokens.
-int dx_tile_n(int rows) { return static_cast<int>(round_up(std::min(rows, tc::kEpiN), 32)); }
+// Columns per tile: as few tiles as 256 columns need, of even width.
+int even_tile_n(int cols) {
+  const int tiles = (cols + tc::kEpiN - 1) / tc::kEpiN;
+  return static_cast<int>(round_up((cols + tiles - 1) / tiles, 32));
+}
 
 // dx on tall tiles: for a vocabulary that makes K long against the drain of a tile.
 bool dx_tall(int vocab) { return vocab >= 16384; }
 
 // Splits of the words in dx's product: the count that ends soonest.  A k-block takes 512
-// clocks of MMAs per 256 features on a pair; a single CTA's streams w at its share of memory bandwidth
+// clocks of MMAs per 256 x 256 on a pair; a single CTA's streams w at its share of memory bandwidth
 // (measured 5.5 TB/s).  Each split's partial sums are written and read once.
 int dx_splits(int rows, int features, int vocab) {
   const bool pair = rows > tc::kBM;
@@ -1087,7 +1094,7 @@ int dx_splits(int rows, int features, int vocab) {
            : (features + tc::kBM - 1) / tc::kBM;
   const int kb = (vocab + tc::kBK - 1) / tc::kBK;
   const int n = pair ? sms() / 2 : sms();
-  const double block = pair ? bm * 2 / 1.6e9 : tc::kBM * tc::kRowBytes * n / 5.5e12;
+  const double block = pair ? bm * 2 / 1.6e9 * even_tile_n(rows) / tc::kEpiN : tc::kBM * tc::kRowBytes * n / 5.5e12;
   double best = 0.0;
   int pick = 1;
   for (int ks = 1; ks <= 32 && ks * 8 <= std::max(kb, 8); ++ks) {
@@ -1239,9 +1246,9 @@ cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const void* w, std::in
                    const void* num, int rows, T* dx, char* ws, const float* scale,
                    unsigned int* to, cudaStream_t st) {
   Dx<T, PAIR, TALL> g{};
-  g.tile_n = PAIR ? tc::kEpiN : dx_tile_n(rows);
+  g.tile_n = even_tile_n(rows);
   if (!make_map(&g.ma, FMT, w, a.features, a.vocab, ldw, 64, 64) ||
-      !make_map(&g.mb, FMT, num, a.vocab, rows, p.ldn, 64, PAIR ? 128 : g.tile_n))
+      !make_map(&g.mb, FMT, num, a.vocab, rows, p.ldn, 64, PAIR ? g.tile_n / 2 : g.tile_n))
     return cudaErrorInvalidValue;
   const int kb = (a.vocab + tc::kBK - 1) / tc::kBK;
   g.num_kb = (kb + p.ksplit - 1) / p.ksplit;
@@ -1280,16 +1287,16 @@ cudaError_t run_dw(const VocabLossArgs& a, const Plan& p, const void* num, const
                    int piece, char* ws, const float* scale, unsigned int* to, cudaStream_t st) {
   Dw<T, TALL> g{};
   g.tma = tma_rows_ok(a.dw, a.features);
+  g.tile_n = g.tma ? tc::kEpiN : even_tile_n(a.features);
   if (!make_map(&g.ma, FMT, num, a.vocab, rows, p.ldn, 64, 64) ||
-      !make_map(&g.mb, FMT, xt, rows, a.features, p.ldt, tc::kBK, 128) ||
+      !make_map(&g.mb, FMT, xt, rows, a.features, p.ldt, tc::kBK, g.tile_n / 2) ||
       (g.tma && !make_map(&g.mdw, FMT, a.dw, a.features, a.vocab, a.features, 64, 32)))
     return cudaErrorInvalidValue;
   g.num_kb = (rows + tc::kBK - 1) / tc::kBK;
-  g.tile_n = tc::kEpiN;
   g.vocab = a.vocab;
   g.features = a.features;
   g.tiles_m = (a.vocab + Dw<T, TALL>::kRows - 1) / Dw<T, TALL>::kRows;
-  g.tiles_n = (a.features + tc::kEpiN - 1) / tc::kEpiN;
+  g.tiles_n = (a.features + g.tile_n - 1) / g.tile_n;
   g.tiles_total = static_cast<long long>(g.tiles_m) * g.tiles_n;
   // measured at 8192 x 4096 x 65536: 33 MB of x^T kept 5.2 GB of DRAM reads, 67 MB 4.4
   g.band = band_of(g.tiles_n, 512ll * rows, 72ll << 20);
