@@ -96,7 +96,7 @@ struct Targets {
   const float* neg_entropy;  // sum q log q
   const std::uint32_t* hit;  // [row][hit_units]: the first target word in each unit of words
   int hit_units;
-  float* z2;              // [row][max(top_k, 1)]: the target words' z2
+  float* z;               // [row][max(top_k, 1)]: the target words' x w, unscaled
 };
 
 // Entry of the hit map: the word's place in its unit, its rank among the row's targets, and
@@ -188,20 +188,19 @@ __device__ __forceinline__ float pick128(const float (&v)[kUnit], int j) {
   return r[0];
 }
 
-// Stores the z2 of the row's target words among the `cols` from n0 on.
+// Stores the row's target logits among the `cols` words from n0 on.
 __device__ __forceinline__ void pick_targets(const LogitsProblem& p, const LogitsTile& t, int row,
                                              int n0, int cols) {
   const int tk = p.targets.top_k;
   if (tk == 0) {
     if (t.hint >= n0 && t.hint < n0 + cols)
-      p.targets.z2[row] = __fmul_rn(pick128(t.v, static_cast<int>(t.hint) - n0), p.scale);
+      p.targets.z[row] = pick128(t.v, static_cast<int>(t.hint) - n0);
     return;
   }
   auto hint = static_cast<std::uint32_t>(t.hint);
   while ((hint & kHitValid) != 0) {
     const std::int64_t at = static_cast<std::int64_t>(row) * tk + (hint >> 8 & 0xFF);
-    p.targets.z2[at] =
-        __fmul_rn(pick128(t.v, static_cast<int>(hint & (kUnit - 1))), p.scale);
+    p.targets.z[at] = pick128(t.v, static_cast<int>(hint & (kUnit - 1)));
     if ((hint & kHitMore) == 0) break;
     hint = next_hit(p.targets, at, row, p.unit);
   }
@@ -456,15 +455,16 @@ __global__ void __launch_bounds__(kStreamThreads, 1) vocab_stream_kernel(const S
     const int w0 = round * kStreamWords + g;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      z[j] = w0 + (j >> 1) * 8 < a.vocab ? __fmul_rn(z[j], a.scale) : -INFINITY;
+      if (w0 + (j >> 1) * 8 >= a.vocab) z[j] = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      if (label[j] == w0) a.targets.z2[2 * t + j] = z[j];
-      if (label[j] == w0 + 8) a.targets.z2[2 * t + j] = z[j + 2];
+      if (label[j] == w0) a.targets.z[2 * t + j] = z[j];
+      if (label[j] == w0 + 8) a.targets.z[2 * t + j] = z[j + 2];
       const float top = fmaxf(z[j], z[j + 2]);
       // -inf adds nothing; NaN has to (fmaxf passes over it)
-      const float ref = top == -INFINITY ? 0.0f : top;
-      join_pair(m[j], s[j], ref, exp2_approx(z[j] - ref) + exp2_approx(z[j + 2] - ref));
+      const float ref = top == -INFINITY ? 0.0f : __fmul_rn(top, a.scale);
+      join_pair(m[j], s[j], ref, exp2_approx(fmaf(z[j], a.scale, -ref)) +
+                                     exp2_approx(fmaf(z[j + 2], a.scale, -ref)));
     }
     if (a.targets.top_k > 0) {
       unsigned rows = __ballot_sync(0xffffffffu, hint != 0u);
@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) vocab_stream_kernel(const S
           const int word = static_cast<int>(hit & (kStreamWords - 1));
           if ((word & 7) == g && row >> 1 == t) {
             const float even = word < 8 ? z[0] : z[2], odd = word < 8 ? z[1] : z[3];
-            a.targets.z2[at] = (row & 1) != 0 ? odd : even;
+            a.targets.z[at] = (row & 1) != 0 ? odd : even;
           }
           if ((hit & kHitMore) == 0) break;
           hit = next_hit(a.targets, at, row, kStreamWords);
@@ -648,6 +648,7 @@ struct FinishArgs {
   float* lse;   // may be null
   const float* dloss;
   float inv_tau;
+  float log2e_tau;     // log2(e) / tau
   const float* scale;  // fp16: the gradient scale, else null
   void* num;
   std::int64_t ldn;
@@ -691,18 +692,19 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
 
   const int tk = max(a.targets.top_k, 1);
   const std::int64_t r0 = static_cast<std::int64_t>(row) * tk;
+  // a target's z2 - mx in one rounding: a confident word's loss is far below z2's last bit
+  const auto above = [&](std::int64_t i) { return fmaf(a.targets.z[i], a.log2e_tau, -mx); };
   if (blockIdx.y == 0) {
     float loss;
     if (n < 0) {
       loss = NAN;
     } else if (a.targets.top_k == 0) {
-      // the references subtract first: a confident word's loss is far below lse's last bit
-      loss = ((mx - a.targets.z2[r0]) + log_sum) * kLn2;
+      loss = (log_sum - above(r0)) * kLn2;
     } else {
       float cross = 0.0f;
       for (int k = threadIdx.x; k < n; k += kFinishThreads)
         if (a.targets.q[r0 + k] != 0.0f)
-          cross += a.targets.q[r0 + k] * (((mx - a.targets.z2[r0 + k]) + log_sum) * kLn2);
+          cross += a.targets.q[r0 + k] * ((log_sum - above(r0 + k)) * kLn2);
       loss = a.targets.neg_entropy[row] + block_reduce(cross, false, red);
     }
     if (threadIdx.x == 0) {
@@ -739,7 +741,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     if (a.targets.top_k == 0) {
       const std::int64_t l = a.targets.labels[row];
       if (threadIdx.x == 0 && n > 0 && l >= c_begin * 8 && l < c_end * 8)
-        d[l] = from_float<T>(g * expm1f(((a.targets.z2[r0] - mx) - log_sum) * kLn2));
+        d[l] = from_float<T>(g * expm1f((above(r0) - log_sum) * kLn2));
     } else {
       for (int k = threadIdx.x; k < n; k += kFinishThreads) {
         const int w = a.targets.index[r0 + k];
@@ -747,7 +749,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
         if (k > 0 && a.targets.index[r0 + k - 1] == w) continue;  // the run's first entry adds all
         float q = a.targets.q[r0 + k];
         for (int j = k + 1; j < n && a.targets.index[r0 + j] == w; ++j) q += a.targets.q[r0 + j];
-        d[w] = from_float<T>(g * (exp2f((a.targets.z2[r0 + k] - mx) - log_sum) - q));
+        d[w] = from_float<T>(g * (exp2f(above(r0 + k) - log_sum) - q));
       }
     }
   }
@@ -1042,7 +1044,8 @@ struct Dw {
 
 // ------------------------------------------------------------------------- planning --
 constexpr std::size_t kNumeratorCap = std::size_t{2} << 30;  // bytes of a piece's numerators
-constexpr int kScoreRows = 16384;                             // tokens of a piece without them
+constexpr std::size_t kStatsCap = std::size_t{256} << 20;      // a score's pairs
+constexpr int kScoreRows = 16384;                             // tokens of a score's piece
 
 // Elements of a 128-byte line: rows that start on one cost the loads of a 64-wide box one
 // line each, others two.
@@ -1130,7 +1133,7 @@ struct Plan {
   std::int64_t ldp;   // row of packed copies of x and w
   bool pack_x, pack_w;
   // byte offsets into the workspace
-  std::size_t stats, z2, index, q, count, entropy, hit, scale, xp, wp, num, xt, partial, sum, bytes;
+  std::size_t stats, z, index, q, count, entropy, hit, scale, xp, wp, num, xt, partial, sum, bytes;
 };
 
 Plan plan_rows(const VocabLossArgs& a, int rows) {
@@ -1155,12 +1158,12 @@ Plan plan_rows(const VocabLossArgs& a, int rows) {
     return o;
   };
   const std::size_t R = rows, H = a.features, V = a.vocab, K = a.top_k;
-  p.stream = !a.gradients && a.tokens <= kStreamTokens && !p.pack_x && !p.pack_w;
+  p.stream = !a.gradients && a.tokens <= kStreamTokens && !p.pack_w;
   p.unit = p.stream ? kStreamWords : logits_tile_n(rows, a.vocab, a.gradients) / 2;
   p.units = p.stream ? sms() : (a.vocab + p.unit - 1) / p.unit;
   p.hit_units = (a.vocab + p.unit - 1) / p.unit;
   p.stats = take(R * p.units * sizeof(float2));
-  p.z2 = take(R * std::max<std::size_t>(K, 1) * 4);
+  p.z = take(R * std::max<std::size_t>(K, 1) * 4);
   p.index = take(R * K * 4);
   p.q = take(R * K * 4);
   p.count = take(K > 0 ? R * 4 : 0);
@@ -1179,7 +1182,10 @@ Plan plan_rows(const VocabLossArgs& a, int rows) {
 
 // Pieces of equal size, each at most what the caps allow.
 Plan plan_within(const VocabLossArgs& a, std::size_t limit, bool* ok) {
-  std::int64_t most = kScoreRows;
+  // a score's pairs are 16 bytes per 256 words
+  std::int64_t most = std::min<std::int64_t>(
+      kScoreRows, static_cast<std::int64_t>(kStatsCap / (16 * ((a.vocab + 255ull) / 256))));
+  most = std::max<std::int64_t>(128, most / 128 * 128);
   if (a.gradients)
     most = std::max<std::int64_t>(128, static_cast<std::int64_t>(kNumeratorCap / (round_up(a.vocab, kLine) * 2)) / 128 * 128);
   int pieces = static_cast<int>((a.tokens + most - 1) / most);
@@ -1334,7 +1340,7 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     }
     Targets tg{};
     tg.top_k = a.top_k;
-    tg.z2 = reinterpret_cast<float*>(ws + p.z2);
+    tg.z = reinterpret_cast<float*>(ws + p.z);
     if (a.top_k == 0) {
       tg.labels = a.labels + t0;
     } else {
@@ -1367,6 +1373,7 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     f.loss = a.loss != nullptr ? a.loss + t0 : nullptr;
     f.lse = a.lse != nullptr ? a.lse + t0 : nullptr;
     f.inv_tau = a.inv_tau;
+    f.log2e_tau = kLog2e * a.inv_tau;
     f.scale = scale;
     f.num = num;
     f.ldn = p.ldn;
