@@ -204,6 +204,98 @@ def test_distillation(cuda, built, T, H, V, K, tau, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,H,V,K", [
+    (300, 600, 20000, 0),    # dx on tall tiles, two of them along the features
+    (131, 1111, 17003, 5),   # rows that suit neither TMA nor lines, uneven tile widths
+    (6200, 72, 700, 0),      # dw on tall tiles
+    (6200, 121, 515, 3),     # the same with rows of dw that TMA cannot address
+    (2500, 1032, 3001, 0),   # several bands of tiles, five tiles of features
+    (777, 264, 2003, 20),
+    (9, 264, 33000, 0),      # few tokens, many words
+    (128, 520, 20001, 64),
+])
+def test_tilings(cuda, built, T, H, V, K, dtype):
+    h = Head(cuda, T, H, V, dtype, K=K, tau=1.5 if K else 1.0, out=0.1, seed=T + V)
+    with Dnn(cuda) as d:
+        assert h.forward(d) == 0
+        cuda.cuda.synchronize()
+        h.check(gradients=False)
+        assert h.backward(d) == 0
+        cuda.cuda.synchronize()
+    h.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,H,V", [(1, 1000, 333), (3, 136, 5000), (7, 8, 17), (8, 2056, 1601)])
+@pytest.mark.parametrize("K", [0, 1, 40])
+def test_few_tokens_scored(cuda, built, T, H, V, K, dtype):
+    h = Head(cuda, T, H, V, dtype, K=K, tau=2.0 if K else 1.0, seed=H)
+    if K:
+        h.index[:, 0] = V - 1
+    with Dnn(cuda) as d:
+        assert h.forward(d) == 0
+        cuda.cuda.synchronize()
+    h.check(gradients=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [5, 40, 300])
+def test_clustered_targets(cuda, built, T):
+    """Up to 256 targets of a token among neighbouring words, some of them equal."""
+    h = Head(cuda, T, 64, 3000, K=256, seed=T)
+    h.index = cuda.randint(1100, 1100 + 180, (T, 256), device="cuda", generator=h.g)
+    h.index[1] = 2999
+    h.index[2, 3:] = -1
+    with Dnn(cuda) as d:
+        assert h.forward(d) == 0
+        cuda.cuda.synchronize()
+        h.check(gradients=False)
+        assert h.backward(d) == 0
+        cuda.cuda.synchronize()
+    h.check()
+
+
+@pytest.mark.gpu
+def test_nan_word_reaches_every_row(cuda, built):
+    """A NaN in one word's weights makes every live row NaN, as the formula has it."""
+    for T in (4, 100, 300):
+        h = Head(cuda, T, 64, 700, seed=T)
+        h.labels[0] = -1
+        h.w[555, 3] = math.nan
+        with Dnn(cuda) as d:
+            assert h.forward(d) == 0
+            cuda.cuda.synchronize()
+        assert h.loss[1:].isnan().all() and h.lse[1:].isnan().all()
+        assert h.loss[0] == 0 and h.lse[0] == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [0, 7])
+def test_captured_in_a_graph(cuda, built, K):
+    """A captured step replays on new inputs at the same addresses."""
+    h = Head(cuda, 200, 96, 900, K=K, seed=1)
+    other = Head(cuda, 200, 96, 900, K=K, seed=2)
+    stream = cuda.cuda.Stream()
+    with Dnn(cuda) as d, cuda.cuda.stream(stream):
+        assert d.L.cudnnSetStream(d.h, C.c_void_p(stream.cuda_stream)) == 0
+        assert h.backward(d) == 0  # grows the workspace before the capture
+        stream.synchronize()
+        graph = cuda.cuda.CUDAGraph()
+        with cuda.cuda.graph(graph, stream=stream):
+            assert h.backward(d) == 0
+        for name in ("x", "w", "dloss", "labels") + (("index", "teacher") if K else ()):
+            getattr(h, name).copy_(getattr(other, name))
+        for t in (h.loss, h.lse, h.dx, h.dw):
+            t.fill_(math.nan)
+        graph.replay()
+        stream.synchronize()
+        del graph
+    h.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("K", [0, 6])
 def test_rows_left_out_may_hold_anything(cuda, built, K, dtype):
     """NaN and infinite hidden states, teachers and upstream gradients of rows that are out."""
