@@ -3,21 +3,33 @@
 //
 // The T x V logits z = x w^T / tau never exist in memory as such.  A call runs over
 // pieces of tokens; in each piece
-//   1. vocab_logits_kernel walks 128-token x BN-word tiles of z.  The fp32 tile stays in
-//      tensor memory; the epilogue reduces it to one (reference, sum) pair per token and
-//      tile, lse's running maximum and sum, and picks the target words' logits.  With
-//      gradients it also writes the tile's numerators 2^(z2 - reference) in 16 bits;
+//   1. Logits walks tiles of z.  The fp32 tile stays in tensor memory and registers; the
+//      epilogue reduces each token's 128 words (a unit) to one (reference, sum) pair, lse's
+//      running maximum and sum, and picks the target words' logits.  With gradients it also
+//      writes the unit's numerators 2^(z2 - reference) in 16 bits;
 //   2. vocab_finish_kernel joins a token's pairs into its log-sum-exp and loss, and turns
 //      the numerators in place into dz = dloss / tau * (p - q);
-//   3. dx = dz w and dw = dz^T x run on the framework's persistent tensor-core loop.
-// All exponents are in powers of two: z2 = z * log2(e), with log2(e) / tau folded into one
-// multiply, so that 2^(z2 - reference) is one fma and one ex2.
+//   3. Dx and Dw multiply dx = dz w and dw = dz^T x.
+// All three products run on the loop of tc_epi_core.cuh.  Scores of up to 8 tokens take
+// vocab_stream_kernel instead of 1.  Exponents are in powers of two: z2 = z * log2(e), with
+// log2(e) / tau folded into one multiply, so that 2^(z2 - reference) is one fma and one ex2.
+//
+// Why the numerators are kept at all: the gradient needs each logit twice, before and after
+// lse is known.  Computing the product again costs 2 H flops per logit, 5 us per 10^6 logits
+// at H = 4096; keeping 16 bits of it costs 6 bytes of traffic, under 1 us.  The piece bounds
+// them to 2 GiB whatever T and V are.
+//
+// What bounds a training step of 8192 x 4096 x 131072 (19.7 ms, 1340 TFLOP/s): the power
+// cap.  The tensor pipe is busy 95 % of the cycles at 1.15-1.4 GHz.  Of a 1546 us score of
+// 2048 x 4096 x 131072 under the cap, 100 us go with the DRAM reads and 155 us with the L2
+// reads of the operands (timed without them), hence the wide tiles and the banded order.
 //
 // Precision: products of the 16-bit inputs accumulate in fp32; maxima, sums, target
 // logits and losses are fp32.  The numerators are rounded to 16 bits in step 1 and again
 // in step 2 (dz is a 16-bit operand of the tensor cores either way; keeping fp32
 // numerators would double the piece's traffic).  The target words, whose p - q cancels,
-// are recomputed in step 2 from their fp32 logits and rounded once.
+// are recomputed in step 2 from their fp32 logits and rounded once.  dx and dw round once
+// more at the end.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -39,6 +51,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+
 // Tile r of a rows x cols grid, walked in bands of `band` rows, down a band's column before
 // the next column: the tiles in flight share their operands' panels, and a band's rows stay
 // in L2 while the columns stream past.
@@ -655,7 +668,8 @@ struct FinishArgs {
 };
 
 // One row per blockIdx.x; blockIdx.y splits its words (each split joins the row's pairs
-// again, a few KB from L2).
+// again, a few KB from L2).  Bound by HBM: it reads and writes the numerators once, 8192 x
+// 131072 in 0.68 ms (6.3 TB/s).
 template <typename T, bool GRAD>
 __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const FinishArgs a) {
   tc::grid_launch_next();
@@ -758,7 +772,8 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
 // xt[h][row] = x[row][h], rows that are left out as zeros (their x may hold anything, and
 // 0 * NaN would reach dw).  K-major x for dw's product: reading x MN-major instead would
 // make both operands MN-major, the slowest form of the tensor-core loop.
-// 64 x 64 tiles, 16 bytes per thread and access (VEC: x's rows allow it; x^T's always do).
+// 64 x 64 tiles, 16 bytes per thread and access (VEC: x's rows allow it; x^T's always do):
+// 8192 x 4096 in 29 us (4.6 TB/s; 2-byte accesses took 78).
 // The tile's pitch of 33 words keeps its column reads to two words of a bank.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
@@ -964,7 +979,8 @@ struct Dw {
   int vocab, features, tiles_m, tiles_n;
   int band;    // tile columns (features) that stay in L2 while dz streams past
   T* dw;
-  float* sum;  // pieces: [word][feature] running sum, else null
+  float* sum;  // pieces: [word][sum_ld] running sum, else null
+  std::int64_t sum_ld;
   bool first, last;
   bool tma;    // dw's rows are 16-byte aligned
   const float* scale;
@@ -1000,12 +1016,19 @@ struct Dw {
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] *= a;
         if (sum != nullptr && w < vocab) {
-          float* o = sum + static_cast<std::int64_t>(w) * features + h0 + g * 32;
+          float* o = sum + static_cast<std::int64_t>(w) * sum_ld + h0 + g * 32;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
+          for (int j = 0; j < 32; j += 4) {  // sum's rows are whole 16-byte runs
             if (g * 32 + j >= cols) continue;
-            if (!first) v[j] += o[j];
-            if (!last) o[j] = v[j];
+            if (!first) {
+              const float4 was = *reinterpret_cast<const float4*>(o + j);
+              v[j] += was.x;
+              v[j + 1] += was.y;
+              v[j + 2] += was.z;
+              v[j + 3] += was.w;
+            }
+            if (!last)
+              *reinterpret_cast<float4*>(o + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
           }
         }
 #pragma unroll
@@ -1043,7 +1066,9 @@ struct Dw {
 };
 
 // ------------------------------------------------------------------------- planning --
-constexpr std::size_t kNumeratorCap = std::size_t{2} << 30;  // bytes of a piece's numerators
+// Bytes of a piece's numerators.  Every further piece reads and writes dw's fp32 sum: 16384 x
+// 1024 x 131072 took 11.9 ms in one piece of 4 GiB or two of 2 GiB, 12.7 in four of 1 GiB.
+constexpr std::size_t kNumeratorCap = std::size_t{2} << 30;
 constexpr std::size_t kStatsCap = std::size_t{256} << 20;      // a score's pairs
 constexpr int kScoreRows = 16384;                             // tokens of a score's piece
 
@@ -1083,12 +1108,14 @@ int even_tile_n(int cols) {
   return static_cast<int>(round_up((cols + tiles - 1) / tiles, 32));
 }
 
-// dx on tall tiles: for a vocabulary that makes K long against the drain of a tile.
-bool dx_tall(int vocab) { return vocab >= 16384; }
+// dx on tall tiles: for a vocabulary that makes K long against the drain of a tile and dz too
+// large for L2.  Measured (loss and dx, flat and tall): 2048 x 2048 x 16384 212-241 and 247 us,
+// x 32768 479 and 492; 4096 x 4096 x 65536 3644 and 3503.
+bool dx_tall(int vocab) { return vocab >= 49152; }
 
 // Splits of the words in dx's product: the count that ends soonest.  A k-block takes 512
-// clocks of MMAs per 256 x 256 on a pair; a single CTA's streams w at its share of memory bandwidth
-// (measured 5.5 TB/s).  Each split's partial sums are written and read once.
+// clocks of MMAs per 256 x 256 on a pair; a single CTA's streams w at its share of memory
+// bandwidth (measured 5.5 TB/s).  Each split's partial sums are written and read once.
 int dx_splits(int rows, int features, int vocab) {
   const bool pair = rows > tc::kBM;
   const int bm = dx_tall(vocab) ? 512 : 256;
@@ -1097,7 +1124,8 @@ int dx_splits(int rows, int features, int vocab) {
            : (features + tc::kBM - 1) / tc::kBM;
   const int kb = (vocab + tc::kBK - 1) / tc::kBK;
   const int n = pair ? sms() / 2 : sms();
-  const double block = pair ? bm * 2 / 1.6e9 * even_tile_n(rows) / tc::kEpiN : tc::kBM * tc::kRowBytes * n / 5.5e12;
+  const double block = pair ? bm * 2 / 1.6e9 * even_tile_n(rows) / tc::kEpiN
+                            : tc::kBM * tc::kRowBytes * n / 5.5e12;
   double best = 0.0;
   int pick = 1;
   for (int ks = 1; ks <= 32 && ks * 8 <= std::max(kb, 8); ++ks) {
@@ -1175,7 +1203,7 @@ Plan plan_rows(const VocabLossArgs& a, int rows) {
   p.num = take(a.gradients ? R * p.ldn * 2 : 0);
   p.xt = take(dw ? H * p.ldt * 2 : 0);
   p.partial = take(p.ksplit > 1 ? p.ksplit * R * H * 4 : 0);
-  p.sum = take(dw && p.pieces > 1 ? V * H * 4 : 0);
+  p.sum = take(dw && p.pieces > 1 ? V * round_up(a.features, 4) * 4 : 0);
   p.bytes = at;
   return p;
 }
@@ -1308,6 +1336,7 @@ cudaError_t run_dw(const VocabLossArgs& a, const Plan& p, const void* num, const
   g.band = band_of(g.tiles_n, 512ll * rows, 72ll << 20);
   g.dw = static_cast<T*>(a.dw);
   g.sum = p.pieces > 1 ? reinterpret_cast<float*>(ws + p.sum) : nullptr;
+  g.sum_ld = round_up(a.features, 4);
   g.first = piece == 0;
   g.last = piece == p.pieces - 1;
   g.scale = scale;
