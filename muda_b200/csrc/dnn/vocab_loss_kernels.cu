@@ -8,7 +8,9 @@
 //      running maximum and sum, and picks the target words' logits.  With gradients it also
 //      writes the unit's numerators 2^(z2 - reference) in 16 bits;
 //   2. vocab_finish_kernel joins a token's pairs into its log-sum-exp and loss, and turns
-//      the numerators in place into dz = dloss / tau * (p - q);
+//      the numerators in place into dz = dloss / tau * (p - q).  Without dw (a frozen head)
+//      bf16 numerators share a power-of-two reference per token instead, and the token's
+//      factor goes into dx's epilogue: that pass over them falls away (kCommon below);
 //   3. Dx and Dw multiply dx = dz w and dw = dz^T x.
 // All three products run on the loop of tc_epi_core.cuh.  Scores of up to 8 tokens take
 // vocab_stream_kernel instead of 1.  Exponents are in powers of two: z2 = z * log2(e), with
@@ -219,6 +221,14 @@ __device__ __forceinline__ void pick_targets(const LogitsProblem& p, const Logit
   }
 }
 
+// What a unit leaves behind besides its pair: nothing, numerators relative to its own
+// maximum (kOwn), or numerators relative to 2^0 (kCommon, bf16: its exponents reach as far as
+// fp32's).  kCommon takes whole references, so that moving numerators from one to another is
+// exact; units beyond 2^+-64 keep their own until the finish has seen the row's maximum.
+// Loss and dx of 4096 x 2048 x 65536: 1768 us with kOwn, 1657 with kCommon.
+enum StoreMode { kNone = 0, kOwn = 1, kCommon = 2 };
+constexpr float kCommonReach = 64.0f;
+
 // Adds a finished accumulator's columns of the unit (taddr: this thread's lane).
 __device__ __forceinline__ void add_chunk(LogitsTile& t, int unit, std::uint32_t taddr,
                                           bool first) {
@@ -240,7 +250,7 @@ __device__ __forceinline__ void add_chunk(LogitsTile& t, int unit, std::uint32_t
 // Reduces the unit's logits to its pair and picks target words; with STORE leaves the
 // numerators in `stage` as two 128-byte-swizzled boxes of 32 rows x 64 words and sends
 // them to memory (the whole warp calls this).
-template <typename T, bool STORE>
+template <typename T, int STORE>
 __device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& t, int row, int n0,
                                             std::uint8_t* stage) {
   const int lane = threadIdx.x & 31;
@@ -256,9 +266,14 @@ __device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& 
   for (int j = 0; j < kUnit; ++j) m[j & 3] = fmaxf(m[j & 3], t.v[j]);
   const float mx = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
   // a row of -inf (or NaN) has no finite maximum: 0 keeps -inf's numerators at 0
-  const float ref = mx == -INFINITY ? 0.0f : __fmul_rn(mx, p.scale);
+  float ref = mx == -INFINITY ? 0.0f : __fmul_rn(mx, p.scale);
+  float shift = 1.0f;
+  if constexpr (STORE == kCommon) {
+    ref = rintf(ref);
+    if (fabsf(ref) <= kCommonReach) shift = __int_as_float((static_cast<int>(ref) + 127) << 23);
+  }
   pick_targets(p, t, row, n0, cols);
-  if constexpr (STORE) {
+  if constexpr (STORE != kNone) {
     // the previous unit's boxes have left the stage
     if (lane == 0) tc::bulk_wait_read_all();
   }
@@ -272,7 +287,11 @@ __device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& 
       e[j] = exp2_approx(fmaf(t.v[g * 8 + j], p.scale, -ref));
       s[j & 3] += e[j];
     }
-    if constexpr (STORE) {
+    if constexpr (STORE == kCommon) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] *= shift;
+    }
+    if constexpr (STORE != kNone) {
       std::uint8_t* box = stage + (g >> 3) * 4096 + lane * 128 + (((g & 7) ^ (lane & 7)) << 4);
       *reinterpret_cast<uint4*>(box) = make_uint4(pack2<T>(e[0], e[1]), pack2<T>(e[2], e[3]),
                                                   pack2<T>(e[4], e[5]), pack2<T>(e[6], e[7]));
@@ -281,7 +300,7 @@ __device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& 
   if (row < p.rows)
     p.stats[static_cast<std::int64_t>(row) * p.units + n0 / p.unit] =
         make_float2(ref, (s[0] + s[1]) + (s[2] + s[3]));
-  if constexpr (STORE) {
+  if constexpr (STORE != kNone) {
     tc::fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0 && row < p.rows) {  // lane 0 has the warp's first row
@@ -293,12 +312,12 @@ __device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& 
 }
 
 // STORE needs units of 128 words: the stage's boxes are 64 wide.
-template <typename T, bool PAIR, bool STORE>
+template <typename T, bool PAIR, int STORE>
 struct Logits : LogitsProblem {
   static constexpr bool kPair = PAIR, kTall = false;
   static constexpr bool kAMn = false;
   static constexpr int kChunk = kLogitsChunk;
-  static constexpr int kStageBytes = STORE ? 8192 : 0;
+  static constexpr int kStageBytes = STORE != kNone ? 8192 : 0;
   using Tile = LogitsTile;
 
   __device__ __forceinline__ int token(const int (&c)[3], int row) const {
@@ -486,7 +505,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1) vocab_stream_kernel(const S
         rows &= rows - 1;
         std::uint32_t hit = __shfl_sync(0xffffffffu, hint, row);
         for (;;) {
-          const std::int64_t at = static_cast<std::int64_t>(row) * a.targets.top_k + (hit >> 8 & 0xFF);
+          const std::int64_t at =
+              static_cast<std::int64_t>(row) * a.targets.top_k + (hit >> 8 & 0xFF);
           const int word = static_cast<int>(hit & (kStreamWords - 1));
           if ((word & 7) == g && row >> 1 == t) {
             const float even = word < 8 ? z[0] : z[2], odd = word < 8 ? z[1] : z[3];
@@ -665,28 +685,46 @@ struct FinishArgs {
   const float* scale;  // fp16: the gradient scale, else null
   void* num;
   std::int64_t ldn;
+  float* row_scale;    // kCommon: dz = row_scale[row] * numerators, 0 for rows left out
 };
+
+// Eight 16-bit values times f.
+template <typename T>
+__device__ __forceinline__ uint4 scaled(uint4 u, float f) {
+  std::uint32_t* w = reinterpret_cast<std::uint32_t*>(&u);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 v = unpack2<T>(w[j]);
+    w[j] = pack2<T>(f * v.x, f * v.y);
+  }
+  return u;
+}
 
 // One row per blockIdx.x; blockIdx.y splits its words (each split joins the row's pairs
 // again, a few KB from L2).  Bound by HBM: it reads and writes the numerators once, 8192 x
 // 131072 in 0.68 ms (6.3 TB/s).
-template <typename T, bool GRAD>
+template <typename T, int STORE>
 __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const FinishArgs a) {
   tc::grid_launch_next();
   tc::grid_wait_previous();
   __shared__ float red[kFinishThreads / 32];
   const int row = blockIdx.x;
   const int n = target_count(a.targets, row, a.vocab);
-  const std::int64_t chunks = a.ldn / 8;
-  const std::int64_t per = (chunks + gridDim.y - 1) / gridDim.y;
-  const std::int64_t c_begin = per * blockIdx.y, c_end = min(chunks, c_begin + per);
+  // this CTA's units, and their 8-word chunks
+  const int u_per = (a.units + gridDim.y - 1) / gridDim.y;
+  const int u_begin = min(a.units, u_per * static_cast<int>(blockIdx.y));
+  const int u_end = min(a.units, u_begin + u_per);
+  const int per_unit = a.unit / 8;
+  const std::int64_t c_begin = static_cast<std::int64_t>(u_begin) * per_unit;
+  const std::int64_t c_end = min(a.ldn / 8, static_cast<std::int64_t>(u_end) * per_unit);
   uint4* num = reinterpret_cast<uint4*>(static_cast<T*>(a.num) + row * a.ldn);
   if (n == 0) {  // left out
     if (blockIdx.y == 0 && threadIdx.x == 0) {
       if (a.loss != nullptr) a.loss[row] = 0.0f;
       if (a.lse != nullptr) a.lse[row] = 0.0f;
+      if constexpr (STORE == kCommon) a.row_scale[row] = 0.0f;
     }
-    if constexpr (GRAD) {
+    if constexpr (STORE == kOwn) {
       for (std::int64_t c = c_begin + threadIdx.x; c < c_end; c += kFinishThreads)
         num[c] = make_uint4(0, 0, 0, 0);
     }
@@ -726,36 +764,45 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
       if (a.lse != nullptr) a.lse[row] = lse2 * kLn2;
     }
   }
-  if constexpr (GRAD) {
+  if constexpr (STORE != kNone) {
     float g = n < 0 ? NAN : a.dloss[row] * a.inv_tau;
     if (a.scale != nullptr) g *= a.scale[0];
-    const int per_unit = a.unit / 8;
-    const auto scaled = [&](uint4 u, std::int64_t c) {
-      const float f = g * exp2f((st[c / per_unit].x - mx) - log_sum);
-      std::uint32_t* w = reinterpret_cast<std::uint32_t*>(&u);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 v = unpack2<T>(w[j]);
-        w[j] = pack2<T>(f * v.x, f * v.y);
+    float base = 0.0f;  // kCommon: the row's reference
+    if constexpr (STORE == kCommon) {
+      if (fabsf(mx) > kCommonReach) base = mx;
+      if (blockIdx.y == 0 && threadIdx.x == 0)
+        a.row_scale[row] = g * exp2f((base - mx) - log_sum);
+      // only units whose reference is not the row's: rare
+      for (int u = u_begin + (threadIdx.x >> 5); u < u_end; u += kFinishThreads / 32) {
+        const float move = (fabsf(st[u].x) > kCommonReach ? st[u].x : 0.0f) - base;
+        if (st[u].y == 0.0f || move == 0.0f) continue;
+        const float f = exp2f(move);
+        const std::int64_t c = static_cast<std::int64_t>(u) * per_unit + (threadIdx.x & 31);
+        if ((threadIdx.x & 31) < per_unit && c < c_end) num[c] = scaled<T>(num[c], f);
       }
-      return u;
-    };
-    std::int64_t c = c_begin + threadIdx.x;
-    for (; c + 3 * kFinishThreads < c_end; c += 4 * kFinishThreads) {
-      uint4 u[4];
+    } else {
+      const auto factor = [&](std::int64_t c) {
+        return g * exp2f((st[c / per_unit].x - mx) - log_sum);
+      };
+      std::int64_t c = c_begin + threadIdx.x;
+      for (; c + 3 * kFinishThreads < c_end; c += 4 * kFinishThreads) {
+        uint4 u[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) u[j] = num[c + j * kFinishThreads];
+        for (int j = 0; j < 4; ++j) u[j] = num[c + j * kFinishThreads];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        num[c + j * kFinishThreads] = scaled(u[j], c + j * kFinishThreads);
+        for (int j = 0; j < 4; ++j)
+          num[c + j * kFinishThreads] = scaled<T>(u[j], factor(c + j * kFinishThreads));
+      }
+      for (; c < c_end; c += kFinishThreads) num[c] = scaled<T>(num[c], factor(c));
     }
-    for (; c < c_end; c += kFinishThreads) num[c] = scaled(num[c], c);
+    // the targets, in the numerators' units: dz, or dz / row_scale
+    const float t = STORE == kCommon ? exp2f((mx - base) + log_sum) : g;
     __syncthreads();
     T* d = static_cast<T*>(a.num) + row * a.ldn;
     if (a.targets.top_k == 0) {
       const std::int64_t l = a.targets.labels[row];
       if (threadIdx.x == 0 && n > 0 && l >= c_begin * 8 && l < c_end * 8)
-        d[l] = from_float<T>(g * expm1f((above(r0) - log_sum) * kLn2));
+        d[l] = from_float<T>(t * expm1f((above(r0) - log_sum) * kLn2));
     } else {
       for (int k = threadIdx.x; k < n; k += kFinishThreads) {
         const int w = a.targets.index[r0 + k];
@@ -763,7 +810,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
         if (k > 0 && a.targets.index[r0 + k - 1] == w) continue;  // the run's first entry adds all
         float q = a.targets.q[r0 + k];
         for (int j = k + 1; j < n && a.targets.index[r0 + j] == w; ++j) q += a.targets.q[r0 + j];
-        d[w] = from_float<T>(g * (exp2f(above(r0 + k) - log_sum) - q));
+        d[w] = from_float<T>(t * (exp2f(above(r0 + k) - log_sum) - q));
       }
     }
   }
@@ -785,7 +832,8 @@ __global__ void __launch_bounds__(256)
   __shared__ bool in[64];
   const int r0 = blockIdx.x * 64, h0 = blockIdx.y * 64;
   if (threadIdx.x < 64)
-    in[threadIdx.x] = r0 + threadIdx.x < rows && target_count(targets, r0 + threadIdx.x, vocab) != 0;
+    in[threadIdx.x] =
+        r0 + threadIdx.x < rows && target_count(targets, r0 + threadIdx.x, vocab) != 0;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -858,6 +906,11 @@ __global__ void __launch_bounds__(256)
 }
 
 // ------------------------------------------------------------------ gradient GEMMs --
+// A row that is left out has factor 0 and gradient 0, whatever its numerators hold.
+__device__ __forceinline__ float by_row(float factor, float v) {
+  return factor == 0.0f ? 0.0f : factor * v;
+}
+
 // dx^T = w^T dz^T: A = w^T is MN-major in w, B = dz is K-major, the faster operand forms;
 // a thread's columns are tokens of one feature, so a warp's stores of one token are 32
 // consecutive features.  The words (K) split across `ksplit` groups of CTAs.  Pairs (more
@@ -883,6 +936,7 @@ struct Dx {
   std::int64_t lddx;
   float* partial;  // ksplit > 1: [split][row][feature]
   const float* scale;
+  const float* row_scale;  // kCommon: [row], else null
 
   const CUtensorMap* __device__ map_a() const { return &ma; }
   const CUtensorMap* __device__ map_b() const { return &mb; }
@@ -916,7 +970,9 @@ struct Dx {
         T* o = dx + static_cast<std::int64_t>(t0) * lddx + h;
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-          if (t0 + j < rows) o[j * lddx] = from_float<T>(a * v[j]);
+          if (t0 + j < rows)
+            o[j * lddx] = from_float<T>(
+                row_scale != nullptr ? by_row(row_scale[t0 + j], v[j]) : a * v[j]);
       }
     }
   }
@@ -927,7 +983,8 @@ struct Dx {
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
     vocab_dx_reduce_kernel(const float* __restrict__ partial, int ksplit, int rows, int features,
-                           T* __restrict__ dx, std::int64_t lddx, const float* scale) {
+                           T* __restrict__ dx, std::int64_t lddx, const float* scale,
+                           const float* row_scale) {
   tc::grid_launch_next();
   tc::grid_wait_previous();
   const float a = scale != nullptr ? scale[1] : 1.0f;
@@ -939,6 +996,7 @@ __global__ void __launch_bounds__(256)
     const std::int64_t r = i / per, h = (i - r * per) * VEC;
     const float* p = partial + r * features + h;
     T* o = dx + r * lddx + h;
+    const float f = row_scale != nullptr ? row_scale[r] : a;
     if constexpr (VEC == 4) {
       float4 s = __ldcs(reinterpret_cast<const float4*>(p));
 #pragma unroll 4
@@ -946,13 +1004,13 @@ __global__ void __launch_bounds__(256)
         const float4 v = __ldcs(reinterpret_cast<const float4*>(p + k * plane));
         s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
       }
-      *reinterpret_cast<uint2*>(o) =
-          make_uint2(pack2<T>(a * s.x, a * s.y), pack2<T>(a * s.z, a * s.w));
+      *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(by_row(f, s.x), by_row(f, s.y)),
+                                                pack2<T>(by_row(f, s.z), by_row(f, s.w)));
     } else {
       float s = __ldcs(p);
 #pragma unroll 4
       for (int k = 1; k < ksplit; ++k) s += __ldcs(p + k * plane);
-      *o = from_float<T>(a * s);
+      *o = from_float<T>(by_row(f, s));
     }
   }
 }
@@ -961,7 +1019,8 @@ __global__ void __launch_bounds__(256)
 // Each epilogue warp stages its words' features as 128-byte-swizzled boxes of 32 x 64 and
 // sends them by TMA; rows that TMA cannot address go out of the stage in coalesced 2-byte
 // stores (aligned 4-byte pairs, with a shuffle where a row starts at an odd element, were
-// slower: 73 against 64 us at 777 x 1111 x 32003).  A call of several pieces adds its pieces in fp32 and rounds once, in the last.
+// slower: 73 against 64 us at 777 x 1111 x 32003).  A call of several pieces adds its
+// pieces in fp32 and rounds once, in the last.
 template <typename T, bool TALL>
 struct Dw {
   static constexpr bool kPair = true, kTall = TALL;
@@ -1055,7 +1114,8 @@ struct Dw {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int col = i * 32 + lane;
-            const T* e = reinterpret_cast<const T*>(stage + r * 128 + (((col >> 3) ^ (r & 7)) << 4));
+            const T* e =
+                reinterpret_cast<const T*>(stage + r * 128 + (((col >> 3) ^ (r & 7)) << 4));
             if (col < cols) o[col] = e[col & 7];
           }
         }
@@ -1151,6 +1211,7 @@ bool tma_rows_ok(const void* p, std::int64_t ld) { return aligned_to(p, 16) && l
 
 struct Plan {
   bool stream;  // scores of few tokens (vocab_stream_kernel)
+  StoreMode store;
   int unit, units;  // words per pair of the logits (stream: per round), pairs per token
   int hit_units;    // entries of a token's hit map
   int rows;    // tokens per piece (the last may have fewer)
@@ -1161,7 +1222,8 @@ struct Plan {
   std::int64_t ldp;   // row of packed copies of x and w
   bool pack_x, pack_w;
   // byte offsets into the workspace
-  std::size_t stats, z, index, q, count, entropy, hit, scale, xp, wp, num, xt, partial, sum, bytes;
+  std::size_t stats, z, index, q, count, entropy, hit, scale, row_scale, xp, wp, num, xt, partial,
+      sum, bytes;
 };
 
 Plan plan_rows(const VocabLossArgs& a, int rows) {
@@ -1186,6 +1248,7 @@ Plan plan_rows(const VocabLossArgs& a, int rows) {
     return o;
   };
   const std::size_t R = rows, H = a.features, V = a.vocab, K = a.top_k;
+  p.store = !a.gradients ? kNone : dw || !a.bf16 ? kOwn : kCommon;
   p.stream = !a.gradients && a.tokens <= kStreamTokens && !p.pack_w;
   p.unit = p.stream ? kStreamWords : logits_tile_n(rows, a.vocab, a.gradients) / 2;
   p.units = p.stream ? sms() : (a.vocab + p.unit - 1) / p.unit;
@@ -1198,6 +1261,7 @@ Plan plan_rows(const VocabLossArgs& a, int rows) {
   p.entropy = take(K > 0 ? R * 4 : 0);
   p.hit = take(K > 0 ? R * p.hit_units * 4 : 0);
   p.scale = take(8);
+  p.row_scale = take(p.store == kCommon ? R * 4 : 0);
   p.xp = take(p.pack_x ? R * p.ldp * 2 : 0);
   p.wp = take(p.pack_w ? V * p.ldp * 2 : 0);
   p.num = take(a.gradients ? R * p.ldn * 2 : 0);
@@ -1215,7 +1279,8 @@ Plan plan_within(const VocabLossArgs& a, std::size_t limit, bool* ok) {
       kScoreRows, static_cast<std::int64_t>(kStatsCap / (16 * ((a.vocab + 255ull) / 256))));
   most = std::max<std::int64_t>(128, most / 128 * 128);
   if (a.gradients)
-    most = std::max<std::int64_t>(128, static_cast<std::int64_t>(kNumeratorCap / (round_up(a.vocab, kLine) * 2)) / 128 * 128);
+    most = std::max<std::int64_t>(
+        128, static_cast<std::int64_t>(kNumeratorCap / (round_up(a.vocab, kLine) * 2)) / 128 * 128);
   int pieces = static_cast<int>((a.tokens + most - 1) / most);
   Plan p{};
   for (;;) {
@@ -1262,7 +1327,7 @@ unsigned int* timeout_counter() {
   return addr[dev];
 }
 
-template <typename T, int FMT, bool PAIR, bool STORE>
+template <typename T, int FMT, bool PAIR, int STORE>
 cudaError_t run_logits(const LogitsProblem& p, unsigned int* timeouts, cudaStream_t st) {
   Logits<T, PAIR, STORE> q;
   static_cast<LogitsProblem&>(q) = p;
@@ -1297,16 +1362,16 @@ cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const void* w, std::in
   g.lddx = a.lddx;
   g.partial = ks > 1 ? reinterpret_cast<float*>(ws + p.partial) : nullptr;
   g.scale = scale;
+  g.row_scale = p.store == kCommon ? reinterpret_cast<float*>(ws + p.row_scale) : nullptr;
   MB200_TRY((tc::launch_tc_epi<Dx<T, PAIR, TALL>, FMT>(g, sms(), to, st)));
   if (ks > 1) {
     const bool vec = a.features % 4 == 0 && a.lddx % 4 == 0 && aligned_to(dx, 8);
     const std::int64_t work = static_cast<std::int64_t>(rows) * a.features / (vec ? 4 : 1);
     const unsigned grid =
         static_cast<unsigned>(std::min<std::int64_t>((work + 255) / 256, sms() * 32));
-    if (vec)
-      MB200_TRY(tc::launch_overlapped(vocab_dx_reduce_kernel<T, 4>, dim3(grid), 256, 0, st, g.partial, ks, rows, a.features, dx, a.lddx, scale));
-    else
-      MB200_TRY(tc::launch_overlapped(vocab_dx_reduce_kernel<T, 1>, dim3(grid), 256, 0, st, g.partial, ks, rows, a.features, dx, a.lddx, scale));
+    MB200_TRY(tc::launch_overlapped(
+        vec ? vocab_dx_reduce_kernel<T, 4> : vocab_dx_reduce_kernel<T, 1>, dim3(grid), 256, 0, st,
+        g.partial, ks, rows, a.features, dx, a.lddx, scale, g.row_scale));
   }
   return cudaSuccess;
 }
@@ -1347,11 +1412,16 @@ template <typename T, int FMT>
 cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st) {
   unsigned int* to = timeout_counter();
   if (to == nullptr) return cudaErrorInvalidDevice;
+  const auto launch = [&](auto kern, long long gx, int gy, int threads, auto... args) {
+    return tc::launch_overlapped(
+        kern, dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), threads, 0, st, args...);
+  };
   const T* w = static_cast<const T*>(a.w);
   std::int64_t ldw = a.features;
   if (p.pack_w) {
     T* wp = reinterpret_cast<T*>(ws + p.wp);
-    MB200_TRY(tc::launch_overlapped(vocab_pack_kernel<T>, dim3(static_cast<unsigned>(sms() * 8)), 256, 0, st, w, ldw, a.vocab, a.features, wp, p.ldp));
+    MB200_TRY(launch(vocab_pack_kernel<T>, sms() * 8, 1, 256, w, ldw, a.vocab, a.features, wp,
+                     p.ldp));
     w = wp;
     ldw = p.ldp;
   }
@@ -1363,7 +1433,8 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     std::int64_t ldx = a.tokens > 1 ? a.ldx : p.ldp;  // one row: its stride is never used
     if (p.pack_x) {
       T* xp = reinterpret_cast<T*>(ws + p.xp);
-      MB200_TRY(tc::launch_overlapped(vocab_pack_kernel<T>, dim3(static_cast<unsigned>(sms() * 8)), 256, 0, st, x, ldx, rows, a.features, xp, p.ldp));
+      MB200_TRY(launch(vocab_pack_kernel<T>, sms() * 8, 1, 256, x, ldx, rows, a.features, xp,
+                       p.ldp));
       x = xp;
       ldx = p.ldp;
     }
@@ -1378,7 +1449,10 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
       int* count = reinterpret_cast<int*>(ws + p.count);
       float* ent = reinterpret_cast<float*>(ws + p.entropy);
       auto* hit = reinterpret_cast<std::uint32_t*>(ws + p.hit);
-      MB200_TRY(tc::launch_overlapped(vocab_targets_kernel, dim3(static_cast<unsigned>((rows + kTargetWarps - 1) / kTargetWarps)), 32 * kTargetWarps, 0, st,  a.teacher_index + t0 * a.top_k, a.teacher_logits + t0 * a.top_k, rows, a.top_k, a.vocab, a.inv_tau, index, q, count, ent, hit, p.hit_units, p.unit));
+      MB200_TRY(launch(vocab_targets_kernel, (rows + kTargetWarps - 1) / kTargetWarps, 1,
+                       32 * kTargetWarps, a.teacher_index + t0 * a.top_k,
+                       a.teacher_logits + t0 * a.top_k, rows, a.top_k, a.vocab, a.inv_tau, index,
+                       q, count, ent, hit, p.hit_units, p.unit));
       tg.index = index;
       tg.q = q;
       tg.count = count;
@@ -1390,7 +1464,8 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     float* scale = nullptr;
     if (a.gradients && !a.bf16) {
       scale = reinterpret_cast<float*>(ws + p.scale);
-      MB200_TRY(tc::launch_overlapped(vocab_grad_scale_kernel, dim3(static_cast<unsigned>(1)), 1024, 0, st, a.dloss + t0, rows, a.vocab, tg, a.inv_tau, scale));
+      MB200_TRY(launch(vocab_grad_scale_kernel, 1, 1, 1024, a.dloss + t0, rows, a.vocab, tg,
+                       a.inv_tau, scale));
     }
 
     FinishArgs f{};
@@ -1409,10 +1484,8 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     if (p.stream) {
       const StreamArgs sa{x, ldx, w, ldw, rows, a.features, a.vocab, kLog2e * a.inv_tau,
                           reinterpret_cast<float2*>(ws + p.stats), tg};
-      const dim3 grid(static_cast<unsigned>(p.units));
-      MB200_TRY(tc::launch_overlapped(vocab_stream_kernel<T>, grid, kStreamThreads, 0, st, sa));
-      MB200_TRY(tc::launch_overlapped(vocab_finish_kernel<T, false>,
-                                      dim3(static_cast<unsigned>(rows)), kFinishThreads, 0, st, f));
+      MB200_TRY(launch(vocab_stream_kernel<T>, p.units, 1, kStreamThreads, sa));
+      MB200_TRY(launch(vocab_finish_kernel<T, kNone>, rows, 1, kFinishThreads, f));
       continue;
     }
 
@@ -1438,31 +1511,33 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     lp.stats = reinterpret_cast<float2*>(ws + p.stats);
     lp.ldn = p.ldn;
     lp.targets = tg;
-    if (pair)
-      MB200_TRY((a.gradients ? run_logits<T, FMT, true, true>(lp, to, st)
-                             : run_logits<T, FMT, true, false>(lp, to, st)));
-    else
-      MB200_TRY((a.gradients ? run_logits<T, FMT, false, true>(lp, to, st)
-                             : run_logits<T, FMT, false, false>(lp, to, st)));
-
-    if (!a.gradients) {
-      MB200_TRY(tc::launch_overlapped(vocab_finish_kernel<T, false>, dim3(static_cast<unsigned>(rows)), kFinishThreads, 0, st, f));
-      continue;
-    }
-    f.dloss = a.dloss + t0;
     // enough CTAs to fill the GPU when there are few rows, each one round of 2048 words at least
     const int parts =
         std::max(1, std::min<int>(4 * sms() / rows, static_cast<int>((p.ldn + 2047) / 2048)));
-    MB200_TRY(tc::launch_overlapped(vocab_finish_kernel<T, true>, dim3(static_cast<unsigned>(rows), static_cast<unsigned>(parts)), kFinishThreads, 0, st, f));
+    if (p.store == kNone) {
+      MB200_TRY((pair ? run_logits<T, FMT, true, kNone>(lp, to, st)
+                      : run_logits<T, FMT, false, kNone>(lp, to, st)));
+      MB200_TRY(launch(vocab_finish_kernel<T, kNone>, rows, 1, kFinishThreads, f));
+      continue;
+    }
+    f.dloss = a.dloss + t0;
+    if (p.store == kOwn) {
+      MB200_TRY((pair ? run_logits<T, FMT, true, kOwn>(lp, to, st)
+                      : run_logits<T, FMT, false, kOwn>(lp, to, st)));
+      MB200_TRY(launch(vocab_finish_kernel<T, kOwn>, rows, parts, kFinishThreads, f));
+    } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+      f.row_scale = reinterpret_cast<float*>(ws + p.row_scale);
+      MB200_TRY((pair ? run_logits<T, FMT, true, kCommon>(lp, to, st)
+                      : run_logits<T, FMT, false, kCommon>(lp, to, st)));
+      MB200_TRY(launch(vocab_finish_kernel<T, kCommon>, rows, parts, kFinishThreads, f));
+    }
 
     T* xt = reinterpret_cast<T*>(ws + p.xt);
     if (a.dw != nullptr) {  // before dx, which may be x itself
-      const dim3 grid(static_cast<unsigned>((rows + 63) / 64),
-                      static_cast<unsigned>((a.features + 63) / 64));
       const bool vec = tma_rows_ok(x, ldx);
-      MB200_TRY(tc::launch_overlapped(
-          vec ? vocab_transpose_kernel<T, true> : vocab_transpose_kernel<T, false>, grid, 256, 0,
-          st, x, ldx, rows, a.features, tg, a.vocab, xt, p.ldt));
+      MB200_TRY(launch(vec ? vocab_transpose_kernel<T, true> : vocab_transpose_kernel<T, false>,
+                       (rows + 63) / 64, (a.features + 63) / 64, 256, x, ldx, rows, a.features, tg,
+                       a.vocab, xt, p.ldt));
     }
     if (a.dx != nullptr) {
       T* dx = static_cast<T*>(a.dx) + t0 * a.lddx;

@@ -368,6 +368,40 @@ def test_large_logits(cuda, built, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,H,V,K", [(1, 64, 129, 0), (7, 1000, 5003, 4), (129, 65, 255, 0),
+                                     (300, 250, 513, 7), (260, 600, 50001, 0),
+                                     (700, 136, 3000, 30)])
+def test_frozen_head(cuda, built, T, H, V, K, dtype):
+    """Only the hidden states' gradient."""
+    h = Head(cuda, T, H, V, dtype, K=K, tau=2.0 if K else 1.0, out=0.2 if T > 4 else 0.0, seed=T)
+    with Dnn(cuda) as d:
+        assert h.backward(d, dw=False) == 0
+        cuda.cuda.synchronize()
+    h.check(dw=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [0, 5])
+@pytest.mark.parametrize("T", [40, 200])
+@pytest.mark.parametrize("offset", [0.0, 60.0, -60.0, 400.0, -400.0])
+@pytest.mark.parametrize("spread", [1.0, 60.0])
+def test_frozen_head_offset_logits(cuda, built, T, K, offset, spread):
+    """Logits far from zero, by a common offset, by their spread, or both; rows that are left
+    out hold NaN."""
+    h = Head(cuda, T, 128, 900, K=K, spread=spread, out=0.2, seed=T + K)
+    h.x[:, 0] = 8.0
+    h.w[:, 0] = offset / 8.0
+    out = (h.index < 0).all(dim=1) if K else h.labels < 0
+    h.x[out] = math.nan
+    with Dnn(cuda) as d:
+        assert h.backward(d, dw=False) == 0
+        cuda.cuda.synchronize()
+    assert (h.dx[out] == 0).all() and (h.loss[out] == 0).all()
+    h.check(dw=False)
+
+
+@pytest.mark.gpu
 def test_infinite_words(cuda, built):
     """A word whose logit is -inf has probability 0; all of them: NaN, as the formula."""
     h = Head(cuda, 33, 64, 300)
@@ -490,7 +524,8 @@ def test_one_gradient_alone_and_in_place(cuda, built, K):
         h.dw.fill_(math.nan)
         assert h.backward(d, dw=False, loss=False) == 0
         cuda.cuda.synchronize()
-        assert cuda.equal(h.dx, dx) and h.dw.isnan().all()
+        h.check(dw=False, loss=False)
+        assert h.dw.isnan().all()
         h.dx.fill_(math.nan)
         assert h.backward(d, dx=False, loss=False) == 0
         cuda.cuda.synchronize()
