@@ -163,7 +163,7 @@ struct LogitsTile {
 // tokens x tile_n words; reading w bounds these.
 struct LogitsProblem {
   CUtensorMap mx;    // x: dims (features, rows), box {64, 128, 1}
-  CUtensorMap mw;    // w: dims (features, vocab), box {64, 128 or tile_n, 1}
+  CUtensorMap mw;    // w: dims (features, vocab), box {64, tile_n or half of it, 1}
   CUtensorMap mnum;  // numerators: dims (ldn, rows), box {64, 32, 1} (gradients only)
   long long tiles_total;
   int num_kb, tile_n, rows, vocab, tiles_m, tiles_n;
@@ -305,13 +305,14 @@ __device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& 
     __syncwarp();
     if (lane == 0 && row < p.rows) {  // lane 0 has the warp's first row
       tc::tma_store_3d(&p.mnum, stage, n0, row, 0);
-      if (n0 + 64 < p.ldn) tc::tma_store_3d(&p.mnum, stage + 4096, n0 + 64, row, 0);
+      if (p.unit > 64 && n0 + 64 < p.ldn)
+        tc::tma_store_3d(&p.mnum, stage + 4096, n0 + 64, row, 0);
       tc::bulk_commit();
     }
   }
 }
 
-// STORE needs units of 128 words: the stage's boxes are 64 wide.
+// STORE needs units of 64 or 128 words: the stage's boxes are 64 wide.
 template <typename T, bool PAIR, int STORE>
 struct Logits : LogitsProblem {
   static constexpr bool kPair = PAIR, kTall = false;
@@ -328,14 +329,14 @@ struct Logits : LogitsProblem {
   }
   __device__ __forceinline__ void begin(Tile& t, const int (&c)[3], int row, int half) const {
     t.hint = target_hint(*this, token(c, row), word(c, half));
-    if (!PAIR && unit < kUnit) {
+    if (unit < kUnit) {
 #pragma unroll
       for (int j = 0; j < kUnit; ++j) t.v[j] = 0.0f;
     }
   }
   __device__ __forceinline__ void chunk(Tile& t, const int (&)[3], int, int, std::uint32_t taddr,
                                         bool first, std::uint8_t*) const {
-    add_chunk(t, PAIR ? kUnit : unit, taddr, first);
+    add_chunk(t, unit, taddr, first);
   }
   __device__ __forceinline__ void end(Tile& t, const int (&c)[3], int row, int half,
                                       std::uint8_t* stage) const {
@@ -1034,7 +1035,7 @@ struct Dw {
   CUtensorMap mdw;  // dw: dims (features, vocab), box {64, 32, 1}, when `tma`
   long long tiles_total;
   int num_kb;
-  int tile_n;  // 256 with `tma`: its boxes are 64 wide
+  int tile_n;  // 128 or 256 with `tma`: its boxes are 64 wide
   int vocab, features, tiles_m, tiles_n;
   int band;    // tile columns (features) that stay in L2 while dz streams past
   T* dw;
@@ -1143,23 +1144,29 @@ int sms() {
   return n > 0 ? n : 148;
 }
 
-// Words per tile of the logits.  Pairs, and the boxes of stored numerators, take 256; a
-// score of at most 128 tokens is bound by reading w, so it takes the multiple of 32 whose
-// whole waves of tiles cover the vocabulary with the least to spare (the widest such: a
-// wider tile reads x less often).
-int logits_tile_n(int rows, int vocab, bool store) {
-  if (rows > tc::kBM || store) return tc::kEpiN;
+// Width of the tiles of `cols` columns in `rows` tile rows on `groups` CTAs or pairs: the
+// multiple of `step` whose waves end soonest.  A k-block of a 256 x n pair tile takes about
+// 256 + n clocks (below 256 columns shared memory, not the MMAs, sets the pace), of a single
+// CTA's tile n times what one word's line takes to arrive.
+int tile_width(std::int64_t rows, int cols, int groups, int step, bool pair) {
   int best = tc::kEpiN;
   std::int64_t least = INT64_MAX;
-  for (int n = tc::kEpiN; n >= 32; n -= 32) {
-    const std::int64_t tiles = (vocab + n - 1) / n;
-    const std::int64_t cost = (tiles + sms() - 1) / sms() * n;
+  for (int n = tc::kEpiN; n >= step; n -= step) {
+    const std::int64_t tiles = rows * ((cols + n - 1) / n);
+    const std::int64_t cost = (tiles + groups - 1) / groups * (pair ? 256 + n : n);
     if (cost < least) {
       least = cost;
       best = n;
     }
   }
   return best;
+}
+
+// Words per tile of the logits; stored numerators need units (half tiles) of 64 or 128.
+int logits_tile_n(int rows, int vocab, bool store) {
+  const bool pair = rows > tc::kBM;
+  return tile_width(pair ? (rows + 255) / 256 : 1, vocab, pair ? sms() / 2 : sms(),
+                    store ? 128 : 32, pair);
 }
 
 // Columns per tile: as few tiles as 256 columns need, of even width.
@@ -1175,7 +1182,8 @@ bool dx_tall(int vocab) { return vocab >= 49152; }
 
 // Splits of the words in dx's product: the count that ends soonest.  A k-block takes 512
 // clocks of MMAs per 256 x 256 on a pair; a single CTA's streams w at its share of memory
-// bandwidth (measured 5.5 TB/s).  Each split's partial sums are written and read once.
+// bandwidth (measured 5.5 TB/s).  Each split's partial sums are written and read once, by one
+// more launch.
 int dx_splits(int rows, int features, int vocab) {
   const bool pair = rows > tc::kBM;
   const int bm = dx_tall(vocab) ? 512 : 256;
@@ -1191,7 +1199,7 @@ int dx_splits(int rows, int features, int vocab) {
   for (int ks = 1; ks <= 32 && ks * 8 <= std::max(kb, 8); ++ks) {
     const double waves = static_cast<double>((tiles * ks + n - 1) / n);
     const double loop = waves * ((kb + ks - 1) / ks) * block;
-    const double join = ks == 1 ? 0.0 : 4e-6 + 8.0 * ks * rows * features / 4.5e12;
+    const double join = ks == 1 ? 0.0 : 6e-6 + 8.0 * ks * rows * features / 4.5e12;
     if (ks == 1 || loop + join < best) {
       best = loop + join;
       pick = ks;
@@ -1386,7 +1394,8 @@ cudaError_t run_dw(const VocabLossArgs& a, const Plan& p, const void* num, const
                    int piece, char* ws, const float* scale, unsigned int* to, cudaStream_t st) {
   Dw<T, TALL> g{};
   g.tma = tma_rows_ok(a.dw, a.features);
-  g.tile_n = g.tma ? tc::kEpiN : even_tile_n(a.features);
+  constexpr int kRows = Dw<T, TALL>::kRows;
+  g.tile_n = tile_width((a.vocab + kRows - 1) / kRows, a.features, sms() / 2, g.tma ? 128 : 32, true);
   if (!make_map(&g.ma, FMT, num, a.vocab, rows, p.ldn, 64, 64) ||
       !make_map(&g.mb, FMT, xt, rows, a.features, p.ldt, tc::kBK, g.tile_n / 2) ||
       (g.tma && !make_map(&g.mdw, FMT, a.dw, a.features, a.vocab, a.features, 64, 32)))
@@ -1394,7 +1403,7 @@ cudaError_t run_dw(const VocabLossArgs& a, const Plan& p, const void* num, const
   g.num_kb = (rows + tc::kBK - 1) / tc::kBK;
   g.vocab = a.vocab;
   g.features = a.features;
-  g.tiles_m = (a.vocab + Dw<T, TALL>::kRows - 1) / Dw<T, TALL>::kRows;
+  g.tiles_m = (a.vocab + kRows - 1) / kRows;
   g.tiles_n = (a.features + g.tile_n - 1) / g.tile_n;
   g.tiles_total = static_cast<long long>(g.tiles_m) * g.tiles_n;
   // measured at 8192 x 4096 x 65536: 33 MB of x^T kept 5.2 GB of DRAM reads, 67 MB 4.4
@@ -1493,7 +1502,8 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     LogitsProblem lp{};
     lp.tile_n = 2 * p.unit;
     if (!make_map(&lp.mx, FMT, x, a.features, rows, ldx, tc::kBK, tc::kBM) ||
-        !make_map(&lp.mw, FMT, w, a.features, a.vocab, ldw, tc::kBK, pair ? 128 : lp.tile_n) ||
+        !make_map(&lp.mw, FMT, w, a.features, a.vocab, ldw, tc::kBK,
+                  pair ? lp.tile_n / 2 : lp.tile_n) ||
         (a.gradients && !make_map(&lp.mnum, FMT, num, p.ldn, rows, p.ldn, 64, 32)))
       return cudaErrorInvalidValue;
     lp.num_kb = (a.features + tc::kBK - 1) / tc::kBK;
