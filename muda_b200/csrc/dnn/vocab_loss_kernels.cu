@@ -674,8 +674,18 @@ __device__ __forceinline__ float block_reduce(float v, bool is_max, float* red) 
   return r;
 }
 
+struct TransposeArgs {
+  const void* x;
+  std::int64_t ldx;
+  int rows, features;
+  bool vec;  // 16-byte reads
+  void* xt;  // null: nothing to do
+  std::int64_t ldt;
+};
+
 struct FinishArgs {
   const float2* stats;  // [row][units]
+  int rows, parts;      // CTAs: one per row and part of its words, then the transpose's
   int units, unit, vocab;
   Targets targets;
   float* loss;  // may be null
@@ -687,7 +697,65 @@ struct FinishArgs {
   void* num;
   std::int64_t ldn;
   float* row_scale;    // kCommon: dz = row_scale[row] * numerators, 0 for rows left out
+  TransposeArgs transpose;  // kOwn: x^T for dw's product, in the same launch
 };
+
+// xt[h][row] = x[row][h], rows that are left out as zeros (their x may hold anything, and
+// 0 * NaN would reach dw).  K-major x for dw's product: reading x MN-major instead would
+// make both operands MN-major, the slowest form of the tensor-core loop.
+// 64 x 64 tiles, 16 bytes per thread and access (reads: where x's rows allow it): 8192 x 4096
+// in 29 us as a launch of its own (4.6 TB/s; 2-byte accesses took 78).
+// The tile's pitch of 33 words keeps its column reads to two words of a bank.
+template <typename T>
+__device__ __forceinline__ void transpose_tile(const TransposeArgs& a, const Targets& targets,
+                                               int vocab, long long block) {
+  __shared__ std::uint32_t tile[64][33];
+  __shared__ bool in[64];
+  const T* x = static_cast<const T*>(a.x);
+  T* xt = static_cast<T*>(a.xt);
+  const std::int64_t ldx = a.ldx, ldt = a.ldt;
+  const int rows = a.rows, features = a.features;
+  const int across = (rows + 63) / 64;
+  const int r0 = static_cast<int>(block % across) * 64, h0 = static_cast<int>(block / across) * 64;
+  if (threadIdx.x < 64)
+    in[threadIdx.x] =
+        r0 + threadIdx.x < rows && target_count(targets, r0 + threadIdx.x, vocab) != 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = (threadIdx.x >> 3) + 32 * i, h = (threadIdx.x & 7) * 8;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (in[r] && h0 + h < features) {
+      const T* src = x + static_cast<std::int64_t>(r0 + r) * ldx + h0 + h;
+      if (a.vec && h0 + h + 8 <= features) {
+        v = *reinterpret_cast<const uint4*>(src);
+      } else {
+        alignas(16) T e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = h0 + h + j < features ? src[j] : from_float<T>(0.0f);
+        v = *reinterpret_cast<const uint4*>(e);
+      }
+    }
+    std::uint32_t* d = &tile[r][h / 2];
+    d[0] = v.x;
+    d[1] = v.y;
+    d[2] = v.z;
+    d[3] = v.w;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int h = (threadIdx.x >> 3) + 32 * i, r = (threadIdx.x & 7) * 8;
+    if (h0 + h >= features || r0 + r >= rows) continue;  // x^T's rows are padded to whole lines
+    std::uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      o[j] = __byte_perm(tile[r + 2 * j][h / 2], tile[r + 2 * j + 1][h / 2],
+                         (h & 1) != 0 ? 0x7632 : 0x5410);
+    *reinterpret_cast<uint4*>(xt + static_cast<std::int64_t>(h0 + h) * ldt + r0 + r) =
+        make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
 
 // Eight 16-bit values times f.
 template <typename T>
@@ -701,26 +769,34 @@ __device__ __forceinline__ uint4 scaled(uint4 u, float f) {
   return u;
 }
 
-// One row per blockIdx.x; blockIdx.y splits its words (each split joins the row's pairs
-// again, a few KB from L2).  Bound by HBM: it reads and writes the numerators once, 8192 x
+// A CTA per row and part of its words (each part joins the row's pairs again, a few KB from
+// L2), then one per tile of the transpose.  Bound by HBM: it reads and writes the numerators once, 8192 x
 // 131072 in 0.68 ms (6.3 TB/s).
 template <typename T, int STORE>
 __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const FinishArgs a) {
   tc::grid_launch_next();
   tc::grid_wait_previous();
   __shared__ float red[kFinishThreads / 32];
-  const int row = blockIdx.x;
+  const long long finish = static_cast<long long>(a.rows) * a.parts;
+  if constexpr (STORE == kOwn) {
+    if (blockIdx.x >= finish) {
+      transpose_tile<T>(a.transpose, a.targets, a.vocab, blockIdx.x - finish);
+      return;
+    }
+  }
+  const int row = static_cast<int>(blockIdx.x % static_cast<unsigned>(a.rows));
+  const int part = static_cast<int>(blockIdx.x / static_cast<unsigned>(a.rows));
   const int n = target_count(a.targets, row, a.vocab);
   // this CTA's units, and their 8-word chunks
-  const int u_per = (a.units + gridDim.y - 1) / gridDim.y;
-  const int u_begin = min(a.units, u_per * static_cast<int>(blockIdx.y));
+  const int u_per = (a.units + a.parts - 1) / a.parts;
+  const int u_begin = min(a.units, u_per * part);
   const int u_end = min(a.units, u_begin + u_per);
   const int per_unit = a.unit / 8;
   const std::int64_t c_begin = static_cast<std::int64_t>(u_begin) * per_unit;
   const std::int64_t c_end = min(a.ldn / 8, static_cast<std::int64_t>(u_end) * per_unit);
   uint4* num = reinterpret_cast<uint4*>(static_cast<T*>(a.num) + row * a.ldn);
   if (n == 0) {  // left out
-    if (blockIdx.y == 0 && threadIdx.x == 0) {
+    if (part == 0 && threadIdx.x == 0) {
       if (a.loss != nullptr) a.loss[row] = 0.0f;
       if (a.lse != nullptr) a.lse[row] = 0.0f;
       if constexpr (STORE == kCommon) a.row_scale[row] = 0.0f;
@@ -747,7 +823,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
   const std::int64_t r0 = static_cast<std::int64_t>(row) * tk;
   // a target's z2 - mx in one rounding: a confident word's loss is far below z2's last bit
   const auto above = [&](std::int64_t i) { return fmaf(a.targets.z[i], a.log2e_tau, -mx); };
-  if (blockIdx.y == 0) {
+  if (part == 0) {
     float loss;
     if (n < 0) {
       loss = NAN;
@@ -771,7 +847,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     float base = 0.0f;  // kCommon: the row's reference
     if constexpr (STORE == kCommon) {
       if (fabsf(mx) > kCommonReach) base = mx;
-      if (blockIdx.y == 0 && threadIdx.x == 0)
+      if (part == 0 && threadIdx.x == 0)
         a.row_scale[row] = g * exp2f((base - mx) - log_sum);
       // only units whose reference is not the row's: rare
       for (int u = u_begin + (threadIdx.x >> 5); u < u_end; u += kFinishThreads / 32) {
@@ -814,61 +890,6 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
         d[w] = from_float<T>(t * (exp2f(above(r0 + k) - log_sum) - q));
       }
     }
-  }
-}
-
-// xt[h][row] = x[row][h], rows that are left out as zeros (their x may hold anything, and
-// 0 * NaN would reach dw).  K-major x for dw's product: reading x MN-major instead would
-// make both operands MN-major, the slowest form of the tensor-core loop.
-// 64 x 64 tiles, 16 bytes per thread and access (VEC: x's rows allow it; x^T's always do):
-// 8192 x 4096 in 29 us (4.6 TB/s; 2-byte accesses took 78).
-// The tile's pitch of 33 words keeps its column reads to two words of a bank.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256)
-    vocab_transpose_kernel(const T* __restrict__ x, std::int64_t ldx, int rows, int features,
-                           Targets targets, int vocab, T* __restrict__ xt, std::int64_t ldt) {
-  tc::grid_launch_next();
-  tc::grid_wait_previous();
-  __shared__ std::uint32_t tile[64][33];
-  __shared__ bool in[64];
-  const int r0 = blockIdx.x * 64, h0 = blockIdx.y * 64;
-  if (threadIdx.x < 64)
-    in[threadIdx.x] =
-        r0 + threadIdx.x < rows && target_count(targets, r0 + threadIdx.x, vocab) != 0;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = (threadIdx.x >> 3) + 32 * i, h = (threadIdx.x & 7) * 8;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (in[r] && h0 + h < features) {
-      const T* src = x + static_cast<std::int64_t>(r0 + r) * ldx + h0 + h;
-      if (VEC && h0 + h + 8 <= features) {
-        v = *reinterpret_cast<const uint4*>(src);
-      } else {
-        alignas(16) T e[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = h0 + h + j < features ? src[j] : from_float<T>(0.0f);
-        v = *reinterpret_cast<const uint4*>(e);
-      }
-    }
-    std::uint32_t* d = &tile[r][h / 2];
-    d[0] = v.x;
-    d[1] = v.y;
-    d[2] = v.z;
-    d[3] = v.w;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int h = (threadIdx.x >> 3) + 32 * i, r = (threadIdx.x & 7) * 8;
-    if (h0 + h >= features || r0 + r >= rows) continue;  // x^T's rows are padded to whole lines
-    std::uint32_t o[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      o[j] = __byte_perm(tile[r + 2 * j][h / 2], tile[r + 2 * j + 1][h / 2],
-                         (h & 1) != 0 ? 0x7632 : 0x5410);
-    *reinterpret_cast<uint4*>(xt + static_cast<std::int64_t>(h0 + h) * ldt + r0 + r) =
-        make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
@@ -1395,7 +1416,8 @@ cudaError_t run_dw(const VocabLossArgs& a, const Plan& p, const void* num, const
   Dw<T, TALL> g{};
   g.tma = tma_rows_ok(a.dw, a.features);
   constexpr int kRows = Dw<T, TALL>::kRows;
-  g.tile_n = tile_width((a.vocab + kRows - 1) / kRows, a.features, sms() / 2, g.tma ? 128 : 32, true);
+  g.tile_n = tile_width((a.vocab + kRows - 1) / kRows, a.features, sms() / 2, g.tma ? 128 : 32,
+                        true);
   if (!make_map(&g.ma, FMT, num, a.vocab, rows, p.ldn, 64, 64) ||
       !make_map(&g.mb, FMT, xt, rows, a.features, p.ldt, tc::kBK, g.tile_n / 2) ||
       (g.tma && !make_map(&g.mdw, FMT, a.dw, a.features, a.vocab, a.features, 64, 32)))
@@ -1421,15 +1443,14 @@ template <typename T, int FMT>
 cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st) {
   unsigned int* to = timeout_counter();
   if (to == nullptr) return cudaErrorInvalidDevice;
-  const auto launch = [&](auto kern, long long gx, int gy, int threads, auto... args) {
-    return tc::launch_overlapped(
-        kern, dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy)), threads, 0, st, args...);
+  const auto launch = [&](auto kern, long long ctas, int threads, auto... args) {
+    return tc::launch_overlapped(kern, dim3(static_cast<unsigned>(ctas)), threads, 0, st, args...);
   };
   const T* w = static_cast<const T*>(a.w);
   std::int64_t ldw = a.features;
   if (p.pack_w) {
     T* wp = reinterpret_cast<T*>(ws + p.wp);
-    MB200_TRY(launch(vocab_pack_kernel<T>, sms() * 8, 1, 256, w, ldw, a.vocab, a.features, wp,
+    MB200_TRY(launch(vocab_pack_kernel<T>, sms() * 8, 256, w, ldw, a.vocab, a.features, wp,
                      p.ldp));
     w = wp;
     ldw = p.ldp;
@@ -1442,7 +1463,7 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     std::int64_t ldx = a.tokens > 1 ? a.ldx : p.ldp;  // one row: its stride is never used
     if (p.pack_x) {
       T* xp = reinterpret_cast<T*>(ws + p.xp);
-      MB200_TRY(launch(vocab_pack_kernel<T>, sms() * 8, 1, 256, x, ldx, rows, a.features, xp,
+      MB200_TRY(launch(vocab_pack_kernel<T>, sms() * 8, 256, x, ldx, rows, a.features, xp,
                        p.ldp));
       x = xp;
       ldx = p.ldp;
@@ -1458,7 +1479,7 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
       int* count = reinterpret_cast<int*>(ws + p.count);
       float* ent = reinterpret_cast<float*>(ws + p.entropy);
       auto* hit = reinterpret_cast<std::uint32_t*>(ws + p.hit);
-      MB200_TRY(launch(vocab_targets_kernel, (rows + kTargetWarps - 1) / kTargetWarps, 1,
+      MB200_TRY(launch(vocab_targets_kernel, (rows + kTargetWarps - 1) / kTargetWarps,
                        32 * kTargetWarps, a.teacher_index + t0 * a.top_k,
                        a.teacher_logits + t0 * a.top_k, rows, a.top_k, a.vocab, a.inv_tau, index,
                        q, count, ent, hit, p.hit_units, p.unit));
@@ -1473,11 +1494,13 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     float* scale = nullptr;
     if (a.gradients && !a.bf16) {
       scale = reinterpret_cast<float*>(ws + p.scale);
-      MB200_TRY(launch(vocab_grad_scale_kernel, 1, 1, 1024, a.dloss + t0, rows, a.vocab, tg,
+      MB200_TRY(launch(vocab_grad_scale_kernel, 1, 1024, a.dloss + t0, rows, a.vocab, tg,
                        a.inv_tau, scale));
     }
 
     FinishArgs f{};
+    f.rows = rows;
+    f.parts = 1;
     f.stats = reinterpret_cast<float2*>(ws + p.stats);
     f.units = p.units;
     f.unit = p.unit;
@@ -1493,8 +1516,8 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     if (p.stream) {
       const StreamArgs sa{x, ldx, w, ldw, rows, a.features, a.vocab, kLog2e * a.inv_tau,
                           reinterpret_cast<float2*>(ws + p.stats), tg};
-      MB200_TRY(launch(vocab_stream_kernel<T>, p.units, 1, kStreamThreads, sa));
-      MB200_TRY(launch(vocab_finish_kernel<T, kNone>, rows, 1, kFinishThreads, f));
+      MB200_TRY(launch(vocab_stream_kernel<T>, p.units, kStreamThreads, sa));
+      MB200_TRY(launch(vocab_finish_kernel<T, kNone>, rows, kFinishThreads, f));
       continue;
     }
 
@@ -1527,28 +1550,29 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     if (p.store == kNone) {
       MB200_TRY((pair ? run_logits<T, FMT, true, kNone>(lp, to, st)
                       : run_logits<T, FMT, false, kNone>(lp, to, st)));
-      MB200_TRY(launch(vocab_finish_kernel<T, kNone>, rows, 1, kFinishThreads, f));
+      MB200_TRY(launch(vocab_finish_kernel<T, kNone>, rows, kFinishThreads, f));
       continue;
     }
     f.dloss = a.dloss + t0;
+    f.parts = parts;
+    T* xt = reinterpret_cast<T*>(ws + p.xt);
+    long long tiles = 0;
+    if (a.dw != nullptr) {  // before dx, which may be x itself
+      f.transpose = {x, ldx, rows, a.features, tma_rows_ok(x, ldx), xt, p.ldt};
+      tiles = static_cast<long long>((rows + 63) / 64) * ((a.features + 63) / 64);
+    }
+    const long long finish = static_cast<long long>(rows) * parts;
     if (p.store == kOwn) {
       MB200_TRY((pair ? run_logits<T, FMT, true, kOwn>(lp, to, st)
                       : run_logits<T, FMT, false, kOwn>(lp, to, st)));
-      MB200_TRY(launch(vocab_finish_kernel<T, kOwn>, rows, parts, kFinishThreads, f));
+      MB200_TRY(launch(vocab_finish_kernel<T, kOwn>, finish + tiles, kFinishThreads, f));
     } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
       f.row_scale = reinterpret_cast<float*>(ws + p.row_scale);
       MB200_TRY((pair ? run_logits<T, FMT, true, kCommon>(lp, to, st)
                       : run_logits<T, FMT, false, kCommon>(lp, to, st)));
-      MB200_TRY(launch(vocab_finish_kernel<T, kCommon>, rows, parts, kFinishThreads, f));
+      MB200_TRY(launch(vocab_finish_kernel<T, kCommon>, finish, kFinishThreads, f));
     }
 
-    T* xt = reinterpret_cast<T*>(ws + p.xt);
-    if (a.dw != nullptr) {  // before dx, which may be x itself
-      const bool vec = tma_rows_ok(x, ldx);
-      MB200_TRY(launch(vec ? vocab_transpose_kernel<T, true> : vocab_transpose_kernel<T, false>,
-                       (rows + 63) / 64, (a.features + 63) / 64, 256, x, ldx, rows, a.features, tg,
-                       a.vocab, xt, p.ldt));
-    }
     if (a.dx != nullptr) {
       T* dx = static_cast<T*>(a.dx) + t0 * a.lddx;
       if (pair && dx_tall(a.vocab))
