@@ -355,14 +355,14 @@ struct Logits : LogitsProblem {
 // against 131072 x 4096 178 us (6.0 TB/s) and 209.
 //
 // A lane keeps its own running (maximum, sum) of the words it sees; the CTA joins them once
-// at the end into one pair per token.  As above, fp32 sums of chunks bound the MMA's drift.
+// at the end into one pair per token.  Every eight MMAs go into an fp32 sum, which bounds the
+// drift of their truncating accumulation.
 constexpr int kStreamTokens = 8;
 constexpr int kStreamWords = 16;    // words per warp and round
 constexpr int kStreamThreads = 512;
 // Steps of 32 features in flight per warp: 8 x 2048 x 32000 took 25.9 us with 4 and 27.5 with
 // 8, 8 x 4096 x 131072 179.8 and 177.
 constexpr int kStreamSteps = 4;
-constexpr int kStreamChunk = 4;     // groups of steps per accumulator: 32 MMAs
 
 struct StreamArgs {
   const void* x;
@@ -476,12 +476,10 @@ __global__ void __launch_bounds__(kStreamThreads, 1) vocab_stream_kernel(const S
         mma_16x8x16<T>(acc, in[i][0].z, in[i][1].z, in[i][0].w, in[i][1].w, b.z, b.w);
         fetch(next_round, next_group, i);
       }
-      if (group % kStreamChunk == kStreamChunk - 1 || !more) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          z[j] = __fadd_rn(z[j], acc[j]);
-          acc[j] = 0.0f;
-        }
+      for (int j = 0; j < 4; ++j) {
+        z[j] = __fadd_rn(z[j], acc[j]);
+        acc[j] = 0.0f;
       }
     }
     // z[0..1]: word g, tokens 2t and 2t + 1; z[2..3]: word g + 8
