@@ -316,12 +316,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kEpiThreads, 1)
   epi_body<P, FMT>(p, timeouts);
 }
 
-// Launches `kern` so that its prologue may overlap the end of the stream's previous kernel
-// (the kernel calls grid_wait_previous() before it touches memory).  tc_epi kernels do not
+// Launches `kern`; with `overlap` its prologue may overlap the end of the stream's previous
+// kernel (it calls grid_wait_previous() before it touches memory).  Overlap only with a
+// kernel that waits for its own predecessor in turn: one's own.  tc_epi kernels do not
 // let the next one start early: its waiting CTAs cost them 2-4 %.
 template <typename... K, typename... A>
 cudaError_t launch_overlapped(void (*kern)(K...), dim3 grid, int threads, std::size_t smem,
-                              cudaStream_t stream, A... args) {
+                              cudaStream_t stream, bool overlap, A... args) {
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
@@ -331,12 +332,13 @@ cudaError_t launch_overlapped(void (*kern)(K...), dim3 grid, int threads, std::s
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = overlap ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kern, static_cast<K>(args)...);
 }
 
 template <class P, int FMT>
-cudaError_t launch_tc_epi(const P& p, int sms, unsigned int* timeouts, cudaStream_t stream) {
+cudaError_t launch_tc_epi(const P& p, int sms, unsigned int* timeouts, cudaStream_t stream,
+                          bool overlap) {
   using S = EpiShape<P>;
   void (*kern)(P, unsigned int*);
   if constexpr (P::kPair)
@@ -356,7 +358,7 @@ cudaError_t launch_tc_epi(const P& p, int sms, unsigned int* timeouts, cudaStrea
   const long long groups = std::min<long long>(p.tiles_total, sms / S::kCtas);
   if (groups <= 0) return cudaSuccess;
   return launch_overlapped(kern, dim3(static_cast<unsigned>(S::kCtas * groups)), kEpiThreads,
-                           S::SMEM, stream, p, timeouts);
+                           S::SMEM, stream, overlap, p, timeouts);
 }
 
 }  // namespace mb200::tc

@@ -43,6 +43,7 @@
 #include <cstdint>
 #include <mutex>
 #include <type_traits>
+#include <utility>
 
 #include "blas/tc_epi_core.cuh"
 #include "common/device.hpp"
@@ -1355,10 +1356,11 @@ unsigned int* timeout_counter() {
 }
 
 template <typename T, int FMT, bool PAIR, int STORE>
-cudaError_t run_logits(const LogitsProblem& p, unsigned int* timeouts, cudaStream_t st) {
+cudaError_t run_logits(const LogitsProblem& p, unsigned int* timeouts, cudaStream_t st,
+                       bool overlap) {
   Logits<T, PAIR, STORE> q;
   static_cast<LogitsProblem&>(q) = p;
-  return tc::launch_tc_epi<Logits<T, PAIR, STORE>, FMT>(q, sms(), timeouts, st);
+  return tc::launch_tc_epi<Logits<T, PAIR, STORE>, FMT>(q, sms(), timeouts, st, overlap);
 }
 
 #define MB200_TRY(expr)                       \
@@ -1390,14 +1392,14 @@ cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const void* w, std::in
   g.partial = ks > 1 ? reinterpret_cast<float*>(ws + p.partial) : nullptr;
   g.scale = scale;
   g.row_scale = p.store == kCommon ? reinterpret_cast<float*>(ws + p.row_scale) : nullptr;
-  MB200_TRY((tc::launch_tc_epi<Dx<T, PAIR, TALL>, FMT>(g, sms(), to, st)));
+  MB200_TRY((tc::launch_tc_epi<Dx<T, PAIR, TALL>, FMT>(g, sms(), to, st, true)));
   if (ks > 1) {
     const bool vec = a.features % 4 == 0 && a.lddx % 4 == 0 && aligned_to(dx, 8);
     const std::int64_t work = static_cast<std::int64_t>(rows) * a.features / (vec ? 4 : 1);
     const unsigned grid =
         static_cast<unsigned>(std::min<std::int64_t>((work + 255) / 256, sms() * 32));
     MB200_TRY(tc::launch_overlapped(
-        vec ? vocab_dx_reduce_kernel<T, 4> : vocab_dx_reduce_kernel<T, 1>, dim3(grid), 256, 0, st,
+        vec ? vocab_dx_reduce_kernel<T, 4> : vocab_dx_reduce_kernel<T, 1>, dim3(grid), 256, 0, st, true,
         g.partial, ks, rows, a.features, dx, a.lddx, scale, g.row_scale));
   }
   return cudaSuccess;
@@ -1434,15 +1436,18 @@ cudaError_t run_dw(const VocabLossArgs& a, const Plan& p, const void* num, const
   g.first = piece == 0;
   g.last = piece == p.pieces - 1;
   g.scale = scale;
-  return tc::launch_tc_epi<Dw<T, TALL>, FMT>(g, sms(), to, st);
+  return tc::launch_tc_epi<Dw<T, TALL>, FMT>(g, sms(), to, st, true);
 }
 
 template <typename T, int FMT>
 cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st) {
   unsigned int* to = timeout_counter();
   if (to == nullptr) return cudaErrorInvalidDevice;
+  // the call's first kernel starts when the stream reaches it, the others overlap
+  bool overlap = false;
   const auto launch = [&](auto kern, long long ctas, int threads, auto... args) {
-    return tc::launch_overlapped(kern, dim3(static_cast<unsigned>(ctas)), threads, 0, st, args...);
+    return tc::launch_overlapped(kern, dim3(static_cast<unsigned>(ctas)), threads, 0, st,
+                                 std::exchange(overlap, true), args...);
   };
   const T* w = static_cast<const T*>(a.w);
   std::int64_t ldw = a.features;
@@ -1545,9 +1550,13 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     // enough CTAs to fill the GPU when there are few rows, each one round of 2048 words at least
     const int parts =
         std::max(1, std::min<int>(4 * sms() / rows, static_cast<int>((p.ldn + 2047) / 2048)));
+    const auto logits = [&](cudaError_t e) {
+      overlap = true;
+      return e;
+    };
     if (p.store == kNone) {
-      MB200_TRY((pair ? run_logits<T, FMT, true, kNone>(lp, to, st)
-                      : run_logits<T, FMT, false, kNone>(lp, to, st)));
+      MB200_TRY(logits(pair ? run_logits<T, FMT, true, kNone>(lp, to, st, overlap)
+                            : run_logits<T, FMT, false, kNone>(lp, to, st, overlap)));
       MB200_TRY(launch(vocab_finish_kernel<T, kNone>, rows, kFinishThreads, f));
       continue;
     }
@@ -1561,13 +1570,13 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     }
     const long long finish = static_cast<long long>(rows) * parts;
     if (p.store == kOwn) {
-      MB200_TRY((pair ? run_logits<T, FMT, true, kOwn>(lp, to, st)
-                      : run_logits<T, FMT, false, kOwn>(lp, to, st)));
+      MB200_TRY(logits(pair ? run_logits<T, FMT, true, kOwn>(lp, to, st, overlap)
+                            : run_logits<T, FMT, false, kOwn>(lp, to, st, overlap)));
       MB200_TRY(launch(vocab_finish_kernel<T, kOwn>, finish + tiles, kFinishThreads, f));
     } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
       f.row_scale = reinterpret_cast<float*>(ws + p.row_scale);
-      MB200_TRY((pair ? run_logits<T, FMT, true, kCommon>(lp, to, st)
-                      : run_logits<T, FMT, false, kCommon>(lp, to, st)));
+      MB200_TRY(logits(pair ? run_logits<T, FMT, true, kCommon>(lp, to, st, overlap)
+                            : run_logits<T, FMT, false, kCommon>(lp, to, st, overlap)));
       MB200_TRY(launch(vocab_finish_kernel<T, kCommon>, finish, kFinishThreads, f));
     }
 
