@@ -27,11 +27,11 @@
 // reads of the operands (timed without them), hence the wide tiles and the banded order.
 //
 // Precision: products of the 16-bit inputs accumulate in fp32; maxima, sums, target
-// logits and losses are fp32.  The numerators are rounded to 16 bits in step 1 and again
-// in step 2 (dz is a 16-bit operand of the tensor cores either way; keeping fp32
-// numerators would double the piece's traffic).  The target words, whose p - q cancels,
-// are recomputed in step 2 from their fp32 logits and rounded once.  dx and dw round once
-// more at the end.
+// logits and losses are fp32.  dz is a 16-bit operand of the tensor cores and rounds once;
+// the 16 bits that carry the numerators to step 2 hold 2 more significant bits than dz
+// (OwnCode; fp32 numerators would double the piece's traffic).  The target words, whose
+// p - q cancels, are recomputed in step 2 from their fp32 logits and rounded once.  dx and
+// dw round once more at the end.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -91,6 +91,35 @@ __device__ __forceinline__ float2 unpack2(std::uint32_t v) {
     return __half22float2(*reinterpret_cast<const __half2*>(&v));
   else
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+
+// kOwn's numerators (0 to 1, relative to their unit's largest) become dz's 16 bits in the
+// finish.  They hold more bits than dz, or the gradients would show a third rounding beside
+// dz's and their own.  They are fp32's bits, rounded and without the sign and the exponent's
+// top: for bf16 7 exponent and 9 mantissa bits (10 significant bits over fp32's range below
+// 1), for fp16 4 and 12 (13 bits down to 2^-14, steps of 2^-26 below).  NaN spoils its
+// neighbour's code, but a NaN's whole row is NaN.
+template <typename T>
+struct OwnCode {
+  static constexpr bool kHalf = std::is_same_v<T, __half>;
+  static constexpr float kDown = kHalf ? 0x1p-112f : 1.0f;  // brings 1's exponent below 2^4
+  static constexpr int kShift = kHalf ? 11 : 14;
+};
+
+template <typename T>
+__device__ __forceinline__ std::uint32_t pack_own(float a, float b) {
+  using Code = OwnCode<T>;
+  const std::uint32_t lo = __float_as_uint(a * Code::kDown) + (1u << (Code::kShift - 1));
+  const std::uint32_t hi = __float_as_uint(b * Code::kDown) + (1u << (Code::kShift - 1));
+  // (nvcc 12.9 drops the upper half where this is written as a shift, a mask and an or)
+  return __byte_perm(lo >> Code::kShift, hi >> Code::kShift, 0x5410);
+}
+
+template <typename T>
+__device__ __forceinline__ float2 unpack_own(std::uint32_t v) {
+  using Code = OwnCode<T>;
+  return make_float2(__uint_as_float((v & 0xffffu) << Code::kShift) * (1.0f / Code::kDown),
+                     __uint_as_float(v >> 16 << Code::kShift) * (1.0f / Code::kDown));
 }
 
 template <typename T>
@@ -294,8 +323,12 @@ __device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& 
     }
     if constexpr (STORE != kNone) {
       std::uint8_t* box = stage + (g >> 3) * 4096 + lane * 128 + (((g & 7) ^ (lane & 7)) << 4);
-      *reinterpret_cast<uint4*>(box) = make_uint4(pack2<T>(e[0], e[1]), pack2<T>(e[2], e[3]),
-                                                  pack2<T>(e[4], e[5]), pack2<T>(e[6], e[7]));
+      std::uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[j] = STORE == kOwn ? pack_own<T>(e[2 * j], e[2 * j + 1])
+                             : pack2<T>(e[2 * j], e[2 * j + 1]);
+      *reinterpret_cast<uint4*>(box) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
   if (row < p.rows)
@@ -756,13 +789,13 @@ __device__ __forceinline__ void transpose_tile(const TransposeArgs& a, const Tar
   }
 }
 
-// Eight 16-bit values times f.
-template <typename T>
+// Eight numerators times f, in T.
+template <typename T, int STORE>
 __device__ __forceinline__ uint4 scaled(uint4 u, float f) {
   std::uint32_t* w = reinterpret_cast<std::uint32_t*>(&u);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float2 v = unpack2<T>(w[j]);
+    const float2 v = STORE == kOwn ? unpack_own<T>(w[j]) : unpack2<T>(w[j]);
     w[j] = pack2<T>(f * v.x, f * v.y);
   }
   return u;
@@ -854,7 +887,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
         if (st[u].y == 0.0f || move == 0.0f) continue;
         const float f = exp2f(move);
         const std::int64_t c = static_cast<std::int64_t>(u) * per_unit + (threadIdx.x & 31);
-        if ((threadIdx.x & 31) < per_unit && c < c_end) num[c] = scaled<T>(num[c], f);
+        if ((threadIdx.x & 31) < per_unit && c < c_end) num[c] = scaled<T, STORE>(num[c], f);
       }
     } else {
       const auto factor = [&](std::int64_t c) {
@@ -867,9 +900,9 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
         for (int j = 0; j < 4; ++j) u[j] = num[c + j * kFinishThreads];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          num[c + j * kFinishThreads] = scaled<T>(u[j], factor(c + j * kFinishThreads));
+          num[c + j * kFinishThreads] = scaled<T, STORE>(u[j], factor(c + j * kFinishThreads));
       }
-      for (; c < c_end; c += kFinishThreads) num[c] = scaled<T>(num[c], factor(c));
+      for (; c < c_end; c += kFinishThreads) num[c] = scaled<T, STORE>(num[c], factor(c));
     }
     // the targets, in the numerators' units: dz, or dz / row_scale
     const float t = STORE == kCommon ? exp2f((mx - base) + log_sum) : g;
