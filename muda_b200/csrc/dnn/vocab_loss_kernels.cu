@@ -21,7 +21,7 @@
 // at H = 4096; keeping 16 bits of it costs 6 bytes of traffic, under 1 us.  The piece bounds
 // them to 2 GiB whatever T and V are.
 //
-// What bounds a training step of 8192 x 4096 x 131072 (19.7 ms, 1340 TFLOP/s): the power
+// What bounds a training step of 8192 x 4096 x 131072 (20.1 ms, 1313 TFLOP/s): the power
 // cap.  The tensor pipe is busy 95 % of the cycles at 1.15-1.4 GHz.  Of a 1546 us score of
 // 2048 x 4096 x 131072 under the cap, 100 us go with the DRAM reads and 155 us with the L2
 // reads of the operands (timed without them), hence the wide tiles and the banded order.
@@ -98,7 +98,9 @@ __device__ __forceinline__ float2 unpack2(std::uint32_t v) {
 // dz's and their own.  They are fp32's bits, rounded and without the sign and the exponent's
 // top: for bf16 7 exponent and 9 mantissa bits (10 significant bits over fp32's range below
 // 1), for fp16 4 and 12 (13 bits down to 2^-14, steps of 2^-26 below).  NaN spoils its
-// neighbour's code, but a NaN's whole row is NaN.
+// neighbour's code, but a NaN's whole row is NaN.  Against numerators in dz's own type:
+// dw's rows of words that are no target 1.01 instead of 1.13 times the error of two
+// roundings, steps 0.5-2 % slower (2048 x 2048 x 32000: 672 -> 679 us).
 template <typename T>
 struct OwnCode {
   static constexpr bool kHalf = std::is_same_v<T, __half>;
