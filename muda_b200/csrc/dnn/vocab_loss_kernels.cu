@@ -928,8 +928,10 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
 }
 
 // dst[r][c] = src[r][c] into rows of ldd elements (a multiple of 64): operands whose rows
-// TMA cannot read in place, or that start off a line.  A thread moves 8 elements: five
-// aligned words around them, shifted by half a word where the row is odd.
+// TMA cannot read in place, or that start off a line.  A thread moves 8 elements: the
+// aligned words around them, shifted by half a word where the row is odd.  There the first
+// word also holds the element before them (never src's first chunk, see below); of the fifth
+// only the half that is theirs is read, the other may lie past src's end.
 template <typename T>
 __global__ void __launch_bounds__(256)
     vocab_pack_kernel(const T* __restrict__ src, std::int64_t lds, std::int64_t rows, int cols,
@@ -954,7 +956,7 @@ __global__ void __launch_bounds__(256)
     std::uint32_t v[5];
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = w[j];
-    v[4] = shift != 0 ? w[4] : 0u;
+    v[4] = shift != 0 ? *reinterpret_cast<const std::uint16_t*>(s + 7) : 0u;
     *reinterpret_cast<uint4*>(d) =
         make_uint4(__funnelshift_r(v[0], v[1], shift), __funnelshift_r(v[1], v[2], shift),
                    __funnelshift_r(v[2], v[3], shift), __funnelshift_r(v[3], v[4], shift));
