@@ -40,8 +40,10 @@
 // `row` is the row in the tile, `half` the column half, taddr the half's first column.  A
 // tall tile calls chunk() twice, for its upper and then its lower 256 rows.
 // Waits are bounded as in tc_gemm_core.cuh: a wait that runs out marks its CTA aborted,
-// counts the event, and every role leaves its loop; all threads (of both CTAs) then meet at
-// a final barrier, so no CTA leaves while the other may still reach its memory.
+// counts the event, and every role leaves its loop, whole warps at a time (the warp votes on
+// its clocks and on the mark: tcgen05.ld and the stores need it together); all threads (of
+// both CTAs) then meet at a final barrier, so no CTA leaves while the other may still reach
+// its memory.
 #pragma once
 
 #include "blas/tc_gemm_core.cuh"
@@ -131,6 +133,8 @@ __device__ __forceinline__ void epi_body(const P& p, unsigned int* timeouts) {
     *aborted = 1;
     atomicAdd(timeouts, 1u);
   };
+  // a whole warp leaves or stays: its lanes could read the flag, or the clock, differently
+  auto stopped = [&]() { return __any_sync(0xffffffffu, *aborted != 0) != 0; };
 
   if (warp == 0) {
     // ---------------- TMA producer of this CTA's rows
@@ -141,7 +145,7 @@ __device__ __forceinline__ void epi_body(const P& p, unsigned int* timeouts) {
     std::uint32_t phase = 0;
     std::uint32_t issued = 0, issued_phase = 0;  // bit per stage
     bool ok = true;
-    for (long long t = first_tile; ok && t < p.tiles_total && !*aborted; t += step) {
+    for (long long t = first_tile; ok && t < p.tiles_total && !stopped(); t += step) {
       int c[3];
       p.coords(t, c);
       int k = p.k_begin(c) * kBK;
@@ -198,7 +202,7 @@ __device__ __forceinline__ void epi_body(const P& p, unsigned int* timeouts) {
       int acc = 0;
       std::uint32_t acc_phase = 0;
       bool ok = true;
-      for (long long t = first_tile; ok && t < p.tiles_total && !*aborted; t += step) {
+      for (long long t = first_tile; ok && t < p.tiles_total && !stopped(); t += step) {
         for (int kb = 0; kb < num_kb; ++kb) {
           const bool first = CK == 0 ? kb == 0 : kb % (CK == 0 ? 1 : CK) == 0;
           const bool last = kb == num_kb - 1 || (CK != 0 && kb % (CK == 0 ? 1 : CK) == CK - 1);
@@ -260,14 +264,14 @@ __device__ __forceinline__ void epi_body(const P& p, unsigned int* timeouts) {
     int acc = 0;
     std::uint32_t acc_phase = 0;
     bool ok = true;
-    for (long long t = first_tile; ok && t < p.tiles_total && !*aborted; t += step) {
+    for (long long t = first_tile; ok && t < p.tiles_total && !stopped(); t += step) {
       int c[3];
       p.coords(t, c);
       typename P::Tile tile;
       p.begin(tile, c, row, half);
       for (int ch = 0; ch < chunks; ++ch) {
-        if (!mbar_wait_idle(&acc_full[acc], acc_phase)) {
-          fail();
+        if (!mbar_wait_warp_idle(&acc_full[acc], acc_phase)) {
+          if (lane == 0) fail();
           ok = false;
           break;
         }

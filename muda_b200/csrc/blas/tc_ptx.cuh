@@ -353,14 +353,14 @@ __device__ __forceinline__ bool mbar_wait_warp(std::uint64_t* bar, std::uint32_t
   }
 }
 
-// mbar_wait that naps between polls: for long waits whose end need not be seen at once
+// mbar_wait_warp that naps between polls: for long waits whose end need not be seen at once
 // (eight epilogue warps polling through a tile cost 2-3 % of a power-limited product).
-__device__ __forceinline__ bool mbar_wait_idle(std::uint64_t* bar, std::uint32_t parity) {
-  if (mbar_try_wait(bar, parity)) return true;
+__device__ __forceinline__ bool mbar_wait_warp_idle(std::uint64_t* bar, std::uint32_t parity) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   const std::uint64_t t0 = global_ns();
-  while (!mbar_try_wait(bar, parity)) {
+  while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
     __nanosleep(100);
-    if (global_ns() - t0 > kWaitLimitNs) return false;
+    if (__any_sync(0xffffffffu, global_ns() - t0 > kWaitLimitNs)) return false;
   }
   return true;
 }
