@@ -280,6 +280,9 @@ cudnnStatus_t cudnnBatchNormalizationForwardTraining(
  * most 2 GiB for 16-bit numerators of a piece of the tokens, plus V*H floats when T
  * needs several pieces).  A workspace given (aligned to 256 bytes) bounds the memory
  * instead: smaller ones mean smaller pieces, down to 128 tokens; BAD_PARAM below that.
+ * Calls on a handle wait for its workspace across streams.  Under stream capture null takes an
+ * allocation of the graph's own instead (a memory node, with CUDA's limits on such graphs), so
+ * replays share nothing with the handle; a workspace given is the caller's to keep and order.
  */
 cudnnStatus_t cudnnGetLinearCrossEntropyWorkspaceSize(cudnnHandle_t handle,
                                                       cudnnTensorDescriptor_t xDesc,

@@ -224,6 +224,49 @@ cudaStream_t stream_of(DnnContext& h) {
   return h.stream;
 }
 
+// Runs fn(workspace) with `need` bytes.  Outside stream capture they are the handle's buffer,
+// ordered after the previous call that used it.  A captured call takes an allocation of its
+// graph's own: the handle's buffer would be shared with replays that its event does not order,
+// and freed under them when a later call needs more.  `optional`: fn(null) when the handle's
+// buffer cannot grow.
+template <class Fn>
+cudnnStatus_t with_workspace(DnnContext& h, std::size_t need, cudaStream_t st, bool optional,
+                             Fn&& fn) {
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &cap) != cudaSuccess) cap = cudaStreamCaptureStatusNone;
+  if (cap != cudaStreamCaptureStatusNone) {
+    void* p = nullptr;
+    if (cudaMallocAsync(&p, need, st) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return CUDNN_STATUS_ALLOC_FAILED;  // the capture may be lost: nothing more goes into it
+    }
+    const cudaError_t e = fn(p);
+    const cudaError_t f = cudaFreeAsync(p, st);
+    return e == cudaSuccess && f == cudaSuccess ? CUDNN_STATUS_SUCCESS
+                                                : CUDNN_STATUS_EXECUTION_FAILED;
+  }
+  std::lock_guard<std::mutex> lk(h.ws_mu);
+  const int dev = mb200::current_device();
+  if (!h.ws || h.ws->bytes < need || h.ws->device != dev) {
+    h.ws.reset();
+    h.ws = mb200::DeviceBuffer::make(need);
+    if (!h.ws) {
+      if (!optional) return CUDNN_STATUS_ALLOC_FAILED;
+      return fn(nullptr) == cudaSuccess ? CUDNN_STATUS_SUCCESS : CUDNN_STATUS_EXECUTION_FAILED;
+    }
+  }
+  if (h.ws_done != nullptr && cudaStreamWaitEvent(st, h.ws_done, 0) != cudaSuccess)
+    return CUDNN_STATUS_EXECUTION_FAILED;
+  if (fn(h.ws->ptr) != cudaSuccess) return CUDNN_STATUS_EXECUTION_FAILED;
+  if (h.ws_done == nullptr &&
+      cudaEventCreateWithFlags(&h.ws_done, cudaEventDisableTiming) != cudaSuccess) {
+    h.ws_done = nullptr;
+    return CUDNN_STATUS_EXECUTION_FAILED;
+  }
+  return cudaEventRecord(h.ws_done, st) == cudaSuccess ? CUDNN_STATUS_SUCCESS
+                                                       : CUDNN_STATUS_EXECUTION_FAILED;
+}
+
 }  // namespace
 
 extern "C" {
@@ -567,30 +610,9 @@ cudnnStatus_t cudnnConvolutionForward(cudnnHandle_t handle, const void* alpha,
         mb200::dnn::launch_conv(x, w, y, plan.shape, dt, a, b, workSpace, need, st);
     return e == cudaSuccess ? CUDNN_STATUS_SUCCESS : CUDNN_STATUS_EXECUTION_FAILED;
   }
-  std::lock_guard<std::mutex> lk(h->ws_mu);
-  const int dev = mb200::current_device();
-  if (!h->ws || h->ws->bytes < need || h->ws->device != dev) {
-    h->ws.reset();
-    h->ws = mb200::DeviceBuffer::make(need);
-  }
-  void* wsp = h->ws ? h->ws->ptr : nullptr;
-  const std::size_t wsb = h->ws ? h->ws->bytes : 0;
-  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(st, &cap) != cudaSuccess) cap = cudaStreamCaptureStatusNone;
-  const bool ordered = cap == cudaStreamCaptureStatusNone && wsp != nullptr;
-  if (ordered && h->ws_done != nullptr && cudaStreamWaitEvent(st, h->ws_done, 0) != cudaSuccess)
-    return CUDNN_STATUS_EXECUTION_FAILED;
-  const cudaError_t e = mb200::dnn::launch_conv(x, w, y, plan.shape, dt, a, b, wsp, wsb, st);
-  if (e != cudaSuccess) return CUDNN_STATUS_EXECUTION_FAILED;
-  if (ordered) {
-    if (h->ws_done == nullptr &&
-        cudaEventCreateWithFlags(&h->ws_done, cudaEventDisableTiming) != cudaSuccess) {
-      h->ws_done = nullptr;
-      return CUDNN_STATUS_EXECUTION_FAILED;
-    }
-    if (cudaEventRecord(h->ws_done, st) != cudaSuccess) return CUDNN_STATUS_EXECUTION_FAILED;
-  }
-  return CUDNN_STATUS_SUCCESS;
+  return with_workspace(*h, need, st, true, [&](void* ws) {
+    return mb200::dnn::launch_conv(x, w, y, plan.shape, dt, a, b, ws, ws != nullptr ? need : 0, st);
+  });
 }
 
 // ---------------------------------------------------------------- softmax --
@@ -777,34 +799,6 @@ bool spans_ok(std::initializer_list<std::pair<const void*, std::size_t>> spans) 
   return true;
 }
 
-// Runs fn(workspace) with `need` bytes of the handle's workspace, ordered after the
-// previous call that used it (the same protocol as the forward convolution).
-template <class Fn>
-cudnnStatus_t with_workspace(DnnContext& h, std::size_t need, cudaStream_t st, Fn&& fn) {
-  std::lock_guard<std::mutex> lk(h.ws_mu);
-  const int dev = mb200::current_device();
-  if (!h.ws || h.ws->bytes < need || h.ws->device != dev) {
-    h.ws.reset();
-    h.ws = mb200::DeviceBuffer::make(need);
-    if (!h.ws) return CUDNN_STATUS_ALLOC_FAILED;
-  }
-  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(st, &cap) != cudaSuccess) cap = cudaStreamCaptureStatusNone;
-  const bool ordered = cap == cudaStreamCaptureStatusNone;
-  if (ordered && h.ws_done != nullptr && cudaStreamWaitEvent(st, h.ws_done, 0) != cudaSuccess)
-    return CUDNN_STATUS_EXECUTION_FAILED;
-  if (fn(h.ws->ptr) != cudaSuccess) return CUDNN_STATUS_EXECUTION_FAILED;
-  if (ordered) {
-    if (h.ws_done == nullptr &&
-        cudaEventCreateWithFlags(&h.ws_done, cudaEventDisableTiming) != cudaSuccess) {
-      h.ws_done = nullptr;
-      return CUDNN_STATUS_EXECUTION_FAILED;
-    }
-    if (cudaEventRecord(h.ws_done, st) != cudaSuccess) return CUDNN_STATUS_EXECUTION_FAILED;
-  }
-  return CUDNN_STATUS_SUCCESS;
-}
-
 cudnnStatus_t status_of(cudaError_t e) {
   return e == cudaSuccess ? CUDNN_STATUS_SUCCESS : CUDNN_STATUS_EXECUTION_FAILED;
 }
@@ -845,7 +839,7 @@ cudnnStatus_t cudnnConvolutionBackwardData(cudnnHandle_t handle, const void* alp
   auto* dxp = static_cast<float*>(dx);
   const std::size_t need = mb200::dnn::conv_bwd_data_tc_workspace(plan.shape);
   if (need > 0) {
-    return with_workspace(*h, need, st, [&](void* ws) {
+    return with_workspace(*h, need, st, false, [&](void* ws) {
       const cudaError_t e =
           mb200::dnn::launch_conv_bwd_data_tc(wp, dyp, dxp, plan.shape, a, b, ws, need, st);
       return e == cudaErrorNotSupported
@@ -885,7 +879,7 @@ cudnnStatus_t cudnnConvolutionBackwardFilter(cudnnHandle_t handle, const void* a
   const cudaStream_t st = stream_of(*h);
   const std::size_t tc_need = mb200::dnn::conv_bwd_filter_tc_workspace(plan.shape);
   const std::size_t simt_need = mb200::dnn::conv_bwd_filter_workspace(plan.shape);
-  return with_workspace(*h, std::max(tc_need, simt_need), st, [&](void* ws) {
+  return with_workspace(*h, std::max(tc_need, simt_need), st, false, [&](void* ws) {
     const auto* xp = static_cast<const float*>(x);
     const auto* dyp = static_cast<const float*>(dy);
     auto* dwp = static_cast<float*>(dw);
@@ -1091,7 +1085,7 @@ cudnnStatus_t cudnnBatchNormalizationForwardTraining(
   };
   const std::size_t need = mb200::dnn::bn_training_workspace(xs.v);
   if (need == 0) return status_of(run(nullptr));
-  return with_workspace(*h, need, st, run);
+  return with_workspace(*h, need, st, false, run);
 }
 
 }  // extern "C"
@@ -1222,7 +1216,7 @@ cudnnStatus_t vocab_run(DnnContext& h, const VocabLossArgs& a, void* workSpace,
     return status_of(mb200::dnn::launch_vocab_loss(a, workSpace, workSpaceSize, st));
   }
   const std::size_t need = mb200::dnn::vocab_loss_workspace(a);
-  return with_workspace(h, need, st, [&](void* p) {
+  return with_workspace(h, need, st, false, [&](void* p) {
     return mb200::dnn::launch_vocab_loss(a, p, need, st);
   });
 }
