@@ -4,9 +4,9 @@
 // The T x V logits z = x w^T / tau never exist in memory as such.  A call runs over
 // pieces of tokens; in each piece
 //   1. Logits walks tiles of z.  The fp32 tile stays in tensor memory and registers; the
-//      epilogue reduces each token's 128 words (a unit) to one (reference, sum) pair, lse's
+//      epilogue reduces each token's 128 words (a unit) to one (maximum, sum) pair, lse's
 //      running maximum and sum, and picks the target words' logits.  With gradients it also
-//      writes the unit's numerators 2^(z2 - reference) in 16 bits;
+//      writes the unit's numerators 2^(z2 - the maximum's) in 16 bits;
 //   2. vocab_finish_kernel joins a token's pairs into its log-sum-exp and loss, and turns
 //      the numerators in place into dz = dloss / tau * (p - q).  Without dw (a frozen head)
 //      bf16 numerators share a power-of-two reference per token instead, and the token's
@@ -14,7 +14,10 @@
 //   3. Dx and Dw multiply dx = dz w and dw = dz^T x.
 // All three products run on the loop of tc_epi_core.cuh.  Scores of up to 8 tokens take
 // vocab_stream_kernel instead of 1.  Exponents are in powers of two: z2 = z * log2(e), with
-// log2(e) / tau folded into one multiply, so that 2^(z2 - reference) is one fma and one ex2.
+// log2(e) / tau folded into one multiply.  The pairs keep the maximum of x w as it is, and
+// differences are taken before they are scaled: a scaled maximum, rounded, may be off by more
+// than the exponentials have room for (half a unit in its last place: 1 at |z2| = 2^24), and
+// that of words masked with the type's lowest value overflows.
 //
 // Why the numerators are kept at all: the gradient needs each logit twice, before and after
 // lse is known.  Computing the product again costs 2 H flops per logit, 5 us per 10^6 logits
@@ -97,9 +100,9 @@ __device__ __forceinline__ float2 unpack2(std::uint32_t v) {
 // finish.  They hold more bits than dz, or the gradients would show a third rounding beside
 // dz's and their own.  They are fp32's bits, rounded and without the sign and the exponent's
 // top: for bf16 7 exponent and 9 mantissa bits (10 significant bits over fp32's range below
-// 1), for fp16 4 and 12 (13 bits down to 2^-14, steps of 2^-26 below).  NaN spoils its
-// neighbour's code, but a NaN's whole row is NaN.  Against numerators in dz's own type:
-// dw's rows of words that are no target 1.01 instead of 1.13 times the error of two
+// 1), for fp16 4 and 12 (13 bits down to 2^-14, steps of 2^-26 below).  NaN does not survive
+// the code, but its unit's sum is NaN and makes the whole row NaN.  Against numerators in dz's
+// own type: dw's rows of words that are no target 1.01 instead of 1.13 times the error of two
 // roundings, steps 0.5-2 % slower (2048 x 2048 x 32000: 672 -> 679 us).
 template <typename T>
 struct OwnCode {
@@ -175,7 +178,7 @@ __device__ __forceinline__ int target_count(const Targets& t, int row, int vocab
 
 // ------------------------------------------------------------------ logits kernels --
 // Most words of an epilogue thread's share of a tile row, its "unit" of one
-// (reference, sum) pair.
+// (maximum, sum) pair.
 constexpr int kUnit = 128;
 
 // k-blocks per accumulator.  Tensor-core accumulation truncates: one chain of 256 MMAs
@@ -202,7 +205,7 @@ struct LogitsProblem {
   int band;           // tile rows that stay in L2 while w streams past
   int unit, units;    // words per unit (tile_n / 2), units per row
   float scale;        // log2(e) / tau
-  float2* stats;      // [row][units] (reference, sum of 2^(z2 - reference))
+  float2* stats;      // [row][units] (maximum of x w, sum of 2^(z2 - the maximum's))
   std::int64_t ldn;
   Targets targets;
 
@@ -255,11 +258,24 @@ __device__ __forceinline__ void pick_targets(const LogitsProblem& p, const Logit
 
 // What a unit leaves behind besides its pair: nothing, numerators relative to its own
 // maximum (kOwn), or numerators relative to 2^0 (kCommon, bf16: its exponents reach as far as
-// fp32's).  kCommon takes whole references, so that moving numerators from one to another is
-// exact; units beyond 2^+-64 keep their own until the finish has seen the row's maximum.
+// fp32's).  Units beyond 2^+-64 keep a reference of their own until the finish has seen the
+// row's maximum: the nearest whole exponent, so that moving numerators from one to another is
+// exact, or the maximum itself where fp32 holds no fraction of the exponent any more.
 // Loss and dx of 4096 x 2048 x 65536: 1768 us with kOwn, 1657 with kCommon.
 enum StoreMode { kNone = 0, kOwn = 1, kCommon = 2 };
-constexpr float kCommonReach = 64.0f;
+constexpr float kCommonReach = 64.0f, kWholeReach = 0x1p22f;
+
+// kCommon's numerators of a unit with this maximum are 2^(z2 - top * scale - whole).
+struct Reference {
+  float top, whole;
+};
+
+__device__ __forceinline__ Reference reference(float top, float scale) {
+  const float whole = rintf(__fmul_rn(top, scale));
+  if (fabsf(whole) <= kCommonReach) return {0.0f, 0.0f};
+  if (fabsf(whole) <= kWholeReach) return {0.0f, whole};
+  return {top, 0.0f};
+}
 
 // Adds a finished accumulator's columns of the unit (taddr: this thread's lane).
 __device__ __forceinline__ void add_chunk(LogitsTile& t, int unit, std::uint32_t taddr,
@@ -296,13 +312,13 @@ __device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& 
   float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int j = 0; j < kUnit; ++j) m[j & 3] = fmaxf(m[j & 3], t.v[j]);
-  const float mx = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+  float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
   // a row of -inf (or NaN) has no finite maximum: 0 keeps -inf's numerators at 0
-  float ref = mx == -INFINITY ? 0.0f : __fmul_rn(mx, p.scale);
+  if (top == -INFINITY) top = 0.0f;
   float shift = 1.0f;
   if constexpr (STORE == kCommon) {
-    ref = rintf(ref);
-    if (fabsf(ref) <= kCommonReach) shift = __int_as_float((static_cast<int>(ref) + 127) << 23);
+    const Reference ref = reference(top, p.scale);
+    shift = exp2_approx(fmaf(top - ref.top, p.scale, -ref.whole));
   }
   pick_targets(p, t, row, n0, cols);
   if constexpr (STORE != kNone) {
@@ -316,7 +332,7 @@ __device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& 
     float e[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      e[j] = exp2_approx(fmaf(t.v[g * 8 + j], p.scale, -ref));
+      e[j] = exp2_approx(__fmul_rn(__fsub_rn(t.v[g * 8 + j], top), p.scale));
       s[j & 3] += e[j];
     }
     if constexpr (STORE == kCommon) {
@@ -333,9 +349,10 @@ __device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& 
       *reinterpret_cast<uint4*>(box) = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
-  if (row < p.rows)
+  if (row < p.rows) {
     p.stats[static_cast<std::int64_t>(row) * p.units + n0 / p.unit] =
-        make_float2(ref, (s[0] + s[1]) + (s[2] + s[3]));
+        make_float2(top, (s[0] + s[1]) + (s[2] + s[3]));
+  }
   if constexpr (STORE != kNone) {
     tc::fence_proxy_async_smem();
     __syncwarp();
@@ -443,8 +460,8 @@ __device__ __forceinline__ void mma_16x8x16(float (&d)[4], std::uint32_t a0, std
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// (m, s) joined with (m2, s2): s counts 2^(z2 - m); s == 0 is an empty pair.
-__device__ __forceinline__ void join_pair(float& m, float& s, float m2, float s2) {
+// (m, s) joined with (m2, s2): s counts 2^((x w - m) scale); s == 0 is an empty pair.
+__device__ __forceinline__ void join_pair(float& m, float& s, float m2, float s2, float scale) {
   if (s2 == 0.0f) return;
   if (s == 0.0f) {
     m = m2;
@@ -452,7 +469,7 @@ __device__ __forceinline__ void join_pair(float& m, float& s, float m2, float s2
     return;
   }
   const float top = fmaxf(m, m2);
-  s = s * exp2_approx(m - top) + s2 * exp2_approx(m2 - top);
+  s = s * exp2_approx((m - top) * scale) + s2 * exp2_approx((m2 - top) * scale);
   m = top;
 }
 
@@ -529,9 +546,9 @@ __global__ void __launch_bounds__(kStreamThreads, 1) vocab_stream_kernel(const S
       if (label[j] == w0 + 8) a.targets.z[2 * t + j] = z[j + 2];
       const float top = fmaxf(z[j], z[j + 2]);
       // -inf adds nothing; NaN has to (fmaxf passes over it)
-      const float ref = top == -INFINITY ? 0.0f : __fmul_rn(top, a.scale);
-      join_pair(m[j], s[j], ref, exp2_approx(fmaf(z[j], a.scale, -ref)) +
-                                     exp2_approx(fmaf(z[j + 2], a.scale, -ref)));
+      const float base = top == -INFINITY ? 0.0f : top;
+      join_pair(m[j], s[j], base, exp2_approx((z[j] - base) * a.scale) +
+                                      exp2_approx((z[j + 2] - base) * a.scale), a.scale);
     }
     if (a.targets.top_k > 0) {
       unsigned rows = __ballot_sync(0xffffffffu, hint != 0u);
@@ -562,7 +579,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) vocab_stream_kernel(const S
     for (int o = 4; o < 32; o <<= 1) {
       const float m2 = __shfl_xor_sync(0xffffffffu, m[j], o);
       const float s2 = __shfl_xor_sync(0xffffffffu, s[j], o);
-      join_pair(m[j], s[j], m2, s2);
+      join_pair(m[j], s[j], m2, s2, a.scale);
     }
     if (g == 0) joined[warp][2 * t + j] = make_float2(m[j], s[j]);
   }
@@ -571,7 +588,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) vocab_stream_kernel(const S
   if (row < a.rows) {
     float2 p = joined[0][row];
     for (int i = 1; i < kStreamThreads / 32; ++i)
-      join_pair(p.x, p.y, joined[i][row].x, joined[i][row].y);
+      join_pair(p.x, p.y, joined[i][row].x, joined[i][row].y, a.scale);
     a.stats[static_cast<std::int64_t>(row) * gridDim.x + blockIdx.x] = p;
   }
 }
@@ -848,15 +865,14 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
   mx = block_reduce(mx, true, red);
   float sum = 0.0f;
   for (int i = threadIdx.x; i < a.units; i += kFinishThreads)
-    if (st[i].y != 0.0f) sum += st[i].y * exp2f(st[i].x - mx);
+    if (st[i].y != 0.0f) sum += st[i].y * exp2f((st[i].x - mx) * a.log2e_tau);
   sum = block_reduce(sum, false, red);
   const float log_sum = log2f(sum);
-  const float lse2 = mx + log_sum;
 
   const int tk = max(a.targets.top_k, 1);
   const std::int64_t r0 = static_cast<std::int64_t>(row) * tk;
-  // a target's z2 - mx in one rounding: a confident word's loss is far below z2's last bit
-  const auto above = [&](std::int64_t i) { return fmaf(a.targets.z[i], a.log2e_tau, -mx); };
+  // a target's z2 above the maximum's: a confident word's loss is far below z2's last bit
+  const auto above = [&](std::int64_t i) { return (a.targets.z[i] - mx) * a.log2e_tau; };
   if (part == 0) {
     float loss;
     if (n < 0) {
@@ -872,20 +888,21 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     }
     if (threadIdx.x == 0) {
       if (a.loss != nullptr) a.loss[row] = loss;
-      if (a.lse != nullptr) a.lse[row] = lse2 * kLn2;
+      if (a.lse != nullptr) a.lse[row] = fmaf(mx, a.inv_tau, log_sum * kLn2);
     }
   }
   if constexpr (STORE != kNone) {
     float g = n < 0 ? NAN : a.dloss[row] * a.inv_tau;
     if (a.scale != nullptr) g *= a.scale[0];
-    float base = 0.0f;  // kCommon: the row's reference
+    float down = 0.0f;  // kCommon: the row's reference below its maximum, in z2
     if constexpr (STORE == kCommon) {
-      if (fabsf(mx) > kCommonReach) base = mx;
-      if (part == 0 && threadIdx.x == 0)
-        a.row_scale[row] = g * exp2f((base - mx) - log_sum);
+      const Reference base = reference(mx, a.log2e_tau);
+      down = fmaf(base.top - mx, a.log2e_tau, base.whole);
+      if (part == 0 && threadIdx.x == 0) a.row_scale[row] = g * exp2f(down - log_sum);
       // only units whose reference is not the row's: rare
       for (int u = u_begin + (threadIdx.x >> 5); u < u_end; u += kFinishThreads / 32) {
-        const float move = (fabsf(st[u].x) > kCommonReach ? st[u].x : 0.0f) - base;
+        const Reference ref = reference(st[u].x, a.log2e_tau);
+        const float move = fmaf(ref.top - base.top, a.log2e_tau, ref.whole - base.whole);
         if (st[u].y == 0.0f || move == 0.0f) continue;
         const float f = exp2f(move);
         const std::int64_t c = static_cast<std::int64_t>(u) * per_unit + (threadIdx.x & 31);
@@ -893,7 +910,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
       }
     } else {
       const auto factor = [&](std::int64_t c) {
-        return g * exp2f((st[c / per_unit].x - mx) - log_sum);
+        return g * exp2f(fmaf(st[c / per_unit].x - mx, a.log2e_tau, -log_sum));
       };
       std::int64_t c = c_begin + threadIdx.x;
       for (; c + 3 * kFinishThreads < c_end; c += 4 * kFinishThreads) {
@@ -907,7 +924,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
       for (; c < c_end; c += kFinishThreads) num[c] = scaled<T, STORE>(num[c], factor(c));
     }
     // the targets, in the numerators' units: dz, or dz / row_scale
-    const float t = STORE == kCommon ? exp2f((mx - base) + log_sum) : g;
+    const float t = STORE == kCommon ? exp2f(log_sum - down) : g;
     __syncthreads();
     T* d = static_cast<T*>(a.num) + row * a.ldn;
     if (a.targets.top_k == 0) {

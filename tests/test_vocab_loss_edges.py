@@ -69,3 +69,172 @@ def test_graph_beside_other_calls_of_the_handle(cuda, built, K, own):
         assert cuda.equal(getattr(small, n), t), n
     del graph
     cuda.cuda.synchronize()
+
+
+def _definition(torch, h):
+    """As Head.definition, of logits below their row's largest: lse less z cancels in 64 bits
+    too where the logits are huge."""
+    w = h.w.double()
+    T, V = h.x.shape[0], w.shape[0]
+    target = torch.zeros(T, V, device="cuda", dtype=torch.float64)
+    entropy = torch.zeros(T, device="cuda", dtype=torch.float64)
+    if h.K:
+        t = torch.where(h.index >= 0, h.teacher.double() / h.tau, -math.inf)
+        live = (t > -math.inf).any(dim=1)
+        q = torch.softmax(t[live], dim=1)
+        target[live] = target[live].scatter_add(1, h.index[live].clamp(min=0), q)
+        entropy[live] = torch.special.xlogy(q, q).sum(dim=1)
+    else:
+        live = h.labels >= 0
+        target[live, h.labels[live]] = 1.0
+    x = torch.where(live[:, None], h.x.double(), 0.0)
+    z = x @ w.t()
+    top = z.amax(dim=1, keepdim=True)
+    z = (z - top) / h.tau
+    total = torch.logsumexp(z, dim=1, keepdim=True)
+    cross = torch.where(target > 0, target * (total - z), 0.0).sum(dim=1)
+    p = torch.exp(z - total)
+    dloss = torch.where(live, h.dloss.double(), 0.0) / h.tau
+    dz = dloss[:, None] * (p - target)
+    return dict(loss=torch.where(live, entropy + cross, 0.0),
+                lse=torch.where(live, (top / h.tau + total)[:, 0], 0.0), dz=dz, dx=dz @ w,
+                dw=dz.t() @ x, live=live, p=p, target=target, x=x, w=w, dloss=dloss)
+
+
+def _check(torch, h, zerr=0.0, dx=True, dw=True, gradients=True):
+    """Outputs against the definition in 64 bits, for logits z / tau that err by zerr at most.
+
+    u is the 16-bit type's unit roundoff.  With exact logits, exponentials, sums and logarithm
+    err by 2^-20 relative, and a difference of two logits as the exponent by 2^-22 of itself:
+    words whose differences pass 32 have no weight, so 2^-16 covers both.  dz: two roundings
+    of a numerator, one at the targets, and fp32's underflow, 2^-126 (fp16: its subnormals as
+    well, steps of 2^-24 of a row's largest, and 2^-36 of the largest dz once scaled); dx, dw:
+    those weighted, fp32 accumulation and one rounding of the result.
+    """
+    ref = _definition(torch, h)
+    live = ref["live"]
+    err = 2.0 ** -16 + 2 * zerr
+    assert ((h.lse.double() - ref["lse"]).abs() <= (2.0 ** -21 * ref["lse"].abs() + err) * live).all()
+    tol = err * (1 + ref["loss"].abs())
+    assert ((h.loss.double() - ref["loss"]).abs() <= tol * live).all()
+    if not gradients:
+        return ref
+    u = {"bf16": 2.0 ** -8, "fp16": 2.0 ** -11}[h.dtype]
+    tiny = {"bf16": 2.0 ** -133, "fp16": 2.0 ** -25}[h.dtype]
+    g = ref["dloss"].abs()[:, None]
+    p = ref["p"] * live[:, None]
+    derr = g * (p * (2 * u * (1 + u) + err) + 2.0 ** -126 * live[:, None])
+    derr += (ref["target"] > 0) * (u * ref["dz"].abs() + g * err)
+    if h.dtype == "fp16":
+        derr += live[:, None] * (g * p.amax(dim=1, keepdim=True) + g.max() * 2.0 ** -12) * 2.0 ** -24
+    x, w = ref["x"].abs(), ref["w"].abs()
+    T, V = p.shape
+    if dx:
+        tol = derr @ w + 1.01 * u * ref["dx"].abs() + ref["dz"].abs() @ w * (V + 32) * 2.0 ** -23
+        assert ((h.dx.double() - ref["dx"]).abs() <= tol + tiny).all()
+    if dw:
+        tol = derr.t() @ x + 1.01 * u * ref["dw"].abs() + ref["dz"].abs().t() @ x * (T + 32) * 2.0 ** -23
+        assert ((h.dw.double() - ref["dw"]).abs() <= tol + tiny).all()
+    return ref
+
+
+def _exact_logits(torch, T, V, dtype, K, tau, bx, bw, step, seed):
+    """A head whose logits bx bw + step m, m whole, have no rounding in fp32."""
+    h = Head(torch, T, 64, V, dtype, K=K, tau=tau, seed=seed)
+
+    def whole(*shape):
+        return torch.randint(-1, 2, shape, device="cuda", generator=h.g).float()
+
+    h.x.copy_(whole(T, 64))
+    h.w.copy_(step * whole(V, 64))
+    h.x[:, 0] = bx
+    h.w[:, 0] = bw
+    h.dloss *= T * tau  # dz of about 1
+    if K:
+        h.teacher *= tau  # a teacher of ordinary spread
+    return h
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T", [4, 40, 300])
+@pytest.mark.parametrize("K,tau,bx,bw,step", [  # cross entropy (K 0) has no temperature
+    (5, 2.0 ** -20, 1.0, 8.0, 2.0 ** -20),     # z / tau about 2^23, words 1 apart
+    (5, 2.0 ** -22, 1.0, 8.0, 2.0 ** -20),     # 2^25, 4 apart
+    (5, 2.0 ** -40, 1.0, -8.0, 2.0 ** -20),    # -2^43, and words far apart
+    (5, 2.0 ** -60, 1.0, 8.0, 2.0 ** -20),
+    (0, 1.0, 2.0 ** 12, 2.0 ** 13, 4.0),       # logits of 2^25, 4 apart
+    (5, 1.0, 2.0 ** 12, 2.0 ** 13, 4.0),
+    (0, 1.0, 2.0 ** 12, -(2.0 ** 13), 4.0),
+])
+def test_logits_beyond_their_exponents_fraction(cuda, built, T, K, dtype, tau, bx, bw, step):
+    """|z| / tau so large that fp32 holds no fraction of it: probabilities come of differences."""
+    h = _exact_logits(cuda, T, 700, dtype, K, tau, bx, bw, step, seed=T + K)
+    with Dnn(cuda) as d:
+        assert h.forward(d) == 0
+        cuda.cuda.synchronize()
+        _check(cuda, h, gradients=False)
+        for t in (h.loss, h.lse):
+            t.fill_(math.nan)
+        assert h.backward(d) == 0
+        cuda.cuda.synchronize()
+        _check(cuda, h)
+        h.dx.fill_(math.nan)
+        assert h.backward(d, dw=False) == 0  # a frozen head
+        cuda.cuda.synchronize()
+    _check(cuda, h, dw=False)
+
+
+def _logit_error(h, words):
+    """Most error of the logits of these words, as the fp32 sums leave it."""
+    a = h.x.double().abs() @ h.w[words].double().abs().t()
+    return a.amax().item() * (h.x.shape[1] + 32) * 2.0 ** -23 / h.tau
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("K,tau", [(0, 1.0), (5, 1.0), (5, 0.5)])
+@pytest.mark.parametrize("T", [4, 40, 300])
+def test_words_masked_with_the_lowest_value(cuda, built, T, K, dtype, tau):
+    """Whole tiles of words at the type's lowest value through one feature of 1: no weight."""
+    h = Head(cuda, T, 64, 1500, dtype, K=K, tau=tau, seed=T + K)
+    h.x[:, 0] = 1.0
+    h.w[:, 0] = 0.0
+    masked = cuda.zeros(1500, dtype=cuda.bool, device="cuda")
+    masked[200:1100] = True
+    h.w[masked, 0] = cuda.finfo(h.w.dtype).min
+    if K:
+        h.index = cuda.where(h.index >= 0, h.index % 200, -1)
+    else:
+        h.labels %= 200
+    zerr = _logit_error(h, ~masked)
+    with Dnn(cuda) as d:
+        assert h.forward(d) == 0
+        cuda.cuda.synchronize()
+        _check(cuda, h, zerr, gradients=False)
+        assert h.backward(d) == 0
+        cuda.cuda.synchronize()
+        ref = _check(cuda, h, zerr, dx=dtype == "bf16")
+        assert (ref["p"][:, masked] == 0).all() and (h.dw[masked] == 0).all()
+        assert h.backward(d, dw=False) == 0
+        cuda.cuda.synchronize()
+        _check(cuda, h, zerr, dx=dtype == "bf16", dw=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [0, 5])
+@pytest.mark.parametrize("T", [4, 40, 300])
+def test_every_word_masked_with_the_lowest_value(cuda, built, T, K):
+    """Masks that leave no word: all have the same logit, and the same weight."""
+    h = Head(cuda, T, 64, 700, K=K, seed=T + K)
+    h.x.zero_()  # beside the lowest value, sums could lose its last bit
+    h.x[:, 0] = 1.0
+    h.w[:, 0] = cuda.finfo(h.w.dtype).min
+    with Dnn(cuda) as d:
+        assert h.forward(d) == 0
+        cuda.cuda.synchronize()
+        _check(cuda, h, gradients=False)
+        assert h.backward(d) == 0
+        cuda.cuda.synchronize()
+    ref = _check(cuda, h, dx=False)
+    assert ((ref["p"] - 1 / 700).abs() < 1e-12).all()
