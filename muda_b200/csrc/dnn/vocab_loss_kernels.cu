@@ -350,8 +350,9 @@ __device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& 
     }
   }
   if (row < p.rows) {
+    const float sum = (s[0] + s[1]) + (s[2] + s[3]);  // 1 at least, or 0: all -inf
     p.stats[static_cast<std::int64_t>(row) * p.units + n0 / p.unit] =
-        make_float2(top, (s[0] + s[1]) + (s[2] + s[3]));
+        make_float2(sum == 0.0f ? -INFINITY : top, sum);
   }
   if constexpr (STORE != kNone) {
     tc::fence_proxy_async_smem();

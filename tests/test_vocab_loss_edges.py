@@ -238,3 +238,22 @@ def test_every_word_masked_with_the_lowest_value(cuda, built, T, K):
         cuda.cuda.synchronize()
     ref = _check(cuda, h, dx=False)
     assert ((ref["p"] - 1 / 700).abs() < 1e-12).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T", [40, 300])
+def test_infinite_words_below_low_logits(cuda, built, T, dtype):
+    """Tiles of words at -inf among words at about -400: no gradient for those rows of dw."""
+    h = Head(cuda, T, 64, 900, dtype, seed=T)
+    h.x[:, 0] = 1.0
+    h.w[:, 0] = -400.0
+    h.w[100:600, 0] = -math.inf
+    h.labels %= 100
+    finite = cuda.ones(900, dtype=cuda.bool, device="cuda")
+    finite[100:600] = False
+    with Dnn(cuda) as d:
+        assert h.backward(d, dx=False) == 0
+        cuda.cuda.synchronize()
+    _check(cuda, h, _logit_error(h, finite), dx=False)
+    assert (h.dw[100:600] == 0).all()
