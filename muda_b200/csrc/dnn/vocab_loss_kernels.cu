@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(32 * kTargetWarps)
     bad |= i >= vocab;
     key[k] = ok ? static_cast<int>(i) : INT_MAX;
     if (ok) {
-      mx = fmaxf(mx, t * inv_tau);
+      mx = fmaxf(mx, t);
       ++valid;
     }
   }
@@ -651,9 +651,10 @@ __global__ void __launch_bounds__(32 * kTargetWarps)
   mx = warp_max(mx);
   valid = warp_sum(valid);
   bad = __any_sync(0xffffffffu, bad);
+  // differences before they are scaled, as in finish_unit
   float total = 0.0f;
   for (int k = lane; k < top_k; k += 32)
-    if (key[k] != INT_MAX) total += expf(teacher_logits[r0 + k] * inv_tau - mx);
+    if (key[k] != INT_MAX) total += expf((teacher_logits[r0 + k] - mx) * inv_tau);
   total = warp_sum(total);
   const float log_total = logf(total);
   float ent = 0.0f;
@@ -663,7 +664,7 @@ __global__ void __launch_bounds__(32 * kTargetWarps)
     for (int j = 0; j < top_k; ++j) rank += key[j] < mine || (key[j] == mine && j < k);
     float qk = 0.0f;
     if (mine != INT_MAX) {
-      const float d = teacher_logits[r0 + k] * inv_tau - mx;
+      const float d = (teacher_logits[r0 + k] - mx) * inv_tau;
       qk = expf(d) / total;
       if (qk != 0.0f) ent += qk * (d - log_total);
     }

@@ -257,3 +257,35 @@ def test_infinite_words_below_low_logits(cuda, built, T, dtype):
         cuda.cuda.synchronize()
     _check(cuda, h, _logit_error(h, finite), dx=False)
     assert (h.dw[100:600] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tau", [3e-7, 1e-9])
+@pytest.mark.parametrize("T", [4, 300])
+def test_teacher_logits_beyond_their_exponents_fraction(cuda, built, T, tau):
+    """Teacher logits 8 + 2^-20 m, 2.7e7 and more once divided, and 3.2 m or more apart."""
+    h = Head(cuda, T, 64, 700, K=9, tau=tau, seed=T)
+    h.w *= tau  # a student of ordinary spread
+    h.dloss *= tau
+    h.teacher = 8.0 + cuda.randint(-9, 9, (T, 9), device="cuda", generator=h.g) * 2.0 ** -20
+    zerr = _logit_error(h, slice(None))
+    with Dnn(cuda) as d:
+        assert h.backward(d) == 0
+        cuda.cuda.synchronize()
+    _check(cuda, h, zerr)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tau", [1.0, 0.5])
+@pytest.mark.parametrize("T", [4, 300])
+def test_teacher_entries_masked_with_the_lowest_value(cuda, built, T, tau):
+    """Entries at fp32's lowest value have no weight beside others, and equal weights alone."""
+    h = Head(cuda, T, 64, 700, K=9, tau=tau, seed=T)
+    h.teacher[:, 3:7] = cuda.finfo(cuda.float32).min
+    h.teacher[::2] = cuda.finfo(cuda.float32).min
+    zerr = _logit_error(h, slice(None))
+    with Dnn(cuda) as d:
+        assert h.backward(d) == 0
+        cuda.cuda.synchronize()
+    ref = _check(cuda, h, zerr)
+    assert ref["live"].all()
