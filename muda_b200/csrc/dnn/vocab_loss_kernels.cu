@@ -22,7 +22,8 @@
 // Why the numerators are kept at all: the gradient needs each logit twice, before and after
 // lse is known.  Computing the product again costs 2 H flops per logit, 5 us per 10^6 logits
 // at H = 4096; keeping 16 bits of it costs 6 bytes of traffic, under 1 us.  The piece bounds
-// them to 2 GiB whatever T and V are.
+// them to 2 GiB whatever T is, and whatever V is up to the 8 million words where 128 tokens,
+// the least piece, reach that.
 //
 // What bounds a training step of 8192 x 4096 x 131072 (20.1 ms, 1313 TFLOP/s): the power
 // cap.  The tensor pipe is busy 95 % of the cycles at 1.15-1.4 GHz.  Of a 1546 us score of
@@ -1206,8 +1207,11 @@ struct Dw {
 // Bytes of a piece's numerators.  Every further piece reads and writes dw's fp32 sum: 16384 x
 // 1024 x 131072 took 11.9 ms in one piece of 4 GiB or two of 2 GiB, 12.7 in four of 1 GiB.
 constexpr std::size_t kNumeratorCap = std::size_t{2} << 30;
-constexpr std::size_t kStatsCap = std::size_t{256} << 20;      // a score's pairs
-constexpr int kScoreRows = 16384;                             // tokens of a score's piece
+// Bytes of everything else that grows with a piece's tokens, and its tokens.  The tokens also
+// bound dw's sums: within a piece the tensor cores truncate, pieces add in fp32.
+constexpr std::size_t kGradientCap = std::size_t{960} << 20, kScoreCap = std::size_t{224} << 20;
+constexpr int kGradientRows = 32768, kScoreRows = 16384;
+constexpr int kLeastRows = 128;
 
 // Elements of a 128-byte line: rows that start on one cost the loads of a 64-wide box one
 // line each, others two.
@@ -1308,6 +1312,7 @@ struct Plan {
   // byte offsets into the workspace
   std::size_t stats, z, index, q, count, entropy, hit, scale, row_scale, xp, wp, num, xt, partial,
       sum, bytes;
+  std::size_t rows_bytes;  // of them, what grows with the tokens, without the numerators
 };
 
 Plan plan_rows(const VocabLossArgs& a, int rows) {
@@ -1347,40 +1352,48 @@ Plan plan_rows(const VocabLossArgs& a, int rows) {
   p.scale = take(8);
   p.row_scale = take(p.store == kCommon ? R * 4 : 0);
   p.xp = take(p.pack_x ? R * p.ldp * 2 : 0);
-  p.wp = take(p.pack_w ? V * p.ldp * 2 : 0);
-  p.num = take(a.gradients ? R * p.ldn * 2 : 0);
+  const std::size_t wp = p.pack_w ? V * p.ldp * 2 : 0, num = a.gradients ? R * p.ldn * 2 : 0;
+  const std::size_t sum = dw && p.pieces > 1 ? V * round_up(a.features, 4) * 4 : 0;
+  p.wp = take(wp);
+  p.num = take(num);
   p.xt = take(dw ? H * p.ldt * 2 : 0);
   p.partial = take(p.ksplit > 1 ? p.ksplit * R * H * 4 : 0);
-  p.sum = take(dw && p.pieces > 1 ? V * round_up(a.features, 4) * 4 : 0);
+  p.sum = take(sum);
   p.bytes = at;
+  p.rows_bytes = at - num - wp - sum;
   return p;
 }
 
-// Pieces of equal size, each at most what the caps allow.
+// Pieces of equal size, each at most what the caps allow; in a workspace that has no room for
+// dw's sum between them but for all tokens at once, one piece.
 Plan plan_within(const VocabLossArgs& a, std::size_t limit, bool* ok) {
-  // a score's pairs are 16 bytes per 256 words
-  std::int64_t most = std::min<std::int64_t>(
-      kScoreRows, static_cast<std::int64_t>(kStatsCap / (16 * ((a.vocab + 255ull) / 256))));
-  most = std::max<std::int64_t>(128, most / 128 * 128);
+  const std::size_t cap = a.gradients ? kGradientCap : kScoreCap;
+  // a token's pairs (and hits), and its share of x^T; the loop below sees to the rest
+  const std::size_t per_row = (a.vocab + 127ull) / 128 * (a.top_k > 0 ? 12 : 8) +
+                              (a.gradients ? 2ull * a.features : 0);
+  std::int64_t most = a.gradients ? kGradientRows : kScoreRows;
+  most = std::min(most, static_cast<std::int64_t>(cap / per_row));
   if (a.gradients)
-    most = std::max<std::int64_t>(
-        128, static_cast<std::int64_t>(kNumeratorCap / (round_up(a.vocab, kLine) * 2)) / 128 * 128);
+    most = std::min(most, static_cast<std::int64_t>(kNumeratorCap / (round_up(a.vocab, kLine) * 2)));
+  most = std::max<std::int64_t>(kLeastRows, most / kLeastRows * kLeastRows);
   int pieces = static_cast<int>((a.tokens + most - 1) / most);
   Plan p{};
   for (;;) {
     std::int64_t rows = (a.tokens + pieces - 1) / pieces;
-    if (pieces > 1) rows = round_up(rows, 128);
+    if (pieces > 1) rows = round_up(rows, kLeastRows);
     p = plan_rows(a, static_cast<int>(std::min<std::int64_t>(rows, a.tokens)));
-    if (p.bytes <= limit) {
+    if (p.bytes <= limit && (p.rows_bytes <= cap || rows <= kLeastRows)) {
       *ok = true;
       return p;
     }
-    if (rows <= 128) break;
+    if (rows <= kLeastRows) break;
     // the next count that makes a piece smaller
-    pieces = static_cast<int>((a.tokens + rows - 128 - 1) / std::max<std::int64_t>(rows - 128, 1));
+    rows -= kLeastRows;
+    pieces = static_cast<int>((a.tokens + rows - 1) / rows);
   }
-  *ok = false;
-  return p;
+  const Plan whole = plan_rows(a, a.tokens);
+  *ok = whole.bytes <= limit;
+  return *ok ? whole : p;
 }
 
 // Map of 16-bit elements: `inner` contiguous, `outer` rows of ld elements.
@@ -1663,8 +1676,8 @@ std::size_t vocab_loss_workspace(const VocabLossArgs& a) noexcept {
 }
 
 std::size_t vocab_loss_min_workspace(const VocabLossArgs& a) noexcept {
-  const std::size_t least = plan_rows(a, std::min(a.tokens, 128)).bytes;
-  return std::min(least, vocab_loss_workspace(a));
+  const std::size_t least = plan_rows(a, std::min(a.tokens, kLeastRows)).bytes;
+  return std::min({least, plan_rows(a, a.tokens).bytes, vocab_loss_workspace(a)});
 }
 
 cudaError_t launch_vocab_loss(const VocabLossArgs& a, void* ws, std::size_t ws_bytes,

@@ -289,3 +289,34 @@ def test_teacher_entries_masked_with_the_lowest_value(cuda, built, T, tau):
         cuda.cuda.synchronize()
     ref = _check(cuda, h, zerr)
     assert ref["live"].all()
+
+
+def test_workspace_stays_bounded_for_any_shape(built):
+    """cudnn.h's bound: 2 GiB of numerators, 1 GiB of what else grows with a piece's tokens,
+    V H floats between pieces, and a copy of w whose rows are not a multiple of 16 bytes."""
+    with Dnn() as d:
+        for V in (2, 256, 5000, 131072, 1000003):
+            for H in (8, 64, 1000, 1001, 4096, 8192):
+                w = d.filter(V, H, 1, 1, dtype=capi.CUDNN_DATA_BFLOAT16)
+                for T in (1, 1000, 30000, 300000, 1 << 24):
+                    x = d.tensor(T, H, 1, 1, dtype=capi.CUDNN_DATA_BFLOAT16)
+                    n = C.c_size_t()
+                    assert d.L.cudnnGetLinearDistillationWorkspaceSize(d.h, x, w, 256, 1,
+                                                                       C.byref(n)) == 0
+                    copy = V * (H + 63) // 64 * 64 * 2 if H % 8 else 0
+                    assert n.value <= (3 << 30) + 4 * V * (H + 3) + copy, (T, H, V)
+                    assert d.L.cudnnGetLinearDistillationWorkspaceSize(d.h, x, w, 256, 0,
+                                                                       C.byref(n)) == 0
+                    assert n.value <= (256 << 20) + copy or V > 1000000, (T, H, V)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("K", [0, 3])
+def test_many_tokens_few_words(cuda, built, K, dtype):
+    """More tokens than one piece of a gradient takes, though their numerators would fit."""
+    h = Head(cuda, 70001, 40, 60, dtype, K=K, out=0.1, seed=8)
+    with Dnn(cuda) as d:
+        assert h.backward(d) == 0
+        cuda.cuda.synchronize()
+    h.check()
