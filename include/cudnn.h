@@ -280,9 +280,10 @@ cudnnStatus_t cudnnBatchNormalizationForwardTraining(
  * call runs over pieces of the tokens that need at most 2 GiB for 16-bit numerators and
  * 1 GiB for what else grows with their number (128 tokens at least, which need more only
  * beyond 8 million words); gradients of several pieces need V*H floats too, and a w whose rows
- * are not a multiple of 16 bytes a copy of it.  A workspace given (aligned to 256 bytes)
- * bounds the memory instead: smaller ones mean smaller pieces, down to 128 tokens; BAD_PARAM
- * below that.
+ * are not a multiple of 16 bytes a copy of it.  The size reported serves either or both
+ * gradients and x and w at any address.  A workspace given (aligned to 256 bytes) bounds the
+ * memory instead: smaller ones mean smaller pieces, down to 128 tokens, and a copy of w in
+ * slices of 16 MiB; BAD_PARAM below that.
  * Calls on a handle wait for its workspace across streams.  Under stream capture null takes an
  * allocation of the graph's own instead (a memory node, with CUDA's limits on such graphs), so
  * replays share nothing with the handle; a workspace given is the caller's to keep and order.

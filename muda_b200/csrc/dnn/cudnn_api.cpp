@@ -1146,11 +1146,9 @@ cudnnStatus_t vocab_workspace(cudnnHandle_t handle, cudnnTensorDescriptor_t xDes
   if (s != CUDNN_STATUS_SUCCESS) return s;
   a.top_k = topK;
   a.gradients = gradients != 0;
-  // any aligned address stands for the operands: only alignment enters the plan
-  void* aligned = reinterpret_cast<void*>(std::uintptr_t{256});
-  a.x = a.w = aligned;
-  if (a.gradients) a.dx = a.dw = aligned;
-  *size = mb200::dnn::vocab_loss_workspace(a);
+  // both gradients, and operands at any address
+  if (a.gradients) a.dx = a.dw = reinterpret_cast<void*>(std::uintptr_t{256});
+  *size = mb200::dnn::vocab_loss_workspace_any(a);
   return CUDNN_STATUS_SUCCESS;
 }
 

@@ -41,9 +41,11 @@ struct VocabLossArgs {
   void* dw;
 };
 
-// Device workspace that lets a call run in the pieces it prefers, and the least it can
-// run in (one piece of 128 tokens at a time).  Only sizes, types and alignment count.
+// Device workspace that lets a call run in the pieces it prefers, one that lets it run in
+// them wherever x and w start, and the least it can run in (one piece of 128 tokens at a
+// time).  Only sizes, types, alignment and which gradients there are count.
 std::size_t vocab_loss_workspace(const VocabLossArgs& a) noexcept;
+std::size_t vocab_loss_workspace_any(const VocabLossArgs& a) noexcept;
 std::size_t vocab_loss_min_workspace(const VocabLossArgs& a) noexcept;
 
 // Runs the call in ws_bytes >= vocab_loss_min_workspace(a) bytes (256-byte aligned).

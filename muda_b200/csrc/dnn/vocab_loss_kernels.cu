@@ -199,10 +199,11 @@ struct LogitsTile {
 // tokens x tile_n words; reading w bounds these.
 struct LogitsProblem {
   CUtensorMap mx;    // x: dims (features, rows), box {64, 128, 1}
-  CUtensorMap mw;    // w: dims (features, vocab), box {64, tile_n or half of it, 1}
+  CUtensorMap mw;    // w or a slice of it: dims (features, words), box {64, tile_n or half, 1}
   CUtensorMap mnum;  // numerators: dims (ldn, rows), box {64, 32, 1} (gradients only)
   long long tiles_total;
   int num_kb, tile_n, rows, vocab, tiles_m, tiles_n;
+  int word0;          // the first word of mw
   int band;           // tile rows that stay in L2 while w streams past
   int unit, units;    // words per unit (tile_n / 2), units per row
   float scale;        // log2(e) / tau
@@ -380,7 +381,7 @@ struct Logits : LogitsProblem {
     return c[1] * (PAIR ? 2 : 1) * tc::kBM + row;
   }
   __device__ __forceinline__ int word(const int (&c)[3], int half) const {
-    return c[2] * tile_n + half * unit;
+    return word0 + c[2] * tile_n + half * unit;
   }
   __device__ __forceinline__ void begin(Tile& t, const int (&c)[3], int row, int half) const {
     t.hint = target_hint(*this, token(c, row), word(c, half));
@@ -1005,14 +1006,15 @@ struct Dx {
   // fewest panels (measured: 8 rows 5.0 GB of DRAM reads at 8192 x 4096 x 65536, 4 rows 5.7).
   static constexpr int kBand = 8;
   struct Tile {};
-  CUtensorMap ma;  // w: dims (features, vocab), box {64, 64, 1}
-  CUtensorMap mb;  // dz: dims (vocab, rows), box {64, tile_n or half of it, 1}
+  CUtensorMap ma;  // w or a slice of it: dims (features, words), box {64, 64, 1}
+  CUtensorMap mb;  // dz of these words: dims (words, rows), box {64, tile_n or half of it, 1}
   long long tiles_total;
   int num_kb;  // k-blocks per split
   int tile_n, rows, features, tiles_m, tiles_n;
   T* dx;
   std::int64_t lddx;
-  float* partial;  // ksplit > 1: [split][row][feature]
+  float* partial;  // several splits or slices: [split][row][feature]
+  bool add;        // to what an earlier slice left in partial
   const float* scale;
   const float* row_scale;  // kCommon: [row], else null
 
@@ -1041,6 +1043,11 @@ struct Dx {
       if (h >= features) continue;
       if (partial != nullptr) {
         float* o = partial + (static_cast<std::int64_t>(c[0]) * rows + t0) * features + h;
+        if (add) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (t0 + j < rows) v[j] += o[static_cast<std::int64_t>(j) * features];
+        }
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           if (t0 + j < rows) o[static_cast<std::int64_t>(j) * features] = v[j];
@@ -1297,6 +1304,10 @@ int band_of(int tiles, std::int64_t tile_bytes, std::int64_t keep) {
 
 bool tma_rows_ok(const void* p, std::int64_t ld) { return aligned_to(p, 16) && ld % 8 == 0; }
 
+// Bytes of a copy of some words at a time, for a w that needs one in a workspace without room
+// for all of it.
+constexpr std::size_t kSliceBytes = std::size_t{16} << 20;
+
 struct Plan {
   bool stream;  // scores of few tokens (vocab_stream_kernel)
   StoreMode store;
@@ -1309,13 +1320,14 @@ struct Plan {
   std::int64_t ldt;   // x^T's row
   std::int64_t ldp;   // row of packed copies of x and w
   bool pack_x, pack_w;
+  int slice;          // words of w that are packed at a time; without pack_w all
   // byte offsets into the workspace
   std::size_t stats, z, index, q, count, entropy, hit, scale, row_scale, xp, wp, num, xt, partial,
       sum, bytes;
   std::size_t rows_bytes;  // of them, what grows with the tokens, without the numerators
 };
 
-Plan plan_rows(const VocabLossArgs& a, int rows) {
+Plan plan_rows(const VocabLossArgs& a, int rows, bool sliced) {
   Plan p{};
   p.rows = rows;
   p.pieces = (a.tokens + rows - 1) / rows;
@@ -1329,7 +1341,6 @@ Plan plan_rows(const VocabLossArgs& a, int rows) {
   // tokens).
   if (rows > tc::kBM && a.ldx % kLine != 0) p.pack_x = true;
   const bool dx = a.gradients && a.dx != nullptr, dw = a.gradients && a.dw != nullptr;
-  p.ksplit = dx ? dx_splits(rows, a.features, a.vocab) : 1;
   std::size_t at = 0;
   auto take = [&](std::size_t n) {
     const std::size_t o = at;
@@ -1342,6 +1353,13 @@ Plan plan_rows(const VocabLossArgs& a, int rows) {
   p.unit = p.stream ? kStreamWords : logits_tile_n(rows, a.vocab, a.gradients) / 2;
   p.units = p.stream ? sms() : (a.vocab + p.unit - 1) / p.unit;
   p.hit_units = (a.vocab + p.unit - 1) / p.unit;
+  p.slice = a.vocab;
+  if (p.pack_w && sliced) {  // whole tiles of the logits, whole k-blocks of dx
+    const int whole = 4 * p.unit;
+    const auto words = static_cast<int>(kSliceBytes / (p.ldp * 2)) / whole * whole;
+    p.slice = std::min(a.vocab, std::max(whole, words));
+  }
+  p.ksplit = dx ? dx_splits(rows, a.features, p.slice) : 1;
   p.stats = take(R * p.units * sizeof(float2));
   p.z = take(R * std::max<std::size_t>(K, 1) * 4);
   p.index = take(R * K * 4);
@@ -1350,14 +1368,15 @@ Plan plan_rows(const VocabLossArgs& a, int rows) {
   p.entropy = take(K > 0 ? R * 4 : 0);
   p.hit = take(K > 0 ? R * p.hit_units * 4 : 0);
   p.scale = take(8);
-  p.row_scale = take(p.store == kCommon ? R * 4 : 0);
+  p.row_scale = take(a.gradients ? R * 4 : 0);
   p.xp = take(p.pack_x ? R * p.ldp * 2 : 0);
-  const std::size_t wp = p.pack_w ? V * p.ldp * 2 : 0, num = a.gradients ? R * p.ldn * 2 : 0;
+  const std::size_t wp = p.pack_w ? static_cast<std::size_t>(p.slice) * p.ldp * 2 : 0;
+  const std::size_t num = a.gradients ? R * p.ldn * 2 : 0;
   const std::size_t sum = dw && p.pieces > 1 ? V * round_up(a.features, 4) * 4 : 0;
   p.wp = take(wp);
   p.num = take(num);
   p.xt = take(dw ? H * p.ldt * 2 : 0);
-  p.partial = take(p.ksplit > 1 ? p.ksplit * R * H * 4 : 0);
+  p.partial = take(p.ksplit > 1 || (dx && p.slice < a.vocab) ? p.ksplit * R * H * 4 : 0);
   p.sum = take(sum);
   p.bytes = at;
   p.rows_bytes = at - num - wp - sum;
@@ -1365,8 +1384,9 @@ Plan plan_rows(const VocabLossArgs& a, int rows) {
 }
 
 // Pieces of equal size, each at most what the caps allow; in a workspace that has no room for
-// dw's sum between them but for all tokens at once, one piece.
-Plan plan_within(const VocabLossArgs& a, std::size_t limit, bool* ok) {
+// dw's sum between them but for all tokens at once, one piece.  A copy of w is made in slices
+// where the workspace has no room for all of it, or where `sliced` says so.
+Plan plan_within(const VocabLossArgs& a, std::size_t limit, bool sliced, bool* ok) {
   const std::size_t cap = a.gradients ? kGradientCap : kScoreCap;
   // a token's pairs (and hits), and its share of x^T; the loop below sees to the rest
   const std::size_t per_row = (a.vocab + 127ull) / 128 * (a.top_k > 0 ? 12 : 8) +
@@ -1381,17 +1401,19 @@ Plan plan_within(const VocabLossArgs& a, std::size_t limit, bool* ok) {
   for (;;) {
     std::int64_t rows = (a.tokens + pieces - 1) / pieces;
     if (pieces > 1) rows = round_up(rows, kLeastRows);
-    p = plan_rows(a, static_cast<int>(std::min<std::int64_t>(rows, a.tokens)));
-    if (p.bytes <= limit && (p.rows_bytes <= cap || rows <= kLeastRows)) {
-      *ok = true;
-      return p;
+    for (int s = sliced; s < 2; ++s) {
+      p = plan_rows(a, static_cast<int>(std::min<std::int64_t>(rows, a.tokens)), s != 0);
+      if (p.bytes <= limit && (p.rows_bytes <= cap || rows <= kLeastRows)) {
+        *ok = true;
+        return p;
+      }
     }
     if (rows <= kLeastRows) break;
     // the next count that makes a piece smaller
     rows -= kLeastRows;
     pieces = static_cast<int>((a.tokens + rows - 1) / rows);
   }
-  const Plan whole = plan_rows(a, a.tokens);
+  const Plan whole = plan_rows(a, a.tokens, true);
   *ok = whole.bytes <= limit;
   return *ok ? whole : p;
 }
@@ -1438,31 +1460,36 @@ cudaError_t run_logits(const LogitsProblem& p, unsigned int* timeouts, cudaStrea
     if (e_ != cudaSuccess) return e_;         \
   } while (0)
 
+// dx of the `words` words from word0 on (w is theirs); the slices of a call add up in partial.
 template <typename T, int FMT, bool PAIR, bool TALL>
 cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const void* w, std::int64_t ldw,
-                   const void* num, int rows, T* dx, char* ws, const float* scale,
-                   unsigned int* to, cudaStream_t st) {
+                   int word0, int words, const T* num, int rows, T* dx, char* ws,
+                   const float* scale, unsigned int* to, cudaStream_t st) {
   Dx<T, PAIR, TALL> g{};
   g.tile_n = even_tile_n(rows);
-  if (!make_map(&g.ma, FMT, w, a.features, a.vocab, ldw, 64, 64) ||
-      !make_map(&g.mb, FMT, num, a.vocab, rows, p.ldn, 64, PAIR ? g.tile_n / 2 : g.tile_n))
+  if (!make_map(&g.ma, FMT, w, a.features, words, ldw, 64, 64) ||
+      !make_map(&g.mb, FMT, num + word0, words, rows, p.ldn, 64, PAIR ? g.tile_n / 2 : g.tile_n))
     return cudaErrorInvalidValue;
-  const int kb = (a.vocab + tc::kBK - 1) / tc::kBK;
-  g.num_kb = (kb + p.ksplit - 1) / p.ksplit;
-  const int ks = (kb + g.num_kb - 1) / g.num_kb;  // no split without words
+  // splits of a whole slice; the last, shorter one has no more of them
+  const auto blocks = [](int n) { return (n + tc::kBK - 1) / tc::kBK; };
+  g.num_kb = (blocks(p.slice) + p.ksplit - 1) / p.ksplit;
+  const int ks = (blocks(p.slice) + g.num_kb - 1) / g.num_kb;  // no split without words
   constexpr int kRows = Dx<T, PAIR, TALL>::kRows;
   g.rows = rows;
   g.features = a.features;
   g.tiles_m = (a.features + kRows - 1) / kRows;
   g.tiles_n = (rows + g.tile_n - 1) / g.tile_n;
-  g.tiles_total = static_cast<long long>(g.tiles_m) * g.tiles_n * ks;
+  g.tiles_total = static_cast<long long>(g.tiles_m) * g.tiles_n *
+                  ((blocks(words) + g.num_kb - 1) / g.num_kb);
   g.dx = dx;
   g.lddx = a.lddx;
-  g.partial = ks > 1 ? reinterpret_cast<float*>(ws + p.partial) : nullptr;
+  const bool parts = ks > 1 || p.slice < a.vocab;
+  g.partial = parts ? reinterpret_cast<float*>(ws + p.partial) : nullptr;
+  g.add = word0 > 0;
   g.scale = scale;
   g.row_scale = p.store == kCommon ? reinterpret_cast<float*>(ws + p.row_scale) : nullptr;
   MB200_TRY((tc::launch_tc_epi<Dx<T, PAIR, TALL>, FMT>(g, sms(), to, st, true)));
-  if (ks > 1) {
+  if (parts && word0 + words == a.vocab) {
     const bool vec = a.features % 4 == 0 && a.lddx % 4 == 0 && aligned_to(dx, 8);
     const std::int64_t work = static_cast<std::int64_t>(rows) * a.features / (vec ? 4 : 1);
     const unsigned grid =
@@ -1518,15 +1545,20 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     return tc::launch_overlapped(kern, dim3(static_cast<unsigned>(ctas)), threads, 0, st,
                                  std::exchange(overlap, true), args...);
   };
+  // the words from word0 on that the products below read at a time
   const T* w = static_cast<const T*>(a.w);
-  std::int64_t ldw = a.features;
-  if (p.pack_w) {
-    T* wp = reinterpret_cast<T*>(ws + p.wp);
-    MB200_TRY(launch(vocab_pack_kernel<T>, sms() * 8, 256, w, ldw, a.vocab, a.features, wp,
-                     p.ldp));
-    w = wp;
-    ldw = p.ldp;
-  }
+  const std::int64_t ldw = p.pack_w ? p.ldp : a.features;
+  const auto words_from = [&](int word0) { return std::min(p.slice, a.vocab - word0); };
+  const auto load_slice = [&](int word0) {
+    if (!p.pack_w) return cudaSuccess;
+    w = reinterpret_cast<T*>(ws + p.wp);
+    return launch(vocab_pack_kernel<T>, sms() * 8, 256,
+                  static_cast<const T*>(a.w) + static_cast<std::int64_t>(word0) * a.features,
+                  static_cast<std::int64_t>(a.features), words_from(word0), a.features,
+                  reinterpret_cast<T*>(ws + p.wp), p.ldp);
+  };
+  const bool sliced = p.slice < a.vocab;
+  if (!sliced) MB200_TRY(load_slice(0));
   T* num = reinterpret_cast<T*>(ws + p.num);
   for (int piece = 0; piece < p.pieces; ++piece) {
     const std::int64_t t0 = static_cast<std::int64_t>(piece) * p.rows;
@@ -1597,8 +1629,6 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     LogitsProblem lp{};
     lp.tile_n = 2 * p.unit;
     if (!make_map(&lp.mx, FMT, x, a.features, rows, ldx, tc::kBK, tc::kBM) ||
-        !make_map(&lp.mw, FMT, w, a.features, a.vocab, ldw, tc::kBK,
-                  pair ? lp.tile_n / 2 : lp.tile_n) ||
         (a.gradients && !make_map(&lp.mnum, FMT, num, p.ldn, rows, p.ldn, 64, 32)))
       return cudaErrorInvalidValue;
     lp.num_kb = (a.features + tc::kBK - 1) / tc::kBK;
@@ -1607,8 +1637,6 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     lp.unit = p.unit;
     lp.units = p.units;
     lp.tiles_m = pair ? (rows + 2 * tc::kBM - 1) / (2 * tc::kBM) : 1;
-    lp.tiles_n = (a.vocab + lp.tile_n - 1) / lp.tile_n;
-    lp.tiles_total = static_cast<long long>(lp.tiles_m) * lp.tiles_n;
     // measured at 8192 x 4096 x 65536: 16 MB of x kept 3.2 GB of DRAM reads, 33 MB 2.0, 50 MB
     // 3.3, all 67 MB 4.5 (the numerators pass through L2 too)
     lp.band = band_of(lp.tiles_m, 512ll * a.features, 36ll << 20);
@@ -1619,13 +1647,24 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     // enough CTAs to fill the GPU when there are few rows, each one round of 2048 words at least
     const int parts =
         std::max(1, std::min<int>(4 * sms() / rows, static_cast<int>((p.ldn + 2047) / 2048)));
-    const auto logits = [&](cudaError_t e) {
-      overlap = true;
-      return e;
+    const auto logits = [&](auto store) {
+      constexpr int kStore = decltype(store)::value;
+      for (lp.word0 = 0; lp.word0 < a.vocab; lp.word0 += p.slice) {
+        const int words = words_from(lp.word0);
+        if (sliced) MB200_TRY(load_slice(lp.word0));
+        if (!make_map(&lp.mw, FMT, w, a.features, words, ldw, tc::kBK,
+                      pair ? lp.tile_n / 2 : lp.tile_n))
+          return cudaErrorInvalidValue;
+        lp.tiles_n = (words + lp.tile_n - 1) / lp.tile_n;
+        lp.tiles_total = static_cast<long long>(lp.tiles_m) * lp.tiles_n;
+        MB200_TRY((pair ? run_logits<T, FMT, true, kStore>(lp, to, st, overlap)
+                        : run_logits<T, FMT, false, kStore>(lp, to, st, overlap)));
+        overlap = true;
+      }
+      return cudaSuccess;
     };
     if (p.store == kNone) {
-      MB200_TRY(logits(pair ? run_logits<T, FMT, true, kNone>(lp, to, st, overlap)
-                            : run_logits<T, FMT, false, kNone>(lp, to, st, overlap)));
+      MB200_TRY(logits(std::integral_constant<int, kNone>{}));
       MB200_TRY(launch(vocab_finish_kernel<T, kNone>, rows, kFinishThreads, f));
       continue;
     }
@@ -1639,24 +1678,25 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     }
     const long long finish = static_cast<long long>(rows) * parts;
     if (p.store == kOwn) {
-      MB200_TRY(logits(pair ? run_logits<T, FMT, true, kOwn>(lp, to, st, overlap)
-                            : run_logits<T, FMT, false, kOwn>(lp, to, st, overlap)));
+      MB200_TRY(logits(std::integral_constant<int, kOwn>{}));
       MB200_TRY(launch(vocab_finish_kernel<T, kOwn>, finish + tiles, kFinishThreads, f));
     } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
       f.row_scale = reinterpret_cast<float*>(ws + p.row_scale);
-      MB200_TRY(logits(pair ? run_logits<T, FMT, true, kCommon>(lp, to, st, overlap)
-                            : run_logits<T, FMT, false, kCommon>(lp, to, st, overlap)));
+      MB200_TRY(logits(std::integral_constant<int, kCommon>{}));
       MB200_TRY(launch(vocab_finish_kernel<T, kCommon>, finish, kFinishThreads, f));
     }
 
     if (a.dx != nullptr) {
       T* dx = static_cast<T*>(a.dx) + t0 * a.lddx;
-      if (pair && dx_tall(a.vocab))
-        MB200_TRY((run_dx<T, FMT, true, true>(a, p, w, ldw, num, rows, dx, ws, scale, to, st)));
-      else if (pair)
-        MB200_TRY((run_dx<T, FMT, true, false>(a, p, w, ldw, num, rows, dx, ws, scale, to, st)));
-      else
-        MB200_TRY((run_dx<T, FMT, false, false>(a, p, w, ldw, num, rows, dx, ws, scale, to, st)));
+      for (int word0 = 0; word0 < a.vocab; word0 += p.slice) {
+        if (sliced) MB200_TRY(load_slice(word0));
+        const auto product = [&](auto kern) {
+          return kern(a, p, w, ldw, word0, words_from(word0), num, rows, dx, ws, scale, to, st);
+        };
+        MB200_TRY(product(!pair              ? run_dx<T, FMT, false, false>
+                          : dx_tall(p.slice) ? run_dx<T, FMT, true, true>
+                                             : run_dx<T, FMT, true, false>));
+      }
     }
     if (a.dw != nullptr) {
       if (rows >= kTallTokens)
@@ -1672,18 +1712,35 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
 
 std::size_t vocab_loss_workspace(const VocabLossArgs& a) noexcept {
   bool ok = false;
-  return plan_within(a, SIZE_MAX, &ok).bytes;
+  return plan_within(a, SIZE_MAX, false, &ok).bytes;
+}
+
+std::size_t vocab_loss_workspace_any(const VocabLossArgs& a) noexcept {
+  std::size_t most = 0;
+  for (const std::uintptr_t x : {256, 2}) {
+    for (const std::uintptr_t w : {256, 2}) {
+      VocabLossArgs b = a;
+      b.x = reinterpret_cast<const void*>(x);
+      b.w = reinterpret_cast<const void*>(w);
+      // all of w is copied only where its rows ask for it, not its address alone
+      bool ok = false;
+      most = std::max(most, plan_within(b, SIZE_MAX, a.features % 8 == 0, &ok).bytes);
+    }
+  }
+  return most;
 }
 
 std::size_t vocab_loss_min_workspace(const VocabLossArgs& a) noexcept {
-  const std::size_t least = plan_rows(a, std::min(a.tokens, kLeastRows)).bytes;
-  return std::min({least, plan_rows(a, a.tokens).bytes, vocab_loss_workspace(a)});
+  bool ok = false;
+  return std::min({plan_rows(a, std::min(a.tokens, kLeastRows), true).bytes,
+                   plan_rows(a, a.tokens, true).bytes,
+                   plan_within(a, SIZE_MAX, true, &ok).bytes});
 }
 
 cudaError_t launch_vocab_loss(const VocabLossArgs& a, void* ws, std::size_t ws_bytes,
                               cudaStream_t stream) noexcept {
   bool ok = false;
-  const Plan p = plan_within(a, ws_bytes, &ok);
+  const Plan p = plan_within(a, ws_bytes, false, &ok);
   if (!ok) return cudaErrorInvalidValue;
   return a.bf16 ? run<__nv_bfloat16, 1>(a, p, static_cast<char*>(ws), stream)
                 : run<__half, 0>(a, p, static_cast<char*>(ws), stream);

@@ -320,3 +320,71 @@ def test_many_tokens_few_words(cuda, built, K, dtype):
         assert h.backward(d) == 0
         cuda.cuda.synchronize()
     h.check()
+
+
+def _moved(torch, t, by):
+    """t's values in memory that starts `by` elements off an aligned address."""
+    flat = torch.empty(t.numel() + by, device="cuda", dtype=t.dtype)
+    m = flat[by:].view(t.shape)
+    m.copy_(t)
+    return m
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("K", [0, 5])
+@pytest.mark.parametrize("T,H,V", [(1, 64, 3000), (5, 136, 700), (100, 128, 2001), (300, 72, 900),
+                                   (40, 65, 700), (1, 1001, 300)])
+@pytest.mark.parametrize("x_by,w_by", [(1, 0), (4, 0), (0, 1), (0, 4), (1, 1), (4, 3)])
+def test_reported_workspace_suffices_at_any_address(cuda, built, T, H, V, K, dtype, x_by, w_by):
+    h = Head(cuda, T, H, V, dtype, K=K, seed=T + H)
+    if T == 1 and K:
+        h.index[0, 0] = V - 1
+    h.x, h.w, h.dw = _moved(cuda, h.x, x_by), _moved(cuda, h.w, w_by), _moved(cuda, h.dw, w_by)
+    with Dnn(cuda) as d:
+        ws = cuda.empty(h.workspace_size(d, 0), device="cuda", dtype=cuda.uint8)
+        assert h.forward(d, ws) == 0
+        cuda.cuda.synchronize()
+        h.check(gradients=False)
+        ws = cuda.empty(h.workspace_size(d, 1), device="cuda", dtype=cuda.uint8)
+        assert h.backward(d, ws) == 0
+        cuda.cuda.synchronize()
+        h.check()
+        h.dx.fill_(math.nan)
+        assert h.backward(d, ws, dw=False) == 0
+        cuda.cuda.synchronize()
+        h.check(dw=False)
+        h.dw.fill_(math.nan)
+        assert h.backward(d, ws, dx=False) == 0
+        cuda.cuda.synchronize()
+        h.check(dx=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("K", [0, 7])
+@pytest.mark.parametrize("T,H,V", [(1, 520, 40000), (60, 520, 31001), (300, 600, 40003),
+                                   (150, 72, 140001), (700, 1031, 20011)])
+def test_head_copied_in_slices(cuda, built, T, H, V, K, dtype):
+    """A w that TMA cannot read, in a workspace with room for 16 MiB of its copy: several
+    slices, with dx's partial sums on flat, tall and single-CTA tiles."""
+    h = Head(cuda, T, H, V, dtype, K=K, out=0.1 if T > 4 else 0.0, seed=T + H)
+    if T == 1:
+        h.index = None if not K else h.index.clamp(min=0)
+    h.w = _moved(cuda, h.w, 4)
+    with Dnn(cuda) as d:
+        for gradients in (0, 1):
+            size = h.workspace_size(d, gradients)
+            if H % 8:  # the reported size has room for all of the copy
+                size -= V * (H + 63) // 64 * 64 * 2 - (17 << 20)
+            ws = cuda.empty(size // 256 * 256, device="cuda", dtype=cuda.uint8)
+            for _ in range(2):
+                for t in (h.loss, h.lse, h.dx, h.dw):
+                    t.fill_(math.nan)
+                assert (h.backward(d, ws) if gradients else h.forward(d, ws)) == 0
+                cuda.cuda.synchronize()
+            h.check(gradients=bool(gradients))
+        h.dx.fill_(math.nan)
+        assert h.backward(d, ws, dw=False) == 0
+        cuda.cuda.synchronize()
+        h.check(dw=False)
