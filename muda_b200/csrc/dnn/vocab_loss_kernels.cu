@@ -751,7 +751,7 @@ struct FinishArgs {
   const float* scale;  // fp16: the gradient scale, else null
   void* num;
   std::int64_t ldn;
-  float* row_scale;    // kCommon: dz = row_scale[row] * numerators, 0 for rows left out
+  float* row_scale;    // dz's row is row_scale[row] times what num holds; 0 for rows left out
   TransposeArgs transpose;  // kOwn: x^T for dw's product, in the same launch
 };
 
@@ -854,7 +854,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     if (part == 0 && threadIdx.x == 0) {
       if (a.loss != nullptr) a.loss[row] = 0.0f;
       if (a.lse != nullptr) a.lse[row] = 0.0f;
-      if constexpr (STORE == kCommon) a.row_scale[row] = 0.0f;
+      if constexpr (STORE != kNone) a.row_scale[row] = 0.0f;
     }
     if constexpr (STORE == kOwn) {
       for (std::int64_t c = c_begin + threadIdx.x; c < c_end; c += kFinishThreads)
@@ -899,6 +899,10 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     float g = n < 0 ? NAN : a.dloss[row] * a.inv_tau;
     if (a.scale != nullptr) g *= a.scale[0];
     float down = 0.0f;  // kCommon: the row's reference below its maximum, in z2
+    if constexpr (STORE == kOwn) {
+      if (part == 0 && threadIdx.x == 0)
+        a.row_scale[row] = a.scale != nullptr ? a.scale[1] : 1.0f;
+    }
     if constexpr (STORE == kCommon) {
       const Reference base = reference(mx, a.log2e_tau);
       down = fmaf(base.top - mx, a.log2e_tau, base.whole);
@@ -985,7 +989,7 @@ __global__ void __launch_bounds__(256)
 }
 
 // ------------------------------------------------------------------ gradient GEMMs --
-// A row that is left out has factor 0 and gradient 0, whatever its numerators hold.
+// A row that is left out has factor 0 and gradient 0, whatever its numerators and w hold.
 __device__ __forceinline__ float by_row(float factor, float v) {
   return factor == 0.0f ? 0.0f : factor * v;
 }
@@ -1015,8 +1019,7 @@ struct Dx {
   std::int64_t lddx;
   float* partial;  // several splits or slices: [split][row][feature]
   bool add;        // to what an earlier slice left in partial
-  const float* scale;
-  const float* row_scale;  // kCommon: [row], else null
+  const float* row_scale;  // [row]
 
   const CUtensorMap* __device__ map_a() const { return &ma; }
   const CUtensorMap* __device__ map_b() const { return &mb; }
@@ -1033,7 +1036,6 @@ struct Dx {
                                         std::uint32_t taddr, bool, std::uint8_t*) const {
     const int h = c[1] * kRows + row;
     const int cols = tile_n / 2;
-    const float a = scale != nullptr ? scale[1] : 1.0f;
 #pragma unroll 1
     for (int c0 = 0; c0 < cols; c0 += 16) {
       float v[16];
@@ -1055,24 +1057,20 @@ struct Dx {
         T* o = dx + static_cast<std::int64_t>(t0) * lddx + h;
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-          if (t0 + j < rows)
-            o[j * lddx] = from_float<T>(
-                row_scale != nullptr ? by_row(row_scale[t0 + j], v[j]) : a * v[j]);
+          if (t0 + j < rows) o[j * lddx] = from_float<T>(by_row(row_scale[t0 + j], v[j]));
       }
     }
   }
 };
 
-// dx = scale * (sum of the splits, in split order); VEC features per thread, 1 where rows
+// dx = row_scale * (sum of the splits, in split order); VEC features per thread, 1 where rows
 // are not whole 16-byte runs.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
     vocab_dx_reduce_kernel(const float* __restrict__ partial, int ksplit, int rows, int features,
-                           T* __restrict__ dx, std::int64_t lddx, const float* scale,
-                           const float* row_scale) {
+                           T* __restrict__ dx, std::int64_t lddx, const float* row_scale) {
   tc::grid_launch_next();
   tc::grid_wait_previous();
-  const float a = scale != nullptr ? scale[1] : 1.0f;
   const std::int64_t plane = static_cast<std::int64_t>(rows) * features;
   const std::int64_t per = features / VEC;
   const std::int64_t total = rows * per;
@@ -1081,7 +1079,7 @@ __global__ void __launch_bounds__(256)
     const std::int64_t r = i / per, h = (i - r * per) * VEC;
     const float* p = partial + r * features + h;
     T* o = dx + r * lddx + h;
-    const float f = row_scale != nullptr ? row_scale[r] : a;
+    const float f = row_scale[r];
     if constexpr (VEC == 4) {
       float4 s = __ldcs(reinterpret_cast<const float4*>(p));
 #pragma unroll 4
@@ -1464,7 +1462,7 @@ cudaError_t run_logits(const LogitsProblem& p, unsigned int* timeouts, cudaStrea
 template <typename T, int FMT, bool PAIR, bool TALL>
 cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const void* w, std::int64_t ldw,
                    int word0, int words, const T* num, int rows, T* dx, char* ws,
-                   const float* scale, unsigned int* to, cudaStream_t st) {
+                   unsigned int* to, cudaStream_t st) {
   Dx<T, PAIR, TALL> g{};
   g.tile_n = even_tile_n(rows);
   if (!make_map(&g.ma, FMT, w, a.features, words, ldw, 64, 64) ||
@@ -1486,8 +1484,7 @@ cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const void* w, std::in
   const bool parts = ks > 1 || p.slice < a.vocab;
   g.partial = parts ? reinterpret_cast<float*>(ws + p.partial) : nullptr;
   g.add = word0 > 0;
-  g.scale = scale;
-  g.row_scale = p.store == kCommon ? reinterpret_cast<float*>(ws + p.row_scale) : nullptr;
+  g.row_scale = reinterpret_cast<float*>(ws + p.row_scale);
   MB200_TRY((tc::launch_tc_epi<Dx<T, PAIR, TALL>, FMT>(g, sms(), to, st, true)));
   if (parts && word0 + words == a.vocab) {
     const bool vec = a.features % 4 == 0 && a.lddx % 4 == 0 && aligned_to(dx, 8);
@@ -1496,7 +1493,7 @@ cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const void* w, std::in
         static_cast<unsigned>(std::min<std::int64_t>((work + 255) / 256, sms() * 32));
     MB200_TRY(tc::launch_overlapped(
         vec ? vocab_dx_reduce_kernel<T, 4> : vocab_dx_reduce_kernel<T, 1>, dim3(grid), 256, 0, st, true,
-        g.partial, ks, rows, a.features, dx, a.lddx, scale, g.row_scale));
+        g.partial, ks, rows, a.features, dx, a.lddx, g.row_scale));
   }
   return cudaSuccess;
 }
@@ -1669,6 +1666,7 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
       continue;
     }
     f.dloss = a.dloss + t0;
+    f.row_scale = reinterpret_cast<float*>(ws + p.row_scale);
     f.parts = parts;
     T* xt = reinterpret_cast<T*>(ws + p.xt);
     long long tiles = 0;
@@ -1681,7 +1679,6 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
       MB200_TRY(logits(std::integral_constant<int, kOwn>{}));
       MB200_TRY(launch(vocab_finish_kernel<T, kOwn>, finish + tiles, kFinishThreads, f));
     } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-      f.row_scale = reinterpret_cast<float*>(ws + p.row_scale);
       MB200_TRY(logits(std::integral_constant<int, kCommon>{}));
       MB200_TRY(launch(vocab_finish_kernel<T, kCommon>, finish, kFinishThreads, f));
     }
@@ -1691,7 +1688,7 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
       for (int word0 = 0; word0 < a.vocab; word0 += p.slice) {
         if (sliced) MB200_TRY(load_slice(word0));
         const auto product = [&](auto kern) {
-          return kern(a, p, w, ldw, word0, words_from(word0), num, rows, dx, ws, scale, to, st);
+          return kern(a, p, w, ldw, word0, words_from(word0), num, rows, dx, ws, to, st);
         };
         MB200_TRY(product(!pair              ? run_dx<T, FMT, false, false>
                           : dx_tall(p.slice) ? run_dx<T, FMT, true, true>

@@ -388,3 +388,25 @@ def test_head_copied_in_slices(cuda, built, T, H, V, K, dtype):
         assert h.backward(d, ws, dw=False) == 0
         cuda.cuda.synchronize()
         h.check(dw=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("K", [0, 5])
+@pytest.mark.parametrize("T,V", [(40, 900), (40, 20001), (300, 900), (300, 20001)])
+def test_rows_left_out_beside_infinite_words(cuda, built, T, V, K, dtype):
+    """Words at -inf leave no NaN in dx's rows that are left out (0 times infinity in the
+    product), on any path of dx: with dw and alone, in one sum and in several."""
+    h = Head(cuda, T, 64, V, dtype, K=K, out=0.3, seed=T + K)
+    h.x.abs_()
+    h.x += 0.5
+    h.w[V // 3:V // 2] = -math.inf
+    out = (h.index < 0).all(dim=1) if K else h.labels < 0
+    assert out.any() and not out.all()
+    with Dnn(cuda) as d:
+        for dw in (True, False):
+            h.dx.fill_(math.nan)
+            assert h.backward(d, dw=dw) == 0
+            cuda.cuda.synchronize()
+            assert (h.dx[out] == 0).all()
+            assert h.dx[~out].isnan().any()
