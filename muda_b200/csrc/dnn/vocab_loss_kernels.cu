@@ -751,7 +751,7 @@ struct FinishArgs {
   const float* scale;  // fp16: the gradient scale, else null
   void* num;
   std::int64_t ldn;
-  float* row_scale;    // dz's row is row_scale[row] times what num holds; 0 for rows left out
+  float2* row_scale;   // dz's row is both factors times what num holds; 0 for rows left out
   TransposeArgs transpose;  // kOwn: x^T for dw's product, in the same launch
 };
 
@@ -854,7 +854,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     if (part == 0 && threadIdx.x == 0) {
       if (a.loss != nullptr) a.loss[row] = 0.0f;
       if (a.lse != nullptr) a.lse[row] = 0.0f;
-      if constexpr (STORE != kNone) a.row_scale[row] = 0.0f;
+      if constexpr (STORE != kNone) a.row_scale[row] = make_float2(0.0f, 0.0f);
     }
     if constexpr (STORE == kOwn) {
       for (std::int64_t c = c_begin + threadIdx.x; c < c_end; c += kFinishThreads)
@@ -901,12 +901,12 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     float down = 0.0f;  // kCommon: the row's reference below its maximum, in z2
     if constexpr (STORE == kOwn) {
       if (part == 0 && threadIdx.x == 0)
-        a.row_scale[row] = a.scale != nullptr ? a.scale[1] : 1.0f;
+        a.row_scale[row] = make_float2(1.0f, a.scale != nullptr ? a.scale[1] : 1.0f);
     }
     if constexpr (STORE == kCommon) {
       const Reference base = reference(mx, a.log2e_tau);
       down = fmaf(base.top - mx, a.log2e_tau, base.whole);
-      if (part == 0 && threadIdx.x == 0) a.row_scale[row] = g * exp2f(down - log_sum);
+      if (part == 0 && threadIdx.x == 0) a.row_scale[row] = make_float2(exp2f(down - log_sum), g);
       // only units whose reference is not the row's: rare
       for (int u = u_begin + (threadIdx.x >> 5); u < u_end; u += kFinishThreads / 32) {
         const Reference ref = reference(st[u].x, a.log2e_tau);
@@ -990,8 +990,10 @@ __global__ void __launch_bounds__(256)
 
 // ------------------------------------------------------------------ gradient GEMMs --
 // A row that is left out has factor 0 and gradient 0, whatever its numerators and w hold.
-__device__ __forceinline__ float by_row(float factor, float v) {
-  return factor == 0.0f ? 0.0f : factor * v;
+// The factors stay two: kCommon's first is down to 2^-64 / V, and its product with a small
+// dloss would leave fp32's range where dx does not.
+__device__ __forceinline__ float by_row(float2 factor, float v) {
+  return factor.x == 0.0f ? 0.0f : factor.x * v * factor.y;
 }
 
 // dx^T = w^T dz^T: A = w^T is MN-major in w, B = dz is K-major, the faster operand forms;
@@ -1019,7 +1021,7 @@ struct Dx {
   std::int64_t lddx;
   float* partial;  // several splits or slices: [split][row][feature]
   bool add;        // to what an earlier slice left in partial
-  const float* row_scale;  // [row]
+  const float2* row_scale;  // [row]
 
   const CUtensorMap* __device__ map_a() const { return &ma; }
   const CUtensorMap* __device__ map_b() const { return &mb; }
@@ -1068,7 +1070,7 @@ struct Dx {
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
     vocab_dx_reduce_kernel(const float* __restrict__ partial, int ksplit, int rows, int features,
-                           T* __restrict__ dx, std::int64_t lddx, const float* row_scale) {
+                           T* __restrict__ dx, std::int64_t lddx, const float2* row_scale) {
   tc::grid_launch_next();
   tc::grid_wait_previous();
   const std::int64_t plane = static_cast<std::int64_t>(rows) * features;
@@ -1079,7 +1081,7 @@ __global__ void __launch_bounds__(256)
     const std::int64_t r = i / per, h = (i - r * per) * VEC;
     const float* p = partial + r * features + h;
     T* o = dx + r * lddx + h;
-    const float f = row_scale[r];
+    const float2 f = row_scale[r];
     if constexpr (VEC == 4) {
       float4 s = __ldcs(reinterpret_cast<const float4*>(p));
 #pragma unroll 4
@@ -1366,7 +1368,7 @@ Plan plan_rows(const VocabLossArgs& a, int rows, bool sliced) {
   p.entropy = take(K > 0 ? R * 4 : 0);
   p.hit = take(K > 0 ? R * p.hit_units * 4 : 0);
   p.scale = take(8);
-  p.row_scale = take(a.gradients ? R * 4 : 0);
+  p.row_scale = take(a.gradients ? R * sizeof(float2) : 0);
   p.xp = take(p.pack_x ? R * p.ldp * 2 : 0);
   const std::size_t wp = p.pack_w ? static_cast<std::size_t>(p.slice) * p.ldp * 2 : 0;
   const std::size_t num = a.gradients ? R * p.ldn * 2 : 0;
@@ -1484,7 +1486,7 @@ cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const void* w, std::in
   const bool parts = ks > 1 || p.slice < a.vocab;
   g.partial = parts ? reinterpret_cast<float*>(ws + p.partial) : nullptr;
   g.add = word0 > 0;
-  g.row_scale = reinterpret_cast<float*>(ws + p.row_scale);
+  g.row_scale = reinterpret_cast<float2*>(ws + p.row_scale);
   MB200_TRY((tc::launch_tc_epi<Dx<T, PAIR, TALL>, FMT>(g, sms(), to, st, true)));
   if (parts && word0 + words == a.vocab) {
     const bool vec = a.features % 4 == 0 && a.lddx % 4 == 0 && aligned_to(dx, 8);
@@ -1666,7 +1668,7 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
       continue;
     }
     f.dloss = a.dloss + t0;
-    f.row_scale = reinterpret_cast<float*>(ws + p.row_scale);
+    f.row_scale = reinterpret_cast<float2*>(ws + p.row_scale);
     f.parts = parts;
     T* xt = reinterpret_cast<T*>(ws + p.xt);
     long long tiles = 0;

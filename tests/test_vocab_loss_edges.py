@@ -410,3 +410,22 @@ def test_rows_left_out_beside_infinite_words(cuda, built, T, V, K, dtype):
             cuda.cuda.synchronize()
             assert (h.dx[out] == 0).all()
             assert h.dx[~out].isnan().any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [0, 5])
+@pytest.mark.parametrize("T", [40, 300])
+@pytest.mark.parametrize("offset", [40.0, -40.0])
+def test_small_upstream_gradients(cuda, built, T, K, offset):
+    """dloss of 1e-24 on logits of about 40: dx of 1e-24 is far inside bf16's range."""
+    h = Head(cuda, T, 64, 900, K=K, out=0.1, seed=T + K)
+    h.x[:, 0] = 8.0
+    h.w[:, 0] = offset / 8.0
+    h.dloss *= T * 1e-24
+    with Dnn(cuda) as d:
+        for dw in (True, False):
+            h.dx.fill_(math.nan)
+            assert h.backward(d, dw=dw) == 0
+            cuda.cuda.synchronize()
+            h.check(dw=dw)
+            assert (h.dx.double().abs() > 0).double().mean() > 0.5
