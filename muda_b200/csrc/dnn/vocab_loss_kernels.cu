@@ -185,7 +185,10 @@ constexpr int kUnit = 128;
 // k-blocks per accumulator.  Tensor-core accumulation truncates: one chain of 256 MMAs
 // (H = 4096) left lse 3.4e-6 off in the 2-norm, chunks of 32 MMAs added in fp32 registers
 // 4e-7, an fp32 product's level.
-constexpr int kLogitsChunk = 8;
+// Up to 8 tokens take 8 MMAs, as their streaming kernel does, so that a width that it cannot
+// read is no less exact (T 4, H 4001: 3.0e-7 and 0.8e-7, streamed at 4000 0.9e-7); with more
+// tokens that would cost up to 37 % (score of 128 x 768 x 50257).
+constexpr int kLogitsChunk = 8, kFewLogitsChunk = 2;
 
 // A thread's logits of one token, and what says whether a target word is among them: the
 // token's label, or its entry of the hit map.  Loaded before the
@@ -369,11 +372,11 @@ __device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& 
 }
 
 // STORE needs units of 64 or 128 words: the stage's boxes are 64 wide.
-template <typename T, bool PAIR, int STORE>
+template <typename T, bool PAIR, int STORE, int CHUNK>
 struct Logits : LogitsProblem {
   static constexpr bool kPair = PAIR, kTall = false;
   static constexpr bool kAMn = false;
-  static constexpr int kChunk = kLogitsChunk;
+  static constexpr int kChunk = CHUNK;
   static constexpr int kStageBytes = STORE != kNone ? 8192 : 0;
   using Tile = LogitsTile;
 
@@ -1446,12 +1449,13 @@ unsigned int* timeout_counter() {
   return addr[dev];
 }
 
-template <typename T, int FMT, bool PAIR, int STORE>
+template <typename T, int FMT, bool PAIR, int STORE, int CHUNK>
 cudaError_t run_logits(const LogitsProblem& p, unsigned int* timeouts, cudaStream_t st,
                        bool overlap) {
-  Logits<T, PAIR, STORE> q;
+  using Problem = Logits<T, PAIR, STORE, CHUNK>;
+  Problem q;
   static_cast<LogitsProblem&>(q) = p;
-  return tc::launch_tc_epi<Logits<T, PAIR, STORE>, FMT>(q, sms(), timeouts, st, overlap);
+  return tc::launch_tc_epi<Problem, FMT>(q, sms(), timeouts, st, overlap);
 }
 
 #define MB200_TRY(expr)                       \
@@ -1656,8 +1660,10 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
           return cudaErrorInvalidValue;
         lp.tiles_n = (words + lp.tile_n - 1) / lp.tile_n;
         lp.tiles_total = static_cast<long long>(lp.tiles_m) * lp.tiles_n;
-        MB200_TRY((pair ? run_logits<T, FMT, true, kStore>(lp, to, st, overlap)
-                        : run_logits<T, FMT, false, kStore>(lp, to, st, overlap)));
+        const auto form = pair                     ? run_logits<T, FMT, true, kStore, kLogitsChunk>
+                          : rows <= kStreamTokens ? run_logits<T, FMT, false, kStore, kFewLogitsChunk>
+                                                  : run_logits<T, FMT, false, kStore, kLogitsChunk>;
+        MB200_TRY(form(lp, to, st, overlap));
         overlap = true;
       }
       return cudaSuccess;

@@ -429,3 +429,23 @@ def test_small_upstream_gradients(cuda, built, T, K, offset):
             cuda.cuda.synchronize()
             h.check(dw=dw)
             assert (h.dx.double().abs() > 0).double().mean() > 0.5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gradients", [False, True])
+def test_odd_width_is_as_exact_for_few_tokens(cuda, built, gradients):
+    """Log-sum-exps of 8 tokens at a width that 16-byte loads cannot read, against those at one
+    that they can: root mean squares over 64 of them scatter by a tenth, so a factor of two
+    is no accident."""
+    def error(H):
+        total = 0.0
+        for seed in range(8):
+            h = Head(cuda, 8, H, 2000, seed=seed)
+            h.x += 14 * h.w[h.labels]  # tokens that one word explains: its logit is the sum
+            with Dnn(cuda) as d:
+                assert (h.backward(d) if gradients and H % 8 else h.forward(d)) == 0
+                cuda.cuda.synchronize()
+            total += (h.lse.double() - _definition(cuda, h)["lse"]).square().sum().item()
+        return math.sqrt(total / 64)
+
+    assert error(4001) <= 2 * error(4000)
