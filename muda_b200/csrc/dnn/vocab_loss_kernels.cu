@@ -35,7 +35,8 @@
 // the 16 bits that carry the numerators to step 2 hold 2 more significant bits than dz
 // (OwnCode; fp32 numerators would double the piece's traffic).  The target words, whose
 // p - q cancels, are recomputed in step 2 from their fp32 logits and rounded once.  dx and
-// dw round once more at the end.
+// dw round once more at the end; their sums run in chains of MMAs whose truncation stays well
+// below that (dx_chain, kGradientRows).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -1270,11 +1271,17 @@ int even_tile_n(int cols) {
 // x 32768 479 and 492; 4096 x 4096 x 65536 3644 and 3503.
 bool dx_tall(int vocab) { return vocab >= 49152; }
 
+// Most words that dx adds up in one chain of truncating MMAs.  Each loses up to half a unit in
+// the sum's last place, all toward zero, and with one large term (the target's) early in the
+// sum they add up: over 110000 words 1.3e-4 of dx, beside 3.0e-4 from fp16's two roundings and
+// 2.4e-3 from bf16's.  A split of this length stays below an eighth of them.
+int dx_chain(bool bf16) { return bf16 ? 262144 : 32768; }
+
 // Splits of the words in dx's product: the count that ends soonest.  A k-block takes 512
 // clocks of MMAs per 256 x 256 on a pair; a single CTA's streams w at its share of memory
 // bandwidth (measured 5.5 TB/s).  Each split's partial sums are written and read once, by one
-// more launch.
-int dx_splits(int rows, int features, int vocab) {
+// more launch.  No split is longer than dx_chain.
+int dx_splits(int rows, int features, int vocab, bool bf16) {
   const bool pair = rows > tc::kBM;
   const int bm = dx_tall(vocab) ? 512 : 256;
   const std::int64_t tiles =
@@ -1284,13 +1291,14 @@ int dx_splits(int rows, int features, int vocab) {
   const int n = pair ? sms() / 2 : sms();
   const double block = pair ? bm * 2 / 1.6e9 * even_tile_n(rows) / tc::kEpiN
                             : tc::kBM * tc::kRowBytes * n / 5.5e12;
+  const int least = (vocab + dx_chain(bf16) - 1) / dx_chain(bf16);
   double best = 0.0;
-  int pick = 1;
-  for (int ks = 1; ks <= 32 && ks * 8 <= std::max(kb, 8); ++ks) {
+  int pick = least;
+  for (int ks = least; ks == least || (ks <= 32 && ks * 8 <= kb); ++ks) {
     const double waves = static_cast<double>((tiles * ks + n - 1) / n);
     const double loop = waves * ((kb + ks - 1) / ks) * block;
     const double join = ks == 1 ? 0.0 : 6e-6 + 8.0 * ks * rows * features / 4.5e12;
-    if (ks == 1 || loop + join < best) {
+    if (ks == least || loop + join < best) {
       best = loop + join;
       pick = ks;
     }
@@ -1362,7 +1370,7 @@ Plan plan_rows(const VocabLossArgs& a, int rows, bool sliced) {
     const auto words = static_cast<int>(kSliceBytes / (p.ldp * 2)) / whole * whole;
     p.slice = std::min(a.vocab, std::max(whole, words));
   }
-  p.ksplit = dx ? dx_splits(rows, a.features, p.slice) : 1;
+  p.ksplit = dx ? dx_splits(rows, a.features, p.slice, a.bf16) : 1;
   p.stats = take(R * p.units * sizeof(float2));
   p.z = take(R * std::max<std::size_t>(K, 1) * 4);
   p.index = take(R * K * 4);
