@@ -266,7 +266,7 @@ cudnnStatus_t cudnnBatchNormalizationForwardTraining(
  * A negative label leaves its token out; a negative teacher index, or a teacher logit of
  * -inf, leaves its entry out, and a token without entries is left out.  A token that is
  * left out has loss 0, logSumExp 0 and no gradient, whatever its x and dloss hold.
- * Equal indices of a token add up.  A label or index of V or more makes its token's loss,
+ * Temperatures are 2^-64 to 2^64.  Equal indices of a token add up.  A label or index of V or more makes its token's loss,
  * and the gradients it enters, NaN.  labels and teacherIndex [T][topK] are int64 (as
  * training programs hold them); teacherLogits [T][topK], loss and logSumExp are float.
  *
@@ -274,7 +274,10 @@ cudnnStatus_t cudnnBatchNormalizationForwardTraining(
  * tokens; it computes the losses too and writes them when loss / logSumExp are not null,
  * so a training step whose dloss is known needs no Forward.  dx (like x; it may be x
  * itself) or dw (like w) may be null with its descriptor: it is not computed.  Results
- * do not depend on the stream's other work: no atomics.
+ * do not depend on the stream's other work: no atomics.  The gradient of the logits is
+ * rounded to 16 bits on its way into both products.  In HALF it is scaled by one power of
+ * two per piece of the tokens (below), so tokens whose |dloss| is 2^-20 of their piece's
+ * largest or less keep fewer bits of it.
  *
  * The workspace: null uses the handle's own (grown to what GetWorkspaceSize reports).  A
  * call runs over pieces of the tokens that need at most 2 GiB for 16-bit numerators and

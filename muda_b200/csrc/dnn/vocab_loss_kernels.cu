@@ -1268,7 +1268,8 @@ int even_tile_n(int cols) {
 
 // dx on tall tiles: for a vocabulary that makes K long against the drain of a tile and dz too
 // large for L2.  Measured (loss and dx, flat and tall): 2048 x 2048 x 16384 212-241 and 247 us,
-// x 32768 479 and 492; 4096 x 4096 x 65536 3644 and 3503.
+// x 32768 479 and 492; 4096 x 4096 x 65536 3644 and 3503; the bound lies between the last two.
+// Widths that leave part of a 512-row tile empty (768, 1280) go by the same rule, unmeasured.
 bool dx_tall(int vocab) { return vocab >= 49152; }
 
 // Most words that dx adds up in one chain of truncating MMAs.  Each loses up to half a unit in
@@ -1514,7 +1515,8 @@ cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const void* w, std::in
 
 // dw on tall tiles: a tall tile drains before its successor starts (about 3000 clocks), but
 // reads 3/4 of the operands.  Measured at 65536 x 4096, 2048 tokens: 684 us flat, 746 tall;
-// 4096: 1367 and 1404; 8192: 3038 and 2836 (x^T no longer fits L2: 6.9 and 4.5 GB of reads).
+// 4096: 1367 and 1404; 8192: 3038 and 2836 (x^T no longer fits L2: 6.9 and 4.5 GB of reads);
+// the bound is the middle of the last two.
 constexpr int kTallTokens = 6144;
 
 template <typename T, int FMT, bool TALL>
