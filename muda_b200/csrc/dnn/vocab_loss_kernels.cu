@@ -31,7 +31,8 @@
 // reads of the operands (timed without them), hence the wide tiles and the banded order.
 //
 // Precision: products of the 16-bit inputs accumulate in fp32; maxima, sums, target
-// logits and losses are fp32.  dz is a 16-bit operand of the tensor cores and rounds once;
+// logits and losses are fp32.  dz is a 16-bit operand of the tensor cores and rounds once
+// (two of them for up to 64 tokens, see kSplit);
 // the 16 bits that carry the numerators to step 2 hold 2 more significant bits than dz
 // (OwnCode; fp32 numerators would double the piece's traffic).  The target words, whose
 // p - q cancels, are recomputed in step 2 from their fp32 logits and rounded once.  dx and
@@ -268,7 +269,14 @@ __device__ __forceinline__ void pick_targets(const LogitsProblem& p, const Logit
 // row's maximum: the nearest whole exponent, so that moving numerators from one to another is
 // exact, or the maximum itself where fp32 holds no fraction of the exponent any more.
 // Loss and dx of 4096 x 2048 x 65536: 1768 us with kOwn, 1657 with kCommon.
-enum StoreMode { kNone = 0, kOwn = 1, kCommon = 2 };
+// kSplit is kOwn whose dz becomes two 16-bit rows, rounded and what rounding left, that both
+// products add up.  With few tokens the target word's one rounding is common to all of a
+// token's dx (and to its row of dw) and does not average out: errors of one token to 64 were
+// 1.25 to 1.45 times one rounding in the mean and up to 2.4, and are 1.00 to 1.03.  w's bytes
+// set the time there: steps of 39 x 6464 x 16408 162 -> 166 us, 64 x 1111 x 32003 123 -> 126,
+// loss and dx of 64 x 2048 x 65536 109 -> 119; at 128 tokens a step would take 16 % more.
+enum StoreMode { kNone = 0, kOwn = 1, kCommon = 2, kSplit = 3 };
+constexpr int kSplitTokens = 64;
 constexpr float kCommonReach = 64.0f, kWholeReach = 0x1p22f;
 
 // kCommon's numerators of a unit with this maximum are 2^(z2 - top * scale - whole).
@@ -754,9 +762,9 @@ struct FinishArgs {
   float log2e_tau;     // log2(e) / tau
   const float* scale;  // fp16: the gradient scale, else null
   void* num;
-  std::int64_t ldn;
+  std::int64_t ldn, pitch;  // words of a row of num, and from a token's row to the next's
   float2* row_scale;   // dz's row is both factors times what num holds; 0 for rows left out
-  TransposeArgs transpose;  // kOwn: x^T for dw's product, in the same launch
+  TransposeArgs transpose;  // with dz: x^T for dw's product, in the same launch
 };
 
 // xt[h][row] = x[row][h], rows that are left out as zeros (their x may hold anything, and
@@ -765,7 +773,8 @@ struct FinishArgs {
 // 64 x 64 tiles, 16 bytes per thread and access (reads: where x's rows allow it): 8192 x 4096
 // in 29 us as a launch of its own (4.6 TB/s; 2-byte accesses took 78).
 // The tile's pitch of 33 words keeps its column reads to two words of a bank.
-template <typename T>
+// TWICE: every token fills two columns of x^T, for dz's two rows.
+template <typename T, bool TWICE>
 __device__ __forceinline__ void transpose_tile(const TransposeArgs& a, const Targets& targets,
                                                int vocab, long long block) {
   __shared__ std::uint32_t tile[64][33];
@@ -806,24 +815,40 @@ __device__ __forceinline__ void transpose_tile(const TransposeArgs& a, const Tar
   for (int i = 0; i < 2; ++i) {
     const int h = (threadIdx.x >> 3) + 32 * i, r = (threadIdx.x & 7) * 8;
     if (h0 + h >= features || r0 + r >= rows) continue;  // x^T's rows are padded to whole lines
-    std::uint32_t o[4];
+    constexpr int kCopies = TWICE ? 2 : 1;
+    std::uint32_t o[4 * kCopies];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      o[j] = __byte_perm(tile[r + 2 * j][h / 2], tile[r + 2 * j + 1][h / 2],
-                         (h & 1) != 0 ? 0x7632 : 0x5410);
-    *reinterpret_cast<uint4*>(xt + static_cast<std::int64_t>(h0 + h) * ldt + r0 + r) =
-        make_uint4(o[0], o[1], o[2], o[3]);
+    for (int j = 0; j < 4 * kCopies; ++j) {
+      if constexpr (TWICE)
+        o[j] = __byte_perm(tile[r + j][h / 2], 0u, (h & 1) != 0 ? 0x3232 : 0x1010);
+      else
+        o[j] = __byte_perm(tile[r + 2 * j][h / 2], tile[r + 2 * j + 1][h / 2],
+                           (h & 1) != 0 ? 0x7632 : 0x5410);
+    }
+    uint4* dst = reinterpret_cast<uint4*>(xt + static_cast<std::int64_t>(h0 + h) * ldt +
+                                          kCopies * (r0 + r));
+#pragma unroll
+    for (int j = 0; j < kCopies; ++j)
+      dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
   }
 }
 
-// Eight numerators times f, in T.
+// What rounding v to r left; 0 for infinities.
+__device__ __forceinline__ float rest(float v, float r) { return v == r ? 0.0f : v - r; }
+
+// Eight numerators times f, in T; kSplit: what their rounding left, in *left.
 template <typename T, int STORE>
-__device__ __forceinline__ uint4 scaled(uint4 u, float f) {
+__device__ __forceinline__ uint4 scaled(uint4 u, float f, uint4* left = nullptr) {
   std::uint32_t* w = reinterpret_cast<std::uint32_t*>(&u);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float2 v = STORE == kOwn ? unpack_own<T>(w[j]) : unpack2<T>(w[j]);
-    w[j] = pack2<T>(f * v.x, f * v.y);
+    float2 v = STORE == kCommon ? unpack2<T>(w[j]) : unpack_own<T>(w[j]);
+    v = make_float2(f * v.x, f * v.y);
+    w[j] = pack2<T>(v.x, v.y);
+    if constexpr (STORE == kSplit) {
+      const float2 r = unpack2<T>(w[j]);
+      reinterpret_cast<std::uint32_t*>(left)[j] = pack2<T>(rest(v.x, r.x), rest(v.y, r.y));
+    }
   }
   return u;
 }
@@ -835,11 +860,12 @@ template <typename T, int STORE>
 __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const FinishArgs a) {
   tc::grid_launch_next();
   tc::grid_wait_previous();
+  constexpr bool kDz = STORE == kOwn || STORE == kSplit;
   __shared__ float red[kFinishThreads / 32];
   const long long finish = static_cast<long long>(a.rows) * a.parts;
-  if constexpr (STORE == kOwn) {
+  if constexpr (kDz) {
     if (blockIdx.x >= finish) {
-      transpose_tile<T>(a.transpose, a.targets, a.vocab, blockIdx.x - finish);
+      transpose_tile<T, STORE == kSplit>(a.transpose, a.targets, a.vocab, blockIdx.x - finish);
       return;
     }
   }
@@ -853,16 +879,19 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
   const int per_unit = a.unit / 8;
   const std::int64_t c_begin = static_cast<std::int64_t>(u_begin) * per_unit;
   const std::int64_t c_end = min(a.ldn / 8, static_cast<std::int64_t>(u_end) * per_unit);
-  uint4* num = reinterpret_cast<uint4*>(static_cast<T*>(a.num) + row * a.ldn);
+  uint4* num = reinterpret_cast<uint4*>(static_cast<T*>(a.num) + row * a.pitch);
+  const std::int64_t low = a.ldn / 8;  // kSplit: from dz's row to that of what rounding left
   if (n == 0) {  // left out
     if (part == 0 && threadIdx.x == 0) {
       if (a.loss != nullptr) a.loss[row] = 0.0f;
       if (a.lse != nullptr) a.lse[row] = 0.0f;
       if constexpr (STORE != kNone) a.row_scale[row] = make_float2(0.0f, 0.0f);
     }
-    if constexpr (STORE == kOwn) {
-      for (std::int64_t c = c_begin + threadIdx.x; c < c_end; c += kFinishThreads)
+    if constexpr (kDz) {
+      for (std::int64_t c = c_begin + threadIdx.x; c < c_end; c += kFinishThreads) {
         num[c] = make_uint4(0, 0, 0, 0);
+        if constexpr (STORE == kSplit) num[low + c] = make_uint4(0, 0, 0, 0);
+      }
     }
     return;
   }
@@ -903,7 +932,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     float g = n < 0 ? NAN : a.dloss[row] * a.inv_tau;
     if (a.scale != nullptr) g *= a.scale[0];
     float down = 0.0f;  // kCommon: the row's reference below its maximum, in z2
-    if constexpr (STORE == kOwn) {
+    if constexpr (kDz) {
       if (part == 0 && threadIdx.x == 0)
         a.row_scale[row] = make_float2(1.0f, a.scale != nullptr ? a.scale[1] : 1.0f);
     }
@@ -924,25 +953,37 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
       const auto factor = [&](std::int64_t c) {
         return g * exp2f(fmaf(st[c / per_unit].x - mx, a.log2e_tau, -log_sum));
       };
+      const auto rescale = [&](std::int64_t c, uint4 u) {
+        if constexpr (STORE == kSplit) {
+          uint4 left;
+          num[c] = scaled<T, STORE>(u, factor(c), &left);
+          num[low + c] = left;
+        } else {
+          num[c] = scaled<T, STORE>(u, factor(c));
+        }
+      };
       std::int64_t c = c_begin + threadIdx.x;
       for (; c + 3 * kFinishThreads < c_end; c += 4 * kFinishThreads) {
         uint4 u[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) u[j] = num[c + j * kFinishThreads];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          num[c + j * kFinishThreads] = scaled<T, STORE>(u[j], factor(c + j * kFinishThreads));
+        for (int j = 0; j < 4; ++j) rescale(c + j * kFinishThreads, u[j]);
       }
-      for (; c < c_end; c += kFinishThreads) num[c] = scaled<T, STORE>(num[c], factor(c));
+      for (; c < c_end; c += kFinishThreads) rescale(c, num[c]);
     }
     // the targets, in the numerators' units: dz, or dz / row_scale
     const float t = STORE == kCommon ? exp2f(log_sum - down) : g;
     __syncthreads();
-    T* d = static_cast<T*>(a.num) + row * a.ldn;
+    const auto put = [&](std::int64_t word, float v) {
+      T* d = reinterpret_cast<T*>(num) + word;
+      *d = from_float<T>(v);
+      if constexpr (STORE == kSplit) d[a.ldn] = from_float<T>(rest(v, static_cast<float>(*d)));
+    };
     if (a.targets.top_k == 0) {
       const std::int64_t l = a.targets.labels[row];
       if (threadIdx.x == 0 && n > 0 && l >= c_begin * 8 && l < c_end * 8)
-        d[l] = from_float<T>(t * expm1f((above(r0) - log_sum) * kLn2));
+        put(l, t * expm1f((above(r0) - log_sum) * kLn2));
     } else {
       for (int k = threadIdx.x; k < n; k += kFinishThreads) {
         const int w = a.targets.index[r0 + k];
@@ -950,7 +991,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
         if (k > 0 && a.targets.index[r0 + k - 1] == w) continue;  // the run's first entry adds all
         float q = a.targets.q[r0 + k];
         for (int j = k + 1; j < n && a.targets.index[r0 + j] == w; ++j) q += a.targets.q[r0 + j];
-        d[w] = from_float<T>(t * (exp2f(above(r0 + k) - log_sum) - q));
+        put(w, t * (exp2f(above(r0 + k) - log_sum) - q));
       }
     }
   }
@@ -1004,8 +1045,8 @@ __device__ __forceinline__ float by_row(float2 factor, float v) {
 // a thread's columns are tokens of one feature, so a warp's stores of one token are 32
 // consecutive features.  The words (K) split across `ksplit` groups of CTAs.  Pairs (more
 // than 128 tokens): 256 features x 256 tokens, or tall tiles of 512; else 128 features x
-// all tokens.
-template <typename T, bool PAIR, bool TALL>
+// all tokens.  SPLIT: a token has two rows of dz side by side, and so do a thread's columns.
+template <typename T, bool PAIR, bool TALL, bool SPLIT>
 struct Dx {
   static constexpr bool kPair = PAIR, kTall = TALL;
   static constexpr bool kAMn = true;
@@ -1017,7 +1058,7 @@ struct Dx {
   static constexpr int kBand = 8;
   struct Tile {};
   CUtensorMap ma;  // w or a slice of it: dims (features, words), box {64, 64, 1}
-  CUtensorMap mb;  // dz of these words: dims (words, rows), box {64, tile_n or half of it, 1}
+  CUtensorMap mb;  // dz of these words: dims (words, its rows), box {64, tile_n or half, 1}
   long long tiles_total;
   int num_kb;  // k-blocks per split
   int tile_n, rows, features, tiles_m, tiles_n;
@@ -1042,27 +1083,32 @@ struct Dx {
                                         std::uint32_t taddr, bool, std::uint8_t*) const {
     const int h = c[1] * kRows + row;
     const int cols = tile_n / 2;
+    constexpr int kTokens = SPLIT ? 8 : 16;  // of 16 columns
 #pragma unroll 1
     for (int c0 = 0; c0 < cols; c0 += 16) {
       float v[16];
       __syncwarp();
       tc::tmem_load_16cols(taddr + static_cast<std::uint32_t>(c0), v);
-      const int t0 = c[2] * tile_n + half * cols + c0;
+      if constexpr (SPLIT) {
+#pragma unroll
+        for (int j = 0; j < kTokens; ++j) v[j] = v[2 * j] + v[2 * j + 1];
+      }
+      const int t0 = (c[2] * tile_n + half * cols + c0) / (16 / kTokens);
       if (h >= features) continue;
       if (partial != nullptr) {
         float* o = partial + (static_cast<std::int64_t>(c[0]) * rows + t0) * features + h;
         if (add) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
+          for (int j = 0; j < kTokens; ++j)
             if (t0 + j < rows) v[j] += o[static_cast<std::int64_t>(j) * features];
         }
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
+        for (int j = 0; j < kTokens; ++j)
           if (t0 + j < rows) o[static_cast<std::int64_t>(j) * features] = v[j];
       } else {
         T* o = dx + static_cast<std::int64_t>(t0) * lddx + h;
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
+        for (int j = 0; j < kTokens; ++j)
           if (t0 + j < rows) o[j * lddx] = from_float<T>(by_row(row_scale[t0 + j], v[j]));
       }
     }
@@ -1328,6 +1374,7 @@ struct Plan {
   int rows;    // tokens per piece (the last may have fewer)
   int pieces;
   int ksplit;
+  int copies;         // rows of dz per token: 2 for kSplit
   std::int64_t ldn;   // numerators' row
   std::int64_t ldt;   // x^T's row
   std::int64_t ldp;   // row of packed copies of x and w
@@ -1344,7 +1391,6 @@ Plan plan_rows(const VocabLossArgs& a, int rows, bool sliced) {
   p.rows = rows;
   p.pieces = (a.tokens + rows - 1) / rows;
   p.ldn = round_up(a.vocab, kLine);
-  p.ldt = round_up(rows, kLine);
   p.ldp = round_up(a.features, kLine);
   p.pack_x = a.tokens > 1 ? !tma_rows_ok(a.x, a.ldx) : !aligned_to(a.x, 16);
   p.pack_w = !tma_rows_ok(a.w, a.features);
@@ -1360,7 +1406,12 @@ Plan plan_rows(const VocabLossArgs& a, int rows, bool sliced) {
     return o;
   };
   const std::size_t R = rows, H = a.features, V = a.vocab, K = a.top_k;
-  p.store = !a.gradients ? kNone : dw || !a.bf16 ? kOwn : kCommon;
+  p.store = !a.gradients           ? kNone
+            : rows <= kSplitTokens ? kSplit
+            : dw || !a.bf16        ? kOwn
+                                   : kCommon;
+  p.copies = p.store == kSplit ? 2 : 1;
+  p.ldt = round_up(p.copies * rows, kLine);
   p.stream = !a.gradients && a.tokens <= kStreamTokens && !p.pack_w;
   p.unit = p.stream ? kStreamWords : logits_tile_n(rows, a.vocab, a.gradients) / 2;
   p.units = p.stream ? sms() : (a.vocab + p.unit - 1) / p.unit;
@@ -1383,7 +1434,7 @@ Plan plan_rows(const VocabLossArgs& a, int rows, bool sliced) {
   p.row_scale = take(a.gradients ? R * sizeof(float2) : 0);
   p.xp = take(p.pack_x ? R * p.ldp * 2 : 0);
   const std::size_t wp = p.pack_w ? static_cast<std::size_t>(p.slice) * p.ldp * 2 : 0;
-  const std::size_t num = a.gradients ? R * p.ldn * 2 : 0;
+  const std::size_t num = a.gradients ? p.copies * R * p.ldn * 2 : 0;
   const std::size_t sum = dw && p.pieces > 1 ? V * round_up(a.features, 4) * 4 : 0;
   p.wp = take(wp);
   p.num = take(num);
@@ -1474,24 +1525,27 @@ cudaError_t run_logits(const LogitsProblem& p, unsigned int* timeouts, cudaStrea
   } while (0)
 
 // dx of the `words` words from word0 on (w is theirs); the slices of a call add up in partial.
-template <typename T, int FMT, bool PAIR, bool TALL>
+template <typename T, int FMT, bool PAIR, bool TALL, bool SPLIT>
 cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const void* w, std::int64_t ldw,
                    int word0, int words, const T* num, int rows, T* dx, char* ws,
                    unsigned int* to, cudaStream_t st) {
-  Dx<T, PAIR, TALL> g{};
-  g.tile_n = even_tile_n(rows);
+  using Problem = Dx<T, PAIR, TALL, SPLIT>;
+  Problem g{};
+  const int dz_rows = p.copies * rows;
+  g.tile_n = even_tile_n(dz_rows);
   if (!make_map(&g.ma, FMT, w, a.features, words, ldw, 64, 64) ||
-      !make_map(&g.mb, FMT, num + word0, words, rows, p.ldn, 64, PAIR ? g.tile_n / 2 : g.tile_n))
+      !make_map(&g.mb, FMT, num + word0, words, dz_rows, p.ldn, 64,
+                PAIR ? g.tile_n / 2 : g.tile_n))
     return cudaErrorInvalidValue;
   // splits of a whole slice; the last, shorter one has no more of them
   const auto blocks = [](int n) { return (n + tc::kBK - 1) / tc::kBK; };
   g.num_kb = (blocks(p.slice) + p.ksplit - 1) / p.ksplit;
   const int ks = (blocks(p.slice) + g.num_kb - 1) / g.num_kb;  // no split without words
-  constexpr int kRows = Dx<T, PAIR, TALL>::kRows;
+  constexpr int kRows = Problem::kRows;
   g.rows = rows;
   g.features = a.features;
   g.tiles_m = (a.features + kRows - 1) / kRows;
-  g.tiles_n = (rows + g.tile_n - 1) / g.tile_n;
+  g.tiles_n = (dz_rows + g.tile_n - 1) / g.tile_n;
   g.tiles_total = static_cast<long long>(g.tiles_m) * g.tiles_n *
                   ((blocks(words) + g.num_kb - 1) / g.num_kb);
   g.dx = dx;
@@ -1500,7 +1554,7 @@ cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const void* w, std::in
   g.partial = parts ? reinterpret_cast<float*>(ws + p.partial) : nullptr;
   g.add = word0 > 0;
   g.row_scale = reinterpret_cast<float2*>(ws + p.row_scale);
-  MB200_TRY((tc::launch_tc_epi<Dx<T, PAIR, TALL>, FMT>(g, sms(), to, st, true)));
+  MB200_TRY((tc::launch_tc_epi<Problem, FMT>(g, sms(), to, st, true)));
   if (parts && word0 + words == a.vocab) {
     const bool vec = a.features % 4 == 0 && a.lddx % 4 == 0 && aligned_to(dx, 8);
     const std::int64_t work = static_cast<std::int64_t>(rows) * a.features / (vec ? 4 : 1);
@@ -1527,11 +1581,12 @@ cudaError_t run_dw(const VocabLossArgs& a, const Plan& p, const void* num, const
   constexpr int kRows = Dw<T, TALL>::kRows;
   g.tile_n = tile_width((a.vocab + kRows - 1) / kRows, a.features, sms() / 2, g.tma ? 128 : 32,
                         true);
-  if (!make_map(&g.ma, FMT, num, a.vocab, rows, p.ldn, 64, 64) ||
-      !make_map(&g.mb, FMT, xt, rows, a.features, p.ldt, tc::kBK, g.tile_n / 2) ||
+  const int dz_rows = p.copies * rows;
+  if (!make_map(&g.ma, FMT, num, a.vocab, dz_rows, p.ldn, 64, 64) ||
+      !make_map(&g.mb, FMT, xt, dz_rows, a.features, p.ldt, tc::kBK, g.tile_n / 2) ||
       (g.tma && !make_map(&g.mdw, FMT, a.dw, a.features, a.vocab, a.features, 64, 32)))
     return cudaErrorInvalidValue;
-  g.num_kb = (rows + tc::kBK - 1) / tc::kBK;
+  g.num_kb = (dz_rows + tc::kBK - 1) / tc::kBK;
   g.vocab = a.vocab;
   g.features = a.features;
   g.tiles_m = (a.vocab + kRows - 1) / kRows;
@@ -1630,6 +1685,7 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     f.scale = scale;
     f.num = num;
     f.ldn = p.ldn;
+    f.pitch = p.copies * p.ldn;
     if (p.stream) {
       const StreamArgs sa{x, ldx, w, ldw, rows, a.features, a.vocab, kLog2e * a.inv_tau,
                           reinterpret_cast<float2*>(ws + p.stats), tg};
@@ -1642,7 +1698,7 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     LogitsProblem lp{};
     lp.tile_n = 2 * p.unit;
     if (!make_map(&lp.mx, FMT, x, a.features, rows, ldx, tc::kBK, tc::kBM) ||
-        (a.gradients && !make_map(&lp.mnum, FMT, num, p.ldn, rows, p.ldn, 64, 32)))
+        (a.gradients && !make_map(&lp.mnum, FMT, num, p.ldn, rows, p.copies * p.ldn, 64, 32)))
       return cudaErrorInvalidValue;
     lp.num_kb = (a.features + tc::kBK - 1) / tc::kBK;
     lp.rows = rows;
@@ -1693,9 +1749,10 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
       tiles = static_cast<long long>((rows + 63) / 64) * ((a.features + 63) / 64);
     }
     const long long finish = static_cast<long long>(rows) * parts;
-    if (p.store == kOwn) {
+    if (p.store == kOwn || p.store == kSplit) {
       MB200_TRY(logits(std::integral_constant<int, kOwn>{}));
-      MB200_TRY(launch(vocab_finish_kernel<T, kOwn>, finish + tiles, kFinishThreads, f));
+      MB200_TRY(launch(p.store == kOwn ? vocab_finish_kernel<T, kOwn> : vocab_finish_kernel<T, kSplit>,
+                       finish + tiles, kFinishThreads, f));
     } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
       MB200_TRY(logits(std::integral_constant<int, kCommon>{}));
       MB200_TRY(launch(vocab_finish_kernel<T, kCommon>, finish, kFinishThreads, f));
@@ -1708,9 +1765,10 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
         const auto product = [&](auto kern) {
           return kern(a, p, w, ldw, word0, words_from(word0), num, rows, dx, ws, to, st);
         };
-        MB200_TRY(product(!pair              ? run_dx<T, FMT, false, false>
-                          : dx_tall(p.slice) ? run_dx<T, FMT, true, true>
-                                             : run_dx<T, FMT, true, false>));
+        MB200_TRY(product(p.store == kSplit  ? run_dx<T, FMT, false, false, true>
+                          : !pair            ? run_dx<T, FMT, false, false, false>
+                          : dx_tall(p.slice) ? run_dx<T, FMT, true, true, false>
+                                             : run_dx<T, FMT, true, false, false>));
       }
     }
     if (a.dw != nullptr) {

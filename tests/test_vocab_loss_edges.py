@@ -473,3 +473,42 @@ def test_dx_over_a_long_vocabulary_shows_two_roundings(cuda, built, dw):
     m, e = cuda.frexp(dz)
     model = (cuda.ldexp((m * 2 ** 11).round() / 2 ** 11, e) @ w).half().double()
     assert (got - want).norm() <= 1.05 * (model - want).norm()
+
+
+def _trained(torch, T, H, V, dtype, K=0, seed=0, **more):
+    """A head whose words explain their tokens more or less, as after training."""
+    h = Head(torch, T, H, V, dtype, K=K, seed=seed, **more)
+    h.x += (12 * torch.rand(T, 1, device="cuda", generator=h.g) * h.w[h.labels].float()).to(h.x.dtype)
+    if K:
+        h.index[:, 0] = h.labels.clamp(min=0)
+    h.dloss = 0.5 + torch.rand(T, device="cuda", generator=h.g)
+    return h
+
+
+def _over_one_rounding(got, exact):
+    """Error of a 16-bit result over that of the exact one rounded once."""
+    return ((got.double() - exact).norm() / (exact.to(got.dtype).double() - exact).norm()).item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,H,V,K", [(1, 512, 5003, 0), (4, 512, 5003, 0), (4, 512, 5003, 16),
+                                     (33, 264, 20000, 0), (64, 1000, 3001, 5), (64, 505, 3001, 0)])
+def test_gradients_of_few_tokens_show_one_rounding(cuda, built, T, H, V, K, dtype):
+    """A token's one large dz would pass its rounding on to all of its dx, and to a row of dw:
+    few tokens carry what that rounding left as well.  The numerators' 2 further bits add 3 %
+    to one rounding at most."""
+    h = _trained(cuda, T, H, V, dtype, K=K, seed=T)
+    with Dnn(cuda) as d:
+        assert h.backward(d) == 0
+        cuda.cuda.synchronize()
+        ref = h.check()
+        assert _over_one_rounding(h.dx, ref["dx"]) <= 1.1
+        assert _over_one_rounding(h.dw, ref["dw"]) <= 1.1
+        assert h.backward(d, dw=False) == 0
+        cuda.cuda.synchronize()
+        assert _over_one_rounding(h.dx, ref["dx"]) <= 1.1
+        dw = h.dw.clone()
+        assert h.backward(d, dx=False) == 0
+        cuda.cuda.synchronize()
+        assert cuda.equal(h.dw, dw)
