@@ -275,9 +275,10 @@ cudnnStatus_t cudnnBatchNormalizationForwardTraining(
  * so a training step whose dloss is known needs no Forward.  dx (like x; it may be x
  * itself) or dw (like w) may be null with its descriptor: it is not computed.  Results
  * do not depend on the stream's other work: no atomics.  The gradient of the logits is
- * rounded to 16 bits on its way into both products.  In HALF it is scaled by one power of
- * two per piece of the tokens (below), so tokens whose |dloss| is 2^-20 of their piece's
- * largest or less keep fewer bits of it.
+ * rounded to 16 bits on its way into both products; what that leaves is added to both for up
+ * to 64 tokens, and to dx at the target words of tokens with up to four of them.  In HALF it
+ * is scaled by one power of two per piece of the tokens (below), so tokens whose |dloss| is
+ * 2^-20 of their piece's largest or less keep fewer bits of it.
  *
  * The workspace: null uses the handle's own (grown to what GetWorkspaceSize reports).  A
  * call runs over pieces of the tokens that need at most 2 GiB for 16-bit numerators and

@@ -9,8 +9,9 @@
 //      writes the unit's numerators 2^(z2 - the maximum's) in 16 bits;
 //   2. vocab_finish_kernel joins a token's pairs into its log-sum-exp and loss, and turns
 //      the numerators in place into dz = dloss / tau * (p - q).  Without dw (a frozen head)
-//      bf16 numerators share a power-of-two reference per token instead, and the token's
-//      factor goes into dx's epilogue: that pass over them falls away (kCommon below);
+//      bf16 numerators of more than 64 tokens share a power-of-two reference per token instead,
+//      and the token's factor goes into dx's epilogue: that pass over them falls away (kCommon
+//      below);
 //   3. Dx and Dw multiply dx = dz w and dw = dz^T x.
 // All three products run on the loop of tc_epi_core.cuh.  Scores of up to 8 tokens take
 // vocab_stream_kernel instead of 1.  Exponents are in powers of two: z2 = z * log2(e), with
@@ -31,13 +32,13 @@
 // reads of the operands (timed without them), hence the wide tiles and the banded order.
 //
 // Precision: products of the 16-bit inputs accumulate in fp32; maxima, sums, target
-// logits and losses are fp32.  dz is a 16-bit operand of the tensor cores and rounds once
-// (two of them for up to 64 tokens, see kSplit);
-// the 16 bits that carry the numerators to step 2 hold 2 more significant bits than dz
-// (OwnCode; fp32 numerators would double the piece's traffic).  The target words, whose
-// p - q cancels, are recomputed in step 2 from their fp32 logits and rounded once.  dx and
-// dw round once more at the end; their sums run in chains of MMAs whose truncation stays well
-// below that (dx_chain, kGradientRows).
+// logits and losses are fp32.  dz is a 16-bit operand of the tensor cores and rounds once; the
+// 16 bits that carry the numerators to step 2 hold 2 more significant bits than dz (OwnCode;
+// fp32 numerators would double the piece's traffic).  The target words, whose p - q cancels,
+// are recomputed in step 2 from their fp32 logits; what the rounding of their dz leaves is
+// added where it does not average out (kSplit, Left).  dx and dw round once more at the end;
+// their sums run in chains of MMAs whose truncation stays well below that (dx_chain,
+// kGradientRows).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -278,6 +279,17 @@ __device__ __forceinline__ void pick_targets(const LogitsProblem& p, const Logit
 enum StoreMode { kNone = 0, kOwn = 1, kCommon = 2, kSplit = 3 };
 constexpr int kSplitTokens = 64;
 constexpr float kCommonReach = 64.0f, kWholeReach = 0x1p22f;
+
+// Without the second row, dx alone gets what the targets' rounding left, in fp32: one entry of
+// {word, left over} per target, for tokens of up to four target words (with more the errors
+// average out).  Those words of w are read again for it, where dx is written.  dx's error over
+// one rounding 1.3-1.6 -> 1.00; loss and dx of 4096 x 2048 x 65536 1723 -> 1750 us, 1024 x 256 x
+// 65536 133 -> 138, 1315 x 1776 x 2464 55.5 -> 62.1, a step of 8192 x 4096 x 131072 the same.
+constexpr int kMostLeft = 4;
+struct Left {
+  int word;
+  float dz;
+};
 
 // kCommon's numerators of a unit with this maximum are 2^(z2 - top * scale - whole).
 struct Reference {
@@ -764,6 +776,7 @@ struct FinishArgs {
   void* num;
   std::int64_t ldn, pitch;  // words of a row of num, and from a token's row to the next's
   float2* row_scale;   // dz's row is both factors times what num holds; 0 for rows left out
+  Left* left;          // [row][max(top_k, 1)], null: not asked for
   TransposeArgs transpose;  // with dz: x^T for dw's product, in the same launch
 };
 
@@ -887,6 +900,10 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
       if (a.lse != nullptr) a.lse[row] = 0.0f;
       if constexpr (STORE != kNone) a.row_scale[row] = make_float2(0.0f, 0.0f);
     }
+    if constexpr (STORE != kNone) {
+      if (a.left != nullptr && part == 0 && threadIdx.x < max(a.targets.top_k, 1))
+        a.left[static_cast<std::int64_t>(row) * max(a.targets.top_k, 1) + threadIdx.x] = {0, 0.0f};
+    }
     if constexpr (kDz) {
       for (std::int64_t c = c_begin + threadIdx.x; c < c_end; c += kFinishThreads) {
         num[c] = make_uint4(0, 0, 0, 0);
@@ -975,23 +992,35 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     // the targets, in the numerators' units: dz, or dz / row_scale
     const float t = STORE == kCommon ? exp2f(log_sum - down) : g;
     __syncthreads();
-    const auto put = [&](std::int64_t word, float v) {
+    const auto put = [&](int word, float v) {
       T* d = reinterpret_cast<T*>(num) + word;
       *d = from_float<T>(v);
-      if constexpr (STORE == kSplit) d[a.ldn] = from_float<T>(rest(v, static_cast<float>(*d)));
+      const float r = rest(v, static_cast<float>(*d));
+      if constexpr (STORE == kSplit) d[a.ldn] = from_float<T>(r);
+      return Left{word, r};
+    };
+    // entry k, from the part that has its word; part 0 for those without one
+    const auto keep = [&](int k, Left l) {
+      if (a.left != nullptr) a.left[r0 + k] = l;
     };
     if (a.targets.top_k == 0) {
       const std::int64_t l = a.targets.labels[row];
       if (threadIdx.x == 0 && n > 0 && l >= c_begin * 8 && l < c_end * 8)
-        put(l, t * expm1f((above(r0) - log_sum) * kLn2));
+        keep(0, put(static_cast<int>(l), t * expm1f((above(r0) - log_sum) * kLn2)));
+      else if (threadIdx.x == 0 && n < 0 && part == 0)
+        keep(0, {0, 0.0f});
     } else {
-      for (int k = threadIdx.x; k < n; k += kFinishThreads) {
-        const int w = a.targets.index[r0 + k];
+      for (int k = threadIdx.x; k < tk; k += kFinishThreads) {
+        const int w = k < n ? a.targets.index[r0 + k] : -1;
+        // the first entry of a run of equal words adds all
+        if (k >= n || (k > 0 && a.targets.index[r0 + k - 1] == w)) {
+          if (part == 0) keep(k, {0, 0.0f});
+          continue;
+        }
         if (w < c_begin * 8 || w >= c_end * 8) continue;
-        if (k > 0 && a.targets.index[r0 + k - 1] == w) continue;  // the run's first entry adds all
         float q = a.targets.q[r0 + k];
         for (int j = k + 1; j < n && a.targets.index[r0 + j] == w; ++j) q += a.targets.q[r0 + j];
-        put(w, t * (exp2f(above(r0 + k) - log_sum) - q));
+        keep(k, put(w, t * (exp2f(above(r0 + k) - log_sum) - q)));
       }
     }
   }
@@ -1041,6 +1070,11 @@ __device__ __forceinline__ float by_row(float2 factor, float v) {
   return factor.x == 0.0f ? 0.0f : factor.x * v * factor.y;
 }
 
+template <typename T>
+__device__ __forceinline__ float add_left(float v, Left l, T w) {
+  return l.dz == 0.0f ? v : fmaf(l.dz, static_cast<float>(w), v);
+}
+
 // dx^T = w^T dz^T: A = w^T is MN-major in w, B = dz is K-major, the faster operand forms;
 // a thread's columns are tokens of one feature, so a warp's stores of one token are 32
 // consecutive features.  The words (K) split across `ksplit` groups of CTAs.  Pairs (more
@@ -1067,6 +1101,9 @@ struct Dx {
   float* partial;  // several splits or slices: [split][row][feature]
   bool add;        // to what an earlier slice left in partial
   const float2* row_scale;  // [row]
+  const Left* left;         // [row][lefts], 0: none; without partial sums
+  int lefts;
+  const T* w;               // all words, rows of `features`
 
   const CUtensorMap* __device__ map_a() const { return &ma; }
   const CUtensorMap* __device__ map_b() const { return &mb; }
@@ -1095,6 +1132,18 @@ struct Dx {
       }
       const int t0 = (c[2] * tile_n + half * cols + c0) / (16 / kTokens);
       if (h >= features) continue;
+      for (int m = 0; m < lefts; ++m) {
+        Left l[kTokens];
+        T x[kTokens];
+#pragma unroll
+        for (int j = 0; j < kTokens; ++j)
+          l[j] = left[static_cast<std::int64_t>(min(t0 + j, rows - 1)) * lefts + m];
+#pragma unroll
+        for (int j = 0; j < kTokens; ++j)
+          x[j] = w[static_cast<std::int64_t>(l[j].word) * features + h];
+#pragma unroll
+        for (int j = 0; j < kTokens; ++j) v[j] = add_left(v[j], l[j], x[j]);
+      }
       if (partial != nullptr) {
         float* o = partial + (static_cast<std::int64_t>(c[0]) * rows + t0) * features + h;
         if (add) {
@@ -1120,7 +1169,8 @@ struct Dx {
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
     vocab_dx_reduce_kernel(const float* __restrict__ partial, int ksplit, int rows, int features,
-                           T* __restrict__ dx, std::int64_t lddx, const float2* row_scale) {
+                           T* __restrict__ dx, std::int64_t lddx, const float2* row_scale,
+                           const Left* left, int lefts, const T* w) {
   tc::grid_launch_next();
   tc::grid_wait_previous();
   const std::int64_t plane = static_cast<std::int64_t>(rows) * features;
@@ -1139,12 +1189,22 @@ __global__ void __launch_bounds__(256)
         const float4 v = __ldcs(reinterpret_cast<const float4*>(p + k * plane));
         s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
       }
+      for (int m = 0; m < lefts; ++m) {
+        const Left l = left[r * lefts + m];
+        const T* x = w + static_cast<std::int64_t>(l.word) * features + h;
+        s = make_float4(add_left(s.x, l, x[0]), add_left(s.y, l, x[1]), add_left(s.z, l, x[2]),
+                        add_left(s.w, l, x[3]));
+      }
       *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(by_row(f, s.x), by_row(f, s.y)),
                                                 pack2<T>(by_row(f, s.z), by_row(f, s.w)));
     } else {
       float s = __ldcs(p);
 #pragma unroll 4
       for (int k = 1; k < ksplit; ++k) s += __ldcs(p + k * plane);
+      for (int m = 0; m < lefts; ++m) {
+        const Left l = left[r * lefts + m];
+        s = add_left(s, l, w[static_cast<std::int64_t>(l.word) * features + h]);
+      }
       *o = from_float<T>(by_row(f, s));
     }
   }
@@ -1380,9 +1440,10 @@ struct Plan {
   std::int64_t ldp;   // row of packed copies of x and w
   bool pack_x, pack_w;
   int slice;          // words of w that are packed at a time; without pack_w all
+  int lefts;          // entries per token of what the targets' rounding left
   // byte offsets into the workspace
-  std::size_t stats, z, index, q, count, entropy, hit, scale, row_scale, xp, wp, num, xt, partial,
-      sum, bytes;
+  std::size_t stats, z, index, q, count, entropy, hit, scale, row_scale, left, xp, wp, num, xt,
+      partial, sum, bytes;
   std::size_t rows_bytes;  // of them, what grows with the tokens, without the numerators
 };
 
@@ -1432,6 +1493,8 @@ Plan plan_rows(const VocabLossArgs& a, int rows, bool sliced) {
   p.hit = take(K > 0 ? R * p.hit_units * 4 : 0);
   p.scale = take(8);
   p.row_scale = take(a.gradients ? R * sizeof(float2) : 0);
+  p.lefts = dx && p.store != kSplit && K <= kMostLeft ? std::max(a.top_k, 1) : 0;
+  p.left = take(R * p.lefts * sizeof(Left));
   p.xp = take(p.pack_x ? R * p.ldp * 2 : 0);
   const std::size_t wp = p.pack_w ? static_cast<std::size_t>(p.slice) * p.ldp * 2 : 0;
   const std::size_t num = a.gradients ? p.copies * R * p.ldn * 2 : 0;
@@ -1526,7 +1589,7 @@ cudaError_t run_logits(const LogitsProblem& p, unsigned int* timeouts, cudaStrea
 
 // dx of the `words` words from word0 on (w is theirs); the slices of a call add up in partial.
 template <typename T, int FMT, bool PAIR, bool TALL, bool SPLIT>
-cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const void* w, std::int64_t ldw,
+cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const T* w, std::int64_t ldw,
                    int word0, int words, const T* num, int rows, T* dx, char* ws,
                    unsigned int* to, cudaStream_t st) {
   using Problem = Dx<T, PAIR, TALL, SPLIT>;
@@ -1554,6 +1617,9 @@ cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const void* w, std::in
   g.partial = parts ? reinterpret_cast<float*>(ws + p.partial) : nullptr;
   g.add = word0 > 0;
   g.row_scale = reinterpret_cast<float2*>(ws + p.row_scale);
+  g.left = reinterpret_cast<const Left*>(ws + p.left);
+  g.lefts = parts ? 0 : p.lefts;
+  g.w = static_cast<const T*>(a.w);
   MB200_TRY((tc::launch_tc_epi<Problem, FMT>(g, sms(), to, st, true)));
   if (parts && word0 + words == a.vocab) {
     const bool vec = a.features % 4 == 0 && a.lddx % 4 == 0 && aligned_to(dx, 8);
@@ -1562,7 +1628,7 @@ cudaError_t run_dx(const VocabLossArgs& a, const Plan& p, const void* w, std::in
         static_cast<unsigned>(std::min<std::int64_t>((work + 255) / 256, sms() * 32));
     MB200_TRY(tc::launch_overlapped(
         vec ? vocab_dx_reduce_kernel<T, 4> : vocab_dx_reduce_kernel<T, 1>, dim3(grid), 256, 0, st, true,
-        g.partial, ks, rows, a.features, dx, a.lddx, g.row_scale));
+        g.partial, ks, rows, a.features, dx, a.lddx, g.row_scale, g.left, p.lefts, g.w));
   }
   return cudaSuccess;
 }
@@ -1741,6 +1807,7 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     }
     f.dloss = a.dloss + t0;
     f.row_scale = reinterpret_cast<float2*>(ws + p.row_scale);
+    f.left = p.lefts > 0 ? reinterpret_cast<Left*>(ws + p.left) : nullptr;
     f.parts = parts;
     T* xt = reinterpret_cast<T*>(ws + p.xt);
     long long tiles = 0;

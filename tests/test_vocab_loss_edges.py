@@ -512,3 +512,29 @@ def test_gradients_of_few_tokens_show_one_rounding(cuda, built, T, H, V, K, dtyp
         assert h.backward(d, dx=False) == 0
         cuda.cuda.synchronize()
         assert cuda.equal(h.dw, dw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,H,V,K", [(100, 512, 20011, 0), (300, 520, 20011, 0), (300, 136, 1500, 3),
+                                     (2000, 512, 2500, 0), (300, 513, 60001, 2)])
+def test_dx_of_few_targets_shows_one_rounding(cuda, built, T, H, V, K, dtype):
+    """dx of up to four target words per token gets what the rounding of their dz left, on flat,
+    tall and single-CTA tiles, in one sum and in several, with dw and for a frozen head.  The
+    other words' roundings average out."""
+    h = _trained(cuda, T, H, V, dtype, K=K, seed=T, out=0.1)
+    with Dnn(cuda) as d:
+        for dw in (True, False):
+            h.dx.fill_(math.nan)
+            assert h.backward(d, dw=dw) == 0
+            cuda.cuda.synchronize()
+            ref = h.check(dw=dw)
+            assert _over_one_rounding(h.dx, ref["dx"]) <= 1.1
+        h.w = _moved(cuda, h.w, 1)  # w copied, in slices where there are more than 16 MiB
+        ws = cuda.empty(h.workspace_size(d, 1) - (V * (H + 63) // 64 * 128 if H % 8 else 0)
+                        + (17 << 20), device="cuda", dtype=cuda.uint8)
+        h.dx.fill_(math.nan)
+        assert h.backward(d, ws) == 0
+        cuda.cuda.synchronize()
+        h.check()
+        assert _over_one_rounding(h.dx, ref["dx"]) <= 1.1
