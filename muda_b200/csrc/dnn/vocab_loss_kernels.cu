@@ -26,7 +26,7 @@
 // them to 2 GiB whatever T is, and whatever V is up to the 8 million words where 128 tokens,
 // the least piece, reach that.
 //
-// What bounds a training step of 8192 x 4096 x 131072 (20.1 ms, 1313 TFLOP/s): the power
+// What bounds a training step of 8192 x 4096 x 131072 (20.3 ms, 1301 TFLOP/s): the power
 // cap.  The tensor pipe is busy 95 % of the cycles at 1.15-1.4 GHz.  Of a 1546 us score of
 // 2048 x 4096 x 131072 under the cap, 100 us go with the DRAM reads and 155 us with the L2
 // reads of the operands (timed without them), hence the wide tiles and the banded order.
