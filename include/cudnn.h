@@ -327,6 +327,115 @@ cudnnStatus_t cudnnLinearDistillationBackward(cudnnHandle_t handle, cudnnTensorD
                                               float* logSumExp, cudnnTensorDescriptor_t dxDesc,
                                               void* dx, cudnnFilterDescriptor_t dwDesc, void* dw);
 
+/* Losses of post-training on the same head (extensions).  nll[t] is the cross entropy above,
+ * the negative log-probability of the label; x, w, labels, the workspace, streams and capture
+ * are as above, and so is a token that a negative label leaves out: 0 in every output, no
+ * gradient, whatever the other inputs hold there.  All float arrays are fp32.
+ *
+ * Policy loss, per token, z = x w^T / temperature:
+ *   ratio = exp(oldNll - nll)            oldNll null: 1, and its gradient as if it were nll
+ *   gain  = min(ratio A, clip(ratio, 1 - clipLow, 1 + clipHigh) A)    A = advantages[t]
+ *           where A < 0 and dualClip >= 1 (0: off): max(gain, dualClip A)
+ *   kl    = exp(d) - d - 1, d = nll - refNll                refNll null: 0, klCoef 0
+ *   loss  = klCoef kl - gain
+ * The gradient is that of the side that min (or max) took, of ratio A where they are equal.
+ * A token whose advantage is 0 has gain 0 at any ratio.  clipLow is 0 to 1, clipHigh, dualClip
+ * and klCoef at most 2^64.
+ *
+ * Preference loss of pairs of sequences: sequence s holds the rows offsets[s] to
+ * offsets[s + 1] - 1 (int64 on the device, 2 * pairs + 1 of them, ascending from 0 at least to T at
+ * most); sequence p is the chosen one of pair p, pairs + p the rejected one.
+ *   L[s] = sum of refNll - nll over the tokens of s that are not left out (refNll null: 0),
+ *          with `averaged` divided by their number
+ *   h    = beta (L[p] - L[pairs + p]) - margin
+ *   loss[p] = SIGMOID: softplus(-h) + labelSmoothing h; HINGE: max(0, 1 - h);
+ *             SQUARED: ((h - 1/2) / beta)^2
+ *   rewards[s] = beta L[s]
+ * beta is 2^-64 to 2^64, labelSmoothing 0 to 1/2 and 0 for the other modes.  A pair with a
+ * sequence of which no token is kept is left out: loss and rewards 0, no gradient.  Rows of no
+ * sequence have an nll and no gradient.  A pair whose offsets do not ascend within 0..T has NaN
+ * for its loss and rewards and no gradient of its own.
+ *
+ * A label of V or more makes its token's outputs NaN, its pair's, and the gradients they enter.
+ * Every output may be null (Forward: not all of them).  Backward computes the outputs too, and
+ * the gradients of sum dloss * loss: dloss holds T floats for a policy loss, `pairs` for a
+ * preference loss.  Logits are computed once, but for preference gradients of more tokens than
+ * one piece has (see the workspace above): a pair's loss takes all its tokens, so each piece's
+ * logits are computed again after them.  Preference losses keep up to 8 bytes of workspace per
+ * token besides. */
+typedef enum {
+  CUDNN_PREFERENCE_SIGMOID = 0,
+  CUDNN_PREFERENCE_HINGE = 1,
+  CUDNN_PREFERENCE_SQUARED = 2,
+} cudnnPreferenceMode_t;
+
+cudnnStatus_t cudnnGetLinearPolicyLossWorkspaceSize(cudnnHandle_t handle,
+                                                    cudnnTensorDescriptor_t xDesc,
+                                                    cudnnFilterDescriptor_t wDesc, int gradients,
+                                                    size_t* sizeInBytes);
+cudnnStatus_t cudnnLinearPolicyLossForward(
+    cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc, const void* x,
+    cudnnFilterDescriptor_t wDesc, const void* w, const int64_t* labels, const float* oldNll,
+    const float* refNll, const float* advantages, double temperature, double clipLow,
+    double clipHigh, double dualClip, double klCoef, void* workSpace, size_t workSpaceSizeInBytes,
+    float* loss, float* nll, float* ratio, float* kl);
+cudnnStatus_t cudnnLinearPolicyLossBackward(
+    cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc, const void* x,
+    cudnnFilterDescriptor_t wDesc, const void* w, const int64_t* labels, const float* oldNll,
+    const float* refNll, const float* advantages, double temperature, double clipLow,
+    double clipHigh, double dualClip, double klCoef, const float* dloss, void* workSpace,
+    size_t workSpaceSizeInBytes, float* loss, float* nll, float* ratio, float* kl,
+    cudnnTensorDescriptor_t dxDesc, void* dx, cudnnFilterDescriptor_t dwDesc, void* dw);
+cudnnStatus_t cudnnGetLinearPreferenceLossWorkspaceSize(cudnnHandle_t handle,
+                                                        cudnnTensorDescriptor_t xDesc,
+                                                        cudnnFilterDescriptor_t wDesc,
+                                                        int gradients, size_t* sizeInBytes);
+cudnnStatus_t cudnnLinearPreferenceLossForward(
+    cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc, const void* x,
+    cudnnFilterDescriptor_t wDesc, const void* w, const int64_t* labels, int pairs,
+    const int64_t* offsets, const float* refNll, cudnnPreferenceMode_t mode, int averaged,
+    double beta, double margin, double labelSmoothing, void* workSpace,
+    size_t workSpaceSizeInBytes, float* loss, float* rewards, float* nll);
+cudnnStatus_t cudnnLinearPreferenceLossBackward(
+    cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc, const void* x,
+    cudnnFilterDescriptor_t wDesc, const void* w, const int64_t* labels, int pairs,
+    const int64_t* offsets, const float* refNll, cudnnPreferenceMode_t mode, int averaged,
+    double beta, double margin, double labelSmoothing, const float* dloss, void* workSpace,
+    size_t workSpaceSizeInBytes, float* loss, float* rewards, float* nll,
+    cudnnTensorDescriptor_t dxDesc, void* dx, cudnnFilterDescriptor_t dwDesc, void* dw);
+
+/* Embeddings (extensions): a table w of V words, a 1x1 filter (k = V, c = H features) as for
+ * the head above, and tokens (int64, one per row of y or dy; rows as x above).
+ *
+ *   Forward    y[t] = alpha w[tokens[t]] + beta y[t]
+ *   Backward   dw[v] = alpha sum of dy[t] over the rows with tokens[t] == v, + beta dw[v]
+ *
+ * Table and rows are of one type (FLOAT, HALF or BFLOAT16), or a FLOAT table has 16-bit rows.
+ * alpha and beta are floats on the host; beta 0 does not read y or dw; sums are fp32 and round
+ * once.  Backward with beta 1 touches only the rows of words that occur (the second micro-batch
+ * of a step, or a table that is also the head, whose dw the losses above have written), others
+ * write all V rows.
+ *
+ * A negative token (padding) stands for a row of zeros: y[t] = beta y[t], and its dy is not
+ * read.  A token of V or more makes its row of y NaN and enters no gradient.  A word's rows are
+ * added in the order of their positions, without atomics: results are the same on every run.
+ *
+ * Backward's workspace: null uses the handle's own, ordered and captured as for the losses
+ * above; GetWorkspaceSize reports what a given one (aligned to 256 bytes) needs. */
+cudnnStatus_t cudnnEmbeddingForward(cudnnHandle_t handle, const void* alpha,
+                                    cudnnFilterDescriptor_t wDesc, const void* w,
+                                    const int64_t* tokens, const void* beta,
+                                    cudnnTensorDescriptor_t yDesc, void* y);
+cudnnStatus_t cudnnGetEmbeddingBackwardWorkspaceSize(cudnnHandle_t handle,
+                                                     cudnnTensorDescriptor_t dyDesc,
+                                                     cudnnFilterDescriptor_t dwDesc,
+                                                     size_t* sizeInBytes);
+cudnnStatus_t cudnnEmbeddingBackward(cudnnHandle_t handle, const void* alpha,
+                                     cudnnTensorDescriptor_t dyDesc, const void* dy,
+                                     const int64_t* tokens, void* workSpace,
+                                     size_t workSpaceSizeInBytes, const void* beta,
+                                     cudnnFilterDescriptor_t dwDesc, void* dw);
+
 #ifdef __cplusplus
 }
 #endif

@@ -100,6 +100,9 @@ CUDNN_CROSS_CORRELATION = 1
 CUDNN_SOFTMAX_FAST = 0
 CUDNN_SOFTMAX_ACCURATE = 1
 CUDNN_SOFTMAX_LOG = 2
+CUDNN_PREFERENCE_SIGMOID = 0
+CUDNN_PREFERENCE_HINGE = 1
+CUDNN_PREFERENCE_SQUARED = 2
 CUDNN_SOFTMAX_MODE_INSTANCE = 0
 CUDNN_SOFTMAX_MODE_CHANNEL = 1
 CUDNN_ACTIVATION_SIGMOID, CUDNN_ACTIVATION_RELU, CUDNN_ACTIVATION_TANH = 0, 1, 2
@@ -163,6 +166,17 @@ CUDNN_PROTOS = {
                                         vp], i32),
     "cudnnLinearDistillationBackward": ([vp, vp, vp, vp, vp, i32, vp, vp, C.c_double, vp, vp, sz,
                                          vp, vp, vp, vp, vp, vp], i32),
+    "cudnnGetLinearPolicyLossWorkspaceSize": ([vp, vp, vp, i32, P(sz)], i32),
+    "cudnnLinearPolicyLossForward": ([vp] * 9 + [C.c_double] * 5 + [vp, sz] + [vp] * 4, i32),
+    "cudnnLinearPolicyLossBackward": ([vp] * 9 + [C.c_double] * 5 + [vp, vp, sz] + [vp] * 8, i32),
+    "cudnnGetLinearPreferenceLossWorkspaceSize": ([vp, vp, vp, i32, P(sz)], i32),
+    "cudnnLinearPreferenceLossForward": ([vp] * 6 + [i32, vp, vp, i32, i32] + [C.c_double] * 3
+                                         + [vp, sz] + [vp] * 3, i32),
+    "cudnnLinearPreferenceLossBackward": ([vp] * 6 + [i32, vp, vp, i32, i32] + [C.c_double] * 3
+                                          + [vp, vp, sz] + [vp] * 7, i32),
+    "cudnnEmbeddingForward": ([vp] * 8, i32),
+    "cudnnGetEmbeddingBackwardWorkspaceSize": ([vp, vp, vp, P(sz)], i32),
+    "cudnnEmbeddingBackward": ([vp] * 6 + [sz, vp, vp, vp], i32),
 }
 
 

@@ -29,6 +29,7 @@
 #include "common/lru.hpp"
 #include "common/registry.hpp"
 #include "dnn/dnn.hpp"
+#include "dnn/embedding.hpp"
 #include "dnn/vocab_loss.hpp"
 
 namespace {
@@ -1093,6 +1094,7 @@ cudnnStatus_t cudnnBatchNormalizationForwardTraining(
 // --------------------------------------------------------------- vocabulary losses --
 namespace {
 
+using mb200::dnn::HeadLoss;
 using mb200::dnn::VocabLossArgs;
 
 // The (n, h, w) positions of a descriptor as rows of c contiguous elements, `ld` apart.
@@ -1134,8 +1136,8 @@ cudnnStatus_t vocab_head(TensorDesc& xd, FilterDesc& wd, VocabLossArgs* a) {
 }
 
 cudnnStatus_t vocab_workspace(cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc,
-                              cudnnFilterDescriptor_t wDesc, int topK, int gradients,
-                              std::size_t* size) {
+                              cudnnFilterDescriptor_t wDesc, int topK, HeadLoss head,
+                              int gradients, std::size_t* size) {
   if (size == nullptr) return CUDNN_STATUS_BAD_PARAM;
   auto h = handles().get(handle);
   auto xd = tensors().get(xDesc);
@@ -1145,6 +1147,7 @@ cudnnStatus_t vocab_workspace(cudnnHandle_t handle, cudnnTensorDescriptor_t xDes
   const cudnnStatus_t s = vocab_head(*xd, *wd, &a);
   if (s != CUDNN_STATUS_SUCCESS) return s;
   a.top_k = topK;
+  a.head = head;
   a.gradients = gradients != 0;
   // both gradients, and operands at any address
   if (a.gradients) a.dx = a.dw = reinterpret_cast<void*>(std::uintptr_t{256});
@@ -1184,28 +1187,50 @@ std::size_t row_span(std::int64_t rows, std::int64_t ld, int c) {
 cudnnStatus_t vocab_run(DnnContext& h, const VocabLossArgs& a, void* workSpace,
                         std::size_t workSpaceSize) {
   const std::size_t T = a.tokens, V = a.vocab, H = a.features, K = a.top_k;
-  const Span x{a.x, row_span(a.tokens, a.ldx, a.features)}, w{a.w, V * H * 2};
-  const Span labels{a.labels, K == 0 ? T * 8 : 0}, index{a.teacher_index, T * K * 8};
-  const Span teacher{a.teacher_logits, T * K * 4};
-  const Span dloss{a.dloss, a.gradients ? T * 4 : 0};
-  const Span loss{a.loss, a.loss != nullptr ? T * 4 : 0}, lse{a.lse, a.lse != nullptr ? T * 4 : 0};
+  const std::size_t P = a.head == HeadLoss::kPreference ? a.preference.pairs : 0;
+  const std::size_t losses = P > 0 ? P : T;
+  const auto floats = [](const float* p, std::size_t n) {
+    return Span{p, p != nullptr ? n * 4 : 0};
+  };
+  const Span x{a.x, row_span(a.tokens, a.ldx, a.features)};
   const Span dx{a.dx, a.dx != nullptr ? row_span(a.tokens, a.lddx, a.features) : 0};
-  const Span dw{a.dw, a.dw != nullptr ? V * H * 2 : 0};
-  const Span ws{workSpace, workSpace != nullptr ? workSpaceSize : 0};
-  for (const auto& [s, align] : {std::pair<Span, std::size_t>{x, 2}, {w, 2}, {labels, 8},
-                                 {index, 8}, {teacher, 4}, {dloss, 4}, {loss, 4}, {lse, 4},
-                                 {dx, 2}, {dw, 2}, {ws, 256}}) {
-    if (s.bytes == 0) continue;
-    if (!mb200::aligned_to(s.p, align) || !mb200::device_span_ok(s.p, s.bytes))
-      return CUDNN_STATUS_BAD_PARAM;
-  }
-  const Span in[] = {x, w, labels, index, teacher, dloss};
-  const Span out[] = {loss, lse, dw, ws, dx};
-  for (int i = 0; i < 5; ++i) {
-    for (int j = 0; j < i; ++j)
-      if (overlap(out[i], out[j])) return CUDNN_STATUS_BAD_PARAM;
-    for (int j = 0; j < 6; ++j)
-      if (!(i == 4 && j == 0) && overlap(out[i], in[j])) return CUDNN_STATUS_BAD_PARAM;
+  // x and dx first: they alone may share memory
+  const std::pair<Span, std::size_t> in[] = {
+      {x, 2},
+      {{a.w, V * H * 2}, 2},
+      {{a.labels, K == 0 ? T * 8 : 0}, 8},
+      {{a.teacher_index, T * K * 8}, 8},
+      {{a.teacher_logits, T * K * 4}, 4},
+      {{a.dloss, a.gradients ? losses * 4 : 0}, 4},
+      {floats(a.policy.old_nll, T), 4},
+      {floats(a.policy.ref_nll, T), 4},
+      {floats(a.policy.advantage, T), 4},
+      {{a.preference.offsets, P > 0 ? (2 * P + 1) * 8 : 0}, 8},
+      {floats(a.preference.ref_nll, T), 4}};
+  const std::pair<Span, std::size_t> out[] = {
+      {dx, 2},
+      {floats(a.loss, T), 4},
+      {floats(a.lse, T), 4},
+      {{a.dw, a.dw != nullptr ? V * H * 2 : 0}, 2},
+      {{workSpace, workSpace != nullptr ? workSpaceSize : 0}, 256},
+      {floats(a.policy.loss, T), 4},
+      {floats(a.policy.ratio, T), 4},
+      {floats(a.policy.kl, T), 4},
+      {floats(a.preference.loss, P), 4},
+      {floats(a.preference.rewards, 2 * P), 4}};
+  const auto usable = [](const std::pair<Span, std::size_t>& s) {
+    return s.first.bytes == 0 || (mb200::aligned_to(s.first.p, s.second) &&
+                                  mb200::device_span_ok(s.first.p, s.first.bytes));
+  };
+  for (const auto& s : in)
+    if (!usable(s)) return CUDNN_STATUS_BAD_PARAM;
+  for (const auto& s : out)
+    if (!usable(s)) return CUDNN_STATUS_BAD_PARAM;
+  for (const auto& o : out) {
+    for (const auto* p = out; p != &o; ++p)
+      if (overlap(o.first, p->first)) return CUDNN_STATUS_BAD_PARAM;
+    for (const auto& i : in)
+      if (!(&o == out && &i == in) && overlap(o.first, i.first)) return CUDNN_STATUS_BAD_PARAM;
   }
   if (!rows_compatible(a, x, dx)) return CUDNN_STATUS_BAD_PARAM;
   const cudaStream_t st = stream_of(h);
@@ -1219,7 +1244,7 @@ cudnnStatus_t vocab_run(DnnContext& h, const VocabLossArgs& a, void* workSpace,
   });
 }
 
-// Argument checks shared by the four calls; `fill` sets the targets.
+// Argument checks shared by the losses' calls; `fill` sets what a loss has of its own.
 template <class Fill>
 cudnnStatus_t vocab_call(cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc, const void* x,
                          cudnnFilterDescriptor_t wDesc, const void* w, bool gradients,
@@ -1228,7 +1253,6 @@ cudnnStatus_t vocab_call(cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc, co
                          cudnnFilterDescriptor_t dwDesc, void* dw, Fill&& fill) {
   try {
     if (x == nullptr || w == nullptr) return CUDNN_STATUS_BAD_PARAM;
-    if (!gradients && loss == nullptr && lse == nullptr) return CUDNN_STATUS_BAD_PARAM;
     if (gradients && (dloss == nullptr || (dx == nullptr && dw == nullptr)))
       return CUDNN_STATUS_BAD_PARAM;
     auto h = handles().get(handle);
@@ -1246,6 +1270,10 @@ cudnnStatus_t vocab_call(cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc, co
     a.gradients = gradients;
     a.dloss = dloss;
     if (!fill(a)) return CUDNN_STATUS_BAD_PARAM;
+    if (!gradients && a.loss == nullptr && a.lse == nullptr && a.policy.loss == nullptr &&
+        a.policy.ratio == nullptr && a.policy.kl == nullptr && a.preference.loss == nullptr &&
+        a.preference.rewards == nullptr)
+      return CUDNN_STATUS_BAD_PARAM;  // nothing to compute
     if (dx != nullptr) {
       auto dxd = tensors().get(dxDesc);
       if (!dxd) return CUDNN_STATUS_BAD_PARAM;
@@ -1278,16 +1306,71 @@ bool fill_labels(VocabLossArgs& a, const std::int64_t* labels) {
   return labels != nullptr;
 }
 
+// 2^-64..2^64: the fp32 reciprocal and its products with log2(e) stay normal
+bool fill_temperature(VocabLossArgs& a, double temperature) {
+  a.inv_tau = static_cast<float>(1.0 / temperature);
+  return temperature >= 0x1p-64 && temperature <= 0x1p64;
+}
+
 bool fill_teacher(VocabLossArgs& a, int topK, const std::int64_t* index, const float* logits,
                   double temperature) {
   if (topK < 1 || topK > mb200::dnn::kVocabMaxTopK || index == nullptr || logits == nullptr)
     return false;
-  // 2^-64..2^64: the fp32 reciprocal and its products with log2(e) stay normal
-  if (!(temperature >= 0x1p-64 && temperature <= 0x1p64)) return false;
   a.top_k = topK;
   a.teacher_index = index;
   a.teacher_logits = logits;
-  a.inv_tau = static_cast<float>(1.0 / temperature);
+  return fill_temperature(a, temperature);
+}
+
+// 2^-64 to 2^64, a bound of the products that a single float takes part in.
+constexpr double kMostFactor = 0x1p64;
+
+bool fill_policy(VocabLossArgs& a, const std::int64_t* labels, const float* old_nll,
+                 const float* ref_nll, const float* advantages, double temperature, double low,
+                 double high, double dual, double kl_coef, float* loss, float* ratio, float* kl) {
+  if (advantages == nullptr || !fill_labels(a, labels) || !fill_temperature(a, temperature))
+    return false;
+  if (!(low >= 0.0 && low <= 1.0 && high >= 0.0 && high <= kMostFactor)) return false;
+  if (!(dual == 0.0 || (dual >= 1.0 && dual <= kMostFactor))) return false;
+  if (!(kl_coef >= 0.0 && kl_coef <= kMostFactor)) return false;
+  if (ref_nll == nullptr && (kl_coef > 0.0 || kl != nullptr)) return false;
+  a.head = HeadLoss::kPolicy;
+  a.policy = {old_nll,
+              ref_nll,
+              advantages,
+              static_cast<float>(1.0 - low),
+              static_cast<float>(1.0 + high),
+              static_cast<float>(dual),
+              static_cast<float>(kl_coef),
+              loss,
+              ratio,
+              kl};
+  return true;
+}
+
+bool fill_preference(VocabLossArgs& a, const std::int64_t* labels, int pairs,
+                     const std::int64_t* offsets, const float* ref_nll,
+                     cudnnPreferenceMode_t mode, int averaged, double beta, double margin,
+                     double smoothing, float* loss, float* rewards) {
+  if (pairs < 1 || pairs > (1 << 29) || offsets == nullptr || !fill_labels(a, labels)) return false;
+  if (mode != CUDNN_PREFERENCE_SIGMOID && mode != CUDNN_PREFERENCE_HINGE &&
+      mode != CUDNN_PREFERENCE_SQUARED)
+    return false;
+  if (!(beta >= 1.0 / kMostFactor && beta <= kMostFactor)) return false;
+  if (!(margin >= -kMostFactor && margin <= kMostFactor)) return false;
+  if (!(smoothing >= 0.0 && smoothing <= (mode == CUDNN_PREFERENCE_SIGMOID ? 0.5 : 0.0)))
+    return false;
+  a.head = HeadLoss::kPreference;
+  a.preference = {pairs,
+                  offsets,
+                  ref_nll,
+                  static_cast<mb200::dnn::PreferenceMode>(mode),
+                  averaged != 0,
+                  beta,
+                  margin,
+                  smoothing,
+                  loss,
+                  rewards};
   return true;
 }
 
@@ -1299,7 +1382,7 @@ cudnnStatus_t cudnnGetLinearCrossEntropyWorkspaceSize(cudnnHandle_t handle,
                                                       cudnnTensorDescriptor_t xDesc,
                                                       cudnnFilterDescriptor_t wDesc, int gradients,
                                                       size_t* sizeInBytes) {
-  return vocab_workspace(handle, xDesc, wDesc, 0, gradients, sizeInBytes);
+  return vocab_workspace(handle, xDesc, wDesc, 0, HeadLoss::kTargets, gradients, sizeInBytes);
 }
 
 cudnnStatus_t cudnnLinearCrossEntropyForward(cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc,
@@ -1329,7 +1412,7 @@ cudnnStatus_t cudnnGetLinearDistillationWorkspaceSize(cudnnHandle_t handle,
                                                       cudnnFilterDescriptor_t wDesc, int topK,
                                                       int gradients, size_t* sizeInBytes) {
   if (topK < 1 || topK > mb200::dnn::kVocabMaxTopK) return CUDNN_STATUS_BAD_PARAM;
-  return vocab_workspace(handle, xDesc, wDesc, topK, gradients, sizeInBytes);
+  return vocab_workspace(handle, xDesc, wDesc, topK, HeadLoss::kTargets, gradients, sizeInBytes);
 }
 
 cudnnStatus_t cudnnLinearDistillationForward(cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc,
@@ -1356,6 +1439,196 @@ cudnnStatus_t cudnnLinearDistillationBackward(cudnnHandle_t handle, cudnnTensorD
                     logSumExp, dxDesc, dx, dwDesc, dw, [&](VocabLossArgs& a) {
                       return fill_teacher(a, topK, teacherIndex, teacherLogits, temperature);
                     });
+}
+
+cudnnStatus_t cudnnGetLinearPolicyLossWorkspaceSize(cudnnHandle_t handle,
+                                                    cudnnTensorDescriptor_t xDesc,
+                                                    cudnnFilterDescriptor_t wDesc, int gradients,
+                                                    size_t* sizeInBytes) {
+  return vocab_workspace(handle, xDesc, wDesc, 0, HeadLoss::kPolicy, gradients, sizeInBytes);
+}
+
+cudnnStatus_t cudnnLinearPolicyLossForward(
+    cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc, const void* x,
+    cudnnFilterDescriptor_t wDesc, const void* w, const int64_t* labels, const float* oldNll,
+    const float* refNll, const float* advantages, double temperature, double clipLow,
+    double clipHigh, double dualClip, double klCoef, void* workSpace, size_t workSpaceSizeInBytes,
+    float* loss, float* nll, float* ratio, float* kl) {
+  return vocab_call(handle, xDesc, x, wDesc, w, false, nullptr, workSpace, workSpaceSizeInBytes,
+                    nll, nullptr, nullptr, nullptr, nullptr, nullptr, [&](VocabLossArgs& a) {
+                      return fill_policy(a, labels, oldNll, refNll, advantages, temperature,
+                                         clipLow, clipHigh, dualClip, klCoef, loss, ratio, kl);
+                    });
+}
+
+cudnnStatus_t cudnnLinearPolicyLossBackward(
+    cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc, const void* x,
+    cudnnFilterDescriptor_t wDesc, const void* w, const int64_t* labels, const float* oldNll,
+    const float* refNll, const float* advantages, double temperature, double clipLow,
+    double clipHigh, double dualClip, double klCoef, const float* dloss, void* workSpace,
+    size_t workSpaceSizeInBytes, float* loss, float* nll, float* ratio, float* kl,
+    cudnnTensorDescriptor_t dxDesc, void* dx, cudnnFilterDescriptor_t dwDesc, void* dw) {
+  return vocab_call(handle, xDesc, x, wDesc, w, true, dloss, workSpace, workSpaceSizeInBytes, nll,
+                    nullptr, dxDesc, dx, dwDesc, dw, [&](VocabLossArgs& a) {
+                      return fill_policy(a, labels, oldNll, refNll, advantages, temperature,
+                                         clipLow, clipHigh, dualClip, klCoef, loss, ratio, kl);
+                    });
+}
+
+cudnnStatus_t cudnnGetLinearPreferenceLossWorkspaceSize(cudnnHandle_t handle,
+                                                        cudnnTensorDescriptor_t xDesc,
+                                                        cudnnFilterDescriptor_t wDesc,
+                                                        int gradients, size_t* sizeInBytes) {
+  return vocab_workspace(handle, xDesc, wDesc, 0, HeadLoss::kPreference, gradients, sizeInBytes);
+}
+
+cudnnStatus_t cudnnLinearPreferenceLossForward(
+    cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc, const void* x,
+    cudnnFilterDescriptor_t wDesc, const void* w, const int64_t* labels, int pairs,
+    const int64_t* offsets, const float* refNll, cudnnPreferenceMode_t mode, int averaged,
+    double beta, double margin, double labelSmoothing, void* workSpace,
+    size_t workSpaceSizeInBytes, float* loss, float* rewards, float* nll) {
+  return vocab_call(handle, xDesc, x, wDesc, w, false, nullptr, workSpace, workSpaceSizeInBytes,
+                    nll, nullptr, nullptr, nullptr, nullptr, nullptr, [&](VocabLossArgs& a) {
+                      return fill_preference(a, labels, pairs, offsets, refNll, mode, averaged,
+                                             beta, margin, labelSmoothing, loss, rewards);
+                    });
+}
+
+cudnnStatus_t cudnnLinearPreferenceLossBackward(
+    cudnnHandle_t handle, cudnnTensorDescriptor_t xDesc, const void* x,
+    cudnnFilterDescriptor_t wDesc, const void* w, const int64_t* labels, int pairs,
+    const int64_t* offsets, const float* refNll, cudnnPreferenceMode_t mode, int averaged,
+    double beta, double margin, double labelSmoothing, const float* dloss, void* workSpace,
+    size_t workSpaceSizeInBytes, float* loss, float* rewards, float* nll,
+    cudnnTensorDescriptor_t dxDesc, void* dx, cudnnFilterDescriptor_t dwDesc, void* dw) {
+  return vocab_call(handle, xDesc, x, wDesc, w, true, dloss, workSpace, workSpaceSizeInBytes, nll,
+                    nullptr, dxDesc, dx, dwDesc, dw, [&](VocabLossArgs& a) {
+                      return fill_preference(a, labels, pairs, offsets, refNll, mode, averaged,
+                                             beta, margin, labelSmoothing, loss, rewards);
+                    });
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------- embeddings --
+namespace {
+
+using mb200::dnn::EmbeddingArgs;
+using mb200::dnn::EmbeddingType;
+
+EmbeddingType embedding_type(cudnnDataType_t t) {
+  return t == CUDNN_DATA_FLOAT  ? EmbeddingType::kF32
+         : t == CUDNN_DATA_HALF ? EmbeddingType::kF16
+                                : EmbeddingType::kBF16;
+}
+
+// Sizes and types of a table and of its tokens' rows.
+cudnnStatus_t embedding_shape(TensorDesc& rows, FilterDesc& table, EmbeddingArgs* a) {
+  const TensorSnap r = snap(rows);
+  const FilterSnap f = snap(table);
+  if (!r.configured || !f.configured || f.h != 1 || f.w != 1 || f.c != r.v.c)
+    return CUDNN_STATUS_BAD_PARAM;
+  if (f.dtype != r.dtype && f.dtype != CUDNN_DATA_FLOAT) return CUDNN_STATUS_NOT_SUPPORTED;
+  std::int64_t n;
+  if (!rows_of(r.v, &n, &a->ld)) return CUDNN_STATUS_NOT_SUPPORTED;
+  if (n > (1 << 30) || f.k > (1 << 30)) return CUDNN_STATUS_NOT_SUPPORTED;
+  a->table = embedding_type(f.dtype);
+  a->rows = embedding_type(r.dtype);
+  a->tokens = static_cast<int>(n);
+  a->features = f.c;
+  a->vocab = f.k;
+  return CUDNN_STATUS_SUCCESS;
+}
+
+// Argument checks shared by both calls; `gradient`: rows are dy, w is dw.
+cudnnStatus_t embedding_call(cudnnHandle_t handle, const void* alpha, const void* beta,
+                             cudnnTensorDescriptor_t rowsDesc, const void* rows,
+                             cudnnFilterDescriptor_t tableDesc, const void* table,
+                             const std::int64_t* tokens, bool gradient, void* workSpace,
+                             std::size_t workSpaceSize) {
+  try {
+    if (alpha == nullptr || beta == nullptr || rows == nullptr || table == nullptr ||
+        tokens == nullptr)
+      return CUDNN_STATUS_BAD_PARAM;
+    auto h = handles().get(handle);
+    auto rd = tensors().get(rowsDesc);
+    auto td = filters().get(tableDesc);
+    if (!h || !rd || !td) return CUDNN_STATUS_BAD_PARAM;
+    EmbeddingArgs a{};
+    const cudnnStatus_t s = embedding_shape(*rd, *td, &a);
+    if (s != CUDNN_STATUS_SUCCESS) return s;
+    a.token = tokens;
+    a.alpha = *static_cast<const float*>(alpha);
+    a.beta = *static_cast<const float*>(beta);
+    a.row = const_cast<void*>(rows);
+    a.w = const_cast<void*>(table);
+    const std::size_t rs = a.rows == EmbeddingType::kF32 ? 4 : 2;
+    const std::size_t ts = a.table == EmbeddingType::kF32 ? 4 : 2;
+    const Span r{rows, (static_cast<std::size_t>(a.tokens - 1) * a.ld + a.features) * rs};
+    const Span w{table, static_cast<std::size_t>(a.vocab) * a.features * ts};
+    const Span t{tokens, static_cast<std::size_t>(a.tokens) * 8};
+    const Span ws{workSpace, workSpace != nullptr ? workSpaceSize : 0};
+    for (const auto& [m, align] :
+         {std::pair<Span, std::size_t>{r, rs}, {w, ts}, {t, 8}, {ws, 256}}) {
+      if (m.bytes == 0) continue;
+      if (!mb200::aligned_to(m.p, align) || !mb200::device_span_ok(m.p, m.bytes))
+        return CUDNN_STATUS_BAD_PARAM;
+    }
+    if (overlap(r, w) || overlap(gradient ? w : r, t) || overlap(ws, r) || overlap(ws, w) ||
+        overlap(ws, t))
+      return CUDNN_STATUS_BAD_PARAM;
+    const cudaStream_t st = stream_of(*h);
+    if (!gradient) return status_of(mb200::dnn::launch_embedding(a, st));
+    const std::size_t need = mb200::dnn::embedding_gradient_workspace(a);
+    if (workSpace != nullptr) {
+      if (workSpaceSize < need) return CUDNN_STATUS_BAD_PARAM;
+      return status_of(mb200::dnn::launch_embedding_gradient(a, workSpace, st));
+    }
+    return with_workspace(*h, need, st, false, [&](void* p) {
+      return mb200::dnn::launch_embedding_gradient(a, p, st);
+    });
+  } catch (const std::bad_alloc&) {
+    return CUDNN_STATUS_ALLOC_FAILED;
+  } catch (...) {
+    return CUDNN_STATUS_INTERNAL_ERROR;
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+cudnnStatus_t cudnnEmbeddingForward(cudnnHandle_t handle, const void* alpha,
+                                    cudnnFilterDescriptor_t wDesc, const void* w,
+                                    const int64_t* tokens, const void* beta,
+                                    cudnnTensorDescriptor_t yDesc, void* y) {
+  return embedding_call(handle, alpha, beta, yDesc, y, wDesc, w, tokens, false, nullptr, 0);
+}
+
+cudnnStatus_t cudnnGetEmbeddingBackwardWorkspaceSize(cudnnHandle_t handle,
+                                                     cudnnTensorDescriptor_t dyDesc,
+                                                     cudnnFilterDescriptor_t dwDesc,
+                                                     size_t* sizeInBytes) {
+  if (sizeInBytes == nullptr) return CUDNN_STATUS_BAD_PARAM;
+  auto h = handles().get(handle);
+  auto dyd = tensors().get(dyDesc);
+  auto dwd = filters().get(dwDesc);
+  if (!h || !dyd || !dwd) return CUDNN_STATUS_BAD_PARAM;
+  EmbeddingArgs a{};
+  const cudnnStatus_t s = embedding_shape(*dyd, *dwd, &a);
+  if (s != CUDNN_STATUS_SUCCESS) return s;
+  *sizeInBytes = mb200::dnn::embedding_gradient_workspace(a);
+  return CUDNN_STATUS_SUCCESS;
+}
+
+cudnnStatus_t cudnnEmbeddingBackward(cudnnHandle_t handle, const void* alpha,
+                                     cudnnTensorDescriptor_t dyDesc, const void* dy,
+                                     const int64_t* tokens, void* workSpace,
+                                     size_t workSpaceSizeInBytes, const void* beta,
+                                     cudnnFilterDescriptor_t dwDesc, void* dw) {
+  return embedding_call(handle, alpha, beta, dyDesc, dy, dwDesc, dw, tokens, true, workSpace,
+                        workSpaceSizeInBytes);
 }
 
 }  // extern "C"

@@ -740,6 +740,155 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
+// ------------------------------------------------------- losses of the tokens' nll --
+struct PolicyTerms {
+  float loss, ratio, kl;
+  float slope;  // d loss / d nll
+};
+
+// exp(d) - 1 - d.  The difference loses |d| / 2 of its digits near 0; the series' first term
+// left out there is 2 d^8 / 10! of it, under 2^-28.
+__device__ __forceinline__ float exp_above_tangent(float d) {
+  if (!(fabsf(d) < 0.5f)) return expm1f(d) - d;
+  float s = 1.0f;
+#pragma unroll
+  for (int k = 9; k >= 3; --k) s = fmaf(s * d, 1.0f / k, 1.0f);
+  return 0.5f * d * d * s;
+}
+
+// The smaller of r A and its clipped form moves the gradient where it is r A (ties too).  An
+// advantage of 0 asks for nothing, whatever the ratio.  NaN anywhere makes all terms that it
+// enters NaN: comparisons are written so that NaN takes the side that keeps it.
+__device__ __forceinline__ PolicyTerms policy_terms(const PolicyLoss& p, int row, float nll) {
+  PolicyTerms t;
+  t.ratio = p.old_nll != nullptr ? expf(p.old_nll[row] - nll) : nll == nll ? 1.0f : nll;
+  const float adv = p.advantage[row];
+  float gain = 0.0f;
+  t.slope = 0.0f;
+  if (adv != 0.0f) {
+    const float bounded = t.ratio < p.lo ? p.lo : t.ratio > p.hi ? p.hi : t.ratio;
+    const float plain = t.ratio * adv, clipped = bounded * adv;
+    const bool moves = !(plain > clipped);
+    gain = moves ? plain : clipped;
+    t.slope = moves ? plain : 0.0f;
+    if (p.dual > 0.0f && adv < 0.0f && gain < p.dual * adv) {
+      gain = p.dual * adv;
+      t.slope = 0.0f;
+    }
+  } else if (t.ratio != t.ratio) {
+    gain = t.slope = t.ratio;
+  }
+  t.loss = -gain;
+  t.kl = 0.0f;
+  if (p.ref_nll != nullptr) {
+    const float d = nll - p.ref_nll[row];
+    t.kl = exp_above_tangent(d);
+    if (p.kl_coef != 0.0f) {
+      t.loss = fmaf(p.kl_coef, t.kl, t.loss);
+      t.slope = fmaf(p.kl_coef, expm1f(d), t.slope);
+    }
+  }
+  return t;
+}
+
+constexpr int kPreferenceThreads = 512;
+
+struct PreferenceArgs {
+  PreferenceLoss p;
+  int tokens;
+  const std::int64_t* labels;
+  const float* nll;
+  const float* dloss;   // [pairs], null: no gradient
+  float* dnll;          // [tokens], holds zeros; rows of the pairs' tokens are written
+};
+
+__device__ __forceinline__ double block_sum(double v, double* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();  // red[] may still be read by the previous sum
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double r = 0.0;
+#pragma unroll
+  for (int i = 0; i < kPreferenceThreads / 32; ++i) r += red[i];
+  return r;
+}
+
+// One CTA per pair: the two sequences' sums, the pair's loss, and the derivative by each of
+// their tokens' nll.  Sums are in 64 bits: the difference of two sums of thousands of tokens is
+// what the loss sees.  A pair whose offsets do not ascend within the tokens is NaN.
+__global__ void __launch_bounds__(kPreferenceThreads)
+    vocab_preference_kernel(const PreferenceArgs a) {
+  tc::grid_launch_next();
+  tc::grid_wait_previous();
+  __shared__ double red[kPreferenceThreads / 32];
+  const int pair = blockIdx.x;
+  std::int64_t begin[2], end[2];
+  double sum[2], n[2];
+  bool bad = false;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int s = pair + k * a.p.pairs;
+    begin[k] = a.p.offsets[s];
+    end[k] = a.p.offsets[s + 1];
+    if (begin[k] < 0 || end[k] < begin[k] || end[k] > a.tokens) {
+      bad = true;
+      begin[k] = end[k] = 0;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    double v = 0.0;
+    int kept = 0;
+#pragma unroll 4
+    for (std::int64_t t = begin[k] + threadIdx.x; t < end[k]; t += kPreferenceThreads) {
+      if (a.labels[t] < 0) continue;
+      v += static_cast<double>(a.p.ref_nll != nullptr ? a.p.ref_nll[t] : 0.0f) - a.nll[t];
+      ++kept;
+    }
+    sum[k] = block_sum(v, red);
+    n[k] = block_sum(kept, red);
+  }
+  const bool live = bad || (n[0] > 0.0 && n[1] > 0.0);
+  double share[2] = {1.0, 1.0};
+  if (a.p.averaged) {
+    share[0] = 1.0 / n[0];
+    share[1] = 1.0 / n[1];
+  }
+  const double beta = a.p.beta;
+  const double gain[2] = {sum[0] * share[0], sum[1] * share[1]};
+  const double h = bad ? NAN : beta * (gain[0] - gain[1]) - a.p.margin;
+  double loss, slope;
+  if (a.p.mode == PreferenceMode::kSigmoid) {
+    const double e = exp(-fabs(h));
+    loss = log1p(e) + (h < 0.0 ? -h : 0.0) + a.p.smoothing * h;
+    slope = a.p.smoothing - (h < 0.0 ? 1.0 : e) / (1.0 + e);
+  } else if (a.p.mode == PreferenceMode::kHinge) {
+    loss = h < 1.0 ? 1.0 - h : h >= 1.0 ? 0.0 : h;
+    slope = h < 1.0 ? -1.0 : h >= 1.0 ? 0.0 : h;
+  } else {
+    const double r = (h - 0.5) / beta;
+    loss = r * r;
+    slope = 2.0 * r / beta;
+  }
+  if (threadIdx.x == 0) {
+    if (a.p.loss != nullptr) a.p.loss[pair] = live ? static_cast<float>(loss) : 0.0f;
+    if (a.p.rewards != nullptr) {
+      for (int k = 0; k < 2; ++k)
+        a.p.rewards[pair + k * a.p.pairs] =
+            bad ? NAN : live ? static_cast<float>(beta * gain[k]) : 0.0f;
+    }
+  }
+  if (a.dloss == nullptr || !live || bad) return;
+  const double g = a.dloss[pair] * slope * beta;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const auto each = static_cast<float>((k == 0 ? -g : g) * share[k]);
+    for (std::int64_t t = begin[k] + threadIdx.x; t < end[k]; t += kPreferenceThreads)
+      a.dnll[t] = each;  // of tokens left out, nothing reads it
+  }
+}
+
 constexpr int kFinishThreads = 256;
 
 __device__ __forceinline__ float block_reduce(float v, bool is_max, float* red) {
@@ -769,6 +918,8 @@ struct FinishArgs {
   Targets targets;
   float* loss;  // may be null
   float* lse;   // may be null
+  PolicyLoss policy;
+  float* dnll;  // kNone: null, or the gradients by the tokens' nll (without a policy zeros)
   const float* dloss;
   float inv_tau;
   float log2e_tau;     // log2(e) / tau
@@ -869,7 +1020,9 @@ __device__ __forceinline__ uint4 scaled(uint4 u, float f, uint4* left = nullptr)
 // A CTA per row and part of its words (each part joins the row's pairs again, a few KB from
 // L2), then one per tile of the transpose.  Bound by HBM: it reads and writes the numerators once, 8192 x
 // 131072 in 0.68 ms (6.3 TB/s).
-template <typename T, int STORE>
+// POLICY: the losses are policy losses, and dloss is of them; a form of its own, for the others'
+// registers' sake.
+template <typename T, int STORE, bool POLICY>
 __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const FinishArgs a) {
   tc::grid_launch_next();
   tc::grid_wait_previous();
@@ -898,6 +1051,13 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     if (part == 0 && threadIdx.x == 0) {
       if (a.loss != nullptr) a.loss[row] = 0.0f;
       if (a.lse != nullptr) a.lse[row] = 0.0f;
+      if constexpr (STORE == kNone) {
+        if (a.dnll != nullptr) a.dnll[row] = 0.0f;
+      }
+      if constexpr (POLICY) {
+        for (float* o : {a.policy.loss, a.policy.ratio, a.policy.kl})
+          if (o != nullptr) o[row] = 0.0f;
+      }
       if constexpr (STORE != kNone) a.row_scale[row] = make_float2(0.0f, 0.0f);
     }
     if constexpr (STORE != kNone) {
@@ -943,10 +1103,29 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     if (threadIdx.x == 0) {
       if (a.loss != nullptr) a.loss[row] = loss;
       if (a.lse != nullptr) a.lse[row] = fmaf(mx, a.inv_tau, log_sum * kLn2);
+      if constexpr (STORE == kNone && !POLICY) {
+        if (a.dnll != nullptr) a.dnll[row] = 0.0f;
+      }
+    }
+  }
+  [[maybe_unused]] float slope = 1.0f;  // of the row's loss by its nll
+  if constexpr (POLICY) {
+    const PolicyTerms t =
+        policy_terms(a.policy, row, n < 0 ? NAN : (log_sum - above(r0)) * kLn2);
+    slope = t.slope;
+    if (part == 0 && threadIdx.x == 0) {
+      if (a.policy.loss != nullptr) a.policy.loss[row] = t.loss;
+      if (a.policy.ratio != nullptr) a.policy.ratio[row] = t.ratio;
+      if (a.policy.kl != nullptr) a.policy.kl[row] = t.kl;
+      if constexpr (STORE == kNone) {
+        if (a.dnll != nullptr) a.dnll[row] = a.dloss[row] * slope;
+      }
     }
   }
   if constexpr (STORE != kNone) {
-    float g = n < 0 ? NAN : a.dloss[row] * a.inv_tau;
+    float g = n < 0 ? NAN : a.dloss[row];
+    if constexpr (POLICY) g *= slope;
+    g *= a.inv_tau;
     if (a.scale != nullptr) g *= a.scale[0];
     float down = 0.0f;  // kCommon: the row's reference below its maximum, in z2
     if constexpr (kDz) {
@@ -1442,8 +1621,8 @@ struct Plan {
   int slice;          // words of w that are packed at a time; without pack_w all
   int lefts;          // entries per token of what the targets' rounding left
   // byte offsets into the workspace
-  std::size_t stats, z, index, q, count, entropy, hit, scale, row_scale, left, xp, wp, num, xt,
-      partial, sum, bytes;
+  std::size_t stats, z, index, q, count, entropy, hit, scale, row_scale, left, dnll, xp, wp, num,
+      xt, partial, sum, bytes;
   std::size_t rows_bytes;  // of them, what grows with the tokens, without the numerators
 };
 
@@ -1495,6 +1674,7 @@ Plan plan_rows(const VocabLossArgs& a, int rows, bool sliced) {
   p.row_scale = take(a.gradients ? R * sizeof(float2) : 0);
   p.lefts = dx && p.store != kSplit && K <= kMostLeft ? std::max(a.top_k, 1) : 0;
   p.left = take(R * p.lefts * sizeof(Left));
+  p.dnll = take(a.head == HeadLoss::kPolicy && a.gradients && !a.bf16 ? R * 4 : 0);
   p.xp = take(p.pack_x ? R * p.ldp * 2 : 0);
   const std::size_t wp = p.pack_w ? static_cast<std::size_t>(p.slice) * p.ldp * 2 : 0;
   const std::size_t num = a.gradients ? p.copies * R * p.ldn * 2 : 0;
@@ -1669,8 +1849,24 @@ cudaError_t run_dw(const VocabLossArgs& a, const Plan& p, const void* num, const
   return tc::launch_tc_epi<Dw<T, TALL>, FMT>(g, sms(), to, st, true);
 }
 
+// What a preference loss keeps of all tokens: their nll, and the gradients by them.
+struct TokenRows {
+  const float* nll;
+  float* dnll;
+};
+
+cudaError_t run_preference(const VocabLossArgs& a, const TokenRows& rows, cudaStream_t st) {
+  const PreferenceArgs g{a.preference, a.tokens, a.labels, rows.nll,
+                         a.gradients ? a.dloss : nullptr, rows.dnll};
+  return tc::launch_overlapped(vocab_preference_kernel,
+                               dim3(static_cast<unsigned>(a.preference.pairs)),
+                               kPreferenceThreads, 0, st, true, g);
+}
+
+// `rows`: of a preference loss, whose gradients take one piece.
 template <typename T, int FMT>
-cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st) {
+cudaError_t run(const VocabLossArgs& a, const Plan& p, const TokenRows& all, char* ws,
+                cudaStream_t st) {
   unsigned int* to = timeout_counter();
   if (to == nullptr) return cudaErrorInvalidDevice;
   // the call's first kernel starts when the stream reaches it, the others overlap
@@ -1730,11 +1926,11 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     }
 
     float* scale = nullptr;
-    if (a.gradients && !a.bf16) {
+    const auto find_scale = [&](const float* dloss) {
       scale = reinterpret_cast<float*>(ws + p.scale);
-      MB200_TRY(launch(vocab_grad_scale_kernel, 1, 1024, a.dloss + t0, rows, a.vocab, tg,
-                       a.inv_tau, scale));
-    }
+      return launch(vocab_grad_scale_kernel, 1, 1024, dloss, rows, a.vocab, tg, a.inv_tau, scale);
+    };
+    if (a.gradients && !a.bf16 && a.head == HeadLoss::kTargets) MB200_TRY(find_scale(a.dloss + t0));
 
     FinishArgs f{};
     f.rows = rows;
@@ -1746,6 +1942,21 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     f.targets = tg;
     f.loss = a.loss != nullptr ? a.loss + t0 : nullptr;
     f.lse = a.lse != nullptr ? a.lse + t0 : nullptr;
+    bool in_finish = a.head == HeadLoss::kPolicy;  // the finish computes policy losses
+    const auto finish_form = [&](auto store) {
+      constexpr int kStore = decltype(store)::value;
+      return in_finish ? vocab_finish_kernel<T, kStore, true> : vocab_finish_kernel<T, kStore, false>;
+    };
+    if (in_finish) {
+      const auto from = [&](auto* q) { return q != nullptr ? q + t0 : nullptr; };
+      f.policy = a.policy;
+      f.policy.old_nll = from(a.policy.old_nll);
+      f.policy.ref_nll = from(a.policy.ref_nll);
+      f.policy.advantage = from(a.policy.advantage);
+      f.policy.loss = from(a.policy.loss);
+      f.policy.ratio = from(a.policy.ratio);
+      f.policy.kl = from(a.policy.kl);
+    }
     f.inv_tau = a.inv_tau;
     f.log2e_tau = kLog2e * a.inv_tau;
     f.scale = scale;
@@ -1756,7 +1967,7 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
       const StreamArgs sa{x, ldx, w, ldw, rows, a.features, a.vocab, kLog2e * a.inv_tau,
                           reinterpret_cast<float2*>(ws + p.stats), tg};
       MB200_TRY(launch(vocab_stream_kernel<T>, p.units, kStreamThreads, sa));
-      MB200_TRY(launch(vocab_finish_kernel<T, kNone>, rows, kFinishThreads, f));
+      MB200_TRY(launch(finish_form(std::integral_constant<int, kNone>{}), rows, kFinishThreads, f));
       continue;
     }
 
@@ -1802,10 +2013,10 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
     };
     if (p.store == kNone) {
       MB200_TRY(logits(std::integral_constant<int, kNone>{}));
-      MB200_TRY(launch(vocab_finish_kernel<T, kNone>, rows, kFinishThreads, f));
+      MB200_TRY(launch(finish_form(std::integral_constant<int, kNone>{}), rows, kFinishThreads, f));
       continue;
     }
-    f.dloss = a.dloss + t0;
+    f.dloss = a.dloss + (a.head == HeadLoss::kPreference ? 0 : t0);
     f.row_scale = reinterpret_cast<float2*>(ws + p.row_scale);
     f.left = p.lefts > 0 ? reinterpret_cast<Left*>(ws + p.left) : nullptr;
     f.parts = parts;
@@ -1816,13 +2027,38 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
       tiles = static_cast<long long>((rows + 63) / 64) * ((a.features + 63) / 64);
     }
     const long long finish = static_cast<long long>(rows) * parts;
+    // A preference needs all its tokens' nll before any gradient, and fp16's scale the gradients
+    // of all rows: a pass over the pairs of (maximum, sum) comes first, and the finish below
+    // goes by the gradients that it left.
+    const auto before_gradients = [&]() -> cudaError_t {
+      const bool preference = a.head == HeadLoss::kPreference;
+      if (!preference && !(a.head == HeadLoss::kPolicy && !a.bf16)) return cudaSuccess;
+      FinishArgs s = f;
+      s.parts = 1;
+      s.loss = preference ? const_cast<float*>(all.nll) : f.loss;
+      s.dnll = preference ? all.dnll : reinterpret_cast<float*>(ws + p.dnll);
+      s.transpose.xt = nullptr;
+      MB200_TRY(launch(finish_form(std::integral_constant<int, kNone>{}), rows, kFinishThreads, s));
+      in_finish = false;
+      if (preference) MB200_TRY(run_preference(a, all, st));
+      f.loss = f.lse = nullptr;
+      f.dloss = s.dnll;
+      if (!a.bf16) {
+        MB200_TRY(find_scale(f.dloss));
+        f.scale = scale;
+      }
+      return cudaSuccess;
+    };
     if (p.store == kOwn || p.store == kSplit) {
       MB200_TRY(logits(std::integral_constant<int, kOwn>{}));
-      MB200_TRY(launch(p.store == kOwn ? vocab_finish_kernel<T, kOwn> : vocab_finish_kernel<T, kSplit>,
+      MB200_TRY(before_gradients());
+      MB200_TRY(launch(p.store == kOwn ? finish_form(std::integral_constant<int, kOwn>{})
+                                       : finish_form(std::integral_constant<int, kSplit>{}),
                        finish + tiles, kFinishThreads, f));
     } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
       MB200_TRY(logits(std::integral_constant<int, kCommon>{}));
-      MB200_TRY(launch(vocab_finish_kernel<T, kCommon>, finish, kFinishThreads, f));
+      MB200_TRY(before_gradients());
+      MB200_TRY(launch(finish_form(std::integral_constant<int, kCommon>{}), finish, kFinishThreads, f));
     }
 
     if (a.dx != nullptr) {
@@ -1848,11 +2084,31 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, char* ws, cudaStream_t st
   return cudaSuccess;
 }
 
+// A preference's rows of all tokens, in front of what a plan needs: its nll where the caller
+// does not take them, and the gradients by them.
+struct RowsPlan {
+  std::size_t nll, dnll, bytes;
+};
+
+RowsPlan rows_plan(const VocabLossArgs& a) {
+  RowsPlan r{};
+  if (a.head != HeadLoss::kPreference) return r;
+  const std::size_t each = (static_cast<std::size_t>(a.tokens) * 4 + 255) / 256 * 256;
+  r.dnll = a.loss == nullptr ? each : 0;
+  r.bytes = r.dnll + (a.gradients ? each : 0);
+  return r;
+}
+
+cudaError_t run_any(const VocabLossArgs& a, const Plan& p, const TokenRows& rows, char* ws,
+                    cudaStream_t st) {
+  return a.bf16 ? run<__nv_bfloat16, 1>(a, p, rows, ws, st) : run<__half, 0>(a, p, rows, ws, st);
+}
+
 }  // namespace
 
 std::size_t vocab_loss_workspace(const VocabLossArgs& a) noexcept {
   bool ok = false;
-  return plan_within(a, SIZE_MAX, false, &ok).bytes;
+  return rows_plan(a).bytes + plan_within(a, SIZE_MAX, false, &ok).bytes;
 }
 
 std::size_t vocab_loss_workspace_any(const VocabLossArgs& a) noexcept {
@@ -1867,23 +2123,53 @@ std::size_t vocab_loss_workspace_any(const VocabLossArgs& a) noexcept {
       most = std::max(most, plan_within(b, SIZE_MAX, a.features % 8 == 0, &ok).bytes);
     }
   }
-  return most;
+  return rows_plan(a).bytes + most;
 }
 
 std::size_t vocab_loss_min_workspace(const VocabLossArgs& a) noexcept {
   bool ok = false;
-  return std::min({plan_rows(a, std::min(a.tokens, kLeastRows), true).bytes,
-                   plan_rows(a, a.tokens, true).bytes,
-                   plan_within(a, SIZE_MAX, true, &ok).bytes});
+  return rows_plan(a).bytes + std::min({plan_rows(a, std::min(a.tokens, kLeastRows), true).bytes,
+                                        plan_rows(a, a.tokens, true).bytes,
+                                        plan_within(a, SIZE_MAX, true, &ok).bytes});
 }
 
-cudaError_t launch_vocab_loss(const VocabLossArgs& a, void* ws, std::size_t ws_bytes,
+cudaError_t launch_vocab_loss(const VocabLossArgs& a, void* workspace, std::size_t ws_bytes,
                               cudaStream_t stream) noexcept {
+  const RowsPlan r = rows_plan(a);
+  if (ws_bytes < r.bytes) return cudaErrorInvalidValue;
   bool ok = false;
-  const Plan p = plan_within(a, ws_bytes, false, &ok);
+  const Plan p = plan_within(a, ws_bytes - r.bytes, false, &ok);
   if (!ok) return cudaErrorInvalidValue;
-  return a.bf16 ? run<__nv_bfloat16, 1>(a, p, static_cast<char*>(ws), stream)
-                : run<__half, 0>(a, p, static_cast<char*>(ws), stream);
+  char* ws = static_cast<char*>(workspace);
+  TokenRows rows{};
+  if (a.head == HeadLoss::kPreference) {
+    rows.nll = a.loss != nullptr ? a.loss : reinterpret_cast<float*>(ws + r.nll);
+    rows.dnll = reinterpret_cast<float*>(ws + r.dnll);
+    ws += r.bytes;
+    if (!a.gradients || p.pieces > 1) {
+      // scores of all tokens, then the pairs; a gradient of several pieces computes its logits
+      // again, as the cross entropies whose dloss is known by now (8 instead of 6 T H V)
+      VocabLossArgs score = a;
+      score.head = HeadLoss::kTargets;
+      score.gradients = false;
+      score.dx = score.dw = nullptr;
+      score.loss = const_cast<float*>(rows.nll);
+      const Plan sp = a.gradients ? plan_within(score, ws_bytes - r.bytes, false, &ok) : p;
+      if (!ok) return cudaErrorInvalidValue;
+      MB200_TRY(run_any(score, sp, rows, ws, stream));
+      if (!a.gradients) return run_preference(a, rows, stream);
+      if (cudaError_t e = cudaMemsetAsync(rows.dnll, 0, std::size_t(a.tokens) * 4, stream);
+          e != cudaSuccess)
+        return e;
+      MB200_TRY(run_preference(a, rows, stream));
+      VocabLossArgs gradient = a;
+      gradient.head = HeadLoss::kTargets;
+      gradient.loss = gradient.lse = nullptr;
+      gradient.dloss = rows.dnll;
+      return run_any(gradient, p, rows, ws, stream);
+    }
+  }
+  return run_any(a, p, rows, ws, stream);
 }
 
 }  // namespace mb200::dnn
