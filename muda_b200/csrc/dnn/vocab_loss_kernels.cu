@@ -918,6 +918,10 @@ struct FinishArgs {
   Targets targets;
   float* loss;  // may be null
   float* lse;   // may be null
+  const void* x;  // kNll, kPolicy: the operands, for the targets' logits
+  std::int64_t ldx;
+  const void* w;
+  int features;
   PolicyLoss policy;
   float* dnll;  // kNone: null, or the gradients by the tokens' nll (without a policy zeros)
   const float* dloss;
@@ -1020,9 +1024,53 @@ __device__ __forceinline__ uint4 scaled(uint4 u, float f, uint4* left = nullptr)
 // A CTA per row and part of its words (each part joins the row's pairs again, a few KB from
 // L2), then one per tile of the transpose.  Bound by HBM: it reads and writes the numerators once, 8192 x
 // 131072 in 0.68 ms (6.3 TB/s).
-// POLICY: the losses are policy losses, and dloss is of them; a form of its own, for the others'
-// registers' sake.
-template <typename T, int STORE, bool POLICY>
+// What the finish computes of a token besides its target losses; forms of their own, for those
+// losses' registers' sake (40 against 62).  kNll: the cross entropy with the target's logit
+// computed again.  kPolicy: the policy loss of that, whose upstream gradient dloss is.
+enum FinishForm { kTargetLoss = 0, kNll = 1, kPolicy = 2 };
+
+// x[row] w[label] in fp32, to about half its last place: H / 256 rounded terms per thread, the
+// threads' sums in 64 bits (the whole CTA calls this).  The tensor cores' sums are short of
+// that by up to 4e-7 of the logit, always toward zero, and a log ratio of two sequences adds
+// the like of it up over their tokens: rewards of 256-token sequences were 1.2e-5 off, their
+// plain fp32 form 6e-7.
+template <typename T>
+__device__ __forceinline__ float target_logit(const T* x, const T* w, int features, double* red) {
+  float part = 0.0f;
+  if (((reinterpret_cast<std::uintptr_t>(x) | reinterpret_cast<std::uintptr_t>(w)) & 15) == 0) {
+    for (int h = threadIdx.x * 8; h < features; h += kFinishThreads * 8) {
+      if (h + 8 <= features) {
+        const uint4 a = *reinterpret_cast<const uint4*>(x + h);
+        const uint4 b = *reinterpret_cast<const uint4*>(w + h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 u = unpack2<T>(reinterpret_cast<const std::uint32_t*>(&a)[j]);
+          const float2 v = unpack2<T>(reinterpret_cast<const std::uint32_t*>(&b)[j]);
+          part = fmaf(u.x, v.x, part);
+          part = fmaf(u.y, v.y, part);
+        }
+      } else {
+        for (int j = h; j < features; ++j)
+          part = fmaf(static_cast<float>(x[j]), static_cast<float>(w[j]), part);
+      }
+    }
+  } else {
+#pragma unroll 8
+    for (int h = threadIdx.x; h < features; h += kFinishThreads)
+      part = fmaf(static_cast<float>(x[h]), static_cast<float>(w[h]), part);
+  }
+  double sum = part;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < kFinishThreads / 32; ++i) sum += red[i];
+  return static_cast<float>(sum);
+}
+
+template <typename T, int STORE, int FORM>
 __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const FinishArgs a) {
   tc::grid_launch_next();
   tc::grid_wait_previous();
@@ -1054,7 +1102,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
       if constexpr (STORE == kNone) {
         if (a.dnll != nullptr) a.dnll[row] = 0.0f;
       }
-      if constexpr (POLICY) {
+      if constexpr (FORM == kPolicy) {
         for (float* o : {a.policy.loss, a.policy.ratio, a.policy.kl})
           if (o != nullptr) o[row] = 0.0f;
       }
@@ -1087,12 +1135,27 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
   const std::int64_t r0 = static_cast<std::int64_t>(row) * tk;
   // a target's z2 above the maximum's: a confident word's loss is far below z2's last bit
   const auto above = [&](std::int64_t i) { return (a.targets.z[i] - mx) * a.log2e_tau; };
+  [[maybe_unused]] float nll = NAN;  // cross entropy
+  if (a.targets.top_k == 0 && n > 0) {
+    nll = (log_sum - above(r0)) * kLn2;
+    if constexpr (FORM != kTargetLoss) {
+      __shared__ double dots[kFinishThreads / 32];
+      const float was = a.targets.z[r0];
+      const float z = target_logit<T>(
+          static_cast<const T*>(a.x) + row * a.ldx,
+          static_cast<const T*>(a.w) + a.targets.labels[row] * a.features, a.features, dots);
+      if (fabsf(z - was) < INFINITY) {  // the target's own share of the sum moves too
+        const float moved = sum + exp2f(above(r0)) * expm1f((z - was) * a.inv_tau);
+        nll = (log2f(moved) - (z - mx) * a.log2e_tau) * kLn2;
+      }
+    }
+  }
   if (part == 0) {
     float loss;
     if (n < 0) {
       loss = NAN;
     } else if (a.targets.top_k == 0) {
-      loss = (log_sum - above(r0)) * kLn2;
+      loss = nll;
     } else {
       float cross = 0.0f;
       for (int k = threadIdx.x; k < n; k += kFinishThreads)
@@ -1103,15 +1166,14 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     if (threadIdx.x == 0) {
       if (a.loss != nullptr) a.loss[row] = loss;
       if (a.lse != nullptr) a.lse[row] = fmaf(mx, a.inv_tau, log_sum * kLn2);
-      if constexpr (STORE == kNone && !POLICY) {
+      if constexpr (STORE == kNone && FORM != kPolicy) {
         if (a.dnll != nullptr) a.dnll[row] = 0.0f;
       }
     }
   }
   [[maybe_unused]] float slope = 1.0f;  // of the row's loss by its nll
-  if constexpr (POLICY) {
-    const PolicyTerms t =
-        policy_terms(a.policy, row, n < 0 ? NAN : (log_sum - above(r0)) * kLn2);
+  if constexpr (FORM == kPolicy) {
+    const PolicyTerms t = policy_terms(a.policy, row, nll);
     slope = t.slope;
     if (part == 0 && threadIdx.x == 0) {
       if (a.policy.loss != nullptr) a.policy.loss[row] = t.loss;
@@ -1124,7 +1186,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
   }
   if constexpr (STORE != kNone) {
     float g = n < 0 ? NAN : a.dloss[row];
-    if constexpr (POLICY) g *= slope;
+    if constexpr (FORM == kPolicy) g *= slope;
     g *= a.inv_tau;
     if (a.scale != nullptr) g *= a.scale[0];
     float down = 0.0f;  // kCommon: the row's reference below its maximum, in z2
@@ -1942,12 +2004,23 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, const TokenRows& all, cha
     f.targets = tg;
     f.loss = a.loss != nullptr ? a.loss + t0 : nullptr;
     f.lse = a.lse != nullptr ? a.lse + t0 : nullptr;
-    bool in_finish = a.head == HeadLoss::kPolicy;  // the finish computes policy losses
+    // scores, and gradients whose finish computes the loss; a preference's comes before it
+    int form = a.head == HeadLoss::kPolicy       ? kPolicy
+               : a.head == HeadLoss::kPreference ? kNll
+                                                 : kTargetLoss;
     const auto finish_form = [&](auto store) {
       constexpr int kStore = decltype(store)::value;
-      return in_finish ? vocab_finish_kernel<T, kStore, true> : vocab_finish_kernel<T, kStore, false>;
+      if constexpr (kStore == kNone) {
+        if (form == kNll) return vocab_finish_kernel<T, kNone, kNll>;
+      }
+      return form == kPolicy ? vocab_finish_kernel<T, kStore, kPolicy>
+                             : vocab_finish_kernel<T, kStore, kTargetLoss>;
     };
-    if (in_finish) {
+    f.x = x;
+    f.ldx = ldx;
+    f.w = a.w;
+    f.features = a.features;
+    if (form == kPolicy) {
       const auto from = [&](auto* q) { return q != nullptr ? q + t0 : nullptr; };
       f.policy = a.policy;
       f.policy.old_nll = from(a.policy.old_nll);
@@ -2039,7 +2112,7 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, const TokenRows& all, cha
       s.dnll = preference ? all.dnll : reinterpret_cast<float*>(ws + p.dnll);
       s.transpose.xt = nullptr;
       MB200_TRY(launch(finish_form(std::integral_constant<int, kNone>{}), rows, kFinishThreads, s));
-      in_finish = false;
+      form = kTargetLoss;
       if (preference) MB200_TRY(run_preference(a, all, st));
       f.loss = f.lse = nullptr;
       f.dloss = s.dnll;
@@ -2150,7 +2223,6 @@ cudaError_t launch_vocab_loss(const VocabLossArgs& a, void* workspace, std::size
       // scores of all tokens, then the pairs; a gradient of several pieces computes its logits
       // again, as the cross entropies whose dloss is known by now (8 instead of 6 T H V)
       VocabLossArgs score = a;
-      score.head = HeadLoss::kTargets;
       score.gradients = false;
       score.dx = score.dw = nullptr;
       score.loss = const_cast<float*>(rows.nll);
