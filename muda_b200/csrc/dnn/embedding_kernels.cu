@@ -6,15 +6,17 @@
 // The gradient adds each word's rows in the order of their positions, without atomics, so
 // results are the same on every run.  Three launches:
 //   1. embedding_sort_kernel orders the tokens by word, positions ascending within a word;
-//   2. embedding_partial_kernel cuts the ordered tokens into blocks and adds up, in fp32, the
-//      blocks' shares of words that occur more often than a block is long;
-//   3. embedding_rows_kernel adds each word's rows, or the partial sums of a frequent one,
-//      and writes its row of dw, zeros (or beta dw) for words that do not occur.
+//   2. embedding_sum_kernel cuts the ordered tokens into blocks of equal length, whatever words
+//      they hold, and adds each block's rows up in fp32: a word that lies within a block gets
+//      its row of dw, one that crosses into another leaves a partial sum.  Beside that it
+//      writes the rows of the words that do not occur;
+//   3. embedding_join_kernel adds the partial sums of the words that cross blocks.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <type_traits>
 
@@ -75,45 +77,46 @@ __device__ __forceinline__ void store_run(T* p, const Run<T, VEC>& r) {
 // ------------------------------------------------------------------------- lookup --
 constexpr int kLookupThreads = 256;
 
-template <typename TW, typename TY, int VEC, int RUNS>
+// A thread has one column of ROWS rows that lie `stride` apart, so the loads of its tokens, of
+// their words' runs and its stores are ROWS at a time and one division finds them all.
+template <typename TW, typename TY, int VEC, int ROWS>
 __global__ void __launch_bounds__(kLookupThreads)
     embedding_kernel(const TW* __restrict__ w, const std::int64_t* __restrict__ token, TY* y,
-                     std::int64_t ldy, int tokens, int features, int vocab, float alpha,
-                     float beta) {
+                     std::int64_t ldy, int tokens, int features, int vocab, int stride,
+                     float alpha, float beta) {
   const unsigned per = features / VEC;  // runs of a row
-  const std::int64_t first = static_cast<std::int64_t>(blockIdx.x) * (kLookupThreads * RUNS);
+  const std::int64_t first = static_cast<std::int64_t>(blockIdx.x) * kLookupThreads;
   const std::int64_t row0 = first / per;
-  const unsigned skip = static_cast<unsigned>(first - row0 * per) + threadIdx.x;
-  Run<TW, VEC> in[RUNS];
-  std::int64_t row[RUNS], word[RUNS];
-  unsigned col[RUNS];
+  const unsigned i = static_cast<unsigned>(first - row0 * per) + threadIdx.x;
+  const unsigned q = i / per;
+  const int col = static_cast<int>(i - q * per) * VEC;
+  const std::int64_t row = row0 + q;
+  if (row >= stride) return;
+  int word[ROWS];  // -1: padding, vocab: past the table
 #pragma unroll
-  for (int j = 0; j < RUNS; ++j) {
-    const unsigned i = skip + j * kLookupThreads;
-    const unsigned q = i / per;
-    row[j] = row0 + q;
-    col[j] = (i - q * per) * VEC;
-    word[j] = row[j] < tokens ? token[row[j]] : -1;
-  }
-#pragma unroll
-  for (int j = 0; j < RUNS; ++j) {
-    if (word[j] >= 0 && word[j] < vocab) {
-      in[j] = load_run<TW, VEC>(w + word[j] * features + col[j]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) in[j].v[e] = from_float<TW>(word[j] < 0 ? 0.0f : NAN);
+  for (int j = 0; j < ROWS; ++j) {
+    word[j] = -1;
+    if (row + j * stride < tokens) {
+      const std::int64_t v = token[row + j * stride];
+      word[j] = v < 0 ? -1 : v >= vocab ? vocab : static_cast<int>(v);
     }
   }
+  Run<TW, VEC> in[ROWS];
 #pragma unroll
-  for (int j = 0; j < RUNS; ++j) {
-    if (row[j] >= tokens) break;
-    TY* o = y + row[j] * ldy + col[j];
+  for (int j = 0; j < ROWS; ++j)
+    if (static_cast<unsigned>(word[j]) < static_cast<unsigned>(vocab))
+      in[j] = load_run<TW, VEC>(w + static_cast<std::int64_t>(word[j]) * features + col);
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j) {
+    if (row + j * stride >= tokens) break;
+    TY* o = y + (row + j * stride) * ldy + col;
     Run<TY, VEC> out, was;
     if (beta != 0.0f) was = load_run<TY, VEC>(o);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
       float v = alpha * static_cast<float>(in[j].v[e]);
-      if (word[j] < 0) v = 0.0f;
+      if (static_cast<unsigned>(word[j]) >= static_cast<unsigned>(vocab))
+        v = word[j] < 0 ? 0.0f : NAN;
       if (beta != 0.0f) v = fmaf(beta, static_cast<float>(was.v[e]), v);
       out.v[e] = from_float<TY>(v);
     }
@@ -132,8 +135,9 @@ __global__ void __launch_bounds__(kLookupThreads)
 constexpr int kOwners = 128, kOwnerBits = 7;
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kDigit = 5;
-constexpr int kSharedList = 2048;  // entries that are sorted in shared memory
-constexpr int kScanAhead = 8;      // loads in flight per lane
+constexpr int kSharedList = 2048;     // entries that are sorted in shared memory
+constexpr int kSharedTokens = 40960;  // tokens whose words it keeps between the two readings
+constexpr int kScanAhead = 8;         // loads in flight per lane
 
 struct Entry {
   int word;  // v / kOwners
@@ -143,12 +147,11 @@ struct Entry {
 struct SortArgs {
   const std::int64_t* token;
   int tokens, vocab;
-  int per_owner;  // words of an owner, at most
   int passes;
   Entry* list[2];  // [tokens] each: longer lists while they are sorted
   int* word;       // [tokens] out: the words in order
   int* pos;        // [tokens] out: and their positions
-  int2* span;      // [owner][per_owner] out: a word's entries, {0, 0}: none
+  int2* span;      // [vocab] out: a word's entries, {0, 0}: none
   int* total;      // out: entries
 };
 
@@ -181,7 +184,8 @@ __device__ __forceinline__ int block_exclusive(int v, int* warps, int* all) {
   return sum - v + (warp > 0 ? before : 0);
 }
 
-__global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const SortArgs a) {
+__global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const SortArgs a) {
+  extern __shared__ int cached[];  // the tokens' words, -1 for those that enter nothing
   __shared__ Entry near[2][kSharedList];
   __shared__ int count[1 << kDigit][kSortWarps + 1];  // a warp's counters in banks of their own
   __shared__ int warps[32];
@@ -191,10 +195,11 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const Sort
   const int owner = blockIdx.x;
   const unsigned before_me = (1u << lane) - 1;
 
-  int2* span = a.span + static_cast<std::int64_t>(owner) * a.per_owner;
-  for (int i = threadIdx.x; i < a.per_owner; i += kSortThreads) span[i] = make_int2(0, 0);
+  for (int v = threadIdx.x * kOwners + owner; v < a.vocab; v += kSortThreads * kOwners)
+    a.span[v] = make_int2(0, 0);
 
-  // the warp's share of the tokens; owner_of is -1 for tokens that enter nothing
+  // the warp's share of the tokens
+  const bool keep = a.tokens <= kSharedTokens;
   const int share = ((a.tokens + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
   const std::int64_t t0 = static_cast<std::int64_t>(warp) * share;
   const std::int64_t t1 = min(t0 + share, static_cast<std::int64_t>(a.tokens));
@@ -213,6 +218,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const Sort
       const int o = v[j] & (kOwners - 1);
       mine += v[j] >= 0 && o == owner;
       below += v[j] >= 0 && o < owner;
+      if (keep && t + 32 * j + lane < t1) cached[t + 32 * j + lane] = v[j];
     }
   }
   mine = warp_sum(mine);
@@ -228,7 +234,10 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const Sort
     for (std::int64_t t = t0; t < t1; t += 32 * kScanAhead) {
       int v[kScanAhead];
 #pragma unroll
-      for (int j = 0; j < kScanAhead; ++j) v[j] = load(t + 32 * j + lane);
+      for (int j = 0; j < kScanAhead; ++j) {
+        const std::int64_t i = t + 32 * j + lane;
+        v[j] = !keep ? load(i) : i < t1 ? cached[i] : -1;
+      }
 #pragma unroll
       for (int j = 0; j < kScanAhead; ++j) {
         const bool me = v[j] >= 0 && (v[j] & (kOwners - 1)) == owner;
@@ -280,191 +289,272 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(const Sort
 
   for (int i = threadIdx.x; i < n; i += kSortThreads) {
     const Entry e = from[i];
-    a.word[base + i] = (e.word << kOwnerBits) + owner;
+    const int word = (e.word << kOwnerBits) + owner;
+    a.word[base + i] = word;
     a.pos[base + i] = e.pos;
-    if (i == 0 || from[i - 1].word != e.word) span[e.word].x = base + i;
-    if (i == n - 1 || from[i + 1].word != e.word) span[e.word].y = base + i + 1;
+    if (i == 0 || from[i - 1].word != e.word) a.span[word].x = base + i;
+    if (i == n - 1 || from[i + 1].word != e.word) a.span[word].y = base + i + 1;
   }
 }
 
-__device__ __forceinline__ int2 span_of(const int2* span, int per_owner, int word) {
-  return span[static_cast<std::int64_t>(word & (kOwners - 1)) * per_owner + (word >> kOwnerBits)];
-}
-
 // ----------------------------------------------------------------------- the sums --
-// A warp adds rows over a slice of the features: RUNS runs of VEC elements per lane, all loads
-// of a row (and of the next) in flight at once.
 struct SumArgs {
   const void* dy;
   std::int64_t ld;
   int features, vocab;
-  int per_owner;
-  int block;      // entries per block
+  int block;  // entries per block, a multiple of 32
   const int* word;
   const int* pos;
   const int2* span;
   const int* total;
-  float* partial;  // [block][2][features]: a block's share of the word that it starts with,
-                   // and of the word that it ends with
+  float* partial;  // [block][2][features]: a block's share of a word that began before it, and
+                   // of one that began in it and goes on behind it
   void* dw;
   float alpha, beta;
 };
 
+constexpr int kSumThreads = 256, kSumWarps = kSumThreads / 32;
+constexpr int kSumCtas = 4;  // per SM
+
+// A slice of the features: RUNS runs of VEC elements per lane, from h on.
 template <int VEC, int RUNS>
 struct Slice {
-  static constexpr int kFeatures = 32 * VEC * RUNS;
-  float v[RUNS][VEC];
+  static constexpr int kFeatures = 32 * VEC * RUNS, kStep = 32 * VEC;
+  alignas(16) float v[RUNS][VEC];
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int r = 0; r < RUNS; ++r)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) v[r][e] = 0.0f;
   }
-  // Adds features h0 + lane * VEC + r * 32 * VEC of the row.
-  template <typename T>
-  __device__ __forceinline__ void add(const Run<T, VEC> (&in)[RUNS]) {
+};
+
+template <int VEC, int RUNS>
+__device__ __forceinline__ void store_partial(const Slice<VEC, RUNS>& s, float* o, int h,
+                                              int features) {
+#pragma unroll
+  for (int r = 0; r < RUNS; ++r)
+    if (h + r * s.kStep < features)
+      store_run<float, VEC>(o + h + r * s.kStep, *reinterpret_cast<const Run<float, VEC>*>(s.v[r]));
+}
+
+// The slice of a word's row of dw, from its sum.
+template <typename TW, int VEC, int RUNS>
+__device__ __forceinline__ void store_row(const Slice<VEC, RUNS>& s, const SumArgs& a, int word,
+                                          int h) {
+  TW* o = static_cast<TW*>(a.dw) + static_cast<std::int64_t>(word) * a.features + h;
+#pragma unroll
+  for (int r = 0; r < RUNS; ++r) {
+    if (h + r * s.kStep >= a.features) continue;
+    Run<TW, VEC> out, was;
+    if (a.beta != 0.0f) was = load_run<TW, VEC>(o + r * s.kStep);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      float v = a.alpha * s.v[r][e];
+      if (a.beta != 0.0f) v = fmaf(a.beta, static_cast<float>(was.v[e]), v);
+      out.v[e] = from_float<TW>(v);
+    }
+    store_run<TW, VEC>(o + r * s.kStep, out);
+  }
+}
+
+// One block's entries: AHEAD rows are loaded at a time and added in order.
+template <typename T, typename TW, int VEC, int RUNS, int AHEAD>
+__device__ __forceinline__ void sum_block(const SumArgs& a, int b, int h, int total) {
+  const int lane = threadIdx.x & 31;
+  const int i0 = b * a.block, i1 = min(total, i0 + a.block);
+  const T* dy = static_cast<const T*>(a.dy) + h;
+  Slice<VEC, RUNS> sum;
+  sum.clear();
+  int current = a.word[i0];
+  bool began_before = i0 > 0 && a.word[i0 - 1] == current;
+  const auto finish = [&](bool goes_on) {
+    if (began_before || goes_on)
+      store_partial(sum, a.partial + (2ll * b + !began_before) * a.features, h, a.features);
+    else
+      store_row<TW>(sum, a, current, h);
+  };
+  for (int i = i0; i < i1; i += 32) {
+    const int n = min(32, i1 - i);
+    const int my_pos = lane < n ? a.pos[i + lane] : 0;
+    const int my_word = lane < n ? a.word[i + lane] : 0;
+    for (int j = 0; j < n; j += AHEAD) {
+      Run<T, VEC> in[AHEAD][RUNS];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int p = __shfl_sync(0xffffffffu, my_pos, (j + k) & 31);
+        if (j + k >= n) continue;
+#pragma unroll
+        for (int r = 0; r < RUNS; ++r)
+          if (h + r * sum.kStep < a.features)
+            in[k][r] = load_run<T, VEC>(dy + p * a.ld + r * sum.kStep);
+      }
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int w = __shfl_sync(0xffffffffu, my_word, (j + k) & 31);
+        if (j + k >= n) continue;
+        if (w != current) {
+          finish(false);
+          sum.clear();
+          current = w;
+          began_before = false;
+        }
+#pragma unroll
+        for (int r = 0; r < RUNS; ++r)
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) sum.v[r][e] += static_cast<float>(in[k][r].v[e]);
+      }
+    }
+  }
+  finish(i1 < total && a.word[i1] == current);
+}
+
+constexpr int kFillRows = 8;
+
+// Rows of words that do not occur: zeros, or beta dw.
+template <typename TW, int VEC>
+__device__ __forceinline__ void fill_rows(const SumArgs& a, int first) {
+  const int lane = threadIdx.x & 31;
+  const int v = first + lane;
+  const bool absent = lane < kFillRows && v < a.vocab && a.span[v].y == 0;
+  unsigned rows = __ballot_sync(0xffffffffu, absent);
+  while (rows != 0) {
+    const int row = first + __ffs(rows) - 1;
+    rows &= rows - 1;
+    TW* o = static_cast<TW*>(a.dw) + static_cast<std::int64_t>(row) * a.features;
+    if (a.beta != 0.0f) {
+      for (int h = lane * VEC; h < a.features; h += 32 * VEC) {
+        Run<TW, VEC> x = load_run<TW, VEC>(o + h);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          x.v[e] = from_float<TW>(a.beta * static_cast<float>(x.v[e]));
+        store_run<TW, VEC>(o + h, x);
+      }
+      continue;
+    }
+    // elements up to the first 16-byte word, whole words, and the elements behind the last
+    constexpr int kWord = 16 / sizeof(TW);
+    const int lead = min(a.features, static_cast<int>((16 - (reinterpret_cast<std::uintptr_t>(o) & 15)) & 15) /
+                                         static_cast<int>(sizeof(TW)));
+    const int whole = (a.features - lead) / kWord;
+    if (lane < lead) o[lane] = from_float<TW>(0.0f);
+#pragma unroll 4
+    for (int i = lane; i < whole; i += 32)
+      __stcs(reinterpret_cast<uint4*>(o + lead) + i, make_uint4(0, 0, 0, 0));
+    const int rest = lead + whole * kWord + lane;
+    if (rest < a.features) o[rest] = from_float<TW>(0.0f);
+  }
+}
+
+// A warp takes a block's slice, or rows to fill, at a time: the sums first, so that their
+// latency hides behind the filling, which takes all the bandwidth that is left.
+template <typename T, typename TW, int VEC, int RUNS, int AHEAD>
+__global__ void __launch_bounds__(kSumThreads, kSumCtas) embedding_sum_kernel(const SumArgs a) {
+  tc::grid_launch_next();
+  tc::grid_wait_previous();
+  using S = Slice<VEC, RUNS>;
+  const unsigned slices = (a.features + S::kFeatures - 1) / S::kFeatures;
+  const int total = *a.total;
+  const std::int64_t sums = static_cast<std::int64_t>((total + a.block - 1) / a.block) * slices;
+  const std::int64_t fills = a.beta == 1.0f ? 0 : (a.vocab + kFillRows - 1) / kFillRows;
+  const std::int64_t step = static_cast<std::int64_t>(gridDim.x) * kSumWarps;
+  for (std::int64_t u = static_cast<std::int64_t>(blockIdx.x) * kSumWarps + (threadIdx.x >> 5);
+       u < sums + fills; u += step) {
+    if (u < sums) {
+      const int b = static_cast<int>(u / slices);
+      const int h = static_cast<int>(u - b * static_cast<std::int64_t>(slices)) * S::kFeatures +
+                    (threadIdx.x & 31) * VEC;
+      sum_block<T, TW, VEC, RUNS, AHEAD>(a, b, h, total);
+    } else {
+      fill_rows<TW, VEC>(a, static_cast<int>(u - sums) * kFillRows);
+    }
+  }
+}
+
+constexpr int kJoinAlone = 32;
+
+// The word that goes on from block b - 1, where it began, into block b: a CTA has kSumWarps
+// slices of it, a warp each; a word of more than kJoinAlone blocks takes the whole CTA for each
+// slice.
+template <typename TW, int VEC, int RUNS>
+__global__ void __launch_bounds__(kSumThreads) embedding_join_kernel(const SumArgs a) {
+  tc::grid_launch_next();
+  tc::grid_wait_previous();
+  using S = Slice<VEC, RUNS>;
+  __shared__ float shared[kSumWarps][S::kFeatures];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int slices = (a.features + S::kFeatures - 1) / S::kFeatures;
+  const int groups = (slices + kSumWarps - 1) / kSumWarps;
+  const int b = static_cast<int>(blockIdx.x / groups) + 1;
+  const int first = static_cast<int>(blockIdx.x % groups) * kSumWarps;
+  const std::int64_t at = static_cast<std::int64_t>(b) * a.block;
+  if (at >= *a.total) return;
+  const int word = a.word[at];
+  if (a.word[at - 1] != word) return;
+  const int2 span = a.span[word];
+  if (span.x < at - a.block) return;  // it began earlier
+  const int n = (span.y - 1) / a.block - b + 2;  // blocks from b - 1 on
+  const auto add = [&](S& s, int k0, int k1, int h) {
+#pragma unroll 4
+    for (int k = k0; k < k1; ++k) {
+      const float* p = a.partial + (2ll * (b - 1 + k) + (k == 0 ? 1 : 0)) * a.features + h;
+#pragma unroll
+      for (int r = 0; r < RUNS; ++r) {
+        if (h + r * S::kStep >= a.features) continue;
+        const Run<float, VEC> x = load_run<float, VEC>(p + r * S::kStep);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s.v[r][e] += x.v[e];
+      }
+    }
+  };
+  S sum;
+  if (n <= kJoinAlone) {
+    const int h = (first + warp) * S::kFeatures + lane * VEC;
+    if (first + warp >= slices) return;
+    sum.clear();
+    add(sum, 0, n, h);
+    store_row<TW>(sum, a, word, h);
+    return;
+  }
+  const int each = (n + kSumWarps - 1) / kSumWarps;
+  for (int slice = first; slice < min(slices, first + kSumWarps); ++slice) {
+    const int h = slice * S::kFeatures + lane * VEC;
+    sum.clear();
+    add(sum, min(n, warp * each), min(n, (warp + 1) * each), h);
 #pragma unroll
     for (int r = 0; r < RUNS; ++r)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[r][e] += static_cast<float>(in[r].v[e]);
-  }
-};
-
-template <typename T, int VEC, int RUNS>
-__device__ __forceinline__ void load_slice(Run<T, VEC> (&in)[RUNS], const T* row, int h,
-                                           int features) {
+      for (int e = 0; e < VEC; ++e) shared[warp][(r * VEC + e) * 32 + lane] = sum.v[r][e];
+    __syncthreads();
+    if (warp == 0) {
+      for (int w = 1; w < kSumWarps; ++w)
 #pragma unroll
-  for (int r = 0; r < RUNS; ++r)
-    if (h + r * 32 * VEC < features) in[r] = load_run<T, VEC>(row + h + r * 32 * VEC);
-}
-
-// Rows pos[i0..i1) of dy.
-template <typename T, int VEC, int RUNS>
-__device__ __forceinline__ void add_rows(Slice<VEC, RUNS>& s, const SumArgs& a, int i0, int i1,
-                                         int h) {
-  const T* dy = static_cast<const T*>(a.dy);
-  constexpr int kAhead = 2;
-  Run<T, VEC> in[kAhead][RUNS] = {};
-  int i = i0;
-  for (; i + kAhead <= i1; i += kAhead) {
+        for (int r = 0; r < RUNS; ++r)
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      load_slice<T, VEC, RUNS>(in[k], dy + a.pos[i + k] * a.ld, h, a.features);
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) s.add(in[k]);
-  }
-  for (; i < i1; ++i) {
-    load_slice<T, VEC, RUNS>(in[0], dy + a.pos[i] * a.ld, h, a.features);
-    s.add(in[0]);
-  }
-}
-
-constexpr int kSumThreads = 256, kSumWarps = kSumThreads / 32;
-
-template <typename T, int VEC, int RUNS>
-__global__ void __launch_bounds__(kSumThreads) embedding_partial_kernel(const SumArgs a) {
-  tc::grid_launch_next();
-  tc::grid_wait_previous();
-  const int lane = threadIdx.x & 31;
-  const int slices = (a.features + Slice<VEC, RUNS>::kFeatures - 1) / Slice<VEC, RUNS>::kFeatures;
-  const int total = *a.total;
-  const std::int64_t units = static_cast<std::int64_t>((total + a.block - 1) / a.block) * slices;
-  for (std::int64_t u = static_cast<std::int64_t>(blockIdx.x) * kSumWarps + (threadIdx.x >> 5);
-       u < units; u += static_cast<std::int64_t>(gridDim.x) * kSumWarps) {
-    const std::int64_t b = u / slices;
-    const int h = static_cast<int>(u - b * slices) * Slice<VEC, RUNS>::kFeatures + lane * VEC;
-    const int i0 = static_cast<int>(b * a.block), i1 = min(total, i0 + a.block);
-    const int2 head = span_of(a.span, a.per_owner, a.word[i0]);
-    const int2 tail = span_of(a.span, a.per_owner, a.word[i1 - 1]);
-#pragma unroll 1
-    for (int k = 0; k < 2; ++k) {
-      const int2 s = k == 0 ? head : tail;
-      if (s.y - s.x <= a.block || (k == 1 && s.x <= i0)) continue;
-      Slice<VEC, RUNS> sum;
-      sum.clear();
-      add_rows<T, VEC, RUNS>(sum, a, max(i0, s.x), min(i1, s.y), h);
-      float* o = a.partial + (2 * b + k) * a.features + h;
-#pragma unroll
-      for (int r = 0; r < RUNS; ++r) {
-        if (h + r * 32 * VEC >= a.features) continue;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) o[r * 32 * VEC + e] = sum.v[r][e];
-      }
+          for (int e = 0; e < VEC; ++e) sum.v[r][e] += shared[w][(r * VEC + e) * 32 + lane];
+      store_row<TW>(sum, a, word, h);
     }
-  }
-}
-
-// TOUCHED: only the words that occur (beta 1), found among the entries; else all words.
-template <typename T, typename TW, int VEC, int RUNS, bool TOUCHED>
-__global__ void __launch_bounds__(kSumThreads) embedding_rows_kernel(const SumArgs a) {
-  tc::grid_launch_next();
-  tc::grid_wait_previous();
-  const int lane = threadIdx.x & 31;
-  const int slices = (a.features + Slice<VEC, RUNS>::kFeatures - 1) / Slice<VEC, RUNS>::kFeatures;
-  const std::int64_t units = static_cast<std::int64_t>(TOUCHED ? *a.total : a.vocab) * slices;
-  for (std::int64_t u = static_cast<std::int64_t>(blockIdx.x) * kSumWarps + (threadIdx.x >> 5);
-       u < units; u += static_cast<std::int64_t>(gridDim.x) * kSumWarps) {
-    const int i = static_cast<int>(u / slices);
-    const int h = static_cast<int>(u % slices) * Slice<VEC, RUNS>::kFeatures + lane * VEC;
-    int word = i;
-    if constexpr (TOUCHED) {
-      word = a.word[i];
-      if (i > 0 && a.word[i - 1] == word) continue;
-    }
-    const int2 s = span_of(a.span, a.per_owner, word);
-    Slice<VEC, RUNS> sum;
-    sum.clear();
-    if (s.y - s.x <= a.block) {
-      add_rows<T, VEC, RUNS>(sum, a, s.x, s.y, h);
-    } else {
-      for (int b = s.x / a.block; b <= (s.y - 1) / a.block; ++b) {
-        const int k = b * static_cast<std::int64_t>(a.block) < s.x ? 1 : 0;
-        const float* p = a.partial + (2ll * b + k) * a.features;
-#pragma unroll
-        for (int r = 0; r < RUNS; ++r) {
-          if (h + r * 32 * VEC >= a.features) continue;
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) sum.v[r][e] += p[h + r * 32 * VEC + e];
-        }
-      }
-    }
-    TW* o = static_cast<TW*>(a.dw) + static_cast<std::int64_t>(word) * a.features + h;
-#pragma unroll
-    for (int r = 0; r < RUNS; ++r) {
-      if (h + r * 32 * VEC >= a.features) continue;
-      Run<TW, VEC> out, was;
-      if (a.beta != 0.0f) was = load_run<TW, VEC>(o + r * 32 * VEC);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        // a word that does not occur has no sum for an infinite alpha to multiply
-        float v = s.y > s.x ? a.alpha * sum.v[r][e] : 0.0f;
-        if (a.beta != 0.0f) v = fmaf(a.beta, static_cast<float>(was.v[e]), v);
-        out.v[e] = from_float<TW>(v);
-      }
-      store_run<TW, VEC>(o + r * 32 * VEC, out);
-    }
+    __syncthreads();
   }
 }
 
 // ------------------------------------------------------------------------- planning --
-// Entries per block: long enough that the partial sums of frequent words are few, short enough
-// that one warp's share of a block or of a word is (the square root of the tokens balances the
-// two, for a word that all of them are).
+// Entries per block: a warp's batch of loads, longer only where that would leave more than
+// 1024 partial sums of one word.
 int block_entries(int tokens) {
-  int n = 16;
-  while (n < 512 && 4ll * n * n < tokens) n *= 2;
+  int n = 32;
+  while (tokens / n > 1024) n *= 2;
   return n;
 }
 
 struct SortPlan {
-  int per_owner, passes, block;
+  int passes, block;
   std::size_t list[2], word, pos, span, total, partial, bytes;
 };
 
 SortPlan plan(const EmbeddingArgs& a) {
   SortPlan p{};
-  p.per_owner = (a.vocab + kOwners - 1) / kOwners;
-  while ((p.per_owner - 1) >> (p.passes * kDigit) != 0) ++p.passes;
+  while ((a.vocab - 1) >> kOwnerBits >> (p.passes * kDigit) != 0) ++p.passes;
   p.block = block_entries(a.tokens);
   std::size_t at = 0;
   const auto take = [&](std::size_t n) {
@@ -476,29 +566,28 @@ SortPlan plan(const EmbeddingArgs& a) {
   for (std::size_t& l : p.list) l = take(a.tokens > kSharedList ? T * sizeof(Entry) : 0);
   p.word = take(T * 4);
   p.pos = take(T * 4);
-  p.span = take(static_cast<std::size_t>(p.per_owner) * kOwners * sizeof(int2));
+  p.span = take(a.vocab * sizeof(int2));
   p.total = take(4);
   p.partial = take((T + p.block - 1) / p.block * 2 * H * 4);
   p.bytes = at;
   return p;
 }
 
-unsigned grid_of(std::int64_t units, int per_cta, int per_sm) {
-  const std::int64_t ctas = (units + per_cta - 1) / per_cta;
-  return static_cast<unsigned>(
-      std::max<std::int64_t>(1, std::min<std::int64_t>(ctas, std::int64_t{sms()} * per_sm)));
-}
+// Rows per thread of the lookup: one where the GPU has room for a thread per run.
+constexpr int kLookupRows = 4;
 
-template <typename TW, typename TY, int VEC, int RUNS>
+template <typename TW, typename TY, int VEC>
 cudaError_t lookup(const EmbeddingArgs& a, cudaStream_t st) {
-  const std::int64_t runs = static_cast<std::int64_t>(a.tokens) * (a.features / VEC);
-  const std::int64_t per = kLookupThreads * RUNS;
-  const std::int64_t ctas = (runs + per - 1) / per;
+  const std::int64_t per = a.features / VEC;
+  const bool one = a.tokens * per <= std::int64_t{sms()} * 2048;
+  const int stride = one ? a.tokens : (a.tokens + kLookupRows - 1) / kLookupRows;
+  const std::int64_t ctas = (stride * per + kLookupThreads - 1) / kLookupThreads;
   if (ctas > INT32_MAX) return cudaErrorInvalidValue;
-  return tc::launch_overlapped(embedding_kernel<TW, TY, VEC, RUNS>,
-                               dim3(static_cast<unsigned>(ctas)), kLookupThreads, 0, st, false,
-                               static_cast<const TW*>(a.w), a.token, static_cast<TY*>(a.row),
-                               a.ld, a.tokens, a.features, a.vocab, a.alpha, a.beta);
+  return tc::launch_overlapped(
+      one ? embedding_kernel<TW, TY, VEC, 1> : embedding_kernel<TW, TY, VEC, kLookupRows>,
+      dim3(static_cast<unsigned>(ctas)), kLookupThreads, 0, st, false,
+      static_cast<const TW*>(a.w), a.token, static_cast<TY*>(a.row), a.ld, a.tokens, a.features,
+      a.vocab, stride, a.alpha, a.beta);
 }
 
 // Whether every row of both operands is whole runs of VEC elements on 16-byte boundaries.
@@ -508,14 +597,13 @@ bool rows_of_runs(const EmbeddingArgs& a, int vec) {
          (a.tokens == 1 || a.ld * rs % 16 == 0) && a.features * ws % 16 == 0;
 }
 
-template <typename T, typename TW, int VEC, int RUNS>
+template <typename T, typename TW, int VEC, int RUNS, int AHEAD>
 cudaError_t gradient(const EmbeddingArgs& a, const SortPlan& p, char* ws, cudaStream_t st) {
   SumArgs s{};
   s.dy = a.row;
   s.ld = a.ld;
   s.features = a.features;
   s.vocab = a.vocab;
-  s.per_owner = p.per_owner;
   s.block = p.block;
   s.word = reinterpret_cast<int*>(ws + p.word);
   s.pos = reinterpret_cast<int*>(ws + p.pos);
@@ -528,18 +616,18 @@ cudaError_t gradient(const EmbeddingArgs& a, const SortPlan& p, char* ws, cudaSt
   constexpr int kSlice = Slice<VEC, RUNS>::kFeatures;
   const std::int64_t slices = (a.features + kSlice - 1) / kSlice;
   const std::int64_t blocks = (a.tokens + p.block - 1) / p.block;
-  if (a.tokens > p.block) {  // else no word is long
-    const cudaError_t e = tc::launch_overlapped(
-        embedding_partial_kernel<T, VEC, RUNS>, dim3(grid_of(blocks * slices, kSumWarps, 8)),
-        kSumThreads, 0, st, true, s);
-    if (e != cudaSuccess) return e;
-  }
-  const bool touched = a.beta == 1.0f;
-  const std::int64_t rows = touched ? a.tokens : a.vocab;
-  return tc::launch_overlapped(touched ? embedding_rows_kernel<T, TW, VEC, RUNS, true>
-                                       : embedding_rows_kernel<T, TW, VEC, RUNS, false>,
-                               dim3(grid_of(rows * slices, kSumWarps, 8)), kSumThreads, 0, st,
-                               true, s);
+  const std::int64_t units =
+      blocks * slices + (a.beta == 1.0f ? 0 : (a.vocab + kFillRows - 1) / kFillRows);
+  const std::int64_t ctas =
+      std::min<std::int64_t>((units + kSumWarps - 1) / kSumWarps, sms() * kSumCtas);
+  const cudaError_t e = tc::launch_overlapped(embedding_sum_kernel<T, TW, VEC, RUNS, AHEAD>,
+                                              dim3(static_cast<unsigned>(ctas)), kSumThreads, 0,
+                                              st, true, s);
+  if (e != cudaSuccess || blocks == 1) return e;
+  const std::int64_t joins = (blocks - 1) * ((slices + kSumWarps - 1) / kSumWarps);
+  if (joins > INT32_MAX) return cudaErrorInvalidValue;
+  return tc::launch_overlapped(embedding_join_kernel<TW, VEC, RUNS>,
+                               dim3(static_cast<unsigned>(joins)), kSumThreads, 0, st, true, s);
 }
 
 }  // namespace
@@ -548,17 +636,32 @@ cudaError_t launch_embedding(const EmbeddingArgs& a, cudaStream_t st) noexcept {
   using T = EmbeddingType;
   const bool wide = rows_of_runs(a, a.rows == T::kF32 ? 4 : 8);
   if (a.rows == T::kF32)
-    return wide ? lookup<float, float, 4, 4>(a, st) : lookup<float, float, 1, 8>(a, st);
+    return wide ? lookup<float, float, 4>(a, st) : lookup<float, float, 1>(a, st);
   if (a.rows == T::kF16) {
     if (a.table == T::kF32)
-      return wide ? lookup<float, __half, 8, 2>(a, st) : lookup<float, __half, 1, 8>(a, st);
-    return wide ? lookup<__half, __half, 8, 4>(a, st) : lookup<__half, __half, 1, 8>(a, st);
+      return wide ? lookup<float, __half, 8>(a, st) : lookup<float, __half, 1>(a, st);
+    return wide ? lookup<__half, __half, 8>(a, st) : lookup<__half, __half, 1>(a, st);
   }
   if (a.table == T::kF32)
-    return wide ? lookup<float, __nv_bfloat16, 8, 2>(a, st)
-                : lookup<float, __nv_bfloat16, 1, 8>(a, st);
-  return wide ? lookup<__nv_bfloat16, __nv_bfloat16, 8, 4>(a, st)
-              : lookup<__nv_bfloat16, __nv_bfloat16, 1, 8>(a, st);
+    return wide ? lookup<float, __nv_bfloat16, 8>(a, st)
+                : lookup<float, __nv_bfloat16, 1>(a, st);
+  return wide ? lookup<__nv_bfloat16, __nv_bfloat16, 8>(a, st)
+              : lookup<__nv_bfloat16, __nv_bfloat16, 1>(a, st);
+}
+
+// Lets the sort use the shared memory that its tokens take, once per device.
+static bool sort_attributes() noexcept {
+  static std::atomic<unsigned long long> set{0};
+  const int dev = current_device();
+  if (dev < 0 || dev >= 64) return false;
+  if ((set.load(std::memory_order_acquire) >> dev & 1ull) != 0) return true;
+  if (cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           kSharedTokens * sizeof(int)) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return false;
+  }
+  set.fetch_or(1ull << dev, std::memory_order_release);
+  return true;
 }
 
 std::size_t embedding_gradient_workspace(const EmbeddingArgs& a) noexcept { return plan(a).bytes; }
@@ -572,32 +675,33 @@ cudaError_t launch_embedding_gradient(const EmbeddingArgs& a, void* workspace,
   s.token = a.token;
   s.tokens = a.tokens;
   s.vocab = a.vocab;
-  s.per_owner = p.per_owner;
   s.passes = p.passes;
   for (int i = 0; i < 2; ++i) s.list[i] = reinterpret_cast<Entry*>(ws + p.list[i]);
   s.word = reinterpret_cast<int*>(ws + p.word);
   s.pos = reinterpret_cast<int*>(ws + p.pos);
   s.span = reinterpret_cast<int2*>(ws + p.span);
   s.total = reinterpret_cast<int*>(ws + p.total);
-  const cudaError_t e =
-      tc::launch_overlapped(embedding_sort_kernel, dim3(kOwners), kSortThreads, 0, st, false, s);
+  if (!sort_attributes()) return cudaErrorInvalidDevice;
+  const std::size_t cached = a.tokens <= kSharedTokens ? a.tokens * sizeof(int) : 0;
+  const cudaError_t e = tc::launch_overlapped(embedding_sort_kernel, dim3(kOwners), kSortThreads,
+                                              cached, st, false, s);
   if (e != cudaSuccess) return e;
   const bool wide = rows_of_runs(a, a.rows == T::kF32 ? 4 : 8);
   if (a.rows == T::kF32)
-    return wide ? gradient<float, float, 4, 4>(a, p, ws, st)
-                : gradient<float, float, 1, 8>(a, p, ws, st);
+    return wide ? gradient<float, float, 4, 1, 4>(a, p, ws, st)
+                : gradient<float, float, 1, 4, 4>(a, p, ws, st);
   if (a.rows == T::kF16) {
     if (a.table == T::kF32)
-      return wide ? gradient<__half, float, 8, 2>(a, p, ws, st)
-                  : gradient<__half, float, 1, 8>(a, p, ws, st);
-    return wide ? gradient<__half, __half, 8, 4>(a, p, ws, st)
-                : gradient<__half, __half, 1, 8>(a, p, ws, st);
+      return wide ? gradient<__half, float, 8, 1, 4>(a, p, ws, st)
+                  : gradient<__half, float, 1, 4, 4>(a, p, ws, st);
+    return wide ? gradient<__half, __half, 8, 1, 4>(a, p, ws, st)
+                : gradient<__half, __half, 1, 4, 4>(a, p, ws, st);
   }
   if (a.table == T::kF32)
-    return wide ? gradient<__nv_bfloat16, float, 8, 2>(a, p, ws, st)
-                : gradient<__nv_bfloat16, float, 1, 8>(a, p, ws, st);
-  return wide ? gradient<__nv_bfloat16, __nv_bfloat16, 8, 4>(a, p, ws, st)
-              : gradient<__nv_bfloat16, __nv_bfloat16, 1, 8>(a, p, ws, st);
+    return wide ? gradient<__nv_bfloat16, float, 8, 1, 4>(a, p, ws, st)
+                : gradient<__nv_bfloat16, float, 1, 4, 4>(a, p, ws, st);
+  return wide ? gradient<__nv_bfloat16, __nv_bfloat16, 8, 1, 4>(a, p, ws, st)
+              : gradient<__nv_bfloat16, __nv_bfloat16, 1, 4, 4>(a, p, ws, st);
 }
 
 }  // namespace mb200::dnn
