@@ -44,34 +44,97 @@ __device__ __forceinline__ T from_float(float v) {
 
 // VEC elements of a row as they lie in memory: whole 16-byte words, or one element.
 template <typename T, int VEC>
-struct alignas(VEC == 1 ? sizeof(T) : 16) Run {
-  T v[VEC];
+struct Run {
+  static constexpr int kWords = sizeof(T) * VEC / 16;
+  uint4 w[kWords];
+};
+template <typename T>
+struct Run<T, 1> {
+  T v;
 };
 
 template <typename T, int VEC>
 __device__ __forceinline__ Run<T, VEC> load_run(const T* p) {
   Run<T, VEC> r;
   if constexpr (VEC == 1) {
-    r.v[0] = *p;
+    r.v = *p;
   } else {
-    constexpr int kWords = sizeof(T) * VEC / 16;
 #pragma unroll
-    for (int i = 0; i < kWords; ++i)
-      reinterpret_cast<uint4*>(&r)[i] = reinterpret_cast<const uint4*>(p)[i];
+    for (int i = 0; i < r.kWords; ++i) r.w[i] = reinterpret_cast<const uint4*>(p)[i];
   }
   return r;
 }
 
-template <typename T, int VEC>
+// ONCE: written past the rows that L2 should keep.
+template <bool ONCE, typename T, int VEC>
 __device__ __forceinline__ void store_run(T* p, const Run<T, VEC>& r) {
   if constexpr (VEC == 1) {
-    *p = r.v[0];
+    *p = r.v;
   } else {
-    constexpr int kWords = sizeof(T) * VEC / 16;
 #pragma unroll
-    for (int i = 0; i < kWords; ++i)
-      __stcs(reinterpret_cast<uint4*>(p) + i, reinterpret_cast<const uint4*>(&r)[i]);
+    for (int i = 0; i < r.kWords; ++i) {
+      if constexpr (ONCE)
+        __stcs(reinterpret_cast<uint4*>(p) + i, r.w[i]);
+      else
+        reinterpret_cast<uint4*>(p)[i] = r.w[i];
+    }
   }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void unpack(const Run<T, VEC>& r, float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    v[0] = static_cast<float>(r.v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < r.kWords; ++i) {
+      const std::uint32_t w[4] = {r.w[i].x, r.w[i].y, r.w[i].z, r.w[i].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (std::is_same_v<T, float>) {
+          v[4 * i + j] = __uint_as_float(w[j]);
+        } else if constexpr (std::is_same_v<T, __half>) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+          v[8 * i + 2 * j] = f.x;
+          v[8 * i + 2 * j + 1] = f.y;
+        } else {  // bf16 is fp32's upper half
+          v[8 * i + 2 * j] = __uint_as_float(w[j] << 16);
+          v[8 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        }
+      }
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ std::uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same_v<T, __half>) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const std::uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const std::uint32_t*>(&h);
+  }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ Run<T, VEC> pack(const float (&v)[VEC]) {
+  Run<T, VEC> r;
+  if constexpr (VEC == 1) {
+    r.v = from_float<T>(v[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < r.kWords; ++i) {
+      if constexpr (std::is_same_v<T, float>)
+        r.w[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]),
+                            __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
+      else
+        r.w[i] = make_uint4(
+            pack2<T>(v[8 * i], v[8 * i + 1]), pack2<T>(v[8 * i + 2], v[8 * i + 3]),
+            pack2<T>(v[8 * i + 4], v[8 * i + 5]), pack2<T>(v[8 * i + 6], v[8 * i + 7]));
+    }
+  }
+  return r;
 }
 
 // ------------------------------------------------------------------------- lookup --
@@ -80,7 +143,7 @@ constexpr int kLookupThreads = 256;
 // A thread has one column of ROWS rows that lie `stride` apart, so the loads of its tokens, of
 // their words' runs and its stores are ROWS at a time and one division finds them all.
 template <typename TW, typename TY, int VEC, int ROWS>
-__global__ void __launch_bounds__(kLookupThreads)
+__global__ void __launch_bounds__(kLookupThreads, ROWS == 1 ? 8 : 5)
     embedding_kernel(const TW* __restrict__ w, const std::int64_t* __restrict__ token, TY* y,
                      std::int64_t ldy, int tokens, int features, int vocab, int stride,
                      float alpha, float beta) {
@@ -110,17 +173,21 @@ __global__ void __launch_bounds__(kLookupThreads)
   for (int j = 0; j < ROWS; ++j) {
     if (row + j * stride >= tokens) break;
     TY* o = y + (row + j * stride) * ldy + col;
-    Run<TY, VEC> out, was;
-    if (beta != 0.0f) was = load_run<TY, VEC>(o);
+    float v[VEC];
+    unpack<TW, VEC>(in[j], v);
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      float v = alpha * static_cast<float>(in[j].v[e]);
+      v[e] *= alpha;
       if (static_cast<unsigned>(word[j]) >= static_cast<unsigned>(vocab))
-        v = word[j] < 0 ? 0.0f : NAN;
-      if (beta != 0.0f) v = fmaf(beta, static_cast<float>(was.v[e]), v);
-      out.v[e] = from_float<TY>(v);
+        v[e] = word[j] < 0 ? 0.0f : NAN;
     }
-    store_run<TY, VEC>(o, out);
+    if (beta != 0.0f) {
+      float was[VEC];
+      unpack<TY, VEC>(load_run<TY, VEC>(o), was);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] = fmaf(beta, was[e], v[e]);
+    }
+    store_run<false>(o, pack<TY, VEC>(v));
   }
 }
 
@@ -135,8 +202,8 @@ __global__ void __launch_bounds__(kLookupThreads)
 constexpr int kOwners = 128, kOwnerBits = 7;
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kDigit = 5;
-constexpr int kSharedList = 2048;     // entries that are sorted in shared memory
-constexpr int kSharedTokens = 40960;  // tokens whose words it keeps between the two readings
+constexpr int kSharedList = 4096;     // entries that are sorted in shared memory
+constexpr int kSharedTokens = 32768;  // tokens whose words it keeps between the two readings
 constexpr int kScanAhead = 8;         // loads in flight per lane
 
 struct Entry {
@@ -148,6 +215,7 @@ struct SortArgs {
   const std::int64_t* token;
   int tokens, vocab;
   int passes;
+  int near_list;   // min(tokens, kSharedList)
   Entry* list[2];  // [tokens] each: longer lists while they are sorted
   int* word;       // [tokens] out: the words in order
   int* pos;        // [tokens] out: and their positions
@@ -185,8 +253,8 @@ __device__ __forceinline__ int block_exclusive(int v, int* warps, int* all) {
 }
 
 __global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const SortArgs a) {
-  extern __shared__ int cached[];  // the tokens' words, -1 for those that enter nothing
-  __shared__ Entry near[2][kSharedList];
+  extern __shared__ Entry near[];  // two lists of near_list entries
+  int* cached = reinterpret_cast<int*>(near + 2 * a.near_list);  // the tokens' words, -1: none
   __shared__ int count[1 << kDigit][kSortWarps + 1];  // a warp's counters in banks of their own
   __shared__ int warps[32];
   tc::grid_launch_next();
@@ -228,8 +296,8 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const S
   at = __shfl_sync(0xffffffffu, at, 0);
   if (owner == kOwners - 1 && threadIdx.x == 0) *a.total = base + n;
 
-  Entry* from = n <= kSharedList ? near[0] : a.list[0] + base;
-  Entry* to = n <= kSharedList ? near[1] : a.list[1] + base;
+  Entry* from = n <= a.near_list ? near : a.list[0] + base;
+  Entry* to = n <= a.near_list ? near + a.near_list : a.list[1] + base;
   if (mine > 0) {
     for (std::int64_t t = t0; t < t1; t += 32 * kScanAhead) {
       int v[kScanAhead];
@@ -314,13 +382,13 @@ struct SumArgs {
 };
 
 constexpr int kSumThreads = 256, kSumWarps = kSumThreads / 32;
-constexpr int kSumCtas = 4;  // per SM
+constexpr int kSumCtas = 3;  // per SM
 
 // A slice of the features: RUNS runs of VEC elements per lane, from h on.
 template <int VEC, int RUNS>
 struct Slice {
   static constexpr int kFeatures = 32 * VEC * RUNS, kStep = 32 * VEC;
-  alignas(16) float v[RUNS][VEC];
+  float v[RUNS][VEC];
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int r = 0; r < RUNS; ++r)
@@ -335,84 +403,95 @@ __device__ __forceinline__ void store_partial(const Slice<VEC, RUNS>& s, float* 
 #pragma unroll
   for (int r = 0; r < RUNS; ++r)
     if (h + r * s.kStep < features)
-      store_run<float, VEC>(o + h + r * s.kStep, *reinterpret_cast<const Run<float, VEC>*>(s.v[r]));
+      store_run<false>(o + h + r * s.kStep, pack<float, VEC>(s.v[r]));
 }
 
-// The slice of a word's row of dw, from its sum.
-template <typename TW, int VEC, int RUNS>
-__device__ __forceinline__ void store_row(const Slice<VEC, RUNS>& s, const SumArgs& a, int word,
-                                          int h) {
-  TW* o = static_cast<TW*>(a.dw) + static_cast<std::int64_t>(word) * a.features + h;
+// The slice of a word's row of dw (o: at h), from its sum and what it was.
+template <bool UPDATE, typename TW, int VEC, int RUNS>
+__device__ __forceinline__ void store_row(const Slice<VEC, RUNS>& s, const SumArgs& a, TW* o, int h,
+                                          const Run<TW, VEC> (&was)[RUNS]) {
 #pragma unroll
   for (int r = 0; r < RUNS; ++r) {
     if (h + r * s.kStep >= a.features) continue;
-    Run<TW, VEC> out, was;
-    if (a.beta != 0.0f) was = load_run<TW, VEC>(o + r * s.kStep);
+    float v[VEC];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      float v = a.alpha * s.v[r][e];
-      if (a.beta != 0.0f) v = fmaf(a.beta, static_cast<float>(was.v[e]), v);
-      out.v[e] = from_float<TW>(v);
+    for (int e = 0; e < VEC; ++e) v[e] = a.alpha * s.v[r][e];
+    if constexpr (UPDATE) {
+      float old[VEC];
+      unpack<TW, VEC>(was[r], old);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] = fmaf(a.beta, old[e], v[e]);
     }
-    store_run<TW, VEC>(o + r * s.kStep, out);
+    store_run<true>(o + r * s.kStep, pack<TW, VEC>(v));
   }
 }
 
-// One block's entries: AHEAD rows are loaded at a time and added in order.
-template <typename T, typename TW, int VEC, int RUNS, int AHEAD>
+// One block's entries: AHEAD rows are loaded at a time and added in order; with beta also the
+// rows of dw of the words that end among them, whose latency would otherwise be a word's each
+// (two micro-batches of 32768 x 2048: 82 -> XX us for the second).
+template <bool UPDATE, typename T, typename TW, int VEC, int RUNS, int AHEAD>
 __device__ __forceinline__ void sum_block(const SumArgs& a, int b, int h, int total) {
   const int lane = threadIdx.x & 31;
   const int i0 = b * a.block, i1 = min(total, i0 + a.block);
   const T* dy = static_cast<const T*>(a.dy) + h;
+  TW* dw = static_cast<TW*>(a.dw) + h;
+  constexpr int kStep = Slice<VEC, RUNS>::kStep;
   Slice<VEC, RUNS> sum;
   sum.clear();
-  int current = a.word[i0];
-  bool began_before = i0 > 0 && a.word[i0 - 1] == current;
-  const auto finish = [&](bool goes_on) {
-    if (began_before || goes_on)
-      store_partial(sum, a.partial + (2ll * b + !began_before) * a.features, h, a.features);
-    else
-      store_row<TW>(sum, a, current, h);
-  };
+  bool began_before = i0 > 0 && a.word[i0 - 1] == a.word[i0];
+  float* partial = a.partial + 2ll * b * a.features;
+  bool open = false;  // the last entry's word goes on behind the block
   for (int i = i0; i < i1; i += 32) {
     const int n = min(32, i1 - i);
     const int my_pos = lane < n ? a.pos[i + lane] : 0;
-    const int my_word = lane < n ? a.word[i + lane] : 0;
+    const int my_word = lane < n ? a.word[i + lane] : -1;
+    const int next = i + lane + 1 < total ? a.word[i + lane + 1] : -1;
+    const unsigned ends = __ballot_sync(0xffffffffu, my_word != next);
+    open = (ends >> (n - 1) & 1u) == 0;
     for (int j = 0; j < n; j += AHEAD) {
       Run<T, VEC> in[AHEAD][RUNS];
+      Run<TW, VEC> was[AHEAD][RUNS];
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         const int p = __shfl_sync(0xffffffffu, my_pos, (j + k) & 31);
+        const int w = __shfl_sync(0xffffffffu, my_word, (j + k) & 31);
         if (j + k >= n) continue;
 #pragma unroll
-        for (int r = 0; r < RUNS; ++r)
-          if (h + r * sum.kStep < a.features)
-            in[k][r] = load_run<T, VEC>(dy + p * a.ld + r * sum.kStep);
+        for (int r = 0; r < RUNS; ++r) {
+          if (h + r * kStep >= a.features) continue;
+          in[k][r] = load_run<T, VEC>(dy + p * a.ld + r * kStep);
+          if (UPDATE && (ends >> (j + k) & 1u) != 0)
+            was[k][r] = load_run<TW, VEC>(dw + static_cast<std::int64_t>(w) * a.features + r * kStep);
+        }
       }
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         const int w = __shfl_sync(0xffffffffu, my_word, (j + k) & 31);
         if (j + k >= n) continue;
-        if (w != current) {
-          finish(false);
-          sum.clear();
-          current = w;
-          began_before = false;
+#pragma unroll
+        for (int r = 0; r < RUNS; ++r) {
+          float v[VEC];
+          unpack<T, VEC>(in[k][r], v);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) sum.v[r][e] += v[e];
         }
-#pragma unroll
-        for (int r = 0; r < RUNS; ++r)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) sum.v[r][e] += static_cast<float>(in[k][r].v[e]);
+        if ((ends >> (j + k) & 1u) == 0) continue;
+        if (began_before)
+          store_partial(sum, partial, h, a.features);
+        else
+          store_row<UPDATE, TW>(sum, a, dw + static_cast<std::int64_t>(w) * a.features, h, was[k]);
+        began_before = false;
+        sum.clear();
       }
     }
   }
-  finish(i1 < total && a.word[i1] == current);
+  if (open) store_partial(sum, partial + (began_before ? 0 : a.features), h, a.features);
 }
 
 constexpr int kFillRows = 8;
 
 // Rows of words that do not occur: zeros, or beta dw.
-template <typename TW, int VEC>
+template <bool UPDATE, typename TW, int VEC>
 __device__ __forceinline__ void fill_rows(const SumArgs& a, int first) {
   const int lane = threadIdx.x & 31;
   const int v = first + lane;
@@ -422,13 +501,13 @@ __device__ __forceinline__ void fill_rows(const SumArgs& a, int first) {
     const int row = first + __ffs(rows) - 1;
     rows &= rows - 1;
     TW* o = static_cast<TW*>(a.dw) + static_cast<std::int64_t>(row) * a.features;
-    if (a.beta != 0.0f) {
+    if constexpr (UPDATE) {
       for (int h = lane * VEC; h < a.features; h += 32 * VEC) {
-        Run<TW, VEC> x = load_run<TW, VEC>(o + h);
+        float v[VEC];
+        unpack<TW, VEC>(load_run<TW, VEC>(o + h), v);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          x.v[e] = from_float<TW>(a.beta * static_cast<float>(x.v[e]));
-        store_run<TW, VEC>(o + h, x);
+        for (int e = 0; e < VEC; ++e) v[e] *= a.beta;
+        store_run<true>(o + h, pack<TW, VEC>(v));
       }
       continue;
     }
@@ -448,7 +527,7 @@ __device__ __forceinline__ void fill_rows(const SumArgs& a, int first) {
 
 // A warp takes a block's slice, or rows to fill, at a time: the sums first, so that their
 // latency hides behind the filling, which takes all the bandwidth that is left.
-template <typename T, typename TW, int VEC, int RUNS, int AHEAD>
+template <bool UPDATE, typename T, typename TW, int VEC, int RUNS, int AHEAD>
 __global__ void __launch_bounds__(kSumThreads, kSumCtas) embedding_sum_kernel(const SumArgs a) {
   tc::grid_launch_next();
   tc::grid_wait_previous();
@@ -464,14 +543,14 @@ __global__ void __launch_bounds__(kSumThreads, kSumCtas) embedding_sum_kernel(co
       const int b = static_cast<int>(u / slices);
       const int h = static_cast<int>(u - b * static_cast<std::int64_t>(slices)) * S::kFeatures +
                     (threadIdx.x & 31) * VEC;
-      sum_block<T, TW, VEC, RUNS, AHEAD>(a, b, h, total);
+      sum_block<UPDATE, T, TW, VEC, RUNS, UPDATE ? AHEAD / 2 : AHEAD>(a, b, h, total);
     } else {
-      fill_rows<TW, VEC>(a, static_cast<int>(u - sums) * kFillRows);
+      fill_rows<UPDATE, TW, VEC>(a, static_cast<int>(u - sums) * kFillRows);
     }
   }
 }
 
-constexpr int kJoinAlone = 32;
+constexpr int kJoinAlone = 128;
 
 // The word that goes on from block b - 1, where it began, into block b: a CTA has kSumWarps
 // slices of it, a warp each; a word of more than kJoinAlone blocks takes the whole CTA for each
@@ -495,16 +574,29 @@ __global__ void __launch_bounds__(kSumThreads) embedding_join_kernel(const SumAr
   if (span.x < at - a.block) return;  // it began earlier
   const int n = (span.y - 1) / a.block - b + 2;  // blocks from b - 1 on
   const auto add = [&](S& s, int k0, int k1, int h) {
-#pragma unroll 4
+#pragma unroll 8
     for (int k = k0; k < k1; ++k) {
       const float* p = a.partial + (2ll * (b - 1 + k) + (k == 0 ? 1 : 0)) * a.features + h;
 #pragma unroll
       for (int r = 0; r < RUNS; ++r) {
         if (h + r * S::kStep >= a.features) continue;
-        const Run<float, VEC> x = load_run<float, VEC>(p + r * S::kStep);
+        float v[VEC];
+        unpack<float, VEC>(load_run<float, VEC>(p + r * S::kStep), v);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) s.v[r][e] += x.v[e];
+        for (int e = 0; e < VEC; ++e) s.v[r][e] += v[e];
       }
+    }
+  };
+  TW* row = static_cast<TW*>(a.dw) + static_cast<std::int64_t>(word) * a.features;
+  const auto store = [&](const S& s, int h) {
+    Run<TW, VEC> was[RUNS];
+    if (a.beta != 0.0f) {
+#pragma unroll
+      for (int r = 0; r < RUNS; ++r)
+        if (h + r * S::kStep < a.features) was[r] = load_run<TW, VEC>(row + h + r * S::kStep);
+      store_row<true, TW>(s, a, row + h, h, was);
+    } else {
+      store_row<false, TW>(s, a, row + h, h, was);
     }
   };
   S sum;
@@ -513,7 +605,7 @@ __global__ void __launch_bounds__(kSumThreads) embedding_join_kernel(const SumAr
     if (first + warp >= slices) return;
     sum.clear();
     add(sum, 0, n, h);
-    store_row<TW>(sum, a, word, h);
+    store(sum, h);
     return;
   }
   const int each = (n + kSumWarps - 1) / kSumWarps;
@@ -532,7 +624,7 @@ __global__ void __launch_bounds__(kSumThreads) embedding_join_kernel(const SumAr
         for (int r = 0; r < RUNS; ++r)
 #pragma unroll
           for (int e = 0; e < VEC; ++e) sum.v[r][e] += shared[w][(r * VEC + e) * 32 + lane];
-      store_row<TW>(sum, a, word, h);
+      store(sum, h);
     }
     __syncthreads();
   }
@@ -620,9 +712,10 @@ cudaError_t gradient(const EmbeddingArgs& a, const SortPlan& p, char* ws, cudaSt
       blocks * slices + (a.beta == 1.0f ? 0 : (a.vocab + kFillRows - 1) / kFillRows);
   const std::int64_t ctas =
       std::min<std::int64_t>((units + kSumWarps - 1) / kSumWarps, sms() * kSumCtas);
-  const cudaError_t e = tc::launch_overlapped(embedding_sum_kernel<T, TW, VEC, RUNS, AHEAD>,
-                                              dim3(static_cast<unsigned>(ctas)), kSumThreads, 0,
-                                              st, true, s);
+  const cudaError_t e =
+      tc::launch_overlapped(a.beta != 0.0f ? embedding_sum_kernel<true, T, TW, VEC, RUNS, AHEAD>
+                                           : embedding_sum_kernel<false, T, TW, VEC, RUNS, AHEAD>,
+                            dim3(static_cast<unsigned>(ctas)), kSumThreads, 0, st, true, s);
   if (e != cudaSuccess || blocks == 1) return e;
   const std::int64_t joins = (blocks - 1) * ((slices + kSumWarps - 1) / kSumWarps);
   if (joins > INT32_MAX) return cudaErrorInvalidValue;
@@ -656,7 +749,8 @@ static bool sort_attributes() noexcept {
   if (dev < 0 || dev >= 64) return false;
   if ((set.load(std::memory_order_acquire) >> dev & 1ull) != 0) return true;
   if (cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           kSharedTokens * sizeof(int)) != cudaSuccess) {
+                           2 * kSharedList * sizeof(Entry) + kSharedTokens * sizeof(int)) !=
+      cudaSuccess) {
     (void)cudaGetLastError();
     return false;
   }
@@ -682,25 +776,27 @@ cudaError_t launch_embedding_gradient(const EmbeddingArgs& a, void* workspace,
   s.span = reinterpret_cast<int2*>(ws + p.span);
   s.total = reinterpret_cast<int*>(ws + p.total);
   if (!sort_attributes()) return cudaErrorInvalidDevice;
-  const std::size_t cached = a.tokens <= kSharedTokens ? a.tokens * sizeof(int) : 0;
+  s.near_list = std::min(a.tokens, kSharedList);
+  const std::size_t shared = 2 * s.near_list * sizeof(Entry) +
+                             (a.tokens <= kSharedTokens ? a.tokens * sizeof(int) : 0);
   const cudaError_t e = tc::launch_overlapped(embedding_sort_kernel, dim3(kOwners), kSortThreads,
-                                              cached, st, false, s);
+                                              shared, st, false, s);
   if (e != cudaSuccess) return e;
   const bool wide = rows_of_runs(a, a.rows == T::kF32 ? 4 : 8);
   if (a.rows == T::kF32)
-    return wide ? gradient<float, float, 4, 1, 4>(a, p, ws, st)
+    return wide ? gradient<float, float, 4, 1, 8>(a, p, ws, st)
                 : gradient<float, float, 1, 4, 4>(a, p, ws, st);
   if (a.rows == T::kF16) {
     if (a.table == T::kF32)
-      return wide ? gradient<__half, float, 8, 1, 4>(a, p, ws, st)
+      return wide ? gradient<__half, float, 8, 1, 8>(a, p, ws, st)
                   : gradient<__half, float, 1, 4, 4>(a, p, ws, st);
-    return wide ? gradient<__half, __half, 8, 1, 4>(a, p, ws, st)
+    return wide ? gradient<__half, __half, 8, 1, 8>(a, p, ws, st)
                 : gradient<__half, __half, 1, 4, 4>(a, p, ws, st);
   }
   if (a.table == T::kF32)
-    return wide ? gradient<__nv_bfloat16, float, 8, 1, 4>(a, p, ws, st)
+    return wide ? gradient<__nv_bfloat16, float, 8, 1, 8>(a, p, ws, st)
                 : gradient<__nv_bfloat16, float, 1, 4, 4>(a, p, ws, st);
-  return wide ? gradient<__nv_bfloat16, __nv_bfloat16, 8, 1, 4>(a, p, ws, st)
+  return wide ? gradient<__nv_bfloat16, __nv_bfloat16, 8, 1, 8>(a, p, ws, st)
               : gradient<__nv_bfloat16, __nv_bfloat16, 1, 4, 4>(a, p, ws, st);
 }
 
