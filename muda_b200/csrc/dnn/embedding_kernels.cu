@@ -4,13 +4,13 @@
 // the words that occur (beta 1).
 //
 // The gradient adds each word's rows in the order of their positions, without atomics, so
-// results are the same on every run.  Three launches:
+// results are the same on every run.  Two launches:
 //   1. embedding_sort_kernel orders the tokens by word, positions ascending within a word;
 //   2. embedding_sum_kernel cuts the ordered tokens into blocks of equal length, whatever words
 //      they hold, and adds each block's rows up in fp32: a word that lies within a block gets
 //      its row of dw, one that crosses into another leaves a partial sum.  Beside that it
-//      writes the rows of the words that do not occur;
-//   3. embedding_join_kernel adds the partial sums of the words that cross blocks.
+//      writes the rows of the words that do not occur.  The warp that leaves a word's last
+//      partial sum adds them up, in the blocks' order (a counter says which that is).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -61,6 +61,19 @@ __device__ __forceinline__ Run<T, VEC> load_run(const T* p) {
   } else {
 #pragma unroll
     for (int i = 0; i < r.kWords; ++i) r.w[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  return r;
+}
+
+// fp32 that other SMs wrote in this launch: from L2.
+template <int VEC>
+__device__ __forceinline__ Run<float, VEC> load_shared_run(const float* p) {
+  Run<float, VEC> r;
+  if constexpr (VEC == 1) {
+    r.v = __ldcg(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < r.kWords; ++i) r.w[i] = __ldcg(reinterpret_cast<const uint4*>(p) + i);
   }
   return r;
 }
@@ -139,55 +152,71 @@ __device__ __forceinline__ Run<T, VEC> pack(const float (&v)[VEC]) {
 
 // ------------------------------------------------------------------------- lookup --
 constexpr int kLookupThreads = 256;
+constexpr int kLookupCtas = 4;  // per SM
 
 // A thread has one column of ROWS rows that lie `stride` apart, so the loads of its tokens, of
-// their words' runs and its stores are ROWS at a time and one division finds them all.
+// their words' runs and its stores are ROWS at a time; it loads the next rows' tokens while
+// this row's runs arrive.
 template <typename TW, typename TY, int VEC, int ROWS>
-__global__ void __launch_bounds__(kLookupThreads, ROWS == 1 ? 8 : 5)
+__global__ void __launch_bounds__(kLookupThreads, kLookupCtas)
     embedding_kernel(const TW* __restrict__ w, const std::int64_t* __restrict__ token, TY* y,
                      std::int64_t ldy, int tokens, int features, int vocab, int stride,
                      float alpha, float beta) {
-  const unsigned per = features / VEC;  // runs of a row
-  const std::int64_t first = static_cast<std::int64_t>(blockIdx.x) * kLookupThreads;
-  const std::int64_t row0 = first / per;
-  const unsigned i = static_cast<unsigned>(first - row0 * per) + threadIdx.x;
-  const unsigned q = i / per;
-  const int col = static_cast<int>(i - q * per) * VEC;
-  const std::int64_t row = row0 + q;
-  if (row >= stride) return;
+  const int per = features / VEC;  // runs of a row
+  const std::int64_t first = static_cast<std::int64_t>(blockIdx.x) * kLookupThreads + threadIdx.x;
+  const std::int64_t step = static_cast<std::int64_t>(gridDim.x) * kLookupThreads;
+  int row = static_cast<int>(min(first / per, static_cast<std::int64_t>(stride)));
+  int col = static_cast<int>(first % per);
+  const int rows_on = static_cast<int>(min(step / per, std::int64_t{1} << 30));
+  const int cols_on = static_cast<int>(step % per);
   int word[ROWS];  // -1: padding, vocab: past the table
+  const auto words = [&](int r) {
 #pragma unroll
-  for (int j = 0; j < ROWS; ++j) {
-    word[j] = -1;
-    if (row + j * stride < tokens) {
-      const std::int64_t v = token[row + j * stride];
-      word[j] = v < 0 ? -1 : v >= vocab ? vocab : static_cast<int>(v);
+    for (int j = 0; j < ROWS; ++j) {
+      word[j] = -1;
+      const std::int64_t t = r + static_cast<std::int64_t>(j) * stride;
+      if (r < stride && t < tokens) {
+        const std::int64_t v = token[t];
+        word[j] = v < 0 ? -1 : v >= vocab ? vocab : static_cast<int>(v);
+      }
     }
-  }
-  Run<TW, VEC> in[ROWS];
+  };
+  words(row);
+  while (row < stride) {
+    Run<TW, VEC> in[ROWS];
+    int is[ROWS];
 #pragma unroll
-  for (int j = 0; j < ROWS; ++j)
-    if (static_cast<unsigned>(word[j]) < static_cast<unsigned>(vocab))
-      in[j] = load_run<TW, VEC>(w + static_cast<std::int64_t>(word[j]) * features + col);
-#pragma unroll
-  for (int j = 0; j < ROWS; ++j) {
-    if (row + j * stride >= tokens) break;
-    TY* o = y + (row + j * stride) * ldy + col;
-    float v[VEC];
-    unpack<TW, VEC>(in[j], v);
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      v[e] *= alpha;
-      if (static_cast<unsigned>(word[j]) >= static_cast<unsigned>(vocab))
-        v[e] = word[j] < 0 ? 0.0f : NAN;
+    for (int j = 0; j < ROWS; ++j) {
+      is[j] = word[j];
+      if (static_cast<unsigned>(is[j]) < static_cast<unsigned>(vocab))
+        in[j] = load_run<TW, VEC>(w + static_cast<std::int64_t>(is[j]) * features + col * VEC);
     }
-    if (beta != 0.0f) {
-      float was[VEC];
-      unpack<TY, VEC>(load_run<TY, VEC>(o), was);
+    const bool wraps = col + cols_on >= per;
+    const int next = row + rows_on + (wraps ? 1 : 0);
+    words(next);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = fmaf(beta, was[e], v[e]);
+    for (int j = 0; j < ROWS; ++j) {
+      const std::int64_t t = row + static_cast<std::int64_t>(j) * stride;
+      if (t >= tokens) break;
+      TY* o = y + t * ldy + col * VEC;
+      float v[VEC];
+      unpack<TW, VEC>(in[j], v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        v[e] *= alpha;
+        if (static_cast<unsigned>(is[j]) >= static_cast<unsigned>(vocab))
+          v[e] = is[j] < 0 ? 0.0f : NAN;
+      }
+      if (beta != 0.0f) {
+        float was[VEC];
+        unpack<TY, VEC>(load_run<TY, VEC>(o), was);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = fmaf(beta, was[e], v[e]);
+      }
+      store_run<false>(o, pack<TY, VEC>(v));
     }
-    store_run<false>(o, pack<TY, VEC>(v));
+    row = next;
+    col += cols_on - (wraps ? per : 0);
   }
 }
 
@@ -228,7 +257,10 @@ struct SortArgs {
   Entry* list[2];  // [tokens] each: longer lists while they are sorted
   int* word;       // [tokens] out: the words in order
   int* pos;        // [tokens] out: and their positions
-  int2* span;      // [vocab] out: a word's entries, {0, 0}: none
+  int2* span;      // [owner][per_owner] out: a word's entries, {0, 0}: none
+  int per_owner;   // words of an owner, at most
+  int* counters;   // out: zeros
+  std::int64_t num_counters;
   int* total;      // out: entries
 };
 
@@ -279,8 +311,11 @@ __global__ void __cluster_dims__(kShare, 1, 1) __launch_bounds__(kSortThreads, 1
   const int owner = blockIdx.x;
   const unsigned before_me = (1u << lane) - 1;
 
-  for (int v = threadIdx.x * kOwners + owner; v < a.vocab; v += kSortThreads * kOwners)
-    a.span[v] = make_int2(0, 0);
+  int2* span = a.span + static_cast<std::int64_t>(owner) * a.per_owner;
+  for (int i = threadIdx.x; i < a.per_owner; i += kSortThreads) span[i] = make_int2(0, 0);
+  for (std::int64_t i = static_cast<std::int64_t>(owner) * kSortThreads + threadIdx.x;
+       i < a.num_counters; i += kOwners * kSortThreads)
+    a.counters[i] = 0;
 
   const int rounds = (a.tokens + a.round - 1) / a.round;
   // Fills keys with round r's tokens and returns how many groups of four they are.
@@ -415,11 +450,10 @@ __global__ void __cluster_dims__(kShare, 1, 1) __launch_bounds__(kSortThreads, 1
 
   for (int i = threadIdx.x; i < n; i += kSortThreads) {
     const Entry e = from[i];
-    const int word = (e.word << kOwnerBits) + owner;
-    a.word[base + i] = word;
+    a.word[base + i] = (e.word << kOwnerBits) + owner;
     a.pos[base + i] = e.pos;
-    if (i == 0 || from[i - 1].word != e.word) a.span[word].x = base + i;
-    if (i == n - 1 || from[i + 1].word != e.word) a.span[word].y = base + i + 1;
+    if (i == 0 || from[i - 1].word != e.word) span[e.word].x = base + i;
+    if (i == n - 1 || from[i + 1].word != e.word) span[e.word].y = base + i + 1;
   }
 }
 
@@ -429,18 +463,26 @@ struct SumArgs {
   std::int64_t ld;
   int features, vocab;
   int block;  // entries per block, a multiple of 32
+  int per_owner;
+  int fill_rows;  // rows that a warp fills at a time
   const int* word;
   const int* pos;
   const int2* span;
   const int* total;
   float* partial;  // [block][2][features]: a block's share of a word that began before it, and
                    // of one that began in it and goes on behind it
+  int* counters;   // [block][3][slices]: partial sums that are there, see join()
   void* dw;
   float alpha, beta;
 };
 
 constexpr int kSumThreads = 256, kSumWarps = kSumThreads / 32;
 constexpr int kSumCtas = 3;  // per SM
+
+__device__ __forceinline__ int2 span_of(const SumArgs& a, int word) {
+  return a.span[static_cast<std::int64_t>(word & (kOwners - 1)) * a.per_owner +
+                (word >> kOwnerBits)];
+}
 
 // A slice of the features: RUNS runs of VEC elements per lane, from h on.
 template <int VEC, int RUNS>
@@ -484,11 +526,85 @@ __device__ __forceinline__ void store_row(const Slice<VEC, RUNS>& s, const SumAr
   }
 }
 
+// The sums of `n` blocks from `first` on, in their order; the first is at `slot`, the others,
+// which the word enters from before, at 0.
+template <int VEC, int RUNS>
+__device__ __forceinline__ void add_partials(Slice<VEC, RUNS>& s, const SumArgs& a, int first,
+                                             int slot, int n, int step, int h) {
+  constexpr int kStep = Slice<VEC, RUNS>::kStep;
+#pragma unroll 4
+  for (int k = 0; k < n; ++k) {
+    const int b = k == 0 ? first : (first / step + k) * step;
+    const float* p = a.partial + (2ll * b + (k == 0 ? slot : 0)) * a.features + h;
+#pragma unroll
+    for (int r = 0; r < RUNS; ++r) {
+      if (h + r * kStep >= a.features) continue;
+      float v[VEC];
+      unpack<float, VEC>(load_shared_run<VEC>(p + r * kStep), v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s.v[r][e] += v[e];
+    }
+  }
+}
+
+// Blocks whose partial sums of one word are joined by themselves first.
+constexpr int kJoin = 32;
+
+// Whether this warp is the last of n to come here.  What the others wrote before is visible
+// then; no warp waits.
+__device__ __forceinline__ bool last_of(int* counter, int n) {
+  __threadfence();
+  __syncwarp();
+  int was = 0;
+  if ((threadIdx.x & 31) == 0) was = atomicAdd(counter, 1);
+  was = __shfl_sync(0xffffffffu, was, 0);
+  __threadfence();
+  return was == n - 1;
+}
+
+// Called by each warp that has left a partial sum of this word's slice, of block b.  The last
+// one adds them up; where they are many, first the last of each kJoin neighbouring blocks those.
+template <bool UPDATE, typename TW, int VEC, int RUNS>
+__device__ __forceinline__ void join(const SumArgs& a, int word, int b, int slice, int slices, int h) {
+  const int2 span = span_of(a, word);
+  const int b0 = span.x / a.block, b1 = (span.y - 1) / a.block;
+  const auto counter = [&](int block, int which) {
+    return a.counters + (3ll * block + which) * slices + slice;
+  };
+  Slice<VEC, RUNS> sum;
+  sum.clear();
+  if (b1 - b0 < kJoin) {
+    if (!last_of(counter(b0, 2), b1 - b0 + 1)) return;
+    add_partials(sum, a, b0, 1, b1 - b0 + 1, 1, h);
+  } else {
+    const int g = b / kJoin;
+    const int first = max(b0, g * kJoin), n = min(b1, g * kJoin + kJoin - 1) - first + 1;
+    const int slot = first == b0 ? 1 : 0;
+    if (!last_of(counter(first, slot), n)) return;
+    add_partials(sum, a, first, slot, n, 1, h);
+    store_partial(sum, a.partial + (2ll * first + slot) * a.features, h, a.features);
+    const int groups = b1 / kJoin - b0 / kJoin + 1;
+    if (!last_of(counter(b0, 2), groups)) return;
+    sum.clear();
+    add_partials(sum, a, b0, 1, groups, kJoin, h);
+  }
+  TW* o = static_cast<TW*>(a.dw) + static_cast<std::int64_t>(word) * a.features + h;
+  Run<TW, VEC> was[RUNS];
+  if constexpr (UPDATE) {
+#pragma unroll
+    for (int r = 0; r < RUNS; ++r)
+      if (h + r * sum.kStep < a.features) was[r] = load_run<TW, VEC>(o + r * sum.kStep);
+  }
+  store_row<UPDATE, TW>(sum, a, o, h, was);
+}
+
 // One block's entries: AHEAD rows are loaded at a time and added in order; with beta also the
 // rows of dw of the words that end among them, whose latency would otherwise be a word's each
 // (two micro-batches of 32768 x 2048: 82 -> XX us for the second).
 template <bool UPDATE, typename T, typename TW, int VEC, int RUNS, int AHEAD>
-__device__ __forceinline__ void sum_block(const SumArgs& a, int b, int h, int total) {
+__device__ __forceinline__ void sum_block(const SumArgs& a, int b, int slice, int slices,
+                                          int total) {
+  const int h = slice * Slice<VEC, RUNS>::kFeatures + (threadIdx.x & 31) * VEC;
   const int lane = threadIdx.x & 31;
   const int i0 = b * a.block, i1 = min(total, i0 + a.block);
   const T* dy = static_cast<const T*>(a.dy) + h;
@@ -499,6 +615,7 @@ __device__ __forceinline__ void sum_block(const SumArgs& a, int b, int h, int to
   bool began_before = i0 > 0 && a.word[i0 - 1] == a.word[i0];
   float* partial = a.partial + 2ll * b * a.features;
   bool open = false;  // the last entry's word goes on behind the block
+  int left = -1;      // the word that began before the block and ended in it
   for (int i = i0; i < i1; i += 32) {
     const int n = min(32, i1 - i);
     const int my_pos = lane < n ? a.pos[i + lane] : 0;
@@ -534,26 +651,34 @@ __device__ __forceinline__ void sum_block(const SumArgs& a, int b, int h, int to
           for (int e = 0; e < VEC; ++e) sum.v[r][e] += v[e];
         }
         if ((ends >> (j + k) & 1u) == 0) continue;
-        if (began_before)
+        if (began_before) {
           store_partial(sum, partial, h, a.features);
-        else
+          left = w;
+        } else {
           store_row<UPDATE, TW>(sum, a, dw + static_cast<std::int64_t>(w) * a.features, h, was[k]);
+        }
         began_before = false;
         sum.clear();
       }
     }
   }
   if (open) store_partial(sum, partial + (began_before ? 0 : a.features), h, a.features);
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {
+    const int w = k == 0 ? left : open ? a.word[i1 - 1] : -1;
+    if (w >= 0) join<UPDATE, TW, VEC, RUNS>(a, w, b, slice, slices, h);
+  }
 }
 
-constexpr int kFillRows = 8;
+// Rows of words that do not occur: zeros, or beta dw.  A warp takes rows of some KB at a time:
+// more, and the last warps are alone with theirs (8 rows of 8 KB each: XX).
+constexpr int kFillBytes = 8192, kMostFillRows = 8;
 
-// Rows of words that do not occur: zeros, or beta dw.
 template <bool UPDATE, typename TW, int VEC>
 __device__ __forceinline__ void fill_rows(const SumArgs& a, int first) {
   const int lane = threadIdx.x & 31;
   const int v = first + lane;
-  const bool absent = lane < kFillRows && v < a.vocab && a.span[v].y == 0;
+  const bool absent = lane < a.fill_rows && v < a.vocab && span_of(a, v).y == 0;
   unsigned rows = __ballot_sync(0xffffffffu, absent);
   while (rows != 0) {
     const int row = first + __ffs(rows) - 1;
@@ -590,101 +715,22 @@ __global__ void __launch_bounds__(kSumThreads, kSumCtas) embedding_sum_kernel(co
   tc::grid_launch_next();
   tc::grid_wait_previous();
   using S = Slice<VEC, RUNS>;
+  // as many rows as the registers hold, with dw's where they are loaded too
+  constexpr int kAhead = !UPDATE ? AHEAD : sizeof(TW) > sizeof(T) ? 3 : AHEAD / 2;
   const unsigned slices = (a.features + S::kFeatures - 1) / S::kFeatures;
   const int total = *a.total;
   const std::int64_t sums = static_cast<std::int64_t>((total + a.block - 1) / a.block) * slices;
-  const std::int64_t fills = a.beta == 1.0f ? 0 : (a.vocab + kFillRows - 1) / kFillRows;
+  const std::int64_t fills = a.beta == 1.0f ? 0 : (a.vocab + a.fill_rows - 1) / a.fill_rows;
   const std::int64_t step = static_cast<std::int64_t>(gridDim.x) * kSumWarps;
   for (std::int64_t u = static_cast<std::int64_t>(blockIdx.x) * kSumWarps + (threadIdx.x >> 5);
        u < sums + fills; u += step) {
     if (u < sums) {
       const int b = static_cast<int>(u / slices);
-      const int h = static_cast<int>(u - b * static_cast<std::int64_t>(slices)) * S::kFeatures +
-                    (threadIdx.x & 31) * VEC;
-      sum_block<UPDATE, T, TW, VEC, RUNS, UPDATE ? AHEAD / 2 : AHEAD>(a, b, h, total);
+      const int slice = static_cast<int>(u - b * static_cast<std::int64_t>(slices));
+      sum_block<UPDATE, T, TW, VEC, RUNS, kAhead>(a, b, slice, slices, total);
     } else {
-      fill_rows<UPDATE, TW, VEC>(a, static_cast<int>(u - sums) * kFillRows);
+      fill_rows<UPDATE, TW, VEC>(a, static_cast<int>(u - sums) * a.fill_rows);
     }
-  }
-}
-
-constexpr int kJoinAlone = 128;
-
-// The word that goes on from block b - 1, where it began, into block b: a CTA has kSumWarps
-// slices of it, a warp each; a word of more than kJoinAlone blocks takes the whole CTA for each
-// slice.
-template <typename TW, int VEC, int RUNS>
-__global__ void __launch_bounds__(kSumThreads) embedding_join_kernel(const SumArgs a) {
-  tc::grid_launch_next();
-  tc::grid_wait_previous();
-  using S = Slice<VEC, RUNS>;
-  __shared__ float shared[kSumWarps][S::kFeatures];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int slices = (a.features + S::kFeatures - 1) / S::kFeatures;
-  const int groups = (slices + kSumWarps - 1) / kSumWarps;
-  const int b = static_cast<int>(blockIdx.x / groups) + 1;
-  const int first = static_cast<int>(blockIdx.x % groups) * kSumWarps;
-  const std::int64_t at = static_cast<std::int64_t>(b) * a.block;
-  if (at >= *a.total) return;
-  const int word = a.word[at];
-  if (a.word[at - 1] != word) return;
-  const int2 span = a.span[word];
-  if (span.x < at - a.block) return;  // it began earlier
-  const int n = (span.y - 1) / a.block - b + 2;  // blocks from b - 1 on
-  const auto add = [&](S& s, int k0, int k1, int h) {
-#pragma unroll 8
-    for (int k = k0; k < k1; ++k) {
-      const float* p = a.partial + (2ll * (b - 1 + k) + (k == 0 ? 1 : 0)) * a.features + h;
-#pragma unroll
-      for (int r = 0; r < RUNS; ++r) {
-        if (h + r * S::kStep >= a.features) continue;
-        float v[VEC];
-        unpack<float, VEC>(load_run<float, VEC>(p + r * S::kStep), v);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) s.v[r][e] += v[e];
-      }
-    }
-  };
-  TW* row = static_cast<TW*>(a.dw) + static_cast<std::int64_t>(word) * a.features;
-  const auto store = [&](const S& s, int h) {
-    Run<TW, VEC> was[RUNS];
-    if (a.beta != 0.0f) {
-#pragma unroll
-      for (int r = 0; r < RUNS; ++r)
-        if (h + r * S::kStep < a.features) was[r] = load_run<TW, VEC>(row + h + r * S::kStep);
-      store_row<true, TW>(s, a, row + h, h, was);
-    } else {
-      store_row<false, TW>(s, a, row + h, h, was);
-    }
-  };
-  S sum;
-  if (n <= kJoinAlone) {
-    const int h = (first + warp) * S::kFeatures + lane * VEC;
-    if (first + warp >= slices) return;
-    sum.clear();
-    add(sum, 0, n, h);
-    store(sum, h);
-    return;
-  }
-  const int each = (n + kSumWarps - 1) / kSumWarps;
-  for (int slice = first; slice < min(slices, first + kSumWarps); ++slice) {
-    const int h = slice * S::kFeatures + lane * VEC;
-    sum.clear();
-    add(sum, min(n, warp * each), min(n, (warp + 1) * each), h);
-#pragma unroll
-    for (int r = 0; r < RUNS; ++r)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) shared[warp][(r * VEC + e) * 32 + lane] = sum.v[r][e];
-    __syncthreads();
-    if (warp == 0) {
-      for (int w = 1; w < kSumWarps; ++w)
-#pragma unroll
-        for (int r = 0; r < RUNS; ++r)
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) sum.v[r][e] += shared[w][(r * VEC + e) * 32 + lane];
-      store(sum, h);
-    }
-    __syncthreads();
   }
 }
 
@@ -697,14 +743,18 @@ int block_entries(int tokens) {
   return n;
 }
 
+constexpr int kLeastSlice = 128;  // features of the narrowest slices
+
 struct SortPlan {
-  int passes, block;
-  std::size_t list[2], word, pos, span, total, partial, bytes;
+  int per_owner, passes, block;
+  std::int64_t num_counters;
+  std::size_t list[2], word, pos, span, total, partial, counters, bytes;
 };
 
 SortPlan plan(const EmbeddingArgs& a) {
   SortPlan p{};
   while ((a.vocab - 1) >> kOwnerBits >> (p.passes * kDigit) != 0) ++p.passes;
+  p.per_owner = (a.vocab + kOwners - 1) / kOwners;
   p.block = block_entries(a.tokens);
   std::size_t at = 0;
   const auto take = [&](std::size_t n) {
@@ -716,9 +766,12 @@ SortPlan plan(const EmbeddingArgs& a) {
   for (std::size_t& l : p.list) l = take(a.tokens > kSharedList ? T * sizeof(Entry) : 0);
   p.word = take(T * 4);
   p.pos = take(T * 4);
-  p.span = take(a.vocab * sizeof(int2));
+  p.span = take(static_cast<std::size_t>(p.per_owner) * kOwners * sizeof(int2));
   p.total = take(4);
-  p.partial = take((T + p.block - 1) / p.block * 2 * H * 4);
+  const std::size_t blocks = (T + p.block - 1) / p.block;
+  p.partial = take(blocks * 2 * H * 4);
+  p.num_counters = blocks * 3 * ((H + kLeastSlice - 1) / kLeastSlice);
+  p.counters = take(p.num_counters * 4);
   p.bytes = at;
   return p;
 }
@@ -726,15 +779,15 @@ SortPlan plan(const EmbeddingArgs& a) {
 // Rows per thread of the lookup: one where the GPU has room for a thread per run.
 constexpr int kLookupRows = 4;
 
-template <typename TW, typename TY, int VEC>
+template <typename TW, typename TY, int VEC, int ROWS = kLookupRows>
 cudaError_t lookup(const EmbeddingArgs& a, cudaStream_t st) {
   const std::int64_t per = a.features / VEC;
   const bool one = a.tokens * per <= std::int64_t{sms()} * 2048;
-  const int stride = one ? a.tokens : (a.tokens + kLookupRows - 1) / kLookupRows;
-  const std::int64_t ctas = (stride * per + kLookupThreads - 1) / kLookupThreads;
-  if (ctas > INT32_MAX) return cudaErrorInvalidValue;
+  const int stride = one ? a.tokens : (a.tokens + ROWS - 1) / ROWS;
+  const std::int64_t ctas = std::min<std::int64_t>(
+      (stride * per + kLookupThreads - 1) / kLookupThreads, sms() * (one ? 8 : kLookupCtas));
   return tc::launch_overlapped(
-      one ? embedding_kernel<TW, TY, VEC, 1> : embedding_kernel<TW, TY, VEC, kLookupRows>,
+      one ? embedding_kernel<TW, TY, VEC, 1> : embedding_kernel<TW, TY, VEC, ROWS>,
       dim3(static_cast<unsigned>(ctas)), kLookupThreads, 0, st, false,
       static_cast<const TW*>(a.w), a.token, static_cast<TY*>(a.row), a.ld, a.tokens, a.features,
       a.vocab, stride, a.alpha, a.beta);
@@ -760,25 +813,24 @@ cudaError_t gradient(const EmbeddingArgs& a, const SortPlan& p, char* ws, cudaSt
   s.span = reinterpret_cast<int2*>(ws + p.span);
   s.total = reinterpret_cast<int*>(ws + p.total);
   s.partial = reinterpret_cast<float*>(ws + p.partial);
+  s.counters = reinterpret_cast<int*>(ws + p.counters);
+  s.per_owner = p.per_owner;
   s.dw = a.w;
   s.alpha = a.alpha;
   s.beta = a.beta;
+  s.fill_rows = std::clamp<int>(kFillBytes / (a.features * sizeof(TW)), 1, kMostFillRows);
   constexpr int kSlice = Slice<VEC, RUNS>::kFeatures;
   const std::int64_t slices = (a.features + kSlice - 1) / kSlice;
   const std::int64_t blocks = (a.tokens + p.block - 1) / p.block;
   const std::int64_t units =
-      blocks * slices + (a.beta == 1.0f ? 0 : (a.vocab + kFillRows - 1) / kFillRows);
+      blocks * slices + (a.beta == 1.0f ? 0 : (a.vocab + s.fill_rows - 1) / s.fill_rows);
   const std::int64_t ctas =
       std::min<std::int64_t>((units + kSumWarps - 1) / kSumWarps, sms() * kSumCtas);
-  const cudaError_t e =
-      tc::launch_overlapped(a.beta != 0.0f ? embedding_sum_kernel<true, T, TW, VEC, RUNS, AHEAD>
-                                           : embedding_sum_kernel<false, T, TW, VEC, RUNS, AHEAD>,
-                            dim3(static_cast<unsigned>(ctas)), kSumThreads, 0, st, true, s);
-  if (e != cudaSuccess || blocks == 1) return e;
-  const std::int64_t joins = (blocks - 1) * ((slices + kSumWarps - 1) / kSumWarps);
-  if (joins > INT32_MAX) return cudaErrorInvalidValue;
-  return tc::launch_overlapped(embedding_join_kernel<TW, VEC, RUNS>,
-                               dim3(static_cast<unsigned>(joins)), kSumThreads, 0, st, true, s);
+  static_assert(kSlice >= kLeastSlice, "the counters are for fewer slices");
+  return tc::launch_overlapped(a.beta != 0.0f
+                                   ? embedding_sum_kernel<true, T, TW, VEC, RUNS, AHEAD>
+                                   : embedding_sum_kernel<false, T, TW, VEC, RUNS, AHEAD>,
+                               dim3(static_cast<unsigned>(ctas)), kSumThreads, 0, st, true, s);
 }
 
 }  // namespace
@@ -790,11 +842,11 @@ cudaError_t launch_embedding(const EmbeddingArgs& a, cudaStream_t st) noexcept {
     return wide ? lookup<float, float, 4>(a, st) : lookup<float, float, 1>(a, st);
   if (a.rows == T::kF16) {
     if (a.table == T::kF32)
-      return wide ? lookup<float, __half, 8>(a, st) : lookup<float, __half, 1>(a, st);
+      return wide ? lookup<float, __half, 8, 2>(a, st) : lookup<float, __half, 1>(a, st);
     return wide ? lookup<__half, __half, 8>(a, st) : lookup<__half, __half, 1>(a, st);
   }
   if (a.table == T::kF32)
-    return wide ? lookup<float, __nv_bfloat16, 8>(a, st)
+    return wide ? lookup<float, __nv_bfloat16, 8, 2>(a, st)
                 : lookup<float, __nv_bfloat16, 1>(a, st);
   return wide ? lookup<__nv_bfloat16, __nv_bfloat16, 8>(a, st)
               : lookup<__nv_bfloat16, __nv_bfloat16, 1>(a, st);
@@ -833,6 +885,9 @@ cudaError_t launch_embedding_gradient(const EmbeddingArgs& a, void* workspace,
   s.pos = reinterpret_cast<int*>(ws + p.pos);
   s.span = reinterpret_cast<int2*>(ws + p.span);
   s.total = reinterpret_cast<int*>(ws + p.total);
+  s.per_owner = p.per_owner;
+  s.counters = reinterpret_cast<int*>(ws + p.counters);
+  s.num_counters = p.num_counters;
   if (!sort_attributes()) return cudaErrorInvalidDevice;
   s.near_list = std::min(a.tokens, kSharedList);
   s.round = a.tokens < kRound ? (a.tokens + 3) / 4 * 4 : kRound;
