@@ -222,26 +222,24 @@ __global__ void __launch_bounds__(kLookupThreads, kLookupCtas)
 
 // ---------------------------------------------------------------------- the order --
 // CTA c owns the words v with v % kOwners == c (frequent words are neighbours in most
-// vocabularies, so ranges of words would leave one CTA most of the tokens).  Every CTA looks at
-// all tokens: it counts those of the owners before it, which gives the place of its own in the
-// ordered list, and takes its own in position order; then it sorts them by word in passes of
-// kDigit bits.  A warp goes over its own contiguous share of the list in both steps, so
-// equal words keep their order, whatever the split between the warps.  Clusters of kShare CTAs
-// read the tokens together, each a share that it writes into all their shared memories; no
-// cluster waits for another.
+// vocabularies, so ranges of words would leave one CTA most of the tokens).  Every CTA reads all
+// tokens: it counts those of the owners before it, which gives the place of its own in the
+// ordered list, takes its own in position order, and sorts them by word.  Many tokens are read
+// by clusters of SHARE neighbouring owners, a contiguous share by each CTA, which hands the
+// cluster's own to their owners' shared memory.  A warp goes over a contiguous share of the
+// list in all steps, so equal words keep their order, whatever the split between the warps.  No
+// CTA or cluster waits for another.
 //
-// Issue and latency bound.  32768 tokens of 50257 words: 25 us where each CTA read all tokens
-// for itself and looked at them one by one, XX us as it is.
+// Latency bound: XX
 constexpr int kOwners = 128, kOwnerBits = 7;
-constexpr int kShare = 4;
+constexpr int kShare = 8, kShareBits = 3;
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-constexpr int kDigit = 5;
+constexpr int kDigit = 5, kDigits = 1 << kDigit;
 constexpr int kSharedList = 4096;  // entries that are sorted in shared memory
-constexpr int kRound = 32768;      // tokens that are looked at at a time
-
-// A token as its owner and the word's number there; kNoKey: it enters nothing.
-constexpr int kKeyBits = 24;
-constexpr std::uint32_t kNoKey = 0xffffffffu;
+constexpr int kScan = 8;           // tokens per lane at a time
+constexpr int kCompared = 128;     // entries that are sorted by comparing each with all
+// Tokens that a cluster reads together: its launch takes 4 us more (XX).
+constexpr int kTogether = 16384;
 
 struct Entry {
   int word;  // v / kOwners
@@ -252,7 +250,6 @@ struct SortArgs {
   const std::int64_t* token;
   int tokens, vocab;
   int passes;
-  int round;       // tokens that are looked at at a time, a multiple of four
   int near_list;   // min(tokens, kSharedList)
   Entry* list[2];  // [tokens] each: longer lists while they are sorted
   int* word;       // [tokens] out: the words in order
@@ -270,46 +267,111 @@ __device__ __forceinline__ int warp_sum(int v) {
   return v;
 }
 
-// v summed over the threads before this one; *all: over all threads.
-__device__ __forceinline__ int block_exclusive(int v, int* warps, int* all) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int sum = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, sum, o);
-    if (lane >= o) sum += u;
+// *p = v in the shared memory of the cluster's CTA `rank`.
+template <int BITS, typename T>
+__device__ __forceinline__ void store_cluster(T* p, int rank, T v) {
+  if constexpr (BITS == 0) {
+    *p = v;
+  } else {
+    const std::uint32_t addr = tc::cluster_addr(p, rank);
+    if constexpr (sizeof(T) == 8) {
+      const auto w = *reinterpret_cast<const uint2*>(&v);
+      asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(w.x), "r"(w.y)
+                   : "memory");
+    } else {
+      asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+    }
   }
-  __syncthreads();  // warps[] may still be read by the previous scan
-  if (lane == 31) warps[warp] = sum;
-  __syncthreads();
-  int w = warps[lane];
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += u;
-  }
-  *all = __shfl_sync(0xffffffffu, w, 31);
-  const int before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
-  return sum - v + (warp > 0 ? before : 0);
 }
 
-__device__ __forceinline__ void store_cluster(std::uint32_t addr, uint4 v) {
-  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y),
-               "r"(v.z), "r"(v.w)
-               : "memory");
+template <int BITS>
+__device__ __forceinline__ void sync_cluster() {
+  if constexpr (BITS == 0)
+    __syncthreads();
+  else
+    tc::cluster_sync();  // at cluster scope: what went to global memory is visible too
 }
 
-__global__ void __cluster_dims__(kShare, 1, 1) __launch_bounds__(kSortThreads, 1)
-    embedding_sort_kernel(const SortArgs a) {
-  extern __shared__ uint4 keys[];  // the round's tokens, four at a time, then the two lists
-  Entry* near = reinterpret_cast<Entry*>(keys + a.round / 4);
-  __shared__ int count[1 << kDigit][kSortWarps + 1];  // a warp's counters in banks of their own
-  __shared__ int warps[32];
+// The lanes of `among` whose low BITS bits (ballots in `bits`) are c's.
+template <int BITS>
+__device__ __forceinline__ unsigned lanes_of(unsigned among, const unsigned (&bits)[BITS + 1],
+                                             int c) {
+#pragma unroll
+  for (int i = 0; i < BITS; ++i) among &= (c >> i & 1) != 0 ? bits[i] : ~bits[i];
+  return among;
+}
+
+// v summed over the lanes up to this one.
+__device__ __forceinline__ int warp_inclusive(int v) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) >= o) v += u;
+  }
+  return v;
+}
+
+template <int BITS>
+__device__ __forceinline__ void sort_body(const SortArgs& a) {
+  constexpr int kCtas = 1 << BITS;  // of the cluster
+  extern __shared__ Entry near[];   // two lists of near_list entries
+  // by digit, by warp: a warp's counters in banks of their own; two passes in turn
+  __shared__ int count[2][kDigits][kSortWarps + 1];
+  __shared__ int totals[2][kDigits];
+  __shared__ int found[kCtas + 1][kSortWarps];  // by owner of the cluster, then those before
+  // of every CTA of the cluster: its tokens of each owner of the cluster, and of those before
+  __shared__ int shares[kCtas][kCtas + 1];
+  // each CTA of the cluster runs before another writes into its shared memory
+  if constexpr (BITS > 0) asm volatile("barrier.cluster.arrive.relaxed.aligned;");
   tc::grid_launch_next();
   tc::grid_wait_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int owner = blockIdx.x;
+  const int owner = blockIdx.x, rank = owner & (kCtas - 1), cluster = owner >> BITS;
   const unsigned before_me = (1u << lane) - 1;
+
+  // the warp's share of the tokens
+  const std::int64_t per_warp =
+      (a.tokens + kCtas * kSortThreads - 1) / (kCtas * kSortThreads) * 32;
+  const std::int64_t t0 = (rank * kSortWarps + warp) * per_warp;
+  const std::int64_t t1 = min(t0 + per_warp, static_cast<std::int64_t>(a.tokens));
+  const bool keep = per_warp <= 32 * kScan;  // in registers between the two readings
+  int v[kScan];
+  const auto load = [&](std::int64_t t) {
+#pragma unroll
+    for (int j = 0; j < kScan; ++j) {
+      const std::int64_t i = t + 32 * j + lane;
+      v[j] = -1;
+      if (i < t1) {
+        const std::int64_t w = a.token[i];
+        if (w >= 0 && w < a.vocab) v[j] = static_cast<int>(w);
+      }
+    }
+  };
+  // Whether the lane's token v is the cluster's, as ballots; its bits as lanes_of wants them.
+  const auto ballots = [&](int w, unsigned (&bits)[BITS + 1]) {
+    const unsigned in =
+        __ballot_sync(0xffffffffu, w >= 0 && (w & (kOwners - 1)) >> BITS == cluster);
+    if (in != 0) {
+#pragma unroll
+      for (int i = 0; i < BITS; ++i) bits[i] = __ballot_sync(0xffffffffu, (w >> i & 1) != 0);
+    }
+    return in;
+  };
+  int below = 0, mine = 0;  // mine: lane c, of the cluster's owner c
+  for (std::int64_t t = t0; t < t1; t += 32 * kScan) {
+    load(t);
+#pragma unroll
+    for (int j = 0; j < kScan; ++j) {
+      below += v[j] >= 0 && (v[j] & (kOwners - 1)) >> BITS < cluster;
+      unsigned bits[BITS + 1];
+      const unsigned in = ballots(v[j], bits);
+      if (in != 0) mine += __popc(lanes_of<BITS>(in, bits, lane));
+    }
+  }
+  below = warp_sum(below);
+  if (lane < kCtas) found[lane][warp] = mine;
+  if (lane == 0) found[kCtas][warp] = below;
+  count[0][warp][lane] = 0;
 
   int2* span = a.span + static_cast<std::int64_t>(owner) * a.per_owner;
   for (int i = threadIdx.x; i < a.per_owner; i += kSortThreads) span[i] = make_int2(0, 0);
@@ -317,136 +379,116 @@ __global__ void __cluster_dims__(kShare, 1, 1) __launch_bounds__(kSortThreads, 1
        i < a.num_counters; i += kOwners * kSortThreads)
     a.counters[i] = 0;
 
-  const int rounds = (a.tokens + a.round - 1) / a.round;
-  // Fills keys with round r's tokens and returns how many groups of four they are.
-  const auto stage = [&](int r) {
-    const std::int64_t t0 = static_cast<std::int64_t>(r) * a.round;
-    const int m = static_cast<int>(min(static_cast<std::int64_t>(a.round), a.tokens - t0));
-    const int groups = (m + 3) / 4;
-    for (int g = tc::cluster_rank() * kSortThreads + threadIdx.x; g < groups;
-         g += kShare * kSortThreads) {
-      std::uint32_t k[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        k[j] = kNoKey;
-        if (4 * g + j < m) {
-          const std::int64_t v = a.token[t0 + 4 * g + j];
-          if (v >= 0 && v < a.vocab)
-            k[j] = static_cast<std::uint32_t>(v & (kOwners - 1)) << kKeyBits |
-                   static_cast<std::uint32_t>(v >> kOwnerBits);
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < kShare; ++c)
-        store_cluster(tc::cluster_addr(keys + g, c), make_uint4(k[0], k[1], k[2], k[3]));
-    }
-    tc::cluster_sync();
-    return groups;
-  };
-  // the warp's groups of them
-  const auto share_of = [&](int groups, int* g1) {
-    const int share = ((groups + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
-    *g1 = min(groups, (warp + 1) * share);
-    return warp * share;
-  };
-  const std::uint32_t lo = static_cast<std::uint32_t>(owner) << kKeyBits;
-  const std::uint32_t hi = static_cast<std::uint32_t>(owner + 1) << kKeyBits;
-  int below = 0, through = 0;  // keys below lo, below hi
-  for (int r = 0; r < rounds; ++r) {
-    int g1;
-    for (int g = share_of(stage(r), &g1) + lane; g < g1; g += 32) {
-      const uint4 k = keys[g];
-      below += (k.x < lo) + (k.y < lo) + (k.z < lo) + (k.w < lo);
-      through += (k.x < hi) + (k.y < hi) + (k.z < hi) + (k.w < hi);
-    }
-    if (rounds > 1) tc::cluster_sync();  // before the next round's tokens
+  if constexpr (BITS > 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  __syncthreads();
+  if (warp <= kCtas) {  // the CTA's sums by owner: found becomes the warps before
+    const int x = found[warp][lane];
+    const int sum = warp_inclusive(x);
+    found[warp][lane] = sum - x;
+    const int all = __shfl_sync(0xffffffffu, sum, 31);
+    if (lane < kCtas) store_cluster<BITS>(&shares[rank][warp], lane, all);
   }
-  int base, n;
-  (void)block_exclusive(below, warps, &base);
-  (void)block_exclusive(through - below, warps, &n);
+  sync_cluster<BITS>();
+  // lane c: the place of the cluster's owner c in the ordered list, its entries, and where
+  // this warp's tokens of it go
+  int base = 0, n = 0, at = 0;
+  if (lane < kCtas) {
+#pragma unroll
+    for (int q = 0; q < kCtas; ++q) {
+      base += shares[q][kCtas];
+      n += shares[q][lane];
+      if (q < rank) at += shares[q][lane];
+    }
+    at += found[lane][warp];
+  }
+  int before = n;  // entries of the cluster's owners up to this one
+#pragma unroll
+  for (int o = 1; o < kCtas; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += u;
+  }
+  base += before - n;
+  for (std::int64_t t = t0; t < t1; t += 32 * kScan) {
+    if (!keep) load(t);
+#pragma unroll
+    for (int j = 0; j < kScan; ++j) {
+      unsigned bits[BITS + 1];
+      const unsigned in = ballots(v[j], bits);
+      if (in == 0) continue;
+      const int c = v[j] & (kCtas - 1);
+      const int to = __shfl_sync(0xffffffffu, at, c), size = __shfl_sync(0xffffffffu, n, c);
+      const int list = __shfl_sync(0xffffffffu, base, c);
+      if ((in >> lane & 1u) != 0) {
+        const int i = to + __popc(lanes_of<BITS>(in, bits, c) & before_me);
+        const Entry e{v[j] >> kOwnerBits, static_cast<int>(t + 32 * j + lane)};
+        if (size <= a.near_list)
+          store_cluster<BITS>(near + i, c, e);
+        else
+          a.list[0][list + i] = e;
+      }
+      at += __popc(lanes_of<BITS>(in, bits, lane));
+    }
+  }
+  n = __shfl_sync(0xffffffffu, n, rank);
+  base = __shfl_sync(0xffffffffu, base, rank);
   if (owner == kOwners - 1 && threadIdx.x == 0) *a.total = base + n;
-
+  sync_cluster<BITS>();  // the list is there
   Entry* from = n <= a.near_list ? near : a.list[0] + base;
   Entry* to = n <= a.near_list ? near + a.near_list : a.list[1] + base;
-  int taken = 0;
-  for (int r = 0; r < rounds; ++r) {
-    const int groups = rounds > 1 ? stage(r) : (a.tokens + 3) / 4;
-    int g1;
-    const int g0 = share_of(groups, &g1);
-    int mine = through - below;
-    if (rounds > 1) {
-      mine = 0;
-      for (int g = g0 + lane; g < g1; g += 32) {
-        const uint4 k = keys[g];
-        mine += (k.x - lo < hi - lo) + (k.y - lo < hi - lo) + (k.z - lo < hi - lo) +
-                (k.w - lo < hi - lo);
-      }
-    }
-    mine = warp_sum(mine);
-    int all;
-    int at = taken + block_exclusive(lane == 0 ? mine : 0, warps, &all);
-    at = __shfl_sync(0xffffffffu, at, 0);
-    taken += all;
-    for (int g = g0; mine > 0 && g < g1; g += 32) {
-      const uint4 k =
-          g + lane < g1 ? keys[g + lane] : make_uint4(kNoKey, kNoKey, kNoKey, kNoKey);
-      const std::uint32_t key[4] = {k.x - lo, k.y - lo, k.z - lo, k.w - lo};
-      int before = 0, own = 0;  // of the lanes before this one, of this lane
-      int group = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const unsigned yes = __ballot_sync(0xffffffffu, key[j] < hi - lo);
-        before += __popc(yes & before_me);
-        group += __popc(yes);
-      }
-      const int t = r * a.round + 4 * (g + lane);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (key[j] >= hi - lo) continue;
-        from[at + before + own] = {static_cast<int>(key[j]), t + j};
-        ++own;
-      }
-      at += group;
-    }
-    if (rounds > 1) tc::cluster_sync();  // before the next round's tokens
-  }
 
-  const int chunk = ((n + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
-  const int i0 = min(n, warp * chunk), i1 = min(n, i0 + chunk);
-  for (int pass = 0; pass < a.passes; ++pass) {
-    const int shift = pass * kDigit;
-    const auto digit = [&](int i) {
-      return i < i1 ? (from[i].word >> shift) & ((1 << kDigit) - 1) : 1 << kDigit;
-    };
-    static_assert(kSortThreads == kSortWarps << kDigit, "one counter per thread");
-    count[threadIdx.x >> 5][lane] = 0;
-    __syncthreads();  // the list and the counters are there
-    for (int i = i0; i < i1; i += 32) {
-      const int d = digit(i + lane);
-      const unsigned same = __match_any_sync(0xffffffffu, d);
-      if (d < 1 << kDigit && (same & before_me) == 0) count[d][warp] += __popc(same);
-      __syncwarp();
+  if (n <= kCompared) {
+    if (static_cast<int>(threadIdx.x) < n) {
+      const Entry e = from[threadIdx.x];
+      int place = 0;
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const int w = from[i].word;
+        place += w < e.word || (w == e.word && i < static_cast<int>(threadIdx.x));
+      }
+      to[place] = e;
     }
-    __syncthreads();
-    int* c = &count[threadIdx.x >> 5][lane];  // digit by digit, warp by warp
-    int all;
-    const int start = block_exclusive(*c, warps, &all);
-    *c = start;
-    __syncthreads();
-    for (int i = i0; i < i1; i += 32) {
-      const int d = digit(i + lane);
-      const unsigned same = __match_any_sync(0xffffffffu, d);
-      if (d < 1 << kDigit) to[count[d][warp] + __popc(same & before_me)] = from[i + lane];
-      __syncwarp();
-      if (d < 1 << kDigit && (same & before_me) == 0) count[d][warp] += __popc(same);
-      __syncwarp();
-    }
-    __syncthreads();
-    Entry* swap = from;
     from = to;
-    to = swap;
+  } else {
+    const int chunk = ((n + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
+    const int i0 = min(n, warp * chunk), i1 = min(n, i0 + chunk);
+    for (int pass = 0; pass < a.passes; ++pass) {
+      const int shift = pass * kDigit;
+      auto& counts = count[pass & 1];
+      const auto digit = [&](int i) {
+        return i < i1 ? (from[i].word >> shift) & (kDigits - 1) : kDigits;
+      };
+      static_assert(kSortWarps == kDigits, "a warp scans a digit's counters");
+      for (int i = i0; i < i1; i += 32) {
+        const int d = digit(i + lane);
+        const unsigned same = __match_any_sync(0xffffffffu, d);
+        if (d < kDigits && (same & before_me) == 0) counts[d][warp] += __popc(same);
+        __syncwarp();
+      }
+      __syncthreads();
+      const int x = counts[warp][lane];  // of digit `warp`, by warp
+      const int upto = warp_inclusive(x);
+      if (lane == 31) totals[pass & 1][warp] = upto;
+      count[(pass + 1) & 1][warp][lane] = 0;
+      __syncthreads();
+      const int digits = totals[pass & 1][lane];
+      const int before_digit = __shfl_sync(0xffffffffu, warp_inclusive(digits) - digits, warp);
+      counts[warp][lane] = before_digit + upto - x;
+      __syncthreads();
+      for (int i = i0; i < i1; i += 32) {
+        const int d = digit(i + lane);
+        const unsigned same = __match_any_sync(0xffffffffu, d);
+        if (d < kDigits) to[counts[d][warp] + __popc(same & before_me)] = from[i + lane];
+        __syncwarp();
+        if (d < kDigits && (same & before_me) == 0) counts[d][warp] += __popc(same);
+        __syncwarp();
+      }
+      __syncthreads();
+      Entry* swap = from;
+      from = to;
+      to = swap;
+    }
   }
-  __syncthreads();  // without passes: the list is there
+  __syncthreads();
 
   for (int i = threadIdx.x; i < n; i += kSortThreads) {
     const Entry e = from[i];
@@ -455,6 +497,15 @@ __global__ void __cluster_dims__(kShare, 1, 1) __launch_bounds__(kSortThreads, 1
     if (i == 0 || from[i - 1].word != e.word) span[e.word].x = base + i;
     if (i == n - 1 || from[i + 1].word != e.word) span[e.word].y = base + i + 1;
   }
+}
+
+__global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const SortArgs a) {
+  sort_body<0>(a);
+}
+
+__global__ void __cluster_dims__(kShare, 1, 1) __launch_bounds__(kSortThreads, 1)
+    embedding_sort_together_kernel(const SortArgs a) {
+  sort_body<kShareBits>(a);
 }
 
 // ----------------------------------------------------------------------- the sums --
@@ -858,11 +909,12 @@ static bool sort_attributes() noexcept {
   const int dev = current_device();
   if (dev < 0 || dev >= 64) return false;
   if ((set.load(std::memory_order_acquire) >> dev & 1ull) != 0) return true;
-  if (cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           kRound * sizeof(std::uint32_t) + 2 * kSharedList * sizeof(Entry)) !=
-      cudaSuccess) {
-    (void)cudaGetLastError();
-    return false;
+  for (auto* kern : {embedding_sort_kernel, embedding_sort_together_kernel}) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             2 * kSharedList * sizeof(Entry)) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return false;
+    }
   }
   set.fetch_or(1ull << dev, std::memory_order_release);
   return true;
@@ -890,10 +942,10 @@ cudaError_t launch_embedding_gradient(const EmbeddingArgs& a, void* workspace,
   s.num_counters = p.num_counters;
   if (!sort_attributes()) return cudaErrorInvalidDevice;
   s.near_list = std::min(a.tokens, kSharedList);
-  s.round = a.tokens < kRound ? (a.tokens + 3) / 4 * 4 : kRound;
-  const std::size_t shared = s.round * sizeof(std::uint32_t) + 2 * s.near_list * sizeof(Entry);
-  const cudaError_t e = tc::launch_overlapped(embedding_sort_kernel, dim3(kOwners), kSortThreads,
-                                              shared, st, false, s);
+  const std::size_t shared = 2 * s.near_list * sizeof(Entry);
+  const cudaError_t e = tc::launch_overlapped(
+      a.tokens < kTogether ? embedding_sort_kernel : embedding_sort_together_kernel, dim3(kOwners),
+      kSortThreads, shared, st, false, s);
   if (e != cudaSuccess) return e;
   const bool wide = rows_of_runs(a, a.rows == T::kF32 ? 4 : 8);
   if (a.rows == T::kF32)
