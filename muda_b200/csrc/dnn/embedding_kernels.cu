@@ -53,6 +53,70 @@ struct Run<T, 1> {
   T v;
 };
 
+// Loads that are left out without `ok` (then the value is -1, or any).  The predicate is inside
+// the asm: a branch around a load makes its result wait for it there.
+__device__ __forceinline__ std::int64_t load8(const std::int64_t* p, bool ok) {
+  std::int64_t v;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %2, 0;\n\t"
+      "mov.b64 %0, -1;\n\t"
+      "@q ld.global.u64 %0, [%1];\n\t}"
+      : "=&l"(v)
+      : "l"(p), "r"(static_cast<int>(ok))
+      : "memory");
+  return v;
+}
+
+__device__ __forceinline__ uint4 load16(const void* p, bool ok) {
+  uint4 v;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+      : "l"(p), "r"(static_cast<int>(ok))
+      : "memory");
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ T load_one(const T* p, bool ok) {
+  if constexpr (sizeof(T) == 4) {
+    float v;
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %2, 0;\n\t"
+        "@q ld.global.f32 %0, [%1];\n\t}"
+        : "=&f"(v)
+        : "l"(p), "r"(static_cast<int>(ok))
+        : "memory");
+    return v;
+  } else {
+    std::uint16_t v;
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %2, 0;\n\t"
+        "@q ld.global.u16 %0, [%1];\n\t}"
+        : "=&h"(v)
+        : "l"(p), "r"(static_cast<int>(ok))
+        : "memory");
+    return *reinterpret_cast<const T*>(&v);
+  }
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ Run<T, VEC> load_run(const T* p, bool ok) {
+  Run<T, VEC> r;
+  if constexpr (VEC == 1) {
+    r.v = load_one(p, ok);
+  } else {
+#pragma unroll
+    for (int i = 0; i < r.kWords; ++i) r.w[i] = load16(reinterpret_cast<const uint4*>(p) + i, ok);
+  }
+  return r;
+}
+
 template <typename T, int VEC>
 __device__ __forceinline__ Run<T, VEC> load_run(const T* p) {
   Run<T, VEC> r;
@@ -173,12 +237,9 @@ __global__ void __launch_bounds__(kLookupThreads, kLookupCtas)
   const auto words = [&](int r) {
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) {
-      word[j] = -1;
       const std::int64_t t = r + static_cast<std::int64_t>(j) * stride;
-      if (r < stride && t < tokens) {
-        const std::int64_t v = token[t];
-        word[j] = v < 0 ? -1 : v >= vocab ? vocab : static_cast<int>(v);
-      }
+      const std::int64_t v = load8(token + t, r < stride && t < tokens);
+      word[j] = v < 0 ? -1 : v >= vocab ? vocab : static_cast<int>(v);
     }
   };
   words(row);
@@ -188,8 +249,8 @@ __global__ void __launch_bounds__(kLookupThreads, kLookupCtas)
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) {
       is[j] = word[j];
-      if (static_cast<unsigned>(is[j]) < static_cast<unsigned>(vocab))
-        in[j] = load_run<TW, VEC>(w + static_cast<std::int64_t>(is[j]) * features + col * VEC);
+      in[j] = load_run<TW, VEC>(w + static_cast<std::int64_t>(is[j]) * features + col * VEC,
+                                static_cast<unsigned>(is[j]) < static_cast<unsigned>(vocab));
     }
     const bool wraps = col + cols_on >= per;
     const int next = row + rows_on + (wraps ? 1 : 0);
@@ -337,14 +398,15 @@ __device__ __forceinline__ void sort_body(const SortArgs& a) {
   const bool keep = per_warp <= 32 * kScan;  // in registers between the two readings
   int v[kScan];
   const auto load = [&](std::int64_t t) {
+    std::int64_t w[kScan];
 #pragma unroll
     for (int j = 0; j < kScan; ++j) {
       const std::int64_t i = t + 32 * j + lane;
-      v[j] = -1;
-      if (i < t1) {
-        const std::int64_t w = a.token[i];
-        if (w >= 0 && w < a.vocab) v[j] = static_cast<int>(w);
-      }
+      w[j] = load8(a.token + i, i < t1);
+    }
+#pragma unroll
+    for (int j = 0; j < kScan; ++j) {
+      v[j] = w[j] >= 0 && w[j] < a.vocab ? static_cast<int>(w[j]) : -1;
     }
   };
   // Whether the lane's token v is the cluster's, as ballots; its bits as lanes_of wants them.
@@ -454,13 +516,20 @@ __device__ __forceinline__ void sort_body(const SortArgs& a) {
     for (int pass = 0; pass < a.passes; ++pass) {
       const int shift = pass * kDigit;
       auto& counts = count[pass & 1];
-      const auto digit = [&](int i) {
-        return i < i1 ? (from[i].word >> shift) & (kDigits - 1) : kDigits;
+      // entry i's digit, and the lanes whose entries have the same (five votes: match.any
+      // took XX)
+      const auto digit = [&](int i, unsigned* same) {
+        const int d = i < i1 ? from[i].word >> shift & (kDigits - 1) : kDigits;
+        unsigned bits[kDigit + 1];
+#pragma unroll
+        for (int k = 0; k < kDigit; ++k) bits[k] = __ballot_sync(0xffffffffu, (d >> k & 1) != 0);
+        *same = lanes_of<kDigit>(__ballot_sync(0xffffffffu, d < kDigits), bits, d);
+        return d;
       };
       static_assert(kSortWarps == kDigits, "a warp scans a digit's counters");
       for (int i = i0; i < i1; i += 32) {
-        const int d = digit(i + lane);
-        const unsigned same = __match_any_sync(0xffffffffu, d);
+        unsigned same;
+        const int d = digit(i + lane, &same);
         if (d < kDigits && (same & before_me) == 0) counts[d][warp] += __popc(same);
         __syncwarp();
       }
@@ -475,8 +544,8 @@ __device__ __forceinline__ void sort_body(const SortArgs& a) {
       counts[warp][lane] = before_digit + upto - x;
       __syncthreads();
       for (int i = i0; i < i1; i += 32) {
-        const int d = digit(i + lane);
-        const unsigned same = __match_any_sync(0xffffffffu, d);
+        unsigned same;
+        const int d = digit(i + lane, &same);
         if (d < kDigits) to[counts[d][warp] + __popc(same & before_me)] = from[i + lane];
         __syncwarp();
         if (d < kDigits && (same & before_me) == 0) counts[d][warp] += __popc(same);
@@ -513,7 +582,7 @@ struct SumArgs {
   const void* dy;
   std::int64_t ld;
   int features, vocab;
-  int block;  // entries per block, a multiple of 32
+  int block;  // entries per block
   int per_owner;
   int fill_rows;  // rows that a warp fills at a time
   const int* word;
@@ -557,8 +626,33 @@ __device__ __forceinline__ void store_partial(const Slice<VEC, RUNS>& s, float* 
       store_run<false>(o + h + r * s.kStep, pack<float, VEC>(s.v[r]));
 }
 
+// What becomes of dw: nothing of it is left, beta of it, or (fp32, beta 1) the sums are added
+// to it.  kAdd's additions are done by L2, each element's one, so that no load's latency is
+// waited for (the second micro-batch of 32768 x 2048: 69 us with kScale, XX).
+enum Update { kWrite = 0, kScale = 1, kAdd = 2 };
+
+template <int VEC>
+__device__ __forceinline__ void add_run(float* p, const float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    asm volatile("red.global.add.f32 [%0], %1;" ::"l"(p), "f"(v[0]) : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; i += 4)
+      asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p + i), "f"(v[i]),
+                   "f"(v[i + 1]), "f"(v[i + 2]), "f"(v[i + 3])
+                   : "memory");
+  }
+}
+
+// Lane `from`'s p.
+template <typename T>
+__device__ __forceinline__ T* shuffled(T* p, int from) {
+  return reinterpret_cast<T*>(
+      __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), from));
+}
+
 // The slice of a word's row of dw (o: at h), from its sum and what it was.
-template <bool UPDATE, typename TW, int VEC, int RUNS>
+template <int UPDATE, typename TW, int VEC, int RUNS>
 __device__ __forceinline__ void store_row(const Slice<VEC, RUNS>& s, const SumArgs& a, TW* o, int h,
                                           const Run<TW, VEC> (&was)[RUNS]) {
 #pragma unroll
@@ -567,7 +661,11 @@ __device__ __forceinline__ void store_row(const Slice<VEC, RUNS>& s, const SumAr
     float v[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = a.alpha * s.v[r][e];
-    if constexpr (UPDATE) {
+    if constexpr (UPDATE == kAdd) {
+      add_run<VEC>(o + r * s.kStep, v);
+      continue;
+    }
+    if constexpr (UPDATE == kScale) {
       float old[VEC];
       unpack<TW, VEC>(was[r], old);
 #pragma unroll
@@ -583,7 +681,7 @@ template <int VEC, int RUNS>
 __device__ __forceinline__ void add_partials(Slice<VEC, RUNS>& s, const SumArgs& a, int first,
                                              int slot, int n, int step, int h) {
   constexpr int kStep = Slice<VEC, RUNS>::kStep;
-#pragma unroll 4
+#pragma unroll 8
   for (int k = 0; k < n; ++k) {
     const int b = k == 0 ? first : (first / step + k) * step;
     const float* p = a.partial + (2ll * b + (k == 0 ? slot : 0)) * a.features + h;
@@ -602,20 +700,20 @@ __device__ __forceinline__ void add_partials(Slice<VEC, RUNS>& s, const SumArgs&
 constexpr int kJoin = 32;
 
 // Whether this warp is the last of n to come here.  What the others wrote before is visible
-// then; no warp waits.
+// then (each lane's writes are ordered before lane 0's release); no warp waits.
 __device__ __forceinline__ bool last_of(int* counter, int n) {
-  __threadfence();
   __syncwarp();
   int was = 0;
-  if ((threadIdx.x & 31) == 0) was = atomicAdd(counter, 1);
+  if ((threadIdx.x & 31) == 0)
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(was) : "l"(counter)
+                 : "memory");
   was = __shfl_sync(0xffffffffu, was, 0);
-  __threadfence();
   return was == n - 1;
 }
 
 // Called by each warp that has left a partial sum of this word's slice, of block b.  The last
 // one adds them up; where they are many, first the last of each kJoin neighbouring blocks those.
-template <bool UPDATE, typename TW, int VEC, int RUNS>
+template <int UPDATE, typename TW, int VEC, int RUNS>
 __device__ __forceinline__ void join(const SumArgs& a, int word, int b, int slice, int slices, int h) {
   const int2 span = span_of(a, word);
   const int b0 = span.x / a.block, b1 = (span.y - 1) / a.block;
@@ -641,7 +739,7 @@ __device__ __forceinline__ void join(const SumArgs& a, int word, int b, int slic
   }
   TW* o = static_cast<TW*>(a.dw) + static_cast<std::int64_t>(word) * a.features + h;
   Run<TW, VEC> was[RUNS];
-  if constexpr (UPDATE) {
+  if constexpr (UPDATE == kScale) {
 #pragma unroll
     for (int r = 0; r < RUNS; ++r)
       if (h + r * sum.kStep < a.features) was[r] = load_run<TW, VEC>(o + r * sum.kStep);
@@ -649,18 +747,40 @@ __device__ __forceinline__ void join(const SumArgs& a, int word, int b, int slic
   store_row<UPDATE, TW>(sum, a, o, h, was);
 }
 
+// s += the run, two features to an instruction.
+template <typename T, int VEC>
+__device__ __forceinline__ void add(float (&s)[VEC], const Run<T, VEC>& r) {
+  float v[VEC];
+  unpack<T, VEC>(r, v);
+  if constexpr (VEC == 1) {
+    s[0] += v[0];
+  } else {
+#pragma unroll
+    for (int e = 0; e < VEC; e += 2)
+      asm("{\n\t.reg .b64 a, b;\n\t"
+          "mov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+          "add.rn.f32x2 a, a, b;\n\t"
+          "mov.b64 {%0, %1}, a;\n\t}"
+          : "+f"(s[e]), "+f"(s[e + 1])
+          : "f"(v[e]), "f"(v[e + 1]));
+  }
+}
+
 // One block's entries: AHEAD rows are loaded at a time and added in order; with beta also the
-// rows of dw of the words that end among them, whose latency would otherwise be a word's each
-// (two micro-batches of 32768 x 2048: 82 -> XX us for the second).
-template <bool UPDATE, typename T, typename TW, int VEC, int RUNS, int AHEAD>
+// rows of dw of the words that end among them, whose latency would otherwise be a word's each.
+// A warp alone takes as long for its instructions as for its loads, so there are no branches or
+// predicates but for words that end: lanes behind the features read the row's first ones, and a
+// last batch its last row again.
+template <int UPDATE, typename T, typename TW, int VEC, int RUNS, int AHEAD>
 __device__ __forceinline__ void sum_block(const SumArgs& a, int b, int slice, int slices,
                                           int total) {
-  const int h = slice * Slice<VEC, RUNS>::kFeatures + (threadIdx.x & 31) * VEC;
   const int lane = threadIdx.x & 31;
+  const int h = slice * Slice<VEC, RUNS>::kFeatures + lane * VEC;
   const int i0 = b * a.block, i1 = min(total, i0 + a.block);
-  const T* dy = static_cast<const T*>(a.dy) + h;
-  TW* dw = static_cast<TW*>(a.dw) + h;
   constexpr int kStep = Slice<VEC, RUNS>::kStep;
+  int at[RUNS];  // the runs' features
+#pragma unroll
+  for (int r = 0; r < RUNS; ++r) at[r] = h + r * kStep < a.features ? h + r * kStep : 0;
   Slice<VEC, RUNS> sum;
   sum.clear();
   bool began_before = i0 > 0 && a.word[i0 - 1] == a.word[i0];
@@ -669,9 +789,11 @@ __device__ __forceinline__ void sum_block(const SumArgs& a, int b, int slice, in
   int left = -1;      // the word that began before the block and ended in it
   for (int i = i0; i < i1; i += 32) {
     const int n = min(32, i1 - i);
-    const int my_pos = lane < n ? a.pos[i + lane] : 0;
-    const int my_word = lane < n ? a.word[i + lane] : -1;
-    const int next = i + lane + 1 < total ? a.word[i + lane + 1] : -1;
+    const int mine = i + min(lane, n - 1);
+    const int my_word = a.word[mine];
+    const int next = mine + 1 < total ? a.word[mine + 1] : -1;
+    const T* my_row = static_cast<const T*>(a.dy) + a.pos[mine] * a.ld;
+    TW* my_dw = static_cast<TW*>(a.dw) + static_cast<std::int64_t>(my_word) * a.features;
     const unsigned ends = __ballot_sync(0xffffffffu, my_word != next);
     open = (ends >> (n - 1) & 1u) == 0;
     for (int j = 0; j < n; j += AHEAD) {
@@ -679,34 +801,27 @@ __device__ __forceinline__ void sum_block(const SumArgs& a, int b, int slice, in
       Run<TW, VEC> was[AHEAD][RUNS];
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
-        const int p = __shfl_sync(0xffffffffu, my_pos, (j + k) & 31);
-        const int w = __shfl_sync(0xffffffffu, my_word, (j + k) & 31);
-        if (j + k >= n) continue;
+        const T* row = shuffled(my_row, (j + k) & 31);
 #pragma unroll
-        for (int r = 0; r < RUNS; ++r) {
-          if (h + r * kStep >= a.features) continue;
-          in[k][r] = load_run<T, VEC>(dy + p * a.ld + r * kStep);
-          if (UPDATE && (ends >> (j + k) & 1u) != 0)
-            was[k][r] = load_run<TW, VEC>(dw + static_cast<std::int64_t>(w) * a.features + r * kStep);
+        for (int r = 0; r < RUNS; ++r) in[k][r] = load_run<T, VEC>(row + at[r]);
+        if constexpr (UPDATE == kScale) {
+          const TW* o = shuffled(my_dw, (j + k) & 31);
+#pragma unroll
+          for (int r = 0; r < RUNS; ++r)
+            was[k][r] = load_run<TW, VEC>(o + at[r], (ends >> (j + k) & 1u) != 0);
         }
       }
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
-        const int w = __shfl_sync(0xffffffffu, my_word, (j + k) & 31);
-        if (j + k >= n) continue;
+        if (j + k >= n) break;
 #pragma unroll
-        for (int r = 0; r < RUNS; ++r) {
-          float v[VEC];
-          unpack<T, VEC>(in[k][r], v);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) sum.v[r][e] += v[e];
-        }
+        for (int r = 0; r < RUNS; ++r) add<T, VEC>(sum.v[r], in[k][r]);
         if ((ends >> (j + k) & 1u) == 0) continue;
         if (began_before) {
           store_partial(sum, partial, h, a.features);
-          left = w;
+          left = __shfl_sync(0xffffffffu, my_word, j + k);
         } else {
-          store_row<UPDATE, TW>(sum, a, dw + static_cast<std::int64_t>(w) * a.features, h, was[k]);
+          store_row<UPDATE, TW>(sum, a, shuffled(my_dw, j + k) + h, h, was[k]);
         }
         began_before = false;
         sum.clear();
@@ -725,7 +840,7 @@ __device__ __forceinline__ void sum_block(const SumArgs& a, int b, int slice, in
 // more, and the last warps are alone with theirs (8 rows of 8 KB each: XX).
 constexpr int kFillBytes = 8192, kMostFillRows = 8;
 
-template <bool UPDATE, typename TW, int VEC>
+template <int UPDATE, typename TW, int VEC>
 __device__ __forceinline__ void fill_rows(const SumArgs& a, int first) {
   const int lane = threadIdx.x & 31;
   const int v = first + lane;
@@ -735,7 +850,7 @@ __device__ __forceinline__ void fill_rows(const SumArgs& a, int first) {
     const int row = first + __ffs(rows) - 1;
     rows &= rows - 1;
     TW* o = static_cast<TW*>(a.dw) + static_cast<std::int64_t>(row) * a.features;
-    if constexpr (UPDATE) {
+    if constexpr (UPDATE == kScale) {
       for (int h = lane * VEC; h < a.features; h += 32 * VEC) {
         float v[VEC];
         unpack<TW, VEC>(load_run<TW, VEC>(o + h), v);
@@ -761,13 +876,13 @@ __device__ __forceinline__ void fill_rows(const SumArgs& a, int first) {
 
 // A warp takes a block's slice, or rows to fill, at a time: the sums first, so that their
 // latency hides behind the filling, which takes all the bandwidth that is left.
-template <bool UPDATE, typename T, typename TW, int VEC, int RUNS, int AHEAD>
+template <int UPDATE, typename T, typename TW, int VEC, int RUNS, int AHEAD>
 __global__ void __launch_bounds__(kSumThreads, kSumCtas) embedding_sum_kernel(const SumArgs a) {
   tc::grid_launch_next();
   tc::grid_wait_previous();
   using S = Slice<VEC, RUNS>;
   // as many rows as the registers hold, with dw's where they are loaded too
-  constexpr int kAhead = !UPDATE ? AHEAD : sizeof(TW) > sizeof(T) ? 3 : AHEAD / 2;
+  constexpr int kAhead = UPDATE != kScale ? AHEAD : sizeof(TW) > sizeof(T) ? 3 : AHEAD / 2;
   const unsigned slices = (a.features + S::kFeatures - 1) / S::kFeatures;
   const int total = *a.total;
   const std::int64_t sums = static_cast<std::int64_t>((total + a.block - 1) / a.block) * slices;
@@ -786,11 +901,15 @@ __global__ void __launch_bounds__(kSumThreads, kSumCtas) embedding_sum_kernel(co
 }
 
 // ------------------------------------------------------------------------- planning --
-// Entries per block: a warp's batch of loads, longer only where that would leave more than
-// 1024 partial sums of one word.
-int block_entries(int tokens) {
-  int n = 32;
-  while (tokens / n > 1024) n *= 2;
+// Entries per block, 8 to 32: few, for the latency of a block's batches of loads, as long as
+// every warp that the GPU holds has one block's slice (256 features) and a frequent word (a
+// twelfth of the tokens) has no more partial sums than a block has entries.  More than 32 only
+// where one word could have more than 1024 partial sums.
+int block_entries(int tokens, int features) {
+  const std::int64_t slices = (features + 255) / 256, warps = std::int64_t{sms()} * kSumCtas * kSumWarps;
+  int n = 8;
+  while (n < 32 && (tokens / n * slices > warps || 25 * n * n < tokens)) n *= 2;
+  while (tokens / n > 1024 && n >= 32) n *= 2;
   return n;
 }
 
@@ -806,7 +925,7 @@ SortPlan plan(const EmbeddingArgs& a) {
   SortPlan p{};
   while ((a.vocab - 1) >> kOwnerBits >> (p.passes * kDigit) != 0) ++p.passes;
   p.per_owner = (a.vocab + kOwners - 1) / kOwners;
-  p.block = block_entries(a.tokens);
+  p.block = block_entries(a.tokens, a.features);
   std::size_t at = 0;
   const auto take = [&](std::size_t n) {
     const std::size_t o = at;
@@ -878,10 +997,13 @@ cudaError_t gradient(const EmbeddingArgs& a, const SortPlan& p, char* ws, cudaSt
   const std::int64_t ctas =
       std::min<std::int64_t>((units + kSumWarps - 1) / kSumWarps, sms() * kSumCtas);
   static_assert(kSlice >= kLeastSlice, "the counters are for fewer slices");
-  return tc::launch_overlapped(a.beta != 0.0f
-                                   ? embedding_sum_kernel<true, T, TW, VEC, RUNS, AHEAD>
-                                   : embedding_sum_kernel<false, T, TW, VEC, RUNS, AHEAD>,
-                               dim3(static_cast<unsigned>(ctas)), kSumThreads, 0, st, true, s);
+  auto kern = a.beta != 0.0f ? embedding_sum_kernel<kScale, T, TW, VEC, RUNS, AHEAD>
+                             : embedding_sum_kernel<kWrite, T, TW, VEC, RUNS, AHEAD>;
+  if constexpr (std::is_same_v<TW, float>) {
+    if (a.beta == 1.0f) kern = embedding_sum_kernel<kAdd, T, TW, VEC, RUNS, AHEAD>;
+  }
+  return tc::launch_overlapped(kern, dim3(static_cast<unsigned>(ctas)), kSumThreads, 0, st, true,
+                               s);
 }
 
 }  // namespace
