@@ -193,6 +193,12 @@ constexpr int kUnit = 128;
 // tokens that would cost up to 37 % (score of 128 x 768 x 50257).
 constexpr int kLogitsChunk = 8, kFewLogitsChunk = 2;
 
+// What a truncating MMA takes from a logit, as a share of it and on average (measured: 4.9e-7 of
+// the logits of 32 MMAs that an lse is made of, 1.2e-7 of 4; 3.7e-7 of large ones of 32).  It is
+// no error of a single cross entropy, but the losses of sequences add it up: their logits, and
+// the exponents' scale, are larger by it (rewards of 250-token sequences XX).
+constexpr double kTruncated = 1.3e-8;
+
 // A thread's logits of one token, and what says whether a target word is among them: the
 // token's label, or its entry of the hit map.  Loaded before the
 // accumulator is waited for, looked at after.
@@ -978,6 +984,7 @@ struct FinishArgs {
   std::int64_t ldx;
   const void* w;
   int features;
+  float truncated;
   PolicyLoss policy;
   float* dnll;  // kNone: null, or the gradients by the tokens' nll (without a policy zeros)
   const float* dloss;
@@ -1201,8 +1208,9 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
           static_cast<const T*>(a.x) + row * a.ldx,
           static_cast<const T*>(a.w) + a.targets.labels[row] * a.features, a.features, dots);
       if (fabsf(z - was) < INFINITY) {  // the target's own share of the sum moves too
-        const float moved = sum + exp2f(above(r0)) * expm1f((z - was) * a.inv_tau);
-        nll = (log2f(moved) - (z - mx) * a.log2e_tau) * kLn2;
+        const float moved =
+            sum + exp2f(above(r0)) * expm1f(((z - was) - was * a.truncated) * a.inv_tau);
+        nll = logf(moved) - ((z - mx) - mx * a.truncated) * a.inv_tau;
       }
     }
   }
@@ -2079,6 +2087,12 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, const TokenRows& all, cha
       return form == kPolicy ? vocab_finish_kernel<T, kStore, kPolicy>
                              : vocab_finish_kernel<T, kStore, kTargetLoss>;
     };
+    float z_scale = kLog2e * a.inv_tau;
+    if (form != kTargetLoss) {
+      const int chunk = 4 * (rows <= kStreamTokens ? kFewLogitsChunk : kLogitsChunk);
+      f.truncated = static_cast<float>(kTruncated * std::min(chunk, (a.features + 15) / 16));
+      z_scale = static_cast<float>(1.4426950408889634 * a.inv_tau * (1.0 + f.truncated));
+    }
     f.x = x;
     f.ldx = ldx;
     f.w = a.w;
@@ -2094,13 +2108,13 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, const TokenRows& all, cha
       f.policy.kl = from(a.policy.kl);
     }
     f.inv_tau = a.inv_tau;
-    f.log2e_tau = kLog2e * a.inv_tau;
+    f.log2e_tau = z_scale;
     f.scale = scale;
     f.num = num;
     f.ldn = p.ldn;
     f.pitch = p.copies * p.ldn;
     if (p.stream) {
-      const StreamArgs sa{x, ldx, w, ldw, rows, a.features, a.vocab, kLog2e * a.inv_tau,
+      const StreamArgs sa{x, ldx, w, ldw, rows, a.features, a.vocab, z_scale,
                           reinterpret_cast<float2*>(ws + p.stats), tg};
       MB200_TRY(launch(vocab_stream_kernel<T>, p.units, kStreamThreads, sa));
       MB200_TRY(launch(finish_form(std::integral_constant<int, kNone>{}), rows, kFinishThreads, f));
@@ -2122,7 +2136,7 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, const TokenRows& all, cha
     // measured at 8192 x 4096 x 65536: 16 MB of x kept 3.2 GB of DRAM reads, 33 MB 2.0, 50 MB
     // 3.3, all 67 MB 4.5 (the numerators pass through L2 too)
     lp.band = band_of(lp.tiles_m, 512ll * a.features, 36ll << 20);
-    lp.scale = kLog2e * a.inv_tau;
+    lp.scale = z_scale;
     lp.stats = reinterpret_cast<float2*>(ws + p.stats);
     lp.ldn = p.ldn;
     lp.targets = tg;

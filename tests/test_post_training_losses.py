@@ -522,8 +522,8 @@ def test_one_gradient_alone_and_in_place(cuda, built, kind, T):
 
 @pytest.mark.gpu
 def test_policy_of_its_own_samples_is_a_weighted_cross_entropy(cuda, built):
-    """With ratio 1 and no divergence the gradient is that of A nll, bit for bit; nll itself is
-    the cross entropy with a more exact target."""
+    """With ratio 1 and no divergence the gradient is that of A nll: both calls are within what
+    either may be off.  nll itself is the cross entropy with a more exact target."""
     h = Policy(cuda, 300, 136, 1000, coef=0.0, old=False, dual=0.0, seed=6)
     with Dnn(cuda) as d:
         assert h.backward(d) == 0
@@ -533,7 +533,13 @@ def test_policy_of_its_own_samples_is_a_weighted_cross_entropy(cuda, built):
         c.dloss = h.dloss * h.advantages
         assert c.backward(d) == 0
         cuda.cuda.synchronize()
-    assert cuda.equal(h.dx, c.dx) and cuda.equal(h.dw, c.dw)
+        c.check()
+        h.check()
+        policy = h.dx, h.dw
+        h.dx, h.dw = c.dx, c.dw
+        h.check()
+        c.dx, c.dw = policy
+        c.check()
     nll, e, _, _ = h.nll64()
     assert ((h.nll - c.loss).abs() <= 2 * e).all()
     assert (h.nll - nll).norm() <= (c.loss - nll).norm()
