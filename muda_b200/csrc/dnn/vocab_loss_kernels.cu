@@ -797,7 +797,77 @@ __device__ __forceinline__ PolicyTerms policy_terms(const PolicyLoss& p, int row
   return t;
 }
 
-constexpr int kPreferenceThreads = 512;
+// The scale of a preference's gradients on their way into dw (more than 64 tokens).  All tokens
+// of a sequence have the same |dnll|, and unlikely targets, whose dz is nearly that, round alike:
+// what a few sequences' rounding leaves does not average out in dw (up to 2.5 times one rounding
+// for a single pair).  Of 64 scales within a factor of two this takes the one that leaves the
+// targets' dz the least, as the vocab_grad_scale_kernel's otherwise: the largest |dnll / tau| comes to
+// (2^12, 2^14].  dw's error over one rounding for 13 pairs of 777 x 1111 x 32003: XX.
+constexpr int kScales = 32, kScaleSamples = 512, kScaleThreads = 512;
+
+// The whole CTA of kScaleThreads calls this.
+template <typename T>
+__device__ __forceinline__ void find_pair_scale(const float* dnll, const float* nll, int rows,
+                                                int vocab, const Targets& targets, float inv_tau,
+                                                float* scale) {
+  __shared__ float red[kScaleThreads / 32], dz[kScaleSamples], left[kScales];
+  constexpr int kWarps = kScaleThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float mx = 0.0f;
+  for (int i = threadIdx.x; i < rows; i += kScaleThreads) {
+    const float g = fabsf(__ldcg(dnll + i) * inv_tau);  // other CTAs may have written it just now
+    if (target_count(targets, i, vocab) > 0 && g < INFINITY) mx = fmaxf(mx, g);
+  }
+  mx = warp_max(mx);
+  if (lane == 0) red[warp] = mx;
+  static_assert(kScaleSamples == kScaleThreads, "a sample per thread");
+  const int row = static_cast<int>(static_cast<std::int64_t>(threadIdx.x) *
+                                   max(rows, kScaleSamples) / kScaleSamples);
+  float target = 0.0f;
+  if (row < rows && target_count(targets, row, vocab) > 0)
+    target = __ldcg(dnll + row) * inv_tau * expm1f(-nll[row]);
+  dz[threadIdx.x] = fabsf(target) < INFINITY ? target : 0.0f;
+  __syncthreads();
+  mx = warp_max(lane < kWarps ? red[lane] : 0.0f);
+  int e = 0;
+  if (mx > 0.0f) frexpf(mx, &e);  // mx in [2^(e-1), 2^e)
+  e = max(-100, min(100, e));
+  for (int c = warp; c < kScales; c += kWarps) {
+    const float s = ldexpf(exp2f(c * (-1.0f / kScales)), 14 - e), undo = exp2f(c * (1.0f / kScales));
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kScaleSamples; i += 32) {
+      const float v = dz[i + lane] * s;
+      const float off = (v - static_cast<float>(from_float<T>(v))) * undo;  // in units of 2^(e-14)
+      sum = fmaf(off, off, sum);
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) left[c] = sum;
+  }
+  __syncthreads();
+  static_assert(kScales == 32, "a scale per lane");
+  if (warp == 0) {
+    const float least = -warp_max(-left[lane]);
+    const int best = __ffs(__ballot_sync(0xffffffffu, left[lane] == least)) - 1;
+    const float s = ldexpf(exp2f(best * (-1.0f / kScales)), 14 - e);
+    if (lane == 0) {
+      scale[0] = s;
+      scale[1] = 1.0f / s;
+    }
+  }
+}
+
+// Of a piece's rows, where a preference's gradients take several.
+template <typename T>
+__global__ void __launch_bounds__(kScaleThreads)
+    vocab_pair_scale_kernel(const float* __restrict__ dnll, const float* __restrict__ nll, int rows,
+                            int vocab, Targets targets, float inv_tau, float* __restrict__ scale) {
+  tc::grid_launch_next();
+  tc::grid_wait_previous();
+  find_pair_scale<T>(dnll, nll, rows, vocab, targets, inv_tau, scale);
+}
+
+constexpr int kPreferenceThreads = kScaleThreads, kPreferenceWarps = kPreferenceThreads / 32;
 
 struct PreferenceArgs {
   PreferenceLoss p;
@@ -806,37 +876,42 @@ struct PreferenceArgs {
   const float* nll;
   const float* dloss;   // [pairs], null: no gradient
   float* dnll;          // [tokens], holds zeros; rows of the pairs' tokens are written
+  // null, or find_pair_scale's for all tokens; its other arguments, and 0
+  float* scale;
+  float inv_tau;
+  int vocab;
+  int* pairs_done;
 };
 
-__device__ __forceinline__ double block_sum(double v, double* red) {
+__device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();  // red[] may still be read by the previous sum
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  double r = 0.0;
-#pragma unroll
-  for (int i = 0; i < kPreferenceThreads / 32; ++i) r += red[i];
-  return r;
+  return v;
 }
 
 // One CTA per pair: the two sequences' sums, the pair's loss, and the derivative by each of
 // their tokens' nll.  Sums are in 64 bits: the difference of two sums of thousands of tokens is
-// what the loss sees.  A pair whose offsets do not ascend within the tokens is NaN.
+// what the loss sees.  A pair whose offsets do not ascend within the tokens is NaN.  The last
+// CTA to come to its end has all pairs' gradients before it for the scale.
+template <typename T>
 __global__ void __launch_bounds__(kPreferenceThreads)
     vocab_preference_kernel(const PreferenceArgs a) {
   tc::grid_launch_next();
   tc::grid_wait_previous();
-  __shared__ double red[kPreferenceThreads / 32];
+  __shared__ double sums[2][kPreferenceWarps];
+  __shared__ int counts[2][kPreferenceWarps];
+  __shared__ bool last;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int pair = blockIdx.x;
   std::int64_t begin[2], end[2];
-  double sum[2], n[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    begin[k] = a.p.offsets[pair + k * a.p.pairs];
+    end[k] = a.p.offsets[pair + k * a.p.pairs + 1];
+  }
   bool bad = false;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const int s = pair + k * a.p.pairs;
-    begin[k] = a.p.offsets[s];
-    end[k] = a.p.offsets[s + 1];
     if (begin[k] < 0 || end[k] < begin[k] || end[k] > a.tokens) {
       bad = true;
       begin[k] = end[k] = 0;
@@ -848,27 +923,39 @@ __global__ void __launch_bounds__(kPreferenceThreads)
     int kept = 0;
 #pragma unroll 4
     for (std::int64_t t = begin[k] + threadIdx.x; t < end[k]; t += kPreferenceThreads) {
-      if (a.labels[t] < 0) continue;
-      v += static_cast<double>(a.p.ref_nll != nullptr ? a.p.ref_nll[t] : 0.0f) - a.nll[t];
-      ++kept;
+      const float ref = a.p.ref_nll != nullptr ? a.p.ref_nll[t] : 0.0f, nll = a.nll[t];
+      const bool in = a.labels[t] >= 0;
+      v += in ? static_cast<double>(ref) - nll : 0.0;
+      kept += in;
     }
-    sum[k] = block_sum(v, red);
-    n[k] = block_sum(kept, red);
+    v = warp_sum(v);
+    kept = warp_sum(kept);
+    if (lane == 0) {
+      sums[k][warp] = v;
+      counts[k][warp] = kept;
+    }
   }
-  const bool live = bad || (n[0] > 0.0 && n[1] > 0.0);
-  double share[2] = {1.0, 1.0};
-  if (a.p.averaged) {
-    share[0] = 1.0 / n[0];
-    share[1] = 1.0 / n[1];
+  __syncthreads();
+  double gain[2], share[2] = {1.0, 1.0};
+  int n[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    gain[k] = warp_sum(lane < kPreferenceWarps ? sums[k][lane] : 0.0);
+    n[k] = warp_sum(lane < kPreferenceWarps ? counts[k][lane] : 0);
+    if (a.p.averaged) {
+      share[k] = 1.0 / n[k];
+      gain[k] *= share[k];
+    }
   }
+  const bool live = bad || (n[0] > 0 && n[1] > 0);
   const double beta = a.p.beta;
-  const double gain[2] = {sum[0] * share[0], sum[1] * share[1]};
   const double h = bad ? NAN : beta * (gain[0] - gain[1]) - a.p.margin;
   double loss, slope;
   if (a.p.mode == PreferenceMode::kSigmoid) {
-    const double e = exp(-fabs(h));
-    loss = log1p(e) + (h < 0.0 ? -h : 0.0) + a.p.smoothing * h;
-    slope = a.p.smoothing - (h < 0.0 ? 1.0 : e) / (1.0 + e);
+    // of h's own size the loss keeps 64 bits; what softplus adds to it is a float
+    const float e = expf(static_cast<float>(-fabs(h)));
+    loss = (h < 0.0 ? -h : 0.0) + a.p.smoothing * h + log1pf(e);
+    slope = a.p.smoothing - (h < 0.0 ? 1.0f : e) / (1.0f + e);
   } else if (a.p.mode == PreferenceMode::kHinge) {
     loss = h < 1.0 ? 1.0 - h : h >= 1.0 ? 0.0 : h;
     slope = h < 1.0 ? -1.0 : h >= 1.0 ? 0.0 : h;
@@ -885,70 +972,26 @@ __global__ void __launch_bounds__(kPreferenceThreads)
             bad ? NAN : live ? static_cast<float>(beta * gain[k]) : 0.0f;
     }
   }
-  if (a.dloss == nullptr || !live || bad) return;
-  const double g = a.dloss[pair] * slope * beta;
+  if (a.dloss == nullptr) return;
+  if (live && !bad) {
+    const double g = a.dloss[pair] * slope * beta;
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const auto each = static_cast<float>((k == 0 ? -g : g) * share[k]);
-    for (std::int64_t t = begin[k] + threadIdx.x; t < end[k]; t += kPreferenceThreads)
-      a.dnll[t] = each;  // of tokens left out, nothing reads it
-  }
-}
-
-// The scale of a preference's gradients on their way into dw (more than 64 tokens).  All tokens
-// of a sequence have the same |dnll|, and unlikely targets, whose dz is nearly that, round alike:
-// what a few sequences' rounding leaves does not average out in dw (up to 2.5 times one rounding
-// for a single pair).  Of 64 scales within a factor of two this takes the one that leaves the
-// targets' dz the least, as the vocab_grad_scale_kernel's otherwise: the largest |dnll / tau| comes to
-// (2^12, 2^14].  dw's error over one rounding for 13 pairs of 777 x 1111 x 32003: XX.
-constexpr int kScales = 64, kScaleSamples = 1024;
-
-template <typename T>
-__global__ void __launch_bounds__(1024)
-    vocab_pair_scale_kernel(const float* __restrict__ dnll, const float* __restrict__ nll, int rows,
-                            int vocab, Targets targets, float inv_tau, float* __restrict__ scale) {
-  tc::grid_launch_next();
-  tc::grid_wait_previous();
-  __shared__ float red[32], dz[kScaleSamples], left[kScales];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float mx = 0.0f;
-  for (int i = threadIdx.x; i < rows; i += 1024) {
-    const float g = fabsf(dnll[i] * inv_tau);
-    if (target_count(targets, i, vocab) > 0 && g < INFINITY) mx = fmaxf(mx, g);
-  }
-  mx = warp_max(mx);
-  if (lane == 0) red[warp] = mx;
-  const int row = static_cast<int>(static_cast<std::int64_t>(threadIdx.x) * max(rows, 1024) / 1024);
-  float target = 0.0f;
-  if (row < rows && target_count(targets, row, vocab) > 0)
-    target = dnll[row] * inv_tau * expm1f(-nll[row]);
-  dz[threadIdx.x] = fabsf(target) < INFINITY ? target : 0.0f;
-  __syncthreads();
-  mx = warp_max(red[lane]);
-  int e = 0;
-  if (mx > 0.0f) frexpf(mx, &e);  // mx in [2^(e-1), 2^e)
-  e = max(-100, min(100, e));
-  for (int c = warp; c < kScales; c += 32) {
-    const float s = ldexpf(exp2f(c * (-1.0f / kScales)), 14 - e), undo = exp2f(c * (1.0f / kScales));
-    float sum = 0.0f;
-#pragma unroll 8
-    for (int i = lane; i < kScaleSamples; i += 32) {
-      const float v = dz[i] * s;
-      const float off = (v - static_cast<float>(from_float<T>(v))) * undo;  // in units of 2^(e-14)
-      sum = fmaf(off, off, sum);
+    for (int k = 0; k < 2; ++k) {
+      const auto each = static_cast<float>((k == 0 ? -g : g) * share[k]);
+      for (std::int64_t t = begin[k] + threadIdx.x; t < end[k]; t += kPreferenceThreads)
+        a.dnll[t] = each;  // of tokens left out, nothing reads it
     }
-    sum = warp_sum(sum);
-    if (lane == 0) left[c] = sum;
   }
+  if (a.scale == nullptr) return;
+  __threadfence();
   __syncthreads();
-  if (threadIdx.x == 0) {
-    int best = 0;
-    for (int c = 1; c < kScales; ++c)
-      if (left[c] < left[best]) best = c;
-    const float s = ldexpf(exp2f(best * (-1.0f / kScales)), 14 - e);
-    scale[0] = s;
-    scale[1] = 1.0f / s;
-  }
+  if (threadIdx.x == 0) last = atomicAdd(a.pairs_done, 1) == static_cast<int>(gridDim.x) - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  Targets targets{};
+  targets.labels = a.labels;
+  find_pair_scale<T>(a.dnll, a.nll, a.tokens, a.vocab, targets, a.inv_tau, a.scale);
 }
 
 constexpr int kFinishThreads = 256;
@@ -986,6 +1029,7 @@ struct FinishArgs {
   int features;
   float truncated;
   PolicyLoss policy;
+  int* pairs_done;  // with dnll: to be set to 0
   float* dnll;  // kNone: null, or the gradients by the tokens' nll (without a policy zeros)
   const float* dloss;
   float inv_tau;
@@ -1093,12 +1137,12 @@ __device__ __forceinline__ uint4 scaled(uint4 u, float f, uint4* left = nullptr)
 enum FinishForm { kTargetLoss = 0, kNll = 1, kPolicy = 2 };
 
 // x[row] w[label] in fp32, to about half its last place: H / 256 rounded terms per thread, the
-// threads' sums in 64 bits (the whole CTA calls this).  The tensor cores' sums are short of
+// threads' sums in 64 bits (the whole CTA calls the second).  The tensor cores' sums are short of
 // that by up to 4e-7 of the logit, always toward zero, and a log ratio of two sequences adds
 // the like of it up over their tokens: rewards of 256-token sequences were 1.2e-5 off, their
 // plain fp32 form 6e-7.
 template <typename T>
-__device__ __forceinline__ float target_logit(const T* x, const T* w, int features, double* red) {
+__device__ __forceinline__ float target_logit_part(const T* x, const T* w, int features) {
   float part = 0.0f;
   if (((reinterpret_cast<std::uintptr_t>(x) | reinterpret_cast<std::uintptr_t>(w)) & 15) == 0) {
     for (int h = threadIdx.x * 8; h < features; h += kFinishThreads * 8) {
@@ -1122,6 +1166,10 @@ __device__ __forceinline__ float target_logit(const T* x, const T* w, int featur
     for (int h = threadIdx.x; h < features; h += kFinishThreads)
       part = fmaf(static_cast<float>(x[h]), static_cast<float>(w[h]), part);
   }
+  return part;
+}
+
+__device__ __forceinline__ float target_logit(float part, double* red) {
   double sum = part;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -1145,6 +1193,9 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
       transpose_tile<T, STORE == kSplit>(a.transpose, a.targets, a.vocab, blockIdx.x - finish);
       return;
     }
+  }
+  if constexpr (STORE == kNone) {
+    if (a.dnll != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *a.pairs_done = 0;
   }
   const int row = static_cast<int>(blockIdx.x % static_cast<unsigned>(a.rows));
   const int part = static_cast<int>(blockIdx.x / static_cast<unsigned>(a.rows));
@@ -1183,6 +1234,13 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     }
     return;
   }
+  [[maybe_unused]] float dot = 0.0f;  // its loads go out before the reductions below
+  if constexpr (FORM != kTargetLoss) {
+    if (n > 0)
+      dot = target_logit_part<T>(static_cast<const T*>(a.x) + row * a.ldx,
+                                 static_cast<const T*>(a.w) + a.targets.labels[row] * a.features,
+                                 a.features);
+  }
   const float2* st = a.stats + static_cast<std::int64_t>(row) * a.units;
   float mx = -INFINITY;
   for (int i = threadIdx.x; i < a.units; i += kFinishThreads)
@@ -1204,9 +1262,7 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     if constexpr (FORM != kTargetLoss) {
       __shared__ double dots[kFinishThreads / 32];
       const float was = a.targets.z[r0];
-      const float z = target_logit<T>(
-          static_cast<const T*>(a.x) + row * a.ldx,
-          static_cast<const T*>(a.w) + a.targets.labels[row] * a.features, a.features, dots);
+      const float z = target_logit(dot, dots);
       if (fabsf(z - was) < INFINITY) {  // the target's own share of the sum moves too
         const float moved =
             sum + exp2f(above(r0)) * expm1f(((z - was) - was * a.truncated) * a.inv_tau);
@@ -1262,14 +1318,24 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
       const Reference base = reference(mx, a.log2e_tau);
       down = fmaf(base.top - mx, a.log2e_tau, base.whole);
       if (part == 0 && threadIdx.x == 0) a.row_scale[row] = make_float2(exp2f(down - log_sum), g);
-      // only units whose reference is not the row's: rare
-      for (int u = u_begin + (threadIdx.x >> 5); u < u_end; u += kFinishThreads / 32) {
-        const Reference ref = reference(st[u].x, a.log2e_tau);
-        const float move = fmaf(ref.top - base.top, a.log2e_tau, ref.whole - base.whole);
-        if (st[u].y == 0.0f || move == 0.0f) continue;
-        const float f = exp2f(move);
-        const std::int64_t c = static_cast<std::int64_t>(u) * per_unit + (threadIdx.x & 31);
-        if ((threadIdx.x & 31) < per_unit && c < c_end) num[c] = scaled<T, STORE>(num[c], f);
+      // only units whose reference is not the row's: rare; a lane looks at a unit (2048 rows of
+      // 512 units: 42 us with a warp at each, XX)
+      const int lane = threadIdx.x & 31;
+      for (int u0 = u_begin + (threadIdx.x & ~31); u0 < u_end; u0 += kFinishThreads) {
+        float move = 0.0f;
+        if (u0 + lane < u_end) {
+          const float2 s = st[u0 + lane];
+          const Reference ref = reference(s.x, a.log2e_tau);
+          if (s.y != 0.0f) move = fmaf(ref.top - base.top, a.log2e_tau, ref.whole - base.whole);
+        }
+        unsigned moved = __ballot_sync(0xffffffffu, move != 0.0f);
+        while (moved != 0) {
+          const int u = __ffs(moved) - 1;
+          moved &= moved - 1;
+          const float f = exp2f(__shfl_sync(0xffffffffu, move, u));
+          const std::int64_t c = static_cast<std::int64_t>(u0 + u) * per_unit + lane;
+          if (lane < per_unit && c < c_end) num[c] = scaled<T, STORE>(num[c], f);
+        }
       }
     } else {
       const auto factor = [&](std::int64_t c) {
@@ -1796,7 +1862,7 @@ Plan plan_rows(const VocabLossArgs& a, int rows, bool sliced) {
   p.count = take(K > 0 ? R * 4 : 0);
   p.entropy = take(K > 0 ? R * 4 : 0);
   p.hit = take(K > 0 ? R * p.hit_units * 4 : 0);
-  p.scale = take(8);
+  p.scale = take(12);  // and the pairs that are done
   p.row_scale = take(a.gradients ? R * sizeof(float2) : 0);
   p.lefts = dx && p.store != kSplit && K <= kMostLeft ? std::max(a.top_k, 1) : 0;
   p.left = take(R * p.lefts * sizeof(Left));
@@ -1981,10 +2047,21 @@ struct TokenRows {
   float* dnll;
 };
 
-cudaError_t run_preference(const VocabLossArgs& a, const TokenRows& rows, cudaStream_t st) {
-  const PreferenceArgs g{a.preference, a.tokens, a.labels, rows.nll,
-                         a.gradients ? a.dloss : nullptr, rows.dnll};
-  return tc::launch_overlapped(vocab_preference_kernel,
+// scale: null, or where to leave the scale of all tokens' gradients.
+template <typename T>
+cudaError_t run_preference(const VocabLossArgs& a, const TokenRows& rows, float* scale,
+                           cudaStream_t st) {
+  const PreferenceArgs g{a.preference,
+                         a.tokens,
+                         a.labels,
+                         rows.nll,
+                         a.gradients ? a.dloss : nullptr,
+                         rows.dnll,
+                         scale,
+                         a.inv_tau,
+                         a.vocab,
+                         reinterpret_cast<int*>(scale != nullptr ? scale + 2 : nullptr)};
+  return tc::launch_overlapped(vocab_preference_kernel<T>,
                                dim3(static_cast<unsigned>(a.preference.pairs)),
                                kPreferenceThreads, 0, st, true, g);
 }
@@ -2052,14 +2129,14 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, const TokenRows& all, cha
     }
 
     float* scale = nullptr;
-    // nll: of a preference
+    float* const scale_at = reinterpret_cast<float*>(ws + p.scale);
+    const bool pair_scale = all.nll != nullptr && p.store == kOwn && a.dw != nullptr;
     const auto find_scale = [&](const float* dloss, const float* nll) -> cudaError_t {
-      const bool pairs = nll != nullptr && p.store == kOwn && a.dw != nullptr;
-      if (!pairs && a.bf16) return cudaSuccess;
-      scale = reinterpret_cast<float*>(ws + p.scale);
-      if (pairs)
-        return launch(vocab_pair_scale_kernel<T>, 1, 1024, dloss, nll, rows, a.vocab, tg, a.inv_tau,
-                      scale);
+      if (!pair_scale && a.bf16) return cudaSuccess;
+      scale = scale_at;
+      if (pair_scale)
+        return launch(vocab_pair_scale_kernel<T>, 1, kScaleThreads, dloss, nll, rows, a.vocab, tg,
+                      a.inv_tau, scale);
       return launch(vocab_grad_scale_kernel, 1, 1024, dloss, rows, a.vocab, tg, a.inv_tau, scale);
     };
     if (a.gradients && a.head == HeadLoss::kTargets)
@@ -2188,12 +2265,16 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, const TokenRows& all, cha
       s.loss = preference ? const_cast<float*>(all.nll) : f.loss;
       s.dnll = preference ? all.dnll : reinterpret_cast<float*>(ws + p.dnll);
       s.transpose.xt = nullptr;
+      s.pairs_done = reinterpret_cast<int*>(scale_at + 2);
       MB200_TRY(launch(finish_form(std::integral_constant<int, kNone>{}), rows, kFinishThreads, s));
       form = kTargetLoss;
-      if (preference) MB200_TRY(run_preference(a, all, st));
       f.loss = f.lse = nullptr;
       f.dloss = s.dnll;
-      MB200_TRY(find_scale(f.dloss, preference ? all.nll : nullptr));
+      if (preference) {
+        if (pair_scale) scale = scale_at;
+        MB200_TRY(run_preference<T>(a, all, scale, st));
+      }
+      if (scale == nullptr) MB200_TRY(find_scale(f.dloss, nullptr));
       f.scale = scale;
       return cudaSuccess;
     };
@@ -2304,11 +2385,12 @@ cudaError_t launch_vocab_loss(const VocabLossArgs& a, void* workspace, std::size
       const Plan sp = a.gradients ? plan_within(score, ws_bytes - r.bytes, false, &ok) : p;
       if (!ok) return cudaErrorInvalidValue;
       MB200_TRY(run_any(score, sp, rows, ws, stream));
-      if (!a.gradients) return run_preference(a, rows, stream);
+      const auto pairs = a.bf16 ? run_preference<__nv_bfloat16> : run_preference<__half>;
+      if (!a.gradients) return pairs(a, rows, nullptr, stream);
       if (cudaError_t e = cudaMemsetAsync(rows.dnll, 0, std::size_t(a.tokens) * 4, stream);
           e != cudaSuccess)
         return e;
-      MB200_TRY(run_preference(a, rows, stream));
+      MB200_TRY(pairs(a, rows, nullptr, stream));
       VocabLossArgs gradient = a;
       gradient.head = HeadLoss::kTargets;
       gradient.loss = gradient.lse = nullptr;
