@@ -297,10 +297,15 @@ constexpr int kShare = 8, kShareBits = 3;
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kDigit = 5, kDigits = 1 << kDigit;
 constexpr int kSharedList = 4096;  // entries that are sorted in shared memory
-constexpr int kScan = 8;           // tokens per lane at a time
+constexpr int kScan = 4;           // tokens per lane at a time
 constexpr int kCompared = 128;     // entries that are sorted by comparing each with all
 // Tokens that a cluster reads together: its launch takes 4 us more (XX).
 constexpr int kTogether = 16384;
+// Bytes of a large dw that the GPU fills in the meantime (beta 0), about what the sort's time
+// has room for: 8192 x 4096 of 128000 words 199 -> 193 us, 32768 x 2048 of 50257 128 -> 121,
+// 1537 x 1111 of 32003 20.4 -> 19.5; a dw of 8 MB 18 -> 20.
+constexpr std::int64_t kFillAtOnce = 16 << 20, kFillPerToken = 2000, kFillTogether = 1000;
+constexpr std::int64_t kFillLeast = 32 << 20;
 
 struct Entry {
   int word;  // v / kOwners
@@ -320,6 +325,8 @@ struct SortArgs {
   int* counters;   // out: zeros
   std::int64_t num_counters;
   int* total;      // out: entries
+  uint4* fill;     // to be set to zeros by the CTAs behind the owners'
+  std::int64_t num_fill;
 };
 
 __device__ __forceinline__ int warp_sum(int v) {
@@ -382,6 +389,16 @@ __device__ __forceinline__ void sort_body(const SortArgs& a) {
   __shared__ int found[kCtas + 1][kSortWarps];  // by owner of the cluster, then those before
   // of every CTA of the cluster: its tokens of each owner of the cluster, and of those before
   __shared__ int shares[kCtas][kCtas + 1];
+  if (blockIdx.x >= kOwners) {
+    tc::grid_launch_next();
+    tc::grid_wait_previous();
+    const std::int64_t step = static_cast<std::int64_t>(gridDim.x - kOwners) * kSortThreads;
+#pragma unroll 4
+    for (std::int64_t i = static_cast<std::int64_t>(blockIdx.x - kOwners) * kSortThreads + threadIdx.x;
+         i < a.num_fill; i += step)
+      __stcs(a.fill + i, make_uint4(0, 0, 0, 0));
+    return;
+  }
   // each CTA of the cluster runs before another writes into its shared memory
   if constexpr (BITS > 0) asm volatile("barrier.cluster.arrive.relaxed.aligned;");
   tc::grid_launch_next();
@@ -568,11 +585,11 @@ __device__ __forceinline__ void sort_body(const SortArgs& a) {
   }
 }
 
-__global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const SortArgs a) {
+__global__ void __launch_bounds__(kSortThreads, 2) embedding_sort_kernel(const SortArgs a) {
   sort_body<0>(a);
 }
 
-__global__ void __cluster_dims__(kShare, 1, 1) __launch_bounds__(kSortThreads, 1)
+__global__ void __cluster_dims__(kShare, 1, 1) __launch_bounds__(kSortThreads, 2)
     embedding_sort_together_kernel(const SortArgs a) {
   sort_body<kShareBits>(a);
 }
@@ -584,6 +601,7 @@ struct SumArgs {
   int features, vocab;
   int block;  // entries per block
   int per_owner;
+  int first_row;  // of those to be filled: the rows before it are zeros already
   int fill_rows;  // rows that a warp fills at a time
   const int* word;
   const int* pos;
@@ -886,7 +904,8 @@ __global__ void __launch_bounds__(kSumThreads, kSumCtas) embedding_sum_kernel(co
   const unsigned slices = (a.features + S::kFeatures - 1) / S::kFeatures;
   const int total = *a.total;
   const std::int64_t sums = static_cast<std::int64_t>((total + a.block - 1) / a.block) * slices;
-  const std::int64_t fills = a.beta == 1.0f ? 0 : (a.vocab + a.fill_rows - 1) / a.fill_rows;
+  const std::int64_t fills =
+      a.beta == 1.0f ? 0 : (a.vocab - a.first_row + a.fill_rows - 1) / a.fill_rows;
   const std::int64_t step = static_cast<std::int64_t>(gridDim.x) * kSumWarps;
   for (std::int64_t u = static_cast<std::int64_t>(blockIdx.x) * kSumWarps + (threadIdx.x >> 5);
        u < sums + fills; u += step) {
@@ -895,7 +914,7 @@ __global__ void __launch_bounds__(kSumThreads, kSumCtas) embedding_sum_kernel(co
       const int slice = static_cast<int>(u - b * static_cast<std::int64_t>(slices));
       sum_block<UPDATE, T, TW, VEC, RUNS, kAhead>(a, b, slice, slices, total);
     } else {
-      fill_rows<UPDATE, TW, VEC>(a, static_cast<int>(u - sums) * a.fill_rows);
+      fill_rows<UPDATE, TW, VEC>(a, a.first_row + static_cast<int>(u - sums) * a.fill_rows);
     }
   }
 }
@@ -971,7 +990,8 @@ bool rows_of_runs(const EmbeddingArgs& a, int vec) {
 }
 
 template <typename T, typename TW, int VEC, int RUNS, int AHEAD>
-cudaError_t gradient(const EmbeddingArgs& a, const SortPlan& p, char* ws, cudaStream_t st) {
+cudaError_t gradient(const EmbeddingArgs& a, const SortPlan& p, int first_row, char* ws,
+                     cudaStream_t st) {
   SumArgs s{};
   s.dy = a.row;
   s.ld = a.ld;
@@ -988,12 +1008,14 @@ cudaError_t gradient(const EmbeddingArgs& a, const SortPlan& p, char* ws, cudaSt
   s.dw = a.w;
   s.alpha = a.alpha;
   s.beta = a.beta;
+  s.first_row = first_row;
   s.fill_rows = std::clamp<int>(kFillBytes / (a.features * sizeof(TW)), 1, kMostFillRows);
   constexpr int kSlice = Slice<VEC, RUNS>::kFeatures;
   const std::int64_t slices = (a.features + kSlice - 1) / kSlice;
   const std::int64_t blocks = (a.tokens + p.block - 1) / p.block;
   const std::int64_t units =
-      blocks * slices + (a.beta == 1.0f ? 0 : (a.vocab + s.fill_rows - 1) / s.fill_rows);
+      blocks * slices +
+      (a.beta == 1.0f ? 0 : (a.vocab - first_row + s.fill_rows - 1) / s.fill_rows);
   const std::int64_t ctas =
       std::min<std::int64_t>((units + kSumWarps - 1) / kSumWarps, sms() * kSumCtas);
   static_assert(kSlice >= kLeastSlice, "the counters are for fewer slices");
@@ -1065,26 +1087,42 @@ cudaError_t launch_embedding_gradient(const EmbeddingArgs& a, void* workspace,
   if (!sort_attributes()) return cudaErrorInvalidDevice;
   s.near_list = std::min(a.tokens, kSharedList);
   const std::size_t shared = 2 * s.near_list * sizeof(Entry);
+  // rows that are set to zero while the tokens are sorted
+  int first_row = 0;
+  const std::int64_t row_bytes =
+      static_cast<std::int64_t>(a.features) * (a.table == EmbeddingType::kF32 ? 4 : 2);
+  unsigned fill_ctas = 0;
+  if (a.beta == 0.0f && aligned_to(a.w, 16) && a.vocab * row_bytes >= kFillLeast) {
+    const std::int64_t bytes =
+        kFillAtOnce + a.tokens * (a.tokens < kTogether ? kFillPerToken : kFillTogether);
+    // multiples of 8 rows are whole 16-byte words
+    first_row = static_cast<int>(std::min<std::int64_t>(a.vocab, bytes / row_bytes) / 8 * 8);
+    s.fill = static_cast<uint4*>(a.w);
+    s.num_fill = first_row * row_bytes / 16;
+    fill_ctas = static_cast<unsigned>(std::min<std::int64_t>(
+        (2 * sms() - kOwners) / kShare, (s.num_fill + kShare * kSortThreads - 1) / (kShare * kSortThreads)));
+    fill_ctas *= kShare;
+  }
   const cudaError_t e = tc::launch_overlapped(
-      a.tokens < kTogether ? embedding_sort_kernel : embedding_sort_together_kernel, dim3(kOwners),
-      kSortThreads, shared, st, false, s);
+      a.tokens < kTogether ? embedding_sort_kernel : embedding_sort_together_kernel,
+      dim3(kOwners + fill_ctas), kSortThreads, shared, st, false, s);
   if (e != cudaSuccess) return e;
   const bool wide = rows_of_runs(a, a.rows == T::kF32 ? 4 : 8);
   if (a.rows == T::kF32)
-    return wide ? gradient<float, float, 4, 1, 8>(a, p, ws, st)
-                : gradient<float, float, 1, 4, 4>(a, p, ws, st);
+    return wide ? gradient<float, float, 4, 1, 8>(a, p, first_row, ws, st)
+                : gradient<float, float, 1, 4, 4>(a, p, first_row, ws, st);
   if (a.rows == T::kF16) {
     if (a.table == T::kF32)
-      return wide ? gradient<__half, float, 8, 1, 8>(a, p, ws, st)
-                  : gradient<__half, float, 1, 4, 4>(a, p, ws, st);
-    return wide ? gradient<__half, __half, 8, 1, 8>(a, p, ws, st)
-                : gradient<__half, __half, 1, 4, 4>(a, p, ws, st);
+      return wide ? gradient<__half, float, 8, 1, 8>(a, p, first_row, ws, st)
+                  : gradient<__half, float, 1, 4, 4>(a, p, first_row, ws, st);
+    return wide ? gradient<__half, __half, 8, 1, 8>(a, p, first_row, ws, st)
+                : gradient<__half, __half, 1, 4, 4>(a, p, first_row, ws, st);
   }
   if (a.table == T::kF32)
-    return wide ? gradient<__nv_bfloat16, float, 8, 1, 8>(a, p, ws, st)
-                : gradient<__nv_bfloat16, float, 1, 4, 4>(a, p, ws, st);
-  return wide ? gradient<__nv_bfloat16, __nv_bfloat16, 8, 1, 8>(a, p, ws, st)
-              : gradient<__nv_bfloat16, __nv_bfloat16, 1, 4, 4>(a, p, ws, st);
+    return wide ? gradient<__nv_bfloat16, float, 8, 1, 8>(a, p, first_row, ws, st)
+                : gradient<__nv_bfloat16, float, 1, 4, 4>(a, p, first_row, ws, st);
+  return wide ? gradient<__nv_bfloat16, __nv_bfloat16, 8, 1, 8>(a, p, first_row, ws, st)
+              : gradient<__nv_bfloat16, __nv_bfloat16, 1, 4, 4>(a, p, first_row, ws, st);
 }
 
 }  // namespace mb200::dnn
