@@ -283,28 +283,26 @@ __global__ void __launch_bounds__(kLookupThreads, kLookupCtas)
 
 // ---------------------------------------------------------------------- the order --
 // CTA c owns the words v with v % kOwners == c (frequent words are neighbours in most
-// vocabularies, so ranges of words would leave one CTA most of the tokens).  Every CTA reads all
-// tokens: it counts those of the owners before it, which gives the place of its own in the
-// ordered list, takes its own in position order, and sorts them by word.  Many tokens are read
-// by clusters of SHARE neighbouring owners, a contiguous share by each CTA, which hands the
-// cluster's own to their owners' shared memory.  A warp goes over a contiguous share of the
-// list in all steps, so equal words keep their order, whatever the split between the warps.  No
-// CTA or cluster waits for another.
+// vocabularies, so ranges of words would leave one CTA most of the tokens).  It finds the place
+// of its own tokens in the ordered list, which is how many the owners before it have, lists its
+// own in position order, and sorts them by word.  Up to kParted tokens every CTA reads them all
+// to that end; more are parted first, by a kernel that orders each of kParts runs of tokens by
+// owner, of which every CTA then collects its own.  A warp goes over a contiguous share of the
+// tokens or of the list in all steps, so equal words keep their order, whatever the split between
+// the warps.  No CTA waits for another.
 //
 // Latency bound: XX
 constexpr int kOwners = 128, kOwnerBits = 7;
-constexpr int kShare = 8, kShareBits = 3;
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kDigit = 5, kDigits = 1 << kDigit;
 constexpr int kSharedList = 4096;  // entries that are sorted in shared memory
 constexpr int kScan = 4;           // tokens per lane at a time
 constexpr int kCompared = 128;     // entries that are sorted by comparing each with all
-// Tokens that a cluster reads together: its launch takes 4 us more (XX).
-constexpr int kTogether = 16384;
+constexpr int kParts = 128, kParted = 8192;
 // Bytes of a large dw that the GPU fills in the meantime (beta 0), about what the sort's time
 // has room for: 8192 x 4096 of 128000 words 199 -> 193 us, 32768 x 2048 of 50257 128 -> 121,
 // 1537 x 1111 of 32003 20.4 -> 19.5; a dw of 8 MB 18 -> 20.
-constexpr std::int64_t kFillAtOnce = 16 << 20, kFillPerToken = 2000, kFillTogether = 1000;
+constexpr std::int64_t kFillAtOnce = 16 << 20, kFillPerToken = 2000, kFillParted = 1000;
 constexpr std::int64_t kFillLeast = 32 << 20;
 
 struct Entry {
@@ -318,6 +316,9 @@ struct SortArgs {
   int passes;
   int near_list;   // min(tokens, kSharedList)
   Entry* list[2];  // [tokens] each: longer lists while they are sorted
+  int share;       // tokens of a part, a multiple of 32; 0: they are not parted
+  Entry* parts;    // [part][share], ordered by owner
+  int* starts;     // [owner or kOwners][part]: where the owner's tokens start in the part
   int* word;       // [tokens] out: the words in order
   int* pos;        // [tokens] out: and their positions
   int2* span;      // [owner][per_owner] out: a word's entries, {0, 0}: none
@@ -333,31 +334,6 @@ __device__ __forceinline__ int warp_sum(int v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
-}
-
-// *p = v in the shared memory of the cluster's CTA `rank`.
-template <int BITS, typename T>
-__device__ __forceinline__ void store_cluster(T* p, int rank, T v) {
-  if constexpr (BITS == 0) {
-    *p = v;
-  } else {
-    const std::uint32_t addr = tc::cluster_addr(p, rank);
-    if constexpr (sizeof(T) == 8) {
-      const auto w = *reinterpret_cast<const uint2*>(&v);
-      asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(w.x), "r"(w.y)
-                   : "memory");
-    } else {
-      asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
-    }
-  }
-}
-
-template <int BITS>
-__device__ __forceinline__ void sync_cluster() {
-  if constexpr (BITS == 0)
-    __syncthreads();
-  else
-    tc::cluster_sync();  // at cluster scope: what went to global memory is visible too
 }
 
 // The lanes of `among` whose low BITS bits (ballots in `bits`) are c's.
@@ -379,19 +355,193 @@ __device__ __forceinline__ int warp_inclusive(int v) {
   return v;
 }
 
-template <int BITS>
-__device__ __forceinline__ void sort_body(const SortArgs& a) {
-  constexpr int kCtas = 1 << BITS;  // of the cluster
-  extern __shared__ Entry near[];   // two lists of near_list entries
+// The token at t as a word, -1 if it enters nothing.
+__device__ __forceinline__ int word_of(const SortArgs& a, std::int64_t token) {
+  return token >= 0 && token < a.vocab ? static_cast<int>(token) : -1;
+}
+
+// CTA q orders its part of the tokens by owner.
+__global__ void __launch_bounds__(kSortThreads) embedding_part_kernel(const SortArgs a) {
+  __shared__ int count[kOwners][kSortWarps + 1];
+  __shared__ int totals[kOwners];
+  tc::grid_launch_next();
+  tc::grid_wait_previous();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, q = blockIdx.x;
+  const unsigned before_me = (1u << lane) - 1;
+  for (int o = warp; o < kOwners; o += kSortWarps) count[o][lane] = 0;
+  __syncthreads();
+  const int per_warp = (a.share + kSortThreads - 1) / kSortThreads * 32;
+  const std::int64_t first = static_cast<std::int64_t>(q) * a.share;
+  const std::int64_t t0 = first + warp * per_warp;
+  const std::int64_t t1 = min(min(t0 + per_warp, first + a.share), static_cast<std::int64_t>(a.tokens));
+  // the lane's token of the 32 from t on, and the lanes whose tokens have the same owner
+  const auto owners = [&](std::int64_t t, int* word) {
+    *word = word_of(a, load8(a.token + t + lane, t + lane < t1));
+    unsigned bits[kOwnerBits + 1];
+#pragma unroll
+    for (int k = 0; k < kOwnerBits; ++k) bits[k] = __ballot_sync(0xffffffffu, (*word >> k & 1) != 0);
+    return lanes_of<kOwnerBits>(__ballot_sync(0xffffffffu, *word >= 0), bits, *word);
+  };
+  for (std::int64_t t = t0; t < t1; t += 32) {
+    int word;
+    const unsigned same = owners(t, &word);
+    if (word >= 0 && (same & before_me) == 0) count[word & (kOwners - 1)][warp] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  constexpr int kEach = kOwners / kSortWarps;  // owners that a warp scans
+  int upto[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int x = count[warp * kEach + k][lane];
+    const int sum = warp_inclusive(x);
+    upto[k] = sum - x;
+    if (lane == 31) totals[warp * kEach + k] = sum;
+  }
+  __syncthreads();
+  int mine = 0;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) mine += totals[lane * kEach + k];
+  int start = __shfl_sync(0xffffffffu, warp_inclusive(mine) - mine, warp);
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int o = warp * kEach + k;
+    count[o][lane] = start + upto[k];
+    if (lane == 0) a.starts[o * kParts + q] = start;
+    start += totals[o];
+  }
+  if (threadIdx.x == kSortThreads - 1) a.starts[kOwners * kParts + q] = start;
+  __syncthreads();
+  Entry* part = a.parts + first;
+  for (std::int64_t t = t0; t < t1; t += 32) {
+    int word;
+    const unsigned same = owners(t, &word);
+    int* at = &count[word & (kOwners - 1)][warp];
+    if (word >= 0)
+      part[*at + __popc(same & before_me)] = {word >> kOwnerBits, static_cast<int>(t) + lane};
+    __syncwarp();
+    if (word >= 0 && (same & before_me) == 0) *at += __popc(same);
+    __syncwarp();
+  }
+}
+
+// Lists the owner's tokens in position order, from parts; returns how many there are and, in
+// *base, how many the owners before it have.
+__device__ __forceinline__ int collect(const SortArgs& a, Entry* near, int owner, int* base,
+                                       Entry** list) {
+  __shared__ int before[kParts + 1], from[kParts], sums[2][kParts / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int start = 0, n = 0, upto = 0;
+  if (threadIdx.x < kParts) {
+    start = a.starts[owner * kParts + threadIdx.x];
+    n = a.starts[(owner + 1) * kParts + threadIdx.x] - start;
+    upto = warp_inclusive(n);
+    const int starts = warp_sum(start);
+    if (lane == 31) {
+      sums[0][warp] = upto;
+      sums[1][warp] = starts;
+    }
+  }
+  __syncthreads();
+  int all = 0, lower = 0;
+  *base = 0;
+#pragma unroll
+  for (int w = 0; w < kParts / 32; ++w) {
+    if (w < warp) lower += sums[0][w];
+    all += sums[0][w];
+    *base += sums[1][w];
+  }
+  if (threadIdx.x < kParts) {
+    before[threadIdx.x] = lower + upto - n;
+    from[threadIdx.x] = threadIdx.x * a.share + start;
+  }
+  __syncthreads();
+  *list = all <= a.near_list ? near : a.list[0] + *base;
+  constexpr int kAtOnce = 4;
+  for (int i0 = threadIdx.x; i0 < all; i0 += kAtOnce * kSortThreads) {
+    Entry e[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int i = min(i0 + j * kSortThreads, all - 1);
+      int q = 0;  // the last part that starts at i or before
+#pragma unroll
+      for (int step = kParts / 2; step > 0; step /= 2)
+        if (before[q + step] <= i) q += step;
+      e[j] = a.parts[from[q] + (i - before[q])];
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j)
+      if (i0 + j * kSortThreads < all) (*list)[i0 + j * kSortThreads] = e[j];
+  }
+  __syncthreads();
+  return all;
+}
+
+// The same, from the tokens.
+__device__ __forceinline__ int select(const SortArgs& a, Entry* near, int owner, int* base,
+                                      Entry** list) {
+  __shared__ int found[2][kSortWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const unsigned before_me = (1u << lane) - 1;
+  const int per_warp = (a.tokens + kSortThreads - 1) / kSortThreads * 32;
+  const int t0 = warp * per_warp, t1 = min(t0 + per_warp, a.tokens);
+  const bool keep = per_warp <= 32 * kScan;  // in registers between the two readings
+  int v[kScan];
+  const auto load = [&](int t) {
+    std::int64_t w[kScan];
+#pragma unroll
+    for (int j = 0; j < kScan; ++j) {
+      const int i = t + 32 * j + lane;
+      w[j] = load8(a.token + i, i < t1);
+    }
+#pragma unroll
+    for (int j = 0; j < kScan; ++j) v[j] = word_of(a, w[j]);
+  };
+  const auto mine = [&](int word) {
+    return __ballot_sync(0xffffffffu, word >= 0 && (word & (kOwners - 1)) == owner);
+  };
+  int below = 0, n = 0;
+  for (int t = t0; t < t1; t += 32 * kScan) {
+    load(t);
+#pragma unroll
+    for (int j = 0; j < kScan; ++j) {
+      below += v[j] >= 0 && (v[j] & (kOwners - 1)) < owner;
+      n += __popc(mine(v[j]));
+    }
+  }
+  below = warp_sum(below);
+  if (lane == 0) {
+    found[0][warp] = n;
+    found[1][warp] = below;
+  }
+  __syncthreads();
+  const int upto = warp_inclusive(found[0][lane]);
+  int at = __shfl_sync(0xffffffffu, upto, warp) - n;
+  const int all = __shfl_sync(0xffffffffu, upto, 31);
+  *base = warp_sum(found[1][lane]);
+  *list = all <= a.near_list ? near : a.list[0] + *base;
+  for (int t = t0; t < t1; t += 32 * kScan) {
+    if (!keep) load(t);
+#pragma unroll
+    for (int j = 0; j < kScan; ++j) {
+      const unsigned in = mine(v[j]);
+      if ((in >> lane & 1u) != 0)
+        (*list)[at + __popc(in & before_me)] = {v[j] >> kOwnerBits, t + 32 * j + lane};
+      at += __popc(in);
+    }
+  }
+  __syncthreads();
+  return all;
+}
+
+__global__ void __launch_bounds__(kSortThreads, 2) embedding_sort_kernel(const SortArgs a) {
+  extern __shared__ Entry near[];  // two lists of near_list entries
   // by digit, by warp: a warp's counters in banks of their own; two passes in turn
   __shared__ int count[2][kDigits][kSortWarps + 1];
   __shared__ int totals[2][kDigits];
-  __shared__ int found[kCtas + 1][kSortWarps];  // by owner of the cluster, then those before
-  // of every CTA of the cluster: its tokens of each owner of the cluster, and of those before
-  __shared__ int shares[kCtas][kCtas + 1];
+  tc::grid_launch_next();
+  tc::grid_wait_previous();
   if (blockIdx.x >= kOwners) {
-    tc::grid_launch_next();
-    tc::grid_wait_previous();
     const std::int64_t step = static_cast<std::int64_t>(gridDim.x - kOwners) * kSortThreads;
 #pragma unroll 4
     for (std::int64_t i = static_cast<std::int64_t>(blockIdx.x - kOwners) * kSortThreads + threadIdx.x;
@@ -399,121 +549,21 @@ __device__ __forceinline__ void sort_body(const SortArgs& a) {
       __stcs(a.fill + i, make_uint4(0, 0, 0, 0));
     return;
   }
-  // each CTA of the cluster runs before another writes into its shared memory
-  if constexpr (BITS > 0) asm volatile("barrier.cluster.arrive.relaxed.aligned;");
-  tc::grid_launch_next();
-  tc::grid_wait_previous();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int owner = blockIdx.x, rank = owner & (kCtas - 1), cluster = owner >> BITS;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, owner = blockIdx.x;
   const unsigned before_me = (1u << lane) - 1;
-
-  // the warp's share of the tokens
-  const std::int64_t per_warp =
-      (a.tokens + kCtas * kSortThreads - 1) / (kCtas * kSortThreads) * 32;
-  const std::int64_t t0 = (rank * kSortWarps + warp) * per_warp;
-  const std::int64_t t1 = min(t0 + per_warp, static_cast<std::int64_t>(a.tokens));
-  const bool keep = per_warp <= 32 * kScan;  // in registers between the two readings
-  int v[kScan];
-  const auto load = [&](std::int64_t t) {
-    std::int64_t w[kScan];
-#pragma unroll
-    for (int j = 0; j < kScan; ++j) {
-      const std::int64_t i = t + 32 * j + lane;
-      w[j] = load8(a.token + i, i < t1);
-    }
-#pragma unroll
-    for (int j = 0; j < kScan; ++j) {
-      v[j] = w[j] >= 0 && w[j] < a.vocab ? static_cast<int>(w[j]) : -1;
-    }
-  };
-  // Whether the lane's token v is the cluster's, as ballots; its bits as lanes_of wants them.
-  const auto ballots = [&](int w, unsigned (&bits)[BITS + 1]) {
-    const unsigned in =
-        __ballot_sync(0xffffffffu, w >= 0 && (w & (kOwners - 1)) >> BITS == cluster);
-    if (in != 0) {
-#pragma unroll
-      for (int i = 0; i < BITS; ++i) bits[i] = __ballot_sync(0xffffffffu, (w >> i & 1) != 0);
-    }
-    return in;
-  };
-  int below = 0, mine = 0;  // mine: lane c, of the cluster's owner c
-  for (std::int64_t t = t0; t < t1; t += 32 * kScan) {
-    load(t);
-#pragma unroll
-    for (int j = 0; j < kScan; ++j) {
-      below += v[j] >= 0 && (v[j] & (kOwners - 1)) >> BITS < cluster;
-      unsigned bits[BITS + 1];
-      const unsigned in = ballots(v[j], bits);
-      if (in != 0) mine += __popc(lanes_of<BITS>(in, bits, lane));
-    }
-  }
-  below = warp_sum(below);
-  if (lane < kCtas) found[lane][warp] = mine;
-  if (lane == 0) found[kCtas][warp] = below;
   count[0][warp][lane] = 0;
-
   int2* span = a.span + static_cast<std::int64_t>(owner) * a.per_owner;
   for (int i = threadIdx.x; i < a.per_owner; i += kSortThreads) span[i] = make_int2(0, 0);
   for (std::int64_t i = static_cast<std::int64_t>(owner) * kSortThreads + threadIdx.x;
        i < a.num_counters; i += kOwners * kSortThreads)
     a.counters[i] = 0;
 
-  if constexpr (BITS > 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-  __syncthreads();
-  if (warp <= kCtas) {  // the CTA's sums by owner: found becomes the warps before
-    const int x = found[warp][lane];
-    const int sum = warp_inclusive(x);
-    found[warp][lane] = sum - x;
-    const int all = __shfl_sync(0xffffffffu, sum, 31);
-    if (lane < kCtas) store_cluster<BITS>(&shares[rank][warp], lane, all);
-  }
-  sync_cluster<BITS>();
-  // lane c: the place of the cluster's owner c in the ordered list, its entries, and where
-  // this warp's tokens of it go
-  int base = 0, n = 0, at = 0;
-  if (lane < kCtas) {
-#pragma unroll
-    for (int q = 0; q < kCtas; ++q) {
-      base += shares[q][kCtas];
-      n += shares[q][lane];
-      if (q < rank) at += shares[q][lane];
-    }
-    at += found[lane][warp];
-  }
-  int before = n;  // entries of the cluster's owners up to this one
-#pragma unroll
-  for (int o = 1; o < kCtas; o <<= 1) {
-    const int u = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += u;
-  }
-  base += before - n;
-  for (std::int64_t t = t0; t < t1; t += 32 * kScan) {
-    if (!keep) load(t);
-#pragma unroll
-    for (int j = 0; j < kScan; ++j) {
-      unsigned bits[BITS + 1];
-      const unsigned in = ballots(v[j], bits);
-      if (in == 0) continue;
-      const int c = v[j] & (kCtas - 1);
-      const int to = __shfl_sync(0xffffffffu, at, c), size = __shfl_sync(0xffffffffu, n, c);
-      const int list = __shfl_sync(0xffffffffu, base, c);
-      if ((in >> lane & 1u) != 0) {
-        const int i = to + __popc(lanes_of<BITS>(in, bits, c) & before_me);
-        const Entry e{v[j] >> kOwnerBits, static_cast<int>(t + 32 * j + lane)};
-        if (size <= a.near_list)
-          store_cluster<BITS>(near + i, c, e);
-        else
-          a.list[0][list + i] = e;
-      }
-      at += __popc(lanes_of<BITS>(in, bits, lane));
-    }
-  }
-  n = __shfl_sync(0xffffffffu, n, rank);
-  base = __shfl_sync(0xffffffffu, base, rank);
-  if (owner == kOwners - 1 && threadIdx.x == 0) *a.total = base + n;
-  sync_cluster<BITS>();  // the list is there
-  Entry* from = n <= a.near_list ? near : a.list[0] + base;
+  int base;
+  Entry* from;
+  const int n = a.share > 0 ? collect(a, near, owner, &base, &from)
+                            : select(a, near, owner, &base, &from);
   Entry* to = n <= a.near_list ? near + a.near_list : a.list[1] + base;
+  if (owner == kOwners - 1 && threadIdx.x == 0) *a.total = base + n;
 
   if (n <= kCompared) {
     if (static_cast<int>(threadIdx.x) < n) {
@@ -533,8 +583,7 @@ __device__ __forceinline__ void sort_body(const SortArgs& a) {
     for (int pass = 0; pass < a.passes; ++pass) {
       const int shift = pass * kDigit;
       auto& counts = count[pass & 1];
-      // entry i's digit, and the lanes whose entries have the same (five votes: match.any
-      // took XX)
+      // entry i's digit, and the lanes whose entries have the same (five votes)
       const auto digit = [&](int i, unsigned* same) {
         const int d = i < i1 ? from[i].word >> shift & (kDigits - 1) : kDigits;
         unsigned bits[kDigit + 1];
@@ -583,15 +632,6 @@ __device__ __forceinline__ void sort_body(const SortArgs& a) {
     if (i == 0 || from[i - 1].word != e.word) span[e.word].x = base + i;
     if (i == n - 1 || from[i + 1].word != e.word) span[e.word].y = base + i + 1;
   }
-}
-
-__global__ void __launch_bounds__(kSortThreads, 2) embedding_sort_kernel(const SortArgs a) {
-  sort_body<0>(a);
-}
-
-__global__ void __cluster_dims__(kShare, 1, 1) __launch_bounds__(kSortThreads, 2)
-    embedding_sort_together_kernel(const SortArgs a) {
-  sort_body<kShareBits>(a);
 }
 
 // ----------------------------------------------------------------------- the sums --
@@ -935,9 +975,9 @@ int block_entries(int tokens, int features) {
 constexpr int kLeastSlice = 128;  // features of the narrowest slices
 
 struct SortPlan {
-  int per_owner, passes, block;
+  int per_owner, passes, block, share;
   std::int64_t num_counters;
-  std::size_t list[2], word, pos, span, total, partial, counters, bytes;
+  std::size_t list[2], parts, starts, word, pos, span, total, partial, counters, bytes;
 };
 
 SortPlan plan(const EmbeddingArgs& a) {
@@ -953,6 +993,9 @@ SortPlan plan(const EmbeddingArgs& a) {
   };
   const std::size_t T = a.tokens, H = a.features;
   for (std::size_t& l : p.list) l = take(a.tokens > kSharedList ? T * sizeof(Entry) : 0);
+  p.share = a.tokens > kParted ? (a.tokens + 32 * kParts - 1) / (32 * kParts) * 32 : 0;
+  p.parts = take(static_cast<std::size_t>(p.share) * kParts * sizeof(Entry));
+  p.starts = take(p.share > 0 ? (kOwners + 1) * kParts * 4 : 0);
   p.word = take(T * 4);
   p.pos = take(T * 4);
   p.span = take(static_cast<std::size_t>(p.per_owner) * kOwners * sizeof(int2));
@@ -1053,12 +1096,10 @@ static bool sort_attributes() noexcept {
   const int dev = current_device();
   if (dev < 0 || dev >= 64) return false;
   if ((set.load(std::memory_order_acquire) >> dev & 1ull) != 0) return true;
-  for (auto* kern : {embedding_sort_kernel, embedding_sort_together_kernel}) {
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             2 * kSharedList * sizeof(Entry)) != cudaSuccess) {
-      (void)cudaGetLastError();
-      return false;
-    }
+  if (cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           2 * kSharedList * sizeof(Entry)) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return false;
   }
   set.fetch_or(1ull << dev, std::memory_order_release);
   return true;
@@ -1086,6 +1127,9 @@ cudaError_t launch_embedding_gradient(const EmbeddingArgs& a, void* workspace,
   s.num_counters = p.num_counters;
   if (!sort_attributes()) return cudaErrorInvalidDevice;
   s.near_list = std::min(a.tokens, kSharedList);
+  s.share = p.share;
+  s.parts = reinterpret_cast<Entry*>(ws + p.parts);
+  s.starts = reinterpret_cast<int*>(ws + p.starts);
   const std::size_t shared = 2 * s.near_list * sizeof(Entry);
   // rows that are set to zero while the tokens are sorted
   int first_row = 0;
@@ -1094,18 +1138,21 @@ cudaError_t launch_embedding_gradient(const EmbeddingArgs& a, void* workspace,
   unsigned fill_ctas = 0;
   if (a.beta == 0.0f && aligned_to(a.w, 16) && a.vocab * row_bytes >= kFillLeast) {
     const std::int64_t bytes =
-        kFillAtOnce + a.tokens * (a.tokens < kTogether ? kFillPerToken : kFillTogether);
+        kFillAtOnce + a.tokens * (a.tokens <= kParted ? kFillPerToken : kFillParted);
     // multiples of 8 rows are whole 16-byte words
     first_row = static_cast<int>(std::min<std::int64_t>(a.vocab, bytes / row_bytes) / 8 * 8);
     s.fill = static_cast<uint4*>(a.w);
     s.num_fill = first_row * row_bytes / 16;
     fill_ctas = static_cast<unsigned>(std::min<std::int64_t>(
-        (2 * sms() - kOwners) / kShare, (s.num_fill + kShare * kSortThreads - 1) / (kShare * kSortThreads)));
-    fill_ctas *= kShare;
+        2 * sms() - kOwners, (s.num_fill + kSortThreads - 1) / kSortThreads));
   }
-  const cudaError_t e = tc::launch_overlapped(
-      a.tokens < kTogether ? embedding_sort_kernel : embedding_sort_together_kernel,
-      dim3(kOwners + fill_ctas), kSortThreads, shared, st, false, s);
+  if (p.share > 0) {
+    const cudaError_t e = tc::launch_overlapped(embedding_part_kernel, dim3(kParts), kSortThreads,
+                                                0, st, false, s);
+    if (e != cudaSuccess) return e;
+  }
+  const cudaError_t e = tc::launch_overlapped(embedding_sort_kernel, dim3(kOwners + fill_ctas),
+                                              kSortThreads, shared, st, p.share > 0, s);
   if (e != cudaSuccess) return e;
   const bool wide = rows_of_runs(a, a.rows == T::kF32 ? 4 : 8);
   if (a.rows == T::kF32)
