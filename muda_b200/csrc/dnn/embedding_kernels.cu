@@ -655,7 +655,11 @@ struct SumArgs {
 };
 
 constexpr int kSumThreads = 256, kSumWarps = kSumThreads / 32;
-constexpr int kSumCtas = 3;  // per SM
+// CTAs per SM.  Where there is work for all warps of the GPU, three with 8 rows in flight keep the
+// most bytes on their way (8192 x 4096 of 128000 words: 192 us, 197 with two and 16 rows); where a
+// warp has one block or none, two whose loads of 16 rows are one latency (4096 x 512 of 8000: 16
+// us, 20 with three).
+constexpr int kManyCtas = 3, kFewCtas = 2;
 
 __device__ __forceinline__ int2 span_of(const SumArgs& a, int word) {
   return a.span[static_cast<std::int64_t>(word & (kOwners - 1)) * a.per_owner +
@@ -934,13 +938,13 @@ __device__ __forceinline__ void fill_rows(const SumArgs& a, int first) {
 
 // A warp takes a block's slice, or rows to fill, at a time: the sums first, so that their
 // latency hides behind the filling, which takes all the bandwidth that is left.
-template <int UPDATE, typename T, typename TW, int VEC, int RUNS, int AHEAD>
-__global__ void __launch_bounds__(kSumThreads, kSumCtas) embedding_sum_kernel(const SumArgs a) {
+template <int UPDATE, typename T, typename TW, int VEC, int RUNS, int AHEAD, int CTAS>
+__global__ void __launch_bounds__(kSumThreads, CTAS) embedding_sum_kernel(const SumArgs a) {
   tc::grid_launch_next();
   tc::grid_wait_previous();
   using S = Slice<VEC, RUNS>;
   // as many rows as the registers hold, with dw's where they are loaded too
-  constexpr int kAhead = UPDATE != kScale ? AHEAD : sizeof(TW) > sizeof(T) ? 3 : AHEAD / 2;
+  constexpr int kAhead = UPDATE != kScale ? AHEAD : sizeof(TW) > sizeof(T) ? AHEAD * 3 / 8 : AHEAD / 2;
   const unsigned slices = (a.features + S::kFeatures - 1) / S::kFeatures;
   const int total = *a.total;
   const std::int64_t sums = static_cast<std::int64_t>((total + a.block - 1) / a.block) * slices;
@@ -960,14 +964,16 @@ __global__ void __launch_bounds__(kSumThreads, kSumCtas) embedding_sum_kernel(co
 }
 
 // ------------------------------------------------------------------------- planning --
-// Entries per block, 8 to 32: few, for the latency of a block's batches of loads, as long as
-// every warp that the GPU holds has one block's slice (256 features) and a frequent word (a
-// twelfth of the tokens) has no more partial sums than a block has entries.  More than 32 only
-// where one word could have more than 1024 partial sums.
+std::int64_t few_warps() { return std::int64_t{sms()} * kFewCtas * kSumWarps; }
+
+// Entries per block: 16, one batch of loads, as long as every warp that the GPU holds has one
+// block's slice (256 features) and a frequent word (a twelfth of the tokens) has no more partial
+// sums than a block has entries; else 32.  More only where one word could have more than 1024
+// partial sums.
 int block_entries(int tokens, int features) {
-  const std::int64_t slices = (features + 255) / 256, warps = std::int64_t{sms()} * kSumCtas * kSumWarps;
-  int n = 8;
-  while (n < 32 && (tokens / n * slices > warps || 25 * n * n < tokens)) n *= 2;
+  const std::int64_t slices = (features + 255) / 256;
+  int n = 16;
+  if (tokens / n * slices > few_warps() || 25 * n * n < tokens) n = 32;
   while (tokens / n > 1024 && n >= 32) n *= 2;
   return n;
 }
@@ -1059,16 +1065,22 @@ cudaError_t gradient(const EmbeddingArgs& a, const SortPlan& p, int first_row, c
   const std::int64_t units =
       blocks * slices +
       (a.beta == 1.0f ? 0 : (a.vocab - first_row + s.fill_rows - 1) / s.fill_rows);
-  const std::int64_t ctas =
-      std::min<std::int64_t>((units + kSumWarps - 1) / kSumWarps, sms() * kSumCtas);
   static_assert(kSlice >= kLeastSlice, "the counters are for fewer slices");
-  auto kern = a.beta != 0.0f ? embedding_sum_kernel<kScale, T, TW, VEC, RUNS, AHEAD>
-                             : embedding_sum_kernel<kWrite, T, TW, VEC, RUNS, AHEAD>;
-  if constexpr (std::is_same_v<TW, float>) {
-    if (a.beta == 1.0f) kern = embedding_sum_kernel<kAdd, T, TW, VEC, RUNS, AHEAD>;
-  }
-  return tc::launch_overlapped(kern, dim3(static_cast<unsigned>(ctas)), kSumThreads, 0, st, true,
-                               s);
+  const auto run = [&](auto ahead, auto ctas_per_sm) {
+    constexpr int kAhead = decltype(ahead)::value, kCtas = decltype(ctas_per_sm)::value;
+    auto kern = a.beta != 0.0f ? embedding_sum_kernel<kScale, T, TW, VEC, RUNS, kAhead, kCtas>
+                               : embedding_sum_kernel<kWrite, T, TW, VEC, RUNS, kAhead, kCtas>;
+    if constexpr (std::is_same_v<TW, float>) {
+      if (a.beta == 1.0f) kern = embedding_sum_kernel<kAdd, T, TW, VEC, RUNS, kAhead, kCtas>;
+    }
+    const std::int64_t ctas =
+        std::min<std::int64_t>((units + kSumWarps - 1) / kSumWarps, sms() * kCtas);
+    return tc::launch_overlapped(kern, dim3(static_cast<unsigned>(ctas)), kSumThreads, 0, st, true,
+                                 s);
+  };
+  if (blocks * slices <= few_warps())
+    return run(std::integral_constant<int, AHEAD>{}, std::integral_constant<int, kFewCtas>{});
+  return run(std::integral_constant<int, AHEAD / 2>{}, std::integral_constant<int, kManyCtas>{});
 }
 
 }  // namespace
@@ -1156,20 +1168,20 @@ cudaError_t launch_embedding_gradient(const EmbeddingArgs& a, void* workspace,
   if (e != cudaSuccess) return e;
   const bool wide = rows_of_runs(a, a.rows == T::kF32 ? 4 : 8);
   if (a.rows == T::kF32)
-    return wide ? gradient<float, float, 4, 1, 8>(a, p, first_row, ws, st)
-                : gradient<float, float, 1, 4, 4>(a, p, first_row, ws, st);
+    return wide ? gradient<float, float, 4, 1, 16>(a, p, first_row, ws, st)
+                : gradient<float, float, 1, 4, 8>(a, p, first_row, ws, st);
   if (a.rows == T::kF16) {
     if (a.table == T::kF32)
-      return wide ? gradient<__half, float, 8, 1, 8>(a, p, first_row, ws, st)
-                  : gradient<__half, float, 1, 4, 4>(a, p, first_row, ws, st);
-    return wide ? gradient<__half, __half, 8, 1, 8>(a, p, first_row, ws, st)
-                : gradient<__half, __half, 1, 4, 4>(a, p, first_row, ws, st);
+      return wide ? gradient<__half, float, 8, 1, 16>(a, p, first_row, ws, st)
+                  : gradient<__half, float, 1, 4, 8>(a, p, first_row, ws, st);
+    return wide ? gradient<__half, __half, 8, 1, 16>(a, p, first_row, ws, st)
+                : gradient<__half, __half, 1, 4, 8>(a, p, first_row, ws, st);
   }
   if (a.table == T::kF32)
-    return wide ? gradient<__nv_bfloat16, float, 8, 1, 8>(a, p, first_row, ws, st)
-                : gradient<__nv_bfloat16, float, 1, 4, 4>(a, p, first_row, ws, st);
-  return wide ? gradient<__nv_bfloat16, __nv_bfloat16, 8, 1, 8>(a, p, first_row, ws, st)
-              : gradient<__nv_bfloat16, __nv_bfloat16, 1, 4, 4>(a, p, first_row, ws, st);
+    return wide ? gradient<__nv_bfloat16, float, 8, 1, 16>(a, p, first_row, ws, st)
+                : gradient<__nv_bfloat16, float, 1, 4, 8>(a, p, first_row, ws, st);
+  return wide ? gradient<__nv_bfloat16, __nv_bfloat16, 8, 1, 16>(a, p, first_row, ws, st)
+              : gradient<__nv_bfloat16, __nv_bfloat16, 1, 4, 8>(a, p, first_row, ws, st);
 }
 
 }  // namespace mb200::dnn
