@@ -142,7 +142,7 @@ def test_gradient(cuda, built, T, H, V, rows, table):
 @pytest.mark.parametrize("rows,table", [("bf16", "bf16"), ("bf16", "fp32"), ("fp32", "fp32")])
 @pytest.mark.parametrize("T,tokens", [
     (20000, "one word"), (20000, "two words of one owner"), (70000, "frequent words"),
-    (70000, "one owner"), (4096, "runs"), (33000, "mostly padding"), (777, "all padding"),
+    (70000, "one owner"), (9000, "one owner"), (4096, "runs"), (33000, "mostly padding"), (777, "all padding"),
 ])
 def test_gradient_of_uneven_counts(cuda, built, T, tokens, rows, table, beta):
     """Words far more frequent than the others, and owners with most of the tokens."""
@@ -163,6 +163,64 @@ def test_gradient_of_uneven_counts(cuda, built, T, tokens, rows, table, beta):
         assert e.backward(d, 1.0, beta) == 0
         cuda.cuda.synchronize()
     e.check_backward(was, 1.0, beta)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,table", [("bf16", "bf16"), ("fp16", "fp32")])
+@pytest.mark.parametrize("T,H,V,shift", [(8192, 1031, 20000, 0), (8193, 1032, 20003, 0),
+                                         (300, 1032, 20003, 0), (9000, 1032, 20003, 1),
+                                         (1, 4096, 6001, 0)])
+def test_gradient_of_large_tables(cuda, built, T, H, V, shift, rows, table):
+    """Tables that are filled while the tokens are sorted, from either end of the counts."""
+    e = Table(cuda, T, H, V, rows, table, seed=T, out=0.1 if T > 1 else 0.0)
+    flat = cuda.full((V * H + shift + 8,), 5.0, device="cuda", dtype=e.w.dtype)
+    e.w = flat[shift:shift + V * H].view(V, H)
+    with Dnn(cuda) as d:
+        assert e.backward(d, 2.0) == 0
+        cuda.cuda.synchronize()
+        e.check_backward(None, 2.0)
+        assert (flat[:shift] == 5).all() and (flat[shift + V * H:] == 5).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [5, 3000])
+def test_few_tokens_of_very_many_words(cuda, built, T):
+    """Accumulation into a table of three million words, after other calls in its workspace."""
+    e = Table(cuda, T, 8, 3_000_000, "bf16", "fp32", seed=T)
+    with Dnn(cuda) as d:
+        ws = cuda.full((e.workspace_size(d),), 255, device="cuda", dtype=cuda.uint8)
+        for _ in range(2):
+            was = e.w.clone()
+            e.tokens = cuda.randint(0, 3_000_000, (T,), device="cuda", generator=e.g)
+            e.tokens[T // 2:] = e.tokens[0]
+            assert e.backward(d, 1.0, 1.0, ws) == 0
+            cuda.cuda.synchronize()
+            e.check_backward(was, 1.0, 1.0)
+
+
+@pytest.mark.gpu
+def test_two_handles_at_once(cuda, built):
+    """Calls of two handles on two streams: each gives the bits that it gives alone."""
+    tables = [Table(cuda, 12000, 264, 900, seed=1), Table(cuda, 5000, 520, 7000, seed=2)]
+    with Dnn(cuda) as a, Dnn(cuda) as b:
+        want = []
+        for e in tables:
+            assert e.backward(a) == 0
+            cuda.cuda.synchronize()
+            e.check_backward(None)
+            want.append(e.w.clone())
+        streams = [cuda.cuda.Stream(), cuda.cuda.Stream()]
+        for d, s in zip((a, b), streams):
+            assert d.L.cudnnSetStream(d.h, C.c_void_p(s.cuda_stream)) == 0
+        for _ in range(10):
+            for e in tables:
+                e.w.fill_(math.nan)
+            cuda.cuda.synchronize()
+            for _ in range(3):
+                for d, e in zip((a, b), tables):
+                    assert e.backward(d) == 0
+            cuda.cuda.synchronize()
+            assert all(cuda.equal(e.w, w) for e, w in zip(tables, want))
 
 
 @pytest.mark.gpu

@@ -656,6 +656,32 @@ def test_captured_in_a_graph(cuda, built, kind, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_pieces_captured_in_a_graph(cuda, built, dtype):
+    """A preference step of several pieces, in a given workspace that held other things."""
+    h = Preference(cuda, 1000, 72, 1500, 7, dtype, out=0.1, first=3)
+    stream = cuda.cuda.Stream()
+    with Dnn(cuda) as d:
+        size = int(h.workspace_size(d, 1) * 0.6)
+        ws = cuda.full((size,), 255, device="cuda", dtype=cuda.uint8)
+        cuda.cuda.synchronize()
+        assert d.L.cudnnSetStream(d.h, C.c_void_p(stream.cuda_stream)) == 0
+        with cuda.cuda.stream(stream):
+            assert h.backward(d, ws) == 0
+            stream.synchronize()
+            graph = cuda.cuda.CUDAGraph()
+            with cuda.cuda.graph(graph, stream=stream):
+                assert h.backward(d, ws) == 0
+            for _ in range(3):
+                h.clear()
+                ws.fill_(255)
+                graph.replay()
+            stream.synchronize()
+        del graph
+    h.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 def test_tied_table_step(cuda, built, dtype):
     """Lookup, policy loss on the same table as head, and both gradients into one dw."""
     from tests.test_embedding import Table
