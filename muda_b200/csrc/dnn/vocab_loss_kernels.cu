@@ -193,12 +193,12 @@ constexpr int kUnit = 128;
 // tokens that would cost up to 37 % (score of 128 x 768 x 50257).
 constexpr int kLogitsChunk = 8, kFewLogitsChunk = 2;
 
-// What a truncating MMA takes from a logit, as a share of it and on average (measured: 4.9e-7 of
-// the logits of 32 MMAs that an lse is made of, 1.2e-7 of 4; 3.7e-7 of large ones of 32).  It is
-// no error of a single cross entropy, but the losses of sequences add it up: their logits, and
-// the exponents' scale, are larger by it (rewards of 250-token
-// sequences 1.7e-6 off, 6e-7 with it; nll on average 4.5e-7 low, 4e-8 and less from H = 512 on).
-constexpr double kTruncated = 1.3e-8;
+// What a truncating MMA takes from a logit, as a share of it and on average (measured as lse's
+// mean error: 4.6e-7 of the logits of 32 MMAs and 0.9e-7 of 4 in bf16, 5.9e-7 and 1.3e-7 in
+// fp16).  It is no error of a single cross entropy, but the losses of sequences add it up: their
+// logits' scale is larger by it.  With that and exact_target_nll rewards of 250-token sequences
+// are 6e-7 off instead of 1.2e-5, and nll is 2e-7 off on average instead of 1.4e-6.
+constexpr double kTruncatedBf16 = 1.45e-8, kTruncatedFp16 = 1.95e-8;
 
 // A thread's logits of one token, and what says whether a target word is among them: the
 // token's label, or its entry of the hit map.  Loaded before the
@@ -1139,9 +1139,7 @@ enum FinishForm { kTargetLoss = 0, kNll = 1, kPolicy = 2 };
 
 // x[row] w[label] in fp32, to about half its last place: H / 256 rounded terms per thread, the
 // threads' sums in 64 bits (the whole CTA calls the second).  The tensor cores' sums are short of
-// that by up to 4e-7 of the logit, always toward zero, and a log ratio of two sequences adds
-// the like of it up over their tokens: rewards of 256-token sequences were 1.2e-5 off, their
-// plain fp32 form 6e-7.
+// that by up to 6e-7 of the logit and more for targets, which are their rows' largest.
 template <typename T>
 __device__ __forceinline__ float target_logit_part(const T* x, const T* w, int features) {
   float part = 0.0f;
@@ -1180,6 +1178,23 @@ __device__ __forceinline__ float target_logit(float part, double* red) {
 #pragma unroll
   for (int i = 0; i < kFinishThreads / 32; ++i) sum += red[i];
   return static_cast<float>(sum);
+}
+
+// The cross entropy of a target whose logit is z, and `was` among the logits that `sum` is of
+// (relative to their maximum mx).  The sums' truncation took from mx what it took from `was`, in
+// proportion: a part that all words of a row have in common (an offset of their logits) has to
+// leave the difference, or a token would be off by 4e-7 of it.  Targets near zero do not tell,
+// so the average counts for an eighth of mx.
+__device__ __forceinline__ float exact_target_nll(float z, float was, float mx, float sum,
+                                                  float log2e_tau, float inv_tau,
+                                                  float truncated) {
+  const float q = was / mx;
+  float r = ((z - was) / mx * q + truncated * 0x1p-6f) / (q * q + 0x1p-6f);
+  if (!(fabsf(r) < 8.0f * truncated)) r = truncated;
+  const float below = ((z - mx) - mx * r) * inv_tau;  // of the maximum's place
+  // the target's own share of the sum moves too
+  const float moved = sum + (expf(below) - exp2f((was - mx) * log2e_tau));
+  return logf(moved) - below;
 }
 
 template <typename T, int STORE, int FORM>
@@ -1264,11 +1279,8 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
       __shared__ double dots[kFinishThreads / 32];
       const float was = a.targets.z[r0];
       const float z = target_logit(dot, dots);
-      if (fabsf(z - was) < INFINITY) {  // the target's own share of the sum moves too
-        const float moved =
-            sum + exp2f(above(r0)) * expm1f(((z - was) - was * a.truncated) * a.inv_tau);
-        nll = logf(moved) - ((z - mx) - mx * a.truncated) * a.inv_tau;
-      }
+      if (fabsf(z - was) < INFINITY && fabsf(mx) < 0x1p20f)
+        nll = exact_target_nll(z, was, mx, sum, a.log2e_tau, a.inv_tau, a.truncated);
     }
   }
   if (part == 0) {
@@ -2168,7 +2180,8 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, const TokenRows& all, cha
     float z_scale = kLog2e * a.inv_tau;
     if (form != kTargetLoss) {
       const int chunk = 4 * (rows <= kStreamTokens ? kFewLogitsChunk : kLogitsChunk);
-      f.truncated = static_cast<float>(kTruncated * std::min(chunk, (a.features + 15) / 16));
+      f.truncated = static_cast<float>((a.bf16 ? kTruncatedBf16 : kTruncatedFp16) *
+                                       std::min(chunk, (a.features + 15) / 16));
       z_scale = static_cast<float>(1.4426950408889634 * a.inv_tau * (1.0 + f.truncated));
     }
     f.x = x;
