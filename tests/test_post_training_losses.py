@@ -708,6 +708,76 @@ def test_tied_table_step(cuda, built, dtype):
         e.check_backward(head, 8.0, 1.0)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["policy", "preference"])
+def test_example_gradients(cuda, built, kind):
+    """The example's steps against autograd in 64 bits.  Its hidden states round to bf16 once and
+    count as inputs.  dz rounds three times at most, dx and dw once each and dw's sum once
+    more: six roundings of the products' magnitudes, and the nll's errors (a share of 2^-10)."""
+    from examples.post_train_table import TiedTable
+
+    T, H, V, scale = 96, 64, 300, 8.0
+    g = cuda.Generator(device="cuda").manual_seed(3)
+    w = (cuda.randn(V, H, device="cuda", generator=g) / 8).bfloat16()
+    tokens = cuda.randint(0, V, (T,), device="cuda", generator=g)
+    tokens[5] = -1
+    labels = cuda.randint(0, V, (T,), device="cuda", generator=g)
+    labels[::6] = -100
+    live = labels >= 0
+    table = TiedTable(V, H, scale)
+    try:
+        x = table.hidden(w, tokens)
+        nll = table.nll(w, tokens, labels)
+        noise = cuda.randn(T, device="cuda", generator=g)
+        ref = nll + noise
+        if kind == "policy":
+            old, A = nll + 0.1 * noise.sign(), cuda.randn(T, device="cuda", generator=g)
+            dloss = cuda.rand(T, device="cuda", generator=g) / T
+            loss, _, dw = table.policy_step(w, tokens, labels, old, ref, A, dloss, kl=0.1)
+        else:
+            offsets = cuda.tensor([0, 20, 50, 70, T], device="cuda")
+            dloss = cuda.rand(2, device="cuda", generator=g)
+            loss, _, dw = table.preference_step(w, tokens, labels, offsets, ref, dloss)
+        cuda.cuda.synchronize()
+    finally:
+        table.close()
+    z = x.double() @ w.double().t()
+    logp = cuda.log_softmax(z, dim=1)
+    n = -logp.gather(1, labels.clamp(min=0)[:, None])[:, 0]
+    n = cuda.where(live, n, 0.0).requires_grad_()
+    if kind == "policy":
+        r, d = cuda.exp(old.double() - n), n - ref.double()
+        gain = cuda.minimum(r * A.double(), r.clamp(0.8, 1.2) * A.double())
+        want = cuda.where(live, 0.1 * (cuda.expm1(d) - d) - gain, 0.0)
+    else:
+        gain = cuda.where(live, ref.double() - n, 0.0)
+        L = cuda.stack([gain[a:b].sum() for a, b in ((0, 20), (20, 50), (50, 70), (70, T))])
+        want = cuda.nn.functional.softplus(-0.1 * (L[:2] - L[2:]))
+    assert ((loss - want).abs() <= 2.0 ** -12 * (1 + want.abs())).all()
+    dn = cuda.autograd.grad((want * dloss.double()).sum(), n)[0]
+    dz = cuda.exp(logp)
+    dz[cuda.arange(T, device="cuda"), labels.clamp(min=0)] -= 1
+    dz = cuda.where(live, dn, 0.0)[:, None] * dz
+
+    def table_gradient(dz, x, w):
+        at = (tokens >= 0).nonzero()[:, 0]
+        return (dz.t() @ x).index_add(0, tokens[at], scale * (dz @ w)[at])
+
+    want = table_gradient(dz, x.double(), w.double())
+    mass = table_gradient(dz.abs(), x.double().abs(), w.double().abs())
+    assert ((dw - want).abs() <= (6.2 * 2.0 ** -8 + 2.0 ** -10) * mass + 2.0 ** -133).all()
+
+
+@pytest.mark.gpu
+def test_example_runs(cuda, built):
+    from examples.post_train_table import train
+
+    policy, preference = train(steps=3, sequences=6, length=16, features=64, vocab=300,
+                               log=lambda *a: None)
+    assert len(policy) == len(preference) == 3
+    assert all(math.isfinite(v) for v in policy + preference)
+
+
 # ------------------------------------------------------------------------ refusals --
 def test_refusals_before_the_device(built):
     bad, unsupported = capi.CUDNN_STATUS_BAD_PARAM, capi.CUDNN_STATUS_NOT_SUPPORTED
