@@ -1725,16 +1725,15 @@ int sms() {
   return n > 0 ? n : 148;
 }
 
-// Width of the tiles of `cols` columns in `rows` tile rows on `groups` CTAs or pairs: the
-// multiple of `step` whose waves end soonest.  A k-block of a 256 x n pair tile takes about
-// 256 + n clocks (below 256 columns shared memory, not the MMAs, sets the pace), of a single
-// CTA's tile n times what one word's line takes to arrive.
-int tile_width(std::int64_t rows, int cols, int groups, int step, bool pair) {
+// Width of the tiles of `cols` columns in `rows` tile rows on `pairs` CTA pairs: the multiple of
+// `step` whose waves end soonest.  A k-block of a 256 x n pair tile takes about 256 + n clocks
+// (below 256 columns shared memory, not the MMAs, sets the pace).
+int pair_tile_width(std::int64_t rows, int cols, int pairs, int step) {
   int best = tc::kEpiN;
   std::int64_t least = INT64_MAX;
   for (int n = tc::kEpiN; n >= step; n -= step) {
     const std::int64_t tiles = rows * ((cols + n - 1) / n);
-    const std::int64_t cost = (tiles + groups - 1) / groups * (pair ? 256 + n : n);
+    const std::int64_t cost = (tiles + pairs - 1) / pairs * (256 + n);
     if (cost < least) {
       least = cost;
       best = n;
@@ -1743,11 +1742,23 @@ int tile_width(std::int64_t rows, int cols, int groups, int step, bool pair) {
   return best;
 }
 
+// The same for tiles of one row on single CTAs.  With every CTA at work a k-block takes about 1450
+// clocks whatever its width (all read the same lines of x at a time; 15 x 1400 x 88432 in tiles
+// of 32 words 341 us, 96: 123, 160: 88, 256: 70), so it is the waves that count; within one wave
+// narrow tiles spread the words over more CTAs (20 x 8192 x 8000: 64 words 51 us, 256: 60).
+int single_tile_width(int cols, int ctas, int step) {
+  const auto waves = [&](int n) { return ((cols + n - 1) / n + ctas - 1) / ctas; };
+  int n = tc::kEpiN;
+  if (waves(n) == 1)
+    while (n > step && waves(n - step) == 1) n -= step;
+  return n;
+}
+
 // Words per tile of the logits; stored numerators need units (half tiles) of 64 or 128.
 int logits_tile_n(int rows, int vocab, bool store) {
-  const bool pair = rows > tc::kBM;
-  return tile_width(pair ? (rows + 255) / 256 : 1, vocab, pair ? sms() / 2 : sms(),
-                    store ? 128 : 32, pair);
+  const int step = store ? 128 : 32;
+  if (rows > tc::kBM) return pair_tile_width((rows + 255) / 256, vocab, sms() / 2, step);
+  return single_tile_width(vocab, sms(), step);
 }
 
 // Columns per tile: as few tiles as 256 columns need, of even width.
@@ -2030,8 +2041,8 @@ cudaError_t run_dw(const VocabLossArgs& a, const Plan& p, const void* num, const
   Dw<T, TALL> g{};
   g.tma = tma_rows_ok(a.dw, a.features);
   constexpr int kRows = Dw<T, TALL>::kRows;
-  g.tile_n = tile_width((a.vocab + kRows - 1) / kRows, a.features, sms() / 2, g.tma ? 128 : 32,
-                        true);
+  g.tile_n = pair_tile_width((a.vocab + kRows - 1) / kRows, a.features, sms() / 2,
+                             g.tma ? 128 : 32);
   const int dz_rows = p.copies * rows;
   if (!make_map(&g.ma, FMT, num, a.vocab, dz_rows, p.ldn, 64, 64) ||
       !make_map(&g.mb, FMT, xt, dz_rows, a.features, p.ldt, tc::kBK, g.tile_n / 2) ||
