@@ -1742,10 +1742,11 @@ int pair_tile_width(std::int64_t rows, int cols, int pairs, int step) {
   return best;
 }
 
-// The same for tiles of one row on single CTAs.  With every CTA at work a k-block takes about 1450
-// clocks whatever its width (all read the same lines of x at a time; 15 x 1400 x 88432 in tiles
-// of 32 words 341 us, 96: 123, 160: 88, 256: 70), so it is the waves that count; within one wave
-// narrow tiles spread the words over more CTAs (20 x 8192 x 8000: 64 words 51 us, 256: 60).
+// The same for tiles of one row on single CTAs.  The ring has as many stages whatever their
+// width, so a k-block takes about 1450 clocks, of latency, up to the width at which memory is
+// busy (15 x 1400 x 88432 in tiles of 32 words 341 us, 96: 123, 160: 88, 256: 70): it is the
+// waves that count.  Within one wave narrow tiles spread the words over more CTAs (20 x 8192 x
+// 8000: 64 words 51 us, 256: 60).
 int single_tile_width(int cols, int ctas, int step) {
   const auto waves = [&](int n) { return ((cols + n - 1) / n + ctas - 1) / ctas; };
   int n = tc::kEpiN;
