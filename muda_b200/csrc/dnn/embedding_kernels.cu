@@ -377,13 +377,15 @@ __global__ void __launch_bounds__(kSortThreads) embedding_part_kernel(const Sort
   const int per_warp = (a.share + kSortThreads - 1) / kSortThreads * 32;
   const std::int64_t first = static_cast<std::int64_t>(q) * a.share;
   const std::int64_t t0 = first + warp * per_warp;
-  const std::int64_t t1 = min(min(t0 + per_warp, first + a.share), static_cast<std::int64_t>(a.tokens));
+  const std::int64_t t1 =
+      min(min(t0 + per_warp, first + a.share), static_cast<std::int64_t>(a.tokens));
   // the lane's token of the 32 from t on, and the lanes whose tokens have the same owner
   const auto owners = [&](std::int64_t t, int* word) {
     *word = word_of(a, load8(a.token + t + lane, t + lane < t1));
     unsigned bits[kOwnerBits + 1];
 #pragma unroll
-    for (int k = 0; k < kOwnerBits; ++k) bits[k] = __ballot_sync(0xffffffffu, (*word >> k & 1) != 0);
+    for (int k = 0; k < kOwnerBits; ++k)
+      bits[k] = __ballot_sync(0xffffffffu, (*word >> k & 1) != 0);
     return lanes_of<kOwnerBits>(__ballot_sync(0xffffffffu, *word >= 0), bits, *word);
   };
   for (std::int64_t t = t0; t < t1; t += 32) {
@@ -547,9 +549,9 @@ __global__ void __launch_bounds__(kSortThreads, 2) embedding_sort_kernel(const S
   tc::grid_wait_previous();
   if (blockIdx.x >= kOwners) {
     const std::int64_t step = static_cast<std::int64_t>(gridDim.x - kOwners) * kSortThreads;
+    const std::int64_t first = static_cast<std::int64_t>(blockIdx.x - kOwners) * kSortThreads;
 #pragma unroll 4
-    for (std::int64_t i = static_cast<std::int64_t>(blockIdx.x - kOwners) * kSortThreads + threadIdx.x;
-         i < a.num_fill; i += step)
+    for (std::int64_t i = first + threadIdx.x; i < a.num_fill; i += step)
       __stcs(a.fill + i, make_uint4(0, 0, 0, 0));
     return;
   }
@@ -662,7 +664,7 @@ struct SumArgs {
 constexpr int kSumThreads = 256, kSumWarps = kSumThreads / 32;
 // CTAs per SM.  Where there is work for all warps of the GPU, three with 8 rows in flight keep the
 // most bytes on their way (8192 x 4096 of 128000 words: 192 us, 197 with two and 16 rows); where a
-// warp has one block or none, two whose loads of 16 rows are one latency (4096 x 512 of 8000: 16
+// warp has one block or none, two whose loads of 16 rows are one latency (4096 x 512 of 8000: 17
 // us, 20 with three).
 constexpr int kManyCtas = 3, kFewCtas = 2;
 
@@ -775,13 +777,15 @@ __device__ __forceinline__ bool last_of(int* counter, int n) {
     asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(was) : "l"(counter)
                  : "memory");
   was = __shfl_sync(0xffffffffu, was, 0);
+  __syncwarp();  // and what lane 0 acquired before the other lanes' reads
   return was == n - 1;
 }
 
 // Called by each warp that has left a partial sum of this word's slice, of block b.  The last
 // one adds them up; where they are many, first the last of each kJoin neighbouring blocks those.
 template <int UPDATE, typename TW, int VEC, int RUNS>
-__device__ __forceinline__ void join(const SumArgs& a, int word, int b, int slice, int slices, int h) {
+__device__ __forceinline__ void join(const SumArgs& a, int word, int b, int slice, int slices,
+                                     int h) {
   const int2 span = span_of(a, word);
   const int b0 = span.x / a.block, b1 = (span.y - 1) / a.block;
   const auto counter = [&](int block, int which) {
@@ -904,7 +908,8 @@ __device__ __forceinline__ void sum_block(const SumArgs& a, int b, int slice, in
 }
 
 // Rows of words that do not occur: zeros, or beta dw.  A warp takes rows of some KB at a time:
-// more, and the last warps are alone with theirs (8 rows of 8 KB: 206 us for all, 203).
+// more, and the last warps are alone with theirs (8192 x 4096 of 128000 words by 8 rows 206 us,
+// by one 203).
 constexpr int kFillBytes = 8192, kMostFillRows = 8;
 
 template <int UPDATE, typename TW, int VEC>
@@ -929,8 +934,8 @@ __device__ __forceinline__ void fill_rows(const SumArgs& a, int first) {
     }
     // elements up to the first 16-byte word, whole words, and the elements behind the last
     constexpr int kWord = 16 / sizeof(TW);
-    const int lead = min(a.features, static_cast<int>((16 - (reinterpret_cast<std::uintptr_t>(o) & 15)) & 15) /
-                                         static_cast<int>(sizeof(TW)));
+    const auto past = static_cast<int>(reinterpret_cast<std::uintptr_t>(o) & 15);
+    const int lead = min(a.features, (16 - past) % 16 / static_cast<int>(sizeof(TW)));
     const int whole = (a.features - lead) / kWord;
     if (lane < lead) o[lane] = from_float<TW>(0.0f);
 #pragma unroll 4
@@ -949,7 +954,9 @@ __global__ void __launch_bounds__(kSumThreads, CTAS) embedding_sum_kernel(const 
   tc::grid_wait_previous();
   using S = Slice<VEC, RUNS>;
   // as many rows as the registers hold, with dw's where they are loaded too
-  constexpr int kAhead = UPDATE != kScale ? AHEAD : sizeof(TW) > sizeof(T) ? AHEAD * 3 / 8 : AHEAD / 2;
+  constexpr int kAhead = UPDATE != kScale           ? AHEAD
+                         : sizeof(TW) > sizeof(T) ? AHEAD * 3 / 8
+                                                  : AHEAD / 2;
   const unsigned slices = (a.features + S::kFeatures - 1) / S::kFeatures;
   const int total = *a.total;
   const std::int64_t sums = static_cast<std::int64_t>((total + a.block - 1) / a.block) * slices;

@@ -801,9 +801,9 @@ __device__ __forceinline__ PolicyTerms policy_terms(const PolicyLoss& p, int row
 // The scale of a preference's gradients on their way into dw (more than 64 tokens).  All tokens
 // of a sequence have the same |dnll|, and unlikely targets, whose dz is nearly that, round alike:
 // what a few sequences' rounding leaves does not average out in dw (up to 2.5 times one rounding
-// for a single pair).  Of 64 scales within a factor of two this takes the one that leaves the
-// targets' dz the least, as the vocab_grad_scale_kernel's otherwise: the largest |dnll / tau| comes to
-// (2^12, 2^14].  dw's error over one rounding is 1.2 to 1.35 with it.
+// for a single pair).  Of 32 scales within a factor of two this takes the one that leaves the
+// targets' dz the least, as the vocab_grad_scale_kernel's otherwise: the largest |dnll / tau|
+// comes to (2^12, 2^14].  dw's error over one rounding is 1.2 to 1.35 with it.
 constexpr int kScales = 32, kScaleSamples = 512, kScaleThreads = 512;
 
 // The whole CTA of kScaleThreads calls this.
@@ -834,7 +834,8 @@ __device__ __forceinline__ void find_pair_scale(const float* dnll, const float* 
   if (mx > 0.0f) frexpf(mx, &e);  // mx in [2^(e-1), 2^e)
   e = max(-100, min(100, e));
   for (int c = warp; c < kScales; c += kWarps) {
-    const float s = ldexpf(exp2f(c * (-1.0f / kScales)), 14 - e), undo = exp2f(c * (1.0f / kScales));
+    const float s = ldexpf(exp2f(c * (-1.0f / kScales)), 14 - e);
+    const float undo = exp2f(c * (1.0f / kScales));
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < kScaleSamples; i += 32) {
@@ -2317,7 +2318,8 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, const TokenRows& all, cha
     } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
       MB200_TRY(logits(std::integral_constant<int, kCommon>{}));
       MB200_TRY(before_gradients());
-      MB200_TRY(launch(finish_form(std::integral_constant<int, kCommon>{}), finish, kFinishThreads, f));
+      MB200_TRY(launch(finish_form(std::integral_constant<int, kCommon>{}), finish, kFinishThreads,
+                       f));
     }
 
     if (a.dx != nullptr) {
