@@ -956,7 +956,8 @@ __global__ void __launch_bounds__(kPreferenceThreads)
   if (a.p.mode == PreferenceMode::kSigmoid) {
     // of h's own size the loss keeps 64 bits; what softplus adds to it is a float
     const float e = expf(static_cast<float>(-fabs(h)));
-    loss = (h < 0.0 ? -h : 0.0) + a.p.smoothing * h + log1pf(e);
+    loss = (h < 0.0 ? -h : 0.0) + log1pf(e);
+    if (a.p.smoothing != 0.0) loss += a.p.smoothing * h;  // h may be infinite
     slope = a.p.smoothing - (h < 0.0 ? 1.0f : e) / (1.0f + e);
   } else if (a.p.mode == PreferenceMode::kHinge) {
     loss = h < 1.0 ? 1.0 - h : h >= 1.0 ? 0.0 : h;

@@ -456,6 +456,21 @@ def test_infinite_ratios(cuda, built, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_infinite_references(cuda, built, dtype):
+    """A reference that did not know a chosen token, and one that did not know a rejected one."""
+    h = Preference(cuda, 100, 64, 300, 3, dtype, lengths=[10] * 6, seed=8)
+    h.ref[3] = math.inf    # pair 0's chosen sequence
+    h.ref[45] = math.inf   # pair 1's rejected one
+    with Dnn(cuda) as d:
+        assert h.backward(d) == 0
+        cuda.cuda.synchronize()
+    assert h.loss[0] == 0 and (h.dx[:10] == 0).all() and (h.dx[30:40] == 0).all()
+    assert h.loss[1] == math.inf and h.dx.isfinite().all() and h.dw.isfinite().all()
+    assert h.rewards[0] == math.inf and h.rewards[4] == math.inf and h.loss[2].isfinite()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("kind", ["policy", "preference"])
 @pytest.mark.parametrize("T,H", [(1000, 72), (385, 65)])
 def test_pieces(cuda, built, T, H, kind, dtype):
