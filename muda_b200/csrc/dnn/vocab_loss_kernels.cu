@@ -756,7 +756,7 @@ struct PolicyTerms {
 // exp(d) - 1 - d.  The difference loses |d| / 2 of its digits near 0; the series' first term
 // left out there is 2 d^8 / 10! of it, under 2^-28.
 __device__ __forceinline__ float exp_above_tangent(float d) {
-  if (!(fabsf(d) < 0.5f)) return expm1f(d) - d;
+  if (!(fabsf(d) < 0.5f)) return d == INFINITY ? d : expm1f(d) - d;
   float s = 1.0f;
 #pragma unroll
   for (int k = 9; k >= 3; --k) s = fmaf(s * d, 1.0f / k, 1.0f);

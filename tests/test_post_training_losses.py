@@ -452,6 +452,15 @@ def test_infinite_ratios(cuda, built, dtype):
         assert h.backward(d) == 0
         cuda.cuda.synchronize()
     assert abs(h.loss[2] - 3.0) < 1e-6 and (h.dx[2] == 0).all() and h.dw.isfinite().all()
+    # references that were sure of the token, or did not know it
+    h.ref[5], h.ref[6] = -math.inf, math.inf
+    h.coef = 0.5
+    with Dnn(cuda) as d:
+        assert h.backward(d, dw=False) == 0
+        cuda.cuda.synchronize()
+    assert (h.kl[5:7] == math.inf).all() and (h.loss[5:7] == math.inf).all()
+    rest = cuda.arange(200, device="cuda") != 5
+    assert h.dx[rest].isfinite().all()  # exp(-inf) - 1 is an ordinary slope
 
 
 @pytest.mark.gpu
