@@ -360,9 +360,9 @@ cudnnStatus_t cudnnLinearDistillationBackward(cudnnHandle_t handle, cudnnTensorD
  * Every output may be null (Forward: not all of them).  Backward computes the outputs too, and
  * the gradients of sum dloss * loss: dloss holds T floats for a policy loss, `pairs` for a
  * preference loss.  Logits are computed once, but for preference gradients of more tokens than
- * one piece has (see the workspace above): a pair's loss takes all its tokens, so each piece's
- * logits are computed again after them.  Preference losses keep up to 8 bytes of workspace per
- * token besides. */
+ * one piece has: a pair's loss takes all its tokens, so each piece's logits are computed again
+ * after them.  To that end a piece of a preference's holds up to 4 GiB of numerators (not 2, see
+ * the workspace above); 8 bytes per token come besides. */
 typedef enum {
   CUDNN_PREFERENCE_SIGMOID = 0,
   CUDNN_PREFERENCE_HINGE = 1,

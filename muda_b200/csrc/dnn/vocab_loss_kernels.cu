@@ -1710,6 +1710,9 @@ struct Dw {
 // Bytes of a piece's numerators.  Every further piece reads and writes dw's fp32 sum: 16384 x
 // 1024 x 131072 took 11.9 ms in one piece of 4 GiB or two of 2 GiB, 12.7 in four of 1 GiB.
 constexpr std::size_t kNumeratorCap = std::size_t{2} << 30;
+// Of a preference's, which computes all logits twice where it takes more than one (12288 x 4096 x
+// 131072: 42 ms in two pieces, 34 in one).
+constexpr std::size_t kPairNumeratorCap = std::size_t{4} << 30;
 // Bytes of everything else that grows with a piece's tokens, and its tokens.  The tokens also
 // bound dw's sums: within a piece the tensor cores truncate, pieces add in fp32.
 constexpr std::size_t kGradientCap = std::size_t{960} << 20, kScoreCap = std::size_t{224} << 20;
@@ -1785,8 +1788,9 @@ int dx_chain(bool bf16) { return bf16 ? 262144 : 32768; }
 // Splits of the words in dx's product: the count that ends soonest.  A k-block takes 512
 // clocks of MMAs per 256 x 256 on a pair; a single CTA's streams w at its share of memory
 // bandwidth (measured 5.5 TB/s).  Each split's partial sums are written and read once, by one
-// more launch.  No split is longer than dx_chain.
-int dx_splits(int rows, int features, int vocab, bool bf16) {
+// more launch.  No split is longer than dx_chain.  `most`: a bound for their number, where chains
+// allow it.
+int dx_splits(int rows, int features, int vocab, bool bf16, std::int64_t most) {
   const bool pair = rows > tc::kBM;
   const int bm = dx_tall(vocab) ? 512 : 256;
   const std::int64_t tiles =
@@ -1799,7 +1803,7 @@ int dx_splits(int rows, int features, int vocab, bool bf16) {
   const int least = (vocab + dx_chain(bf16) - 1) / dx_chain(bf16);
   double best = 0.0;
   int pick = least;
-  for (int ks = least; ks == least || (ks <= 32 && ks * 8 <= kb); ++ks) {
+  for (int ks = least; ks == least || (ks <= most && ks * 8 <= kb); ++ks) {
     const double waves = static_cast<double>((tiles * ks + n - 1) / n);
     const double loop = waves * ((kb + ks - 1) / ks) * block;
     const double join = ks == 1 ? 0.0 : 6e-6 + 8.0 * ks * rows * features / 4.5e12;
@@ -1881,7 +1885,12 @@ Plan plan_rows(const VocabLossArgs& a, int rows, bool sliced) {
     const auto words = static_cast<int>(kSliceBytes / (p.ldp * 2)) / whole * whole;
     p.slice = std::min(a.vocab, std::max(whole, words));
   }
-  p.ksplit = dx ? dx_splits(rows, a.features, p.slice, a.bf16) : 1;
+  // a preference's partial sums of dx take at most half of what a piece may, or they would cost it
+  // its one piece
+  std::int64_t splits = 32;
+  if (a.head == HeadLoss::kPreference)
+    splits = std::min<std::int64_t>(splits, kGradientCap / 2 / (R * H * 4));
+  p.ksplit = dx ? dx_splits(rows, a.features, p.slice, a.bf16, splits) : 1;
   p.stats = take(R * p.units * sizeof(float2));
   p.z = take(R * std::max<std::size_t>(K, 1) * 4);
   p.index = take(R * K * 4);
@@ -1918,8 +1927,10 @@ Plan plan_within(const VocabLossArgs& a, std::size_t limit, bool sliced, bool* o
                               (a.gradients ? 2ull * a.features : 0);
   std::int64_t most = a.gradients ? kGradientRows : kScoreRows;
   most = std::min(most, static_cast<std::int64_t>(cap / per_row));
+  const std::size_t numerators =
+      a.head == HeadLoss::kPreference ? kPairNumeratorCap : kNumeratorCap;
   if (a.gradients)
-    most = std::min(most, static_cast<std::int64_t>(kNumeratorCap / (round_up(a.vocab, kLine) * 2)));
+    most = std::min(most, static_cast<std::int64_t>(numerators / (round_up(a.vocab, kLine) * 2)));
   most = std::max<std::int64_t>(kLeastRows, most / kLeastRows * kLeastRows);
   int pieces = static_cast<int>((a.tokens + most - 1) / most);
   Plan p{};
