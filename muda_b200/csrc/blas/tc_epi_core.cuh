@@ -26,6 +26,7 @@
 //   static constexpr bool kPair, kTall;   // kTall implies kPair and kChunk 0
 //   static constexpr bool kAMn;       // A MN-major (64 x 64 boxes), else K-major; B is K-major
 //   static constexpr int kChunk;      // k-blocks per accumulator, 0: the whole tile
+//   static constexpr int kMaxN;       // most of tile_n, 256 or less: less leaves room for stages
 //   static constexpr int kStageBytes; // shared memory of an epilogue warp, a multiple of 1024
 //   long long tiles_total;  int num_kb;  int tile_n;
 //   const CUtensorMap* map_a() / map_b();           // K-major boxes: 64 x 128 rows of A,
@@ -60,7 +61,7 @@ struct EpiShape {
   static constexpr int kHalves = P::kTall ? 2 : 1;
   static constexpr int A_HALF = kBM * kRowBytes;
   static constexpr int A_STAGE = kHalves * A_HALF;           // this CTA's rows of A
-  static constexpr int B_STAGE = kEpiN / kCtas * kRowBytes;  // and of B
+  static constexpr int B_STAGE = P::kMaxN / kCtas * kRowBytes;  // and of B
   static constexpr int STAGE = A_STAGE + B_STAGE;
   static constexpr int EPI = kEpiWarps * P::kStageBytes;
   static constexpr int BAR_BYTES = 256;

@@ -400,11 +400,11 @@ __device__ __forceinline__ void finish_unit(const LogitsProblem& p, LogitsTile& 
 }
 
 // STORE needs units of 64 or 128 words: the stage's boxes are 64 wide.
-template <typename T, bool PAIR, int STORE, int CHUNK>
+template <typename T, bool PAIR, int STORE, int CHUNK, int MAXN>
 struct Logits : LogitsProblem {
   static constexpr bool kPair = PAIR, kTall = false;
   static constexpr bool kAMn = false;
-  static constexpr int kChunk = CHUNK;
+  static constexpr int kChunk = CHUNK, kMaxN = MAXN;
   static constexpr int kStageBytes = STORE != kNone ? 8192 : 0;
   using Tile = LogitsTile;
 
@@ -1470,7 +1470,7 @@ template <typename T, bool PAIR, bool TALL, bool SPLIT>
 struct Dx {
   static constexpr bool kPair = PAIR, kTall = TALL;
   static constexpr bool kAMn = true;
-  static constexpr int kChunk = 0;
+  static constexpr int kChunk = 0, kMaxN = tc::kEpiN;
   static constexpr int kStageBytes = 0;
   static constexpr int kRows = (TALL ? 4 : PAIR ? 2 : 1) * tc::kBM;  // features per tile
   // With K this long nothing stays in L2 from tile to tile: 8 x 9 tiles in flight read the
@@ -1606,7 +1606,7 @@ template <typename T, bool TALL>
 struct Dw {
   static constexpr bool kPair = true, kTall = TALL;
   static constexpr bool kAMn = true;
-  static constexpr int kChunk = 0;
+  static constexpr int kChunk = 0, kMaxN = tc::kEpiN;
   static constexpr int kStageBytes = 4096;
   static constexpr int kRows = (TALL ? 4 : 2) * tc::kBM;  // words per tile
   struct Tile {};
@@ -1982,10 +1982,10 @@ unsigned int* timeout_counter() {
   return addr[dev];
 }
 
-template <typename T, int FMT, bool PAIR, int STORE, int CHUNK>
+template <typename T, int FMT, bool PAIR, int STORE, int CHUNK, int MAXN = tc::kEpiN>
 cudaError_t run_logits(const LogitsProblem& p, unsigned int* timeouts, cudaStream_t st,
                        bool overlap) {
-  using Problem = Logits<T, PAIR, STORE, CHUNK>;
+  using Problem = Logits<T, PAIR, STORE, CHUNK, MAXN>;
   Problem q;
   static_cast<LogitsProblem&>(q) = p;
   return tc::launch_tc_epi<Problem, FMT>(q, sms(), timeouts, st, overlap);
@@ -2273,9 +2273,16 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, const TokenRows& all, cha
           return cudaErrorInvalidValue;
         lp.tiles_n = (words + lp.tile_n - 1) / lp.tile_n;
         lp.tiles_total = static_cast<long long>(lp.tiles_m) * lp.tiles_n;
-        const auto form = pair                     ? run_logits<T, FMT, true, kStore, kLogitsChunk>
-                          : rows <= kStreamTokens ? run_logits<T, FMT, false, kStore, kFewLogitsChunk>
-                                                  : run_logits<T, FMT, false, kStore, kLogitsChunk>;
+        auto form = run_logits<T, FMT, true, kStore, kLogitsChunk>;
+        if (!pair) {
+          // narrow tiles: latency sets their pace, which more stages hide (loss and dx of 20 x 8192 x
+          // 8000 91 -> 78 us, a step of 6 x 4096 x 18000 130 -> 117)
+          const bool few = rows <= kStreamTokens, narrow = lp.tile_n <= 128;
+          form = few ? narrow ? run_logits<T, FMT, false, kStore, kFewLogitsChunk, 128>
+                              : run_logits<T, FMT, false, kStore, kFewLogitsChunk>
+                 : narrow ? run_logits<T, FMT, false, kStore, kLogitsChunk, 128>
+                          : run_logits<T, FMT, false, kStore, kLogitsChunk>;
+        }
         MB200_TRY(form(lp, to, st, overlap));
         overlap = true;
       }
