@@ -330,7 +330,8 @@ cudnnStatus_t cudnnLinearDistillationBackward(cudnnHandle_t handle, cudnnTensorD
 /* Losses of post-training on the same head (extensions).  nll[t] is the cross entropy above,
  * the negative log-probability of the label; x, w, labels, the workspace, streams and capture
  * are as above, and so is a token that a negative label leaves out: 0 in every output, no
- * gradient, whatever the other inputs hold there.  All float arrays are fp32.
+ * gradient, whatever the other inputs hold there.  All float arrays are fp32.  Device memory is
+ * the current device's: another one's is BAD_PARAM.
  *
  * Policy loss, per token, z = x w^T / temperature:
  *   ratio = exp(oldNll - nll)            oldNll null: 1, and its gradient as if it were nll
@@ -420,8 +421,9 @@ cudnnStatus_t cudnnLinearPreferenceLossBackward(
  * read.  A token of V or more makes its row of y NaN and enters no gradient.  A word's rows are
  * added in the order of their positions, without atomics: results are the same on every run.
  *
- * Backward's workspace: null uses the handle's own, ordered and captured as for the losses
- * above; GetWorkspaceSize reports what a given one (aligned to 256 bytes) needs. */
+ * Device memory is the current device's: another one's is BAD_PARAM.  Backward's workspace: null
+ * uses the handle's own, ordered and captured as for the losses above; GetWorkspaceSize reports
+ * what a given one (aligned to 256 bytes) needs. */
 cudnnStatus_t cudnnEmbeddingForward(cudnnHandle_t handle, const void* alpha,
                                     cudnnFilterDescriptor_t wDesc, const void* w,
                                     const int64_t* tokens, const void* beta,

@@ -1183,6 +1183,16 @@ std::size_t row_span(std::int64_t rows, std::int64_t ld, int c) {
   return static_cast<std::size_t>((rows - 1) * ld + c) * 2;
 }
 
+// Whether p is not another device's memory (which this one may or may not reach).
+bool on_this_device(const void* p) {
+  cudaPointerAttributes attr{};
+  if (cudaPointerGetAttributes(&attr, p) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return false;
+  }
+  return attr.type != cudaMemoryTypeDevice || attr.device == mb200::current_device();
+}
+
 // Checks the pointers of `a` (sizes are set) and runs it.
 cudnnStatus_t vocab_run(DnnContext& h, const VocabLossArgs& a, void* workSpace,
                         std::size_t workSpaceSize) {
@@ -1218,9 +1228,10 @@ cudnnStatus_t vocab_run(DnnContext& h, const VocabLossArgs& a, void* workSpace,
       {floats(a.policy.kl, T), 4},
       {floats(a.preference.loss, P), 4},
       {floats(a.preference.rewards, 2 * P), 4}};
-  const auto usable = [](const std::pair<Span, std::size_t>& s) {
+  const auto usable = [&](const std::pair<Span, std::size_t>& s) {
     return s.first.bytes == 0 || (mb200::aligned_to(s.first.p, s.second) &&
-                                  mb200::device_span_ok(s.first.p, s.first.bytes));
+                                  mb200::device_span_ok(s.first.p, s.first.bytes) &&
+                                  (a.head == HeadLoss::kTargets || on_this_device(s.first.p)));
   };
   for (const auto& s : in)
     if (!usable(s)) return CUDNN_STATUS_BAD_PARAM;
@@ -1572,7 +1583,8 @@ cudnnStatus_t embedding_call(cudnnHandle_t handle, const void* alpha, const void
     for (const auto& [m, align] :
          {std::pair<Span, std::size_t>{r, rs}, {w, ts}, {t, 8}, {ws, 256}}) {
       if (m.bytes == 0) continue;
-      if (!mb200::aligned_to(m.p, align) || !mb200::device_span_ok(m.p, m.bytes))
+      if (!mb200::aligned_to(m.p, align) || !mb200::device_span_ok(m.p, m.bytes) ||
+          !on_this_device(m.p))
         return CUDNN_STATUS_BAD_PARAM;
     }
     if (overlap(r, w) || overlap(gradient ? w : r, t) || overlap(ws, r) || overlap(ws, w) ||

@@ -546,3 +546,19 @@ def test_refusals_of_memory(cuda, built):
         assert given(_p(ws), size) == 0
         cuda.cuda.synchronize()
         e.check_backward(None)
+
+
+@pytest.mark.gpu
+def test_refuses_another_devices_memory(cuda, built):
+    if cuda.cuda.device_count() < 2:
+        pytest.skip("needs two devices")
+    bad = capi.CUDNN_STATUS_BAD_PARAM
+    e = Table(cuda, 32, 64, 100)
+    with Dnn(cuda) as d:
+        for name in ("rows", "w", "tokens"):
+            here = getattr(e, name)
+            setattr(e, name, here.to("cuda:1"))
+            assert e.forward(d) == bad and e.backward(d) == bad, name
+            setattr(e, name, here)
+        ws = cuda.empty(e.workspace_size(d), device="cuda:1", dtype=cuda.uint8)
+        assert e.backward(d, ws=ws) == bad

@@ -879,6 +879,23 @@ def test_workspace_bounds(built):
 
 
 @pytest.mark.gpu
+def test_refuses_another_devices_memory(cuda, built):
+    if cuda.cuda.device_count() < 2:
+        pytest.skip("needs two devices")
+    bad = capi.CUDNN_STATUS_BAD_PARAM
+    with Dnn(cuda) as d:
+        for h, names in ((Policy(cuda, 32, 64, 100), ("labels", "old", "ref", "advantages", "dloss")),
+                         (Preference(cuda, 32, 64, 100, 2), ("labels", "offsets", "ref", "dloss"))):
+            for name in names + h.outputs + ("x", "w", "dx", "dw"):
+                here = getattr(h, name)
+                setattr(h, name, here.to("cuda:1"))
+                assert h.backward(d) == bad, name
+                setattr(h, name, here)
+            ws = cuda.empty(h.workspace_size(d, 1), device="cuda:1", dtype=cuda.uint8)
+            assert h.backward(d, ws) == bad
+
+
+@pytest.mark.gpu
 def test_refusals_of_memory(cuda, built):
     bad = capi.CUDNN_STATUS_BAD_PARAM
     p, q = Policy(cuda, 32, 64, 100), Preference(cuda, 32, 64, 100, 2)
