@@ -33,6 +33,8 @@
 //                                                   // 64 x tile_n (pair: tile_n / 2) of B
 //   void coords(long long t, int (&c)[3]) const;    // c[1], c[2]: tile row and column
 //   int k_begin(const int (&c)[3]) const;           // first k-block of the tile
+//   bool next_early() const;                        // whether the next kernel may start once a
+//                                                   // CTA's loads are out
 //   struct Tile;                                    // per-thread epilogue state
 //   void begin(Tile&, c, int row, int half) const;  // before the accumulator is waited for
 //   void chunk(Tile&, c, int row, int half, uint32_t taddr, bool first, uint8_t* stage) const;
@@ -184,6 +186,7 @@ __device__ __forceinline__ void epi_body(const P& p, unsigned int* timeouts) {
         }
       }
     }
+    if (p.next_early()) grid_launch_next();
     // Drain: a pair's copies all complete on the even CTA's barriers.
     if (rank == 0) {
       for (int s = 0; s < STAGES; ++s)
@@ -324,7 +327,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kEpiThreads, 1)
 // Launches `kern`; with `overlap` its prologue may overlap the end of the stream's previous
 // kernel (it calls grid_wait_previous() before it touches memory).  Overlap only with a
 // kernel that waits for its own predecessor in turn: one's own.  tc_epi kernels do not
-// let the next one start early: its waiting CTAs cost them 2-4 %.
+// let the next one start before their loads are out: its waiting CTAs cost them 2-4 %.
 template <typename... K, typename... A>
 cudaError_t launch_overlapped(void (*kern)(K...), dim3 grid, int threads, std::size_t smem,
                               cudaStream_t stream, bool overlap, A... args) {

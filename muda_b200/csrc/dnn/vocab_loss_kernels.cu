@@ -190,7 +190,7 @@ constexpr int kUnit = 128;
 // 4e-7, an fp32 product's level.
 // Up to 8 tokens take 8 MMAs, as their streaming kernel does, so that a width that it cannot
 // read is no less exact (T 4, H 4001: 3.0e-7 and 0.8e-7, streamed at 4000 0.9e-7); with more
-// tokens that would cost up to 37 % (score of 128 x 768 x 50257).
+// tokens that would cost up to 10 % (score of 20 x 8192 x 8000, 47.8 -> 52.8 us).
 constexpr int kLogitsChunk = 8, kFewLogitsChunk = 2;
 
 // What a truncating MMA takes from a logit, as a share of it and on average (measured as lse's
@@ -223,6 +223,8 @@ struct LogitsProblem {
   float2* stats;      // [row][units] (maximum of x w, sum of 2^(z2 - the maximum's))
   std::int64_t ldn;
   Targets targets;
+  bool score_next;    // a short score's finish comes next and starts on the last tiles' time (20 x
+                      // 8192 x 8000 47.8 -> 46.0 us; gradients and long scores gained nothing)
 
   const CUtensorMap* __device__ map_a() const { return &mx; }
   const CUtensorMap* __device__ map_b() const { return &mw; }
@@ -231,6 +233,7 @@ struct LogitsProblem {
     banded(static_cast<int>(t), tiles_m, tiles_n, band, &c[1], &c[2]);
   }
   __device__ int k_begin(const int (&)[3]) const { return 0; }
+  __device__ bool next_early() const { return score_next; }
 };
 
 __device__ __forceinline__ std::int64_t target_hint(const LogitsProblem& p, int row, int n0) {
@@ -1031,6 +1034,7 @@ struct FinishArgs {
   const void* w;
   int features;
   float truncated;
+  bool early;  // x w of the targets before the logits are done: x is the caller's, no copy of it
   PolicyLoss policy;
   int* pairs_done;  // with dnll: to be set to 0
   float* dnll;  // kNone: null, or the gradients by the tokens' nll (without a policy zeros)
@@ -1202,6 +1206,18 @@ __device__ __forceinline__ float exact_target_nll(float z, float was, float mx, 
 template <typename T, int STORE, int FORM>
 __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const FinishArgs a) {
   tc::grid_launch_next();
+  // the caller's x, w and labels, which no kernel of a call writes before this one
+  const auto target_part = [&](int row, std::int64_t label) {
+    return target_logit_part<T>(static_cast<const T*>(a.x) + row * a.ldx,
+                                static_cast<const T*>(a.w) + label * a.features, a.features);
+  };
+  [[maybe_unused]] float dot = 0.0f;
+  if constexpr (STORE == kNone && FORM != kTargetLoss) {
+    if (a.early) {  // a CTA per row
+      const std::int64_t label = a.targets.labels[blockIdx.x];
+      if (label >= 0 && label < a.vocab) dot = target_part(blockIdx.x, label);
+    }
+  }
   tc::grid_wait_previous();
   constexpr bool kDz = STORE == kOwn || STORE == kSplit;
   __shared__ float red[kFinishThreads / 32];
@@ -1252,12 +1268,8 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Fini
     }
     return;
   }
-  [[maybe_unused]] float dot = 0.0f;  // its loads go out before the reductions below
-  if constexpr (FORM != kTargetLoss) {
-    if (n > 0)
-      dot = target_logit_part<T>(static_cast<const T*>(a.x) + row * a.ldx,
-                                 static_cast<const T*>(a.w) + a.targets.labels[row] * a.features,
-                                 a.features);
+  if constexpr (FORM != kTargetLoss) {  // its loads go out before the reductions below
+    if (n > 0 && !(STORE == kNone && a.early)) dot = target_part(row, a.targets.labels[row]);
   }
   const float2* st = a.stats + static_cast<std::int64_t>(row) * a.units;
   float mx = -INFINITY;
@@ -1491,6 +1503,7 @@ struct Dx {
   int lefts;
   const T* w;               // all words, rows of `features`
 
+  __device__ bool next_early() const { return false; }
   const CUtensorMap* __device__ map_a() const { return &ma; }
   const CUtensorMap* __device__ map_b() const { return &mb; }
   __device__ void coords(long long t, int (&c)[3]) const {
@@ -1625,6 +1638,7 @@ struct Dw {
   bool tma;    // dw's rows are 16-byte aligned
   const float* scale;
 
+  __device__ bool next_early() const { return false; }
   const CUtensorMap* __device__ map_a() const { return &ma; }
   const CUtensorMap* __device__ map_b() const { return &mb; }
   __device__ void coords(long long t, int (&c)[3]) const {
@@ -2209,8 +2223,9 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, const TokenRows& all, cha
                                        std::min(chunk, (a.features + 15) / 16));
       z_scale = static_cast<float>(1.4426950408889634 * a.inv_tau * (1.0 + f.truncated));
     }
-    f.x = x;
-    f.ldx = ldx;
+    f.early = p.store == kNone && rows <= tc::kBM;
+    f.x = f.early ? static_cast<const T*>(a.x) + t0 * a.ldx : x;
+    f.ldx = f.early ? (a.tokens > 1 ? a.ldx : 0) : ldx;
     f.w = a.w;
     f.features = a.features;
     if (form == kPolicy) {
@@ -2288,6 +2303,7 @@ cudaError_t run(const VocabLossArgs& a, const Plan& p, const TokenRows& all, cha
       }
       return cudaSuccess;
     };
+    lp.score_next = f.early;
     if (p.store == kNone) {
       MB200_TRY(logits(std::integral_constant<int, kNone>{}));
       MB200_TRY(launch(finish_form(std::integral_constant<int, kNone>{}), rows, kFinishThreads, f));
