@@ -419,7 +419,7 @@ cudnnStatus_t cudnnLinearPreferenceLossBackward(
  *
  * A negative token (padding) stands for a row of zeros: y[t] = beta y[t], and its dy is not
  * read.  A token of V or more makes its row of y NaN and enters no gradient.  A word's rows are
- * added in the order of their positions, without atomics: results are the same on every run.
+ * added in the order of their positions: results are the same on every run.
  *
  * Device memory is the current device's: another one's is BAD_PARAM.  Backward's workspace: null
  * uses the handle's own, ordered and captured as for the losses above; GetWorkspaceSize reports

@@ -1193,6 +1193,15 @@ bool on_this_device(const void* p) {
   return attr.type != cudaMemoryTypeDevice || attr.device == mb200::current_device();
 }
 
+bool is_device_memory(const void* p) {
+  cudaPointerAttributes attr{};
+  if (cudaPointerGetAttributes(&attr, p) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return false;
+  }
+  return attr.type == cudaMemoryTypeDevice;
+}
+
 // Checks the pointers of `a` (sizes are set) and runs it.
 cudnnStatus_t vocab_run(DnnContext& h, const VocabLossArgs& a, void* workSpace,
                         std::size_t workSpaceSize) {
@@ -1592,6 +1601,7 @@ cudnnStatus_t embedding_call(cudnnHandle_t handle, const void* alpha, const void
       return CUDNN_STATUS_BAD_PARAM;
     const cudaStream_t st = stream_of(*h);
     if (!gradient) return status_of(mb200::dnn::launch_embedding(a, st));
+    a.device_table = is_device_memory(table);
     const std::size_t need = mb200::dnn::embedding_gradient_workspace(a);
     if (workSpace != nullptr) {
       if (workSpaceSize < need) return CUDNN_STATUS_BAD_PARAM;

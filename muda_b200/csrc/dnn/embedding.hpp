@@ -24,6 +24,7 @@ struct EmbeddingArgs {
   void* row;           // lookup: y; gradient: dy (read only)
   std::int64_t ld;     // elements from one row to the next
   void* w;             // lookup: the table (read only); gradient: dw; rows packed
+  bool device_table;   // gradient: dw is device memory, neither managed nor the host's
 };
 
 cudaError_t launch_embedding(const EmbeddingArgs& a, cudaStream_t stream) noexcept;

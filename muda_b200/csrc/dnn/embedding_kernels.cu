@@ -695,10 +695,15 @@ __device__ __forceinline__ void store_partial(const Slice<VEC, RUNS>& s, float* 
       store_run<false>(o + h + r * s.kStep, pack<float, VEC>(s.v[r]));
 }
 
-// What becomes of dw: nothing of it is left, beta of it, or (fp32, beta 1) the sums are added
-// to it.  kAdd's additions are done by L2, each element's one, so that no load's latency is
+// What becomes of dw: nothing of it is left, beta of it, or (fp32 device memory, beta 1) the sums
+// are added to it.  kAdd's additions are done by L2, each element's one, so that no load's latency is
 // waited for (the second micro-batch of 32768 x 2048: 69 us with kScale, 60).
 enum Update { kWrite = 0, kScale = 1, kAdd = 2 };
+
+// They take numbers below 2^-126 for zeros.  A sum of kLeastAdded or more does not see that: what
+// dw was rounds away, and no cancellation leaves so little (both are multiples of 2^-124 then, or
+// dw is the smaller by half).  Runs with a lesser sum are loaded.
+constexpr float kLeastAdded = 0x1p-100f;
 
 template <int VEC>
 __device__ __forceinline__ void add_run(float* p, const float (&v)[VEC]) {
@@ -731,8 +736,17 @@ __device__ __forceinline__ void store_row(const Slice<VEC, RUNS>& s, const SumAr
 #pragma unroll
     for (int e = 0; e < VEC; ++e) v[e] = a.alpha * s.v[r][e];
     if constexpr (UPDATE == kAdd) {
-      add_run<VEC>(o + r * s.kStep, v);
-      continue;
+      bool small = false;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) small |= !(fabsf(v[e]) >= kLeastAdded);
+      if (!small) {
+        add_run<VEC>(o + r * s.kStep, v);
+        continue;
+      }
+      float old[VEC];
+      unpack<TW, VEC>(load_run<TW, VEC>(o + r * s.kStep), old);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) v[e] += old[e];
     }
     if constexpr (UPDATE == kScale) {
       float old[VEC];
@@ -1083,7 +1097,7 @@ cudaError_t gradient(const EmbeddingArgs& a, const SortPlan& p, int first_row, c
     auto kern = a.beta != 0.0f ? embedding_sum_kernel<kScale, T, TW, VEC, RUNS, kAhead, kCtas>
                                : embedding_sum_kernel<kWrite, T, TW, VEC, RUNS, kAhead, kCtas>;
     if constexpr (std::is_same_v<TW, float>) {
-      if (a.beta == 1.0f) kern = embedding_sum_kernel<kAdd, T, TW, VEC, RUNS, kAhead, kCtas>;
+      if (a.beta == 1.0f && a.device_table) kern = embedding_sum_kernel<kAdd, T, TW, VEC, RUNS, kAhead, kCtas>;
     }
     const std::int64_t ctas =
         std::min<std::int64_t>((units + kSumWarps - 1) / kSumWarps, sms() * kCtas);

@@ -549,6 +549,45 @@ def test_refusals_of_memory(cuda, built):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", ["bf16", "fp32"])
+@pytest.mark.parametrize("T,H", [(100, 512), (100, 37), (3, 64), (20000, 64)])
+@pytest.mark.parametrize("beta", [1.0, 0.5])
+def test_sums_and_tables_of_subnormals(cuda, built, rows, T, H, beta):
+    """Sums of mixed sizes into a table of them: zeros, subnormals, cancellations."""
+    e = Table(cuda, T, H, 64, rows=rows, table="fp32", seed=T + H)
+    sizes = cuda.tensor([0.0, 2.0 ** -133, 2.0 ** -127, 2.0 ** -125, 2.0 ** -101, 2.0 ** -99, 1.0],
+                        device="cuda")
+
+    def mixed(t):
+        s = sizes[cuda.randint(0, len(sizes), t.shape, device="cuda", generator=e.g)]
+        sign = cuda.randint(0, 2, t.shape, device="cuda", generator=e.g) * 2 - 1
+        t.copy_((s * sign).to(t.dtype))
+
+    mixed(e.rows)
+    mixed(e.w)
+    e.rows[::2] = 0.0
+    e.w[5] = -e.rows[e.tokens == 5].float().sum(0)
+    was = e.w.clone()
+    with Dnn(cuda) as d:
+        assert e.backward(d, beta=beta) == 0
+    cuda.cuda.synchronize()
+    e.check_backward(was, beta=beta)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("beta", [0.0, 0.5, 1.0])
+def test_gradient_into_pinned_memory(cuda, built, beta):
+    e = Table(cuda, 300, 64, 100, rows="bf16", table="fp32")
+    device = e.w
+    e.w = device.cpu().pin_memory()
+    with Dnn(cuda) as d:
+        assert e.backward(d, beta=beta) == 0
+    cuda.cuda.synchronize()
+    e.w, was = e.w.cuda(), device
+    e.check_backward(was, beta=beta)
+
+
+@pytest.mark.gpu
 def test_refuses_another_devices_memory(cuda, built):
     if cuda.cuda.device_count() < 2:
         pytest.skip("needs two devices")
