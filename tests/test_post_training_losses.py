@@ -679,6 +679,55 @@ def test_captured_in_a_graph(cuda, built, kind, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("kind", ["policy", "preference"])
+@pytest.mark.parametrize("T,H,V", [(4, 4096, 900), (6, 1031, 2000), (20, 4096, 3001),
+                                   (128, 264, 5000), (100, 1031, 700)])
+def test_short_scores_follow_their_inputs(cuda, built, kind, T, H, V, captured):
+    """Scores in a row, each after kernels that write its inputs where the last one's were."""
+    make = lambda s: (Policy(cuda, T, H, V, seed=s) if kind == "policy"  # noqa: E731
+                      else Preference(cuda, T, H, V, 2, seed=s))
+    h, sets = make(0), [make(s) for s in (1, 2, 3)]
+    names = ("x", "w", "labels", "ref") + (("old", "advantages") if kind == "policy"
+                                           else ("offsets",))
+    stream = cuda.cuda.Stream()
+    with Dnn(cuda) as d:
+        for s in sets:
+            assert s.forward(d) == 0
+        cuda.cuda.synchronize()
+        assert d.L.cudnnSetStream(d.h, C.c_void_p(stream.cuda_stream)) == 0
+        got = [[cuda.empty_like(getattr(h, n)) for n in h.outputs] for _ in sets]
+
+        def scores():
+            for s, outs in zip(sets, got):
+                for n in names:
+                    getattr(h, n).copy_(getattr(s, n))
+                assert h.forward(d) == 0
+                for n, o in zip(h.outputs, outs):
+                    o.copy_(getattr(h, n))
+
+        with cuda.cuda.stream(stream):
+            scores()
+            if captured:
+                stream.synchronize()
+                graph = cuda.cuda.CUDAGraph()
+                with cuda.cuda.graph(graph, stream=stream):
+                    scores()
+                for outs in got:
+                    for o in outs:
+                        o.fill_(math.nan)
+                for _ in range(3):
+                    graph.replay()
+            stream.synchronize()
+        if captured:
+            del graph
+    for s, outs in zip(sets, got):
+        s.check(gradients=False)
+        for n, o in zip(h.outputs, outs):
+            assert cuda.equal(o, getattr(s, n)), n
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 def test_pieces_captured_in_a_graph(cuda, built, dtype):
     """A preference step of several pieces, in a given workspace that held other things."""
