@@ -1190,17 +1190,20 @@ __device__ __forceinline__ float target_logit(float part, double* red) {
 // (relative to their maximum mx).  The sums' truncation took from mx what it took from `was`, in
 // proportion: a part that all words of a row have in common (an offset of their logits) has to
 // leave the difference, or a token would be off by 4e-7 of it.  Targets near zero do not tell,
-// so the average counts for an eighth of mx.
+// so the average counts for an eighth of mx.  Where the target is its row's largest word z is
+// that word's logit too: any other difference is noise, which a small temperature multiplies.
+// The other words' share of the sum is never negative, so neither is what this returns; NaN in
+// it stays.
 __device__ __forceinline__ float exact_target_nll(float z, float was, float mx, float sum,
                                                   float log2e_tau, float inv_tau,
                                                   float truncated) {
   const float q = was / mx;
   float r = ((z - was) / mx * q + truncated * 0x1p-6f) / (q * q + 0x1p-6f);
   if (!(fabsf(r) < 8.0f * truncated)) r = truncated;
-  const float below = ((z - mx) - mx * r) * inv_tau;  // of the maximum's place
-  // the target's own share of the sum moves too
-  const float moved = sum + (expf(below) - exp2f((was - mx) * log2e_tau));
-  return logf(moved) - below;
+  const float below = was == mx ? 0.0f : ((z - mx) - mx * r) * inv_tau;  // of the maximum's place
+  float rest = sum - exp2f((was - mx) * log2e_tau);
+  if (rest < 0.0f) rest = 0.0f;
+  return below < 0.0f ? logf(rest + expf(below)) - below : log1pf(rest * expf(-below));
 }
 
 template <typename T, int STORE, int FORM>

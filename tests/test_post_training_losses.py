@@ -478,6 +478,108 @@ def test_infinite_references(cuda, built, dtype):
     assert h.rewards[0] == math.inf and h.rewards[4] == math.inf and h.loss[2].isfinite()
 
 
+def _sure(h, cancelling, equal=1):
+    """Makes each token's label its row's largest word, with `equal` - 1 other words that equal
+    it: 32 above the others, which are of order 1; or, cancelling, 0.25 above them, in logits of
+    order 0 that are sums of +-768.  There the tensor cores' sums may be off by 2^-14 (the last
+    place kept of numbers below 2^10, in 24 bits) for each of 17 terms of 32 MMAs, 0.033."""
+    torch, (T, H), V = h.torch, h.x.shape, len(h.w)
+    own = torch.arange(T, device="cuda")
+    half = (H - 256) // 2
+    assert T <= 256 <= H and T * equal <= V and half == 128
+    h.labels = own.clone()
+    if cancelling:
+        x = 1 + torch.rand(T, half, device="cuda", generator=h.g)
+        w = torch.rand(V, half, device="cuda", generator=h.g) * 8
+        h.x[:, 256:] = torch.cat([x, x], dim=1).to(h.x.dtype)
+        h.w[:, 256:] = torch.cat([w, -w], dim=1).to(h.w.dtype)
+    h.x[:, :256], h.w[:, :256] = 0.0, 0.0
+    h.x[own, own] = 0.5 if cancelling else 8.0
+    h.w[own, own] = 0.5 if cancelling else 4.0
+    for k in range(1, equal):
+        h.w[k * T:(k + 1) * T] = h.w[:T]
+    z = h.x.double() @ h.w.double().t()
+    others = z.clone()
+    for k in range(equal):
+        others[own, own + k * T] = -math.inf
+    assert (z[own, own] - others.amax(dim=1) > (0.24 if cancelling else 20)).all()
+
+
+TEMPERATURES = [1.0, 1e-3, 1e-5, 1e-7, 1e-8, 2.0 ** -30, 2.0 ** -40, 2.0 ** -64]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("cancelling", [False, True])
+@pytest.mark.parametrize("T", [4, 40, 200])
+def test_sure_labels_at_any_temperature(cuda, built, T, cancelling, dtype):
+    """The label's share is 1 to the last bit below 2^-7 (a gap of 0.17 / tau above 18): its nll
+    is 0, not the noise of its logit over the temperature, and so are its gradients."""
+    h = Policy(cuda, T, 512, 1200, dtype, coef=0.0, old=False, ref=False)
+    _sure(h, cancelling)
+    h.ref = cuda.zeros(T, device="cuda")
+    for h.tau in TEMPERATURES:
+        for h.old in (None, cuda.zeros(T, device="cuda")):
+            for dw in (None, False, True):  # scores, a frozen head, steps
+                h.clear()
+                with Dnn(cuda) as d:
+                    assert (h.forward(d) if dw is None else h.backward(d, dw=dw)) == 0
+                    cuda.cuda.synchronize()
+                assert (h.nll >= 0).all(), h.tau
+                if h.tau == 1.0:
+                    h.check(gradients=False, outputs=("nll",))
+                    continue
+                assert (h.nll == 0).all() and (h.ratio == 1).all() and (h.kl == 0).all(), h.tau
+                assert (h.loss == -h.advantages).all(), h.tau
+                assert dw is None or (h.dx == 0).all(), h.tau
+                assert not dw or (h.dw == 0).all(), h.tau
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("cancelling", [False, True])
+@pytest.mark.parametrize("T,equal", [(4, 2), (40, 3), (200, 5)])
+def test_equal_words_at_any_temperature(cuda, built, T, equal, cancelling, dtype):
+    """Words with the label's own row share with it at any temperature: nll is log(equal), of
+    which log1p rounds to 2 units of its last place at most."""
+    h = Policy(cuda, T, 512, 1200, dtype, coef=0.0, old=False, ref=False)
+    _sure(h, cancelling, equal)
+    for h.tau in TEMPERATURES[1:]:
+        h.clear()
+        with Dnn(cuda) as d:
+            assert h.forward(d, outputs=("nll", "ratio", "loss")) == 0
+            cuda.cuda.synchronize()
+        assert (abs(h.nll - math.log(equal)) <= 2.0 ** -22 * math.log(equal)).all(), h.tau
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("tau", TEMPERATURES[1:])
+@pytest.mark.parametrize("T", [4, 40, 200])
+def test_any_label_at_any_temperature(cuda, built, T, tau, dtype):
+    """Labels that are not their rows' largest words: nll to its logits' errors over tau."""
+    h = Policy(cuda, T, 512, 1200, dtype, tau=tau, coef=0.0, old=False, ref=False)
+    with Dnn(cuda) as d:
+        assert h.forward(d, outputs=("nll",)) == 0
+        cuda.cuda.synchronize()
+    assert (h.nll >= 0).all()
+    h.check(gradients=False, outputs=("nll",))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("cancelling", [False, True])
+@pytest.mark.parametrize("T", [4, 40, 200])
+def test_sequences_of_sure_labels(cuda, built, T, cancelling, dtype):
+    h = Preference(cuda, T, 512, 1200, 2, dtype, ref=False, lengths=[T // 4] * 4)
+    _sure(h, cancelling)
+    with Dnn(cuda) as d:
+        assert h.forward(d) == 0
+        cuda.cuda.synchronize()
+    assert (h.nll >= 0).all()
+    h.check(gradients=False)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("kind", ["policy", "preference"])
