@@ -957,10 +957,12 @@ __global__ void __launch_bounds__(kPreferenceThreads)
   const double h = bad ? NAN : beta * (gain[0] - gain[1]) - a.p.margin;
   double loss, slope;
   if (a.p.mode == PreferenceMode::kSigmoid) {
-    // of h's own size the loss keeps 64 bits; what softplus adds to it is a float
+    // of h's own size the loss keeps 64 bits; what softplus adds to it is a float.  h may be
+    // infinite: its two multiples, -h and smoothing h, are one, and 0 of it is 0
     const float e = expf(static_cast<float>(-fabs(h)));
-    loss = (h < 0.0 ? -h : 0.0) + log1pf(e);
-    if (a.p.smoothing != 0.0) loss += a.p.smoothing * h;  // h may be infinite
+    const double part = h < 0.0 ? a.p.smoothing - 1.0 : a.p.smoothing;
+    loss = log1pf(e);
+    if (part != 0.0) loss += part * h;
     slope = a.p.smoothing - (h < 0.0 ? 1.0f : e) / (1.0f + e);
   } else if (a.p.mode == PreferenceMode::kHinge) {
     loss = h < 1.0 ? 1.0 - h : h >= 1.0 ? 0.0 : h;

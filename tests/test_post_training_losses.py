@@ -510,6 +510,36 @@ TEMPERATURES = [1.0, 1e-3, 1e-5, 1e-7, 1e-8, 2.0 ** -30, 2.0 ** -40, 2.0 ** -64]
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("smoothing", [0.0, 0.1, 0.5])
+def test_infinite_references_with_smoothing(cuda, built, smoothing, dtype):
+    """softplus(-h) + smoothing h of h = inf and -inf: |h| times smoothing and 1 - smoothing.  The
+    slopes are smoothing and smoothing - 1, so that the gradients are a sum of nll's."""
+    h = Preference(cuda, 100, 64, 300, 3, dtype, smoothing=smoothing, lengths=[10] * 6, seed=8)
+    h.ref[3] = math.inf    # pair 0's chosen sequence
+    h.ref[45] = math.inf   # pair 1's rejected one
+    with Dnn(cuda) as d:
+        assert h.backward(d) == 0
+        cuda.cuda.synchronize()
+    assert h.loss[0] == (math.inf if smoothing else 0.0) and h.loss[1] == math.inf
+    assert h.loss[2].isfinite() and h.dw.isfinite().all()
+    nll, _, _, zerr = h.nll64()
+    p = cuda.softmax(h.x.double() @ h.w.double().t(), dim=1)
+    target = cuda.nn.functional.one_hot(h.labels, 300)
+    u = U[dtype]
+    for pair, slope in ((0, smoothing), (1, smoothing - 1)):
+        g = h.dloss[pair].item() * slope * h.beta
+        for s, sign in ((pair, -1), (3 + pair, 1)):
+            rows = slice(10 * s, 10 * s + 10)
+            dx = sign * g * (p - target)[rows] @ h.w.double()
+            # a word's dz rounds three times, and half a step of fp16's least kept (2^-26) besides;
+            # p is off by its logits' errors; dx rounds once
+            err = abs(g) * ((p + target)[rows] * (3 * u + 2 * zerr[rows, None] + 2.0 ** -18) + 2.0 ** -26)
+            t = err @ h.w.double().abs() + 1.01 * u * dx.abs() + TINY[dtype]
+            assert ((h.dx[rows].double() - dx).abs() <= t).all(), (pair, s)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("cancelling", [False, True])
 @pytest.mark.parametrize("T", [4, 40, 200])
 def test_sure_labels_at_any_temperature(cuda, built, T, cancelling, dtype):
