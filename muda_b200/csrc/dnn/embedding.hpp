@@ -9,8 +9,11 @@
 
 #include <cuda_runtime_api.h>
 
+#include <algorithm>
 #include <cstddef>
 #include <cstdint>
+
+#include "common/device.hpp"
 
 namespace mb200::dnn {
 
@@ -33,5 +36,38 @@ cudaError_t launch_embedding(const EmbeddingArgs& a, cudaStream_t stream) noexce
 std::size_t embedding_gradient_workspace(const EmbeddingArgs& a) noexcept;
 cudaError_t launch_embedding_gradient(const EmbeddingArgs& a, void* workspace,
                                       cudaStream_t stream) noexcept;
+
+// ----------------------------------------------------------- a part of the gradient's plan --
+// CTAs of the sort, their threads, and the most tokens that it does not part first.
+constexpr int kEmbeddingOwners = 128, kEmbeddingSortThreads = 1024, kEmbeddingParted = 8192;
+// Bytes of a large dw that the GPU fills in the meantime (beta 0), about what the sort's time
+// has room for: 8192 x 4096 of 128000 words 199 -> 193 us, 32768 x 2048 of 50257 128 -> 121,
+// 1537 x 1111 of 32003 20.4 -> 19.5; a dw of 8 MB 18 -> 20.
+constexpr std::int64_t kFillAtOnce = 16 << 20, kFillPerToken = 2000, kFillParted = 1000;
+constexpr std::int64_t kFillLeast = 32 << 20;
+
+struct EmbeddingFill {
+  int rows;            // from the first on; the sums' launch sees to the others
+  std::int64_t words;  // of 16 bytes
+  unsigned ctas;       // behind the sort's own
+};
+
+// The sort's CTAs come first, two to an SM: a GPU (or a part of one) of 64 SMs or fewer has room
+// for no others, and leaves all rows to the sums.
+inline EmbeddingFill embedding_fill(const EmbeddingArgs& a, int sms) noexcept {
+  const std::int64_t row_bytes =
+      static_cast<std::int64_t>(a.features) * (a.table == EmbeddingType::kF32 ? 4 : 2);
+  const std::int64_t spare = 2ll * sms - kEmbeddingOwners;
+  if (a.beta != 0.0f || !aligned_to(a.w, 16) || a.vocab * row_bytes < kFillLeast || spare <= 0)
+    return {0, 0, 0};
+  const std::int64_t bytes =
+      kFillAtOnce + a.tokens * (a.tokens <= kEmbeddingParted ? kFillPerToken : kFillParted);
+  // multiples of 8 rows are whole 16-byte words
+  const auto rows = static_cast<int>(std::min<std::int64_t>(a.vocab, bytes / row_bytes) / 8 * 8);
+  const std::int64_t words = rows * row_bytes / 16;
+  return {rows, words,
+          static_cast<unsigned>(std::min<std::int64_t>(
+              spare, (words + kEmbeddingSortThreads - 1) / kEmbeddingSortThreads))};
+}
 
 }  // namespace mb200::dnn

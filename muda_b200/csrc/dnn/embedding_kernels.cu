@@ -295,18 +295,14 @@ __global__ void __launch_bounds__(kLookupThreads, kLookupCtas)
 // Latency bound: 1537 tokens of 32003 words 6 us, 8192 of 128000 9 us, 32768 of 50257 5 us and
 // then 12 (clusters of eight that read the tokens together: 18, and 4 more to be launched; a
 // frequent word's owner has 2400 of these and sorts the longest).
-constexpr int kOwners = 128, kOwnerBits = 7;
-constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
+constexpr int kOwners = kEmbeddingOwners, kOwnerBits = 7;
+static_assert(kOwners == 1 << kOwnerBits);
+constexpr int kSortThreads = kEmbeddingSortThreads, kSortWarps = kSortThreads / 32;
 constexpr int kDigit = 5, kDigits = 1 << kDigit;
 constexpr int kSharedList = 4096;  // entries that are sorted in shared memory
 constexpr int kScan = 4;           // tokens per lane at a time
 constexpr int kCompared = 128;     // entries that are sorted by comparing each with all
-constexpr int kParts = 128, kParted = 8192;
-// Bytes of a large dw that the GPU fills in the meantime (beta 0), about what the sort's time
-// has room for: 8192 x 4096 of 128000 words 199 -> 193 us, 32768 x 2048 of 50257 128 -> 121,
-// 1537 x 1111 of 32003 20.4 -> 19.5; a dw of 8 MB 18 -> 20.
-constexpr std::int64_t kFillAtOnce = 16 << 20, kFillPerToken = 2000, kFillParted = 1000;
-constexpr std::int64_t kFillLeast = 32 << 20;
+constexpr int kParts = 128, kParted = kEmbeddingParted;
 
 struct Entry {
   int word;  // v / kOwners
@@ -1170,27 +1166,16 @@ cudaError_t launch_embedding_gradient(const EmbeddingArgs& a, void* workspace,
   s.parts = reinterpret_cast<Entry*>(ws + p.parts);
   s.starts = reinterpret_cast<int*>(ws + p.starts);
   const std::size_t shared = 2 * s.near_list * sizeof(Entry);
-  // rows that are set to zero while the tokens are sorted
-  int first_row = 0;
-  const std::int64_t row_bytes =
-      static_cast<std::int64_t>(a.features) * (a.table == EmbeddingType::kF32 ? 4 : 2);
-  unsigned fill_ctas = 0;
-  if (a.beta == 0.0f && aligned_to(a.w, 16) && a.vocab * row_bytes >= kFillLeast) {
-    const std::int64_t bytes =
-        kFillAtOnce + a.tokens * (a.tokens <= kParted ? kFillPerToken : kFillParted);
-    // multiples of 8 rows are whole 16-byte words
-    first_row = static_cast<int>(std::min<std::int64_t>(a.vocab, bytes / row_bytes) / 8 * 8);
-    s.fill = static_cast<uint4*>(a.w);
-    s.num_fill = first_row * row_bytes / 16;
-    fill_ctas = static_cast<unsigned>(std::min<std::int64_t>(
-        2 * sms() - kOwners, (s.num_fill + kSortThreads - 1) / kSortThreads));
-  }
+  const EmbeddingFill fill = embedding_fill(a, sms());
+  const int first_row = fill.rows;
+  s.fill = static_cast<uint4*>(a.w);
+  s.num_fill = fill.words;
   if (p.share > 0) {
     const cudaError_t e = tc::launch_overlapped(embedding_part_kernel, dim3(kParts), kSortThreads,
                                                 0, st, false, s);
     if (e != cudaSuccess) return e;
   }
-  const cudaError_t e = tc::launch_overlapped(embedding_sort_kernel, dim3(kOwners + fill_ctas),
+  const cudaError_t e = tc::launch_overlapped(embedding_sort_kernel, dim3(kOwners + fill.ctas),
                                               kSortThreads, shared, st, p.share > 0, s);
   if (e != cudaSuccess) return e;
   const bool wide = rows_of_runs(a, a.rows == T::kF32 ? 4 : 8);

@@ -10,10 +10,11 @@ result's type (2^-8 for bf16, 2^-11 for fp16, 2^-24 for fp32) and `tiny` half a 
 
 import ctypes as C
 import math
+import subprocess
 
 import pytest
 
-from muda_b200 import capi
+from muda_b200 import build, capi
 from tests.helpers import Dnn, fptr
 
 U = {"bf16": 2.0 ** -8, "fp16": 2.0 ** -11, "fp32": 2.0 ** -24}
@@ -585,6 +586,46 @@ def test_gradient_into_pinned_memory(cuda, built, beta):
     cuda.cuda.synchronize()
     e.w, was = e.w.cuda(), device
     e.check_backward(was, beta=beta)
+
+PLAN = r"""
+#include <cstdio>
+#include <cstdlib>
+#include "dnn/embedding.hpp"
+int main(int, char** v) {
+  using namespace mb200::dnn;
+  EmbeddingArgs a{};
+  a.table = std::atoi(v[1]) == 4 ? EmbeddingType::kF32 : EmbeddingType::kBF16;
+  a.tokens = std::atoi(v[2]);
+  a.features = std::atoi(v[3]);
+  a.vocab = std::atoi(v[4]);
+  a.w = reinterpret_cast<void*>(std::uintptr_t{256});
+  for (int sms = 1; sms <= 160; ++sms) {
+    const EmbeddingFill f = embedding_fill(a, sms);
+    std::printf("%d %d %lld %u\n", sms, f.rows, static_cast<long long>(f.words), f.ctas);
+  }
+}
+"""
+
+
+def test_filling_beside_the_sort_on_any_number_of_sms(tmp_path):
+    """Rows that the sort's launch fills have CTAs that fill them, behind the sort's own 128 and
+    not beyond what the GPU holds beside them."""
+    src, exe = tmp_path / "plan.cpp", tmp_path / "plan"
+    src.write_text(PLAN)
+    subprocess.run([build.CXX, "-std=c++17", f"-I{build.CSRC}", f"-I{build.CUDA_HOME / 'include'}",
+                    str(src), "-o", str(exe)], check=True)
+    for size, T, H, V in ((2, 8192, 4096, 128000), (2, 32768, 2048, 50257), (4, 1, 512, 20000),
+                          (2, 1537, 1111, 32003), (4, 10, 1 << 20, 9), (2, 5, 8, 1000)):
+        out = subprocess.run([str(exe), *map(str, (size, T, H, V))], check=True,
+                             capture_output=True, text=True).stdout
+        plans = [tuple(map(int, line.split())) for line in out.splitlines()]
+        assert len(plans) == 160
+        for sms, rows, words, ctas in plans:
+            assert 0 <= rows <= V and words * 16 == rows * H * size, (sms, rows, words)
+            assert (ctas > 0) == (rows > 0), (sms, rows, ctas)
+            assert ctas <= max(0, 2 * sms - 128) and ctas * 1024 < words + 1024, (sms, ctas)
+        large = V * H * size >= 32 << 20 and 16 << 20 >= 8 * H * size
+        assert (plans[147][1] > 0) == large
 
 
 @pytest.mark.gpu
