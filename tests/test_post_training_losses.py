@@ -613,6 +613,115 @@ def test_sequences_of_sure_labels(cuda, built, T, cancelling, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("kind", ["policy", "preference"])
+@pytest.mark.parametrize("T,H,V", [(15, 264, 88432), (100, 65, 40000), (128, 72, 50257)])
+def test_few_tokens_of_several_waves(cuda, built, T, H, V, kind, dtype):
+    """Up to 128 tokens of so many words that a CTA takes several tiles of them."""
+    _both(cuda, Policy(cuda, T, H, V, dtype, out=0.2, seed=T) if kind == "policy" else
+          Preference(cuda, T, H, V, 3, dtype, seed=T, lengths=[T // 6] * 6))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["policy", "preference"])
+@pytest.mark.parametrize("T", [4, 100, 300])
+def test_nan_word_reaches_every_token(cuda, built, kind, T):
+    """A NaN in a word that is no token's label, beside labels that are their rows' largest words."""
+    h = (Policy(cuda, T, 64, 700, seed=T) if kind == "policy" else
+         Preference(cuda, T, 64, 700, 2, seed=T, lengths=[T // 4] * 4))
+    h.labels.clamp_(max=500)
+    h.labels[0] = -1
+    h.x.copy_(h.w[h.labels.clamp(min=0)].float() * 16)
+    h.w[555, 3] = math.nan
+    with Dnn(cuda) as d:
+        assert h.forward(d) == 0
+        cuda.cuda.synchronize()
+    assert h.nll[1:].isnan().all() and h.nll[0] == 0
+    if kind == "policy":
+        assert h.loss[1:].isnan().all()
+    else:  # of 4 tokens the first is all of its sequence: a pair that is left out
+        assert h.loss[1].isnan() and (h.loss[0] == 0 if T == 4 else h.loss[0].isnan())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("T,H,calls", [(8, 1024, 40), (100, 1024, 4), (2000, 1024, 1)])
+def test_mean_error_of_nll(cuda, built, T, H, calls, dtype):
+    """What the tensor cores' sums lose on average is made up for.  A chain of n MMAs is short of
+    a logit by a share of about 1.45e-8 n (bf16; fp16 1.95e-8), the chains are of 32 MMAs (8 for up
+    to 8 tokens).  That alone would leave nll off by this share of the likely words' logits, about
+    16, above the label's: no more than half of it may be left, and four standard errors."""
+    share = (8 if T <= 8 else 32) * (1.45e-8 if dtype == "bf16" else 1.95e-8)
+    off, lost = [], []
+    for seed in range(calls):
+        h = Policy(cuda, T, H, 8000, dtype, seed=seed, old=False, ref=False, coef=0.0)
+        likely = cuda.randint(0, 8000, (T,), device="cuda", generator=h.g)
+        h.x.copy_(h.x.float() + 16 * h.w[likely].float())
+        with Dnn(cuda) as d:
+            assert h.forward(d, outputs=("nll",)) == 0
+            cuda.cuda.synchronize()
+        z = h.x.double() @ h.w.double().t()
+        label = z.gather(1, h.labels[:, None])[:, 0]
+        off.append(h.nll.double() - (cuda.logsumexp(z, dim=1) - label))
+        lost.append(share * ((cuda.softmax(z, dim=1) * z).sum(dim=1) - label))
+    off, lost = cuda.cat(off), cuda.cat(lost)
+    noise = off.std() / math.sqrt(len(off))
+    assert lost.mean() > 12 * noise  # the inputs tell
+    assert off.mean().abs() <= 0.5 * lost.mean() + 4 * noise
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_preference_piece_of_four_gib(cuda, built, dtype):
+    """One piece of 2^31 numerators, the most that a preference's gradients take: every output
+    against its definition, computed by blocks of tokens."""
+    torch, T, H, V, u = cuda, 16384, 64, 131072, U[dtype]
+
+    class Large(Preference):
+        def nll64(self):
+            if not hasattr(self, "kept"):
+                parts = []
+                for a in range(0, T, 1024):
+                    part = Policy.__new__(Policy)
+                    part.torch, part.tau, part.w = torch, self.tau, self.w
+                    part.x, part.labels = self.x[a:a + 1024], self.labels[a:a + 1024]
+                    parts.append(LossHead.nll64(part))
+                self.kept = [torch.cat(p) for p in zip(*parts)]
+            return tuple(t.clone() for t in self.kept)
+
+    h = Large(cuda, T, H, V, 7, dtype, out=0.1, seed=3)
+    with Dnn(cuda) as d:
+        assert h.workspace_size(d, 1) > 4 << 30  # one piece
+        assert h.backward(d) == 0
+        cuda.cuda.synchronize()
+    h.check(gradients=False)
+    _, _, dnll, derr = h.expected()
+    _, _, live, zerr = h.nll64()
+    w = h.w.double()
+    dw64, dwerr, dwsum = (torch.zeros(V, H, device="cuda", dtype=torch.float64) for _ in range(3))
+    for a in range(0, T, 1024):
+        s = slice(a, a + 1024)
+        on, x, e = live[s, None], h.x[s].double(), zerr[s, None]
+        p = torch.softmax(x @ w.t(), dim=1) * on
+        target = torch.zeros_like(p).scatter_(1, h.labels[s, None].clamp(min=0), 1.0) * on
+        g = dnll[s, None]
+        dz = g * (p - target)
+        err = g.abs() * p * (2 * u * (1 + u) + 2 * e + 2.0 ** -18)
+        err += target * (u * dz.abs() + g.abs() * (2.0 ** -19 + 2 * e) * 2)
+        err += derr[s, None] * (p - target).abs() * (1 + 2 * u)
+        if dtype == "fp16":
+            err += on * (g.abs() * p.amax(dim=1, keepdim=True) + dnll.abs().max() * 2.0 ** -12) * 2.0 ** -24
+        dx64 = dz @ w
+        t = err @ w.abs() + u * dx64.abs() * 1.01 + (dz.abs() @ w.abs()) * (V + 32) * 2.0 ** -23
+        assert ((h.dx[s].double() - dx64).abs() <= t + TINY[dtype]).all(), a
+        dw64 += dz.t() @ x
+        dwerr += err.t() @ x.abs()
+        dwsum += dz.abs().t() @ x.abs()
+    t = dwerr + u * dw64.abs() * 1.01 + dwsum * (T + 32) * 2.0 ** -23 + TINY[dtype]
+    assert ((h.dw.double() - dw64).abs() <= t).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("kind", ["policy", "preference"])
 @pytest.mark.parametrize("T,H", [(1000, 72), (385, 65)])
 def test_pieces(cuda, built, T, H, kind, dtype):
     """Given workspaces from the least to the preferred: every piece count gives the result."""
