@@ -266,8 +266,8 @@ cudnnStatus_t cudnnBatchNormalizationForwardTraining(
  * A negative label leaves its token out; a negative teacher index, or a teacher logit of
  * -inf, leaves its entry out, and a token without entries is left out.  A token that is
  * left out has loss 0, logSumExp 0 and no gradient, whatever its x and dloss hold.
- * Temperatures are 2^-64 to 2^64.  Equal indices of a token add up.  A label or index of V or more makes its token's loss,
- * and the gradients it enters, NaN.  labels and teacherIndex [T][topK] are int64 (as
+ * Temperatures are 2^-64 to 2^64.  Equal indices of a token add up.  A label or index of V or
+ * more makes its token's loss, and the gradients it enters, NaN.  labels and teacherIndex [T][topK] are int64 (as
  * training programs hold them); teacherLogits [T][topK], loss and logSumExp are float.
  *
  * Backward computes the gradients of sum_t dloss[t] * loss[t] in one pass over the
@@ -330,8 +330,8 @@ cudnnStatus_t cudnnLinearDistillationBackward(cudnnHandle_t handle, cudnnTensorD
 /* Losses of post-training on the same head (extensions).  nll[t] is the cross entropy above,
  * the negative log-probability of the label; x, w, labels, the workspace, streams and capture
  * are as above, and so is a token that a negative label leaves out: 0 in every output, no
- * gradient, whatever the other inputs hold there.  All float arrays are fp32.  Device memory is
- * the current device's: another one's is BAD_PARAM.
+ * gradient, whatever the other inputs hold there.  nll is 0 or more, at any temperature.  All
+ * float arrays are fp32.  Device memory is the current device's: another one's is BAD_PARAM.
  *
  * Policy loss, per token, z = x w^T / temperature:
  *   ratio = exp(oldNll - nll)            oldNll null: 1, and its gradient as if it were nll
@@ -352,6 +352,7 @@ cudnnStatus_t cudnnLinearDistillationBackward(cudnnHandle_t handle, cudnnTensorD
  *   loss[p] = SIGMOID: softplus(-h) + labelSmoothing h; HINGE: max(0, 1 - h);
  *             SQUARED: ((h - 1/2) / beta)^2
  *   rewards[s] = beta L[s]
+ * An infinite h (a reference that did not know a token) has the loss that is its limit.
  * beta is 2^-64 to 2^64, labelSmoothing 0 to 1/2 and 0 for the other modes.  A pair with a
  * sequence of which no token is kept is left out: loss and rewards 0, no gradient.  Rows of no
  * sequence have an nll and no gradient.  A pair whose offsets do not ascend within 0..T has NaN
@@ -363,7 +364,10 @@ cudnnStatus_t cudnnLinearDistillationBackward(cudnnHandle_t handle, cudnnTensorD
  * preference loss.  Logits are computed once, but for preference gradients of more tokens than
  * one piece has: a pair's loss takes all its tokens, so each piece's logits are computed again
  * after them.  To that end a piece of a preference's holds up to 4 GiB of numerators (not 2, see
- * the workspace above); 8 bytes per token come besides. */
+ * the workspace above); 8 bytes per token come besides.  A preference's gradients of more than 64
+ * tokens are scaled on their way into dw in BFLOAT16 as well, and in both types by the power of
+ * two above or less, down to half of it: a sequence's tokens share one gradient, and the factor
+ * that leaves least of it to rounding is taken. */
 typedef enum {
   CUDNN_PREFERENCE_SIGMOID = 0,
   CUDNN_PREFERENCE_HINGE = 1,

@@ -197,7 +197,7 @@ constexpr int kLogitsChunk = 8, kFewLogitsChunk = 2;
 // mean error: 4.6e-7 of the logits of 32 MMAs and 0.9e-7 of 4 in bf16, 5.9e-7 and 1.3e-7 in
 // fp16).  It is no error of a single cross entropy, but the losses of sequences add it up: their
 // logits' scale is larger by it.  With that and exact_target_nll rewards of 250-token sequences
-// are 6e-7 off instead of 1.2e-5, and nll is 2e-7 off on average instead of 1.4e-6.
+// are 6e-7 off instead of 1.2e-5, and nll is 3e-7 or less off on average instead of 1.4e-6.
 constexpr double kTruncatedBf16 = 1.45e-8, kTruncatedFp16 = 1.95e-8;
 
 // A thread's logits of one token, and what says whether a target word is among them: the
@@ -1137,9 +1137,6 @@ __device__ __forceinline__ uint4 scaled(uint4 u, float f, uint4* left = nullptr)
   return u;
 }
 
-// A CTA per row and part of its words (each part joins the row's pairs again, a few KB from
-// L2), then one per tile of the transpose.  Bound by HBM: it reads and writes the numerators once, 8192 x
-// 131072 in 0.68 ms (6.3 TB/s).
 // What the finish computes of a token besides its target losses; forms of their own, for those
 // losses' registers' sake (40 against 62).  kNll: the cross entropy with the target's logit
 // computed again.  kPolicy: the policy loss of that, whose upstream gradient dloss is.
@@ -1208,6 +1205,11 @@ __device__ __forceinline__ float exact_target_nll(float z, float was, float mx, 
   return below < 0.0f ? logf(rest + expf(below)) - below : log1pf(rest * expf(-below));
 }
 
+// A CTA per row and part of its words (each part joins the row's pairs again, a few KB from
+// L2), then one per tile of the transpose.  Bound by HBM: it reads and writes the numerators once,
+// 8192 x 131072 in 0.68 ms (6.3 TB/s).  kNll and kPolicy read x's row and the label's word too,
+// each part again.  Scores of up to 128 tokens (`early`, a CTA per row) do so before they wait
+// for the logits: x, w and labels are the caller's, and no kernel of a call writes them before.
 template <typename T, int STORE, int FORM>
 __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const FinishArgs a) {
   tc::grid_launch_next();
